@@ -191,12 +191,20 @@ MLORA_API int mlora_merge(const void* w0, const void* a, const void* b, void* w_
 #define MLORA_QUANT_NF4 1
 #define MLORA_QUANT_INT4 2
 #define MLORA_QUANT_INT8 3
+/*   MXFP4: codes uint8 [N, K/2] (nibbles as NF4), each an e2m1 number (sign in
+ *         bit 3; magnitudes 0, .5, 1, 1.5, 2, 3, 4, 6); scales uint8
+ *         [N, ceil(K/32)] = E + 127 of a block's factor 2^E (255: the block is
+ *         NaN); group = 32, no zeros; w = e2m1 * 2^E, exact in BF16.  No
+ *         reference counterpart. */
+#define MLORA_QUANT_MXFP4 4
 
 /* Quantises w [N,K] (BF16/F16/F32) into codes/scales/zeros (zeros unused for
  * NF4).  NF4: per (row, block of `group`) absmax, nearest level (first on
  * ties).  INT4/INT8: asymmetric per (row, group): scale = (max-min)/(2^b-1)
  * rounded up to fp16, zero = rint(-min/scale), q = rint(w/scale) + zero, both
- * clamped to [0, 2^b-1].  The reference has no quantiser; this is the format's
+ * clamped to [0, 2^b-1].  MXFP4: per (row, 32 features) E = max(floor(log2
+ * max|w|) - 2, -127), code = w / 2^E to nearest even, saturating at 6; a block
+ * holding an infinity or NaN gets scale 255 and codes 0.  The reference has no quantiser; this is the format's
  * producer for the kernels below. */
 MLORA_API int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme,
                              int64_t group, void* codes, void* scales, void* zeros, void* stream);
@@ -226,7 +234,7 @@ MLORA_API size_t mlora_qlora_lean_workspace_bytes(int64_t M, int64_t K, int64_t 
 /* The prepared scale table of a quantised weight: its per-row scales re-laid
  * as [ceil(K/group), N rounded up to 4] -- fp32 absmax for NF4, (scale, zero)
  * fp16 pairs for INT4/INT8 -- so that one TMA box holds a block of rows'
- * scales.  The decode kernel and the fused kernel read scales only from it;
+ * scales; for MXFP4, the fp4 product's blocks of 128 rows x 128 features.  The decode kernel and the fused kernel read scales only from it;
  * without one, each call builds it in its workspace.  No reference
  * counterpart (the reference reads its per-row scales directly,
  * kernels/lora_quantized.metal:122, :64-65). */
@@ -242,7 +250,10 @@ MLORA_API int mlora_qlora_prepare_scales(int scheme, const void* scales, const v
  * the fused kernel's main loop (lean workspace); up to 16 tokens without
  * saved_xa, a GEMV dequantises in registers.  group (NF4 block size / INT
  * group) must be 64, 128 or 256; K a multiple of 32 (4-bit) or 16 (INT8).
- * saved_xa as for mlora_lora_forward. */
+ * saved_xa as for mlora_lora_forward.
+ * MXFP4 (group 32; BF16 or F16): y = Q4(x) . deq(W)^T + (alpha/r)(x . a^T) . b^T,
+ * where Q4 rounds x to MXFP4 by the rule of mlora_quantize; both factors go to
+ * the fp4 tensor cores as they are.  There is no lean path for it. */
 MLORA_API int mlora_qlora_forward(const void* x, int scheme, const void* codes, const void* scales,
                                   const void* zeros, int64_t group, const void* a, const void* b,
                                   void* y, void* saved_xa, int64_t M, int64_t K, int64_t N,
@@ -259,7 +270,8 @@ MLORA_API int mlora_qlora_forward_ex(const void* x, int scheme, const void* code
 /* Gradients through the quantised base (frozen, as in QLoRA): dx = dy . deq(W)
  * + s (dy . b) . a (staged or lean as for the forward; dx may be NULL, then
  * the codes are not read), da, db as mlora_lora_backward_ex (flags:
- * MLORA_BWD_ACCUMULATE). */
+ * MLORA_BWD_ACCUMULATE, MLORA_BWD_GRADS_16BIT).  MXFP4: dx = dy . deq(W) + ...
+ * with 16-bit operands (the rounding of x is passed straight through). */
 MLORA_API int mlora_qlora_backward(const void* dy, const void* x, int scheme, const void* codes,
                                    const void* scales, const void* zeros, int64_t group,
                                    const void* a, const void* b, const void* saved_xa, void* dx,
@@ -274,6 +286,40 @@ MLORA_API int mlora_qlora_backward_ex(const void* dy, const void* x, int scheme,
                                       int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
                                       float clip_value, int dtype, int flags, void* workspace,
                                       size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit activation checkpoints ----------------------------------------
+ * MXINT8: x [M, K] as codes int8, rows ld >= K bytes apart, and scale words
+ * uint8 [ceil(K/128), M rounded up to 4, 4]: byte (g, m, i) = E + 127 of
+ * features 128 g + 32 i .. + 31 of row m; value = code / 64 * 2^E with
+ * E = max(floor(log2 max|x|), -127) over the block, code = 64 x / 2^E to
+ * nearest even, clamped to +-127 (scale 255 and codes 0 for a block holding an
+ * infinity or NaN).  mlora_act_restore gives the values back in `dtype` (exact
+ * in BF16).  Scales are 4-byte aligned; 16-byte aligned codes and scales with
+ * ld % 16 == 0 are what the backward below takes.  No reference counterpart
+ * (its trainer keeps x in the compute dtype). */
+MLORA_API size_t mlora_act_checkpoint_scales_bytes(int64_t M, int64_t K);
+MLORA_API int mlora_act_checkpoint(const void* x, int dtype, int64_t M, int64_t K, void* codes,
+                                   int64_t ld, void* scales, void* stream);
+MLORA_API int mlora_act_restore(const void* codes, int64_t ld, const void* scales, int64_t M,
+                                int64_t K, void* out, int dtype, void* stream);
+
+/* mlora_lora_backward_ex / mlora_qlora_backward_ex with a checkpoint in the
+ * place of x: da = s (dy . b)^T . x^ with x^ the checkpoint's values, db from
+ * saved_xa (required), BF16 or F16, all of their flags and workspaces. */
+MLORA_API int mlora_lora_backward_ckpt(const void* dy, const void* ckpt_codes, int64_t ckpt_ld,
+                                       const void* ckpt_scales, const void* w0, const void* a,
+                                       const void* b, const void* saved_xa, void* dx, void* da,
+                                       void* db, int64_t M, int64_t K, int64_t N, int64_t r,
+                                       float alpha, float clip_value, int dtype, int flags,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+MLORA_API int mlora_qlora_backward_ckpt(const void* dy, const void* ckpt_codes, int64_t ckpt_ld,
+                                        const void* ckpt_scales, int scheme, const void* codes,
+                                        const void* scales, const void* zeros,
+                                        const void* prepared, int64_t group, const void* a,
+                                        const void* b, const void* saved_xa, void* dx, void* da,
+                                        void* db, int64_t M, int64_t K, int64_t N, int64_t r,
+                                        float alpha, float clip_value, int dtype, int flags,
+                                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- multiple adapters in one batch ------------------------------------ */
 

@@ -29,6 +29,7 @@ BWD_GRADS_16BIT = 8
 QUANT_NF4 = 1
 QUANT_INT4 = 2
 QUANT_INT8 = 3
+QUANT_MXFP4 = 4
 
 DTYPE_BF16 = 0
 DTYPE_F16 = 1
@@ -90,6 +91,14 @@ SIGNATURES: dict[str, tuple] = {
                                      i64, f32, i32, vp, sz, vp]),
     "mlora_qlora_backward_ex": (i32, [vp, vp, i32, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, vp,
                                       i64, i64, i64, i64, f32, f32, i32, i32, vp, sz, vp]),
+    "mlora_act_checkpoint_scales_bytes": (sz, [i64, i64]),
+    "mlora_act_checkpoint": (i32, [vp, i32, i64, i64, vp, i64, vp, vp]),
+    "mlora_act_restore": (i32, [vp, i64, vp, i64, i64, vp, i32, vp]),
+    "mlora_lora_backward_ckpt": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
+                                       i64, f32, f32, i32, i32, vp, sz, vp]),
+    "mlora_qlora_backward_ckpt": (i32, [vp, vp, i64, vp, i32, vp, vp, vp, vp, i64, vp, vp, vp, vp,
+                                        vp, vp, i64, i64, i64, i64, f32, f32, i32, i32, vp, sz,
+                                        vp]),
     "mlora_adamw_step": (i32, [vp, vp, vp, vp, vp, i64, f32, f32, f32, f32, f32, i32, vp, vp]),
     "mlora_sgd_step": (i32, [vp, vp, i64, f32, i32, vp, vp]),
     "mlora_adam_state_step": (i32, [vp, f32, f32, vp]),

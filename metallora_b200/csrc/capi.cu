@@ -485,14 +485,35 @@ int lora_backward_f32(const float* dy, const float* x, const float* w0, const fl
 // Phases of the 16-bit backward (flags MLORA_BWD_DEFER_DX / MLORA_BWD_DX_ONLY).
 constexpr int kPhaseAll = 0, kPhaseDeferDx = 1, kPhaseDx = 2;
 
+// An MXINT8 checkpoint standing in for x in the backward (see MxWgradArgs).
+struct Ckpt {
+  const void* codes;
+  int64_t ld;
+  const void* scales;
+};
+
+int check_ckpt(const Ckpt& c, int64_t K, const void* saved_xa, int dtype) {
+  if (!c.codes || !c.scales) return fail(MLORA_ERR_INVALID_ARG, "NULL checkpoint pointer");
+  if (!aligned16(c.codes) || !aligned16(c.scales) || c.ld < K || c.ld % 16)
+    return fail(MLORA_ERR_INVALID_ARG,
+                "checkpoint codes and scales must be 16-byte aligned, code rows a multiple of 16 "
+                "bytes apart");
+  if (saved_xa == nullptr)
+    return fail(MLORA_ERR_INVALID_ARG, "a checkpointed backward needs saved_xa");
+  if (dtype == MLORA_DTYPE_F32)
+    return fail(MLORA_ERR_UNSUPPORTED, "a checkpointed backward takes BF16 or F16");
+  return MLORA_OK;
+}
+
 // Backward of the 16-bit LoRA linear (dense W0, or a quantised W0 described
-// by qdx): rank projections, dA/dB weight gradients, dx GEMM.
+// by qdx): rank projections, dA/dB weight gradients, dx GEMM.  With `ckpt`, dA
+// reads the checkpoint instead of x (then unused).
 int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* qdx,
                const void* a, const void* b, const void* saved_xa, void* dx, float* da,
                float* db, int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
                float clip_value, bool accumulate, int dtype, void* workspace,
                size_t workspace_bytes, cudaStream_t s, int phase = kPhaseAll,
-               bool grads16 = false) {
+               bool grads16 = false, const Ckpt* ckpt = nullptr) {
   int rc;
   const BwdPlan need = plan_backward(nullptr, M, K, N, r, saved_xa == nullptr);
   if (workspace == nullptr || workspace_bytes < need.bytes || !aligned16(workspace))
@@ -575,7 +596,26 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
     w[1].out = da;
     w[1].ldo = K;
     w[1].transposed = true;
-    if ((rc = launch_wgrad(w, 2, s))) return rc;
+    if (ckpt != nullptr) w[0].splits = wgrad_splits(M, N, 1);
+    if ((rc = launch_wgrad(w, ckpt != nullptr ? 1 : 2, s))) return rc;
+    if (ckpt != nullptr) {
+      MxWgradArgs g;
+      g.codes = ckpt->codes;
+      g.scales = ckpt->scales;
+      g.ld = ckpt->ld;
+      g.st = p.u_t;
+      g.ld_st = pad8(M);
+      g.M = M;
+      g.K = K;
+      g.r = r;
+      g.R = p.R;
+      g.out = da;
+      g.accumulate = accumulate;
+      g.out16 = grads16;
+      g.clip = clip_value;
+      g.elt = elt;
+      if ((rc = launch_mx_wgrad(g, s))) return rc;
+    }
   }
   if (phase == kPhaseDeferDx) return MLORA_OK;
 
@@ -866,11 +906,13 @@ int mlora_lora_backward(const void* dy, const void* x, const void* w0, const voi
                                 clip_value, dtype, 0, workspace, workspace_bytes, stream);
 }
 
-int mlora_lora_backward_ex(const void* dy, const void* x, const void* w0, const void* a,
-                           const void* b, const void* saved_xa, void* dx, float* da, float* db,
-                           int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
-                           float clip_value, int dtype, int flags, void* workspace,
-                           size_t workspace_bytes, void* stream) {
+namespace {
+// mlora_lora_backward_ex, or with `ckpt` (x then NULL) mlora_lora_backward_ckpt.
+int lora_backward_any(const void* dy, const void* x, const Ckpt* ckpt, const void* w0,
+                      const void* a, const void* b, const void* saved_xa, void* dx, void* da,
+                      void* db, int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
+                      float clip_value, int dtype, int flags, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   const bool accumulate = (flags & MLORA_BWD_ACCUMULATE) != 0;
   if (flags & ~(MLORA_BWD_ACCUMULATE | MLORA_BWD_DEFER_DX | MLORA_BWD_DX_ONLY |
                 MLORA_BWD_GRADS_16BIT))
@@ -884,7 +926,9 @@ int mlora_lora_backward_ex(const void* dy, const void* x, const void* w0, const 
                     : (flags & MLORA_BWD_DX_ONLY) ? kPhaseDx : kPhaseAll;
   int rc = check_shapes(M, K, N, r, dtype);
   if (rc) return rc;
-  if (!dy || !x || !a || !b || !da || !db) return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (!dy || (!x && ckpt == nullptr) || !a || !b || !da || !db)
+    return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (ckpt != nullptr && (rc = check_ckpt(*ckpt, K, saved_xa, dtype))) return rc;
   if ((dx == nullptr) != (w0 == nullptr))
     return fail(MLORA_ERR_INVALID_ARG, "w0 and dx must be both set or both NULL");
   if (phase != kPhaseAll && (dx == nullptr || dtype == MLORA_DTYPE_F32))
@@ -896,12 +940,35 @@ int mlora_lora_backward_ex(const void* dy, const void* x, const void* w0, const 
   if (dtype == MLORA_DTYPE_F32)
     return lora_backward_f32(static_cast<const float*>(dy), static_cast<const float*>(x),
                              static_cast<const float*>(w0), static_cast<const float*>(a),
-                             static_cast<const float*>(b), static_cast<float*>(dx), da, db, M, K,
+                             static_cast<const float*>(b), static_cast<float*>(dx),
+                             static_cast<float*>(da), static_cast<float*>(db), M, K,
                              N, r, alpha, clip_value, accumulate, workspace, workspace_bytes,
                              static_cast<cudaStream_t>(stream));
-  return backward16(dy, x, w0, nullptr, a, b, saved_xa, dx, da, db, M, K, N, r, alpha, clip_value,
+  return backward16(dy, x, w0, nullptr, a, b, saved_xa, dx, static_cast<float*>(da),
+                    static_cast<float*>(db), M, K, N, r, alpha, clip_value,
                     accumulate, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream),
-                    phase, grads16);
+                    phase, grads16, ckpt);
+}
+}  // namespace
+
+int mlora_lora_backward_ex(const void* dy, const void* x, const void* w0, const void* a,
+                           const void* b, const void* saved_xa, void* dx, float* da, float* db,
+                           int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
+                           float clip_value, int dtype, int flags, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  return lora_backward_any(dy, x, nullptr, w0, a, b, saved_xa, dx, da, db, M, K, N, r, alpha,
+                           clip_value, dtype, flags, workspace, workspace_bytes, stream);
+}
+
+int mlora_lora_backward_ckpt(const void* dy, const void* ckpt_codes, int64_t ckpt_ld,
+                             const void* ckpt_scales, const void* w0, const void* a, const void* b,
+                             const void* saved_xa, void* dx, void* da, void* db, int64_t M,
+                             int64_t K, int64_t N, int64_t r, float alpha, float clip_value,
+                             int dtype, int flags, void* workspace, size_t workspace_bytes,
+                             void* stream) {
+  const Ckpt c{ckpt_codes, ckpt_ld, ckpt_scales};
+  return lora_backward_any(dy, nullptr, &c, w0, a, b, saved_xa, dx, da, db, M, K, N, r, alpha,
+                           clip_value, dtype, flags, workspace, workspace_bytes, stream);
 }
 
 long long mlora_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
@@ -994,12 +1061,36 @@ int mlora_grad_norm_clip(const float* grad, int64_t n, float max_norm, float* ou
 
 namespace {
 int check_quant(int scheme, int64_t N, int64_t K, int64_t group) {
-  if (scheme != MLORA_QUANT_NF4 && scheme != MLORA_QUANT_INT4 && scheme != MLORA_QUANT_INT8)
-    return fail(MLORA_ERR_INVALID_ARG, "scheme must be NF4, INT4 or INT8");
+  if (scheme != MLORA_QUANT_NF4 && scheme != MLORA_QUANT_INT4 && scheme != MLORA_QUANT_INT8 &&
+      scheme != MLORA_QUANT_MXFP4)
+    return fail(MLORA_ERR_INVALID_ARG, "scheme must be NF4, INT4, INT8 or MXFP4");
   if (N <= 0 || K <= 0 || group <= 0) return fail(MLORA_ERR_INVALID_ARG, "N, K, group must be positive");
+  if (scheme == MLORA_QUANT_MXFP4 && group != 32)
+    return fail(MLORA_ERR_INVALID_ARG, "MXFP4 blocks hold 32 features: group must be 32");
   if (scheme != MLORA_QUANT_INT8 && (K % 2))
     return fail(MLORA_ERR_INVALID_ARG, "4-bit codes pack two per byte: K must be even");
   return MLORA_OK;
+}
+
+// Schemes whose weights carry zero points.
+bool has_zeros(int scheme) { return scheme == MLORA_QUANT_INT4 || scheme == MLORA_QUANT_INT8; }
+
+MxScales plain_scales(const void* scales, int64_t rows, int64_t K) {
+  return MxScales{static_cast<uint8_t*>(const_cast<void*>(scales)), rows, (K + 31) / 32, kMxPlain};
+}
+// Checkpoint scale words [ceil(K / 128), rows rounded up to 4].
+MxScales group_scales(const void* scales, int64_t rows, int64_t K) {
+  return MxScales{static_cast<uint8_t*>(const_cast<void*>(scales)), (rows + 3) / 4 * 4,
+                  (K + 31) / 32, kMxGroups};
+}
+
+// One weight matrix [N, K] in `out` (out_dtype).
+int dequantize_weight(int scheme, const void* codes, const void* scales, const void* zeros,
+                      int64_t N, int64_t K, int64_t group, void* out, int out_dtype,
+                      cudaStream_t s) {
+  if (scheme == MLORA_QUANT_MXFP4)
+    return launch_mx_dequantize(4, codes, K / 2, plain_scales(scales, N, K), N, K, out, out_dtype, s);
+  return launch_dequantize(scheme, codes, scales, zeros, N, K, group, out, out_dtype, s);
 }
 }  // namespace
 
@@ -1007,11 +1098,14 @@ int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme,
                    void* codes, void* scales, void* zeros, void* stream) {
   int rc = check_quant(scheme, N, K, group);
   if (rc) return rc;
-  if (!w || !codes || !scales || (scheme != MLORA_QUANT_NF4 && !zeros))
+  if (!w || !codes || !scales || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
   if (w_dtype < MLORA_DTYPE_BF16 || w_dtype > MLORA_DTYPE_F32)
     return fail(MLORA_ERR_INVALID_ARG, "weight dtype must be BF16, F16 or F32");
   if ((rc = check_device())) return rc;
+  if (scheme == MLORA_QUANT_MXFP4)
+    return launch_mx_quantize(4, w, w_dtype, N, K, codes, K / 2, plain_scales(scales, N, K),
+                              static_cast<cudaStream_t>(stream));
   return launch_quantize(w, w_dtype, N, K, scheme, group, codes, scales, zeros,
                          static_cast<cudaStream_t>(stream));
 }
@@ -1020,13 +1114,50 @@ int mlora_dequantize(int scheme, const void* codes, const void* scales, const vo
                      int64_t N, int64_t K, int64_t group, void* out, int out_dtype, void* stream) {
   int rc = check_quant(scheme, N, K, group);
   if (rc) return rc;
-  if (!codes || !scales || !out || (scheme != MLORA_QUANT_NF4 && !zeros))
+  if (!codes || !scales || !out || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
   if (out_dtype < MLORA_DTYPE_BF16 || out_dtype > MLORA_DTYPE_F32)
     return fail(MLORA_ERR_INVALID_ARG, "out dtype must be BF16, F16 or F32");
   if ((rc = check_device())) return rc;
-  return launch_dequantize(scheme, codes, scales, zeros, N, K, group, out, out_dtype,
+  return dequantize_weight(scheme, codes, scales, zeros, N, K, group, out, out_dtype,
                            static_cast<cudaStream_t>(stream));
+}
+
+// ---- activation checkpoints -----------------------------------------------------
+
+size_t mlora_act_checkpoint_scales_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return 0;
+  return static_cast<size_t>((K + 127) / 128) * ((M + 3) / 4 * 4) * 4;
+}
+
+namespace {
+int check_act(const void* x, int dtype, const void* codes, int64_t ld, const void* scales,
+              int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0) return fail(MLORA_ERR_INVALID_ARG, "M and K must be positive");
+  if (!x || !codes || !scales) return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
+  if (dtype < MLORA_DTYPE_BF16 || dtype > MLORA_DTYPE_F32)
+    return fail(MLORA_ERR_INVALID_ARG, "dtype must be BF16, F16 or F32");
+  if (ld < K) return fail(MLORA_ERR_INVALID_ARG, "code rows overlap: ld is below K");
+  if (reinterpret_cast<uintptr_t>(scales) & 3u)
+    return fail(MLORA_ERR_INVALID_ARG, "scales must be 4-byte aligned");
+  return check_device();
+}
+}  // namespace
+
+int mlora_act_checkpoint(const void* x, int dtype, int64_t M, int64_t K, void* codes, int64_t ld,
+                         void* scales, void* stream) {
+  int rc = check_act(x, dtype, codes, ld, scales, M, K);
+  if (rc) return rc;
+  return launch_mx_quantize(8, x, dtype, M, K, codes, ld, group_scales(scales, M, K),
+                            static_cast<cudaStream_t>(stream));
+}
+
+int mlora_act_restore(const void* codes, int64_t ld, const void* scales, int64_t M, int64_t K,
+                      void* out, int dtype, void* stream) {
+  int rc = check_act(out, dtype, codes, ld, scales, M, K);
+  if (rc) return rc;
+  return launch_mx_dequantize(8, codes, ld, group_scales(scales, M, K), M, K, out, dtype,
+                              static_cast<cudaStream_t>(stream));
 }
 
 namespace {
@@ -1034,6 +1165,12 @@ int check_qlora(int scheme, int64_t M, int64_t K, int64_t N, int64_t r, int64_t 
   int rc = check_shapes(M, K, N, r, dtype);
   if (rc) return rc;
   if ((rc = check_quant(scheme, N, K, group))) return rc;
+  if (scheme == MLORA_QUANT_MXFP4) {
+    if (dtype == MLORA_DTYPE_F32)
+      return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base takes BF16 or F16 activations");
+    if (K % 32) return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base needs K a multiple of 32");
+    return MLORA_OK;
+  }
   if (dtype != MLORA_DTYPE_BF16)
     return fail(MLORA_ERR_UNSUPPORTED, "quantised-base paths take BF16 activations");
   if (group != 64 && group != 128 && group != 256)
@@ -1043,7 +1180,8 @@ int check_qlora(int scheme, int64_t M, int64_t K, int64_t N, int64_t r, int64_t 
   return MLORA_OK;
 }
 
-size_t qscales_bytes(int64_t N, int64_t K, int64_t group) {
+size_t qscales_bytes(int64_t N, int64_t K, int64_t group, int scheme = 0) {
+  if (scheme == MLORA_QUANT_MXFP4) return static_cast<size_t>(mx_atoms_bytes(N, K));
   return align_up(static_cast<size_t>((K + group - 1) / group) * prepared_ld(N) * 4, 256);
 }
 
@@ -1053,6 +1191,7 @@ size_t qscales_bytes(int64_t N, int64_t K, int64_t group) {
 int prep_scales(int scheme, const void* scales, const void* zeros, int64_t N, int64_t K,
                 int64_t group, void* scales_t, cudaStream_t s) {
   const int64_t G = (K + group - 1) / group;
+  if (scheme == MLORA_QUANT_MXFP4) return launch_mx_prepare_scales(scales, N, K, scales_t, s);
   if (scheme == MLORA_QUANT_NF4)
     return launch_transpose_f32(static_cast<const float*>(scales), N, G, prepared_ld(N),
                                 static_cast<float*>(scales_t), s);
@@ -1083,33 +1222,112 @@ size_t qfwd_lean_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int scheme, i
 size_t qbwd_lean_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int64_t group) {
   return plan_backward(nullptr, M, K, N, r, true).bytes + qscales_bytes(N, K, group);
 }
+
+// ---- MXFP4 base: x as fp4 codes and scale atoms, s.x.A^T rows ----------------
+struct MxFwdPlan {
+  int64_t R, R64;
+  void* xq;
+  void* xs;
+  void* xa_rows;
+  void* atoms;  // the weight's, when the caller brings no prepared table
+  size_t bytes;
+};
+
+MxFwdPlan plan_mx_forward(void* ws, int64_t M, int64_t K, int64_t N, int64_t r, bool own_table) {
+  MxFwdPlan p;
+  p.R = rank_tile(r);
+  p.R64 = pad64(p.R);
+  Carve c(ws);
+  p.xq = c.take(static_cast<size_t>(M) * (K / 2));
+  p.xs = c.take(static_cast<size_t>(mx_atoms_bytes(M, K)));
+  p.xa_rows = c.take(static_cast<size_t>(M) * p.R64 * 2);
+  p.atoms = own_table ? c.take(static_cast<size_t>(mx_atoms_bytes(N, K))) : nullptr;
+  p.bytes = align_up(c.off, 256);
+  return p;
+}
+
+int mx_forward(const void* x, const void* codes, const void* scales, const void* prepared,
+               const void* a, const void* b, void* y, void* saved_xa, int64_t M, int64_t K,
+               int64_t N, int64_t r, float alpha, int dtype, void* workspace,
+               size_t workspace_bytes, cudaStream_t s) {
+  int rc;
+  const MxFwdPlan need = plan_mx_forward(nullptr, M, K, N, r, prepared == nullptr);
+  if (workspace == nullptr || workspace_bytes < need.bytes)
+    return fail(MLORA_ERR_WORKSPACE, "MXFP4 forward workspace needs " + std::to_string(need.bytes) + " bytes");
+  const MxFwdPlan p = plan_mx_forward(workspace, M, K, N, r, prepared == nullptr);
+  const Elt elt = dtype == MLORA_DTYPE_BF16 ? Elt::kBF16 : Elt::kF16;
+  const void* atoms = prepared;
+  if (atoms == nullptr) {
+    if ((rc = launch_mx_prepare_scales(scales, N, K, p.atoms, s))) return rc;
+    atoms = p.atoms;
+  }
+  const MxScales xs{static_cast<uint8_t*>(p.xs), M, (K + 31) / 32, kMxAtoms};
+  if ((rc = launch_mx_quantize(4, x, dtype, M, K, p.xq, K / 2, xs, s))) return rc;
+  RankArgs ra;
+  ra.x = x;
+  ra.l = a;
+  ra.M = M;
+  ra.K = K;
+  ra.r = r;
+  ra.R = p.R;
+  ra.ldx = K;
+  ra.ldl = K;
+  ra.scale = alpha / static_cast<float>(r);
+  ra.out_rows = p.xa_rows;
+  ra.ld_rows = p.R64;
+  ra.out_t = saved_xa;
+  ra.ld_t = pad8(M);
+  ra.splits = rank_splits(M, K);
+  ra.elt = elt;
+  if ((rc = launch_rank(ra, s))) return rc;
+  MxGemmArgs g;
+  g.xq = p.xq;
+  g.xs = p.xs;
+  g.wq = codes;
+  g.ws = atoms;
+  g.x2 = p.xa_rows;
+  g.w2 = b;
+  g.d = y;
+  g.M = M;
+  g.N = N;
+  g.K = K;
+  g.R = p.R;
+  g.w2_rows = r;
+  g.ldx2 = p.R64;
+  g.ldw2 = r;
+  g.ldd = N;
+  g.elt = elt;
+  return launch_mx_gemm(g, s);
+}
 }  // namespace
 
 size_t mlora_qlora_lean_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int scheme,
                                         int64_t group, int backward) {
   if (M <= 0 || K <= 0 || N <= 0 || r <= 0 || group <= 0) return 0;
+  if (scheme == MLORA_QUANT_MXFP4)  // no lean kernel: dx stages the weight, dA/dB alone do not
+    return backward ? plan_backward(nullptr, M, K, N, r, true).bytes
+                    : plan_mx_forward(nullptr, M, K, N, r, true).bytes;
   return backward ? qbwd_lean_bytes(M, K, N, r, group) : qfwd_lean_bytes(M, K, N, r, scheme, group);
 }
 
 size_t mlora_qlora_forward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int scheme,
                                            int64_t group) {
-  (void)scheme;
   if (M <= 0 || K <= 0 || N <= 0 || r <= 0 || group <= 0) return 0;
+  if (scheme == MLORA_QUANT_MXFP4) return plan_mx_forward(nullptr, M, K, N, r, true).bytes;
   const size_t staged = staged_w_bytes(N, K) + plan_forward(nullptr, M, K, r, true).bytes;
   return std::max(staged, qfwd_lean_bytes(M, K, N, r, scheme, group));
 }
 
 size_t mlora_qlora_prepared_scales_bytes(int scheme, int64_t N, int64_t K, int64_t group) {
   if (N <= 0 || K <= 0 || group <= 0) return 0;
-  (void)scheme;
-  return qscales_bytes(N, K, group);
+  return qscales_bytes(N, K, group, scheme);
 }
 
 int mlora_qlora_prepare_scales(int scheme, const void* scales, const void* zeros, int64_t N,
                                int64_t K, int64_t group, void* out, void* stream) {
   int rc = check_quant(scheme, N, K, group);
   if (rc) return rc;
-  if (!scales || !out || (scheme != MLORA_QUANT_NF4 && !zeros))
+  if (!scales || !out || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
   if ((rc = check_ptrs16({scales, zeros, out}))) return rc;
   if ((rc = check_device())) return rc;
@@ -1131,12 +1349,15 @@ int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const v
                            size_t workspace_bytes, void* stream) {
   int rc = check_qlora(scheme, M, K, N, r, group, dtype);
   if (rc) return rc;
-  if (!x || !codes || !scales || !a || !b || !y || (scheme != MLORA_QUANT_NF4 && !zeros))
+  if (!x || !codes || !scales || !a || !b || !y || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
   if ((rc = check_ptrs16({x, codes, scales, zeros, prepared, a, b, y, saved_xa, workspace})))
     return rc;
   if ((rc = check_device())) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (scheme == MLORA_QUANT_MXFP4)
+    return mx_forward(x, codes, scales, prepared, a, b, y, saved_xa, M, K, N, r, alpha, dtype,
+                      workspace, workspace_bytes, s);
   if (saved_xa == nullptr && use_gemv(M, K, dtype)) {
     const void* table = prepared;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1217,9 +1438,9 @@ int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const v
 
 size_t mlora_qlora_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r,
                                             int scheme, int64_t group) {
-  (void)scheme;
   if (M <= 0 || K <= 0 || N <= 0 || r <= 0 || group <= 0) return 0;
   const size_t staged = staged_w_bytes(N, K) + plan_backward(nullptr, M, K, N, r, true).bytes;
+  if (scheme == MLORA_QUANT_MXFP4) return staged;
   return std::max(staged, qbwd_lean_bytes(M, K, N, r, group));
 }
 
@@ -1234,17 +1455,24 @@ int mlora_qlora_backward(const void* dy, const void* x, int scheme, const void* 
                                  workspace, workspace_bytes, stream);
 }
 
-int mlora_qlora_backward_ex(const void* dy, const void* x, int scheme, const void* codes,
-                            const void* scales, const void* zeros, const void* prepared,
-                            int64_t group, const void* a, const void* b, const void* saved_xa,
-                            void* dx, float* da, float* db, int64_t M, int64_t K, int64_t N,
-                            int64_t r, float alpha, float clip_value, int dtype, int flags,
-                            void* workspace, size_t workspace_bytes, void* stream) {
+namespace {
+// mlora_qlora_backward_ex, or with `ckpt` (x then NULL) mlora_qlora_backward_ckpt.
+int qlora_backward_any(const void* dy, const void* x, const Ckpt* ckpt, int scheme,
+                       const void* codes, const void* scales, const void* zeros,
+                       const void* prepared, int64_t group, const void* a, const void* b,
+                       const void* saved_xa, void* dx, void* da_, void* db_, int64_t M, int64_t K,
+                       int64_t N, int64_t r, float alpha, float clip_value, int dtype, int flags,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+  float* da = static_cast<float*>(da_);
+  float* db = static_cast<float*>(db_);
   int rc = check_qlora(scheme, M, K, N, r, group, dtype);
   if (rc) return rc;
-  if (flags & ~MLORA_BWD_ACCUMULATE) return fail(MLORA_ERR_INVALID_ARG, "unknown flags");
-  if (!dy || !x || !a || !b || !da || !db) return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
-  if (dx && (!codes || !scales || (scheme != MLORA_QUANT_NF4 && !zeros)))
+  if (flags & ~(MLORA_BWD_ACCUMULATE | MLORA_BWD_GRADS_16BIT))
+    return fail(MLORA_ERR_INVALID_ARG, "unknown flags");
+  if (!dy || (!x && ckpt == nullptr) || !a || !b || !da || !db)
+    return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (ckpt != nullptr && (rc = check_ckpt(*ckpt, K, saved_xa, dtype))) return rc;
+  if (dx && (!codes || !scales || (has_zeros(scheme) && !zeros)))
     return fail(MLORA_ERR_INVALID_ARG, "dx needs the quantised weight");
   if ((rc = check_ptrs16({dy, x, codes, scales, zeros, prepared, a, b, saved_xa, dx, da, db,
                           workspace})))
@@ -1252,19 +1480,23 @@ int mlora_qlora_backward_ex(const void* dy, const void* x, int scheme, const voi
   if ((rc = check_device())) return rc;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool accumulate = (flags & MLORA_BWD_ACCUMULATE) != 0;
+  const bool grads16 = (flags & MLORA_BWD_GRADS_16BIT) != 0;
   const size_t bytes = plan_backward(nullptr, M, K, N, r, saved_xa == nullptr).bytes;
   if (dx == nullptr)  // weight gradients only: the base weight is not read
     return backward16(dy, x, nullptr, nullptr, a, b, saved_xa, nullptr, da, db, M, K, N, r, alpha,
-                      clip_value, accumulate, dtype, workspace, workspace_bytes, s);
+                      clip_value, accumulate, dtype, workspace, workspace_bytes, s, kPhaseAll, grads16,
+                      ckpt);
   const size_t wbytes = staged_w_bytes(N, K);
   if (workspace != nullptr && workspace_bytes >= wbytes + bytes) {
-    if ((rc = launch_dequantize(scheme, codes, scales, zeros, N, K, group, workspace,
-                                MLORA_DTYPE_BF16, s)))
+    if ((rc = dequantize_weight(scheme, codes, scales, zeros, N, K, group, workspace, dtype, s)))
       return rc;
     return backward16(dy, x, workspace, nullptr, a, b, saved_xa, dx, da, db, M, K, N, r, alpha,
                       clip_value, accumulate, dtype, static_cast<uint8_t*>(workspace) + wbytes,
-                      workspace_bytes - wbytes, s);
+                      workspace_bytes - wbytes, s, kPhaseAll, grads16, ckpt);
   }
+  if (scheme == MLORA_QUANT_MXFP4)
+    return fail(MLORA_ERR_WORKSPACE, "MXFP4 backward workspace needs " +
+                                         std::to_string(wbytes + bytes) + " bytes");
   const size_t sbytes = qscales_bytes(N, K, group);
   if (workspace == nullptr || workspace_bytes < bytes + sbytes)
     return fail(MLORA_ERR_WORKSPACE, "qlora backward workspace needs " +
@@ -1283,8 +1515,34 @@ int mlora_qlora_backward_ex(const void* dy, const void* x, int scheme, const voi
   q.scales_t = scales_t;
   q.group = group;
   return backward16(dy, x, nullptr, &q, a, b, saved_xa, dx, da, db, M, K, N, r, alpha, clip_value,
-                    accumulate, dtype, workspace, bytes, s);
+                    accumulate, dtype, workspace, bytes, s, kPhaseAll, grads16, ckpt);
 }
+}  // namespace
+
+int mlora_qlora_backward_ex(const void* dy, const void* x, int scheme, const void* codes,
+                            const void* scales, const void* zeros, const void* prepared,
+                            int64_t group, const void* a, const void* b, const void* saved_xa,
+                            void* dx, float* da, float* db, int64_t M, int64_t K, int64_t N,
+                            int64_t r, float alpha, float clip_value, int dtype, int flags,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  return qlora_backward_any(dy, x, nullptr, scheme, codes, scales, zeros, prepared, group, a, b,
+                            saved_xa, dx, da, db, M, K, N, r, alpha, clip_value, dtype, flags,
+                            workspace, workspace_bytes, stream);
+}
+
+int mlora_qlora_backward_ckpt(const void* dy, const void* ckpt_codes, int64_t ckpt_ld,
+                              const void* ckpt_scales, int scheme, const void* codes,
+                              const void* scales, const void* zeros, const void* prepared,
+                              int64_t group, const void* a, const void* b, const void* saved_xa,
+                              void* dx, void* da, void* db, int64_t M, int64_t K, int64_t N,
+                              int64_t r, float alpha, float clip_value, int dtype, int flags,
+                              void* workspace, size_t workspace_bytes, void* stream) {
+  const Ckpt c{ckpt_codes, ckpt_ld, ckpt_scales};
+  return qlora_backward_any(dy, nullptr, &c, scheme, codes, scales, zeros, prepared, group, a, b,
+                            saved_xa, dx, da, db, M, K, N, r, alpha, clip_value, dtype, flags,
+                            workspace, workspace_bytes, stream);
+}
+
 
 size_t mlora_multi_lora_forward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r,
                                                 int64_t n, int dtype) {

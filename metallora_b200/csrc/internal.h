@@ -254,6 +254,60 @@ int launch_pack_scale_zero(const void* scales, const void* zeros, int64_t rows, 
 // rounded up to 4 so every table row starts on a 16-byte boundary (TMA).
 inline int64_t prepared_ld(int64_t rows) { return (rows + 3) / 4 * 4; }
 
+// --------------------------------------------------- microscaled formats ------
+// Scale bytes (power-of-two exponent + 127) of 32-feature blocks of `rows` rows:
+//   kMxPlain : [rows, blocks], blocks = ceil(K / 32);
+//   kMxGroups: [ceil(K / 128), rows, 4], one word per row and 128 features;
+//   kMxAtoms : [ceil(rows / 128), ceil(K / 128), 512], the fp4 product's atoms.
+enum MxLayout : int { kMxPlain = 0, kMxGroups = 1, kMxAtoms = 2 };
+struct MxScales {
+  uint8_t* data;
+  int64_t rows, blocks;
+  int layout;
+};
+// bits = 4 (MXFP4) or 8 (MXINT8); code rows start ld bytes apart.
+int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K, void* codes,
+                       int64_t ld, const MxScales& sc, cudaStream_t s);
+int launch_mx_dequantize(int bits, const void* codes, int64_t ld, const MxScales& sc, int64_t M,
+                         int64_t K, void* out, int out_dtype, cudaStream_t s);
+int launch_mx_prepare_scales(const void* scales, int64_t rows, int64_t K, void* atoms,
+                             cudaStream_t s);
+inline int64_t mx_atoms_bytes(int64_t rows, int64_t K) {
+  return (rows + 127) / 128 * ((K + 127) / 128) * 512;
+}
+
+// Y[M, N] = Q4(x) . W4^T + X2 . W2^T, both fp4 operands as codes [rows, K/2] and
+// scale atoms; x2 [M, R64] and w2 [N, r] 16-bit as in GemmArgs.
+struct MxGemmArgs {
+  const void* xq;
+  const void* xs;
+  const void* wq;
+  const void* ws;
+  const void* x2 = nullptr;
+  const void* w2 = nullptr;
+  void* d = nullptr;
+  int64_t M = 0, N = 0, K = 0, R = 0, w2_rows = 0;
+  int64_t ldx2 = 0, ldw2 = 0, ldd = 0;
+  Elt elt = Elt::kBF16;  // of x2, w2 and d
+};
+int launch_mx_gemm(const MxGemmArgs& a, cudaStream_t s);
+
+// da[j, p] = sum_m st[j, m] * x^[m, p] for an MXINT8 checkpoint x^ [M, K] (code
+// rows ld bytes apart, kMxGroups scales); output as WgradArgs (transposed).
+struct MxWgradArgs {
+  const void* codes;
+  const void* scales;
+  int64_t ld;
+  const void* st;
+  int64_t ld_st;
+  int64_t M, K, r, R;
+  void* out;
+  bool accumulate, out16;
+  float clip;
+  Elt elt;
+};
+int launch_mx_wgrad(const MxWgradArgs& a, cudaStream_t s);
+
 // ---------------------------------------------------------------- optimizer --
 int norm_grid();
 int launch_grad_norm(const float* g, int64_t n, float max_norm, float* partials,

@@ -1,0 +1,144 @@
+// Microscaled block formats (device side): one power-of-two scale X = 2^E for
+// 32 consecutive features of a row, held as the byte E + 127 (255 = NaN).
+//
+//   MXFP4 : E = max(floor(log2 amax) - 2, -127), code = e2m1(x / X) rounded to
+//           nearest even on {0, .5, 1, 1.5, 2, 3, 4, 6}, saturating at 6;
+//           two codes a byte, the even feature in the low nibble.
+//   MXINT8: E = max(floor(log2 amax), -127), code = clamp(rint(64 x / X), +-127),
+//           value = code / 64 * X.
+// amax = 0 gives byte 0 and codes 0; a block holding an infinity or a NaN gives
+// byte 255 and codes 0, so all its values read back as NaN.
+//
+// Every step is exact except the rounding to the code: X is a power of two, so
+// x / X only moves the exponent, and a value (at most 8 significant bits) is
+// exact in bf16.  In fp16 it is exact too while X >= 2^-18; below that the
+// smallest values round to fp16's subnormal grid.
+#pragma once
+
+#include <stdint.h>
+#include <cuda_fp16.h>
+
+#include "ptx.cuh"
+
+namespace mlora {
+
+constexpr int kMxBlock = 32;
+
+// The scale byte of a block from the bits of max|x| (integer maximum of the
+// absolute values' bits, which orders NaN above infinity above the finite).
+__device__ __forceinline__ uint32_t mx_scale_byte_fp4(uint32_t amax_bits) {
+  const uint32_t f = amax_bits >> 23;  // biased exponent; 0 for zero and subnormals
+  return f == 255u ? 255u : (f > 2u ? f - 2u : 0u);
+}
+__device__ __forceinline__ uint32_t mx_scale_byte_int8(uint32_t amax_bits) {
+  return amax_bits >> 23;
+}
+
+// 1 / X for a scale byte (0 for the NaN byte, whose codes are 0).
+__device__ __forceinline__ float mx_inv_scale(uint32_t byte) {
+  if (byte == 255u) return 0.f;
+  return __uint_as_float(byte == 254u ? 0x00400000u : (254u - byte) << 23);
+}
+// X for a scale byte (NaN for 255).
+__device__ __forceinline__ float mx_scale(uint32_t byte) {
+  if (byte == 255u) return __uint_as_float(0x7FC00000u);
+  return __uint_as_float(byte == 0u ? 0x00400000u : byte << 23);
+}
+
+// Eight e2m1 codes, v[0] in the lowest nibble.
+__device__ __forceinline__ uint32_t mx_pack_e2m1(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b8 b0, b1, b2, b3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+      "mov.b32 %0, {b0, b1, b2, b3};\n\t"
+      "}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// The four pairs of e2m1 values of eight codes (exact in f16).
+__device__ __forceinline__ void mx_unpack_e2m1(uint32_t w, float (&v)[8]) {
+  uint32_t h[4];
+  asm("{\n\t"
+      ".reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t"
+      "}"
+      : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+      : "r"(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// Four int8 codes of values already divided by X / 64 and clamped to +-127:
+// adding 1.5 * 2^23 rounds to the nearest integer (ties to even) and leaves
+// its two's complement in the low byte.
+__device__ __forceinline__ uint32_t mx_pack_int8(float a, float b, float c, float d) {
+  constexpr float kMagic = 12582912.f;
+  const uint32_t ua = __float_as_uint(__fadd_rn(a, kMagic)), ub = __float_as_uint(__fadd_rn(b, kMagic));
+  const uint32_t uc = __float_as_uint(__fadd_rn(c, kMagic)), ud = __float_as_uint(__fadd_rn(d, kMagic));
+  return __byte_perm(__byte_perm(ua, ub, 0x0040u), __byte_perm(uc, ud, 0x0040u), 0x5410u);
+}
+
+// --------------------------------------------------- fp4 tensor-core product --
+// tcgen05.mma kind::mxf4 (K = 64 codes a step): A and B are K-major code rows in
+// shared memory; their scale bytes sit in TMEM.  The scale bytes of 128 rows x
+// 128 features form one 512-byte atom: byte (row % 32) * 16 + (row / 32) * 4 +
+// (block % 4), which one tcgen05.cp spreads over 4 TMEM columns (lane = row %
+// 32, column = row / 32, repeated in the four lane quarters).  A K step reads
+// two of a column's four bytes, picked by the scale id (0 or 2) of the
+// instruction descriptor.
+constexpr uint32_t kMxAtomBytes = 512;
+
+// [4,6) B scale id; [7,10) a format, [10,12) b format (1 = e2m1); [17,23) N >> 3;
+// [23] scale type (1 = power of two); [27,29) M >> 7; [29,31) A scale id.
+__host__ __device__ constexpr uint32_t make_idesc_mxf4(uint32_t M, uint32_t N, uint32_t sf_id) {
+  return (sf_id << 4) | (1u << 7) | (1u << 10) | ((N >> 3) << 17) | (1u << 23) | ((M >> 7) << 27) |
+         (sf_id << 29);
+}
+
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                          uint32_t idesc, uint32_t sfa_tmem, uint32_t sfb_tmem,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], "
+      "p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// One scale atom from shared memory (16-byte aligned) to 4 TMEM columns.
+// tcgen05.cp and tcgen05.mma of one thread execute in issue order.
+__device__ __forceinline__ void tmem_cp_scale_atom(uint32_t taddr, uint32_t saddr) {
+  const uint64_t desc = make_smem_desc(saddr, 16u, 128u, kLayoutNone);
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
+}
+
+// Untiled bulk copy global -> shared (16-byte aligned addresses and size).
+__device__ __forceinline__ void bulk_load(void* smem_dst, const void* gmem_src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(gmem_src)), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+}  // namespace mlora

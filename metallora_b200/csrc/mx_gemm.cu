@@ -1,0 +1,305 @@
+// LoRA linear over an MXFP4 base on the fp4 tensor cores:
+//
+//     Y[M, N] = Q4(x) . W4^T  +  X2[M, R] . W2^T        (X2 = s x A^T, W2 = B)
+//
+// Both factors of the base product are MXFP4 (mx.cuh): tcgen05.mma kind::mxf4
+// multiplies code rows and applies the block scales itself, so nothing is
+// dequantised.  The rank-r block is appended as 16-bit kind::f16 steps into the
+// same TMEM accumulator, as in the dense kernel, so Y is written once.
+//
+// A shared-memory row of 128 bytes is 256 codes or 64 16-bit values, so both
+// kinds of k-block share one stage layout (128-byte swizzle, K-major) and one
+// ring; a main block also carries its scale atoms.
+#include <atomic>
+#include <string>
+#include <type_traits>
+
+#include "cluster_reduce.cuh"
+#include "internal.h"
+#include "mx.cuh"
+#include "../../include/metallora_b200.h"
+
+namespace mlora {
+namespace {
+
+constexpr int kBK4 = 256;                        // fp4 reduction per main k-block
+constexpr int kBK16 = 64;                        // 16-bit reduction per rank k-block
+constexpr uint32_t kRowBytes = 128;              // of either
+constexpr uint32_t kSfBytes = 2 * kMxAtomBytes;  // scales of 128 rows x 256 features
+
+// ---------------------------------------------------------------------------
+// Few tokens (M <= 128): the weight rows are the MMA's M side (128 a tile) and
+// the tokens its N side, so one pass over the weight serves all tokens.
+// Bound by the weight's HBM traffic; the reduction is split over the CTAs of a
+// cluster so that about two CTAs per SM stream it, and their partial tiles are
+// summed through distributed shared memory in fixed order (cluster_reduce).
+constexpr int kSkinnyThreads = 192;
+constexpr int kSkinnyMaxSplits = 8;
+
+__host__ __device__ constexpr uint32_t skinny_stage_bytes(int NT) {
+  return (128 + NT) * kRowBytes + 2 * kSfBytes;
+}
+__host__ __device__ constexpr int skinny_stages(int NT) {
+  return static_cast<int>((NT <= 32 ? 100u : 200u) * 1024u / skinny_stage_bytes(NT));
+}
+constexpr size_t skinny_smem(int NT) {
+  return 1024 + skinny_stages(NT) * skinny_stage_bytes(NT) + 256;
+}
+// accumulator columns, then two sets of (8 weight, 8 token) scale columns
+__host__ __device__ constexpr uint32_t skinny_acc_cols(int NT) { return NT; }
+__host__ __device__ constexpr uint32_t skinny_tmem_cols(int NT) {
+  return NT + 32 <= 64 ? 64u : (NT + 32 <= 128 ? 128u : 256u);
+}
+
+struct SkinnyParams {
+  int M, N, K;
+  int num_kb_main, num_kb_extra, R;
+  int splits;
+  int atoms_k;  // scale atoms along K per 128 rows
+  void* d;
+  long long ldd;
+  uint32_t* status;
+};
+
+// Grid (weight tiles, splits), cluster (1, splits, 1).
+template <int NT, bool kBF16>
+__global__ void __launch_bounds__(kSkinnyThreads)
+    mx_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
+                     const __grid_constant__ CUtensorMap tm_ws, const __grid_constant__ CUtensorMap tm_xs,
+                     const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ CUtensorMap tm_x2,
+                     const SkinnyParams p) {
+  using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
+  constexpr int S = skinny_stages(NT);
+  constexpr uint32_t kStage = skinny_stage_bytes(NT);
+  constexpr uint32_t kXOff = 128 * kRowBytes;
+  constexpr uint32_t kWsOff = kXOff + NT * kRowBytes;
+  constexpr uint32_t kXsOff = kWsOff + kSfBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * kStage);
+  uint64_t* empty_bar = full_bar + S;
+  uint64_t* done_bar = empty_bar + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+
+  const uint32_t warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+    mbar_init(done_bar, 1);
+    fence_mbarrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, skinny_tmem_cols(NT));
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  const int n0 = static_cast<int>(blockIdx.x) * 128;
+  const uint32_t crank = cluster_ctarank();
+  const int total_kb = p.num_kb_main + p.num_kb_extra;
+  const int per = (total_kb + p.splits - 1) / p.splits;
+  const int kb_begin = static_cast<int>(crank) * per;
+  const int kb_end = min(total_kb, kb_begin + per);
+  const bool has_work = kb_begin < kb_end;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      bool armed[S];
+      uint32_t armed_parity[S];
+      for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
+      bool prev_done = false;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
+        uint8_t* st = smem + stage * kStage;
+        uint64_t* bar = &full_bar[stage];
+        const bool extra = kb >= p.num_kb_main;
+        mbar_arrive_expect_tx(bar, extra ? (128 + NT) * kRowBytes : kStage);
+        armed[stage] = true;
+        armed_parity[stage] = phase;
+        // the weight does not come from the kernels before this one; the token
+        // operands do
+        if (extra) {
+          const int k0 = (kb - p.num_kb_main) * kBK16;
+          tma_load_2d(st, &tm_w2, bar, k0, n0);
+        } else {
+          tma_load_2d(st, &tm_w, bar, kb * static_cast<int>(kRowBytes), n0);
+          tma_load_2d(st + kWsOff, &tm_ws, bar, 0, static_cast<int>(blockIdx.x) * p.atoms_k + 2 * kb);
+        }
+        if (!prev_done) {
+          asm volatile("griddepcontrol.wait;" ::: "memory");
+          prev_done = true;
+        }
+        if (extra) {
+          tma_load_2d(st + kXOff, &tm_x2, bar, (kb - p.num_kb_main) * kBK16, 0);
+        } else {
+          tma_load_2d(st + kXOff, &tm_x, bar, kb * static_cast<int>(kRowBytes), 0);
+          tma_load_2d(st + kXsOff, &tm_xs, bar, 0, 2 * kb);
+        }
+        if (++stage == S) stage = 0, phase ^= 1u;
+      }
+      for (int s = 0; s < S; ++s)
+        if (armed[s]) mbar_wait(&full_bar[s], armed_parity[s], p.status, kDevTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (has_work && elect_one()) {
+      constexpr uint32_t idesc16 = make_idesc_f16(128, NT, false, false, kBF16);
+      uint32_t stage = 0, phase = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) break;
+        tc_fence_after();
+        const uint32_t sw = smem_u32(smem + stage * kStage);
+        const uint32_t sx = sw + kXOff;
+        const uint32_t first = kb == kb_begin ? 0u : 1u;
+        if (kb >= p.num_kb_main) {
+          const int rem = p.R - (kb - p.num_kb_main) * kBK16;
+          const int nk = rem >= kBK16 ? 4 : rem / 16;
+          for (int k = 0; k < nk; ++k)
+            umma_f16(tmem, desc_kmajor_sw128(sw, k), desc_kmajor_sw128(sx, k), idesc16,
+                     first | static_cast<uint32_t>(k != 0));
+        } else {
+          const uint32_t sfa = tmem + skinny_acc_cols(NT) + static_cast<uint32_t>(kb & 1) * 16u;
+          const uint32_t sfb = sfa + 8u;
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            tmem_cp_scale_atom(sfa + 4 * a, sw + kWsOff + a * kMxAtomBytes);
+            tmem_cp_scale_atom(sfb + 4 * a, sw + kXsOff + a * kMxAtomBytes);
+          }
+          // codes past K are zero-filled; a step that lies past K entirely would
+          // also read scales that belong to other rows, so it is left out
+          const int nk = min(4, (p.K - kb * kBK4 + 63) / 64);
+          for (int k = 0; k < nk; ++k)
+            umma_mxf4(tmem, desc_kmajor_sw128(sw, k), desc_kmajor_sw128(sx, k),
+                      make_idesc_mxf4(128, NT, 2u * (k & 1)), sfa + 4 * (k >> 1), sfb + 4 * (k >> 1),
+                      first | static_cast<uint32_t>(k != 0));
+        }
+        umma_commit(&empty_bar[stage]);
+        if (++stage == S) stage = 0, phase ^= 1u;
+      }
+      umma_commit(done_bar);
+    }
+  }
+  const bool epi = warp >= 2;
+  const int row_local = static_cast<int>((warp & 3u) * 32 + lane_id());
+  const int n = n0 + row_local;
+  bool have = false;
+  if (epi && has_work) {
+    have = mbar_wait(done_bar, 0, p.status, kDevTimeoutAccFull);
+    tc_fence_after();
+  }
+  T* const out = reinterpret_cast<T*>(p.d) + n;
+  const bool live = epi && n < p.N;
+  auto emit = [&](int j, float v0, float v1) {
+    if (!live) return;
+    if (j < p.M) out[j * p.ldd] = static_cast<T>(v0);
+    if (j + 1 < p.M) out[(j + 1) * p.ldd] = static_cast<T>(v1);
+  };
+  cluster_reduce<NT>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
+                     reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, skinny_tmem_cols(NT));
+  }
+}
+
+int cuda_launch_error(cudaError_t e, const char* what) {
+  set_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return MLORA_ERR_CUDA;
+}
+
+// Tensor maps of an fp4 operand: code rows [rows, K/2] and scale atoms.
+bool map_codes(CUtensorMap* m, const void* codes, int64_t rows, int64_t K, uint32_t box_rows) {
+  return make_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, static_cast<uint64_t>(K / 2),
+                      static_cast<uint64_t>(rows), static_cast<uint64_t>(K / 2), kRowBytes, box_rows,
+                      true);
+}
+bool map_atoms(CUtensorMap* m, const void* atoms, int64_t rows, int64_t K) {
+  const uint64_t n = static_cast<uint64_t>(mx_atoms_bytes(rows, K) / kMxAtomBytes);
+  return make_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, atoms, kMxAtomBytes / 4, n, kMxAtomBytes,
+                      kMxAtomBytes / 4, 2, false);
+}
+
+template <int NT, bool kBF16>
+int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
+  CUtensorMap tw, tx, tws, txs, tw2, tx2;
+  if (!map_codes(&tw, a.wq, a.N, a.K, 128) || !map_codes(&tx, a.xq, a.M, a.K, NT) ||
+      !map_atoms(&tws, a.ws, a.N, a.K) || !map_atoms(&txs, a.xs, a.M, a.K))
+    return MLORA_ERR_INVALID_ARG;
+  if (a.R > 0) {
+    const int64_t r64 = (a.R + 63) / 64 * 64;
+    if (!make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, 128) ||
+        !make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, NT))
+      return MLORA_ERR_INVALID_ARG;
+  } else {
+    tw2 = tw;
+    tx2 = tx;
+  }
+  SkinnyParams p;
+  p.M = static_cast<int>(a.M);
+  p.N = static_cast<int>(a.N);
+  p.K = static_cast<int>(a.K);
+  p.num_kb_main = static_cast<int>((a.K + kBK4 - 1) / kBK4);
+  p.R = static_cast<int>(a.R);
+  p.num_kb_extra = static_cast<int>((a.R + kBK16 - 1) / kBK16);
+  p.atoms_k = static_cast<int>((a.K + 127) / 128);
+  p.d = a.d;
+  p.ldd = a.ldd;
+  p.status = device_status_ptr();
+  const int64_t tiles = (a.N + 127) / 128;
+  const int64_t slots = (NT <= 32 ? 2 : 1) * static_cast<int64_t>(num_sms());
+  int splits = 1;
+  while (splits * 2 <= kSkinnyMaxSplits && splits * 2 * tiles <= slots &&
+         splits * 4 <= p.num_kb_main + p.num_kb_extra)
+    splits *= 2;
+  p.splits = splits;
+  auto kern = mx_skinny_kernel<NT, kBF16>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(skinny_smem(NT)));
+  if (e != cudaSuccess) return cuda_launch_error(e, "cudaFuncSetAttribute(mx skinny)");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits));
+  cfg.blockDim = dim3(kSkinnyThreads);
+  cfg.dynamicSmemBytes = skinny_smem(NT);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = static_cast<unsigned>(splits);
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LaunchScope scope(kKindGemm, stream);
+  e = cudaLaunchKernelEx(&cfg, kern, tw, tx, tws, txs, tw2, tx2, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx skinny launch");
+}
+
+template <bool kBF16>
+int dispatch(const MxGemmArgs& a, cudaStream_t s) {
+  if (a.M <= 16) return launch_skinny<16, kBF16>(a, s);
+  if (a.M <= 32) return launch_skinny<32, kBF16>(a, s);
+  if (a.M <= 64) return launch_skinny<64, kBF16>(a, s);
+  return launch_skinny<128, kBF16>(a, s);
+}
+
+}  // namespace
+
+int launch_mx_gemm(const MxGemmArgs& args, cudaStream_t s) {
+  for (int64_t m0 = 0; m0 < args.M; m0 += 128) {
+    MxGemmArgs a = args;
+    a.M = args.M - m0 < 128 ? args.M - m0 : 128;
+    a.xq = static_cast<const uint8_t*>(args.xq) + m0 * (args.K / 2);
+    a.xs = static_cast<const uint8_t*>(args.xs) + mx_atoms_bytes(m0, args.K);
+    a.x2 = static_cast<const uint8_t*>(args.x2) + m0 * args.ldx2 * 2;
+    a.d = static_cast<uint8_t*>(args.d) + m0 * args.ldd * 2;
+    const int rc = a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
+    if (rc) return rc;
+  }
+  return MLORA_OK;
+}
+
+}  // namespace mlora

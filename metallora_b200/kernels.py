@@ -35,6 +35,14 @@ def _need_cuda(*ts: torch.Tensor) -> None:
             raise DeviceError("metallora_b200 kernels take CUDA tensors (no CPU fallback)")
 
 
+def _need_current(*ts: torch.Tensor) -> None:
+    """Launches go to the current device: tensors of another one are refused."""
+    cur = torch.cuda.current_device()
+    for t in ts:
+        if t is not None and t.get_device() != cur:
+            raise DeviceError(f"tensor on {t.device}, but cuda:{cur} is the current device")
+
+
 def _dtype_code(t: torch.Tensor) -> int:
     try:
         return _DT[t.dtype]
@@ -119,6 +127,30 @@ def lora_linear_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor, b: tor
     return y, saved
 
 
+def _as_ckpt(x, saved_xa, dy2d):
+    """``x`` if it is an activation checkpoint the backward can take, else None."""
+    if torch.is_tensor(x):
+        return None
+    x.check()
+    _need_cuda(dy2d, x.codes)
+    _need_current(dy2d, x.codes)
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise ShapeError("a checkpointed backward takes bf16/fp16 activations")
+    if saved_xa is None:
+        raise ShapeError("a checkpointed backward needs the forward's saved_xa")
+    return x
+
+
+def _ckpt_args(ckpt):
+    return _ptr(ckpt.codes), ckpt.codes.stride(0), _ptr(ckpt.scales)
+
+
+def _check_saved(saved_xa, r: int, M: int, dtype: torch.dtype) -> None:
+    _check_2d("saved_xa", saved_xa, (rank_tile(r), (M + 7) // 8 * 8), dtype)
+    if not saved_xa.is_contiguous():
+        raise ShapeError("saved_xa must be contiguous")
+
+
 def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | None,
                     a: torch.Tensor, b: torch.Tensor, alpha: float,
                     saved_xa: torch.Tensor | None = None, clip_value: float = 0.0,
@@ -132,11 +164,14 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
     > 0 clips them elementwise after the full reduction (ops.py:155).  With ``da_out`` and
     ``db_out`` (contiguous fp32 [r, K] / [N, r], rank a multiple of 8) the
     gradients are ADDED into those buffers (written over them when
-    ``accumulate`` is False) and returned."""
-    _need_cuda(dy2d, x2d, a, b)
+    ``accumulate`` is False) and returned.  ``x2d`` may be an MXINT8
+    ``quant.ActivationCheckpoint`` of x: dA is then taken from its values, and
+    ``saved_xa`` is required."""
+    ckpt = _as_ckpt(x2d, saved_xa, dy2d)
+    _need_cuda(dy2d, a, b) if ckpt is not None else _need_cuda(dy2d, x2d, a, b)
     dt = x2d.dtype
     code = _dtype_code(x2d)
-    M, K = x2d.shape
+    M, K = x2d.shape if ckpt is None else (ckpt.rows, ckpt.shape[-1])
     N = dy2d.shape[1]
     r_orig = a.shape[0]
     a_p, b_p, alpha_p, r = _pad_rank(a, b, alpha)
@@ -145,12 +180,16 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
     _check_2d("grad_output", dy2d, (M, N), dt)
     _check_2d("A", a_p, (r, K), dt)
     _check_2d("B", b_p, (N, r), dt)
+    if saved_xa is not None:
+        _check_saved(saved_xa, r, M, dt)
     if need_dx:
         if w0 is None:
             raise ShapeError("dx needs W0")
         _check_2d("W0", w0, (N, K), dt)
         w0 = w0.contiguous()
-    dy2d, x2d, a_p, b_p = (t.contiguous() for t in (dy2d, x2d, a_p, b_p))
+    dy2d, a_p, b_p = dy2d.contiguous(), a_p.contiguous(), b_p.contiguous()
+    if ckpt is None:
+        x2d = x2d.contiguous()
     lib = _lib.load()
     dx = torch.empty((M, K), dtype=dt, device=x2d.device) if need_dx else None
     flags = 0
@@ -178,10 +217,13 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
             return dx, da, db
         return dx, da[:r_orig].contiguous(), db[:, :r_orig].contiguous()
     ws = _workspace(lib.mlora_lora_backward_workspace_bytes(M, K, N, r, code), x2d.device)
-    st = lib.mlora_lora_backward_ex(_ptr(dy2d), _ptr(x2d), _ptr(w0) if need_dx else None,
-                                    _ptr(a_p), _ptr(b_p), _ptr(saved_xa), _ptr(dx), _ptr(da),
-                                    _ptr(db), M, K, N, r, float(alpha_p), float(clip_value), code,
-                                    flags, _ptr(ws), ws.numel(), _stream())
+    tail = (_ptr(w0) if need_dx else None, _ptr(a_p), _ptr(b_p), _ptr(saved_xa), _ptr(dx), _ptr(da),
+            _ptr(db), M, K, N, r, float(alpha_p), float(clip_value), code, flags, _ptr(ws),
+            ws.numel(), _stream())
+    if ckpt is not None:
+        st = lib.mlora_lora_backward_ckpt(_ptr(dy2d), *_ckpt_args(ckpt), *tail)
+    else:
+        st = lib.mlora_lora_backward_ex(_ptr(dy2d), _ptr(x2d), *tail)
     _lib.check(st, "mlora_lora_backward")
     if into:
         return dx, da, db
@@ -199,13 +241,15 @@ def lora_linear_bwd_split(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tenso
     ``da_out``/``db_out`` (fp32, added or written as ``accumulate`` says) --
     and returns ``finish``, which enqueues the dx GEMM and returns dx.  Work
     that needs only dA/dB (a gradient exchange on another stream) can be
-    started between the two and overlaps the GEMM."""
-    _need_cuda(dy2d, x2d, a, b)
+    started between the two and overlaps the GEMM.  ``x2d`` may be an activation
+    checkpoint, as for ``lora_linear_bwd``."""
+    ckpt = _as_ckpt(x2d, saved_xa, dy2d)
+    _need_cuda(dy2d, a, b) if ckpt is not None else _need_cuda(dy2d, x2d, a, b)
     dt = x2d.dtype
     if dt == torch.float32:
         raise ShapeError("the split backward takes bf16/fp16 tensors")
     code = _dtype_code(x2d)
-    M, K = x2d.shape
+    M, K = x2d.shape if ckpt is None else (ckpt.rows, ckpt.shape[-1])
     N = dy2d.shape[1]
     r = a.shape[0]
     if r % 8:
@@ -217,7 +261,11 @@ def lora_linear_bwd_split(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tenso
     for name, t, shp in (("da_out", da_out, (r, K)), ("db_out", db_out, (N, r))):
         if t.dtype != torch.float32 or tuple(t.shape) != shp or not t.is_contiguous():
             raise ShapeError(f"{name} must be a contiguous fp32 tensor of shape {shp}")
-    dy2d, x2d, w0, a, b = (t.contiguous() for t in (dy2d, x2d, w0, a, b))
+    dy2d, w0, a, b = (t.contiguous() for t in (dy2d, w0, a, b))
+    if ckpt is None:
+        x2d = x2d.contiguous()
+    else:
+        _check_saved(saved_xa, r, M, dt)
     lib = _lib.load()
     dx = torch.empty((M, K), dtype=dt, device=x2d.device)
     ws = _workspace(lib.mlora_lora_backward_workspace_bytes(M, K, N, r, code), x2d.device)
@@ -229,10 +277,12 @@ def lora_linear_bwd_split(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tenso
         return lambda: dx
 
     def call(phase):
-        st = lib.mlora_lora_backward_ex(_ptr(dy2d), _ptr(x2d), _ptr(w0), _ptr(a), _ptr(b),
-                                        _ptr(saved_xa), _ptr(dx), _ptr(da_out), _ptr(db_out), M, K,
-                                        N, r, float(alpha), 0.0, code, flags | phase, _ptr(ws),
-                                        ws.numel(), _stream())
+        tail = (_ptr(w0), _ptr(a), _ptr(b), _ptr(saved_xa), _ptr(dx), _ptr(da_out), _ptr(db_out),
+                M, K, N, r, float(alpha), 0.0, code, flags | phase, _ptr(ws), ws.numel(), _stream())
+        if ckpt is not None:
+            st = lib.mlora_lora_backward_ckpt(_ptr(dy2d), *_ckpt_args(ckpt), *tail)
+        else:
+            st = lib.mlora_lora_backward_ex(_ptr(dy2d), _ptr(x2d), *tail)
         _lib.check(st, "mlora_lora_backward_ex")
 
     call(_lib.BWD_DEFER_DX)
@@ -372,25 +422,36 @@ def _qlora_ws_bytes(lib, qw, M, K, N, r, backward, need_w=True):
     return fn(M, K, N, r, qw.code, qw.group)
 
 
+def _qlora_dtype(x2d, qw) -> torch.dtype:
+    """The activations' dtype, checked against what the base's scheme takes."""
+    if getattr(qw, "scheme", None) == "mxfp4":
+        if x2d.dtype not in (torch.bfloat16, torch.float16):
+            raise ShapeError("an MXFP4 base takes bf16 or fp16 activations")
+        _need_current(x2d if torch.is_tensor(x2d) else x2d.codes, qw.codes)
+    elif x2d.dtype != torch.bfloat16:
+        raise ShapeError("quantised-base LoRA takes bf16 activations")
+    return x2d.dtype
+
+
 def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, alpha: float,
                      save_xa: bool = False):
     """y = x.deq(W)^T + (alpha/r).(x.A^T).B^T for a quantised base ``qw``
     (metallora_b200.quant.QuantizedWeight); x, A, B bf16.  ``qw.lean`` selects
-    the fused kernel that dequantises in its main loop (no dense copy of W)."""
+    the fused kernel that dequantises in its main loop (no dense copy of W).
+    An MXFP4 base takes bf16 or fp16 and multiplies x rounded to MXFP4."""
     _need_cuda(x2d, a, b)
-    if x2d.dtype != torch.bfloat16:
-        raise ShapeError("quantised-base LoRA takes bf16 activations")
+    dt = _qlora_dtype(x2d, qw)
     M, K = x2d.shape
     N = qw.shape[0]
     if qw.shape[1] != K:
         raise ShapeError(f"x has {K} features, the quantised weight {qw.shape[1]}")
     a, b, alpha, r = _pad_rank(a, b, alpha)
-    _check_2d("A", a, (r, K), torch.bfloat16)
-    _check_2d("B", b, (N, r), torch.bfloat16)
+    _check_2d("A", a, (r, K), dt)
+    _check_2d("B", b, (N, r), dt)
     x2d, a, b = x2d.contiguous(), a.contiguous(), b.contiguous()
-    y = torch.empty((M, N), dtype=torch.bfloat16, device=x2d.device)
-    saved = (torch.empty((rank_tile(r), (M + 7) // 8 * 8), dtype=torch.bfloat16,
-                         device=x2d.device) if save_xa else None)
+    y = torch.empty((M, N), dtype=dt, device=x2d.device)
+    saved = (torch.empty((rank_tile(r), (M + 7) // 8 * 8), dtype=dt, device=x2d.device)
+             if save_xa else None)
     if M == 0:  # no tokens: empty output, nothing to launch
         return y, saved
     lib = _lib.load()
@@ -398,7 +459,7 @@ def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, al
     st = lib.mlora_qlora_forward_ex(_ptr(x2d), qw.code, _ptr(qw.codes), _ptr(qw.scales),
                                     _ptr(qw.zeros), _ptr(qw.prepared_scales()), qw.group, _ptr(a),
                                     _ptr(b), _ptr(y), _ptr(saved), M, K, N, r, float(alpha),
-                                    _lib.DTYPE_BF16, _ptr(ws), ws.numel(), _stream())
+                                    _dtype_code(x2d), _ptr(ws), ws.numel(), _stream())
     _lib.check(st, "mlora_qlora_forward_ex")
     return y, saved
 
@@ -406,20 +467,28 @@ def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, al
 def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor,
                      alpha: float, saved_xa: torch.Tensor | None = None, clip_value: float = 0.0,
                      need_dx: bool = True, da_out: torch.Tensor | None = None,
-                     db_out: torch.Tensor | None = None, accumulate: bool = True):
+                     db_out: torch.Tensor | None = None, accumulate: bool = True,
+                     grad_dtype: torch.dtype | None = None):
     """(dx, dA, dB) through a frozen quantised base (staged or lean as the forward);
-    ``da_out``/``db_out``/``accumulate`` as in ``lora_linear_bwd``."""
-    _need_cuda(dy2d, x2d, a, b)
-    M, K = x2d.shape
+    ``da_out``/``db_out``/``accumulate``/``grad_dtype`` and an activation
+    checkpoint in the place of ``x2d`` as in ``lora_linear_bwd``."""
+    ckpt = _as_ckpt(x2d, saved_xa, dy2d)
+    _need_cuda(dy2d, a, b) if ckpt is not None else _need_cuda(dy2d, x2d, a, b)
+    dt = _qlora_dtype(x2d, qw)
+    M, K = x2d.shape if ckpt is None else (ckpt.rows, ckpt.shape[-1])
     N = dy2d.shape[1]
     r_orig = a.shape[0]
     a_p, b_p, alpha_p, r = _pad_rank(a, b, alpha)
-    _check_2d("grad_output", dy2d, (M, N), torch.bfloat16)
-    _check_2d("A", a_p, (r, K), torch.bfloat16)
-    _check_2d("B", b_p, (N, r), torch.bfloat16)
-    dy2d, x2d, a_p, b_p = (t.contiguous() for t in (dy2d, x2d, a_p, b_p))
+    _check_2d("grad_output", dy2d, (M, N), dt)
+    _check_2d("A", a_p, (r, K), dt)
+    _check_2d("B", b_p, (N, r), dt)
+    dy2d, a_p, b_p = dy2d.contiguous(), a_p.contiguous(), b_p.contiguous()
+    if ckpt is None:
+        x2d = x2d.contiguous()
+    else:
+        _check_saved(saved_xa, r, M, dt)
     lib = _lib.load()
-    dx = torch.empty((M, K), dtype=torch.bfloat16, device=x2d.device) if need_dx else None
+    dx = torch.empty((M, K), dtype=dt, device=x2d.device) if need_dx else None
     flags = 0
     into = da_out is not None or db_out is not None
     if into:
@@ -428,8 +497,11 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
         da, db = da_out, db_out
         flags = _lib.BWD_ACCUMULATE if accumulate else 0
     else:
-        da = torch.empty((r, K), dtype=torch.float32, device=x2d.device)
-        db = torch.empty((N, r), dtype=torch.float32, device=x2d.device)
+        gdt = torch.float32
+        if grad_dtype is not None and grad_dtype == dt:
+            gdt, flags = dt, _lib.BWD_GRADS_16BIT
+        da = torch.empty((r, K), dtype=gdt, device=x2d.device)
+        db = torch.empty((N, r), dtype=gdt, device=x2d.device)
     if M == 0:  # no tokens: the sums over tokens are zero; nothing to launch
         if not (into and accumulate):
             da.zero_()
@@ -439,12 +511,15 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
         return dx, da[:r_orig].contiguous(), db[:, :r_orig].contiguous()
     ws = _workspace(_qlora_ws_bytes(lib, qw, M, K, N, r, backward=True, need_w=need_dx),
                     x2d.device)
-    st = lib.mlora_qlora_backward_ex(_ptr(dy2d), _ptr(x2d), qw.code, _ptr(qw.codes),
-                                     _ptr(qw.scales), _ptr(qw.zeros),
-                                     _ptr(qw.prepared_scales()) if need_dx else None, qw.group,
-                                     _ptr(a_p), _ptr(b_p), _ptr(saved_xa), _ptr(dx), _ptr(da),
-                                     _ptr(db), M, K, N, r, float(alpha_p), float(clip_value),
-                                     _lib.DTYPE_BF16, flags, _ptr(ws), ws.numel(), _stream())
+    tail = (qw.code, _ptr(qw.codes), _ptr(qw.scales), _ptr(qw.zeros),
+            _ptr(qw.prepared_scales()) if need_dx and qw.scheme != "mxfp4" else None, qw.group,
+            _ptr(a_p), _ptr(b_p), _ptr(saved_xa), _ptr(dx), _ptr(da), _ptr(db), M, K, N, r,
+            float(alpha_p), float(clip_value), _dtype_code(x2d), flags, _ptr(ws), ws.numel(),
+            _stream())
+    if ckpt is not None:
+        st = lib.mlora_qlora_backward_ckpt(_ptr(dy2d), *_ckpt_args(ckpt), *tail)
+    else:
+        st = lib.mlora_qlora_backward_ex(_ptr(dy2d), _ptr(x2d), *tail)
     _lib.check(st, "mlora_qlora_backward_ex")
     if into:
         return dx, da, db

@@ -25,11 +25,14 @@ class LoRALinear(nn.Module):
     Parameters mirror the reference (layers.py:41-50); ``device``/``dtype``
     are the usual torch factory arguments.  ``W0`` is a frozen ``Parameter``
     when ``freeze_base`` (the reference stops its gradient, layers.py:77-78).
+    ``activation_checkpoint="mxint8"`` keeps the input for the backward in 8
+    bits (see ``ops.lora_forward``); ``forward(x, checkpoint=c)`` uses one made
+    by ``quant.checkpoint_activation`` that several layers share.
     """
 
     def __init__(self, in_features: int, out_features: int, rank: int = 8, alpha: float = 16.0,
                  dropout: float = 0.0, use_bias: bool = False, freeze_base: bool = True,
-                 device=None, dtype=None):
+                 device=None, dtype=None, activation_checkpoint: str | None = None):
         super().__init__()
         if in_features <= 0:
             raise ConfigurationError(f"in_features must be positive, got {in_features}")
@@ -38,6 +41,8 @@ class LoRALinear(nn.Module):
         validate_rank(rank)
         validate_alpha(alpha)
         validate_probability(dropout, "dropout")
+        if activation_checkpoint not in (None, "mxint8"):
+            raise ConfigurationError(f"unknown activation checkpoint {activation_checkpoint!r}")
 
         self.in_features = in_features
         self.out_features = out_features
@@ -46,6 +51,7 @@ class LoRALinear(nn.Module):
         self.dropout = dropout
         self.freeze_base = freeze_base
         self.merged = False
+        self.activation_checkpoint = activation_checkpoint
 
         fk = {"device": device, "dtype": dtype}
         self.W0 = nn.Parameter(torch.zeros((out_features, in_features), **fk),
@@ -70,18 +76,21 @@ class LoRALinear(nn.Module):
     def scale(self) -> float:
         return self.alpha / self.rank
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, checkpoint=None) -> torch.Tensor:
         """layers.py:83-106: any leading shape; the bias is added after the op."""
+        if checkpoint is None and torch.is_grad_enabled():
+            checkpoint = self.activation_checkpoint
         if self.qweight is not None:
             out = qlora_forward(x, self.qweight, self.A, self.B, alpha=self.alpha,
-                                _compute=self._compute_ab, _sink=self._grad_sink)
+                                _compute=self._compute_ab, _sink=self._grad_sink,
+                                checkpoint=checkpoint)
         elif self.merged:
             out = _k.linear(x.reshape(-1, x.shape[-1]), self.W0).reshape(*x.shape[:-1],
                                                                          self.out_features)
         else:
             out = lora_forward(x, self.W0, self.A, self.B, alpha=self.alpha, dropout=self.dropout,
                                training=self.training, _compute=self._compute_ab,
-                               _sink=self._grad_sink)
+                               _sink=self._grad_sink, checkpoint=checkpoint)
         if self.bias is not None:
             out = out + self.bias
         return out
@@ -121,8 +130,8 @@ class LoRALinear(nn.Module):
     def quantize_base(self, scheme: str = "nf4", group: int | None = None,
                       lean: bool = False) -> "LoRALinear":
         """Replaces the frozen base W0 by its quantised form (QLoRA): NF4 with
-        per-block absmax, or group-wise INT4/INT8 (the formats of
-        kernels/lora_quantized.metal).  The dense W0 is released.  ``lean``
+        per-block absmax, group-wise INT4/INT8 (the formats of
+        kernels/lora_quantized.metal), or MXFP4.  The dense W0 is released.  ``lean``
         keeps the per-call workspace free of a dequantised copy (see
         metallora_b200.quant.quantize)."""
         from .quant import quantize

@@ -11,7 +11,43 @@ from __future__ import annotations
 import torch
 
 from . import kernels as _k
-from .exceptions import ShapeError
+from .exceptions import ConfigurationError, ShapeError
+
+
+def _checkpoint(x2d, checkpoint):
+    """The activation checkpoint of ``x2d`` that ``checkpoint`` asks for: None,
+    "mxint8" (made here), or one the caller made of the same x."""
+    from .quant import ActivationCheckpoint, checkpoint_activation
+    if checkpoint is None:
+        return None
+    if x2d.dtype not in (torch.bfloat16, torch.float16):
+        raise ConfigurationError("activation checkpoints take bf16 or fp16 activations")
+    if isinstance(checkpoint, ActivationCheckpoint):
+        checkpoint.check()
+        if checkpoint.rows != x2d.shape[0] or checkpoint.shape[-1] != x2d.shape[1] or \
+                checkpoint.dtype != x2d.dtype or checkpoint.device != x2d.device:
+            raise ShapeError(f"the checkpoint is of {tuple(checkpoint.shape)} {checkpoint.dtype} on "
+                             f"{checkpoint.device}, x is {tuple(x2d.shape)} {x2d.dtype} on "
+                             f"{x2d.device}")
+        return checkpoint
+    if checkpoint != "mxint8":
+        raise ConfigurationError(f"unknown activation checkpoint {checkpoint!r}; use 'mxint8' or "
+                                 "an ActivationCheckpoint")
+    return checkpoint_activation(x2d)
+
+
+def _keep_x(ctx, x2d, ckpt) -> tuple:
+    """What the forward saves of x: (x, None), or the checkpoint's codes and
+    scales (rebuilt by ``_kept_x``)."""
+    ctx.x_meta = None if ckpt is None else (tuple(x2d.shape), x2d.dtype)
+    return (x2d, None) if ckpt is None else (ckpt.codes, ckpt.scales)
+
+
+def _kept_x(ctx, x2d, scales):
+    if ctx.x_meta is None:
+        return x2d
+    from .quant import ActivationCheckpoint
+    return ActivationCheckpoint(x2d, scales, *ctx.x_meta)
 
 
 def _sink_accumulates(sink) -> bool:
@@ -34,10 +70,10 @@ class _LoRALinearFn(torch.autograd.Function):
     exchange) overlaps that GEMM."""
 
     @staticmethod
-    def forward(ctx, x2d, w0, a, b, alpha, compute, sink):
+    def forward(ctx, x2d, w0, a, b, alpha, compute, sink, checkpoint=None):
         a_c, b_c = compute if compute is not None else (a.to(x2d.dtype), b.to(x2d.dtype))
         y, saved = _k.lora_linear_fwd(x2d, w0, a_c, b_c, alpha, save_xa=True)
-        ctx.save_for_backward(x2d, w0, a_c, b_c, saved)
+        ctx.save_for_backward(*_keep_x(ctx, x2d, _checkpoint(x2d, checkpoint)), w0, a_c, b_c, saved)
         ctx.alpha = alpha
         ctx.sink = sink
         ctx.ab_dtypes = (a.dtype, b.dtype)
@@ -45,7 +81,8 @@ class _LoRALinearFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x2d, w0, a_c, b_c, saved = ctx.saved_tensors
+        x2d, scales, w0, a_c, b_c, saved = ctx.saved_tensors
+        x2d = _kept_x(ctx, x2d, scales)
         need_dx = ctx.needs_input_grad[0]
         sink = ctx.sink
         on_grads = sink[3] if sink is not None and len(sink) > 3 else None
@@ -72,10 +109,10 @@ class _LoRALinearFn(torch.autograd.Function):
         if dx is not None and not need_dx:
             dx = None
         if sink is not None:
-            return dx, dw0, None, None, None, None, None
+            return dx, dw0, None, None, None, None, None, None
         da = da.to(ctx.ab_dtypes[0]) if ctx.needs_input_grad[2] else None
         db = db.to(ctx.ab_dtypes[1]) if ctx.needs_input_grad[3] else None
-        return dx, dw0, da, db, None, None, None
+        return dx, dw0, da, db, None, None, None, None
 
 
 class _QLoRALinearFn(torch.autograd.Function):
@@ -83,60 +120,80 @@ class _QLoRALinearFn(torch.autograd.Function):
     the base; A/B handled as in _LoRALinearFn."""
 
     @staticmethod
-    def forward(ctx, x2d, a, b, qw, alpha, compute, sink):
+    def forward(ctx, x2d, a, b, qw, alpha, compute, sink, checkpoint=None):
         a_c, b_c = compute if compute is not None else (a.to(x2d.dtype), b.to(x2d.dtype))
         y, saved = _k.qlora_linear_fwd(x2d, qw, a_c, b_c, alpha, save_xa=True)
-        ctx.save_for_backward(x2d, a_c, b_c, saved)
+        ctx.save_for_backward(*_keep_x(ctx, x2d, _checkpoint(x2d, checkpoint)), a_c, b_c, saved)
         ctx.qw, ctx.alpha, ctx.sink = qw, alpha, sink
         ctx.ab_dtypes = (a.dtype, b.dtype)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x2d, a_c, b_c, saved = ctx.saved_tensors
+        x2d, scales, a_c, b_c, saved = ctx.saved_tensors
+        x2d = _kept_x(ctx, x2d, scales)
         sink = ctx.sink
         need_dx = ctx.needs_input_grad[0]
+        # 16-bit gradients straight from the kernel where no cast would follow
+        same = ctx.qw.scheme == "mxfp4" and ctx.ab_dtypes[0] == ctx.ab_dtypes[1] == x2d.dtype
         dx, da, db = _k.qlora_linear_bwd(dy.contiguous(), x2d, ctx.qw, a_c, b_c, ctx.alpha, saved,
                                          0.0, need_dx=need_dx,
                                          da_out=sink[0] if sink else None,
                                          db_out=sink[1] if sink else None,
-                                         accumulate=_sink_accumulates(sink))
+                                         accumulate=_sink_accumulates(sink),
+                                         grad_dtype=x2d.dtype if same else None)
         if sink is not None and len(sink) > 3 and sink[3] is not None:
             sink[3]()
         if sink is not None:
-            return dx, None, None, None, None, None, None
+            return dx, None, None, None, None, None, None, None
         da = da.to(ctx.ab_dtypes[0]) if ctx.needs_input_grad[1] else None
         db = db.to(ctx.ab_dtypes[1]) if ctx.needs_input_grad[2] else None
-        return dx, da, db, None, None, None, None
+        return dx, da, db, None, None, None, None, None
 
 
-def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=None):  # noqa: N803
+def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=None,  # noqa: N803
+                  checkpoint=None):
     """LoRA forward over a quantised base (``quant.QuantizedWeight``):
     ``x.deq(W)^T + (alpha/rank).(x.A^T).B^T`` with the dequantisation fused
-    into the GEMM (replaces qlora_forward_nf4/int4, lora_quantized.metal:29-164)."""
+    into the GEMM (replaces qlora_forward_nf4/int4, lora_quantized.metal:29-164).
+    An MXFP4 base multiplies x rounded to MXFP4 (the gradient passes straight
+    through that rounding).  ``checkpoint`` as for ``lora_forward``."""
     shp = x.shape
-    out = _QLoRALinearFn.apply(x.reshape(-1, shp[-1]), A, B, qweight, float(alpha), _compute,
-                               _sink)
+    x2d = x.reshape(-1, shp[-1])
+    if qweight.scheme == "mxfp4" and not (torch.is_grad_enabled() and
+                                          (x.requires_grad or A.requires_grad or B.requires_grad)):
+        a, b = _compute if _compute is not None else (A.to(x.dtype), B.to(x.dtype))
+        out = _k.qlora_linear_fwd(x2d, qweight, a, b, float(alpha))[0]
+    else:
+        out = _QLoRALinearFn.apply(x2d, A, B, qweight, float(alpha), _compute, _sink, checkpoint)
     return out.reshape(*shp[:-1], qweight.shape[0])
 
 
-def _apply(x2d, W0, A, B, alpha, compute=None, sink=None):
-    return _LoRALinearFn.apply(x2d, W0, A, B, float(alpha), compute, sink)
+def _apply(x2d, W0, A, B, alpha, compute=None, sink=None, checkpoint=None):
+    return _LoRALinearFn.apply(x2d, W0, A, B, float(alpha), compute, sink, checkpoint)
 
 
 def lora_forward(x, W0, A, B, alpha: float = 16.0, dropout: float = 0.0,  # noqa: N803
                  training: bool = False, use_metal: bool = True, kernel_kwargs: dict | None = None,
-                 _compute=None, _sink=None):
+                 _compute=None, _sink=None, checkpoint=None):
     """LoRA forward ``h = x.W0^T + (alpha/rank).(x.A^T).B^T`` (ops.py:32-103).
 
     x is [batch, seq, in] or [seq, in] (any leading shape works); rank is read
     from ``B.shape[1]`` (ops.py:73).  With ``training`` and ``dropout > 0`` the
     dropout mask multiplies the LoRA term only, as at ops.py:96-98.
+
+    ``checkpoint`` keeps x for the backward in 8 bits instead of 16: "mxint8"
+    quantises it here, a ``quant.ActivationCheckpoint`` of x is used as it is
+    (layers that share an input share one).  dA then comes from the
+    checkpoint's values; y, dx and dB do not change.  It needs a frozen W0 and
+    no dropout, which read x itself.
     """
     if x.shape[-1] != W0.shape[1]:
         raise ShapeError(f"x last dim {x.shape[-1]} != in_features {W0.shape[1]}")
     shp = x.shape
     x2d = x.reshape(-1, shp[-1])
+    if checkpoint is not None and (W0.requires_grad or (training and dropout > 0)):
+        raise ConfigurationError("an activation checkpoint needs a frozen W0 and no dropout")
     if training and dropout > 0:
         # ops.py:96-98: output = w0x + scale * bax * mask / (1 - dropout)
         zero_b = torch.zeros_like(B)
@@ -146,7 +203,7 @@ def lora_forward(x, W0, A, B, alpha: float = 16.0, dropout: float = 0.0,  # noqa
         mask = torch.bernoulli(torch.full_like(bax, 1.0 - dropout))
         out = w0x + scale * bax * mask / (1.0 - dropout)
     else:
-        out = _apply(x2d, W0, A, B, alpha, _compute, _sink)
+        out = _apply(x2d, W0, A, B, alpha, _compute, _sink, checkpoint)
     return out.reshape(*shp[:-1], W0.shape[0])
 
 
@@ -158,13 +215,25 @@ def lora_forward_inference(x, w_merged):
 
 
 def lora_backward(grad_output, x, A, B, alpha: float = 16.0, clip_value: float = 1.0,  # noqa: N803
-                  use_metal: bool = True):
+                  use_metal: bool = True, saved_xa=None):
     """Gradients of A and B (ops.py:117-155), clipped elementwise to
-    +-clip_value after the full reduction, returned in A's/B's dtype."""
+    +-clip_value after the full reduction, returned in A's/B's dtype.
+
+    x may be an 8-bit ``quant.ActivationCheckpoint``: dA is taken from its
+    values, and dB from ``saved_xa``, the (alpha/rank) x.A^T that the forward
+    kept (``kernels.lora_linear_fwd(..., save_xa=True)``), or without it from
+    the checkpoint's values too."""
     g = grad_output.reshape(-1, grad_output.shape[-1])
+    if not torch.is_tensor(x):
+        clip = float(clip_value) if clip_value is not None else 0.0
+        if saved_xa is None:
+            x = x.dequantize().reshape(-1, x.shape[-1])
+        _, da, db = _k.lora_linear_bwd(g, x, None, A, B, alpha, saved_xa, clip, need_dx=False,
+                                       grad_dtype=A.dtype if A.dtype == B.dtype else None)
+        return da.to(A.dtype), db.to(B.dtype)
     xx = x.reshape(-1, x.shape[-1])
     clip = float(clip_value) if clip_value is not None else 0.0
-    _, da, db = _k.lora_linear_bwd(g, xx, None, A, B, alpha, None, clip, need_dx=False)
+    _, da, db = _k.lora_linear_bwd(g, xx, None, A, B, alpha, saved_xa, clip, need_dx=False)
     return da.to(A.dtype), db.to(B.dtype)
 
 

@@ -8,6 +8,19 @@ fp32 absmax ``[N, ceil(K/group)]`` for NF4 (:122, :135), fp16 scale and zero
 ``group = K``).  ``quantize`` runs on the GPU (the reference ships no
 quantiser); ``dequantize`` returns fp32 values bit-identical to the
 reference's ``dequant_nf4``/``dequant_int4``.
+
+Two formats have no reference counterpart.  Both give 32 consecutive features
+of a row one power-of-two factor ``2^E``, kept as the byte ``E + 127``:
+
+* MXFP4 weights (``quantize(w, "mxfp4")``): ``w = e2m1 * 2^E`` with ``E =
+  floor(log2 max|w|) - 2``, codes packed as NF4's, scales uint8
+  ``[N, ceil(K/32)]``.  The forward multiplies them by activations rounded to
+  the same format, on the fp4 tensor cores, with nothing dequantised.
+* MXINT8 activation checkpoints (``checkpoint_activation(x)``): ``x = code / 64
+  * 2^E`` with ``E = floor(log2 max|x|)``.  The LoRA backward takes one in the
+  place of x, at half the bytes of a 16-bit x.
+
+E is at least -127; a block that holds an infinity or a NaN reads back as NaN.
 """
 from __future__ import annotations
 
@@ -16,11 +29,15 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .exceptions import QuantizationError, ShapeError
-from .kernels import _dtype_code, _need_cuda, _ptr, _stream
+from .exceptions import DeviceError, QuantizationError, ShapeError
+from .kernels import _dtype_code, _need_cuda, _need_current, _ptr, _stream
 
-SCHEMES = {"nf4": _lib.QUANT_NF4, "int4": _lib.QUANT_INT4, "int8": _lib.QUANT_INT8}
-DEFAULT_GROUP = {"nf4": 64, "int4": 128, "int8": 128}
+SCHEMES = {"nf4": _lib.QUANT_NF4, "int4": _lib.QUANT_INT4, "int8": _lib.QUANT_INT8,
+           "mxfp4": _lib.QUANT_MXFP4}
+DEFAULT_GROUP = {"nf4": 64, "int4": 128, "int8": 128, "mxfp4": 32}
+_SCALE_DTYPE = {"nf4": torch.float32, "int4": torch.float16, "int8": torch.float16,
+                "mxfp4": torch.uint8}
+_WITH_ZEROS = ("int4", "int8")
 
 
 @dataclass
@@ -52,8 +69,9 @@ class QuantizedWeight:
         return dequantize(self, dtype)
 
     def prepared_scales(self) -> torch.Tensor:
-        """The TMA-ready scale table [groups, rows rounded to 4] the GPU kernels
-        read (built once, on first use, and kept with the weight)."""
+        """The TMA-ready scale table the GPU kernels read: [groups, rows rounded
+        to 4], or for MXFP4 the product's blocks of 128 rows x 128 features
+        (built once, on first use, and kept with the weight)."""
         t = getattr(self, "_prepared", None)
         if t is None or t.device != self.codes.device:
             lib = _lib.load()
@@ -73,30 +91,41 @@ class QuantizedWeight:
         return d
 
 
+def _check_mxfp4(scheme: str, group, lean: bool) -> None:
+    if scheme != "mxfp4":
+        return
+    if group not in (None, 0, 32):
+        raise QuantizationError(f"mxfp4 blocks hold 32 features, got group {group}")
+    if lean:
+        raise QuantizationError("mxfp4 has no lean form: its forward dequantises nothing")
+
+
 def quantize(w: torch.Tensor, scheme: str = "nf4", group: int | None = None,
              lean: bool = False) -> QuantizedWeight:
     """Quantises a 2-D CUDA weight [N, K] (bf16/fp16/fp32).  ``lean`` makes the
     LoRA kernels dequantise inside the GEMM main loop instead of staging a
-    bf16 copy of the weight in their workspace (less memory, slower)."""
+    bf16 copy of the weight in their workspace (less memory, slower); MXFP4,
+    whose forward stages nothing, takes neither it nor another group."""
     if scheme not in SCHEMES:
         raise QuantizationError(f"unknown scheme {scheme!r}; use one of {sorted(SCHEMES)}")
+    _check_mxfp4(scheme, group, lean)
     _need_cuda(w)
     if w.dim() != 2:
         raise ShapeError("quantize takes a 2-D weight [out_features, in_features]")
     group = group or DEFAULT_GROUP[scheme]
     N, K = w.shape
+    if scheme == "mxfp4":
+        _need_current(w)
+        if N == 0 or K == 0:
+            raise ShapeError("quantize takes a weight with at least one row and one column")
     if scheme != "int8" and K % 2:
         raise QuantizationError("4-bit codes pack two per byte: in_features must be even")
     G = -(-K // group)
     w = w.contiguous()
     dev = w.device
     codes = torch.empty((N, K if scheme == "int8" else K // 2), dtype=torch.uint8, device=dev)
-    if scheme == "nf4":
-        scales = torch.empty((N, G), dtype=torch.float32, device=dev)
-        zeros = None
-    else:
-        scales = torch.empty((N, G), dtype=torch.float16, device=dev)
-        zeros = torch.empty((N, G), dtype=torch.float16, device=dev)
+    scales = torch.empty((N, G), dtype=_SCALE_DTYPE[scheme], device=dev)
+    zeros = torch.empty((N, G), dtype=torch.float16, device=dev) if scheme in _WITH_ZEROS else None
     st = _lib.load().mlora_quantize(_ptr(w), _dtype_code(w), N, K, SCHEMES[scheme], group,
                                     _ptr(codes), _ptr(scales), _ptr(zeros), _stream())
     _lib.check(st, "mlora_quantize")
@@ -107,6 +136,8 @@ def dequantize(qw: QuantizedWeight, dtype: torch.dtype = torch.float32) -> torch
     """Dense [N, K] weights: fp32 = the reference's dequantised values (bit
     exact); bf16/fp16 = those values rounded, the operand the GEMMs use."""
     N, K = qw.shape
+    if qw.scheme == "mxfp4":
+        _need_current(qw.codes)
     out = torch.empty((N, K), dtype=dtype, device=qw.device)
     st = _lib.load().mlora_dequantize(qw.code, _ptr(qw.codes), _ptr(qw.scales), _ptr(qw.zeros), N,
                                       K, qw.group, _ptr(out), _dtype_code(out), _stream())
@@ -119,16 +150,109 @@ def from_reference_layout(scheme: str, codes, scales, zeros, shape, group,
     """Wraps tensors already in the reference layout (e.g. loaded from disk)."""
     if scheme not in SCHEMES:
         raise QuantizationError(f"unknown scheme {scheme!r}")
+    _check_mxfp4(scheme, int(group), lean)
+    if scheme == "mxfp4":
+        N, K = int(shape[0]), int(shape[1])
+        for part, t, shp in (("codes", codes, (N, K // 2)), ("scales", scales, (N, -(-K // 32)))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shp:
+                raise QuantizationError(f"mxfp4 {part}: expected {shp} uint8, got "
+                                        f"{tuple(t.shape)} {t.dtype}")
+        if zeros is not None:
+            raise QuantizationError("mxfp4 has no zero points")
     return QuantizedWeight(scheme, codes.contiguous(), scales.contiguous(),
                            None if zeros is None else zeros.contiguous(), int(group),
                            (int(shape[0]), int(shape[1])), lean)
+
+
+# ------------------------------------------------- activation checkpoints --
+
+@dataclass
+class ActivationCheckpoint:
+    """The MXINT8 form of activations x, kept for the backward instead of x.
+
+    ``codes`` int8 [M, K], rows a multiple of 16 bytes apart; ``scales`` uint8
+    [ceil(K/128), M rounded up to 4, 4]: byte (g, m, i) belongs to features
+    ``128 g + 32 i`` .. ``+ 31`` of row m.  ``shape`` is x's; its leading
+    dimensions make up the M rows."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    shape: tuple[int, ...]
+    dtype: torch.dtype
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    @property
+    def rows(self) -> int:
+        n = 1
+        for d in self.shape[:-1]:
+            n *= d
+        return n
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.scales.numel()
+
+    def check(self) -> None:
+        """Raises unless the tensors have the layout the kernels read."""
+        M, K = self.rows, self.shape[-1]
+        if self.codes.dtype != torch.int8 or tuple(self.codes.shape) != (M, K):
+            raise ShapeError(f"checkpoint codes must be int8 {(M, K)}, got "
+                             f"{tuple(self.codes.shape)} {self.codes.dtype}")
+        want = (-(-K // 128), -(-M // 4) * 4, 4)
+        if self.scales.dtype != torch.uint8 or tuple(self.scales.shape) != want or \
+                not self.scales.is_contiguous():
+            raise ShapeError(f"checkpoint scales must be contiguous uint8 {want}, got "
+                             f"{tuple(self.scales.shape)} {self.scales.dtype}")
+        if M and (self.codes.stride(1) != 1 or self.codes.stride(0) < K
+                  or self.codes.stride(0) % 16):
+            raise ShapeError("checkpoint code rows must be contiguous and a multiple of 16 bytes "
+                             f"apart, got strides {tuple(self.codes.stride())}")
+        if self.scales.device != self.codes.device:
+            raise DeviceError("checkpoint codes and scales are on different devices")
+
+    def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
+        """The values, shaped as x, in ``dtype`` (default: x's; exact in bf16)."""
+        self.check()
+        _need_cuda(self.codes)
+        _need_current(self.codes)
+        out = torch.empty(self.shape, dtype=dtype or self.dtype, device=self.device)
+        if out.numel():
+            st = _lib.load().mlora_act_restore(_ptr(self.codes), self.codes.stride(0),
+                                               _ptr(self.scales), self.rows, self.shape[-1],
+                                               _ptr(out), _dtype_code(out), _stream())
+            _lib.check(st, "mlora_act_restore")
+        return out
+
+
+def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
+    """Quantises activations [..., K] (bf16/fp16/fp32) to MXINT8.  Layers that
+    share an input can share one checkpoint: ``c = checkpoint_activation(x)``,
+    then ``q_proj(x, checkpoint=c)``, ``k_proj(x, checkpoint=c)``, ..."""
+    _need_cuda(x)
+    _need_current(x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ShapeError("checkpoint_activation takes activations with at least one feature")
+    code = _dtype_code(x)
+    shape = tuple(x.shape)
+    K = shape[-1]
+    M = x.numel() // K
+    x = x.detach().contiguous()
+    ld = -(-K // 16) * 16
+    codes = torch.empty((M, ld), dtype=torch.int8, device=x.device)[:, :K]
+    scales = torch.empty((-(-K // 128), -(-M // 4) * 4, 4), dtype=torch.uint8, device=x.device)
+    if M:
+        st = _lib.load().mlora_act_checkpoint(_ptr(x), code, M, K, _ptr(codes), ld, _ptr(scales),
+                                              _stream())
+        _lib.check(st, "mlora_act_checkpoint")
+    return ActivationCheckpoint(codes, scales, shape, x.dtype)
 
 
 # ------------------------------------------------------------ pack format --
 # The reference has no on-disk form for a quantised base.  This one keeps the
 # kernels' layout unchanged: one safetensors file holding, per weight,
 # ``{name}.codes`` (uint8), ``{name}.scales`` (fp32 absmax for NF4, fp16 for
-# INT4/INT8) and, for INT4/INT8, ``{name}.zeros`` (fp16); the safetensors
+# INT4/INT8, uint8 for MXFP4) and, for INT4/INT8, ``{name}.zeros`` (fp16); the safetensors
 # header metadata carries ``format`` = PACK_FORMAT and ``weights`` = a JSON map
 # name -> {scheme, group, out_features, in_features}.  Files written here load
 # without any conversion and are validated shape by shape on load.
@@ -140,8 +264,7 @@ def _expected_shapes(scheme: str, N: int, K: int, group: int):
     per_byte = 1 if scheme == "int8" else 2
     groups = -(-K // group)
     codes = (N, -(-K // per_byte))
-    scale_dt = torch.float32 if scheme == "nf4" else torch.float16
-    return codes, (N, groups), scale_dt
+    return codes, (N, groups), _SCALE_DTYPE[scheme]
 
 
 def pack_quantized(weights: dict[str, QuantizedWeight]) -> tuple[dict, dict]:
@@ -175,7 +298,7 @@ def unpack_quantized(tensors: dict, metadata: dict, device=None,
             raise QuantizationError(f"{name}: unknown scheme {scheme!r}")
         codes_shape, scales_shape, scale_dt = _expected_shapes(scheme, N, K, group)
         want = {"codes": (codes_shape, torch.uint8), "scales": (scales_shape, scale_dt)}
-        if scheme != "nf4":
+        if scheme in _WITH_ZEROS:
             want["zeros"] = (scales_shape, torch.float16)
         got = {}
         for part, (shape, dt) in want.items():

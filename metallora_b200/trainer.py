@@ -76,6 +76,9 @@ class TrainingConfig:
 
     output_dir: str = "./lora_output"
 
+    # "mxint8": every LoRALinear keeps its input for the backward in 8 bits
+    activation_checkpoint: str | None = None
+
 
 @dataclass
 class TrainingState:
@@ -285,6 +288,12 @@ class LoRATrainer:
         self.model = model
         for p in model.parameters():
             p.requires_grad_(False)
+        if c.activation_checkpoint is not None:
+            if c.activation_checkpoint != "mxint8":
+                raise ConfigurationError(f"unknown activation checkpoint {c.activation_checkpoint!r}")
+            for m in model.modules():
+                if isinstance(m, LoRALinear):
+                    m.activation_checkpoint = c.activation_checkpoint
         self.params = FlatLoRAParams(model)
         self.optimizer = self._create_optimizer()
         self.state = TrainingState()
