@@ -131,14 +131,27 @@ __device__ __forceinline__ void tmem_cp_scale_atom(uint32_t taddr, uint32_t sadd
                : "memory");
 }
 
-// Untiled bulk copy global -> shared (16-byte aligned addresses and size).
-__device__ __forceinline__ void bulk_load(void* smem_dst, const void* gmem_src, uint32_t bytes,
-                                          uint64_t* bar) {
+// The same over a CTA pair (issued by the even CTA): the M side's scales in each
+// CTA are its own 128 rows', the N side's those of all N columns.
+__device__ __forceinline__ void umma_mxf4_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t sfa_tmem,
+                                               uint32_t sfb_tmem, uint32_t accumulate) {
   asm volatile(
-      "cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-          smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(gmem_src)), "r"(bytes), "r"(smem_u32(bar))
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], "
+      "p;\n\t"
+      "}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa_tmem), "r"(sfb_tmem), "r"(accumulate)
       : "memory");
+}
+
+// Each CTA of the pair copies the atom at this offset of its own shared memory.
+__device__ __forceinline__ void tmem_cp_scale_atom_pair(uint32_t taddr, uint32_t saddr) {
+  const uint64_t desc = make_smem_desc(saddr, 16u, 128u, kLayoutNone);
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
+               : "memory");
 }
 
 }  // namespace mlora

@@ -206,6 +206,262 @@ __global__ void __launch_bounds__(kSkinnyThreads)
   }
 }
 
+// ---------------------------------------------------------------------------
+// More tokens: persistent CTA pairs (cta_group::2), one 256 x 256 tile a pair at
+// a time, as the dense pair GEMM.  Each CTA stages its own 128 rows of x and of
+// W (16 KB each a k-block of 256) and the scale atoms of its x rows and of all
+// 256 W rows.  The fp4 MMA is four times the bf16 rate, so staging is what
+// bounds it: 35 KB a CTA feed about 540 clocks of MMA.
+//
+// The scales need TMEM next to the accumulator, so the accumulator is not
+// double-buffered; eight epilogue warps take it into registers at once and hand
+// it back before they convert and store.
+constexpr int kPairStages = 6;
+constexpr int kHalf = 128;
+constexpr int kPairN = 256;
+constexpr uint32_t kPairOpBytes = kHalf * kRowBytes;  // 16 KB
+constexpr uint32_t kPairStageBytes = 2 * kPairOpBytes + 3 * kSfBytes;
+constexpr int kPairEpiWarps = 8;
+constexpr int kPairThreads = 64 + 32 * kPairEpiWarps;
+constexpr size_t kPairSmem = 1024 + kPairStages * kPairStageBytes + 256;
+constexpr uint32_t kPairTmemCols = 512;  // 256 accumulator, two sets of 8 + 16 scale columns
+
+struct PairParams {
+  int M, N, K;
+  int num_kb_main, num_kb_extra, R;
+  int tiles_m, tiles_n, num_tiles, group_m;
+  int atoms_k;
+  int vec_ok;
+  void* d;
+  long long ldd;
+  uint32_t* status;
+};
+
+// Groups of group_m tile rows, tile rows fastest inside a group (the dense
+// kernel's order: the tiles in flight cover a compact block).
+__device__ __forceinline__ void pair_tile(const PairParams& p, int tile, int& tm, int& tn) {
+  const int per_group = p.group_m * p.tiles_n;
+  const int g = tile / per_group;
+  const int rem = tile - g * per_group;
+  const int rows = min(p.group_m, p.tiles_m - g * p.group_m);
+  tm = g * p.group_m + rem % rows;
+  tn = rem / rows;
+}
+
+template <bool kBF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    mx_pair_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_w,
+                   const __grid_constant__ CUtensorMap tm_xs, const __grid_constant__ CUtensorMap tm_ws,
+                   const __grid_constant__ CUtensorMap tm_x2, const __grid_constant__ CUtensorMap tm_w2,
+                   const PairParams p) {
+  using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
+  constexpr uint32_t kWOff = kPairOpBytes;
+  constexpr uint32_t kXsOff = 2 * kPairOpBytes;
+  constexpr uint32_t kWsOff = kXsOff + kSfBytes;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kPairStages * kPairStageBytes);
+  uint64_t* empty_bar = full_bar + kPairStages;
+  uint64_t* acc_full = empty_bar + kPairStages;
+  uint64_t* acc_empty = acc_full + 1;
+  uint64_t* drain_bar = acc_empty + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+
+  const uint32_t warp = warp_id();
+  const uint32_t lane = lane_id();
+  const uint32_t crank = cluster_ctarank();
+  const bool lead = crank == 0;
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+  const int num_pairs = static_cast<int>(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 2 * kPairEpiWarps);
+    mbar_init(drain_bar, 1);
+    fence_mbarrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+    prefetch_tmap(&tm_xs);
+    prefetch_tmap(&tm_ws);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, kPairTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers initialised and TMEM allocated
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int total_kb = p.num_kb_main + p.num_kb_extra;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      const uint32_t lead_full = mapa_shared(smem_u32(full_bar), 0);
+      uint32_t stage = 0, phase = 0;
+      bool armed[kPairStages];
+      uint32_t armed_parity[kPairStages];
+      for (int s = 0; s < kPairStages; ++s) armed[s] = false, armed_parity[s] = 0;
+      bool ok = true;
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
+        int tm, tn;
+        pair_tile(p, tile, tm, tn);
+        const int m0 = tm * (2 * kHalf) + static_cast<int>(crank) * kHalf;
+        const int n0 = tn * kPairN + static_cast<int>(crank) * kHalf;
+        for (int kb = 0; kb < total_kb; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          uint8_t* st = smem + stage * kPairStageBytes;
+          const bool extra = kb >= p.num_kb_main;
+          if (lead) {
+            mbar_arrive_expect_tx(&full_bar[stage], extra ? 4 * kPairOpBytes : 2 * kPairStageBytes);
+            armed[stage] = true;
+            armed_parity[stage] = phase;
+          }
+          const uint32_t bar = lead_full + stage * 8u;
+          if (extra) {
+            const int k0 = (kb - p.num_kb_main) * kBK16;
+            tma_load_2d_pair(st, &tm_x2, bar, k0, m0);
+            tma_load_2d_pair(st + kWOff, &tm_w2, bar, k0, n0);
+          } else {
+            const int k0 = kb * static_cast<int>(kRowBytes);
+            tma_load_2d_pair(st, &tm_x, bar, k0, m0);
+            tma_load_2d_pair(st + kWOff, &tm_w, bar, k0, n0);
+            // (a row tile past the end lands on rows past the table: zeros)
+            tma_load_2d_pair(st + kXsOff, &tm_xs, bar, 0, (m0 >> 7) * p.atoms_k + 2 * kb);
+            tma_load_2d_pair(st + kWsOff, &tm_ws, bar, 0, 2 * tn * p.atoms_k + 2 * kb);
+            tma_load_2d_pair(st + kWsOff + kSfBytes, &tm_ws, bar, 0,
+                             (2 * tn + 1) * p.atoms_k + 2 * kb);
+          }
+          if (++stage == kPairStages) stage = 0, phase ^= 1u;
+        }
+      }
+      for (int s = 0; s < kPairStages; ++s)
+        if (armed[s]) mbar_wait(&full_bar[s], armed_parity[s], p.status, kDevTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (lead && elect_one()) {
+      constexpr uint32_t idesc16 = make_idesc_f16(2 * kHalf, kPairN, false, false, kBF16);
+      const uint32_t peer_empty = mapa_shared(smem_u32(empty_bar), 1);
+      const uint32_t peer_acc_full = mapa_shared(smem_u32(acc_full), 1);
+      uint32_t stage = 0, phase = 0, acc_phase = 0, set = 0;
+      bool ok = true;
+      for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
+        if (!mbar_wait(acc_empty, acc_phase ^ 1u, p.status, kDevTimeoutAccEmpty)) break;
+        acc_phase ^= 1u;
+        tc_fence_after();
+        for (int kb = 0; kb < total_kb; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sx = smem_u32(smem + stage * kPairStageBytes);
+          const uint32_t sw = sx + kWOff;
+          if (kb >= p.num_kb_main) {
+            const int rem = p.R - (kb - p.num_kb_main) * kBK16;
+            const int nk = rem >= kBK16 ? 4 : rem / 16;
+            for (int k = 0; k < nk; ++k)
+              umma_f16_pair(tmem, desc_kmajor_sw128(sx, k), desc_kmajor_sw128(sw, k), idesc16,
+                            (kb | k) != 0 ? 1u : 0u);
+          } else {
+            const uint32_t sfa = tmem + kPairN + set * 32u;
+            const uint32_t sfb = sfa + 8u;
+            set ^= 1u;
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              tmem_cp_scale_atom_pair(sfa + 4 * a, sx + kXsOff + a * kMxAtomBytes);
+              tmem_cp_scale_atom_pair(sfb + 8 * a, sx + kWsOff + a * kMxAtomBytes);
+              tmem_cp_scale_atom_pair(sfb + 8 * a + 4, sx + kWsOff + kSfBytes + a * kMxAtomBytes);
+            }
+            // as in the kernel above: steps that lie past K entirely are left out
+            const int nk = min(4, (p.K - kb * kBK4 + 63) / 64);
+            for (int k = 0; k < nk; ++k)
+              umma_mxf4_pair(tmem, desc_kmajor_sw128(sx, k), desc_kmajor_sw128(sw, k),
+                             make_idesc_mxf4(2 * kHalf, kPairN, 2u * (k & 1)), sfa + 4 * (k >> 1),
+                             sfb + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
+          }
+          umma_commit_pair(smem_u32(&empty_bar[stage]));
+          umma_commit_pair(peer_empty + stage * 8u);
+          if (++stage == kPairStages) stage = 0, phase ^= 1u;
+        }
+        if (!ok) break;
+        umma_commit_pair(smem_u32(acc_full));
+        umma_commit_pair(peer_acc_full);
+      }
+      umma_commit_pair(smem_u32(drain_bar));
+      mbar_wait(drain_bar, 0, p.status, kDevTimeoutDrain);
+    }
+  } else {
+    const uint32_t quarter = warp & 3u;  // TMEM lanes [32 quarter, 32 quarter + 32)
+    const int col0 = warp >= 6 ? 128 : 0;
+    const uint32_t lead_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
+    uint32_t acc_phase = 0;
+    for (int tile = pair; tile < p.num_tiles; tile += num_pairs) {
+      int tm, tn;
+      pair_tile(p, tile, tm, tn);
+      const int m = tm * (2 * kHalf) + static_cast<int>(crank) * kHalf +
+                    static_cast<int>(quarter * 32 + lane);
+      const int n0 = tn * kPairN + col0;
+      if (!mbar_wait(acc_full, acc_phase, p.status, kDevTimeoutAccFull)) break;
+      acc_phase ^= 1u;
+      __syncwarp();
+      tc_fence_after();
+      uint32_t r[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        tmem_ld_32x32b_x32(tmem + ((quarter * 32u) << 16) + col0 + c * 32, r[c]);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
+      if (m >= p.M) continue;
+      T* out = reinterpret_cast<T*>(p.d) + static_cast<long long>(m) * p.ldd + n0;
+      if (p.vec_ok) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            if (n0 + c * 32 + q * 8 >= p.N) continue;
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              v[i] = pack2<T>(__uint_as_float(r[c][q * 8 + 2 * i]),
+                              __uint_as_float(r[c][q * 8 + 2 * i + 1]));
+            *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (n0 + c * 32 + i < p.N)
+              out[c * 32 + i] = static_cast<T>(__uint_as_float(r[c][i]));
+      }
+    }
+  }
+
+  // After a failure the odd CTA may still have copies in flight that no barrier
+  // of its own tracks: give them time to land before the pair exits.
+  if (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no arrival or copy from the other CTA is still pending
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, kPairTmemCols);
+  }
+}
+
 int cuda_launch_error(cudaError_t e, const char* what) {
   set_error(std::string(what) + ": " + cudaGetErrorString(e));
   return MLORA_ERR_CUDA;
@@ -279,27 +535,76 @@ int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
 }
 
 template <bool kBF16>
+int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
+  CUtensorMap tx, tw, txs, tws, tx2, tw2;
+  if (!map_codes(&tx, a.xq, a.M, a.K, kHalf) || !map_codes(&tw, a.wq, a.N, a.K, kHalf) ||
+      !map_atoms(&txs, a.xs, a.M, a.K) || !map_atoms(&tws, a.ws, a.N, a.K))
+    return MLORA_ERR_INVALID_ARG;
+  if (a.R > 0) {
+    const int64_t r64 = (a.R + 63) / 64 * 64;
+    if (!make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, kHalf) ||
+        !make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, kHalf))
+      return MLORA_ERR_INVALID_ARG;
+  } else {
+    tx2 = tx;
+    tw2 = tw;
+  }
+  PairParams p;
+  p.M = static_cast<int>(a.M);
+  p.N = static_cast<int>(a.N);
+  p.K = static_cast<int>(a.K);
+  p.num_kb_main = static_cast<int>((a.K + kBK4 - 1) / kBK4);
+  p.R = static_cast<int>(a.R);
+  p.num_kb_extra = static_cast<int>((a.R + kBK16 - 1) / kBK16);
+  p.tiles_m = static_cast<int>((a.M + 2 * kHalf - 1) / (2 * kHalf));
+  p.tiles_n = static_cast<int>((a.N + kPairN - 1) / kPairN);
+  p.num_tiles = p.tiles_m * p.tiles_n;
+  p.group_m = p.tiles_m < 8 ? p.tiles_m : 8;
+  p.atoms_k = static_cast<int>((a.K + 127) / 128);
+  p.d = a.d;
+  p.ldd = a.ldd;
+  p.vec_ok = a.N % 8 == 0 && a.ldd % 8 == 0 && (reinterpret_cast<uintptr_t>(a.d) & 15u) == 0;
+  p.status = device_status_ptr();
+  auto kern = mx_pair_kernel<kBF16>;
+  static std::atomic<int> max_pairs[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int pairs = dev < 64 ? max_pairs[dev].load(std::memory_order_acquire) : 0;
+  if (pairs == 0) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(kPairSmem));
+    if (e != cudaSuccess) return cuda_launch_error(e, "cudaFuncSetAttribute(mx pair)");
+    // clusters that can be resident at once (GPCs may leave an SM unpaired)
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / 2 * 2));
+    cfg.blockDim = dim3(kPairThreads);
+    cfg.dynamicSmemBytes = kPairSmem;
+    if (cudaOccupancyMaxActiveClusters(&pairs, kern, &cfg) != cudaSuccess || pairs <= 0) {
+      cudaGetLastError();
+      pairs = num_sms() / 2;
+    }
+    if (dev < 64) max_pairs[dev].store(pairs, std::memory_order_release);
+  }
+  const int grid = 2 * (p.num_tiles < pairs ? p.num_tiles : pairs);
+  LaunchScope scope(kKindGemm, stream);
+  kern<<<grid, kPairThreads, kPairSmem, stream>>>(tx, tw, txs, tws, tx2, tw2, p);
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx pair launch");
+}
+
+template <bool kBF16>
 int dispatch(const MxGemmArgs& a, cudaStream_t s) {
   if (a.M <= 16) return launch_skinny<16, kBF16>(a, s);
   if (a.M <= 32) return launch_skinny<32, kBF16>(a, s);
   if (a.M <= 64) return launch_skinny<64, kBF16>(a, s);
-  return launch_skinny<128, kBF16>(a, s);
+  if (a.M <= 128) return launch_skinny<128, kBF16>(a, s);
+  return launch_pair<kBF16>(a, s);
 }
 
 }  // namespace
 
-int launch_mx_gemm(const MxGemmArgs& args, cudaStream_t s) {
-  for (int64_t m0 = 0; m0 < args.M; m0 += 128) {
-    MxGemmArgs a = args;
-    a.M = args.M - m0 < 128 ? args.M - m0 : 128;
-    a.xq = static_cast<const uint8_t*>(args.xq) + m0 * (args.K / 2);
-    a.xs = static_cast<const uint8_t*>(args.xs) + mx_atoms_bytes(m0, args.K);
-    a.x2 = static_cast<const uint8_t*>(args.x2) + m0 * args.ldx2 * 2;
-    a.d = static_cast<uint8_t*>(args.d) + m0 * args.ldd * 2;
-    const int rc = a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
-    if (rc) return rc;
-  }
-  return MLORA_OK;
+int launch_mx_gemm(const MxGemmArgs& a, cudaStream_t s) {
+  return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
 }
 
 }  // namespace mlora
