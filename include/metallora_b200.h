@@ -303,6 +303,22 @@ MLORA_API int mlora_act_checkpoint(const void* x, int dtype, int64_t M, int64_t 
 MLORA_API int mlora_act_restore(const void* codes, int64_t ld, const void* scales, int64_t M,
                                 int64_t K, void* out, int dtype, void* stream);
 
+/* mlora_lora_forward / mlora_qlora_forward_ex that also write x's checkpoint
+ * (codes and scales 16-byte aligned, ckpt_ld a multiple of 16; BF16 or F16), from
+ * the read of x that makes (alpha/r) x . a^T. */
+MLORA_API int mlora_lora_forward_ckpt(const void* x, const void* w0, const void* a, const void* b,
+                                      void* y, void* saved_xa, void* ckpt_codes, int64_t ckpt_ld,
+                                      void* ckpt_scales, int64_t M, int64_t K, int64_t N,
+                                      int64_t r, float alpha, int dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+MLORA_API int mlora_qlora_forward_ckpt(const void* x, int scheme, const void* codes,
+                                       const void* scales, const void* zeros,
+                                       const void* prepared, int64_t group, const void* a,
+                                       const void* b, void* y, void* saved_xa, void* ckpt_codes,
+                                       int64_t ckpt_ld, void* ckpt_scales, int64_t M, int64_t K,
+                                       int64_t N, int64_t r, float alpha, int dtype,
+                                       void* workspace, size_t workspace_bytes, void* stream);
+
 /* mlora_lora_backward_ex / mlora_qlora_backward_ex with a checkpoint in the
  * place of x: da = s (dy . b)^T . x^ with x^ the checkpoint's values, db from
  * saved_xa (required), BF16 or F16, all of their flags and workspaces. */

@@ -94,6 +94,10 @@ SIGNATURES: dict[str, tuple] = {
     "mlora_act_checkpoint_scales_bytes": (sz, [i64, i64]),
     "mlora_act_checkpoint": (i32, [vp, i32, i64, i64, vp, i64, vp, vp]),
     "mlora_act_restore": (i32, [vp, i64, vp, i64, i64, vp, i32, vp]),
+    "mlora_lora_forward_ckpt": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, vp, i64, i64, i64, i64, f32,
+                                      i32, vp, sz, vp]),
+    "mlora_qlora_forward_ckpt": (i32, [vp, i32, vp, vp, vp, vp, i64, vp, vp, vp, vp, vp, i64, vp,
+                                       i64, i64, i64, i64, f32, i32, vp, sz, vp]),
     "mlora_lora_backward_ckpt": (i32, [vp, vp, i64, vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64,
                                        i64, f32, f32, i32, i32, vp, sz, vp]),
     "mlora_qlora_backward_ckpt": (i32, [vp, vp, i64, vp, i32, vp, vp, vp, vp, i64, vp, vp, vp, vp,

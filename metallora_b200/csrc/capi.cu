@@ -754,6 +754,19 @@ bool make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, cons
   return true;
 }
 
+int set_max_smem(const void* kern, size_t bytes, std::atomic<bool>* done) {
+  const int dev = current_device();
+  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return MLORA_OK;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(bytes));
+  if (e != cudaSuccess) {
+    set_error(std::string("cudaFuncSetAttribute: ") + cudaGetErrorString(e));
+    return MLORA_ERR_CUDA;
+  }
+  if (dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+  return MLORA_OK;
+}
+
 uint32_t* device_status_ptr() { return dev_info().status; }
 int num_sms() {
   const int s = dev_info().sms;
@@ -814,11 +827,13 @@ size_t mlora_lora_forward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64
 namespace {
 // 16-bit LoRA forward (decode kernel for <= 16 tokens without saved_xa, else
 // rank kernel + tcgen05 GEMM) writing y rows with stride ldy.
+// With `ckpt` the kernel that makes s.x.A^T also writes x's MXINT8 checkpoint.
 int lora_forward16(const void* x, const void* w0, const void* a, const void* b, void* y,
                    int64_t ldy, void* saved_xa, int64_t M, int64_t K, int64_t N, int64_t r,
-                   float alpha, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+                   float alpha, int dtype, void* workspace, size_t workspace_bytes, void* stream,
+                   const Ckpt* ckpt = nullptr) {
   int rc;
-  if (saved_xa == nullptr && use_gemv(M, K, dtype))
+  if (saved_xa == nullptr && ckpt == nullptr && use_gemv(M, K, dtype))
     return run_gemv(0, x, w0, nullptr, 64, a, b, y, M, K, N, r, alpha, workspace,
                     workspace_bytes, static_cast<cudaStream_t>(stream), ldy);
   const FwdPlan need = plan_forward(nullptr, M, K, r, saved_xa == nullptr);
@@ -844,7 +859,27 @@ int lora_forward16(const void* x, const void* w0, const void* a, const void* b, 
   ra.ld_t = pad8(M);
   ra.splits = p.splits;
   ra.elt = elt;
-  if ((rc = launch_rank(ra, s))) return rc;
+  if (ckpt != nullptr) {
+    MxPrepArgs pa;
+    pa.x = x;
+    pa.a = a;
+    pa.M = M;
+    pa.K = K;
+    pa.r = r;
+    pa.R = p.R;
+    pa.scale = ra.scale;
+    pa.out_rows = ra.out_rows;
+    pa.ld_rows = ra.ld_rows;
+    pa.out_t = ra.out_t;
+    pa.ld_t = ra.ld_t;
+    pa.q8 = const_cast<void*>(ckpt->codes);
+    pa.ld8 = ckpt->ld;
+    pa.q8_scales = const_cast<void*>(ckpt->scales);
+    pa.elt = elt;
+    if ((rc = launch_mx_prep(pa, s))) return rc;
+  } else if ((rc = launch_rank(ra, s))) {
+    return rc;
+  }
 
   GemmArgs ga;
   ga.x = x;
@@ -870,11 +905,19 @@ int lora_forward16(const void* x, const void* w0, const void* a, const void* b, 
 }
 }  // namespace
 
-int mlora_lora_forward(const void* x, const void* w0, const void* a, const void* b, void* y,
-                       void* saved_xa, int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
-                       int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+namespace {
+// The checkpoint a forward writes.
+int check_ckpt_out(const Ckpt& c, int64_t K, int dtype) {
+  return check_ckpt(c, K, c.codes, dtype);
+}
+
+int lora_forward_any(const void* x, const void* w0, const void* a, const void* b, void* y,
+                     void* saved_xa, const Ckpt* ckpt, int64_t M, int64_t K, int64_t N, int64_t r,
+                     float alpha, int dtype, void* workspace, size_t workspace_bytes,
+                     void* stream) {
   int rc = check_shapes(M, K, N, r, dtype, false);
   if (rc) return rc;
+  if (ckpt != nullptr && (rc = check_ckpt_out(*ckpt, K, dtype))) return rc;
   if (!x || !w0 || !a || !b || !y) return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
   if (!aligned16(x) || !aligned16(w0) || !aligned16(a) || !aligned16(b) || !aligned16(y) ||
       (saved_xa && !aligned16(saved_xa)))
@@ -888,7 +931,24 @@ int mlora_lora_forward(const void* x, const void* w0, const void* a, const void*
                             static_cast<cudaStream_t>(stream));
   }
   return lora_forward16(x, w0, a, b, y, N, saved_xa, M, K, N, r, alpha, dtype, workspace,
-                        workspace_bytes, stream);
+                        workspace_bytes, stream, ckpt);
+}
+}  // namespace
+
+int mlora_lora_forward(const void* x, const void* w0, const void* a, const void* b, void* y,
+                       void* saved_xa, int64_t M, int64_t K, int64_t N, int64_t r, float alpha,
+                       int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return lora_forward_any(x, w0, a, b, y, saved_xa, nullptr, M, K, N, r, alpha, dtype, workspace,
+                          workspace_bytes, stream);
+}
+
+int mlora_lora_forward_ckpt(const void* x, const void* w0, const void* a, const void* b, void* y,
+                            void* saved_xa, void* ckpt_codes, int64_t ckpt_ld, void* ckpt_scales,
+                            int64_t M, int64_t K, int64_t N, int64_t r, float alpha, int dtype,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+  const Ckpt c{ckpt_codes, ckpt_ld, ckpt_scales};
+  return lora_forward_any(x, w0, a, b, y, saved_xa, &c, M, K, N, r, alpha, dtype, workspace,
+                          workspace_bytes, stream);
 }
 
 size_t mlora_lora_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int dtype) {
@@ -1249,7 +1309,7 @@ MxFwdPlan plan_mx_forward(void* ws, int64_t M, int64_t K, int64_t N, int64_t r, 
 int mx_forward(const void* x, const void* codes, const void* scales, const void* prepared,
                const void* a, const void* b, void* y, void* saved_xa, int64_t M, int64_t K,
                int64_t N, int64_t r, float alpha, int dtype, void* workspace,
-               size_t workspace_bytes, cudaStream_t s) {
+               size_t workspace_bytes, cudaStream_t s, const Ckpt* ckpt = nullptr) {
   int rc;
   const MxFwdPlan need = plan_mx_forward(nullptr, M, K, N, r, prepared == nullptr);
   if (workspace == nullptr || workspace_bytes < need.bytes)
@@ -1261,25 +1321,27 @@ int mx_forward(const void* x, const void* codes, const void* scales, const void*
     if ((rc = launch_mx_prepare_scales(scales, N, K, p.atoms, s))) return rc;
     atoms = p.atoms;
   }
-  const MxScales xs{static_cast<uint8_t*>(p.xs), M, (K + 31) / 32, kMxAtoms};
-  if ((rc = launch_mx_quantize(4, x, dtype, M, K, p.xq, K / 2, xs, s))) return rc;
-  RankArgs ra;
-  ra.x = x;
-  ra.l = a;
-  ra.M = M;
-  ra.K = K;
-  ra.r = r;
-  ra.R = p.R;
-  ra.ldx = K;
-  ra.ldl = K;
-  ra.scale = alpha / static_cast<float>(r);
-  ra.out_rows = p.xa_rows;
-  ra.ld_rows = p.R64;
-  ra.out_t = saved_xa;
-  ra.ld_t = pad8(M);
-  ra.splits = rank_splits(M, K);
-  ra.elt = elt;
-  if ((rc = launch_rank(ra, s))) return rc;
+  MxPrepArgs pa;
+  pa.x = x;
+  pa.a = a;
+  pa.M = M;
+  pa.K = K;
+  pa.r = r;
+  pa.R = p.R;
+  pa.scale = alpha / static_cast<float>(r);
+  pa.out_rows = p.xa_rows;
+  pa.ld_rows = p.R64;
+  pa.out_t = saved_xa;
+  pa.ld_t = pad8(M);
+  pa.q4 = p.xq;
+  pa.q4_atoms = p.xs;
+  if (ckpt != nullptr) {
+    pa.q8 = const_cast<void*>(ckpt->codes);
+    pa.ld8 = ckpt->ld;
+    pa.q8_scales = const_cast<void*>(ckpt->scales);
+  }
+  pa.elt = elt;
+  if ((rc = launch_mx_prep(pa, s))) return rc;
   MxGemmArgs g;
   g.xq = p.xq;
   g.xs = p.xs;
@@ -1297,6 +1359,7 @@ int mx_forward(const void* x, const void* codes, const void* scales, const void*
   g.ldw2 = r;
   g.ldd = N;
   g.elt = elt;
+  g.overlap_prev = prepared != nullptr;  // else the table's kernel precedes too
   return launch_mx_gemm(g, s);
 }
 }  // namespace
@@ -1342,13 +1405,15 @@ int mlora_qlora_forward(const void* x, int scheme, const void* codes, const void
                                 M, K, N, r, alpha, dtype, workspace, workspace_bytes, stream);
 }
 
-int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const void* scales,
-                           const void* zeros, const void* prepared, int64_t group, const void* a,
-                           const void* b, void* y, void* saved_xa, int64_t M, int64_t K, int64_t N,
-                           int64_t r, float alpha, int dtype, void* workspace,
-                           size_t workspace_bytes, void* stream) {
+namespace {
+int qlora_forward_any(const void* x, int scheme, const void* codes, const void* scales,
+                      const void* zeros, const void* prepared, int64_t group, const void* a,
+                      const void* b, void* y, void* saved_xa, const Ckpt* ckpt, int64_t M,
+                      int64_t K, int64_t N, int64_t r, float alpha, int dtype, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   int rc = check_qlora(scheme, M, K, N, r, group, dtype);
   if (rc) return rc;
+  if (ckpt != nullptr && (rc = check_ckpt_out(*ckpt, K, dtype))) return rc;
   if (!x || !codes || !scales || !a || !b || !y || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
   if ((rc = check_ptrs16({x, codes, scales, zeros, prepared, a, b, y, saved_xa, workspace})))
@@ -1357,8 +1422,8 @@ int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const v
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (scheme == MLORA_QUANT_MXFP4)
     return mx_forward(x, codes, scales, prepared, a, b, y, saved_xa, M, K, N, r, alpha, dtype,
-                      workspace, workspace_bytes, s);
-  if (saved_xa == nullptr && use_gemv(M, K, dtype)) {
+                      workspace, workspace_bytes, s, ckpt);
+  if (saved_xa == nullptr && ckpt == nullptr && use_gemv(M, K, dtype)) {
     const void* table = prepared;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     size_t ws_bytes = workspace_bytes;
@@ -1379,10 +1444,15 @@ int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const v
     if ((rc = launch_dequantize(scheme, codes, scales, zeros, N, K, group, workspace,
                                 MLORA_DTYPE_BF16, s)))
       return rc;
-    return mlora_lora_forward(x, workspace, a, b, y, saved_xa, M, K, N, r, alpha, dtype,
-                              static_cast<uint8_t*>(workspace) + wbytes, workspace_bytes - wbytes,
-                              stream);
+    return lora_forward_any(x, workspace, a, b, y, saved_xa, ckpt, M, K, N, r, alpha, dtype,
+                            static_cast<uint8_t*>(workspace) + wbytes, workspace_bytes - wbytes,
+                            stream);
   }
+  // the lean path keeps the plain rank kernel: the checkpoint is a pass of its own
+  if (ckpt != nullptr && (rc = mlora_act_checkpoint(x, dtype, M, K, const_cast<void*>(ckpt->codes),
+                                                    ckpt->ld, const_cast<void*>(ckpt->scales),
+                                                    stream)))
+    return rc;
   const size_t sbytes = qscales_bytes(N, K, group);
   const FwdPlan need = plan_forward(nullptr, M, K, r, saved_xa == nullptr);
   if (workspace == nullptr || workspace_bytes < need.bytes + sbytes)
@@ -1434,6 +1504,27 @@ int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const v
   q.up_ld = r;
   q.up_cols = r;
   return launch_qgemm(q, s);
+}
+}  // namespace
+
+int mlora_qlora_forward_ex(const void* x, int scheme, const void* codes, const void* scales,
+                           const void* zeros, const void* prepared, int64_t group, const void* a,
+                           const void* b, void* y, void* saved_xa, int64_t M, int64_t K, int64_t N,
+                           int64_t r, float alpha, int dtype, void* workspace,
+                           size_t workspace_bytes, void* stream) {
+  return qlora_forward_any(x, scheme, codes, scales, zeros, prepared, group, a, b, y, saved_xa,
+                           nullptr, M, K, N, r, alpha, dtype, workspace, workspace_bytes, stream);
+}
+
+int mlora_qlora_forward_ckpt(const void* x, int scheme, const void* codes, const void* scales,
+                             const void* zeros, const void* prepared, int64_t group,
+                             const void* a, const void* b, void* y, void* saved_xa,
+                             void* ckpt_codes, int64_t ckpt_ld, void* ckpt_scales, int64_t M,
+                             int64_t K, int64_t N, int64_t r, float alpha, int dtype,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+  const Ckpt c{ckpt_codes, ckpt_ld, ckpt_scales};
+  return qlora_forward_any(x, scheme, codes, scales, zeros, prepared, group, a, b, y, saved_xa, &c,
+                           M, K, N, r, alpha, dtype, workspace, workspace_bytes, stream);
 }
 
 size_t mlora_qlora_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r,

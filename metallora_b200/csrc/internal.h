@@ -7,6 +7,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 namespace mlora {
@@ -276,6 +277,32 @@ inline int64_t mx_atoms_bytes(int64_t rows, int64_t K) {
   return (rows + 127) / 128 * ((K + 127) / 128) * 512;
 }
 
+// s x A^T (out_rows [M, ld_rows] with columns past R zeroed, out_t [R, ld_t];
+// either may be null) and from the same read of x [M, K] its MXFP4 operand (q4
+// codes [M, K/2] and kMxAtoms scales; K % 32 == 0) and / or its MXINT8
+// checkpoint (q8 codes ld8 bytes apart, 16-byte aligned rows; kMxGroups scales).
+struct MxPrepArgs {
+  const void* x;
+  const void* a;  // [r, K]
+  int64_t M, K, r, R;
+  float scale;
+  void* out_rows = nullptr;
+  int64_t ld_rows = 0;
+  void* out_t = nullptr;
+  int64_t ld_t = 0;
+  void* q4 = nullptr;
+  void* q4_atoms = nullptr;
+  void* q8 = nullptr;
+  int64_t ld8 = 0;
+  void* q8_scales = nullptr;
+  Elt elt;
+};
+int launch_mx_prep(const MxPrepArgs& a, cudaStream_t s);
+
+// Sets a kernel's dynamic shared-memory limit once per device (`done`: one flag
+// per device; a repeated call with the same value is harmless).
+int set_max_smem(const void* kern, size_t bytes, std::atomic<bool>* done);
+
 // Y[M, N] = Q4(x) . W4^T + X2 . W2^T, both fp4 operands as codes [rows, K/2] and
 // scale atoms; x2 [M, R64] and w2 [N, r] 16-bit as in GemmArgs.
 struct MxGemmArgs {
@@ -289,6 +316,9 @@ struct MxGemmArgs {
   int64_t M = 0, N = 0, K = 0, R = 0, w2_rows = 0;
   int64_t ldx2 = 0, ldw2 = 0, ldd = 0;
   Elt elt = Elt::kBF16;  // of x2, w2 and d
+  // programmatic dependent of the kernel that wrote xq, xs and x2 (nothing else
+  // it reads came from that kernel)
+  bool overlap_prev = false;
 };
 int launch_mx_gemm(const MxGemmArgs& a, cudaStream_t s);
 

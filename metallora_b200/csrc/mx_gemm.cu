@@ -110,34 +110,41 @@ __global__ void __launch_bounds__(kSkinnyThreads)
       bool armed[S];
       uint32_t armed_parity[S];
       for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
-      bool prev_done = false;
-      for (int kb = kb_begin; kb < kb_end; ++kb) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
-        uint8_t* st = smem + stage * kStage;
-        uint64_t* bar = &full_bar[stage];
-        const bool extra = kb >= p.num_kb_main;
-        mbar_arrive_expect_tx(bar, extra ? (128 + NT) * kRowBytes : kStage);
-        armed[stage] = true;
-        armed_parity[stage] = phase;
-        // the weight does not come from the kernels before this one; the token
-        // operands do
-        if (extra) {
-          const int k0 = (kb - p.num_kb_main) * kBK16;
-          tma_load_2d(st, &tm_w2, bar, k0, n0);
+      auto load_weight = [&](int kb, uint8_t* st, uint64_t* bar) {
+        if (kb >= p.num_kb_main) {
+          mbar_arrive_expect_tx(bar, (128 + NT) * kRowBytes);
+          tma_load_2d(st, &tm_w2, bar, (kb - p.num_kb_main) * kBK16, n0);
         } else {
+          mbar_arrive_expect_tx(bar, kStage);
           tma_load_2d(st, &tm_w, bar, kb * static_cast<int>(kRowBytes), n0);
           tma_load_2d(st + kWsOff, &tm_ws, bar, 0, static_cast<int>(blockIdx.x) * p.atoms_k + 2 * kb);
         }
-        if (!prev_done) {
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          prev_done = true;
-        }
-        if (extra) {
+      };
+      auto load_tokens = [&](int kb, uint8_t* st, uint64_t* bar) {
+        if (kb >= p.num_kb_main) {
           tma_load_2d(st + kXOff, &tm_x2, bar, (kb - p.num_kb_main) * kBK16, 0);
         } else {
           tma_load_2d(st + kXOff, &tm_x, bar, kb * static_cast<int>(kRowBytes), 0);
           tma_load_2d(st + kXsOff, &tm_xs, bar, 0, 2 * kb);
         }
+      };
+      // the weight does not come from the kernel before this one, the token
+      // operands do: a ring of weight blocks is on its way before the wait
+      const int ahead = min(S, kb_end - kb_begin);
+      for (int i = 0; i < ahead; ++i) {
+        load_weight(kb_begin + i, smem + i * kStage, &full_bar[i]);
+        armed[i] = true;
+      }
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < ahead; ++i) load_tokens(kb_begin + i, smem + i * kStage, &full_bar[i]);
+      if (ahead == S) phase = 1;
+      stage = ahead == S ? 0u : static_cast<uint32_t>(ahead);
+      for (int kb = kb_begin + ahead; kb < kb_end; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
+        armed[stage] = true;
+        armed_parity[stage] = phase;
+        load_weight(kb, smem + stage * kStage, &full_bar[stage]);
+        load_tokens(kb, smem + stage * kStage, &full_bar[stage]);
         if (++stage == S) stage = 0, phase ^= 1u;
       }
       for (int s = 0; s < S; ++s)
@@ -513,23 +520,25 @@ int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
     splits *= 2;
   p.splits = splits;
   auto kern = mx_skinny_kernel<NT, kBF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(skinny_smem(NT)));
-  if (e != cudaSuccess) return cuda_launch_error(e, "cudaFuncSetAttribute(mx skinny)");
+  static std::atomic<bool> attr_set[64];
+  if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), skinny_smem(NT), attr_set))
+    return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits));
   cfg.blockDim = dim3(kSkinnyThreads);
   cfg.dynamicSmemBytes = skinny_smem(NT);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = static_cast<unsigned>(splits);
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.overlap_prev ? 2 : 1;
   LaunchScope scope(kKindGemm, stream);
-  e = cudaLaunchKernelEx(&cfg, kern, tw, tx, tws, txs, tw2, tx2, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, tws, txs, tw2, tx2, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx skinny launch");
 }
@@ -586,9 +595,19 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
     if (dev < 64) max_pairs[dev].store(pairs, std::memory_order_release);
   }
   const int grid = 2 * (p.num_tiles < pairs ? p.num_tiles : pairs);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.overlap_prev ? 1 : 0;
   LaunchScope scope(kKindGemm, stream);
-  kern<<<grid, kPairThreads, kPairSmem, stream>>>(tx, tw, txs, tws, tx2, tw2, p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, txs, tws, tx2, tw2, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx pair launch");
 }
 

@@ -1,0 +1,394 @@
+// One pass over the activations of a LoRA linear: the rank projection
+//
+//     s x A^T        (rows [M, R64] for the GEMM, transposed [R, M] for the backward)
+//
+// on the tensor cores, and from the same shared-memory tiles x's MXFP4 operand
+// of the fp4 product and / or its MXINT8 checkpoint (mx.cuh).  HBM-bound: x is
+// read once, where separate kernels read it once each.
+//
+// CTA = 128 tokens x one range of features; the ranges of a token tile are one
+// cluster (cluster_reduce).  Warp 0 copies [128 x 64] tiles of x and [R x 64]
+// tiles of A (TMA ring), warp 1 issues the UMMAs, warps 2-9 quantise: a thread
+// owns one block of 32 features, so the block maximum needs no exchange.  A
+// stage is free when the UMMAs and all eight warps are done with it.
+#include <atomic>
+#include <string>
+#include <type_traits>
+
+#include "cluster_reduce.cuh"
+#include "internal.h"
+#include "mx.cuh"
+#include "quant.cuh"
+#include "../../include/metallora_b200.h"
+
+namespace mlora {
+namespace {
+
+constexpr int kQuantWarps = 8;
+constexpr int kThreads = 64 + 32 * kQuantWarps;
+constexpr int kBK = 64;
+constexpr uint32_t kXBytes = 128 * kBK * 2;
+constexpr int kMaxSplits = 8;
+
+__host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
+__host__ __device__ constexpr uint32_t stage_bytes(int R) { return kXBytes + R * 128u; }
+__host__ __device__ constexpr int num_stages(int R) {
+  const int n = static_cast<int>((ctas_per_sm(R) == 2 ? 108u : 200u) * 1024u / stage_bytes(R));
+  return n > 8 ? 8 : n;
+}
+constexpr size_t smem_bytes(int R) { return 1024 + num_stages(R) * stage_bytes(R) + 256; }
+__host__ __device__ constexpr uint32_t tmem_cols(int R) {
+  return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
+}
+
+struct PrepParams {
+  long long M, K;
+  int num_kb, splits;
+  float scale;
+  void* out_rows;
+  long long ld_rows;
+  void* out_t;
+  long long ld_t;
+  uint8_t* q4;       // codes [M, K/2], or nullptr
+  uint8_t* q4_atoms;
+  long long atoms_k;
+  uint8_t* q8;       // codes [M, ld8], or nullptr
+  long long ld8;
+  uint8_t* q8_scales;  // words [ceil(K/128), rows8]
+  long long rows8;
+  uint32_t* status;
+};
+
+// The bits of max|x| (as fp32) of the 32 16-bit values in w.
+template <typename T>
+__device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[16]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+  m = max(m & 0xFFFFu, m >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return m << 16;
+  else
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+}
+
+// The two values of a word as packed fp32.
+template <typename T>
+__device__ __forceinline__ uint64_t widen2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return (static_cast<uint64_t>(w & 0xFFFF0000u) << 32) | (w << 16);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return f2_pack(f.x, f.y);
+  }
+}
+
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// 32 e2m1 codes; inv = 1 / X.
+template <typename T>
+__device__ __forceinline__ uint4 block_fp4(const uint32_t (&w)[16], float inv) {
+  const uint64_t ii = f2_pack(inv, inv);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const uint64_t p = f2_mul(widen2<T>(w[4 * i + h]), ii);
+      v[2 * h] = f2_lo(p);
+      v[2 * h + 1] = f2_hi(p);
+    }
+    o[i] = mx_pack_e2m1(v);
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// 32 int8 codes; inv64 = 64 / X.  The product is exact, so the fused add of
+// 1.5 * 2^23 is the one rounding; its low 16 bits are the code, clamped there.
+template <typename T>
+__device__ __forceinline__ void block_int8(const uint32_t (&w)[16], float inv64, uint4& lo, uint4& hi) {
+  const uint64_t ii = f2_pack(inv64, inv64);
+  const uint64_t mm = f2_pack(12582912.f, 12582912.f);
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t h[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t p = f2_fma(widen2<T>(w[2 * i + j]), ii, mm);
+      const uint32_t s = __byte_perm(static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32), 0x5410u);
+      h[j] = __vmaxs2(__vmins2(s, 0x007F007Fu), 0xFF81FF81u);
+    }
+    o[i] = __byte_perm(h[0], h[1], 0x6420u);
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// Grid (token tiles, splits), cluster (1, splits, 1).
+template <int R, bool kBF16>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
+    mx_prep_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_a,
+                   const PrepParams p) {
+  using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
+  constexpr int S = num_stages(R);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R));
+  uint64_t* empty_bar = full_bar + S;
+  uint64_t* done_bar = empty_bar + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+
+  const uint32_t warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1 + kQuantWarps);
+    mbar_init(done_bar, 1);
+    fence_mbarrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, tmem_cols(R));
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // the product may start its set-up and stream its weight
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int tile = static_cast<int>(blockIdx.x);
+  const uint32_t crank = cluster_ctarank();
+  const int per = (p.num_kb + p.splits - 1) / p.splits;
+  const int kb_begin = static_cast<int>(crank) * per;
+  const int kb_end = min(p.num_kb, kb_begin + per);
+  const bool has_work = kb_begin < kb_end;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      bool armed[S];
+      uint32_t armed_parity[S];
+      for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
+        uint8_t* st = smem + stage * stage_bytes(R);
+        mbar_arrive_expect_tx(&full_bar[stage], stage_bytes(R));
+        armed[stage] = true;
+        armed_parity[stage] = phase;
+        tma_load_2d(st, &tm_x, &full_bar[stage], kb * kBK, tile * 128);
+        tma_load_2d(st + kXBytes, &tm_a, &full_bar[stage], kb * kBK, 0);
+        if (++stage == S) stage = 0, phase ^= 1u;
+      }
+      for (int s = 0; s < S; ++s)
+        if (armed[s]) mbar_wait(&full_bar[s], armed_parity[s], p.status, kDevTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (has_work && elect_one()) {
+      constexpr uint32_t idesc = make_idesc_f16(128, R, false, false, kBF16);
+      uint32_t stage = 0, phase = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) break;
+        tc_fence_after();
+        const uint32_t sx = smem_u32(smem + stage * stage_bytes(R));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f16(tmem, desc_kmajor_sw128(sx, k), desc_kmajor_sw128(sx + kXBytes, k), idesc,
+                   (kb != kb_begin || k != 0) ? 1u : 0u);
+        umma_commit(&empty_bar[stage]);
+        if (++stage == S) stage = 0, phase ^= 1u;
+      }
+      umma_commit(done_bar);
+    }
+  } else if (has_work) {
+    // lanes 2i, 2i+1: the two blocks of one row's 64 features
+    const int ct = static_cast<int>(threadIdx.x) - 64;
+    const int r = ct >> 1, b = ct & 1;
+    const long long row = static_cast<long long>(tile) * 128 + r;
+    const bool live = row < p.M;
+    uint32_t stage = 0, phase = 0;
+    for (int kb = kb_begin; kb < kb_end; ++kb) {
+      if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) break;
+      uint32_t w[16];
+      const uint8_t* src = smem + stage * stage_bytes(R) + r * 128;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 q = *reinterpret_cast<const uint4*>(src + (((4 * b + i) ^ (r & 7)) << 4));
+        w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+      }
+      __syncwarp();
+      if (lane_id() == 0) mbar_arrive(&empty_bar[stage]);
+      if (++stage == S) stage = 0, phase ^= 1u;
+
+      const uint32_t amax = block_amax<T>(w);
+      const long long k = static_cast<long long>(kb) * kBK + 32 * b;
+      const bool in = live && k < p.K;
+      if (p.q4 != nullptr) {
+        const uint32_t byte = mx_scale_byte_fp4(amax);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, byte, 1);
+        if (live && b == 0)
+          *reinterpret_cast<uint16_t*>(p.q4_atoms +
+                                       ((row >> 7) * p.atoms_k + (kb >> 1)) * kMxAtomBytes +
+                                       (r & 31) * 16 + (r >> 5) * 4 + (kb & 1) * 2) =
+              static_cast<uint16_t>(byte | (other << 8));
+        uint4 c = block_fp4<T>(w, mx_inv_scale(byte));
+        if (byte == 255u) c = make_uint4(0, 0, 0, 0);
+        if (in) *reinterpret_cast<uint4*>(p.q4 + row * (p.K >> 1) + (k >> 1)) = c;
+      }
+      if (p.q8 != nullptr) {
+        const uint32_t byte = mx_scale_byte_int8(amax);
+        const uint32_t other = __shfl_xor_sync(0xffffffffu, byte, 1);
+        if (live && b == 0) {
+          uint16_t* dst = reinterpret_cast<uint16_t*>(p.q8_scales + ((kb >> 1) * p.rows8 + row) * 4) +
+                          (kb & 1);
+          *dst = static_cast<uint16_t>(byte | (other << 8));
+          if (kb + 1 == p.num_kb && (kb & 1) == 0) dst[1] = 0;  // the word's blocks past K
+        }
+        uint4 lo, hi;
+        if (byte >= 6u) {
+          block_int8<T>(w, byte == 255u ? 0.f : mx_inv_scale(byte) * 64.f, lo, hi);
+        } else {
+          // 64 / X is past fp32's range: X = 2^(byte - 127) moved up by 2^8 together
+          // with the values (exact: they are below 2^-120)
+          uint32_t u[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t v = f2_mul(widen2<T>(w[i]), f2_pack(256.f, 256.f));
+            u[i] = pack2<__nv_bfloat16>(f2_lo(v), f2_hi(v));
+          }
+          block_int8<__nv_bfloat16>(u, mx_inv_scale(byte + 8u) * 64.f, lo, hi);
+        }
+        if (byte == 255u) lo = hi = make_uint4(0, 0, 0, 0);
+        if (in) {
+          uint8_t* dst = p.q8 + row * p.ld8 + k;
+          if (k + 32 <= p.K) {
+            *reinterpret_cast<uint4*>(dst) = lo;
+            *reinterpret_cast<uint4*>(dst + 16) = hi;
+          } else {  // K is a multiple of 8: the row ends between two 8-byte groups
+            const uint32_t o[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (k + 8 * i < p.K)
+                *reinterpret_cast<uint2*>(dst + 8 * i) = make_uint2(o[2 * i], o[2 * i + 1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+  const bool epi = warp >= 2 && warp < 6;
+  const int row_local = static_cast<int>((warp & 3u) * 32 + lane_id());
+  const long long row = static_cast<long long>(tile) * 128 + row_local;
+  bool have = false;
+  if (warp >= 2 && has_work) {
+    have = mbar_wait(done_bar, 0, p.status, kDevTimeoutAccFull);
+    tc_fence_after();
+  }
+  const bool live = epi && row < p.M;
+  auto emit = [&](int j, float v0, float v1) {
+    if (!live) return;
+    v0 *= p.scale;
+    v1 *= p.scale;
+    if (p.out_rows != nullptr)
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j) =
+          pack2<T>(v0, v1);
+    if (p.out_t != nullptr) {
+      T* dst = reinterpret_cast<T*>(p.out_t) + row;
+      dst[static_cast<long long>(j) * p.ld_t] = static_cast<T>(v0);
+      dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(v1);
+    }
+  };
+  cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
+                    reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+  if (live && crank == 0 && p.out_rows != nullptr) {  // zero columns past R
+    T* dst = reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows;
+    for (long long j = R; j < p.ld_rows; j += 8)
+      *reinterpret_cast<uint4*>(dst + j) = make_uint4(0, 0, 0, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols(R));
+  }
+}
+
+int cuda_launch_error(cudaError_t e, const char* what) {
+  set_error(std::string(what) + ": " + cudaGetErrorString(e));
+  return MLORA_ERR_CUDA;
+}
+
+template <int R, bool kBF16>
+int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
+  CUtensorMap tx, ta;
+  if (!make_tmap_2d_16b(&tx, a.x, a.K, a.M, a.K, kBK, 128) ||
+      !make_tmap_2d_16b(&ta, a.a, a.K, a.r, a.K, kBK, R))
+    return MLORA_ERR_INVALID_ARG;
+  PrepParams p;
+  p.M = a.M;
+  p.K = a.K;
+  p.num_kb = static_cast<int>((a.K + kBK - 1) / kBK);
+  p.scale = a.scale;
+  p.out_rows = a.out_rows;
+  p.ld_rows = a.ld_rows;
+  p.out_t = a.out_t;
+  p.ld_t = a.ld_t;
+  p.q4 = static_cast<uint8_t*>(a.q4);
+  p.q4_atoms = static_cast<uint8_t*>(a.q4_atoms);
+  p.atoms_k = (a.K + 127) / 128;
+  p.q8 = static_cast<uint8_t*>(a.q8);
+  p.ld8 = a.ld8;
+  p.q8_scales = static_cast<uint8_t*>(a.q8_scales);
+  p.rows8 = (a.M + 3) / 4 * 4;
+  p.status = device_status_ptr();
+  const int64_t tiles = (a.M + 127) / 128;
+  // one wave of resident CTAs, at least four k-blocks a split
+  const int64_t slots = static_cast<int64_t>(ctas_per_sm(R)) * num_sms();
+  int splits = 1;
+  while (splits * 2 <= kMaxSplits && splits * 2 * tiles <= slots && splits * 8 <= p.num_kb)
+    splits *= 2;
+  p.splits = splits;
+  auto kern = mx_prep_kernel<R, kBF16>;
+  static std::atomic<bool> attr_set[64];
+  if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes(R);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = static_cast<unsigned>(splits);
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LaunchScope scope(kKindRank, stream);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, ta, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx prep launch");
+}
+
+template <bool kB>
+int dispatch(const MxPrepArgs& a, cudaStream_t s) {
+  switch (a.R) {
+    case 16: return launch_typed<16, kB>(a, s);
+    case 32: return launch_typed<32, kB>(a, s);
+    case 64: return launch_typed<64, kB>(a, s);
+    case 128: return launch_typed<128, kB>(a, s);
+    case 256: return launch_typed<256, kB>(a, s);
+    default: set_error("unsupported padded rank"); return MLORA_ERR_UNSUPPORTED;
+  }
+}
+
+}  // namespace
+
+int launch_mx_prep(const MxPrepArgs& a, cudaStream_t s) {
+  return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
+}
+
+}  // namespace mlora

@@ -271,7 +271,8 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   const int64_t m4 = (a.M + 3) / 4 * 4, groups = (a.K + 127) / 128;
   if (!make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, static_cast<uint64_t>(a.K),
                     static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.ld), 128, kBM, false) ||
-      !make_tmap_2d(&ts, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.scales, static_cast<uint64_t>(m4),
+      // (rows past M, which pad the words, are not read: their bytes are not set)
+      !make_tmap_2d(&ts, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.scales, static_cast<uint64_t>(a.M),
                     static_cast<uint64_t>(groups), static_cast<uint64_t>(m4) * 4, kBM, 1, false) ||
       !make_tmap_2d_16b(&tu, a.st, a.M, a.R, a.ld_st, kBM, R))
     return MLORA_ERR_INVALID_ARG;
@@ -292,9 +293,8 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
     splits *= 2;
   p.splits = splits;
   auto kern = mx_wgrad_kernel<R, kBF16>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem_bytes(R)));
-  if (e != cudaSuccess) return cuda_launch_error(e, "cudaFuncSetAttribute(mx wgrad)");
+  static std::atomic<bool> attr_set[64];
+  if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(groups * splits));
   cfg.blockDim = dim3(kThreads);
@@ -308,7 +308,7 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   LaunchScope scope(kKindWgrad, stream);
-  e = cudaLaunchKernelEx(&cfg, kern, tc, ts, tu, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tc, ts, tu, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx wgrad launch");
 }

@@ -21,7 +21,13 @@ from .exceptions import DeviceError, ShapeError
 _DT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 
 
+# the current stream's handle without building a Stream object (~3 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream() -> int:
+    if _raw_stream is not None:
+        return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -98,11 +104,12 @@ def _check_2d(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype) -> N
 
 
 def lora_linear_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
-                    alpha: float, save_xa: bool = False):
+                    alpha: float, save_xa: bool = False, ckpt_out=None):
     """y = x.W0^T + (alpha/r).(x.A^T).B^T for 2-D x [M, K].
 
     Returns (y, saved_xa); saved_xa is the [R, ceil8(M)] rank intermediate the
-    backward can reuse (bf16/fp16 only), else None."""
+    backward can reuse (bf16/fp16 only), else None.  ``ckpt_out`` (a
+    ``quant.empty_checkpoint`` of x) receives x's MXINT8 checkpoint."""
     _need_cuda(x2d, w0, a, b)
     dt = x2d.dtype
     code = _dtype_code(x2d)
@@ -121,8 +128,13 @@ def lora_linear_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor, b: tor
         return y, saved
     lib = _lib.load()
     ws = _workspace(lib.mlora_lora_forward_workspace_bytes(M, K, N, r, code), x2d.device)
-    st = lib.mlora_lora_forward(_ptr(x2d), _ptr(w0), _ptr(a), _ptr(b), _ptr(y), _ptr(saved), M, K,
-                                N, r, float(alpha), code, _ptr(ws), ws.numel(), _stream())
+    head = (_ptr(x2d), _ptr(w0), _ptr(a), _ptr(b), _ptr(y), _ptr(saved))
+    tail = (M, K, N, r, float(alpha), code, _ptr(ws), ws.numel(), _stream())
+    if ckpt_out is not None:
+        _check_ckpt_out(ckpt_out, x2d)
+        st = lib.mlora_lora_forward_ckpt(*head, *_ckpt_args(ckpt_out), *tail)
+    else:
+        st = lib.mlora_lora_forward(*head, *tail)
     _lib.check(st, "mlora_lora_forward")
     return y, saved
 
@@ -143,6 +155,13 @@ def _as_ckpt(x, saved_xa, dy2d):
 
 def _ckpt_args(ckpt):
     return _ptr(ckpt.codes), ckpt.codes.stride(0), _ptr(ckpt.scales)
+
+
+def _check_ckpt_out(ckpt, x2d) -> None:
+    ckpt.check()
+    if (ckpt.rows, ckpt.shape[-1], ckpt.dtype, ckpt.device) != (*x2d.shape, x2d.dtype, x2d.device):
+        raise ShapeError("the checkpoint to fill does not match x")
+    _need_current(x2d)
 
 
 def _check_saved(saved_xa, r: int, M: int, dtype: torch.dtype) -> None:
@@ -434,11 +453,12 @@ def _qlora_dtype(x2d, qw) -> torch.dtype:
 
 
 def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, alpha: float,
-                     save_xa: bool = False):
+                     save_xa: bool = False, ckpt_out=None):
     """y = x.deq(W)^T + (alpha/r).(x.A^T).B^T for a quantised base ``qw``
     (metallora_b200.quant.QuantizedWeight); x, A, B bf16.  ``qw.lean`` selects
     the fused kernel that dequantises in its main loop (no dense copy of W).
-    An MXFP4 base takes bf16 or fp16 and multiplies x rounded to MXFP4."""
+    An MXFP4 base takes bf16 or fp16 and multiplies x rounded to MXFP4.
+    ``ckpt_out`` as for ``lora_linear_fwd``."""
     _need_cuda(x2d, a, b)
     dt = _qlora_dtype(x2d, qw)
     M, K = x2d.shape
@@ -456,10 +476,14 @@ def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, al
         return y, saved
     lib = _lib.load()
     ws = _workspace(_qlora_ws_bytes(lib, qw, M, K, N, r, backward=False), x2d.device)
-    st = lib.mlora_qlora_forward_ex(_ptr(x2d), qw.code, _ptr(qw.codes), _ptr(qw.scales),
-                                    _ptr(qw.zeros), _ptr(qw.prepared_scales()), qw.group, _ptr(a),
-                                    _ptr(b), _ptr(y), _ptr(saved), M, K, N, r, float(alpha),
-                                    _dtype_code(x2d), _ptr(ws), ws.numel(), _stream())
+    head = (_ptr(x2d), qw.code, _ptr(qw.codes), _ptr(qw.scales), _ptr(qw.zeros),
+            _ptr(qw.prepared_scales()), qw.group, _ptr(a), _ptr(b), _ptr(y), _ptr(saved))
+    tail = (M, K, N, r, float(alpha), _dtype_code(x2d), _ptr(ws), ws.numel(), _stream())
+    if ckpt_out is not None:
+        _check_ckpt_out(ckpt_out, x2d)
+        st = lib.mlora_qlora_forward_ckpt(*head, *_ckpt_args(ckpt_out), *tail)
+    else:
+        st = lib.mlora_qlora_forward_ex(*head, *tail)
     _lib.check(st, "mlora_qlora_forward_ex")
     return y, saved
 

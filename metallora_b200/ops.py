@@ -15,11 +15,11 @@ from .exceptions import ConfigurationError, ShapeError
 
 
 def _checkpoint(x2d, checkpoint):
-    """The activation checkpoint of ``x2d`` that ``checkpoint`` asks for: None,
-    "mxint8" (made here), or one the caller made of the same x."""
-    from .quant import ActivationCheckpoint, checkpoint_activation
+    """(checkpoint of ``x2d`` or None, whether the forward has to fill it):
+    ``checkpoint`` is None, "mxint8", or one the caller made of the same x."""
+    from .quant import ActivationCheckpoint, empty_checkpoint
     if checkpoint is None:
-        return None
+        return None, False
     if x2d.dtype not in (torch.bfloat16, torch.float16):
         raise ConfigurationError("activation checkpoints take bf16 or fp16 activations")
     if isinstance(checkpoint, ActivationCheckpoint):
@@ -29,11 +29,12 @@ def _checkpoint(x2d, checkpoint):
             raise ShapeError(f"the checkpoint is of {tuple(checkpoint.shape)} {checkpoint.dtype} on "
                              f"{checkpoint.device}, x is {tuple(x2d.shape)} {x2d.dtype} on "
                              f"{x2d.device}")
-        return checkpoint
+        return checkpoint, False
     if checkpoint != "mxint8":
         raise ConfigurationError(f"unknown activation checkpoint {checkpoint!r}; use 'mxint8' or "
                                  "an ActivationCheckpoint")
-    return checkpoint_activation(x2d)
+    _k._need_cuda(x2d)
+    return empty_checkpoint(x2d.shape, x2d.dtype, x2d.device), True
 
 
 def _keep_x(ctx, x2d, ckpt) -> tuple:
@@ -72,8 +73,10 @@ class _LoRALinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2d, w0, a, b, alpha, compute, sink, checkpoint=None):
         a_c, b_c = compute if compute is not None else (a.to(x2d.dtype), b.to(x2d.dtype))
-        y, saved = _k.lora_linear_fwd(x2d, w0, a_c, b_c, alpha, save_xa=True)
-        ctx.save_for_backward(*_keep_x(ctx, x2d, _checkpoint(x2d, checkpoint)), w0, a_c, b_c, saved)
+        ckpt, fill = _checkpoint(x2d, checkpoint)
+        y, saved = _k.lora_linear_fwd(x2d, w0, a_c, b_c, alpha, save_xa=True,
+                                      ckpt_out=ckpt if fill else None)
+        ctx.save_for_backward(*_keep_x(ctx, x2d, ckpt), w0, a_c, b_c, saved)
         ctx.alpha = alpha
         ctx.sink = sink
         ctx.ab_dtypes = (a.dtype, b.dtype)
@@ -122,8 +125,10 @@ class _QLoRALinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x2d, a, b, qw, alpha, compute, sink, checkpoint=None):
         a_c, b_c = compute if compute is not None else (a.to(x2d.dtype), b.to(x2d.dtype))
-        y, saved = _k.qlora_linear_fwd(x2d, qw, a_c, b_c, alpha, save_xa=True)
-        ctx.save_for_backward(*_keep_x(ctx, x2d, _checkpoint(x2d, checkpoint)), a_c, b_c, saved)
+        ckpt, fill = _checkpoint(x2d, checkpoint)
+        y, saved = _k.qlora_linear_fwd(x2d, qw, a_c, b_c, alpha, save_xa=True,
+                                       ckpt_out=ckpt if fill else None)
+        ctx.save_for_backward(*_keep_x(ctx, x2d, ckpt), a_c, b_c, saved)
         ctx.qw, ctx.alpha, ctx.sink = qw, alpha, sink
         ctx.ab_dtypes = (a.dtype, b.dtype)
         return y
@@ -159,14 +164,14 @@ def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=No
     An MXFP4 base multiplies x rounded to MXFP4 (the gradient passes straight
     through that rounding).  ``checkpoint`` as for ``lora_forward``."""
     shp = x.shape
-    x2d = x.reshape(-1, shp[-1])
+    x2d = x if len(shp) == 2 else x.reshape(-1, shp[-1])
     if qweight.scheme == "mxfp4" and not (torch.is_grad_enabled() and
                                           (x.requires_grad or A.requires_grad or B.requires_grad)):
         a, b = _compute if _compute is not None else (A.to(x.dtype), B.to(x.dtype))
         out = _k.qlora_linear_fwd(x2d, qweight, a, b, float(alpha))[0]
     else:
         out = _QLoRALinearFn.apply(x2d, A, B, qweight, float(alpha), _compute, _sink, checkpoint)
-    return out.reshape(*shp[:-1], qweight.shape[0])
+    return out if len(shp) == 2 else out.reshape(*shp[:-1], qweight.shape[0])
 
 
 def _apply(x2d, W0, A, B, alpha, compute=None, sink=None, checkpoint=None):

@@ -225,27 +225,36 @@ class ActivationCheckpoint:
         return out
 
 
+def empty_checkpoint(shape, dtype: torch.dtype, device) -> ActivationCheckpoint:
+    """An uninitialised checkpoint of activations of this shape: the buffers a
+    forward fills (``kernels.lora_linear_fwd(..., ckpt_out=)``)."""
+    shape = tuple(shape)
+    if not shape or shape[-1] == 0:
+        raise ShapeError("a checkpoint is of activations with at least one feature")
+    K, M = shape[-1], 1
+    for d in shape[:-1]:
+        M *= d
+    ld = -(-K // 16) * 16
+    codes = torch.empty((M, ld), dtype=torch.int8, device=device)
+    scales = torch.empty((-(-K // 128), -(-M // 4) * 4, 4), dtype=torch.uint8, device=device)
+    return ActivationCheckpoint(codes if ld == K else codes[:, :K], scales, shape, dtype)
+
+
 def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
     """Quantises activations [..., K] (bf16/fp16/fp32) to MXINT8.  Layers that
     share an input can share one checkpoint: ``c = checkpoint_activation(x)``,
     then ``q_proj(x, checkpoint=c)``, ``k_proj(x, checkpoint=c)``, ..."""
     _need_cuda(x)
     _need_current(x)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ShapeError("checkpoint_activation takes activations with at least one feature")
     code = _dtype_code(x)
-    shape = tuple(x.shape)
-    K = shape[-1]
-    M = x.numel() // K
-    x = x.detach().contiguous()
-    ld = -(-K // 16) * 16
-    codes = torch.empty((M, ld), dtype=torch.int8, device=x.device)[:, :K]
-    scales = torch.empty((-(-K // 128), -(-M // 4) * 4, 4), dtype=torch.uint8, device=x.device)
-    if M:
-        st = _lib.load().mlora_act_checkpoint(_ptr(x), code, M, K, _ptr(codes), ld, _ptr(scales),
-                                              _stream())
+    c = empty_checkpoint(x.shape, x.dtype, x.device)
+    if x.numel():
+        x = x.detach().contiguous()
+        st = _lib.load().mlora_act_checkpoint(x.data_ptr(), code, c.codes.shape[0], x.shape[-1],
+                                              c.codes.data_ptr(), c.codes.stride(0),
+                                              c.scales.data_ptr(), _stream())
         _lib.check(st, "mlora_act_checkpoint")
-    return ActivationCheckpoint(codes, scales, shape, x.dtype)
+    return c
 
 
 # ------------------------------------------------------------ pack format --
