@@ -238,7 +238,7 @@ struct PairParams {
   int num_kb_main, num_kb_extra, R;
   int tiles_m, tiles_n, num_tiles, group_m;
   int atoms_k;
-  int vec_ok;
+  int vec_ok;  // rows of d allow 32-byte (2), 16-byte (1) or single (0) stores
   void* d;
   long long ldd;
   uint32_t* status;
@@ -433,14 +433,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            if (n0 + c * 32 + q * 8 >= p.N) continue;
-            uint32_t v[4];
+          for (int q = 0; q < 2; ++q) {
+            const int n = c * 32 + q * 16;
+            uint32_t v[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              v[i] = pack2<T>(__uint_as_float(r[c][q * 8 + 2 * i]),
-                              __uint_as_float(r[c][q * 8 + 2 * i + 1]));
-            *reinterpret_cast<uint4*>(out + c * 32 + q * 8) = make_uint4(v[0], v[1], v[2], v[3]);
+            for (int i = 0; i < 8; ++i)
+              v[i] = pack2<T>(__uint_as_float(r[c][q * 16 + 2 * i]),
+                              __uint_as_float(r[c][q * 16 + 2 * i + 1]));
+            if (p.vec_ok == 2) {
+              if (n0 + n < p.N) st_global_32b(out + n, v);
+            } else {
+              if (n0 + n < p.N)
+                *reinterpret_cast<uint4*>(out + n) = make_uint4(v[0], v[1], v[2], v[3]);
+              if (n0 + n + 8 < p.N)
+                *reinterpret_cast<uint4*>(out + n + 8) = make_uint4(v[4], v[5], v[6], v[7]);
+            }
           }
       } else {
 #pragma unroll
@@ -572,7 +579,10 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   p.atoms_k = static_cast<int>((a.K + 127) / 128);
   p.d = a.d;
   p.ldd = a.ldd;
-  p.vec_ok = a.N % 8 == 0 && a.ldd % 8 == 0 && (reinterpret_cast<uintptr_t>(a.d) & 15u) == 0;
+  const uintptr_t d_addr = reinterpret_cast<uintptr_t>(a.d);
+  p.vec_ok = a.N % 16 == 0 && a.ldd % 16 == 0 && d_addr % 32 == 0 ? 2
+             : a.N % 8 == 0 && a.ldd % 8 == 0 && d_addr % 16 == 0 ? 1
+                                                                  : 0;
   p.status = device_status_ptr();
   auto kern = mx_pair_kernel<kBF16>;
   static std::atomic<int> max_pairs[64];
