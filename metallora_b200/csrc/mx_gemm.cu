@@ -426,7 +426,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(lead_acc_empty);
+      if (lane == 0) mbar_arrive_cluster_relaxed(lead_acc_empty);
       if (m >= p.M) continue;
       T* out = reinterpret_cast<T*>(p.d) + static_cast<long long>(m) * p.ldd + n0;
       if (p.vec_ok) {

@@ -329,6 +329,14 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
                : "memory");
 }
 
+// The same without the release: it orders no memory accesses, and so does not
+// wait for this thread's outstanding global stores.  Enough to hand back TMEM:
+// tcgen05.wait::ld and tcgen05.fence::before_thread_sync come before it.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr)
+               : "memory");
+}
+
 // 2-D tile load into this CTA's shared memory whose completion is counted on
 // an mbarrier of the pair's even CTA (`bar_cluster`).
 __device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map,
