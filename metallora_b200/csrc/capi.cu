@@ -524,7 +524,46 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
 
   // kPhaseDeferDx stops before the dx GEMM (s.dy.B stays in the workspace);
   // kPhaseDx runs only that GEMM, from the workspace of a deferred call.
-  if (phase != kPhaseDx) {
+  if (phase != kPhaseDx && ckpt != nullptr) {
+    // dy's two products, then dA from the checkpoint
+    LoraBwdArgs l;
+    l.dy = dy;
+    l.b = b;
+    l.xa_t = saved_xa;
+    l.ld_xa = pad8(M);
+    l.M = M;
+    l.N = N;
+    l.r = r;
+    l.R = p.R;
+    l.scale = scale;
+    l.u_rows = dx ? p.u_rows : nullptr;
+    l.ld_rows = p.R64;
+    l.u_t = p.u_t;
+    l.ld_t = pad8(M);
+    l.db = db;
+    l.accumulate = accumulate;
+    l.out16 = grads16;
+    l.clip = clip_value;
+    l.elt = elt;
+    if ((rc = launch_lora_bwd(l, s))) return rc;
+    MxWgradArgs g;
+    g.codes = ckpt->codes;
+    g.scales = ckpt->scales;
+    g.ld = ckpt->ld;
+    g.st = p.u_t;
+    g.ld_st = pad8(M);
+    g.M = M;
+    g.K = K;
+    g.r = r;
+    g.R = p.R;
+    g.out = da;
+    g.accumulate = accumulate;
+    g.out16 = grads16;
+    g.clip = clip_value;
+    g.elt = elt;
+    g.overlap_prev = true;
+    if ((rc = launch_mx_wgrad(g, s))) return rc;
+  } else if (phase != kPhaseDx) {
     // B^T, zero-padded to R rows: the K-major operand of the U = s.dy.B projection.
     if ((rc = launch_transpose_pad(b, N, r, r, p.bt, p.R, elt, s))) return rc;
 
@@ -596,26 +635,7 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
     w[1].out = da;
     w[1].ldo = K;
     w[1].transposed = true;
-    if (ckpt != nullptr) w[0].splits = wgrad_splits(M, N, 1);
-    if ((rc = launch_wgrad(w, ckpt != nullptr ? 1 : 2, s))) return rc;
-    if (ckpt != nullptr) {
-      MxWgradArgs g;
-      g.codes = ckpt->codes;
-      g.scales = ckpt->scales;
-      g.ld = ckpt->ld;
-      g.st = p.u_t;
-      g.ld_st = pad8(M);
-      g.M = M;
-      g.K = K;
-      g.r = r;
-      g.R = p.R;
-      g.out = da;
-      g.accumulate = accumulate;
-      g.out16 = grads16;
-      g.clip = clip_value;
-      g.elt = elt;
-      if ((rc = launch_mx_wgrad(g, s))) return rc;
-    }
+    if ((rc = launch_wgrad(w, 2, s))) return rc;
   }
   if (phase == kPhaseDeferDx) return MLORA_OK;
 
@@ -659,8 +679,9 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
     ga.out_dtype = dtype;
     // in one call the weight-gradient kernel was launched just before: the
     // GEMM starts on SMs it frees; its X2 (s.dy.B) was complete before that
-    // kernel passed its own wait, and dy, W0 before the call
-    ga.overlap_prev = phase == kPhaseAll;
+    // kernel passed its own wait, and dy, W0 before the call.  (The kernel that
+    // takes a checkpoint lets no dependent start early.)
+    ga.overlap_prev = phase == kPhaseAll && ckpt == nullptr;
     if ((rc = launch_gemm(ga, s))) return rc;
   }
 
@@ -732,6 +753,14 @@ bool make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, cons
                   uint64_t inner, uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,
                   uint32_t box_outer, bool swizzle128) {
   (void)esize;
+  return make_tmap_2d_swizzled(map, dt, base, inner, outer, row_stride_bytes, box_inner, box_outer,
+                               swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                          : CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+bool make_tmap_2d_swizzled(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
+                           uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                           uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (fn == nullptr) {
     set_error("cuTensorMapEncodeTiled entry point unavailable");
@@ -742,8 +771,7 @@ bool make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, cons
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
   CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (code " + std::to_string(static_cast<int>(r)) +

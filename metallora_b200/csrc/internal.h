@@ -27,6 +27,9 @@ bool make_tmap_2d_16b(CUtensorMap* map, const void* base, uint64_t inner, uint64
 bool make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, uint32_t esize, const void* base,
                   uint64_t inner, uint64_t outer, uint64_t row_stride_bytes, uint32_t box_inner,
                   uint32_t box_outer, bool swizzle128);
+bool make_tmap_2d_swizzled(CUtensorMap* map, CUtensorMapDataType dt, const void* base,
+                           uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
+                           uint32_t box_inner, uint32_t box_outer, CUtensorMapSwizzle swizzle);
 
 // ---- launch accounting / opt-in profiling ----------------------------------
 // Kernel kinds for mlora_profile_* (index into the per-kind totals).
@@ -200,6 +203,28 @@ struct WgradArgs {
 int wgrad_splits(int64_t M, int64_t P, int nproblems);
 int launch_wgrad(const WgradArgs* probs, int nprobs, cudaStream_t stream);
 
+// ------------------------------------------- both products of dy, one launch --
+// U = scale dy.B: u_rows [M, ld_rows] (may be null; columns past R zeroed) and
+// u_t [R, ld_t]; db (+)= clip(dy^T . xa_t^T) [N, r].  dy [M, N], b [N, r],
+// xa_t [R, ld_xa] (rows >= r are zero).
+struct LoraBwdArgs {
+  const void* dy;
+  const void* b;
+  const void* xa_t;
+  int64_t ld_xa;
+  int64_t M, N, r, R;
+  float scale;
+  void* u_rows;
+  int64_t ld_rows;
+  void* u_t;
+  int64_t ld_t;
+  void* db;
+  bool accumulate, out16;
+  float clip;
+  Elt elt;
+};
+int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t stream);
+
 // ---------------------------------------------------------------- peers ------
 // One-shot all-reduce over peer memory (see peer.cu); counter: one zeroed
 // device word per communicator, reset by the kernel.
@@ -335,6 +360,7 @@ struct MxWgradArgs {
   bool accumulate, out16;
   float clip;
   Elt elt;
+  bool overlap_prev = false;  // programmatic dependent of the kernel that wrote st
 };
 int launch_mx_wgrad(const MxWgradArgs& a, cudaStream_t s);
 

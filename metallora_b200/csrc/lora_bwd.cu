@@ -1,0 +1,298 @@
+// The two products of the LoRA backward that read dy, in one launch:
+//
+//     U  = s dy . B           (rows [M, R64] and transposed [R, M])
+//     dB = dy^T . (s x A^T)   ([N, r])
+//
+// U reduces over features, dB over tokens, so neither is a by-product of the
+// other's pass; but run side by side they read dy at about the same time, so it
+// comes from HBM once and from L2 the second time, and one launch's start and
+// reduction tail are paid instead of two.  B is read as it lies ([N, r], the
+// MMA's MN-major operand): no transposed copy.
+//
+// A cluster owns one 128-row tile of U or of dB and splits its reduction; the
+// partial tiles meet through distributed shared memory in fixed order
+// (cluster_reduce).  Warp 0 copies, warp 1 issues the UMMAs, warps 2-5 store.
+#include <atomic>
+#include <string>
+#include <type_traits>
+
+#include "cluster_reduce.cuh"
+#include "internal.h"
+#include "ptx.cuh"
+#include "../../include/metallora_b200.h"
+
+namespace mlora {
+namespace {
+
+constexpr int kThreads = 192;
+constexpr int kBK = 64;
+constexpr uint32_t kDyBytes = 128 * kBK * 2;   // [128 x 64] of dy
+constexpr uint32_t kHalfBytes = 64 * kBK * 2;  // one MN-major box
+constexpr int kMaxSplits = 8;
+
+__host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
+__host__ __device__ constexpr uint32_t stage_bytes(int R) { return kDyBytes + R * 128u; }
+__host__ __device__ constexpr int num_stages(int R) {
+  const int n = static_cast<int>((ctas_per_sm(R) == 2 ? 108u : 200u) * 1024u / stage_bytes(R));
+  return n > 8 ? 8 : n;
+}
+constexpr size_t smem_bytes(int R) { return 1024 + num_stages(R) * stage_bytes(R) + 256; }
+__host__ __device__ constexpr uint32_t tmem_cols(int R) {
+  return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
+}
+
+// B's tile [64 rows x R columns], R contiguous: one box of R columns in the
+// swizzle of its row length (32, 64 or 128 bytes), or boxes of 64 columns.
+__host__ __device__ constexpr uint32_t b_row_bytes(int R) { return R >= 64 ? 128u : R * 2u; }
+template <int R>
+__device__ __forceinline__ uint64_t desc_b(uint32_t saddr, uint32_t k16_step) {
+  constexpr uint32_t row = b_row_bytes(R);
+  constexpr uint32_t layout = row == 128u ? kLayoutSW128 : (row == 64u ? kLayoutSW64 : kLayoutSW32);
+  return make_smem_desc(saddr + k16_step * 16u * row, 64u * row, 8u * row, layout);
+}
+
+struct BwdParams {
+  long long M, N;
+  int r;
+  int tiles_db, kb_u, kb_db, splits;
+  float scale, clip;
+  void* u_rows;
+  long long ld_rows;
+  void* u_t;
+  long long ld_t;
+  void* db;
+  int accumulate, out16;
+  uint32_t* status;
+};
+
+// 1-D grid, cluster (splits, 1, 1): tile b / splits (dB's tiles first: with more
+// tokens than features theirs is the longer reduction), range b % splits.
+template <int R, bool kBF16>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
+    lora_bwd_kernel(const __grid_constant__ CUtensorMap tm_dy_rows,
+                    const __grid_constant__ CUtensorMap tm_dy_cols,
+                    const __grid_constant__ CUtensorMap tm_b,
+                    const __grid_constant__ CUtensorMap tm_xa, const BwdParams p) {
+  using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
+  constexpr int S = num_stages(R);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R));
+  uint64_t* empty_bar = full_bar + S;
+  uint64_t* done_bar = empty_bar + S;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
+
+  const uint32_t warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
+    mbar_init(done_bar, 1);
+    fence_mbarrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, tmem_cols(R));
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // the dA kernel may start its set-up and stream its codes
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  const int cid = static_cast<int>(blockIdx.x) / p.splits;
+  const bool is_db = cid < p.tiles_db;
+  const int tile = is_db ? cid : cid - p.tiles_db;
+  const uint32_t crank = cluster_ctarank();
+  const int num_kb = is_db ? p.kb_db : p.kb_u;
+  const int per = (num_kb + p.splits - 1) / p.splits;
+  const int kb_begin = static_cast<int>(crank) * per;
+  const int kb_end = min(num_kb, kb_begin + per);
+  const bool has_work = kb_begin < kb_end;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      bool armed[S];
+      uint32_t armed_parity[S];
+      for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
+        uint8_t* sa = smem + stage * stage_bytes(R);
+        uint8_t* sb = sa + kDyBytes;
+        uint64_t* bar = &full_bar[stage];
+        mbar_arrive_expect_tx(bar, stage_bytes(R));
+        armed[stage] = true;
+        armed_parity[stage] = phase;
+        if (is_db) {
+          tma_load_2d(sa, &tm_dy_cols, bar, tile * 128, kb * kBK);
+          tma_load_2d(sa + kHalfBytes, &tm_dy_cols, bar, tile * 128 + 64, kb * kBK);
+          tma_load_2d(sb, &tm_xa, bar, kb * kBK, 0);
+        } else {
+          tma_load_2d(sa, &tm_dy_rows, bar, kb * kBK, tile * 128);
+#pragma unroll
+          for (int i = 0; i < (R + 63) / 64; ++i)
+            tma_load_2d(sb + i * 64 * b_row_bytes(R), &tm_b, bar, i * 64, kb * kBK);
+        }
+        if (++stage == S) stage = 0, phase ^= 1u;
+      }
+      for (int s = 0; s < S; ++s)
+        if (armed[s]) mbar_wait(&full_bar[s], armed_parity[s], p.status, kDevTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (has_work && elect_one()) {
+      constexpr uint32_t idesc_u = make_idesc_f16(128, R, false, true, kBF16);
+      constexpr uint32_t idesc_db = make_idesc_f16(128, R, true, false, kBF16);
+      uint32_t stage = 0, phase = 0;
+      for (int kb = kb_begin; kb < kb_end; ++kb) {
+        if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) break;
+        tc_fence_after();
+        const uint32_t sa = smem_u32(smem + stage * stage_bytes(R));
+        const uint32_t sb = sa + kDyBytes;
+        if (is_db) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem, desc_mnmajor_sw128(sa, k, kHalfBytes), desc_kmajor_sw128(sb, k), idesc_db,
+                     (kb != kb_begin || k != 0) ? 1u : 0u);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16(tmem, desc_kmajor_sw128(sa, k), desc_b<R>(sb, k), idesc_u,
+                     (kb != kb_begin || k != 0) ? 1u : 0u);
+        }
+        umma_commit(&empty_bar[stage]);
+        if (++stage == S) stage = 0, phase ^= 1u;
+      }
+      umma_commit(done_bar);
+    }
+  }
+  const bool epi = warp >= 2;
+  const int row_local = static_cast<int>((warp & 3u) * 32 + lane_id());
+  const long long row = static_cast<long long>(tile) * 128 + row_local;
+  bool have = false;
+  if (epi && has_work) {
+    have = mbar_wait(done_bar, 0, p.status, kDevTimeoutAccFull);
+    tc_fence_after();
+  }
+  const bool live = epi && row < (is_db ? p.N : p.M);
+  auto emit = [&](int j, float v0, float v1) {
+    if (!live) return;
+    if (is_db) {
+      float v[2] = {v0, v1};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (j + i >= p.r) continue;
+        if (p.clip > 0.f) v[i] = fminf(fmaxf(v[i], -p.clip), p.clip);
+        const long long at = row * p.r + j + i;
+        if (p.out16) {
+          T* d = reinterpret_cast<T*>(p.db) + at;
+          *d = static_cast<T>(p.accumulate ? static_cast<float>(*d) + v[i] : v[i]);
+        } else {
+          float* d = reinterpret_cast<float*>(p.db) + at;
+          *d = p.accumulate ? *d + v[i] : v[i];
+        }
+      }
+      return;
+    }
+    v0 *= p.scale;
+    v1 *= p.scale;
+    if (p.u_rows != nullptr)
+      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows + j) =
+          pack2<T>(v0, v1);
+    T* dst = reinterpret_cast<T*>(p.u_t) + row;
+    dst[static_cast<long long>(j) * p.ld_t] = static_cast<T>(v0);
+    dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(v1);
+  };
+  cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
+                    reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+  if (live && !is_db && crank == 0 && p.u_rows != nullptr) {  // zero columns past R
+    T* dst = reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows;
+    for (long long j = R; j < p.ld_rows; j += 8)
+      *reinterpret_cast<uint4*>(dst + j) = make_uint4(0, 0, 0, 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols(R));
+  }
+}
+
+template <int R, bool kBF16>
+int launch_typed(const LoraBwdArgs& a, cudaStream_t stream) {
+  CUtensorMap tr, tc, tb, tx;
+  const CUtensorMapSwizzle sw = b_row_bytes(R) == 128u  ? CU_TENSOR_MAP_SWIZZLE_128B
+                                : b_row_bytes(R) == 64u ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                        : CU_TENSOR_MAP_SWIZZLE_32B;
+  if (!make_tmap_2d_16b(&tr, a.dy, a.N, a.M, a.N, kBK, 128) ||
+      !make_tmap_2d_16b(&tc, a.dy, a.N, a.M, a.N, 64, kBK) ||
+      !make_tmap_2d_swizzled(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT16, a.b, static_cast<uint64_t>(a.r),
+                             static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.r) * 2,
+                             R >= 64 ? 64 : R, kBK, sw) ||
+      !make_tmap_2d_16b(&tx, a.xa_t, a.M, a.R, a.ld_xa, kBK, R))
+    return MLORA_ERR_INVALID_ARG;
+  BwdParams p;
+  p.M = a.M;
+  p.N = a.N;
+  p.r = static_cast<int>(a.r);
+  p.tiles_db = static_cast<int>((a.N + 127) / 128);
+  p.kb_u = static_cast<int>((a.N + kBK - 1) / kBK);
+  p.kb_db = static_cast<int>((a.M + kBK - 1) / kBK);
+  p.scale = a.scale;
+  p.clip = a.clip;
+  p.u_rows = a.u_rows;
+  p.ld_rows = a.ld_rows;
+  p.u_t = a.u_t;
+  p.ld_t = a.ld_t;
+  p.db = a.db;
+  p.accumulate = a.accumulate ? 1 : 0;
+  p.out16 = a.out16 ? 1 : 0;
+  p.status = device_status_ptr();
+  const int64_t tiles = p.tiles_db + (a.M + 127) / 128;
+  const int64_t slots = static_cast<int64_t>(ctas_per_sm(R)) * num_sms();
+  const int longest = p.kb_u > p.kb_db ? p.kb_u : p.kb_db;
+  int splits = 1;
+  while (splits * 2 <= kMaxSplits && splits * 2 * tiles * 2 <= slots * 3 && splits * 8 <= longest)
+    splits *= 2;
+  p.splits = splits;
+  auto kern = lora_bwd_kernel<R, kBF16>;
+  static std::atomic<bool> attr_set[64];
+  if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem_bytes(R);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LaunchScope scope(kKindRank, stream);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tr, tc, tb, tx, p);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e == cudaSuccess) return MLORA_OK;
+  set_error(std::string("lora backward launch: ") + cudaGetErrorString(e));
+  return MLORA_ERR_CUDA;
+}
+
+template <bool kB>
+int dispatch(const LoraBwdArgs& a, cudaStream_t s) {
+  switch (a.R) {
+    case 16: return launch_typed<16, kB>(a, s);
+    case 32: return launch_typed<32, kB>(a, s);
+    case 64: return launch_typed<64, kB>(a, s);
+    case 128: return launch_typed<128, kB>(a, s);
+    case 256: return launch_typed<256, kB>(a, s);
+    default: set_error("unsupported padded rank"); return MLORA_ERR_UNSUPPORTED;
+  }
+}
+
+}  // namespace
+
+int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t s) {
+  return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
+}
+
+}  // namespace mlora

@@ -144,21 +144,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       bool armed[S];
       uint32_t armed_parity[S];
       for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
-      bool prev_done = false;
-      for (int kb = kb_begin; kb < kb_end; ++kb) {
-        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
-        uint8_t* st = stages + stage * stage_bytes(R);
-        uint64_t* bar = &full_bar[stage];
+      auto load_codes = [&](int kb, uint8_t* st, uint64_t* bar) {
         mbar_arrive_expect_tx(bar, R * 128u + kCodeBytes + kScaleBytes);
-        armed[stage] = true;
-        armed_parity[stage] = phase;
         tma_load_2d(st + kCodeOff, &tm_codes, bar, tile * 128, kb * kBM);
         tma_load_2d(st + kScaleOff, &tm_scales, bar, kb * kBM, tile);
-        if (!prev_done) {  // U comes from the kernel before this one
-          asm volatile("griddepcontrol.wait;" ::: "memory");
-          prev_done = true;
-        }
-        tma_load_2d(st, &tm_st, bar, kb * kBM, 0);
+      };
+      // U comes from the kernel before this one, the checkpoint does not: a ring
+      // of code blocks is on its way before the wait
+      const int ahead = min(S, kb_end - kb_begin);
+      for (int i = 0; i < ahead; ++i) {
+        load_codes(kb_begin + i, stages + i * stage_bytes(R), &full_bar[i]);
+        armed[i] = true;
+      }
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < ahead; ++i)
+        tma_load_2d(stages + i * stage_bytes(R), &tm_st, &full_bar[i], (kb_begin + i) * kBM, 0);
+      if (ahead == S) phase = 1;
+      for (int kb = kb_begin + ahead; kb < kb_end; ++kb) {
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
+        uint8_t* st = stages + stage * stage_bytes(R);
+        armed[stage] = true;
+        armed_parity[stage] = phase;
+        load_codes(kb, st, &full_bar[stage]);
+        tma_load_2d(st, &tm_st, &full_bar[stage], kb * kBM, 0);
         if (++stage == S) stage = 0, phase ^= 1u;
       }
       for (int s = 0; s < S; ++s)
@@ -300,13 +308,15 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem_bytes(R);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.overlap_prev ? 2 : 1;
   LaunchScope scope(kKindWgrad, stream);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tc, ts, tu, p);
   if (e == cudaSuccess) e = cudaGetLastError();
