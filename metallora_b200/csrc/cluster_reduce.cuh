@@ -30,13 +30,15 @@ __device__ __forceinline__ void load_acc_row(uint32_t taddr_row, float (&acc)[R]
 // A second barrier keeps every CTA resident until its peers have read it.
 // Columns go in passes of CP (R > 128: two passes), each read from TMEM at
 // `taddr` (this thread's lane) when `have` (zeros otherwise).  Every thread of
-// the CTA calls this; only epilogue threads (`epi`) move data.
+// the CTA calls this; only epilogue threads (`epi`) move data.  A cluster may
+// hold several such groups of S CTAs side by side: `first` is the cluster rank
+// of this group's first CTA, `crank` the rank within the group.
 __host__ __device__ constexpr int reduce_cols(int R) { return R <= 128 ? R : 128; }
 
 template <int R, typename Emit>
 __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float* buf, int S,
                                                uint32_t crank, int row_local, bool epi,
-                                               Emit&& emit) {
+                                               Emit&& emit, uint32_t first = 0) {
   constexpr int CP = reduce_cols(R);
 #pragma unroll 1
   for (int pass = 0; pass < R / CP; ++pass) {
@@ -58,7 +60,7 @@ __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float*
       const uint32_t base = smem_u32(buf) + static_cast<uint32_t>(row_local) * 4u;
       uint32_t peer[8];
 #pragma unroll
-      for (int s = 0; s < 8; ++s) peer[s] = s < S ? mapa_shared(base, static_cast<uint32_t>(s)) : 0u;
+      for (int s = 0; s < 8; ++s) peer[s] = s < S ? mapa_shared(base, first + static_cast<uint32_t>(s)) : 0u;
 #pragma unroll 1
       for (int jj = 0; jj < W; jj += 2) {
         const uint32_t off0 = static_cast<uint32_t>(j0 + jj) * 512u;

@@ -9,9 +9,11 @@
 // reduction tail are paid instead of two.  B is read as it lies ([N, r], the
 // MMA's MN-major operand): no transposed copy.
 //
-// A cluster owns one 128-row tile of U or of dB and splits its reduction; the
-// partial tiles meet through distributed shared memory in fixed order
-// (cluster_reduce).  Warp 0 copies, warp 1 issues the UMMAs, warps 2-5 store.
+// A CTA owns one 128-row tile of U or of dB and one range of its reduction; the
+// ranges of a tile lie in one cluster, and their partial tiles meet through
+// distributed shared memory in fixed order (cluster_reduce).  The two products
+// are split apart from each other, so that all CTAs have about the same number
+// of k-blocks.  Warp 0 copies, warp 1 issues the UMMAs, warps 2-5 store.
 #include <atomic>
 #include <string>
 #include <type_traits>
@@ -54,7 +56,9 @@ __device__ __forceinline__ uint64_t desc_b(uint32_t saddr, uint32_t k16_step) {
 struct BwdParams {
   long long M, N;
   int r;
-  int tiles_db, kb_u, kb_db, splits;
+  int tiles_u, tiles_db, kb_u, kb_db;
+  int splits_u, splits_db;  // ranges a tile (powers of two)
+  int ctas_u;               // CTAs of U's tiles, whole clusters; then dB's
   float scale, clip;
   void* u_rows;
   long long ld_rows;
@@ -65,8 +69,8 @@ struct BwdParams {
   uint32_t* status;
 };
 
-// 1-D grid, cluster (splits, 1, 1): tile b / splits (dB's tiles first: with more
-// tokens than features theirs is the longer reduction), range b % splits.
+// 1-D grid, cluster (max(splits_u, splits_db), 1, 1).  A cluster holds tiles of
+// one product only; the last one of each may hold CTAs without a tile.
 template <int R, bool kBF16>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     lora_bwd_kernel(const __grid_constant__ CUtensorMap tm_dy_rows,
@@ -99,14 +103,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   // the dA kernel may start its set-up and stream its codes
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int cid = static_cast<int>(blockIdx.x) / p.splits;
-  const bool is_db = cid < p.tiles_db;
-  const int tile = is_db ? cid : cid - p.tiles_db;
-  const uint32_t crank = cluster_ctarank();
+  const bool is_db = static_cast<int>(blockIdx.x) >= p.ctas_u;
+  const int splits = is_db ? p.splits_db : p.splits_u;
+  const int id = static_cast<int>(blockIdx.x) - (is_db ? p.ctas_u : 0);
+  const int tile = id / splits;
+  const uint32_t crank = static_cast<uint32_t>(id % splits);
+  const uint32_t first = cluster_ctarank() - crank;
   const int num_kb = is_db ? p.kb_db : p.kb_u;
-  const int per = (num_kb + p.splits - 1) / p.splits;
+  const int per = (num_kb + splits - 1) / splits;
   const int kb_begin = static_cast<int>(crank) * per;
-  const int kb_end = min(num_kb, kb_begin + per);
+  const int kb_end =
+      tile < (is_db ? p.tiles_db : p.tiles_u) ? min(num_kb, kb_begin + per) : kb_begin;
   const bool has_work = kb_begin < kb_end;
 
   if (warp == 0) {
@@ -203,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(v1);
   };
   cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
-                    reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+                    reinterpret_cast<float*>(smem), splits, crank, row_local, epi, emit, first);
   if (live && !is_db && crank == 0 && p.u_rows != nullptr) {  // zero columns past R
     T* dst = reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows;
     for (long long j = R; j < p.ld_rows; j += 8)
@@ -247,24 +254,40 @@ int launch_typed(const LoraBwdArgs& a, cudaStream_t stream) {
   p.accumulate = a.accumulate ? 1 : 0;
   p.out16 = a.out16 ? 1 : 0;
   p.status = device_status_ptr();
-  const int64_t tiles = p.tiles_db + (a.M + 127) / 128;
+  p.tiles_u = static_cast<int>((a.M + 127) / 128);
+  // Halve the longer range while all CTAs stay resident at once (and a range
+  // keeps four k-blocks).  8192 x 4096: 128 + 128 CTAs of 32 blocks each; 1001 x
+  // 11008: 64 of 22 and 172 of 8.
   const int64_t slots = static_cast<int64_t>(ctas_per_sm(R)) * num_sms();
-  const int longest = p.kb_u > p.kb_db ? p.kb_u : p.kb_db;
-  int splits = 1;
-  while (splits * 2 <= kMaxSplits && splits * 2 * tiles * 2 <= slots * 3 && splits * 8 <= longest)
-    splits *= 2;
-  p.splits = splits;
+  int64_t su = 1, sd = 1;
+  while (true) {
+    const bool can_u = su < kMaxSplits && su * 8 <= p.kb_u &&
+                       2 * su * p.tiles_u + sd * p.tiles_db <= slots;
+    const bool can_d = sd < kMaxSplits && sd * 8 <= p.kb_db &&
+                       su * p.tiles_u + 2 * sd * p.tiles_db <= slots;
+    if (can_u && (!can_d || p.kb_u / su >= p.kb_db / sd))
+      su *= 2;
+    else if (can_d)
+      sd *= 2;
+    else
+      break;
+  }
+  const int64_t cluster = su > sd ? su : sd;
+  p.splits_u = static_cast<int>(su);
+  p.splits_db = static_cast<int>(sd);
+  p.ctas_u = static_cast<int>((p.tiles_u * su + cluster - 1) / cluster * cluster);
+  const int64_t ctas_db = (p.tiles_db * sd + cluster - 1) / cluster * cluster;
   auto kern = lora_bwd_kernel<R, kBF16>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles * splits));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas_u + ctas_db));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem_bytes(R);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
