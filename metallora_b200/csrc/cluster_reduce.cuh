@@ -9,14 +9,14 @@ namespace mlora {
 // Loads this thread's accumulator row (R fp32 columns) from TMEM into `acc`.
 template <int R>
 __device__ __forceinline__ void load_acc_row(uint32_t taddr_row, float (&acc)[R]) {
+  uint32_t r[R / 16][16];
 #pragma unroll
-  for (int c = 0; c < R / 16; ++c) {
-    uint32_t r[16];
-    tmem_ld_32x32b_x16(taddr_row + c * 16, r);
-    tmem_ld_wait();
+  for (int c = 0; c < R / 16; ++c) tmem_ld_32x32b_x16(taddr_row + c * 16, r[c]);
+  tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = __uint_as_float(r[i]);
-  }
+  for (int c = 0; c < R / 16; ++c)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) acc[c * 16 + i] = __uint_as_float(r[c][i]);
 }
 
 // Cross-CTA split reduction through distributed shared memory.  The S CTAs of
@@ -28,12 +28,48 @@ __device__ __forceinline__ void load_acc_row(uint32_t taddr_row, float (&acc)[R]
 // of all 128 rows over s = 0..S-1 in that order -- fixed order, so results are
 // bitwise reproducible -- and hands pairs of columns to `emit(j, v_j, v_j+1)`.
 // A second barrier keeps every CTA resident until its peers have read it.
+// One CTA alone (S = 1) emits straight from its registers, without a barrier.
 // Columns go in passes of CP (R > 128: two passes), each read from TMEM at
 // `taddr` (this thread's lane) when `have` (zeros otherwise).  Every thread of
 // the CTA calls this; only epilogue threads (`epi`) move data.  A cluster may
 // hold several such groups of S CTAs side by side: `first` is the cluster rank
 // of this group's first CTA, `crank` the rank within the group.
 __host__ __device__ constexpr int reduce_cols(int R) { return R <= 128 ? R : 128; }
+
+// This CTA's slice of the columns: W = CP / S of them from j0, the sums of the
+// S peers' values.  Up to 32 loads are in flight before the first sum: each is a
+// trip to another SM (with two at a time, 64 columns over two CTAs took 13 us).
+template <int CP, int S, typename Emit>
+__device__ __forceinline__ void sum_slices(const float* buf, int crank, uint32_t first,
+                                           int row_local, int j_base, Emit&& emit) {
+  constexpr int W = CP / S;
+  constexpr int B = W < 32 / S ? W : 32 / S;
+  static_assert(W >= 2 && W % B == 0 && B % 2 == 0, "columns come in pairs");
+  const int j0 = crank * W;
+  const uint32_t base = smem_u32(buf) + static_cast<uint32_t>(row_local) * 4u;
+  uint32_t peer[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) peer[s] = mapa_shared(base, first + static_cast<uint32_t>(s));
+#pragma unroll 1
+  for (int jj = 0; jj < W; jj += B) {
+    const uint32_t off = static_cast<uint32_t>(j0 + jj) * 512u;
+    float a[B][S];
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+#pragma unroll
+      for (int s = 0; s < S; ++s) a[i][s] = ld_shared_cluster_f32(peer[s] + off + i * 512u);
+#pragma unroll
+    for (int i = 0; i < B; i += 2) {
+      float v0 = 0.f, v1 = 0.f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        v0 += a[i][s];
+        v1 += a[i + 1][s];
+      }
+      emit(j_base + j0 + jj + i, v0, v1);
+    }
+  }
+}
 
 template <int R, typename Emit>
 __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float* buf, int S,
@@ -50,34 +86,24 @@ __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float*
 #pragma unroll
         for (int j = 0; j < CP; ++j) acc[j] = 0.f;
       }
+      if (S == 1) {  // the whole sum is here
 #pragma unroll
-      for (int j = 0; j < CP; ++j) buf[j * 128 + row_local] = acc[j];
+        for (int j = 0; j < CP; j += 2) emit(pass * CP + j, 0.f + acc[j], 0.f + acc[j + 1]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < CP; ++j) buf[j * 128 + row_local] = acc[j];
+      }
     }
+    if (S == 1) continue;
     cluster_sync();
     if (epi) {
-      const int W = CP / S;
-      const int j0 = static_cast<int>(crank) * W;
-      const uint32_t base = smem_u32(buf) + static_cast<uint32_t>(row_local) * 4u;
-      uint32_t peer[8];
-#pragma unroll
-      for (int s = 0; s < 8; ++s) peer[s] = s < S ? mapa_shared(base, first + static_cast<uint32_t>(s)) : 0u;
-#pragma unroll 1
-      for (int jj = 0; jj < W; jj += 2) {
-        const uint32_t off0 = static_cast<uint32_t>(j0 + jj) * 512u;
-        float a[8], b[8];
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          a[s] = s < S ? ld_shared_cluster_f32(peer[s] + off0) : 0.f;
-          b[s] = s < S ? ld_shared_cluster_f32(peer[s] + off0 + 512u) : 0.f;
-        }
-        float v0 = 0.f, v1 = 0.f;
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-          v0 += a[s];
-          v1 += b[s];
-        }
-        emit(pass * CP + j0 + jj, v0, v1);
-      }
+      const int c = static_cast<int>(crank);
+      if (S == 2)
+        sum_slices<CP, 2>(buf, c, first, row_local, pass * CP, emit);
+      else if (S == 4)
+        sum_slices<CP, 4>(buf, c, first, row_local, pass * CP, emit);
+      else
+        sum_slices<CP, 8>(buf, c, first, row_local, pass * CP, emit);
     }
     cluster_sync();
   }

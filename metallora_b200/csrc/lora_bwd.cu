@@ -184,19 +184,24 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   auto emit = [&](int j, float v0, float v1) {
     if (!live) return;
     if (is_db) {
-      float v[2] = {v0, v1};
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (j + i >= p.r) continue;
-        if (p.clip > 0.f) v[i] = fminf(fmaxf(v[i], -p.clip), p.clip);
-        const long long at = row * p.r + j + i;
-        if (p.out16) {
-          T* d = reinterpret_cast<T*>(p.db) + at;
-          *d = static_cast<T>(p.accumulate ? static_cast<float>(*d) + v[i] : v[i]);
-        } else {
-          float* d = reinterpret_cast<float*>(p.db) + at;
-          *d = p.accumulate ? *d + v[i] : v[i];
+      if (j >= p.r) return;  // r is a multiple of 8: pairs of columns are whole
+      if (p.clip > 0.f) {
+        v0 = fminf(fmaxf(v0, -p.clip), p.clip);
+        v1 = fminf(fmaxf(v1, -p.clip), p.clip);
+      }
+      const long long at = row * p.r + j;
+      if (p.out16) {
+        uint32_t* d = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.db) + at);
+        if (p.accumulate) {
+          const uint32_t old = *d;
+          v0 += static_cast<float>(reinterpret_cast<const T*>(&old)[0]);
+          v1 += static_cast<float>(reinterpret_cast<const T*>(&old)[1]);
         }
+        *d = pack2<T>(v0, v1);
+      } else {
+        float2* d = reinterpret_cast<float2*>(reinterpret_cast<float*>(p.db) + at);
+        const float2 old = p.accumulate ? *d : make_float2(0.f, 0.f);
+        *d = p.accumulate ? make_float2(old.x + v0, old.y + v1) : make_float2(v0, v1);
       }
       return;
     }
