@@ -2,6 +2,8 @@
 // shared by the kernels that split their reduction dimension.
 #pragma once
 
+#include <type_traits>
+
 #include "ptx.cuh"
 
 namespace mlora {
@@ -36,6 +38,53 @@ __device__ __forceinline__ void load_acc_row(uint32_t taddr_row, float (&acc)[R]
 // of this group's first CTA, `crank` the rank within the group.
 __host__ __device__ constexpr int reduce_cols(int R) { return R <= 128 ? R : 128; }
 
+// Hands N consecutive column sums from column j to `emit`: all at once to one
+// that takes an array, in pairs to one that takes (j, v_j, v_j+1).
+template <int N, typename Emit>
+__device__ __forceinline__ void emit_columns(Emit& emit, int j, const float (&v)[N]) {
+  if constexpr (std::is_invocable<Emit&, int, float, float>::value) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) emit(j + i, v[i], v[i + 1]);
+  } else {
+    emit(j, v);
+  }
+}
+
+// N consecutive 16-bit values (rounded to nearest) or fp32 values of a row, in
+// the widest stores: a sector written in parts costs L2 a pass for each.  `dst`
+// is aligned to N values, up to 16 bytes; `wide`: to 32 bytes.
+template <typename T, int N>
+__device__ __forceinline__ void store_columns(T* dst, const float (&v)[N], bool wide) {
+  constexpr int W = N * static_cast<int>(sizeof(T)) / 4;  // 32-bit words
+  uint32_t w[W];
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    if constexpr (sizeof(T) == 2)
+      w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    else
+      w[i] = __float_as_uint(v[i]);
+  }
+  uint32_t* d = reinterpret_cast<uint32_t*>(dst);
+  if constexpr (W == 1) {
+    *d = w[0];
+  } else if constexpr (W == 2) {
+    *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < W; i += 4) {
+      if (wide && W % 8 == 0) {
+        if (i % 8 == 0) {
+          const uint32_t q[8] = {w[i],           w[i + 1],       w[i + 2],       w[i + 3],
+                                 w[(i + 4) % W], w[(i + 5) % W], w[(i + 6) % W], w[(i + 7) % W]};
+          st_global_32b(d + i, q);
+        }
+      } else {
+        *reinterpret_cast<uint4*>(d + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+      }
+    }
+  }
+}
+
 // This CTA's slice of the columns: W = CP / S of them from j0, the sums of the
 // S peers' values.  Up to 32 loads are in flight before the first sum: each is a
 // trip to another SM (with two at a time, 64 columns over two CTAs took 13 us).
@@ -58,16 +107,14 @@ __device__ __forceinline__ void sum_slices(const float* buf, int crank, uint32_t
     for (int i = 0; i < B; ++i)
 #pragma unroll
       for (int s = 0; s < S; ++s) a[i][s] = ld_shared_cluster_f32(peer[s] + off + i * 512u);
+    float v[B];
 #pragma unroll
-    for (int i = 0; i < B; i += 2) {
-      float v0 = 0.f, v1 = 0.f;
+    for (int i = 0; i < B; ++i) {
+      v[i] = 0.f;
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        v0 += a[i][s];
-        v1 += a[i + 1][s];
-      }
-      emit(j_base + j0 + jj + i, v0, v1);
+      for (int s = 0; s < S; ++s) v[i] += a[i][s];
     }
+    emit_columns(emit, j_base + j0 + jj, v);
   }
 }
 
@@ -88,7 +135,12 @@ __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float*
       }
       if (S == 1) {  // the whole sum is here
 #pragma unroll
-        for (int j = 0; j < CP; j += 2) emit(pass * CP + j, 0.f + acc[j], 0.f + acc[j + 1]);
+        for (int j = 0; j < CP; j += 16) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0.f + acc[j + i];
+          emit_columns(emit, pass * CP + j, v);
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < CP; ++j) buf[j * 128 + row_local] = acc[j];

@@ -66,6 +66,8 @@ struct BwdParams {
   long long ld_t;
   void* db;
   int accumulate, out16;
+  int wide;  // dB's rows start on 32 bytes
+  int wide_rows;  // the row output starts on 32 bytes (its rows are 128 apart)
   uint32_t* status;
 };
 
@@ -181,38 +183,41 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     tc_fence_after();
   }
   const bool live = epi && row < (is_db ? p.N : p.M);
-  auto emit = [&](int j, float v0, float v1) {
+  auto emit = [&](int j, const auto& in) {
     if (!live) return;
-    if (is_db) {
-      if (j >= p.r) return;  // r is a multiple of 8: pairs of columns are whole
-      if (p.clip > 0.f) {
-        v0 = fminf(fmaxf(v0, -p.clip), p.clip);
-        v1 = fminf(fmaxf(v1, -p.clip), p.clip);
-      }
-      const long long at = row * p.r + j;
-      if (p.out16) {
-        uint32_t* d = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.db) + at);
-        if (p.accumulate) {
-          const uint32_t old = *d;
-          v0 += static_cast<float>(reinterpret_cast<const T*>(&old)[0]);
-          v1 += static_cast<float>(reinterpret_cast<const T*>(&old)[1]);
-        }
-        *d = pack2<T>(v0, v1);
-      } else {
-        float2* d = reinterpret_cast<float2*>(reinterpret_cast<float*>(p.db) + at);
-        const float2 old = p.accumulate ? *d : make_float2(0.f, 0.f);
-        *d = p.accumulate ? make_float2(old.x + v0, old.y + v1) : make_float2(v0, v1);
-      }
+    constexpr int C = std::extent<typename std::remove_reference<decltype(in)>::type>::value;
+    float v[C];
+    if (!is_db) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[i] = in[i] * p.scale;
+      if (p.u_rows != nullptr)
+        store_columns<T>(reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows + j, v, p.wide_rows != 0);
+      T* dst = reinterpret_cast<T*>(p.u_t) + row + j * p.ld_t;
+#pragma unroll
+      for (int i = 0; i < C; ++i) dst[i * p.ld_t] = static_cast<T>(v[i]);
       return;
     }
-    v0 *= p.scale;
-    v1 *= p.scale;
-    if (p.u_rows != nullptr)
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows + j) =
-          pack2<T>(v0, v1);
-    T* dst = reinterpret_cast<T*>(p.u_t) + row;
-    dst[static_cast<long long>(j) * p.ld_t] = static_cast<T>(v0);
-    dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(v1);
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      v[i] = p.clip > 0.f ? fminf(fmaxf(in[i], -p.clip), p.clip) : in[i];
+    const long long at = row * p.r + j;
+    if (p.accumulate || j + C > p.r) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        if (j + i >= p.r) continue;
+        if (p.out16) {
+          T* d = reinterpret_cast<T*>(p.db) + at + i;
+          *d = static_cast<T>(p.accumulate ? static_cast<float>(*d) + v[i] : v[i]);
+        } else {
+          float* d = reinterpret_cast<float*>(p.db) + at + i;
+          *d = p.accumulate ? *d + v[i] : v[i];
+        }
+      }
+    } else if (p.out16) {
+      store_columns<T>(reinterpret_cast<T*>(p.db) + at, v, p.wide != 0);
+    } else {
+      store_columns<float>(reinterpret_cast<float*>(p.db) + at, v, p.wide != 0);
+    }
   };
   cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
                     reinterpret_cast<float*>(smem), splits, crank, row_local, epi, emit, first);
@@ -258,6 +263,8 @@ int launch_typed(const LoraBwdArgs& a, cudaStream_t stream) {
   p.db = a.db;
   p.accumulate = a.accumulate ? 1 : 0;
   p.out16 = a.out16 ? 1 : 0;
+  p.wide = a.r % 16 == 0 && reinterpret_cast<uintptr_t>(a.db) % 32 == 0;
+  p.wide_rows = reinterpret_cast<uintptr_t>(a.u_rows) % 32 == 0;
   p.status = device_status_ptr();
   p.tiles_u = static_cast<int>((a.M + 127) / 128);
   // Halve the longer range while all CTAs stay resident at once (and a range

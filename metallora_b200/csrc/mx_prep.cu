@@ -56,6 +56,7 @@ struct PrepParams {
   long long ld8;
   uint8_t* q8_scales;  // words [ceil(K/128), rows8]
   long long rows8;
+  int wide_rows;  // the row output starts on 32 bytes (its rows are 128 apart)
   uint32_t* status;
 };
 
@@ -289,17 +290,18 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     tc_fence_after();
   }
   const bool live = epi && row < p.M;
-  auto emit = [&](int j, float v0, float v1) {
+  auto emit = [&](int j, const auto& in) {
     if (!live) return;
-    v0 *= p.scale;
-    v1 *= p.scale;
+    constexpr int C = std::extent<typename std::remove_reference<decltype(in)>::type>::value;
+    float v[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = in[i] * p.scale;
     if (p.out_rows != nullptr)
-      *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j) =
-          pack2<T>(v0, v1);
+      store_columns<T>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j, v, p.wide_rows != 0);
     if (p.out_t != nullptr) {
-      T* dst = reinterpret_cast<T*>(p.out_t) + row;
-      dst[static_cast<long long>(j) * p.ld_t] = static_cast<T>(v0);
-      dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(v1);
+      T* dst = reinterpret_cast<T*>(p.out_t) + row + j * p.ld_t;
+#pragma unroll
+      for (int i = 0; i < C; ++i) dst[i * p.ld_t] = static_cast<T>(v[i]);
     }
   };
   cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
@@ -344,6 +346,7 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   p.ld8 = a.ld8;
   p.q8_scales = static_cast<uint8_t*>(a.q8_scales);
   p.rows8 = (a.M + 3) / 4 * 4;
+  p.wide_rows = reinterpret_cast<uintptr_t>(a.out_rows) % 32 == 0;
   p.status = device_status_ptr();
   const int64_t tiles = (a.M + 127) / 128;
   // one wave of resident CTAs, at least four k-blocks a split
