@@ -283,9 +283,10 @@ inline int64_t prepared_ld(int64_t rows) { return (rows + 3) / 4 * 4; }
 // --------------------------------------------------- microscaled formats ------
 // Scale bytes (power-of-two exponent + 127) of 32-feature blocks of `rows` rows:
 //   kMxPlain : [rows, blocks], blocks = ceil(K / 32);
-//   kMxGroups: [ceil(K / 128), rows, 4], one word per row and 128 features;
-//   kMxAtoms : [ceil(rows / 128), ceil(K / 128), 512], the fp4 product's atoms.
-enum MxLayout : int { kMxPlain = 0, kMxGroups = 1, kMxAtoms = 2 };
+//   kMxGroups: [ceil(K / 128), rows, 4], one word per row and 128 features.
+// The fp4 product reads its operands' scale bytes as atoms [ceil(rows / 128),
+// ceil(K / 128), 512] (mx.cuh).
+enum MxLayout : int { kMxPlain = 0, kMxGroups = 1 };
 struct MxScales {
   uint8_t* data;
   int64_t rows, blocks;
@@ -304,7 +305,7 @@ inline int64_t mx_atoms_bytes(int64_t rows, int64_t K) {
 
 // s x A^T (out_rows [M, ld_rows] with columns past R zeroed, out_t [R, ld_t];
 // either may be null) and from the same read of x [M, K] its MXFP4 operand (q4
-// codes [M, K/2] and kMxAtoms scales; K % 32 == 0) and / or its MXINT8
+// codes [M, K/2] and scale atoms; K % 32 == 0) and / or its MXINT8
 // checkpoint (q8 codes ld8 bytes apart, 16-byte aligned rows; kMxGroups scales).
 struct MxPrepArgs {
   const void* x;

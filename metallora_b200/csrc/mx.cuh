@@ -18,7 +18,10 @@
 #include <stdint.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "ptx.cuh"
+#include "quant.cuh"
 
 namespace mlora {
 
@@ -90,6 +93,142 @@ __device__ __forceinline__ uint32_t mx_pack_int8(float a, float b, float c, floa
   const uint32_t ua = __float_as_uint(__fadd_rn(a, kMagic)), ub = __float_as_uint(__fadd_rn(b, kMagic));
   const uint32_t uc = __float_as_uint(__fadd_rn(c, kMagic)), ud = __float_as_uint(__fadd_rn(d, kMagic));
   return __byte_perm(__byte_perm(ua, ub, 0x0040u), __byte_perm(uc, ud, 0x0040u), 0x5410u);
+}
+
+// ------------------------------------------------------- a block of a thread --
+// 32 consecutive 16-bit values (16 words) or 16 codes held by one thread: packed
+// fp32 pairs, two or three instructions a value.
+
+// The bits of max|x| (as fp32) of the 32 16-bit values in w.
+template <typename T>
+__device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[16]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+  m = max(m & 0xFFFFu, m >> 16);
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    return m << 16;
+  else
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+}
+
+// The two values of a word as packed fp32.
+template <typename T>
+__device__ __forceinline__ uint64_t widen2(uint32_t w) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    return (static_cast<uint64_t>(w & 0xFFFF0000u) << 32) | (w << 16);
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return f2_pack(f.x, f.y);
+  }
+}
+
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// The 32 e2m1 codes of a block with this scale byte.
+template <typename T>
+__device__ __forceinline__ uint4 block_fp4(const uint32_t (&w)[16], uint32_t byte) {
+  const float inv = mx_inv_scale(byte);
+  const uint64_t ii = f2_pack(inv, inv);
+  uint32_t o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float v[8];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
+      const uint64_t p = f2_mul(widen2<T>(w[4 * i + h]), ii);
+      v[2 * h] = f2_lo(p);
+      v[2 * h + 1] = f2_hi(p);
+    }
+    o[i] = mx_pack_e2m1(v);
+  }
+  return byte == 255u ? make_uint4(0, 0, 0, 0) : make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// 32 int8 codes; inv64 = 64 / X.  The product is exact, so the fused add of
+// 1.5 * 2^23 is the one rounding; its low 16 bits are the code, clamped there.
+template <typename T>
+__device__ __forceinline__ void block_int8_scaled(const uint32_t (&w)[16], float inv64, uint4& lo,
+                                                  uint4& hi) {
+  const uint64_t ii = f2_pack(inv64, inv64);
+  const uint64_t mm = f2_pack(12582912.f, 12582912.f);
+  uint32_t o[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    uint32_t h[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const uint64_t p = f2_fma(widen2<T>(w[2 * i + j]), ii, mm);
+      const uint32_t s = __byte_perm(static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32), 0x5410u);
+      h[j] = __vmaxs2(__vmins2(s, 0x007F007Fu), 0xFF81FF81u);
+    }
+    o[i] = __byte_perm(h[0], h[1], 0x6420u);
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
+}
+
+// The 32 int8 codes of a block with this scale byte.
+template <typename T>
+__device__ __forceinline__ void block_int8(const uint32_t (&w)[16], uint32_t byte, uint4& lo,
+                                           uint4& hi) {
+  if (byte >= 6u) {
+    block_int8_scaled<T>(w, mx_inv_scale(byte) * 64.f, lo, hi);
+  } else {
+    // 64 / X is past fp32's range: X = 2^(byte - 127) is moved up by 2^8 together
+    // with the values (exact: they are below 2^-120)
+    uint32_t u[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const uint64_t v = f2_mul(widen2<T>(w[i]), f2_pack(256.f, 256.f));
+      u[i] = pack2<__nv_bfloat16>(f2_lo(v), f2_hi(v));
+    }
+    block_int8_scaled<__nv_bfloat16>(u, mx_inv_scale(byte + 8u) * 64.f, lo, hi);
+  }
+  if (byte == 255u) lo = hi = make_uint4(0, 0, 0, 0);  // 0 * inf made NaN of them
+}
+
+// Sixteen MXINT8 codes times X / 64, in T (rounded to nearest where fp16 is
+// subnormal, else exact).  The byte with
+// its sign bit flipped is u = code + 128; placed in the mantissa of
+// 2^(23+k) (2^k = X / 64) it makes 2^k (2^23 + u), and subtracting
+// 2^k (2^23 + 128) leaves code * 2^k exactly.
+template <typename T>
+__device__ __forceinline__ void expand16(const uint4& q, uint32_t byte, uint4& lo, uint4& hi) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t o[8];
+  if (byte <= 237u) {
+    const uint32_t magic = (byte + 17u) << 23;
+    const float c = __uint_as_float(magic | 0x80u);
+    const uint64_t cc = f2_pack(c, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = w[i] ^ 0x80808080u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t a = __byte_perm(u, magic, 0x7640u | (2 * h));
+        const uint32_t b = __byte_perm(u, magic, 0x7640u | (2 * h + 1));
+        const uint64_t v = f2_sub((static_cast<uint64_t>(b) << 32) | a, cc);
+        o[2 * i + h] = pack2<T>(f2_lo(v), f2_hi(v));
+      }
+    }
+  } else {  // exponents the mantissa form cannot hold, and the NaN byte
+    const float X = mx_scale(byte);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float a = static_cast<float>(static_cast<int8_t>(w[i] >> (16 * h))) * (1.f / 64.f);
+        const float b = static_cast<float>(static_cast<int8_t>(w[i] >> (16 * h + 8))) * (1.f / 64.f);
+        o[2 * i + h] = pack2<T>(__fmul_rn(a, X), __fmul_rn(b, X));
+      }
+  }
+  lo = make_uint4(o[0], o[1], o[2], o[3]);
+  hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
 // --------------------------------------------------- fp4 tensor-core product --

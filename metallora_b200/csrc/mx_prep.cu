@@ -18,7 +18,6 @@
 #include "cluster_reduce.cuh"
 #include "internal.h"
 #include "mx.cuh"
-#include "quant.cuh"
 #include "../../include/metallora_b200.h"
 
 namespace mlora {
@@ -59,77 +58,6 @@ struct PrepParams {
   int wide_rows;  // the row output starts on 32 bytes (its rows are 128 apart)
   uint32_t* status;
 };
-
-// The bits of max|x| (as fp32) of the 32 16-bit values in w.
-template <typename T>
-__device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[16]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-  m = max(m & 0xFFFFu, m >> 16);
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return m << 16;
-  else
-    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
-}
-
-// The two values of a word as packed fp32.
-template <typename T>
-__device__ __forceinline__ uint64_t widen2(uint32_t w) {
-  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    return (static_cast<uint64_t>(w & 0xFFFF0000u) << 32) | (w << 16);
-  } else {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-    return f2_pack(f.x, f.y);
-  }
-}
-
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
-// 32 e2m1 codes; inv = 1 / X.
-template <typename T>
-__device__ __forceinline__ uint4 block_fp4(const uint32_t (&w)[16], float inv) {
-  const uint64_t ii = f2_pack(inv, inv);
-  uint32_t o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float v[8];
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-      const uint64_t p = f2_mul(widen2<T>(w[4 * i + h]), ii);
-      v[2 * h] = f2_lo(p);
-      v[2 * h + 1] = f2_hi(p);
-    }
-    o[i] = mx_pack_e2m1(v);
-  }
-  return make_uint4(o[0], o[1], o[2], o[3]);
-}
-
-// 32 int8 codes; inv64 = 64 / X.  The product is exact, so the fused add of
-// 1.5 * 2^23 is the one rounding; its low 16 bits are the code, clamped there.
-template <typename T>
-__device__ __forceinline__ void block_int8(const uint32_t (&w)[16], float inv64, uint4& lo, uint4& hi) {
-  const uint64_t ii = f2_pack(inv64, inv64);
-  const uint64_t mm = f2_pack(12582912.f, 12582912.f);
-  uint32_t o[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t h[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint64_t p = f2_fma(widen2<T>(w[2 * i + j]), ii, mm);
-      const uint32_t s = __byte_perm(static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32), 0x5410u);
-      h[j] = __vmaxs2(__vmins2(s, 0x007F007Fu), 0xFF81FF81u);
-    }
-    o[i] = __byte_perm(h[0], h[1], 0x6420u);
-  }
-  lo = make_uint4(o[0], o[1], o[2], o[3]);
-  hi = make_uint4(o[4], o[5], o[6], o[7]);
-}
 
 // Grid (token tiles, splits), cluster (1, splits, 1).
 template <int R, bool kBF16>
@@ -236,8 +164,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
                                        ((row >> 7) * p.atoms_k + (kb >> 1)) * kMxAtomBytes +
                                        (r & 31) * 16 + (r >> 5) * 4 + (kb & 1) * 2) =
               static_cast<uint16_t>(byte | (other << 8));
-        uint4 c = block_fp4<T>(w, mx_inv_scale(byte));
-        if (byte == 255u) c = make_uint4(0, 0, 0, 0);
+        const uint4 c = block_fp4<T>(w, byte);
         if (in) *reinterpret_cast<uint4*>(p.q4 + row * (p.K >> 1) + (k >> 1)) = c;
       }
       if (p.q8 != nullptr) {
@@ -250,20 +177,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
           if (kb + 1 == p.num_kb && (kb & 1) == 0) dst[1] = 0;  // the word's blocks past K
         }
         uint4 lo, hi;
-        if (byte >= 6u) {
-          block_int8<T>(w, byte == 255u ? 0.f : mx_inv_scale(byte) * 64.f, lo, hi);
-        } else {
-          // 64 / X is past fp32's range: X = 2^(byte - 127) moved up by 2^8 together
-          // with the values (exact: they are below 2^-120)
-          uint32_t u[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t v = f2_mul(widen2<T>(w[i]), f2_pack(256.f, 256.f));
-            u[i] = pack2<__nv_bfloat16>(f2_lo(v), f2_hi(v));
-          }
-          block_int8<__nv_bfloat16>(u, mx_inv_scale(byte + 8u) * 64.f, lo, hi);
-        }
-        if (byte == 255u) lo = hi = make_uint4(0, 0, 0, 0);
+        block_int8<T>(w, byte, lo, hi);
         if (in) {
           uint8_t* dst = p.q8 + row * p.ld8 + k;
           if (k + 32 <= p.K) {

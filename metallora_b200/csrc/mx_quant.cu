@@ -1,10 +1,11 @@
 // Quantisers and dequantisers of the microscaled block formats (mx.cuh):
 // MXFP4 weights and GEMM operands, MXINT8 activation checkpoints.
 //
-// One warp owns up to 1024 consecutive features of one row, 8 a lane and step,
-// so four lanes share a block and the block maximum is two shuffles.  HBM-bound:
-// x is read once, codes and scales are written once.  The four steps' loads are
-// issued before the first is used.
+// HBM-bound: x is read once, codes and scales are written once (and the reverse).
+// Rows of whole blocks of 16-bit values: a thread owns blocks (64 bytes, moved as
+// 32-byte sectors), the maximum needs no exchange, and the codes come from packed
+// pairs.  Other rows (a tail block, odd strides, fp32): a warp owns up to 1024
+// features of a row, 8 a lane and step, so four lanes share a block.
 #include <string>
 
 #include "internal.h"
@@ -59,12 +60,104 @@ __device__ __forceinline__ void store_scales(const MxScales& sc, int64_t row, in
       for (int i = 0; i < 4; ++i)
         if (4 * g + i < sc.blocks) dst[i] = static_cast<uint8_t>(word >> (8 * i));
     }
-  } else if (sc.layout == kMxGroups) {
-    reinterpret_cast<uint32_t*>(sc.data)[g * sc.rows + row] = word;
   } else {
-    const int64_t groups = (sc.blocks + 3) >> 2;
-    uint8_t* atom = sc.data + ((row >> 7) * groups + g) * kMxAtomBytes;
-    *reinterpret_cast<uint32_t*>(atom + (row & 31) * 16 + ((row >> 5) & 3) * 4) = word;
+    reinterpret_cast<uint32_t*>(sc.data)[g * sc.rows + row] = word;
+  }
+}
+
+// Thread t of a CTA owns blocks t, t + 256 of the CTA's 512.
+constexpr int kOwn = 2;
+
+__device__ __forceinline__ uint8_t* scale_of(const MxScales& sc, uint32_t block, uint32_t per_row) {
+  if (sc.layout == kMxPlain) return sc.data + block;
+  const uint32_t row = block / per_row, b = block - row * per_row;
+  return sc.data + (static_cast<int64_t>(b >> 2) * sc.rows + row) * 4 + (b & 3u);
+}
+
+__device__ __forceinline__ void ld_global_32b(const void* p, uint32_t* v) {
+  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
+                 "=r"(v[6]), "=r"(v[7])
+               : "l"(p));
+}
+
+// x, codes: [blocks] of 32 values, without gaps between the rows.
+template <int kBits, typename T>
+__global__ void __launch_bounds__(kMxThreads)
+    mx_quantize_blocks_kernel(const T* __restrict__ x, uint32_t blocks, uint32_t per_row,
+                              uint8_t* __restrict__ codes, const MxScales sc) {
+  const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
+  uint32_t w[kOwn][16];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const uint32_t b = b0 + i * kMxThreads;
+    if (b >= blocks) continue;
+    ld_global_32b(x + static_cast<int64_t>(b) * 32, w[i]);
+    ld_global_32b(x + static_cast<int64_t>(b) * 32 + 16, w[i] + 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const uint32_t b = b0 + i * kMxThreads;
+    if (b >= blocks) continue;
+    const uint32_t amax = block_amax<T>(w[i]);
+    const uint32_t byte = kBits == 4 ? mx_scale_byte_fp4(amax) : mx_scale_byte_int8(amax);
+    *scale_of(sc, b, per_row) = static_cast<uint8_t>(byte);
+    if constexpr (kBits == 4) {
+      reinterpret_cast<uint4*>(codes)[b] = block_fp4<T>(w[i], byte);
+    } else {
+      uint4 lo, hi;
+      block_int8<T>(w[i], byte, lo, hi);
+      const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+      st_global_32b(codes + static_cast<int64_t>(b) * 32, v);
+    }
+  }
+}
+
+template <int kBits, typename O>
+__global__ void __launch_bounds__(kMxThreads)
+    mx_dequantize_blocks_kernel(const uint8_t* __restrict__ codes, const MxScales sc,
+                                uint32_t blocks, uint32_t per_row, O* __restrict__ out) {
+  const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
+  uint32_t c[kOwn][kBits], byte[kOwn];
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const uint32_t b = b0 + i * kMxThreads;
+    if (b >= blocks) continue;
+    byte[i] = __ldg(scale_of(sc, b, per_row));
+    if constexpr (kBits == 4) {
+      const uint4 q = __ldg(reinterpret_cast<const uint4*>(codes) + b);
+      c[i][0] = q.x, c[i][1] = q.y, c[i][2] = q.z, c[i][3] = q.w;
+    } else {
+      ld_global_32b(codes + static_cast<int64_t>(b) * 32, c[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const uint32_t b = b0 + i * kMxThreads;
+    if (b >= blocks) continue;
+    O* dst = out + static_cast<int64_t>(b) * 32;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[8];
+      if constexpr (kBits == 4) {
+        const float X = mx_scale(byte[i]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float u[8];
+          mx_unpack_e2m1(c[i][2 * h + j], u);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[4 * j + k] = pack2<O>(__fmul_rn(u[2 * k], X), __fmul_rn(u[2 * k + 1], X));
+        }
+      } else {
+        uint4 lo, hi;
+        expand16<O>(make_uint4(c[i][4 * h], c[i][4 * h + 1], c[i][4 * h + 2], c[i][4 * h + 3]),
+                    byte[i], lo, hi);
+        v[0] = lo.x, v[1] = lo.y, v[2] = lo.z, v[3] = lo.w;
+        v[4] = hi.x, v[5] = hi.y, v[6] = hi.z, v[7] = hi.w;
+      }
+      st_global_32b(dst + 16 * h, v);
+    }
   }
 }
 
@@ -271,10 +364,39 @@ void run_dequantize(int bits, bool vec, dim3 grid, const void* codes, int64_t ld
         : mx_dequantize_kernel<8, O, false><<<grid, kMxThreads, 0, s>>>(c, ld, sc, M, K, o);
 }
 
+// Whether rows of K 16-bit values at `wide` and codes `code_bytes` apart go block
+// by block: whole blocks without gaps, sectors aligned, 32-bit block numbers.  A
+// checkpoint's scale words hold four blocks, so its rows hold whole words.
+bool whole_blocks(const void* wide, int dtype, const void* codes, int64_t ld, int64_t code_bytes,
+                  const MxScales& sc, int64_t M, int64_t K) {
+  return dtype != MLORA_DTYPE_F32 && K % (sc.layout == kMxPlain ? 32 : 128) == 0 &&
+         ld == code_bytes && aligned(wide, 32) && aligned(codes, 32) &&
+         M * (K / kMxBlock) < (int64_t(1) << 31);
+}
+
 }  // namespace
 
 int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K, void* codes,
                        int64_t ld, const MxScales& sc, cudaStream_t s) {
+  if (whole_blocks(x, dtype, codes, ld, K * bits / 8, sc, M, K)) {
+    const auto blocks = static_cast<uint32_t>(M * (K / kMxBlock));
+    const auto per_row = static_cast<uint32_t>(K / kMxBlock);
+    const unsigned grid = (blocks + kMxThreads * kOwn - 1) / (kMxThreads * kOwn);
+    auto* c = static_cast<uint8_t*>(codes);
+    LaunchScope scope(kKindQuant, s);
+    if (dtype == MLORA_DTYPE_BF16) {
+      const auto* xt = static_cast<const __nv_bfloat16*>(x);
+      bits == 4
+          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc)
+          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc);
+    } else {
+      const auto* xt = static_cast<const __half*>(x);
+      bits == 4
+          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc)
+          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc);
+    }
+    return launched("mx quantize");
+  }
   dim3 grid;
   if (int rc = mx_grid(M, K, &grid)) return rc;
   // whole 8-feature groups, 16-byte loads, 4- (fp4) or 8-byte (int8) stores
@@ -292,6 +414,25 @@ int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K,
 
 int launch_mx_dequantize(int bits, const void* codes, int64_t ld, const MxScales& sc, int64_t M,
                          int64_t K, void* out, int out_dtype, cudaStream_t s) {
+  if (whole_blocks(out, out_dtype, codes, ld, K * bits / 8, sc, M, K)) {
+    const auto blocks = static_cast<uint32_t>(M * (K / kMxBlock));
+    const auto per_row = static_cast<uint32_t>(K / kMxBlock);
+    const unsigned grid = (blocks + kMxThreads * kOwn - 1) / (kMxThreads * kOwn);
+    const auto* c = static_cast<const uint8_t*>(codes);
+    LaunchScope scope(kKindQuant, s);
+    if (out_dtype == MLORA_DTYPE_BF16) {
+      auto* o = static_cast<__nv_bfloat16*>(out);
+      bits == 4
+          ? mx_dequantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o)
+          : mx_dequantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o);
+    } else {
+      auto* o = static_cast<__half*>(out);
+      bits == 4
+          ? mx_dequantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o)
+          : mx_dequantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o);
+    }
+    return launched("mx dequantize");
+  }
   dim3 grid;
   if (int rc = mx_grid(M, K, &grid)) return rc;
   const uintptr_t st = bits == 4 ? 4 : 8;

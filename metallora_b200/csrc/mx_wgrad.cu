@@ -18,7 +18,6 @@
 #include "cluster_reduce.cuh"
 #include "internal.h"
 #include "mx.cuh"
-#include "quant.cuh"
 #include "../../include/metallora_b200.h"
 
 namespace mlora {
@@ -55,44 +54,6 @@ struct MxWgradParams {
   float clip;
   uint32_t* status;
 };
-
-// Sixteen codes (one chunk of a token's row) times X / 64 in T.  The byte with
-// its sign bit flipped is u = code + 128; placed in the mantissa of
-// 2^(23+k) (2^k = X / 64) it makes 2^k (2^23 + u), and subtracting
-// 2^k (2^23 + 128) leaves code * 2^k exactly.
-template <typename T>
-__device__ __forceinline__ void expand16(const uint4& q, uint32_t byte, uint4& lo, uint4& hi) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  uint32_t o[8];
-  if (byte <= 237u) {
-    const uint32_t magic = (byte + 17u) << 23;
-    const float c = __uint_as_float(magic | 0x80u);
-    const uint64_t cc = f2_pack(c, c);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t u = w[i] ^ 0x80808080u;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t a = __byte_perm(u, magic, 0x7640u | (2 * h));
-        const uint32_t b = __byte_perm(u, magic, 0x7640u | (2 * h + 1));
-        const uint64_t v = f2_sub((static_cast<uint64_t>(b) << 32) | a, cc);
-        o[2 * i + h] = pack2<T>(f2_lo(v), f2_hi(v));
-      }
-    }
-  } else {  // exponents the mantissa form cannot hold, and the NaN byte
-    const float X = mx_scale(byte);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float a = static_cast<float>(static_cast<int8_t>(w[i] >> (16 * h))) * (1.f / 64.f);
-        const float b = static_cast<float>(static_cast<int8_t>(w[i] >> (16 * h + 8))) * (1.f / 64.f);
-        o[2 * i + h] = pack2<T>(__fmul_rn(a, X), __fmul_rn(b, X));
-      }
-  }
-  lo = make_uint4(o[0], o[1], o[2], o[3]);
-  hi = make_uint4(o[4], o[5], o[6], o[7]);
-}
 
 // 1-D grid, cluster (splits, 1, 1): CTA b works on feature tile b / splits over
 // token range b % splits (= its cluster rank).
