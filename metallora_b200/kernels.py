@@ -120,10 +120,10 @@ def lora_linear_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor, b: tor
     _check_2d("A", a, (r, K), dt)
     _check_2d("B", b, (N, r), dt)
     x2d, w0, a, b = (t.contiguous() for t in (x2d, w0, a, b))
-    y = torch.empty((M, N), dtype=dt, device=x2d.device)
+    y = x2d.new_empty((M, N))
     saved = None
     if save_xa and dt != torch.float32:
-        saved = torch.empty((rank_tile(r), (M + 7) // 8 * 8), dtype=dt, device=x2d.device)
+        saved = x2d.new_empty((rank_tile(r), (M + 7) // 8 * 8))
     if M == 0:  # no tokens: empty output, nothing to launch
         return y, saved
     lib = _lib.load()
@@ -210,7 +210,7 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
     if ckpt is None:
         x2d = x2d.contiguous()
     lib = _lib.load()
-    dx = torch.empty((M, K), dtype=dt, device=x2d.device) if need_dx else None
+    dx = dy2d.new_empty((M, K)) if need_dx else None
     flags = 0
     into = da_out is not None or db_out is not None
     if into:
@@ -223,11 +223,12 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
         da, db = da_out, db_out
         flags = _lib.BWD_ACCUMULATE if accumulate else 0
     else:
-        gdt = torch.float32
         if grad_dtype is not None and grad_dtype == dt and dt != torch.float32:
-            gdt, flags = dt, _lib.BWD_GRADS_16BIT
-        da = torch.empty((r, K), dtype=gdt, device=x2d.device)
-        db = torch.empty((N, r), dtype=gdt, device=x2d.device)
+            flags = _lib.BWD_GRADS_16BIT
+            da, db = dy2d.new_empty((r, K)), dy2d.new_empty((N, r))
+        else:
+            da = dy2d.new_empty((r, K), dtype=torch.float32)
+            db = dy2d.new_empty((N, r), dtype=torch.float32)
     if M == 0:  # no tokens: the sums over tokens are zero; nothing to launch
         if not (into and accumulate):
             da.zero_()
@@ -469,9 +470,8 @@ def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, al
     _check_2d("A", a, (r, K), dt)
     _check_2d("B", b, (N, r), dt)
     x2d, a, b = x2d.contiguous(), a.contiguous(), b.contiguous()
-    y = torch.empty((M, N), dtype=dt, device=x2d.device)
-    saved = (torch.empty((rank_tile(r), (M + 7) // 8 * 8), dtype=dt, device=x2d.device)
-             if save_xa else None)
+    y = x2d.new_empty((M, N))
+    saved = x2d.new_empty((rank_tile(r), (M + 7) // 8 * 8)) if save_xa else None
     if M == 0:  # no tokens: empty output, nothing to launch
         return y, saved
     lib = _lib.load()
@@ -512,7 +512,7 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
     else:
         _check_saved(saved_xa, r, M, dt)
     lib = _lib.load()
-    dx = torch.empty((M, K), dtype=dt, device=x2d.device) if need_dx else None
+    dx = dy2d.new_empty((M, K)) if need_dx else None
     flags = 0
     into = da_out is not None or db_out is not None
     if into:
@@ -521,11 +521,12 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
         da, db = da_out, db_out
         flags = _lib.BWD_ACCUMULATE if accumulate else 0
     else:
-        gdt = torch.float32
         if grad_dtype is not None and grad_dtype == dt:
-            gdt, flags = dt, _lib.BWD_GRADS_16BIT
-        da = torch.empty((r, K), dtype=gdt, device=x2d.device)
-        db = torch.empty((N, r), dtype=gdt, device=x2d.device)
+            flags = _lib.BWD_GRADS_16BIT
+            da, db = dy2d.new_empty((r, K)), dy2d.new_empty((N, r))
+        else:
+            da = dy2d.new_empty((r, K), dtype=torch.float32)
+            db = dy2d.new_empty((N, r), dtype=torch.float32)
     if M == 0:  # no tokens: the sums over tokens are zero; nothing to launch
         if not (into and accumulate):
             da.zero_()

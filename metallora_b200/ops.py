@@ -228,14 +228,17 @@ def lora_backward(grad_output, x, A, B, alpha: float = 16.0, clip_value: float =
     values, and dB from ``saved_xa``, the (alpha/rank) x.A^T that the forward
     kept (``kernels.lora_linear_fwd(..., save_xa=True)``), or without it from
     the checkpoint's values too."""
-    g = grad_output.reshape(-1, grad_output.shape[-1])
+    g = grad_output
+    if g.dim() != 2:
+        g = g.reshape(-1, g.shape[-1])
     if not torch.is_tensor(x):
         clip = float(clip_value) if clip_value is not None else 0.0
         if saved_xa is None:
             x = x.dequantize().reshape(-1, x.shape[-1])
         _, da, db = _k.lora_linear_bwd(g, x, None, A, B, alpha, saved_xa, clip, need_dx=False,
                                        grad_dtype=A.dtype if A.dtype == B.dtype else None)
-        return da.to(A.dtype), db.to(B.dtype)
+        return (da if da.dtype == A.dtype else da.to(A.dtype),
+                db if db.dtype == B.dtype else db.to(B.dtype))
     xx = x.reshape(-1, x.shape[-1])
     clip = float(clip_value) if clip_value is not None else 0.0
     _, da, db = _k.lora_linear_bwd(g, xx, None, A, B, alpha, saved_xa, clip, need_dx=False)

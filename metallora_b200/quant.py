@@ -195,20 +195,20 @@ class ActivationCheckpoint:
 
     def check(self) -> None:
         """Raises unless the tensors have the layout the kernels read."""
+        codes, scales = self.codes, self.scales
         M, K = self.rows, self.shape[-1]
-        if self.codes.dtype != torch.int8 or tuple(self.codes.shape) != (M, K):
+        if codes.dtype != torch.int8 or codes.shape != (M, K):
             raise ShapeError(f"checkpoint codes must be int8 {(M, K)}, got "
-                             f"{tuple(self.codes.shape)} {self.codes.dtype}")
+                             f"{tuple(codes.shape)} {codes.dtype}")
         want = (-(-K // 128), -(-M // 4) * 4, 4)
-        if self.scales.dtype != torch.uint8 or tuple(self.scales.shape) != want or \
-                not self.scales.is_contiguous():
+        if scales.dtype != torch.uint8 or scales.shape != want or not scales.is_contiguous():
             raise ShapeError(f"checkpoint scales must be contiguous uint8 {want}, got "
-                             f"{tuple(self.scales.shape)} {self.scales.dtype}")
-        if M and (self.codes.stride(1) != 1 or self.codes.stride(0) < K
-                  or self.codes.stride(0) % 16):
+                             f"{tuple(scales.shape)} {scales.dtype}")
+        ld, one = codes.stride()
+        if M and (one != 1 or ld < K or ld % 16):
             raise ShapeError("checkpoint code rows must be contiguous and a multiple of 16 bytes "
-                             f"apart, got strides {tuple(self.codes.stride())}")
-        if self.scales.device != self.codes.device:
+                             f"apart, got strides {(ld, one)}")
+        if scales.device != codes.device:
             raise DeviceError("checkpoint codes and scales are on different devices")
 
     def dequantize(self, dtype: torch.dtype | None = None) -> torch.Tensor:
@@ -216,7 +216,7 @@ class ActivationCheckpoint:
         self.check()
         _need_cuda(self.codes)
         _need_current(self.codes)
-        out = torch.empty(self.shape, dtype=dtype or self.dtype, device=self.device)
+        out = self.codes.new_empty(self.shape, dtype=dtype or self.dtype)
         if out.numel():
             st = _lib.load().mlora_act_restore(_ptr(self.codes), self.codes.stride(0),
                                                _ptr(self.scales), self.rows, self.shape[-1],
