@@ -195,6 +195,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     }
     __syncwarp();
   }
+  // the reduction below parks sums in the stages: every warp has read its tiles
+  if (warp >= 2) named_bar_sync(1, 32 * kQuantWarps);
   const bool epi = warp >= 2 && warp < 6;
   const int row_local = static_cast<int>((warp & 3u) * 32 + lane_id());
   const long long row = static_cast<long long>(tile) * 128 + row_local;

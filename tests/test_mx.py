@@ -267,6 +267,14 @@ def _fwd_inputs(M, K, N, r, dt, cuda, seed=0):
     return tuple(t.to(cuda) for t in (x, w, a, b))
 
 
+def _dirty(cuda):
+    """Leaves memory that the next buffers come from full of NaN bytes, so that a
+    kernel which reads what nothing wrote, or too early, shows."""
+    keep = [torch.full((n,), 255, dtype=torch.uint8, device=cuda)
+            for n in (1 << 12, 1 << 16, 1 << 20, 1 << 24)]
+    del keep
+
+
 def _fwd_check(y, x, qw, a, b, alpha):
     dt, h = x.dtype, _half_step(x.dtype)
     r, K = a.shape
@@ -289,7 +297,8 @@ SHAPES = [(1, 32, 8, 8), (1, 4096, 1024, 64), (2, 64, 24, 16), (16, 256, 128, 8)
           (17, 96, 1000, 16), (31, 160, 264, 8), (32, 512, 128, 32), (33, 544, 72, 16),
           (64, 1024, 384, 16), (65, 2080, 200, 128), (100, 128, 512, 256), (128, 320, 640, 16),
           (129, 256, 256, 16), (200, 4096, 264, 8), (256, 512, 256, 64), (257, 224, 520, 16),
-          (300, 1056, 1000, 24), (513, 768, 768, 16)]
+          (300, 1056, 1000, 24), (513, 768, 768, 16), (16, 4096, 256, 16), (5, 928, 280, 16),
+          (3, 3904, 136, 8), (30, 4224, 200, 64), (101, 5248, 136, 24), (59, 8160, 264, 32)]
 
 
 @pytest.mark.gpu
@@ -298,8 +307,10 @@ SHAPES = [(1, 32, 8, 8), (1, 4096, 1024, 64), (2, 64, 24, 16), (16, 256, 128, 8)
 def test_forward(cuda, dt, M, K, N, r):
     x, w, a, b = _fwd_inputs(M, K, N, r, dt, cuda)
     qw = quant.quantize(w, "mxfp4")
+    _dirty(cuda)
     y, saved = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True)
     _fwd_check(y, x, qw, a, b, 32.0)
+    _dirty(cuda)
     y2, none = kernels.qlora_linear_fwd(x, qw, a, b, 32.0)
     assert none is None and torch.equal(y, y2)  # bitwise repeatable
     with torch.no_grad():
@@ -409,9 +420,11 @@ GRAD_SHAPES = [(1, 8, 8, 8), (7, 40, 24, 16), (63, 128, 72, 8), (64, 64, 64, 16)
 @pytest.mark.parametrize("M,K,N,r", GRAD_SHAPES)
 def test_gradients_from_checkpoint(cuda, dt, M, K, N, r):
     x, w, a, b, dy, saved = _grad_inputs(M, K, N, r, dt, cuda)
+    _dirty(cuda)
     c = quant.checkpoint_activation(x)
     xh = _ckpt_values(c)
     for gdt in (None, dt):
+        _dirty(cuda)
         dx, da, db = kernels.lora_linear_bwd(dy, c, None, a, b, 32.0, saved, need_dx=False,
                                              grad_dtype=gdt)
         assert dx is None and da.dtype == db.dtype == (gdt or FP32)
@@ -514,14 +527,17 @@ def _step(x, qw, a, b, dy, checkpoint):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [BF16, FP16])
-@pytest.mark.parametrize("M,K,N,r", [(5, 64, 24, 8), (100, 288, 136, 20), (300, 512, 264, 64)])
+@pytest.mark.parametrize("M,K,N,r", [(5, 64, 24, 8), (100, 288, 136, 20), (300, 512, 264, 64),
+                                     (20, 4096, 72, 16)])
 def test_step(cuda, dt, M, K, N, r):
     """Forward and backward over an MXFP4 base with and without a checkpoint:
     the checkpoint changes dA alone; dx = dy.W + s (dy.B).A."""
     x, w, a, b = _fwd_inputs(M, K, N, r, dt, cuda)
     dy = (torch.randn(M, N, generator=_gen(4)) * 0.1).to(dt).to(cuda)
     qw = quant.quantize(w, "mxfp4")
+    _dirty(cuda)
     y, dx, da, db = _step(x, qw, a, b, dy, "mxint8")
+    _dirty(cuda)
     y0, dx0, da0, db0 = _step(x, qw, a, b, dy, None)
     shared = quant.checkpoint_activation(x)
     y1, dx1, da1, db1 = _step(x, qw, a, b, dy, shared)
@@ -542,6 +558,39 @@ def test_step(cuda, dt, M, K, N, r):
     w_err = 0.0 if dt == BF16 else np.abs(DY).sum(1, keepdims=True) * _tiny(dt)
     acc = u_err @ np.abs(A) + 1.01 * (N + r) * ACC * mag + w_err
     assert np.all(np.abs(_np(dx) - ref) <= acc + h * (np.abs(ref) + acc) + _tiny(dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("K", [8, 40, 200, 232, 1000, 1056, 4096])
+def test_forward_writes_the_checkpoint(cuda, dt, K):
+    """The checkpoint a forward makes is the one of ``checkpoint_activation``, at
+    every value the format has to round, saturate or refuse, word padding
+    included; the forward's own outputs are those without it."""
+    e = _edge_rows(dt)
+    x = torch.cat([e.repeat(1, -(-K // e.shape[1]))[:, :K],
+                   e.flip(1).repeat(1, -(-K // e.shape[1]))[:, :K], _acts(151, K, dt, 2)]).to(cuda)
+    g = _gen(1)
+    w = (torch.randn(72, K, generator=g) * 0.05).to(dt).to(cuda)
+    a = (torch.randn(16, K, generator=g) / K ** 0.5).to(dt).to(cuda)
+    b = (torch.randn(72, 16, generator=g) * 0.1).to(dt).to(cuda)
+    want = quant.checkpoint_activation(x)
+    runs = [lambda o: kernels.lora_linear_fwd(x, w, a, b, 32.0, save_xa=True, ckpt_out=o)]
+    if K % 32 == 0:
+        qw = quant.quantize(w, "mxfp4")
+        runs.append(lambda o: kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True, ckpt_out=o))
+    for run in runs:
+        _dirty(cuda)
+        got = quant.empty_checkpoint(x.shape, dt, cuda)
+        y, saved = run(got)
+        assert torch.equal(got.codes, want.codes)
+        assert torch.equal(got.scales[:, : x.shape[0]], want.scales[:, : x.shape[0]])
+        y0, saved0 = run(None)
+        same = ~(torch.isnan(y) & torch.isnan(y0))
+        assert torch.equal(y[same], y0[same])
+        M = x.shape[0]
+        same = ~(torch.isnan(saved[:, :M]) & torch.isnan(saved0[:, :M]))
+        assert torch.equal(saved[:, :M][same], saved0[:, :M][same])
 
 
 @pytest.mark.gpu
