@@ -149,11 +149,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         const uint4 q = *reinterpret_cast<const uint4*>(src + (((4 * b + i) ^ (r & 7)) << 4));
         w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
       }
-      __syncwarp();
-      if (lane_id() == 0) mbar_arrive(&empty_bar[stage]);
+      // The stage is free once its words are in registers, and they are once the
+      // whole warp's maximum is known: an arrive after the loads alone overtook
+      // them (a late load then read the tile copied next; seen in 1 of 8 runs of
+      // 4096 x 4096).  The maximum's bits are never all set.
+      const uint32_t amax = block_amax<T>(w);
+      if (__reduce_max_sync(0xffffffffu, amax) != 0xFFFFFFFFu && lane_id() == 0)
+        mbar_arrive(&empty_bar[stage]);
       if (++stage == S) stage = 0, phase ^= 1u;
 
-      const uint32_t amax = block_amax<T>(w);
       const long long k = static_cast<long long>(kb) * kBK + 32 * b;
       const bool in = live && k < p.K;
       if (p.q4 != nullptr) {
