@@ -13,6 +13,8 @@ product of two fp32 values, ~2^-16 relative error each).
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from . import _lib
@@ -58,6 +60,17 @@ def _dtype_code(t: torch.Tensor) -> int:
 
 def _workspace(nbytes: int, device) -> torch.Tensor:
     return torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=device)
+
+
+@functools.lru_cache(maxsize=256)
+def _mx_ws_bytes(M: int, K: int, N: int, r: int, backward: bool, need_w: bool) -> int:
+    """Workspace of a call over an MXFP4 base (a function of the sizes alone)."""
+    lib = _lib.load()
+    args = (M, K, N, r, _lib.QUANT_MXFP4, 32)
+    if not backward:
+        return lib.mlora_qlora_forward_workspace_bytes(*args)
+    return (lib.mlora_qlora_backward_workspace_bytes(*args) if need_w
+            else lib.mlora_qlora_lean_workspace_bytes(*args, 1))
 
 
 def is_metal_available() -> bool:
@@ -435,6 +448,8 @@ def grad_norm_clip(grad: torch.Tensor, max_norm: float, out: torch.Tensor | None
 def _qlora_ws_bytes(lib, qw, M, K, N, r, backward, need_w=True):
     """Staged workspace (a bf16 copy of deq(W), fastest) unless the weight asks
     for the lean fused-dequant kernel, or the call does not read the weight."""
+    if qw.scheme == "mxfp4":
+        return _mx_ws_bytes(M, K, N, r, backward, need_w)
     if getattr(qw, "lean", False) or not need_w:
         return lib.mlora_qlora_lean_workspace_bytes(M, K, N, r, qw.code, qw.group, int(backward))
     fn = (lib.mlora_qlora_backward_workspace_bytes if backward
@@ -475,10 +490,12 @@ def qlora_linear_fwd(x2d: torch.Tensor, qw, a: torch.Tensor, b: torch.Tensor, al
     if M == 0:  # no tokens: empty output, nothing to launch
         return y, saved
     lib = _lib.load()
-    ws = _workspace(_qlora_ws_bytes(lib, qw, M, K, N, r, backward=False), x2d.device)
-    head = (_ptr(x2d), qw.code, _ptr(qw.codes), _ptr(qw.scales), _ptr(qw.zeros),
-            _ptr(qw.prepared_scales()), qw.group, _ptr(a), _ptr(b), _ptr(y), _ptr(saved))
-    tail = (M, K, N, r, float(alpha), _dtype_code(x2d), _ptr(ws), ws.numel(), _stream())
+    ws = x2d.new_empty(_qlora_ws_bytes(lib, qw, M, K, N, r, backward=False), dtype=torch.uint8)
+    zeros = qw.zeros
+    head = (x2d.data_ptr(), qw.code, qw.codes.data_ptr(), qw.scales.data_ptr(),
+            None if zeros is None else zeros.data_ptr(), qw.prepared_scales().data_ptr(), qw.group,
+            a.data_ptr(), b.data_ptr(), y.data_ptr(), None if saved is None else saved.data_ptr())
+    tail = (M, K, N, r, float(alpha), _DT[dt], ws.data_ptr(), ws.numel(), _stream())
     if ckpt_out is not None:
         _check_ckpt_out(ckpt_out, x2d)
         st = lib.mlora_qlora_forward_ckpt(*head, *_ckpt_args(ckpt_out), *tail)
@@ -534,13 +551,13 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
         if into:
             return dx, da, db
         return dx, da[:r_orig].contiguous(), db[:, :r_orig].contiguous()
-    ws = _workspace(_qlora_ws_bytes(lib, qw, M, K, N, r, backward=True, need_w=need_dx),
-                    x2d.device)
-    tail = (qw.code, _ptr(qw.codes), _ptr(qw.scales), _ptr(qw.zeros),
+    ws = dy2d.new_empty(_qlora_ws_bytes(lib, qw, M, K, N, r, backward=True, need_w=need_dx),
+                        dtype=torch.uint8)
+    tail = (qw.code, qw.codes.data_ptr(), qw.scales.data_ptr(), _ptr(qw.zeros),
             _ptr(qw.prepared_scales()) if need_dx and qw.scheme != "mxfp4" else None, qw.group,
-            _ptr(a_p), _ptr(b_p), _ptr(saved_xa), _ptr(dx), _ptr(da), _ptr(db), M, K, N, r,
-            float(alpha_p), float(clip_value), _dtype_code(x2d), flags, _ptr(ws), ws.numel(),
-            _stream())
+            a_p.data_ptr(), b_p.data_ptr(), _ptr(saved_xa), _ptr(dx), da.data_ptr(),
+            db.data_ptr(), M, K, N, r, float(alpha_p), float(clip_value), _DT[dt], flags,
+            ws.data_ptr(), ws.numel(), _stream())
     if ckpt is not None:
         st = lib.mlora_qlora_backward_ckpt(_ptr(dy2d), *_ckpt_args(ckpt), *tail)
     else:

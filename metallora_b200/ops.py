@@ -34,7 +34,7 @@ def _checkpoint(x2d, checkpoint):
         raise ConfigurationError(f"unknown activation checkpoint {checkpoint!r}; use 'mxint8' or "
                                  "an ActivationCheckpoint")
     _k._need_cuda(x2d)
-    return empty_checkpoint(x2d.shape, x2d.dtype, x2d.device), True
+    return empty_checkpoint(x2d), True
 
 
 def _keep_x(ctx, x2d, ckpt) -> tuple:

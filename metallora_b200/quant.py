@@ -225,19 +225,19 @@ class ActivationCheckpoint:
         return out
 
 
-def empty_checkpoint(shape, dtype: torch.dtype, device) -> ActivationCheckpoint:
-    """An uninitialised checkpoint of activations of this shape: the buffers a
+def empty_checkpoint(like: torch.Tensor) -> ActivationCheckpoint:
+    """An uninitialised checkpoint of activations like these: the buffers a
     forward fills (``kernels.lora_linear_fwd(..., ckpt_out=)``)."""
-    shape = tuple(shape)
+    shape = tuple(like.shape)
     if not shape or shape[-1] == 0:
         raise ShapeError("a checkpoint is of activations with at least one feature")
     K, M = shape[-1], 1
     for d in shape[:-1]:
         M *= d
     ld = -(-K // 16) * 16
-    codes = torch.empty((M, ld), dtype=torch.int8, device=device)
-    scales = torch.empty((-(-K // 128), -(-M // 4) * 4, 4), dtype=torch.uint8, device=device)
-    return ActivationCheckpoint(codes if ld == K else codes[:, :K], scales, shape, dtype)
+    codes = like.new_empty((M, ld), dtype=torch.int8)
+    scales = like.new_empty((-(-K // 128), -(-M // 4) * 4, 4), dtype=torch.uint8)
+    return ActivationCheckpoint(codes if ld == K else codes[:, :K], scales, shape, like.dtype)
 
 
 def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
@@ -247,7 +247,7 @@ def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
     _need_cuda(x)
     _need_current(x)
     code = _dtype_code(x)
-    c = empty_checkpoint(x.shape, x.dtype, x.device)
+    c = empty_checkpoint(x)
     if x.numel():
         x = x.detach().contiguous()
         st = _lib.load().mlora_act_checkpoint(x.data_ptr(), code, c.codes.shape[0], x.shape[-1],

@@ -340,7 +340,7 @@ def test_many_runs_agree(cuda, M, K, N, r):
     bad = torch.zeros(6, device=cuda)
     first = None
     for _ in range(100):
-        c = quant.empty_checkpoint(x.shape, BF16, cuda)
+        c = quant.empty_checkpoint(x)
         y, saved = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True, ckpt_out=c)
         _, da, db = kernels.lora_linear_bwd(dy, c, None, a, b, 32.0, saved, need_dx=False)
         got = (y, saved[:, :M], da, db)
@@ -606,7 +606,7 @@ def test_forward_writes_the_checkpoint(cuda, dt, K):
         runs.append(lambda o: kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True, ckpt_out=o))
     for run in runs:
         _dirty(cuda)
-        got = quant.empty_checkpoint(x.shape, dt, cuda)
+        got = quant.empty_checkpoint(x)
         y, saved = run(got)
         assert torch.equal(got.codes, want.codes)
         assert torch.equal(got.scales[:, : x.shape[0]], want.scales[:, : x.shape[0]])
