@@ -134,14 +134,26 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       umma_commit(done_bar);
     }
   } else if (has_work) {
-    // lanes 2i, 2i+1: the two blocks of one row's 64 features
-    const int ct = static_cast<int>(threadIdx.x) - 64;
-    const int r = ct >> 1, b = ct & 1;
+    // Lanes 2i, 2i+1: the two blocks of one row's 64 features, 16 rows a warp.  A
+    // tile of few tokens leaves warps without rows: they take every second, fourth
+    // or eighth k-block instead (one token, K 4096: the pass 5.0 -> 3.9 us).
+    const int qw = static_cast<int>(warp) - 2;
+    const long long rows = p.M - static_cast<long long>(tile) * 128;
+    const int row_warps = rows > 64 ? 8 : (rows > 32 ? 4 : (rows > 16 ? 2 : 1));
+    const int turns = kQuantWarps / row_warps, turn = qw / row_warps;
+    const int r = (qw % row_warps) * 16 + static_cast<int>(lane_id() >> 1);
+    const int b = static_cast<int>(lane_id() & 1u);
     const long long row = static_cast<long long>(tile) * 128 + r;
     const bool live = row < p.M;
     uint32_t stage = 0, phase = 0;
     for (int kb = kb_begin; kb < kb_end; ++kb) {
       if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) break;
+      if ((kb - kb_begin) % turns != turn) {  // another warp's block
+        __syncwarp();
+        if (lane_id() == 0) mbar_arrive(&empty_bar[stage]);
+        if (++stage == S) stage = 0, phase ^= 1u;
+        continue;
+      }
       uint32_t w[16];
       const uint8_t* src = smem + stage * stage_bytes(R) + r * 128;
 #pragma unroll
