@@ -161,4 +161,102 @@ __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float*
   }
 }
 
+// The same reduction by pushing: each CTA stores its partial columns into the
+// receive buffer of the CTA that sums them, one cluster barrier later every CTA
+// sums what it received from its own shared memory, and nothing has to outlive
+// that.  Against pulling (cluster_reduce) this saves a barrier and the round
+// trips of the loads; it needs `recv` to itself (push_bytes(R)) and the barrier
+// arrival of push_begin() at the kernel's start, which tells that a peer's
+// shared memory may be written.  Same order of the sums, same bits.
+__host__ __device__ constexpr uint32_t push_bytes(int R) { return reduce_cols(R) * 512u; }
+
+// All threads of the CTA, once, before any work.
+__device__ __forceinline__ void push_begin() {
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+
+__device__ __forceinline__ void st_shared_cluster_f32(uint32_t cluster_addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_addr), "f"(v) : "memory");
+}
+
+// Sends column j of this thread's row to the CTA that owns it: slot [source]
+// [column of the slice][row] there.
+template <int CP, int S>
+__device__ __forceinline__ void push_columns(const float (&acc)[CP], float* recv, uint32_t crank,
+                                             uint32_t first, int row_local) {
+  constexpr int W = CP / S;
+  const uint32_t at = smem_u32(recv) + (crank * W * 128u + static_cast<uint32_t>(row_local)) * 4u;
+#pragma unroll
+  for (int c = 0; c < S; ++c) {
+    const uint32_t dst = mapa_shared(at, first + static_cast<uint32_t>(c));
+#pragma unroll
+    for (int i = 0; i < W; ++i) st_shared_cluster_f32(dst + i * 512u, acc[c * W + i]);
+  }
+}
+
+template <int CP, int S, typename Emit>
+__device__ __forceinline__ void sum_received(const float* recv, int crank, int row_local, int j_base,
+                                             Emit&& emit) {
+  constexpr int W = CP / S;
+  constexpr int B = W < 16 ? W : 16;
+#pragma unroll 1
+  for (int jj = 0; jj < W; jj += B) {
+    float v[B];
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int s = 0; s < S; ++s) v[i] += recv[(s * W + jj + i) * 128 + row_local];
+    }
+    emit_columns(emit, j_base + crank * W + jj, v);
+  }
+}
+
+template <int R, typename Emit>
+__device__ __forceinline__ void cluster_push_reduce(uint32_t taddr, bool have, float* recv, int S,
+                                                    uint32_t crank, int row_local, bool epi,
+                                                    Emit&& emit, uint32_t first = 0) {
+  constexpr int CP = reduce_cols(R);
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");  // push_begin of all CTAs
+#pragma unroll 1
+  for (int pass = 0; pass < R / CP; ++pass) {
+    if (pass > 0) cluster_sync();  // the slots have been summed
+    if (epi) {
+      float acc[CP];
+      if (have) {
+        load_acc_row<CP>(taddr + pass * CP, acc);
+      } else {
+#pragma unroll
+        for (int j = 0; j < CP; ++j) acc[j] = 0.f;
+      }
+      if (S == 1) {
+#pragma unroll
+        for (int j = 0; j < CP; j += 16) {
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0.f + acc[j + i];
+          emit_columns(emit, pass * CP + j, v);
+        }
+      } else if (S == 2) {
+        push_columns<CP, 2>(acc, recv, crank, first, row_local);
+      } else if (S == 4) {
+        push_columns<CP, 4>(acc, recv, crank, first, row_local);
+      } else {
+        push_columns<CP, 8>(acc, recv, crank, first, row_local);
+      }
+    }
+    if (S == 1) continue;
+    cluster_sync();
+    if (epi) {
+      const int c = static_cast<int>(crank);
+      if (S == 2)
+        sum_received<CP, 2>(recv, c, row_local, pass * CP, emit);
+      else if (S == 4)
+        sum_received<CP, 4>(recv, c, row_local, pass * CP, emit);
+      else
+        sum_received<CP, 8>(recv, c, row_local, pass * CP, emit);
+    }
+  }
+}
+
 }  // namespace mlora

@@ -11,7 +11,7 @@
 //
 // A CTA owns one 128-row tile of U or of dB and one range of its reduction; the
 // ranges of a tile lie in one cluster, and their partial tiles meet through
-// distributed shared memory in fixed order (cluster_reduce).  The two products
+// distributed shared memory in fixed order (cluster_push_reduce).  The two products
 // are split apart from each other, so that all CTAs have about the same number
 // of k-blocks.  Warp 0 copies, warp 1 issues the UMMAs, warps 2-5 store.
 #include <atomic>
@@ -35,10 +35,13 @@ constexpr int kMaxSplits = 8;
 __host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
 __host__ __device__ constexpr uint32_t stage_bytes(int R) { return kDyBytes + R * 128u; }
 __host__ __device__ constexpr int num_stages(int R) {
-  const int n = static_cast<int>((ctas_per_sm(R) == 2 ? 108u : 200u) * 1024u / stage_bytes(R));
+  const uint32_t room = (ctas_per_sm(R) == 2 ? 110u : 220u) * 1024u - push_bytes(R);
+  const int n = static_cast<int>(room / stage_bytes(R));
   return n > 8 ? 8 : n;
 }
-constexpr size_t smem_bytes(int R) { return 1024 + num_stages(R) * stage_bytes(R) + 256; }
+constexpr size_t smem_bytes(int R) {
+  return 1024 + num_stages(R) * stage_bytes(R) + push_bytes(R) + 256;
+}
 __host__ __device__ constexpr uint32_t tmem_cols(int R) {
   return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
 }
@@ -83,12 +86,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   constexpr int S = num_stages(R);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R));
+  float* recv = reinterpret_cast<float*>(smem + S * stage_bytes(R));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R) + push_bytes(R));
   uint64_t* empty_bar = full_bar + S;
   uint64_t* done_bar = empty_bar + S;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
 
   const uint32_t warp = warp_id();
+  push_begin();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
     mbar_init(done_bar, 1);
@@ -219,8 +224,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       store_columns<float>(reinterpret_cast<float*>(p.db) + at, v, p.wide != 0);
     }
   };
-  cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
-                    reinterpret_cast<float*>(smem), splits, crank, row_local, epi, emit, first);
+  cluster_push_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have, recv, splits,
+                         crank, row_local, epi, emit, first);
   if (live && !is_db && crank == 0 && p.u_rows != nullptr) {  // zero columns past R
     T* dst = reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows;
     for (long long j = R; j < p.ld_rows; j += 8)

@@ -32,7 +32,7 @@ constexpr uint32_t kSfBytes = 2 * kMxAtomBytes;  // scales of 128 rows x 256 fea
 // the tokens its N side, so one pass over the weight serves all tokens.
 // Bound by the weight's HBM traffic; the reduction is split over the CTAs of a
 // cluster so that about two CTAs per SM stream it, and their partial tiles are
-// summed through distributed shared memory in fixed order (cluster_reduce).
+// summed through distributed shared memory in fixed order (cluster_push_reduce).
 constexpr int kSkinnyThreads = 192;
 constexpr int kSkinnyMaxSplits = 8;
 
@@ -40,10 +40,11 @@ __host__ __device__ constexpr uint32_t skinny_stage_bytes(int NT) {
   return (128 + NT) * kRowBytes + 2 * kSfBytes;
 }
 __host__ __device__ constexpr int skinny_stages(int NT) {
-  return static_cast<int>((NT <= 32 ? 100u : 200u) * 1024u / skinny_stage_bytes(NT));
+  return static_cast<int>(((NT <= 32 ? 110u : 220u) * 1024u - push_bytes(NT)) /
+                          skinny_stage_bytes(NT));
 }
 constexpr size_t skinny_smem(int NT) {
-  return 1024 + skinny_stages(NT) * skinny_stage_bytes(NT) + 256;
+  return 1024 + skinny_stages(NT) * skinny_stage_bytes(NT) + push_bytes(NT) + 256;
 }
 // accumulator columns, then two sets of (8 weight, 8 token) scale columns
 __host__ __device__ constexpr uint32_t skinny_acc_cols(int NT) { return NT; }
@@ -76,12 +77,14 @@ __global__ void __launch_bounds__(kSkinnyThreads)
   constexpr uint32_t kXsOff = kWsOff + kSfBytes;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * kStage);
+  float* recv = reinterpret_cast<float*>(smem + S * kStage);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * kStage + push_bytes(NT));
   uint64_t* empty_bar = full_bar + S;
   uint64_t* done_bar = empty_bar + S;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
 
   const uint32_t warp = warp_id();
+  push_begin();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
     mbar_init(done_bar, 1);
@@ -203,8 +206,8 @@ __global__ void __launch_bounds__(kSkinnyThreads)
     if (j < p.M) out[j * p.ldd] = static_cast<T>(v0);
     if (j + 1 < p.M) out[(j + 1) * p.ldd] = static_cast<T>(v1);
   };
-  cluster_reduce<NT>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
-                     reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+  cluster_push_reduce<NT>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have, recv,
+                          p.splits, crank, row_local, epi, emit);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {

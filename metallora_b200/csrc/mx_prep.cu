@@ -7,7 +7,7 @@
 // read once, where separate kernels read it once each.
 //
 // CTA = 128 tokens x one range of features; the ranges of a token tile are one
-// cluster (cluster_reduce).  Warp 0 copies [128 x 64] tiles of x and [R x 64]
+// cluster (cluster_push_reduce).  Warp 0 copies [128 x 64] tiles of x and [R x 64]
 // tiles of A (TMA ring), warp 1 issues the UMMAs, warps 2-9 quantise: a thread
 // owns one block of 32 features, so the block maximum needs no exchange.  A
 // stage is free when the UMMAs and all eight warps are done with it.
@@ -32,10 +32,13 @@ constexpr int kMaxSplits = 8;
 __host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
 __host__ __device__ constexpr uint32_t stage_bytes(int R) { return kXBytes + R * 128u; }
 __host__ __device__ constexpr int num_stages(int R) {
-  const int n = static_cast<int>((ctas_per_sm(R) == 2 ? 108u : 200u) * 1024u / stage_bytes(R));
+  const uint32_t room = (ctas_per_sm(R) == 2 ? 110u : 220u) * 1024u - push_bytes(R);
+  const int n = static_cast<int>(room / stage_bytes(R));
   return n > 8 ? 8 : n;
 }
-constexpr size_t smem_bytes(int R) { return 1024 + num_stages(R) * stage_bytes(R) + 256; }
+constexpr size_t smem_bytes(int R) {
+  return 1024 + num_stages(R) * stage_bytes(R) + push_bytes(R) + 256;
+}
 __host__ __device__ constexpr uint32_t tmem_cols(int R) {
   return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
 }
@@ -68,12 +71,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   constexpr int S = num_stages(R);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R));
+  float* recv = reinterpret_cast<float*>(smem + S * stage_bytes(R));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R) + push_bytes(R));
   uint64_t* empty_bar = full_bar + S;
   uint64_t* done_bar = empty_bar + S;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
 
   const uint32_t warp = warp_id();
+  push_begin();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1 + kQuantWarps);
     mbar_init(done_bar, 1);
@@ -211,8 +216,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     }
     __syncwarp();
   }
-  // the reduction below parks sums in the stages: every warp has read its tiles
-  if (warp >= 2) named_bar_sync(1, 32 * kQuantWarps);
   const bool epi = warp >= 2 && warp < 6;
   const int row_local = static_cast<int>((warp & 3u) * 32 + lane_id());
   const long long row = static_cast<long long>(tile) * 128 + row_local;
@@ -236,8 +239,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       for (int i = 0; i < C; ++i) dst[i * p.ld_t] = static_cast<T>(v[i]);
     }
   };
-  cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
-                    reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+  cluster_push_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have, recv,
+                         p.splits, crank, row_local, epi, emit);
   if (live && crank == 0 && p.out_rows != nullptr) {  // zero columns past R
     T* dst = reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows;
     for (long long j = R; j < p.ld_rows; j += 8)

@@ -9,7 +9,7 @@
 //
 // CTA = 128 features x one range of tokens; the ranges of a tile are one
 // cluster whose partial sums meet through distributed shared memory in fixed
-// order (cluster_reduce).  Warp 0 copies 64-token blocks of codes, scale words
+// order (cluster_reduce.cuh).  Warp 0 copies 64-token blocks of codes, scale words
 // and U^T (TMA ring), warps 2-9 expand the codes into the swizzled MN-major
 // operand, warp 1 issues the UMMAs, warps 2-5 store the tile.
 #include <string>
@@ -33,14 +33,19 @@ constexpr uint32_t kHalfBytes = kOpBytes / 2;
 constexpr int kOps = 2;                              // expanded operands in flight
 constexpr int kMaxSplits = 8;
 
+// Pushed sums where their buffer leaves room for the ring; from rank 64 on it
+// would take half of it, and the sums are pulled from the stages instead.
+__host__ __device__ constexpr bool pushed(int R) { return R <= 32; }
+__host__ __device__ constexpr uint32_t recv_bytes(int R) { return pushed(R) ? push_bytes(R) : 0u; }
 __host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
 __host__ __device__ constexpr uint32_t stage_bytes(int R) { return R * 128u + kCodeBytes + 1024u; }
 __host__ __device__ constexpr int num_stages(int R) {
-  const uint32_t room = (ctas_per_sm(R) == 2 ? 108u : 200u) * 1024u - kOps * kOpBytes;
+  const uint32_t room =
+      (ctas_per_sm(R) == 2 ? 110u : 220u) * 1024u - kOps * kOpBytes - recv_bytes(R);
   return static_cast<int>(room / stage_bytes(R)) > 8 ? 8 : static_cast<int>(room / stage_bytes(R));
 }
 constexpr size_t smem_bytes(int R) {
-  return 1024 + kOps * kOpBytes + num_stages(R) * stage_bytes(R) + 256;
+  return 1024 + kOps * kOpBytes + num_stages(R) * stage_bytes(R) + recv_bytes(R) + 256;
 }
 __host__ __device__ constexpr uint32_t tmem_cols(int R) {
   return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
@@ -67,7 +72,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
   uint8_t* stages = smem + kOps * kOpBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stages + S * stage_bytes(R));
+  float* recv = reinterpret_cast<float*>(stages + S * stage_bytes(R));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(stages + S * stage_bytes(R) + recv_bytes(R));
   uint64_t* empty_bar = full_bar + S;
   uint64_t* op_full = empty_bar + S;      // [kOps]
   uint64_t* op_empty = op_full + kOps;    // [kOps]
@@ -77,6 +83,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   constexpr uint32_t kScaleOff = kCodeOff + kCodeBytes;
 
   const uint32_t warp = warp_id();
+  if constexpr (pushed(R)) push_begin();
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) mbar_init(&full_bar[s], 1), mbar_init(&empty_bar[s], 1);
     for (int b = 0; b < kOps; ++b) mbar_init(&op_full[b], kConvWarps), mbar_init(&op_empty[b], 1);
@@ -219,8 +226,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       }
     }
   };
-  cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
-                    reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
+  const uint32_t taddr = tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16);
+  if constexpr (pushed(R))
+    cluster_push_reduce<R>(taddr, have, recv, p.splits, crank, row_local, epi, emit);
+  else
+    cluster_reduce<R>(taddr, have, reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi,
+                      emit);
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
