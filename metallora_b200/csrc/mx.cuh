@@ -99,17 +99,23 @@ __device__ __forceinline__ uint32_t mx_pack_int8(float a, float b, float c, floa
 // 32 consecutive 16-bit values (16 words) or 16 codes held by one thread: packed
 // fp32 pairs, two or three instructions a value.
 
-// The bits of max|x| (as fp32) of the 32 16-bit values in w.
+// The bits of max|x| (as fp32) of the 32 16-bit values in w; a NaN among them
+// gives a NaN.  Four running maxima keep the chain short.
 template <typename T>
 __device__ __forceinline__ uint32_t block_amax(const uint32_t (&w)[16]) {
-  uint32_t m = 0;
+  using T2 = typename std::conditional<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162,
+                                       __half2>::type;
+  T2 m[4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-  m = max(m & 0xFFFFu, m >> 16);
-  if constexpr (std::is_same<T, __nv_bfloat16>::value)
-    return m << 16;
-  else
-    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m))));
+  for (int i = 0; i < 4; ++i) m[i] = __habs2(*reinterpret_cast<const T2*>(&w[i]));
+#pragma unroll
+  for (int i = 4; i < 16; ++i)
+    m[i & 3] = __hmax2_nan(m[i & 3], __habs2(*reinterpret_cast<const T2*>(&w[i])));
+  m[0] = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
+  const float2 f = std::is_same<T, __nv_bfloat16>::value
+                       ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&m[0]))
+                       : __half22float2(*reinterpret_cast<const __half2*>(&m[0]));
+  return max(__float_as_uint(f.x), __float_as_uint(f.y)) & 0x7FFFFFFFu;
 }
 
 // The two values of a word as packed fp32.
@@ -150,34 +156,37 @@ __device__ __forceinline__ uint4 block_fp4(const uint32_t (&w)[16], uint32_t byt
 }
 
 // 32 int8 codes; inv64 = 64 / X.  The product is exact, so the fused add of
-// 1.5 * 2^23 is the one rounding; its low 16 bits are the code, clamped there.
+// 1.5 * 2^23 is the one rounding; its low 16 bits are the code.  Only a block
+// whose maximum is at least 127.5 / 64 X (`high`) can reach 128 and is clamped.
 template <typename T>
-__device__ __forceinline__ void block_int8_scaled(const uint32_t (&w)[16], float inv64, uint4& lo,
-                                                  uint4& hi) {
+__device__ __forceinline__ void block_int8_scaled(const uint32_t (&w)[16], float inv64, bool high,
+                                                  uint4& lo, uint4& hi) {
   const uint64_t ii = f2_pack(inv64, inv64);
   const uint64_t mm = f2_pack(12582912.f, 12582912.f);
-  uint32_t o[8];
+  uint32_t h[16], o[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t h[2];
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint64_t p = f2_fma(widen2<T>(w[2 * i + j]), ii, mm);
-      const uint32_t s = __byte_perm(static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32), 0x5410u);
-      h[j] = __vmaxs2(__vmins2(s, 0x007F007Fu), 0xFF81FF81u);
-    }
-    o[i] = __byte_perm(h[0], h[1], 0x6420u);
+  for (int i = 0; i < 16; ++i) {
+    const uint64_t p = f2_fma(widen2<T>(w[i]), ii, mm);
+    h[i] = __byte_perm(static_cast<uint32_t>(p), static_cast<uint32_t>(p >> 32), 0x5410u);
   }
+  if (high) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) h[i] = __vmaxs2(__vmins2(h[i], 0x007F007Fu), 0xFF81FF81u);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i] = __byte_perm(h[2 * i], h[2 * i + 1], 0x6420u);
   lo = make_uint4(o[0], o[1], o[2], o[3]);
   hi = make_uint4(o[4], o[5], o[6], o[7]);
 }
 
-// The 32 int8 codes of a block with this scale byte.
+// The 32 int8 codes of a block with this maximum.
 template <typename T>
-__device__ __forceinline__ void block_int8(const uint32_t (&w)[16], uint32_t byte, uint4& lo,
+__device__ __forceinline__ void block_int8(const uint32_t (&w)[16], uint32_t amax_bits, uint4& lo,
                                            uint4& hi) {
+  const uint32_t byte = mx_scale_byte_int8(amax_bits);
+  const bool high = (amax_bits & 0x7FFFFFu) >= 0x7F0000u;  // (subnormals are below it as values)
   if (byte >= 6u) {
-    block_int8_scaled<T>(w, mx_inv_scale(byte) * 64.f, lo, hi);
+    block_int8_scaled<T>(w, mx_inv_scale(byte) * 64.f, high, lo, hi);
   } else {
     // 64 / X is past fp32's range: X = 2^(byte - 127) is moved up by 2^8 together
     // with the values (exact: they are below 2^-120)
@@ -187,7 +196,7 @@ __device__ __forceinline__ void block_int8(const uint32_t (&w)[16], uint32_t byt
       const uint64_t v = f2_mul(widen2<T>(w[i]), f2_pack(256.f, 256.f));
       u[i] = pack2<__nv_bfloat16>(f2_lo(v), f2_hi(v));
     }
-    block_int8_scaled<__nv_bfloat16>(u, mx_inv_scale(byte + 8u) * 64.f, lo, hi);
+    block_int8_scaled<__nv_bfloat16>(u, mx_inv_scale(byte + 8u) * 64.f, true, lo, hi);
   }
   if (byte == 255u) lo = hi = make_uint4(0, 0, 0, 0);  // 0 * inf made NaN of them
 }

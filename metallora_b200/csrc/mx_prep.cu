@@ -150,10 +150,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     const int b = static_cast<int>(lane_id() & 1u);
     const long long row = static_cast<long long>(tile) * 128 + r;
     const bool live = row < p.M;
+    uint8_t* const q4_row = p.q4 + row * (p.K >> 1);
+    uint8_t* const q4_atom = p.q4_atoms + (row >> 7) * p.atoms_k * kMxAtomBytes + (r & 31) * 16 +
+                             (r >> 5) * 4;
+    uint8_t* const q8_row = p.q8 + row * p.ld8;
+    uint8_t* const q8_word = p.q8_scales + row * 4;
     uint32_t stage = 0, phase = 0;
     for (int kb = kb_begin; kb < kb_end; ++kb) {
       if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) break;
-      if ((kb - kb_begin) % turns != turn) {  // another warp's block
+      if (((kb - kb_begin) & (turns - 1)) != turn) {  // another warp's block
         __syncwarp();
         if (lane_id() == 0) mbar_arrive(&empty_bar[stage]);
         if (++stage == S) stage = 0, phase ^= 1u;
@@ -175,32 +180,29 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         mbar_arrive(&empty_bar[stage]);
       if (++stage == S) stage = 0, phase ^= 1u;
 
-      const long long k = static_cast<long long>(kb) * kBK + 32 * b;
+      const int k = kb * kBK + 32 * b;
       const bool in = live && k < p.K;
       if (p.q4 != nullptr) {
         const uint32_t byte = mx_scale_byte_fp4(amax);
         const uint32_t other = __shfl_xor_sync(0xffffffffu, byte, 1);
         if (live && b == 0)
-          *reinterpret_cast<uint16_t*>(p.q4_atoms +
-                                       ((row >> 7) * p.atoms_k + (kb >> 1)) * kMxAtomBytes +
-                                       (r & 31) * 16 + (r >> 5) * 4 + (kb & 1) * 2) =
+          *reinterpret_cast<uint16_t*>(q4_atom + (kb >> 1) * kMxAtomBytes + (kb & 1) * 2) =
               static_cast<uint16_t>(byte | (other << 8));
         const uint4 c = block_fp4<T>(w, byte);
-        if (in) *reinterpret_cast<uint4*>(p.q4 + row * (p.K >> 1) + (k >> 1)) = c;
+        if (in) *reinterpret_cast<uint4*>(q4_row + (k >> 1)) = c;
       }
       if (p.q8 != nullptr) {
         const uint32_t byte = mx_scale_byte_int8(amax);
         const uint32_t other = __shfl_xor_sync(0xffffffffu, byte, 1);
         if (live && b == 0) {
-          uint16_t* dst = reinterpret_cast<uint16_t*>(p.q8_scales + ((kb >> 1) * p.rows8 + row) * 4) +
-                          (kb & 1);
+          uint16_t* dst = reinterpret_cast<uint16_t*>(q8_word + (kb >> 1) * p.rows8 * 4) + (kb & 1);
           *dst = static_cast<uint16_t>(byte | (other << 8));
           if (kb + 1 == p.num_kb && (kb & 1) == 0) dst[1] = 0;  // the word's blocks past K
         }
         uint4 lo, hi;
-        block_int8<T>(w, byte, lo, hi);
+        block_int8<T>(w, amax, lo, hi);
         if (in) {
-          uint8_t* dst = p.q8 + row * p.ld8 + k;
+          uint8_t* dst = q8_row + k;
           if (k + 32 <= p.K) {
             *reinterpret_cast<uint4*>(dst) = lo;
             *reinterpret_cast<uint4*>(dst + 16) = hi;

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kMxThreads)
       reinterpret_cast<uint4*>(codes)[b] = block_fp4<T>(w[i], byte);
     } else {
       uint4 lo, hi;
-      block_int8<T>(w[i], byte, lo, hi);
+      block_int8<T>(w[i], amax, lo, hi);
       const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
       st_global_32b(codes + static_cast<int64_t>(b) * 32, v);
     }
