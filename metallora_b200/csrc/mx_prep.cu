@@ -56,6 +56,7 @@ struct PrepParams {
   long long atoms_k;
   uint8_t* q8;       // codes [M, ld8], or nullptr
   long long ld8;
+  int wide8;           // code rows start on 32 bytes
   uint8_t* q8_scales;  // words [ceil(K/128), rows8]
   long long rows8;
   int wide_rows;  // the row output starts on 32 bytes (its rows are 128 apart)
@@ -203,7 +204,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         block_int8<T>(w, amax, lo, hi);
         if (in) {
           uint8_t* dst = q8_row + k;
-          if (k + 32 <= p.K) {
+          if (k + 32 <= p.K && p.wide8) {
+            const uint32_t v[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+            st_global_32b(dst, v);
+          } else if (k + 32 <= p.K) {
             *reinterpret_cast<uint4*>(dst) = lo;
             *reinterpret_cast<uint4*>(dst + 16) = hi;
           } else {  // K is a multiple of 8: the row ends between two 8-byte groups
@@ -281,6 +285,7 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   p.atoms_k = (a.K + 127) / 128;
   p.q8 = static_cast<uint8_t*>(a.q8);
   p.ld8 = a.ld8;
+  p.wide8 = a.ld8 % 32 == 0 && reinterpret_cast<uintptr_t>(a.q8) % 32 == 0;
   p.q8_scales = static_cast<uint8_t*>(a.q8_scales);
   p.rows8 = (a.M + 3) / 4 * 4;
   p.wide_rows = reinterpret_cast<uintptr_t>(a.out_rows) % 32 == 0;
