@@ -1190,6 +1190,8 @@ int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme,
     return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
   if (w_dtype < MLORA_DTYPE_BF16 || w_dtype > MLORA_DTYPE_F32)
     return fail(MLORA_ERR_INVALID_ARG, "weight dtype must be BF16, F16 or F32");
+  if (scheme == MLORA_QUANT_MXFP4 && (reinterpret_cast<uintptr_t>(scales) & 3u))
+    return fail(MLORA_ERR_INVALID_ARG, "MXFP4 scales must be 4-byte aligned");
   if ((rc = check_device())) return rc;
   if (scheme == MLORA_QUANT_MXFP4)
     return launch_mx_quantize(4, w, w_dtype, N, K, codes, K / 2, plain_scales(scales, N, K),

@@ -636,6 +636,12 @@ int dispatch(const MxGemmArgs& a, cudaStream_t s) {
 }  // namespace
 
 int launch_mx_gemm(const MxGemmArgs& a, cudaStream_t s) {
+  // scale atoms are addressed by a 32-bit tensor-map row
+  const int64_t most = (int64_t(1) << 31) * kMxAtomBytes;
+  if (mx_atoms_bytes(a.M, a.K) >= most || mx_atoms_bytes(a.N, a.K) >= most) {
+    set_error("MXFP4 product: an operand has more than 2^31 blocks of 128 x 128");
+    return MLORA_ERR_UNSUPPORTED;
+  }
   return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
 }
 

@@ -71,7 +71,9 @@ class QuantizedWeight:
     def prepared_scales(self) -> torch.Tensor:
         """The TMA-ready scale table the GPU kernels read: [groups, rows rounded
         to 4], or for MXFP4 the product's blocks of 128 rows x 128 features
-        (built once, on first use, and kept with the weight)."""
+        (built once, on first use -- for MXFP4 when the weight is made -- and
+        kept with the weight; a table built while a graph is captured belongs to
+        that graph and is not kept)."""
         t = getattr(self, "_prepared", None)
         if t is None or t.device != self.codes.device:
             lib = _lib.load()
@@ -81,7 +83,8 @@ class QuantizedWeight:
             st = lib.mlora_qlora_prepare_scales(self.code, _ptr(self.scales), _ptr(self.zeros), N,
                                                 K, self.group, _ptr(t), _stream())
             _lib.check(st, "mlora_qlora_prepare_scales")
-            object.__setattr__(self, "_prepared", t)
+            if not torch.cuda.is_current_stream_capturing():
+                object.__setattr__(self, "_prepared", t)
         return t
 
     def state_dict(self) -> dict[str, torch.Tensor]:
@@ -129,7 +132,16 @@ def quantize(w: torch.Tensor, scheme: str = "nf4", group: int | None = None,
     st = _lib.load().mlora_quantize(_ptr(w), _dtype_code(w), N, K, SCHEMES[scheme], group,
                                     _ptr(codes), _ptr(scales), _ptr(zeros), _stream())
     _lib.check(st, "mlora_quantize")
-    return QuantizedWeight(scheme, codes, scales, zeros, group, (N, K), lean)
+    return _with_table(QuantizedWeight(scheme, codes, scales, zeros, group, (N, K), lean))
+
+
+def _with_table(qw: QuantizedWeight) -> QuantizedWeight:
+    """An MXFP4 weight on the GPU gets its table at once, in the order of its codes
+    on the stream: no later call, on whatever stream, is the one that makes it."""
+    if qw.scheme == "mxfp4" and qw.codes.is_cuda:
+        _need_current(qw.codes, qw.scales)
+        qw.prepared_scales()
+    return qw
 
 
 def dequantize(qw: QuantizedWeight, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -159,9 +171,9 @@ def from_reference_layout(scheme: str, codes, scales, zeros, shape, group,
                                         f"{tuple(t.shape)} {t.dtype}")
         if zeros is not None:
             raise QuantizationError("mxfp4 has no zero points")
-    return QuantizedWeight(scheme, codes.contiguous(), scales.contiguous(),
-                           None if zeros is None else zeros.contiguous(), int(group),
-                           (int(shape[0]), int(shape[1])), lean)
+    return _with_table(QuantizedWeight(scheme, codes.contiguous(), scales.contiguous(),
+                                       None if zeros is None else zeros.contiguous(), int(group),
+                                       (int(shape[0]), int(shape[1])), lean))
 
 
 # ------------------------------------------------- activation checkpoints --
