@@ -209,6 +209,11 @@ MLORA_API int mlora_merge(const void* w0, const void* a, const void* b, void* w_
 MLORA_API int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme,
                              int64_t group, void* codes, void* scales, void* zeros, void* stream);
 
+/* mlora_quantize for MXFP4 together with the weight's prepared scale table (see
+ * mlora_qlora_prepare_scales), in one pass over w where K % 128 == 0. */
+MLORA_API int mlora_quantize_mxfp4(const void* w, int w_dtype, int64_t N, int64_t K, void* codes,
+                                   void* scales, void* table, void* stream);
+
 /* out [N,K] = dequantised weights in out_dtype.  F32 output is bit-identical to
  * the reference's dequant_nf4 / dequant_int4 (lora_quantized.metal:17-25);
  * BF16/F16 output is that value rounded to nearest even -- exactly the operand

@@ -66,6 +66,7 @@ SIGNATURES: dict[str, tuple] = {
     "mlora_merge_workspace_bytes": (sz, [i64, i64, i64, i32]),
     "mlora_merge": (i32, [vp, vp, vp, vp, i64, i64, i64, f32, i32, vp, sz, vp]),
     "mlora_quantize": (i32, [vp, i32, i64, i64, i32, i64, vp, vp, vp, vp]),
+    "mlora_quantize_mxfp4": (i32, [vp, i32, i64, i64, vp, vp, vp, vp]),
     "mlora_dequantize": (i32, [i32, vp, vp, vp, i64, i64, i64, vp, i32, vp]),
     "mlora_qlora_forward_workspace_bytes": (sz, [i64, i64, i64, i64, i32, i64]),
     "mlora_qlora_backward_workspace_bytes": (sz, [i64, i64, i64, i64, i32, i64]),

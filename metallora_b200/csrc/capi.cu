@@ -515,10 +515,11 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
                size_t workspace_bytes, cudaStream_t s, int phase = kPhaseAll,
                bool grads16 = false, const Ckpt* ckpt = nullptr) {
   int rc;
-  const BwdPlan need = plan_backward(nullptr, M, K, N, r, saved_xa == nullptr);
+  const bool two_t = saved_xa == nullptr || ckpt != nullptr;  // [R, M] besides U's
+  const BwdPlan need = plan_backward(nullptr, M, K, N, r, two_t);
   if (workspace == nullptr || workspace_bytes < need.bytes || !aligned16(workspace))
     return fail(MLORA_ERR_WORKSPACE, "backward workspace needs " + std::to_string(need.bytes) + " bytes");
-  const BwdPlan p = plan_backward(workspace, M, K, N, r, saved_xa == nullptr);
+  const BwdPlan p = plan_backward(workspace, M, K, N, r, two_t);
   const Elt elt = dtype == MLORA_DTYPE_BF16 ? Elt::kBF16 : Elt::kF16;
   const float scale = alpha / static_cast<float>(r);
 
@@ -539,6 +540,7 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
     l.u_rows = dx ? p.u_rows : nullptr;
     l.ld_rows = p.R64;
     l.u_t = p.u_t;
+    l.u_lo = p.xa_t;  // not needed for s.x.A^T: that is the caller's
     l.ld_t = pad8(M);
     l.db = db;
     l.accumulate = accumulate;
@@ -551,6 +553,7 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
     g.scales = ckpt->scales;
     g.ld = ckpt->ld;
     g.st = p.u_t;
+    g.st_lo = p.xa_t;
     g.ld_st = pad8(M);
     g.M = M;
     g.K = K;
@@ -1200,6 +1203,26 @@ int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme,
                          static_cast<cudaStream_t>(stream));
 }
 
+int mlora_quantize_mxfp4(const void* w, int w_dtype, int64_t N, int64_t K, void* codes,
+                         void* scales, void* table, void* stream) {
+  if (!table) return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
+  if (!aligned16(table)) return fail(MLORA_ERR_INVALID_ARG, "the table must be 16-byte aligned");
+  bool made = false;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int rc = check_quant(MLORA_QUANT_MXFP4, N, K, 32);
+  if (rc) return rc;
+  if (!w || !codes || !scales) return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
+  if (w_dtype < MLORA_DTYPE_BF16 || w_dtype > MLORA_DTYPE_F32)
+    return fail(MLORA_ERR_INVALID_ARG, "weight dtype must be BF16, F16 or F32");
+  if (reinterpret_cast<uintptr_t>(scales) & 3u)
+    return fail(MLORA_ERR_INVALID_ARG, "MXFP4 scales must be 4-byte aligned");
+  if ((rc = check_device())) return rc;
+  if ((rc = launch_mx_quantize(4, w, w_dtype, N, K, codes, K / 2, plain_scales(scales, N, K), s,
+                               table, &made)))
+    return rc;
+  return made ? MLORA_OK : launch_mx_prepare_scales(scales, N, K, table, s);
+}
+
 int mlora_dequantize(int scheme, const void* codes, const void* scales, const void* zeros,
                      int64_t N, int64_t K, int64_t group, void* out, int out_dtype, void* stream) {
   int rc = check_quant(scheme, N, K, group);
@@ -1602,7 +1625,8 @@ int qlora_backward_any(const void* dy, const void* x, const Ckpt* ckpt, int sche
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const bool accumulate = (flags & MLORA_BWD_ACCUMULATE) != 0;
   const bool grads16 = (flags & MLORA_BWD_GRADS_16BIT) != 0;
-  const size_t bytes = plan_backward(nullptr, M, K, N, r, saved_xa == nullptr).bytes;
+  const size_t bytes =
+      plan_backward(nullptr, M, K, N, r, saved_xa == nullptr || ckpt != nullptr).bytes;
   if (dx == nullptr)  // weight gradients only: the base weight is not read
     return backward16(dy, x, nullptr, nullptr, a, b, saved_xa, nullptr, da, db, M, K, N, r, alpha,
                       clip_value, accumulate, dtype, workspace, workspace_bytes, s, kPhaseAll, grads16,

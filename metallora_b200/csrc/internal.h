@@ -205,7 +205,8 @@ int launch_wgrad(const WgradArgs* probs, int nprobs, cudaStream_t stream);
 
 // ------------------------------------------- both products of dy, one launch --
 // U = scale dy.B: u_rows [M, ld_rows] (may be null; columns past R zeroed) and
-// u_t [R, ld_t]; db (+)= clip(dy^T . xa_t^T) [N, r].  dy [M, N], b [N, r],
+// its transpose in two 16-bit parts, u_t + u_lo [R, ld_t] each (u_lo is what
+// rounding to u_t left over); db (+)= clip(dy^T . xa_t^T) [N, r].  dy [M, N], b [N, r],
 // xa_t [R, ld_xa] (rows >= r are zero).
 struct LoraBwdArgs {
   const void* dy;
@@ -217,6 +218,7 @@ struct LoraBwdArgs {
   void* u_rows;
   int64_t ld_rows;
   void* u_t;
+  void* u_lo;
   int64_t ld_t;
   void* db;
   bool accumulate, out16;
@@ -293,8 +295,11 @@ struct MxScales {
   int layout;
 };
 // bits = 4 (MXFP4) or 8 (MXINT8); code rows start ld bytes apart.
+// `atoms` (optional, bits = 4): the scale atoms too, where the rows allow it in
+// the same pass (*atoms_made tells).
 int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K, void* codes,
-                       int64_t ld, const MxScales& sc, cudaStream_t s);
+                       int64_t ld, const MxScales& sc, cudaStream_t s, void* atoms = nullptr,
+                       bool* atoms_made = nullptr);
 int launch_mx_dequantize(int bits, const void* codes, int64_t ld, const MxScales& sc, int64_t M,
                          int64_t K, void* out, int out_dtype, cudaStream_t s);
 int launch_mx_prepare_scales(const void* scales, int64_t rows, int64_t K, void* atoms,
@@ -348,13 +353,14 @@ struct MxGemmArgs {
 };
 int launch_mx_gemm(const MxGemmArgs& a, cudaStream_t s);
 
-// da[j, p] = sum_m st[j, m] * x^[m, p] for an MXINT8 checkpoint x^ [M, K] (code
+// da[j, p] = sum_m (st[j, m] + st_lo[j, m]) * x^[m, p] for an MXINT8 checkpoint x^ [M, K] (code
 // rows ld bytes apart, kMxGroups scales); output as WgradArgs (transposed).
 struct MxWgradArgs {
   const void* codes;
   const void* scales;
   int64_t ld;
   const void* st;
+  const void* st_lo;
   int64_t ld_st;
   int64_t M, K, r, R;
   void* out;

@@ -1,6 +1,6 @@
 // The two products of the LoRA backward that read dy, in one launch:
 //
-//     U  = s dy . B           (rows [M, R64] and transposed [R, M])
+//     U  = s dy . B           (rows [M, R64]; transposed [R, M] in two 16-bit parts)
 //     dB = dy^T . (s x A^T)   ([N, r])
 //
 // U reduces over features, dB over tokens, so neither is a by-product of the
@@ -66,6 +66,7 @@ struct BwdParams {
   void* u_rows;
   long long ld_rows;
   void* u_t;
+  void* u_lo;
   long long ld_t;
   void* db;
   int accumulate, out16;
@@ -197,9 +198,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       for (int i = 0; i < C; ++i) v[i] = in[i] * p.scale;
       if (p.u_rows != nullptr)
         store_columns<T>(reinterpret_cast<T*>(p.u_rows) + row * p.ld_rows + j, v, p.wide_rows != 0);
-      T* dst = reinterpret_cast<T*>(p.u_t) + row + j * p.ld_t;
+      // both parts for dA: with the first alone, U's rounding weighs as much in dA
+      // as the rounding of dA itself
+      T* hi = reinterpret_cast<T*>(p.u_t) + row + j * p.ld_t;
+      T* lo = reinterpret_cast<T*>(p.u_lo) + row + j * p.ld_t;
 #pragma unroll
-      for (int i = 0; i < C; ++i) dst[i * p.ld_t] = static_cast<T>(v[i]);
+      for (int i = 0; i < C; ++i) {
+        const T h = static_cast<T>(v[i]);
+        hi[i * p.ld_t] = h;
+        lo[i * p.ld_t] = static_cast<T>(v[i] - static_cast<float>(h));
+      }
       return;
     }
 #pragma unroll
@@ -264,6 +272,7 @@ int launch_typed(const LoraBwdArgs& a, cudaStream_t stream) {
   p.u_rows = a.u_rows;
   p.ld_rows = a.ld_rows;
   p.u_t = a.u_t;
+  p.u_lo = a.u_lo;
   p.ld_t = a.ld_t;
   p.db = a.db;
   p.accumulate = a.accumulate ? 1 : 0;

@@ -85,7 +85,8 @@ __device__ __forceinline__ void ld_global_32b(const void* p, uint32_t* v) {
 template <int kBits, typename T>
 __global__ void __launch_bounds__(kMxThreads)
     mx_quantize_blocks_kernel(const T* __restrict__ x, uint32_t blocks, uint32_t per_row,
-                              uint8_t* __restrict__ codes, const MxScales sc) {
+                              uint8_t* __restrict__ codes, const MxScales sc,
+                              uint8_t* __restrict__ atoms) {
   const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
   uint32_t w[kOwn][16];
 #pragma unroll
@@ -102,6 +103,11 @@ __global__ void __launch_bounds__(kMxThreads)
     const uint32_t amax = block_amax<T>(w[i]);
     const uint32_t byte = kBits == 4 ? mx_scale_byte_fp4(amax) : mx_scale_byte_int8(amax);
     *scale_of(sc, b, per_row) = static_cast<uint8_t>(byte);
+    if (kBits == 4 && atoms != nullptr) {  // rows of whole atoms
+      const uint32_t row = b / per_row, k = b - row * per_row;
+      atoms[(static_cast<int64_t>(row >> 7) * (per_row >> 2) + (k >> 2)) * kMxAtomBytes +
+            (row & 31u) * 16 + ((row >> 5) & 3u) * 4 + (k & 3u)] = static_cast<uint8_t>(byte);
+    }
     if constexpr (kBits == 4) {
       reinterpret_cast<uint4*>(codes)[b] = block_fp4<T>(w[i], byte);
     } else {
@@ -377,26 +383,31 @@ bool whole_blocks(const void* wide, int dtype, const void* codes, int64_t ld, in
 }  // namespace
 
 int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K, void* codes,
-                       int64_t ld, const MxScales& sc, cudaStream_t s) {
+                       int64_t ld, const MxScales& sc, cudaStream_t s, void* atoms,
+                       bool* atoms_made) {
   if (whole_blocks(x, dtype, codes, ld, K * bits / 8, sc, M, K)) {
     const auto blocks = static_cast<uint32_t>(M * (K / kMxBlock));
     const auto per_row = static_cast<uint32_t>(K / kMxBlock);
     const unsigned grid = (blocks + kMxThreads * kOwn - 1) / (kMxThreads * kOwn);
     auto* c = static_cast<uint8_t*>(codes);
+    // (a group that is not whole would leave padding bytes of its atoms unset)
+    auto* t = K % 128 == 0 ? static_cast<uint8_t*>(atoms) : nullptr;
+    if (atoms_made != nullptr) *atoms_made = t != nullptr;
     LaunchScope scope(kKindQuant, s);
     if (dtype == MLORA_DTYPE_BF16) {
       const auto* xt = static_cast<const __nv_bfloat16*>(x);
       bits == 4
-          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc)
-          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc);
+          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t)
+          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t);
     } else {
       const auto* xt = static_cast<const __half*>(x);
       bits == 4
-          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc)
-          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc);
+          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t)
+          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t);
     }
     return launched("mx quantize");
   }
+  if (atoms_made != nullptr) *atoms_made = false;
   dim3 grid;
   if (int rc = mx_grid(M, K, &grid)) return rc;
   // whole 8-feature groups, 16-byte loads, 4- (fp4) or 8-byte (int8) stores

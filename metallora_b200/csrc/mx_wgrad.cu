@@ -3,8 +3,10 @@
 //     dA[j, p] = sum_m U[m, j] . x^[m, p]          U = s dy B, x^ the checkpoint
 //
 // The checkpoint's values are exact in bf16 (mx.cuh), so the codes are turned
-// into 16-bit operands inside the kernel and the tensor cores do the sum: the
-// only roundings are U's (already 16-bit) and, for fp16, values below 2^-24.
+// into 16-bit operands inside the kernel and the tensor cores do the sum.  U
+// comes as two 16-bit parts, two MMAs into one accumulator: what is left of its
+// rounding is 2^-16 (fp16 2^-22, or its subnormal step), and for fp16 the
+// rounding of checkpoint values below 2^-24.
 // HBM-bound on the codes, half the bytes of a 16-bit x.
 //
 // CTA = 128 features x one range of tokens; the ranges of a tile are one
@@ -38,7 +40,8 @@ constexpr int kMaxSplits = 8;
 __host__ __device__ constexpr bool pushed(int R) { return R <= 32; }
 __host__ __device__ constexpr uint32_t recv_bytes(int R) { return pushed(R) ? push_bytes(R) : 0u; }
 __host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
-__host__ __device__ constexpr uint32_t stage_bytes(int R) { return R * 128u + kCodeBytes + 1024u; }
+// [R x 64] of both parts of U^T, codes, scale words
+__host__ __device__ constexpr uint32_t stage_bytes(int R) { return R * 256u + kCodeBytes + 1024u; }
 __host__ __device__ constexpr int num_stages(int R) {
   const uint32_t room =
       (ctas_per_sm(R) == 2 ? 110u : 220u) * 1024u - kOps * kOpBytes - recv_bytes(R);
@@ -66,7 +69,8 @@ template <int R, bool kBF16>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     mx_wgrad_kernel(const __grid_constant__ CUtensorMap tm_codes,
                     const __grid_constant__ CUtensorMap tm_scales,
-                    const __grid_constant__ CUtensorMap tm_st, const MxWgradParams p) {
+                    const __grid_constant__ CUtensorMap tm_st,
+                    const __grid_constant__ CUtensorMap tm_lo, const MxWgradParams p) {
   using T = typename std::conditional<kBF16, __nv_bfloat16, __half>::type;
   constexpr int S = num_stages(R);
   extern __shared__ uint8_t smem_raw[];
@@ -79,7 +83,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   uint64_t* op_empty = op_full + kOps;    // [kOps]
   uint64_t* done_bar = op_empty + kOps;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
-  constexpr uint32_t kCodeOff = R * 128u;
+  constexpr uint32_t kLoOff = R * 128u;
+  constexpr uint32_t kCodeOff = R * 256u;
   constexpr uint32_t kScaleOff = kCodeOff + kCodeBytes;
 
   const uint32_t warp = warp_id();
@@ -113,9 +118,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       uint32_t armed_parity[S];
       for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
       auto load_codes = [&](int kb, uint8_t* st, uint64_t* bar) {
-        mbar_arrive_expect_tx(bar, R * 128u + kCodeBytes + kScaleBytes);
+        mbar_arrive_expect_tx(bar, R * 256u + kCodeBytes + kScaleBytes);
         tma_load_2d(st + kCodeOff, &tm_codes, bar, tile * 128, kb * kBM);
         tma_load_2d(st + kScaleOff, &tm_scales, bar, kb * kBM, tile);
+      };
+      auto load_u = [&](int kb, uint8_t* st, uint64_t* bar) {
+        tma_load_2d(st, &tm_st, bar, kb * kBM, 0);
+        tma_load_2d(st + kLoOff, &tm_lo, bar, kb * kBM, 0);
       };
       // U comes from the kernel before this one, the checkpoint does not: a ring
       // of code blocks is on its way before the wait
@@ -126,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       }
       asm volatile("griddepcontrol.wait;" ::: "memory");
       for (int i = 0; i < ahead; ++i)
-        tma_load_2d(stages + i * stage_bytes(R), &tm_st, &full_bar[i], (kb_begin + i) * kBM, 0);
+        load_u(kb_begin + i, stages + i * stage_bytes(R), &full_bar[i]);
       if (ahead == S) phase = 1;
       for (int kb = kb_begin + ahead; kb < kb_end; ++kb) {
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) break;
@@ -134,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         armed[stage] = true;
         armed_parity[stage] = phase;
         load_codes(kb, st, &full_bar[stage]);
-        tma_load_2d(st, &tm_st, &full_bar[stage], kb * kBM, 0);
+        load_u(kb, st, &full_bar[stage]);
         if (++stage == S) stage = 0, phase ^= 1u;
       }
       for (int s = 0; s < S; ++s)
@@ -154,6 +163,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         for (int k = 0; k < 4; ++k)
           umma_f16(tmem, desc_mnmajor_sw128(sa, k, kHalfBytes), desc_kmajor_sw128(sb, k), idesc,
                    (kb != kb_begin || k != 0) ? 1u : 0u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          umma_f16(tmem, desc_mnmajor_sw128(sa, k, kHalfBytes), desc_kmajor_sw128(sb + kLoOff, k),
+                   idesc, 1u);
         umma_commit(&empty_bar[stage]);
         umma_commit(&op_empty[op]);
         if (++stage == S) stage = 0, phase ^= 1u;
@@ -247,14 +260,15 @@ int cuda_launch_error(cudaError_t e, const char* what) {
 
 template <int R, bool kBF16>
 int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
-  CUtensorMap tc, ts, tu;
+  CUtensorMap tc, ts, tu, tl;
   const int64_t m4 = (a.M + 3) / 4 * 4, groups = (a.K + 127) / 128;
   if (!make_tmap_2d(&tc, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, a.codes, static_cast<uint64_t>(a.K),
                     static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.ld), 128, kBM, false) ||
       // (rows past M, which pad the words, are not read: their bytes are not set)
       !make_tmap_2d(&ts, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, a.scales, static_cast<uint64_t>(a.M),
                     static_cast<uint64_t>(groups), static_cast<uint64_t>(m4) * 4, kBM, 1, false) ||
-      !make_tmap_2d_16b(&tu, a.st, a.M, a.R, a.ld_st, kBM, R))
+      !make_tmap_2d_16b(&tu, a.st, a.M, a.R, a.ld_st, kBM, R) ||
+      !make_tmap_2d_16b(&tl, a.st_lo, a.M, a.R, a.ld_st, kBM, R))
     return MLORA_ERR_INVALID_ARG;
   MxWgradParams p;
   p.P = static_cast<int>(a.K);
@@ -290,7 +304,7 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = a.overlap_prev ? 2 : 1;
   LaunchScope scope(kKindWgrad, stream);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tc, ts, tu, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tc, ts, tu, tl, p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx wgrad launch");
 }

@@ -118,9 +118,7 @@ def quantize(w: torch.Tensor, scheme: str = "nf4", group: int | None = None,
     group = group or DEFAULT_GROUP[scheme]
     N, K = w.shape
     if scheme == "mxfp4":
-        _need_current(w)
-        if N == 0 or K == 0:
-            raise ShapeError("quantize takes a weight with at least one row and one column")
+        return _quantize_mxfp4(w.contiguous())
     if scheme != "int8" and K % 2:
         raise QuantizationError("4-bit codes pack two per byte: in_features must be even")
     G = -(-K // group)
@@ -132,7 +130,25 @@ def quantize(w: torch.Tensor, scheme: str = "nf4", group: int | None = None,
     st = _lib.load().mlora_quantize(_ptr(w), _dtype_code(w), N, K, SCHEMES[scheme], group,
                                     _ptr(codes), _ptr(scales), _ptr(zeros), _stream())
     _lib.check(st, "mlora_quantize")
-    return _with_table(QuantizedWeight(scheme, codes, scales, zeros, group, (N, K), lean))
+    return QuantizedWeight(scheme, codes, scales, zeros, group, (N, K), lean)
+
+
+def _quantize_mxfp4(w: torch.Tensor) -> QuantizedWeight:
+    _need_current(w)
+    N, K = w.shape
+    if N == 0 or K == 0:
+        raise ShapeError("quantize takes a weight with at least one row and one column")
+    lib = _lib.load()
+    codes = w.new_empty((N, K // 2), dtype=torch.uint8)
+    scales = w.new_empty((N, -(-K // 32)), dtype=torch.uint8)
+    table = w.new_empty(lib.mlora_qlora_prepared_scales_bytes(_lib.QUANT_MXFP4, N, K, 32),
+                        dtype=torch.uint8)
+    st = lib.mlora_quantize_mxfp4(w.data_ptr(), _dtype_code(w), N, K, codes.data_ptr(),
+                                  scales.data_ptr(), table.data_ptr(), _stream())
+    _lib.check(st, "mlora_quantize_mxfp4")
+    qw = QuantizedWeight("mxfp4", codes, scales, None, 32, (N, K))
+    object.__setattr__(qw, "_prepared", table)
+    return qw
 
 
 def _with_table(qw: QuantizedWeight) -> QuantizedWeight:
@@ -150,7 +166,7 @@ def dequantize(qw: QuantizedWeight, dtype: torch.dtype = torch.float32) -> torch
     N, K = qw.shape
     if qw.scheme == "mxfp4":
         _need_current(qw.codes)
-    out = torch.empty((N, K), dtype=dtype, device=qw.device)
+    out = qw.codes.new_empty((N, K), dtype=dtype)
     st = _lib.load().mlora_dequantize(qw.code, _ptr(qw.codes), _ptr(qw.scales), _ptr(qw.zeros), N,
                                       K, qw.group, _ptr(out), _dtype_code(out), _stream())
     _lib.check(st, "mlora_dequantize")

@@ -213,6 +213,11 @@ def test_mxfp4_quantize_exact(cuda, dt, rows, k):
     qw = quant.quantize(w.to(cuda), "mxfp4")
     val, byte = mx_oracle.mxfp4(_np(w))
     np.testing.assert_array_equal(qw.scales.cpu().numpy(), byte)
+    # the product's table: 512-byte blocks of 128 rows x 4 scale bytes
+    tab = qw._prepared.view(-(-rows // 128), -(-k // 128), 32, 4, 4).permute(0, 3, 2, 1, 4)
+    tab = tab.reshape(-(-rows // 128) * 128, -1).cpu().numpy()
+    np.testing.assert_array_equal(tab[:rows, : byte.shape[1]], byte)
+    assert not tab[:rows, byte.shape[1]:].any()
     np.testing.assert_array_equal(mx_oracle.unpack_fp4(qw.codes.cpu().numpy(), byte), val)
     for out in (FP32, BF16):
         np.testing.assert_array_equal(_np(qw.dequantize(out)), val)
@@ -419,18 +424,18 @@ def _ckpt_values(c):
     return c.codes.cpu().numpy() / 64.0 * np.repeat(s, 32, -1)[:, : c.shape[-1]]
 
 
-def _grad_check(da, db, dy, xh, saved, a, b, alpha, old=None, clip=None):
-    """dA = s (dy.B)^T.x^ with s dy.B rounded to 16 bits, dB = dy^T.saved."""
+def _grad_check(da, db, dy, xh, saved, a, b, alpha, old=None, clip=None, parts=2):
+    """dA = s (dy.B)^T.x^ with s dy.B in `parts` 16-bit parts, dB = dy^T.saved."""
     dt, h = dy.dtype, _half_step(dy.dtype)
     r, N, M = a.shape[0], b.shape[0], dy.shape[0]
     s = alpha / r
     DY, B, S = _np(dy), _np(b), _np(saved)[:r, :M]
     u = s * DY @ B
-    u_err = N * ACC * (s * np.abs(DY) @ np.abs(B)) + h * np.abs(u) + _tiny(dt)
+    u_err = N * ACC * (s * np.abs(DY) @ np.abs(B)) + h ** parts * np.abs(u) + _tiny(dt)
     ref_a, mag_a = u.T @ xh, np.abs(u).T @ np.abs(xh)
     # x^ itself is exact in bf16 and, above fp16's subnormals, in fp16
     x_err = 0.0 if dt == BF16 else np.abs(u).sum(0)[:, None] * _tiny(dt)
-    tol_a = u_err.T @ np.abs(xh) + 1.01 * M * ACC * mag_a + x_err
+    tol_a = u_err.T @ np.abs(xh) + 1.01 * parts * M * ACC * mag_a + x_err
     ref_b, tol_b = DY.T @ S.T, M * ACC * (np.abs(DY).T @ np.abs(S).T)
     for got, ref, tol, o in ((da, ref_a, tol_a, 0), (db, ref_b, tol_b, 1)):
         if clip:
@@ -587,7 +592,7 @@ def test_step(cuda, dt, M, K, N, r):
     _fwd_check(y, x, qw, a, b, 32.0)
     _, saved = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True)
     _grad_check(da, db, dy, _ckpt_values(shared), saved, a, b, 32.0)
-    _grad_check(da0, db0, dy, _np(x), saved, a, b, 32.0)
+    _grad_check(da0, db0, dy, _np(x), saved, a, b, 32.0, parts=1)
     h, s = _half_step(dt), 32.0 / r
     W = mx_oracle.unpack_fp4(qw.codes.cpu().numpy(), qw.scales.cpu().numpy())
     DY, A, B = _np(dy), _np(a), _np(b)
