@@ -27,7 +27,6 @@ constexpr int kQuantWarps = 8;
 constexpr int kThreads = 64 + 32 * kQuantWarps;
 constexpr int kBK = 64;
 constexpr uint32_t kXBytes = 128 * kBK * 2;
-constexpr int kMaxSplits = 8;
 
 __host__ __device__ constexpr int ctas_per_sm(int R) { return R <= 64 ? 2 : 1; }
 __host__ __device__ constexpr uint32_t stage_bytes(int R) { return kXBytes + R * 128u; }
@@ -291,11 +290,9 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   p.wide_rows = reinterpret_cast<uintptr_t>(a.out_rows) % 32 == 0;
   p.status = device_status_ptr();
   const int64_t tiles = (a.M + 127) / 128;
-  // one wave of resident CTAs, at least four k-blocks a split
-  const int64_t slots = static_cast<int64_t>(ctas_per_sm(R)) * num_sms();
-  int splits = 1;
-  while (splits * 2 <= kMaxSplits && splits * 2 * tiles <= slots && splits * 8 <= p.num_kb)
-    splits *= 2;
+  // the plain rank projection's split, so that s x A^T has the same bits with and
+  // without a checkpoint (up to rank 64 it is also one wave of these CTAs)
+  const int splits = rank_splits(a.M, a.K);
   p.splits = splits;
   auto kern = mx_prep_kernel<R, kBF16>;
   static std::atomic<bool> attr_set[64];

@@ -51,6 +51,11 @@ def _kept_x(ctx, x2d, scales):
     return ActivationCheckpoint(x2d, scales, *ctx.x_meta)
 
 
+def _cast_ab(a, b, dtype):
+    """A and B in ``dtype`` (``Tensor.to`` costs about 1 us where it changes nothing)."""
+    return (a if a.dtype == dtype else a.to(dtype)), (b if b.dtype == dtype else b.to(dtype))
+
+
 def _sink_accumulates(sink) -> bool:
     return sink is None or len(sink) < 3 or bool(sink[2])
 
@@ -72,7 +77,7 @@ class _LoRALinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2d, w0, a, b, alpha, compute, sink, checkpoint=None):
-        a_c, b_c = compute if compute is not None else (a.to(x2d.dtype), b.to(x2d.dtype))
+        a_c, b_c = compute if compute is not None else _cast_ab(a, b, x2d.dtype)
         ckpt, fill = _checkpoint(x2d, checkpoint)
         y, saved = _k.lora_linear_fwd(x2d, w0, a_c, b_c, alpha, save_xa=True,
                                       ckpt_out=ckpt if fill else None)
@@ -124,7 +129,7 @@ class _QLoRALinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2d, a, b, qw, alpha, compute, sink, checkpoint=None):
-        a_c, b_c = compute if compute is not None else (a.to(x2d.dtype), b.to(x2d.dtype))
+        a_c, b_c = compute if compute is not None else _cast_ab(a, b, x2d.dtype)
         ckpt, fill = _checkpoint(x2d, checkpoint)
         y, saved = _k.qlora_linear_fwd(x2d, qw, a_c, b_c, alpha, save_xa=True,
                                        ckpt_out=ckpt if fill else None)
@@ -151,9 +156,10 @@ class _QLoRALinearFn(torch.autograd.Function):
             sink[3]()
         if sink is not None:
             return dx, None, None, None, None, None, None, None
-        da = da.to(ctx.ab_dtypes[0]) if ctx.needs_input_grad[1] else None
-        db = db.to(ctx.ab_dtypes[1]) if ctx.needs_input_grad[2] else None
-        return dx, da, db, None, None, None, None, None
+        if not same:
+            da, db = da.to(ctx.ab_dtypes[0]), db.to(ctx.ab_dtypes[1])
+        return (dx, da if ctx.needs_input_grad[1] else None,
+                db if ctx.needs_input_grad[2] else None, None, None, None, None, None)
 
 
 def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=None,  # noqa: N803
@@ -167,7 +173,7 @@ def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=No
     x2d = x if len(shp) == 2 else x.reshape(-1, shp[-1])
     if qweight.scheme == "mxfp4" and not (torch.is_grad_enabled() and
                                           (x.requires_grad or A.requires_grad or B.requires_grad)):
-        a, b = _compute if _compute is not None else (A.to(x.dtype), B.to(x.dtype))
+        a, b = _compute if _compute is not None else _cast_ab(A, B, x.dtype)
         out = _k.qlora_linear_fwd(x2d, qweight, a, b, float(alpha))[0]
     else:
         out = _QLoRALinearFn.apply(x2d, A, B, qweight, float(alpha), _compute, _sink, checkpoint)
@@ -190,8 +196,9 @@ def lora_forward(x, W0, A, B, alpha: float = 16.0, dropout: float = 0.0,  # noqa
     ``checkpoint`` keeps x for the backward in 8 bits instead of 16: "mxint8"
     quantises it here, a ``quant.ActivationCheckpoint`` of x is used as it is
     (layers that share an input share one).  dA then comes from the
-    checkpoint's values; y, dx and dB do not change.  It needs a frozen W0 and
-    no dropout, which read x itself.
+    checkpoint's values; y does not change, and dx and dB at most in the order
+    of their fp32 sums.  It needs a frozen W0 and no dropout, which read x
+    itself.
     """
     if x.shape[-1] != W0.shape[1]:
         raise ShapeError(f"x last dim {x.shape[-1]} != in_features {W0.shape[1]}")

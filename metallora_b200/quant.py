@@ -276,11 +276,12 @@ def checkpoint_activation(x: torch.Tensor) -> ActivationCheckpoint:
     _need_current(x)
     code = _dtype_code(x)
     c = empty_checkpoint(x)
-    if x.numel():
-        x = x.detach().contiguous()
-        st = _lib.load().mlora_act_checkpoint(x.data_ptr(), code, c.codes.shape[0], x.shape[-1],
-                                              c.codes.data_ptr(), c.codes.stride(0),
-                                              c.scales.data_ptr(), _stream())
+    M, K = c.codes.shape
+    if M:
+        if not x.is_contiguous():
+            x = x.detach().contiguous()
+        st = _lib.load().mlora_act_checkpoint(x.data_ptr(), code, M, K, c.codes.data_ptr(),
+                                              c.codes.stride(0), c.scales.data_ptr(), _stream())
         _lib.check(st, "mlora_act_checkpoint")
     return c
 
