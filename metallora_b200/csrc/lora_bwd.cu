@@ -9,6 +9,10 @@
 // reduction tail are paid instead of two.  B is read as it lies ([N, r], the
 // MMA's MN-major operand): no transposed copy.
 //
+// Measured, dy 8192 x 4096, r 16: 17 us, 11 of them streaming (67.8 MB from HBM,
+// 152 MB from L2 to the SMs: 13 TB/s, which bounds it), 3 to the first MMA, 2-3 of
+// reduction.  The two launches and the transpose it replaces took 31 us.
+//
 // A CTA owns one 128-row tile of U or of dB and one range of its reduction; the
 // ranges of a tile lie in one cluster, and their partial tiles meet through
 // distributed shared memory in fixed order (cluster_push_reduce).  The two products

@@ -30,9 +30,12 @@ constexpr uint32_t kSfBytes = 2 * kMxAtomBytes;  // scales of 128 rows x 256 fea
 // ---------------------------------------------------------------------------
 // Few tokens (M <= 128): the weight rows are the MMA's M side (128 a tile) and
 // the tokens its N side, so one pass over the weight serves all tokens.
-// Bound by the weight's HBM traffic; the reduction is split over the CTAs of a
-// cluster so that about two CTAs per SM stream it, and their partial tiles are
-// summed through distributed shared memory in fixed order (cluster_push_reduce).
+// Bound by latency: one token through 4096 -> 11008 takes 12.3 us with the pass
+// before it, of which the weight's 24 MB are 3.7 at the measured bandwidth; a ring
+// of weight blocks is loaded while that pass still runs.  The reduction is split
+// over the CTAs of a cluster so that about two CTAs per SM stream it, and their
+// partial tiles are summed through distributed shared memory in fixed order
+// (cluster_push_reduce).
 constexpr int kSkinnyThreads = 192;
 constexpr int kSkinnyMaxSplits = 8;
 
@@ -220,12 +223,20 @@ __global__ void __launch_bounds__(kSkinnyThreads)
 // More tokens: persistent CTA pairs (cta_group::2), one 256 x 256 tile a pair at
 // a time, as the dense pair GEMM.  Each CTA stages its own 128 rows of x and of
 // W (16 KB each a k-block of 256) and the scale atoms of its x rows and of all
-// 256 W rows.  The fp4 MMA is four times the bf16 rate, so staging is what
-// bounds it: 35 KB a CTA feed about 540 clocks of MMA.
+// 256 W rows.
 //
 // The scales need TMEM next to the accumulator, so the accumulator is not
 // double-buffered; eight epilogue warps take it into registers at once and hand
 // it back before they convert and store.
+//
+// Measured, 4096 x 4096 -> 11008, R 64: about 75 us = 5.0 PFLOP/s.  A tile takes
+// 11.5-12.5 thousand cycles: 8.7 of MMA (64 fp4 of 128 cycles, 4 bf16), 1.4 of
+// scale copies (they run in the MMAs' queue, 15 cycles each), 0.9 until the
+// accumulator is free again, 1-2 of waiting for operands (834 MB come from L2;
+// with one MMA in four issued, the copies alone take 53 us).  9.3 tiles a pair
+// leave the tenth wave a third full, and the chip's power cap holds it at
+// 1.63 GHz.  Tried and slower: copying a block's scales ahead of the MMAs of the
+// block before (107 against 95 us); no effect: raster groups of 1 to 32.
 constexpr int kPairStages = 6;
 constexpr int kHalf = 128;
 constexpr int kPairN = 256;

@@ -11,6 +11,11 @@
 // tiles of A (TMA ring), warp 1 issues the UMMAs, warps 2-9 quantise: a thread
 // owns one block of 32 features, so the block maximum needs no exchange.  A
 // stage is free when the UMMAs and all eight warps are done with it.
+//
+// Measured under ncu: 16.7 us for 4096 x 4096 with the fp4 operand (floor 6.6), 30
+// us for 8192 x 4096 with fp4 operand and checkpoint (118 MB, floor 18).  There
+// the quantising warps bound it: about 230 instructions a thread and block, issue
+// slots 56 % used by 16 warps an SM.  At a few tokens it is latency: 4 us.
 #include <atomic>
 #include <string>
 #include <type_traits>

