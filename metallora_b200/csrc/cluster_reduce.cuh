@@ -33,9 +33,7 @@ __device__ __forceinline__ void load_acc_row(uint32_t taddr_row, float (&acc)[R]
 // One CTA alone (S = 1) emits straight from its registers, without a barrier.
 // Columns go in passes of CP (R > 128: two passes), each read from TMEM at
 // `taddr` (this thread's lane) when `have` (zeros otherwise).  Every thread of
-// the CTA calls this; only epilogue threads (`epi`) move data.  A cluster may
-// hold several such groups of S CTAs side by side: `first` is the cluster rank
-// of this group's first CTA, `crank` the rank within the group.
+// the CTA calls this; only epilogue threads (`epi`) move data.
 __host__ __device__ constexpr int reduce_cols(int R) { return R <= 128 ? R : 128; }
 
 // Hands N consecutive column sums from column j to `emit`: all at once to one
@@ -89,8 +87,8 @@ __device__ __forceinline__ void store_columns(T* dst, const float (&v)[N], bool 
 // S peers' values.  Up to 32 loads are in flight before the first sum: each is a
 // trip to another SM (with two at a time, 64 columns over two CTAs took 13 us).
 template <int CP, int S, typename Emit>
-__device__ __forceinline__ void sum_slices(const float* buf, int crank, uint32_t first,
-                                           int row_local, int j_base, Emit&& emit) {
+__device__ __forceinline__ void sum_slices(const float* buf, int crank, int row_local,
+                                           int j_base, Emit&& emit) {
   constexpr int W = CP / S;
   constexpr int B = W < 32 / S ? W : 32 / S;
   static_assert(W >= 2 && W % B == 0 && B % 2 == 0, "columns come in pairs");
@@ -98,7 +96,7 @@ __device__ __forceinline__ void sum_slices(const float* buf, int crank, uint32_t
   const uint32_t base = smem_u32(buf) + static_cast<uint32_t>(row_local) * 4u;
   uint32_t peer[S];
 #pragma unroll
-  for (int s = 0; s < S; ++s) peer[s] = mapa_shared(base, first + static_cast<uint32_t>(s));
+  for (int s = 0; s < S; ++s) peer[s] = mapa_shared(base, static_cast<uint32_t>(s));
 #pragma unroll 1
   for (int jj = 0; jj < W; jj += B) {
     const uint32_t off = static_cast<uint32_t>(j0 + jj) * 512u;
@@ -121,7 +119,7 @@ __device__ __forceinline__ void sum_slices(const float* buf, int crank, uint32_t
 template <int R, typename Emit>
 __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float* buf, int S,
                                                uint32_t crank, int row_local, bool epi,
-                                               Emit&& emit, uint32_t first = 0) {
+                                               Emit&& emit) {
   constexpr int CP = reduce_cols(R);
 #pragma unroll 1
   for (int pass = 0; pass < R / CP; ++pass) {
@@ -151,11 +149,11 @@ __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float*
     if (epi) {
       const int c = static_cast<int>(crank);
       if (S == 2)
-        sum_slices<CP, 2>(buf, c, first, row_local, pass * CP, emit);
+        sum_slices<CP, 2>(buf, c, row_local, pass * CP, emit);
       else if (S == 4)
-        sum_slices<CP, 4>(buf, c, first, row_local, pass * CP, emit);
+        sum_slices<CP, 4>(buf, c, row_local, pass * CP, emit);
       else
-        sum_slices<CP, 8>(buf, c, first, row_local, pass * CP, emit);
+        sum_slices<CP, 8>(buf, c, row_local, pass * CP, emit);
     }
     cluster_sync();
   }
@@ -167,7 +165,9 @@ __device__ __forceinline__ void cluster_reduce(uint32_t taddr, bool have, float*
 // that.  Against pulling (cluster_reduce) this saves a barrier and the round
 // trips of the loads; it needs `recv` to itself (push_bytes(R)) and the barrier
 // arrival of push_begin() at the kernel's start, which tells that a peer's
-// shared memory may be written.  Same order of the sums, same bits.
+// shared memory may be written.  Same order of the sums, same bits.  A cluster may
+// hold several groups of S CTAs side by side: `first` is the cluster rank of this
+// group's first CTA, `crank` the rank within the group.
 __host__ __device__ constexpr uint32_t push_bytes(int R) { return reduce_cols(R) * 512u; }
 
 // All threads of the CTA, once, before any work.

@@ -252,7 +252,7 @@ struct PairParams {
   int num_kb_main, num_kb_extra, R;
   int tiles_m, tiles_n, num_tiles, group_m;
   int atoms_k;
-  int vec_ok;  // rows of d allow 32-byte (2), 16-byte (1) or single (0) stores
+  int wide;  // rows of d start on 32 bytes (else on 16)
   void* d;
   long long ldd;
   uint32_t* status;
@@ -443,34 +443,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (lane == 0) mbar_arrive_cluster_relaxed(lead_acc_empty);
       if (m >= p.M) continue;
       T* out = reinterpret_cast<T*>(p.d) + static_cast<long long>(m) * p.ldd + n0;
-      if (p.vec_ok) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int n = c * 32 + q * 16;
-            uint32_t v[8];
+        for (int q = 0; q < 2; ++q) {
+          const int n = c * 32 + q * 16;
+          uint32_t v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              v[i] = pack2<T>(__uint_as_float(r[c][q * 16 + 2 * i]),
-                              __uint_as_float(r[c][q * 16 + 2 * i + 1]));
-            if (p.vec_ok == 2) {
-              if (n0 + n < p.N) st_global_32b(out + n, v);
-            } else {
-              if (n0 + n < p.N)
-                *reinterpret_cast<uint4*>(out + n) = make_uint4(v[0], v[1], v[2], v[3]);
-              if (n0 + n + 8 < p.N)
-                *reinterpret_cast<uint4*>(out + n + 8) = make_uint4(v[4], v[5], v[6], v[7]);
-            }
+          for (int i = 0; i < 8; ++i)
+            v[i] = pack2<T>(__uint_as_float(r[c][q * 16 + 2 * i]),
+                            __uint_as_float(r[c][q * 16 + 2 * i + 1]));
+          if (p.wide) {
+            if (n0 + n < p.N) st_global_32b(out + n, v);
+          } else {
+            if (n0 + n < p.N)
+              *reinterpret_cast<uint4*>(out + n) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (n0 + n + 8 < p.N)
+              *reinterpret_cast<uint4*>(out + n + 8) = make_uint4(v[4], v[5], v[6], v[7]);
           }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (n0 + c * 32 + i < p.N)
-              out[c * 32 + i] = static_cast<T>(__uint_as_float(r[c][i]));
-      }
+        }
     }
   }
 
@@ -513,15 +504,10 @@ int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
   if (!map_codes(&tw, a.wq, a.N, a.K, 128) || !map_codes(&tx, a.xq, a.M, a.K, NT) ||
       !map_atoms(&tws, a.ws, a.N, a.K) || !map_atoms(&txs, a.xs, a.M, a.K))
     return MLORA_ERR_INVALID_ARG;
-  if (a.R > 0) {
-    const int64_t r64 = (a.R + 63) / 64 * 64;
-    if (!make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, 128) ||
-        !make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, NT))
-      return MLORA_ERR_INVALID_ARG;
-  } else {
-    tw2 = tw;
-    tx2 = tx;
-  }
+  const int64_t r64 = (a.R + 63) / 64 * 64;
+  if (!make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, 128) ||
+      !make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, NT))
+    return MLORA_ERR_INVALID_ARG;
   SkinnyParams p;
   p.M = static_cast<int>(a.M);
   p.N = static_cast<int>(a.N);
@@ -570,15 +556,10 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   if (!map_codes(&tx, a.xq, a.M, a.K, kHalf) || !map_codes(&tw, a.wq, a.N, a.K, kHalf) ||
       !map_atoms(&txs, a.xs, a.M, a.K) || !map_atoms(&tws, a.ws, a.N, a.K))
     return MLORA_ERR_INVALID_ARG;
-  if (a.R > 0) {
-    const int64_t r64 = (a.R + 63) / 64 * 64;
-    if (!make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, kHalf) ||
-        !make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, kHalf))
-      return MLORA_ERR_INVALID_ARG;
-  } else {
-    tx2 = tx;
-    tw2 = tw;
-  }
+  const int64_t r64 = (a.R + 63) / 64 * 64;
+  if (!make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, kHalf) ||
+      !make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, kHalf))
+    return MLORA_ERR_INVALID_ARG;
   PairParams p;
   p.M = static_cast<int>(a.M);
   p.N = static_cast<int>(a.N);
@@ -593,10 +574,8 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   p.atoms_k = static_cast<int>((a.K + 127) / 128);
   p.d = a.d;
   p.ldd = a.ldd;
-  const uintptr_t d_addr = reinterpret_cast<uintptr_t>(a.d);
-  p.vec_ok = a.N % 16 == 0 && a.ldd % 16 == 0 && d_addr % 32 == 0 ? 2
-             : a.N % 8 == 0 && a.ldd % 8 == 0 && d_addr % 16 == 0 ? 1
-                                                                  : 0;
+  // (N and ldd are multiples of 8 and d starts on 16 bytes: the caller's checks)
+  p.wide = a.N % 16 == 0 && a.ldd % 16 == 0 && reinterpret_cast<uintptr_t>(a.d) % 32 == 0;
   p.status = device_status_ptr();
   auto kern = mx_pair_kernel<kBF16>;
   static std::atomic<int> max_pairs[64];

@@ -241,8 +241,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     float v[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = in[i] * p.scale;
-    if (p.out_rows != nullptr)
-      store_columns<T>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j, v, p.wide_rows != 0);
+    store_columns<T>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j, v, p.wide_rows != 0);
     if (p.out_t != nullptr) {
       T* dst = reinterpret_cast<T*>(p.out_t) + row + j * p.ld_t;
 #pragma unroll
@@ -251,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   };
   cluster_push_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have, recv,
                          p.splits, crank, row_local, epi, emit);
-  if (live && crank == 0 && p.out_rows != nullptr) {  // zero columns past R
+  if (live && crank == 0) {  // zero columns past R
     T* dst = reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows;
     for (long long j = R; j < p.ld_rows; j += 8)
       *reinterpret_cast<uint4*>(dst + j) = make_uint4(0, 0, 0, 0);
