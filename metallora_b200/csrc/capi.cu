@@ -773,9 +773,16 @@ bool make_tmap_2d_swizzled(CUtensorMap* map, CUtensorMapDataType dt, const void*
   cuuint64_t strides[1] = {row_stride_bytes};
   cuuint32_t box[2] = {box_inner, box_outer};
   cuuint32_t estr[2] = {1, 1};
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  // A host thread without a context yet (its memory came from an allocator's
+  // cache; a framework's backward thread): the driver call needs the one that the
+  // runtime's calls would bind by themselves.
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaSetDevice(current_device()) == cudaSuccess) r = encode();
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (code " + std::to_string(static_cast<int>(r)) +
               ") for dims " + std::to_string(inner) + "x" + std::to_string(outer) + " box " +
@@ -1282,6 +1289,8 @@ int check_qlora(int scheme, int64_t M, int64_t K, int64_t N, int64_t r, int64_t 
     if (dtype == MLORA_DTYPE_F32)
       return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base takes BF16 or F16 activations");
     if (K % 32) return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base needs K a multiple of 32");
+    if (M > (int64_t(1) << 31) - 256)  // row numbers are 32 bits up to the last tile's end
+      return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base takes fewer than 2^31 - 255 tokens");
     return MLORA_OK;
   }
   if (dtype != MLORA_DTYPE_BF16)

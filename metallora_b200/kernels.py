@@ -179,8 +179,19 @@ def _check_ckpt_out(ckpt, x2d) -> None:
 
 def _check_saved(saved_xa, r: int, M: int, dtype: torch.dtype) -> None:
     _check_2d("saved_xa", saved_xa, (rank_tile(r), (M + 7) // 8 * 8), dtype)
+    _need_cuda(saved_xa)
     if not saved_xa.is_contiguous():
         raise ShapeError("saved_xa must be contiguous")
+
+
+def _check_grad_out(da_out, db_out, r: int, r_orig: int, K: int, N: int) -> None:
+    if r != r_orig:
+        raise ShapeError("gradient accumulation buffers need a rank that is a multiple of 8")
+    for name, t, shp in (("da_out", da_out, (r, K)), ("db_out", db_out, (N, r))):
+        if t is None or t.dtype != torch.float32 or tuple(t.shape) != shp or \
+                not t.is_contiguous():
+            raise ShapeError(f"{name} must be a contiguous fp32 tensor of shape {shp}")
+    _need_cuda(da_out, db_out)
 
 
 def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | None,
@@ -227,12 +238,7 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
     flags = 0
     into = da_out is not None or db_out is not None
     if into:
-        if r != r_orig:
-            raise ShapeError("gradient accumulation buffers need a rank that is a multiple of 8")
-        for name, t, shp in (("da_out", da_out, (r, K)), ("db_out", db_out, (N, r))):
-            if t is None or t.dtype != torch.float32 or tuple(t.shape) != shp or \
-                    not t.is_contiguous():
-                raise ShapeError(f"{name} must be a contiguous fp32 tensor of shape {shp}")
+        _check_grad_out(da_out, db_out, r, r_orig, K, N)
         da, db = da_out, db_out
         flags = _lib.BWD_ACCUMULATE if accumulate else 0
     else:
@@ -291,13 +297,11 @@ def lora_linear_bwd_split(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tenso
     _check_2d("W0", w0, (N, K), dt)
     _check_2d("A", a, (r, K), dt)
     _check_2d("B", b, (N, r), dt)
-    for name, t, shp in (("da_out", da_out, (r, K)), ("db_out", db_out, (N, r))):
-        if t.dtype != torch.float32 or tuple(t.shape) != shp or not t.is_contiguous():
-            raise ShapeError(f"{name} must be a contiguous fp32 tensor of shape {shp}")
+    _check_grad_out(da_out, db_out, r, r, K, N)
     dy2d, w0, a, b = (t.contiguous() for t in (dy2d, w0, a, b))
     if ckpt is None:
         x2d = x2d.contiguous()
-    else:
+    if saved_xa is not None:
         _check_saved(saved_xa, r, M, dt)
     lib = _lib.load()
     dx = torch.empty((M, K), dtype=dt, device=x2d.device)
@@ -518,6 +522,9 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
     dt = _qlora_dtype(x2d, qw)
     M, K = x2d.shape if ckpt is None else (ckpt.rows, ckpt.shape[-1])
     N = dy2d.shape[1]
+    if tuple(qw.shape) != (N, K):
+        raise ShapeError(f"the quantised weight is {tuple(qw.shape)}, grad_output and x are of "
+                         f"{(N, K)}")
     r_orig = a.shape[0]
     a_p, b_p, alpha_p, r = _pad_rank(a, b, alpha)
     _check_2d("grad_output", dy2d, (M, N), dt)
@@ -526,15 +533,14 @@ def qlora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, qw, a: torch.Tensor,
     dy2d, a_p, b_p = dy2d.contiguous(), a_p.contiguous(), b_p.contiguous()
     if ckpt is None:
         x2d = x2d.contiguous()
-    else:
+    if saved_xa is not None:
         _check_saved(saved_xa, r, M, dt)
     lib = _lib.load()
     dx = dy2d.new_empty((M, K)) if need_dx else None
     flags = 0
     into = da_out is not None or db_out is not None
     if into:
-        if r != r_orig:
-            raise ShapeError("gradient accumulation buffers need a rank that is a multiple of 8")
+        _check_grad_out(da_out, db_out, r, r_orig, K, N)
         da, db = da_out, db_out
         flags = _lib.BWD_ACCUMULATE if accumulate else 0
     else:

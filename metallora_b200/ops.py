@@ -47,8 +47,11 @@ def _keep_x(ctx, x2d, ckpt) -> tuple:
 def _kept_x(ctx, x2d, scales):
     if ctx.x_meta is None:
         return x2d
-    from .quant import ActivationCheckpoint
-    return ActivationCheckpoint(x2d, scales, *ctx.x_meta)
+    from .quant import ActivationCheckpoint, empty_checkpoint
+    ckpt = ActivationCheckpoint(x2d, scales, *ctx.x_meta)
+    if x2d.stride(0) % 16:  # a saved-tensor hook (offloading) gave it back without its row gaps
+        ckpt.codes = empty_checkpoint(x2d).codes.copy_(x2d)
+    return ckpt
 
 
 def _cast_ab(a, b, dtype):
@@ -171,8 +174,8 @@ def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=No
     through that rounding).  ``checkpoint`` as for ``lora_forward``."""
     shp = x.shape
     x2d = x if len(shp) == 2 else x.reshape(-1, shp[-1])
-    if qweight.scheme == "mxfp4" and not (torch.is_grad_enabled() and
-                                          (x.requires_grad or A.requires_grad or B.requires_grad)):
+    grad = torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad)
+    if qweight.scheme == "mxfp4" and checkpoint is None and not grad:
         a, b = _compute if _compute is not None else _cast_ab(A, B, x.dtype)
         out = _k.qlora_linear_fwd(x2d, qweight, a, b, float(alpha))[0]
     else:

@@ -51,6 +51,26 @@ class QuantizedWeight:
     shape: tuple[int, int]
     lean: bool = False  # fused in-loop dequant (no transient bf16 copy of W per call)
 
+    def __post_init__(self):
+        if self.scheme == "mxfp4":
+            self._check_mxfp4_parts()
+
+    def _check_mxfp4_parts(self) -> None:
+        """The kernels size their reads by ``shape`` alone, so the parts have to fit it."""
+        _check_mxfp4(self.scheme, self.group, self.lean)
+        N, K = self.shape
+        for part, t, shp in (("codes", self.codes, (N, K // 2)),
+                             ("scales", self.scales, (N, -(-K // 32)))):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shp or not t.is_contiguous():
+                raise QuantizationError(f"mxfp4 {part}: expected contiguous {shp} uint8, got "
+                                        f"{tuple(t.shape)} {t.dtype}")
+        if K % 2:
+            raise QuantizationError("4-bit codes pack two per byte: in_features must be even")
+        if self.codes.device != self.scales.device:
+            raise QuantizationError("mxfp4 codes and scales are on different devices")
+        if self.zeros is not None:
+            raise QuantizationError("mxfp4 has no zero points")
+
     @property
     def code(self) -> int:
         return SCHEMES[self.scheme]
@@ -86,6 +106,16 @@ class QuantizedWeight:
             if not torch.cuda.is_current_stream_capturing():
                 object.__setattr__(self, "_prepared", t)
         return t
+
+    def check_table(self, table: torch.Tensor) -> None:
+        """Raises unless ``table`` has the size of this weight's ``prepared_scales``."""
+        N, K = self.shape
+        need = _lib.load().mlora_qlora_prepared_scales_bytes(self.code, N, K, self.group)
+        if table.dtype != torch.uint8 or table.numel() != need or not table.is_contiguous() or \
+                table.device != self.codes.device:
+            raise ShapeError(f"the prepared scales must be {need} contiguous bytes on "
+                             f"{self.codes.device}, got {tuple(table.shape)} {table.dtype} on "
+                             f"{table.device}")
 
     def state_dict(self) -> dict[str, torch.Tensor]:
         d = {"codes": self.codes, "scales": self.scales}
@@ -178,15 +208,6 @@ def from_reference_layout(scheme: str, codes, scales, zeros, shape, group,
     """Wraps tensors already in the reference layout (e.g. loaded from disk)."""
     if scheme not in SCHEMES:
         raise QuantizationError(f"unknown scheme {scheme!r}")
-    _check_mxfp4(scheme, int(group), lean)
-    if scheme == "mxfp4":
-        N, K = int(shape[0]), int(shape[1])
-        for part, t, shp in (("codes", codes, (N, K // 2)), ("scales", scales, (N, -(-K // 32)))):
-            if t.dtype != torch.uint8 or tuple(t.shape) != shp:
-                raise QuantizationError(f"mxfp4 {part}: expected {shp} uint8, got "
-                                        f"{tuple(t.shape)} {t.dtype}")
-        if zeros is not None:
-            raise QuantizationError("mxfp4 has no zero points")
     return _with_table(QuantizedWeight(scheme, codes.contiguous(), scales.contiguous(),
                                        None if zeros is None else zeros.contiguous(), int(group),
                                        (int(shape[0]), int(shape[1])), lean))

@@ -195,6 +195,8 @@ def _qweight(x, codes, scales, zeros, prepared, scheme, group, lean) -> Quantize
     qw = QuantizedWeight(scheme, codes, scales, zeros, int(group), (codes.shape[0], x.shape[-1]),
                          bool(lean))
     if prepared is not None:
+        if scheme == "mxfp4":
+            qw.check_table(prepared)
         object.__setattr__(qw, "_prepared", prepared)
     return qw
 

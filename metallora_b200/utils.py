@@ -87,7 +87,7 @@ def load_quantized_bases(model: nn.Module, path: str | Path, name: str = "base",
     """Installs the quantised bases saved by ``save_quantized_bases`` into the
     matching LoRA modules (their dense W0 is released, as ``quantize_base``
     does); each weight must match the module's [out, in] shape."""
-    from .quant import load_quantized
+    from .quant import _with_table, load_quantized
 
     load_path = Path(path) / f"{name}.safetensors"
     if not load_path.is_file():
@@ -101,9 +101,9 @@ def load_quantized_bases(model: nn.Module, path: str | Path, name: str = "base",
             raise AdapterError(f"{mname}: quantised base {tuple(qw.shape)} does not match "
                                f"({m.out_features}, {m.in_features})")
         dev = m.A.device
-        m.qweight = type(qw)(qw.scheme, qw.codes.to(dev), qw.scales.to(dev),
-                             None if qw.zeros is None else qw.zeros.to(dev), qw.group, qw.shape,
-                             qw.lean)
+        m.qweight = _with_table(type(qw)(qw.scheme, qw.codes.to(dev), qw.scales.to(dev),
+                                         None if qw.zeros is None else qw.zeros.to(dev), qw.group,
+                                         qw.shape, qw.lean))
         m.W0 = nn.Parameter(torch.empty(0, device=dev, dtype=m.W0.dtype), requires_grad=False)
     return model
 

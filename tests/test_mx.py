@@ -851,3 +851,235 @@ def test_empty_batch(cuda):
     qw = quant.quantize(w, "mxfp4")
     y, dx, da, db = _step(x[:0], qw, a, b, torch.empty(0, 24, dtype=BF16, device=cuda), "mxint8")
     assert y.shape == (0, 24) and dx.shape == (0, 64) and not da.any() and not db.any()
+
+
+# ------------------------------------------------- calls at the edges of the API --
+
+def test_weight_parts_refusals():
+    """The kernels size their reads by the shape: parts that do not fit it, or a
+    table of another size, are refused however the weight was made."""
+    codes, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(4, 2, dtype=torch.uint8)
+    ok = dict(scheme="mxfp4", codes=codes, scales=scales, zeros=None, group=32, shape=(4, 64))
+    qw = quant.QuantizedWeight(**ok)
+    for change in ({"codes": codes[:3]}, {"scales": scales[:, :1]}, {"scales": scales.float()},
+                   {"codes": codes.t().contiguous().t()}, {"zeros": scales}, {"group": 64},
+                   {"lean": True}, {"shape": (4, 66)},
+                   {"shape": (4, 65), "scales": torch.zeros(4, 3, dtype=torch.uint8)},
+                   {"scales": scales.to("meta")}):
+        with pytest.raises(QuantizationError):
+            quant.QuantizedWeight(**{**ok, **change})
+    qw.check_table(torch.zeros(512, dtype=torch.uint8))
+    for bad in (torch.zeros(511, dtype=torch.uint8), torch.zeros(512, dtype=torch.int8),
+                torch.zeros(1024, dtype=torch.uint8)[::2],
+                torch.zeros(512, dtype=torch.uint8, device="meta")):
+        with pytest.raises(ShapeError):
+            qw.check_table(bad)
+
+
+def test_gradient_buffer_refusals():
+    """Host tensors and wrong shapes are refused before any launch."""
+    saved = torch.zeros(16, 8, dtype=BF16)
+    with pytest.raises(DeviceError):
+        kernels._check_saved(saved, 8, 7, BF16)
+    for bad in (saved[:8], saved.half()):
+        with pytest.raises(ShapeError):
+            kernels._check_saved(bad, 8, 7, BF16)
+    da, db = torch.zeros(8, 64), torch.zeros(24, 8)
+    with pytest.raises(DeviceError):
+        kernels._check_grad_out(da, db, 8, 8, 64, 24)
+    for bad in ((None, db, 8, 8), (da, None, 8, 8), (da.half(), db, 8, 8), (da[:, :32], db, 8, 8),
+                (da, db.t().contiguous().t(), 8, 8), (da, db, 8, 7)):
+        with pytest.raises(ShapeError):
+            kernels._check_grad_out(*bad, 64, 24)
+
+
+def test_too_many_tokens_are_refused():
+    """Past 2^31 - 256 tokens a row number of the last tile would not fit 32 bits."""
+    lib = _lib.load()
+    buf = C.create_string_buffer(1 << 12)
+    p = (C.addressof(buf) + 255) // 256 * 256
+    mx = _lib.QUANT_MXFP4
+    for M in ((1 << 31) - 255, (1 << 31) - 1, 1 << 31):
+        rc = lib.mlora_qlora_forward_ex(p, mx, p, p, None, p, 32, p, p, p, None, M, 32, 8, 8, 1.0, 0, p,
+                                        1 << 10, None)
+        assert rc == _lib.MLORA_ERR_UNSUPPORTED, M
+
+
+@pytest.mark.gpu
+def test_more_refusals(cuda):
+    x, w, a, b, dy, saved = _grad_inputs(16, 64, 64, 8, BF16, cuda)
+    qw, c = quant.quantize(w, "mxfp4"), quant.checkpoint_activation(x)
+    with pytest.raises(ShapeError):  # a weight of other sizes than dy and x
+        kernels.qlora_linear_bwd(dy, x, quant.quantize(w[:32], "mxfp4"), a, b, 32.0, saved)
+    with pytest.raises(DeviceError):
+        ops.lora_backward(dy, c, a, b, 32.0, saved_xa=saved.cpu())
+    for bad in ("fp8", quant.checkpoint_activation(x[:8])):
+        with torch.no_grad(), pytest.raises(MetalLoRAError):
+            ops.qlora_forward(x, qw, a, b, 32.0, checkpoint=bad)
+    table = qw.prepared_scales()
+    with pytest.raises(ShapeError):
+        torch.ops.metal_lora.qlora_fwd(x, qw.codes, qw.scales, None, table[:256], "mxfp4", 32, False, a,
+                                       b, 32.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [1000, 1024])
+def test_checkpoint_through_saved_tensor_hooks(cuda, K):
+    """Offloaded to the host between forward and backward (which closes the gaps
+    between the rows of K 1000), a checkpoint gives the same gradients."""
+    x, w, a, b = _fwd_inputs(70, K, 72, 16, BF16, cuda)
+    dy = torch.randn(70, 72, generator=_gen(8)).to(BF16).to(cuda)
+    leaves = [t.requires_grad_(True) for t in (x, a, b)]
+    want = torch.autograd.grad(ops.lora_forward(x, w, a, b, 32.0, checkpoint="mxint8"), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = ops.lora_forward(x, w, a, b, 32.0, checkpoint="mxint8")
+    got = torch.autograd.grad(y, leaves, dy)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_loaded_bases_bring_their_table(cuda, tmp_path):
+    """A loaded MXFP4 base has its table before its first product, whichever
+    stream that runs on."""
+    from metallora_b200.utils import load_quantized_bases, save_quantized_bases
+
+    def net():
+        torch.manual_seed(3)
+        m = torch.nn.Sequential(LoRALinear(96, 136, rank=8, device=cuda, dtype=BF16))
+        with torch.no_grad():
+            m[0].W0.normal_(0, 0.1)
+            m[0].B.normal_(0, 0.1)
+        return m
+    m = net()
+    m[0].quantize_base("mxfp4")
+    save_quantized_bases(m, tmp_path)
+    m2 = load_quantized_bases(net(), tmp_path)
+    assert getattr(m2[0].qweight, "_prepared", None) is not None
+    x = _acts(33, 96, BF16, 1).to(cuda)
+    assert torch.equal(m(x), m2(x))
+
+
+@pytest.mark.gpu
+def test_host_threads(cuda):
+    """Two host threads, each on its stream, get the serial results."""
+    import threading
+    x, w, a, b = _fwd_inputs(200, 512, 264, 16, BF16, cuda)
+    dy = torch.randn(200, 264, generator=_gen(8)).to(BF16).to(cuda)
+    qw = quant.quantize(w, "mxfp4")
+    inputs = [(x, dy), (x.flip(0).contiguous(), dy.flip(0).contiguous())]
+    want = [_step(v, qw, a, b, d, "mxint8") for v, d in inputs]
+    torch.cuda.synchronize()
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = _step(inputs[i][0], qw, a, b, inputs[i][1], "mxint8")
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failed, failed
+    for i in range(2):
+        assert all(torch.equal(p, q) for p, q in zip(got[i], want[i]))
+
+
+@pytest.mark.gpu
+def test_thread_without_a_context(cuda):
+    """The first CUDA work of a host thread may be any of the calls: its buffers
+    come from the allocator's cache, so nothing before has bound a context."""
+    import threading
+    x, w, a, b, dy, saved = _grad_inputs(70, 1024, 72, 16, BF16, cuda)
+    qw, c = quant.quantize(w, "mxfp4"), quant.checkpoint_activation(x)
+    calls = [lambda: kernels.lora_linear_fwd(x, w, a, b, 32.0, save_xa=True),
+             lambda: kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True),
+             lambda: kernels.lora_linear_bwd(dy, c, w, a, b, 32.0, saved),
+             lambda: kernels.qlora_linear_bwd(dy, c, qw, a, b, 32.0, saved),
+             lambda: (quant.checkpoint_activation(x).dequantize(), qw.dequantize(BF16))]
+    for call in calls:
+        want, got = call(), []
+
+        def work():
+            try:
+                got.append(call())
+            except Exception as e:  # noqa: BLE001
+                got.append(e)
+        t = threading.Thread(target=work)
+        t.start()
+        t.join(60)
+        assert got and not isinstance(got[0], Exception), got
+        torch.cuda.synchronize()
+        # (rows past the tokens of saved_xa are not written)
+        assert all(torch.equal(p[:, :70], q[:, :70]) for p, q in zip(want, got[0]))
+
+
+@pytest.mark.gpu
+def test_captured_training_step(cuda):
+    """Forward and backward through autograd captured once, replayed on new inputs."""
+    x, w, a, b = _fwd_inputs(150, 288, 136, 16, BF16, cuda)
+    dy = torch.randn(150, 136, generator=_gen(8)).to(BF16).to(cuda)
+    qw = quant.quantize(w, "mxfp4")
+    want = [_step(v, qw, a, b, dy, "mxint8") for v in (x, x.flip(0).contiguous())]
+    leaves = [t.detach().clone().requires_grad_(True) for t in (x, a, b)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ops.qlora_forward(leaves[0], qw, leaves[1], leaves[2], 32.0, checkpoint="mxint8")
+        grads = torch.autograd.grad(y, leaves, dy)
+    for v, ref in ((x, want[0]), (x.flip(0), want[1]), (x, want[0])):
+        with torch.no_grad():
+            leaves[0].copy_(v)
+        _dirty(cuda)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p.detach(), q) for p, q in zip((y, *grads), ref))
+
+
+@pytest.mark.gpu
+def test_split_backward_of_a_checkpoint(cuda):
+    """The two-call backward gives the one call's results, added and written."""
+    x, w, a, b, dy, saved = _grad_inputs(150, 288, 136, 16, BF16, cuda)
+    c = quant.checkpoint_activation(x)
+    dx, da, db = kernels.lora_linear_bwd(dy, c, w, a, b, 32.0, saved)
+    for accumulate in (False, True):
+        ga, gb = torch.ones_like(da), torch.ones_like(db)
+        finish = kernels.lora_linear_bwd_split(dy, c, w, a, b, 32.0, saved, ga, gb, accumulate=accumulate)
+        _dirty(cuda)
+        assert torch.equal(finish(), dx)
+        assert torch.equal(ga, da + 1 if accumulate else da)
+        assert torch.equal(gb, db + 1 if accumulate else db)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 elements in x, y and dy: the last rows are those of the same
+    call on them alone, and gradients of a dy that is zero elsewhere theirs."""
+    M, K, N, r, n = 264200, 8192, 8200, 16, 200
+    g = torch.Generator(device=cuda).manual_seed(0)
+    x = torch.randn(M, K, device=cuda, dtype=BF16, generator=g)
+    w = torch.randn(N, K, device=cuda, dtype=BF16, generator=g) * 0.05
+    a = torch.randn(r, K, device=cuda, dtype=BF16, generator=g) / K ** 0.5
+    b = torch.randn(N, r, device=cuda, dtype=BF16, generator=g) * 0.1
+    qw = quant.quantize(w, "mxfp4")
+    tail = x[-n:].clone()
+    c = quant.checkpoint_activation(x)
+    ct = quant.checkpoint_activation(tail)
+    assert torch.equal(c.codes[-n:], ct.codes) and torch.equal(c.scales[:, M - n:M], ct.scales[:, :n])
+    assert torch.equal(c.dequantize()[-n:], ct.dequantize())
+    made = quant.empty_checkpoint(x)
+    y, saved = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True, ckpt_out=made)
+    assert torch.equal(made.codes, c.codes) and torch.equal(made.scales[:, :M], c.scales[:, :M])
+    del c
+    _fwd_check(y[-16:], tail[-16:], qw, a, b, 32.0)
+    del y, x
+    dy = torch.zeros(M, N, device=cuda, dtype=BF16)
+    dy[-n:] = torch.randn(n, N, device=cuda, dtype=BF16, generator=g) * 0.1
+    _, da, db = kernels.lora_linear_bwd(dy, made, None, a, b, 32.0, saved, need_dx=False)
+    # (adding exact zeros changes no partial sum: the bound of the n rows holds)
+    _grad_check(da, db, dy[-n:], _ckpt_values(ct), saved[:, M - n:M], a, b, 32.0)
+    assert _lib.device_status() == 0
