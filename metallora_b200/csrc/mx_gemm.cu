@@ -326,39 +326,58 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       uint32_t armed_parity[kPairStages];
       for (int s = 0; s < kPairStages; ++s) armed[s] = false, armed_parity[s] = 0;
       bool ok = true;
-      asm volatile("griddepcontrol.wait;" ::: "memory");
-      for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
-        int tm, tn;
-        pair_tile(p, tile, tm, tn);
-        const int m0 = tm * (2 * kHalf) + static_cast<int>(crank) * kHalf;
+      // (a row tile past the end lands on rows past the scale table: zeros)
+      auto load_w = [&](int kb, int tn, uint32_t s) {
+        uint8_t* st = smem + s * kPairStageBytes;
+        const uint32_t bar = lead_full + s * 8u;
         const int n0 = tn * kPairN + static_cast<int>(crank) * kHalf;
-        for (int kb = 0; kb < total_kb; ++kb) {
+        if (kb >= p.num_kb_main) {
+          tma_load_2d_pair(st + kWOff, &tm_w2, bar, (kb - p.num_kb_main) * kBK16, n0);
+        } else {
+          tma_load_2d_pair(st + kWOff, &tm_w, bar, kb * static_cast<int>(kRowBytes), n0);
+          tma_load_2d_pair(st + kWsOff, &tm_ws, bar, 0, 2 * tn * p.atoms_k + 2 * kb);
+          tma_load_2d_pair(st + kWsOff + kSfBytes, &tm_ws, bar, 0,
+                           (2 * tn + 1) * p.atoms_k + 2 * kb);
+        }
+      };
+      auto load_x = [&](int kb, int tm, uint32_t s) {
+        uint8_t* st = smem + s * kPairStageBytes;
+        const uint32_t bar = lead_full + s * 8u;
+        const int m0 = tm * (2 * kHalf) + static_cast<int>(crank) * kHalf;
+        if (kb >= p.num_kb_main) {
+          tma_load_2d_pair(st, &tm_x2, bar, (kb - p.num_kb_main) * kBK16, m0);
+        } else {
+          tma_load_2d_pair(st, &tm_x, bar, kb * static_cast<int>(kRowBytes), m0);
+          tma_load_2d_pair(st + kXsOff, &tm_xs, bar, 0, (m0 >> 7) * p.atoms_k + 2 * kb);
+        }
+      };
+      auto arm = [&](int kb, uint32_t s, uint32_t parity) {
+        if (!lead) return;
+        mbar_arrive_expect_tx(&full_bar[s],
+                              kb >= p.num_kb_main ? 4 * kPairOpBytes : 2 * kPairStageBytes);
+        armed[s] = true;
+        armed_parity[s] = parity;
+      };
+      // W, its scales and W2 do not come from the kernel before this one: the first
+      // tile's ring of them is on its way before the wait (every pair has a tile)
+      int tm, tn;
+      pair_tile(p, pair, tm, tn);
+      const int ahead = min(kPairStages, total_kb);
+      for (int i = 0; i < ahead; ++i) arm(i, i, 0), load_w(i, tn, i);
+      asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < ahead; ++i) load_x(i, tm, i);
+      if (ahead == kPairStages) phase = 1;
+      stage = ahead == kPairStages ? 0u : static_cast<uint32_t>(ahead);
+      for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
+        pair_tile(p, tile, tm, tn);
+        for (int kb = tile == pair ? ahead : 0; kb < total_kb; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) {
             ok = false;
             break;
           }
-          uint8_t* st = smem + stage * kPairStageBytes;
-          const bool extra = kb >= p.num_kb_main;
-          if (lead) {
-            mbar_arrive_expect_tx(&full_bar[stage], extra ? 4 * kPairOpBytes : 2 * kPairStageBytes);
-            armed[stage] = true;
-            armed_parity[stage] = phase;
-          }
-          const uint32_t bar = lead_full + stage * 8u;
-          if (extra) {
-            const int k0 = (kb - p.num_kb_main) * kBK16;
-            tma_load_2d_pair(st, &tm_x2, bar, k0, m0);
-            tma_load_2d_pair(st + kWOff, &tm_w2, bar, k0, n0);
-          } else {
-            const int k0 = kb * static_cast<int>(kRowBytes);
-            tma_load_2d_pair(st, &tm_x, bar, k0, m0);
-            tma_load_2d_pair(st + kWOff, &tm_w, bar, k0, n0);
-            // (a row tile past the end lands on rows past the table: zeros)
-            tma_load_2d_pair(st + kXsOff, &tm_xs, bar, 0, (m0 >> 7) * p.atoms_k + 2 * kb);
-            tma_load_2d_pair(st + kWsOff, &tm_ws, bar, 0, 2 * tn * p.atoms_k + 2 * kb);
-            tma_load_2d_pair(st + kWsOff + kSfBytes, &tm_ws, bar, 0,
-                             (2 * tn + 1) * p.atoms_k + 2 * kb);
-          }
+          arm(kb, stage, phase);
+          load_x(kb, tm, stage);
+          load_w(kb, tn, stage);
           if (++stage == kPairStages) stage = 0, phase ^= 1u;
         }
       }
