@@ -25,11 +25,12 @@ _DT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.flo
 
 # the current stream's handle without building a Stream object (~3 us a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream() -> int:
     if _raw_stream is not None:
-        return _raw_stream(torch.cuda.current_device())
+        return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
 
 
@@ -71,6 +72,11 @@ def _mx_ws_bytes(M: int, K: int, N: int, r: int, backward: bool, need_w: bool) -
         return lib.mlora_qlora_forward_workspace_bytes(*args)
     return (lib.mlora_qlora_backward_workspace_bytes(*args) if need_w
             else lib.mlora_qlora_lean_workspace_bytes(*args, 1))
+
+
+@functools.lru_cache(maxsize=256)
+def _bwd_ws_bytes(M: int, K: int, N: int, r: int, code: int) -> int:
+    return _lib.load().mlora_lora_backward_workspace_bytes(M, K, N, r, code)
 
 
 def is_metal_available() -> bool:
@@ -255,7 +261,7 @@ def lora_linear_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor | No
         if into:
             return dx, da, db
         return dx, da[:r_orig].contiguous(), db[:, :r_orig].contiguous()
-    ws = _workspace(lib.mlora_lora_backward_workspace_bytes(M, K, N, r, code), x2d.device)
+    ws = dy2d.new_empty(_bwd_ws_bytes(M, K, N, r, code), dtype=torch.uint8)
     tail = (_ptr(w0) if need_dx else None, _ptr(a_p), _ptr(b_p), _ptr(saved_xa), _ptr(dx), _ptr(da),
             _ptr(db), M, K, N, r, float(alpha_p), float(clip_value), code, flags, _ptr(ws),
             ws.numel(), _stream())
