@@ -682,9 +682,9 @@ int backward16(const void* dy, const void* x, const void* w0, const QGemmArgs* q
     ga.out_dtype = dtype;
     // in one call the weight-gradient kernel was launched just before: the
     // GEMM starts on SMs it frees; its X2 (s.dy.B) was complete before that
-    // kernel passed its own wait, and dy, W0 before the call.  (The kernel that
-    // takes a checkpoint lets no dependent start early.)
-    ga.overlap_prev = phase == kPhaseAll && ckpt == nullptr;
+    // kernel passed its own wait, and dy, W0 before the call (or, for a copy of W0
+    // made in it, before the first of these kernels)
+    ga.overlap_prev = phase == kPhaseAll;
     if ((rc = launch_gemm(ga, s))) return rc;
   }
 

@@ -112,8 +112,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // the dA kernel may start its set-up and stream its codes
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const bool is_db = static_cast<int>(blockIdx.x) >= p.ctas_u;
   const int splits = is_db ? p.splits_db : p.splits_u;
@@ -130,6 +128,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
 
   if (warp == 0) {
     if (elect_one()) {
+      grid_wait();  // nothing is read, and so nothing written, before
+      launch_dependents();  // the dA kernel may start its set-up and stream its codes
       uint32_t stage = 0, phase = 0;
       bool armed[S];
       uint32_t armed_parity[S];
@@ -315,13 +315,15 @@ int launch_typed(const LoraBwdArgs& a, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem_bytes(R);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   LaunchScope scope(kKindRank, stream);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tr, tc, tb, tx, p);
   if (e == cudaSuccess) e = cudaGetLastError();

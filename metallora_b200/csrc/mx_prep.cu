@@ -97,8 +97,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // the product may start its set-up and stream its weight
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int tile = static_cast<int>(blockIdx.x);
   const uint32_t crank = cluster_ctarank();
@@ -109,6 +107,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
 
   if (warp == 0) {
     if (elect_one()) {
+      grid_wait();  // nothing is read, and so nothing written, before
+      launch_dependents();  // the product may start its set-up and stream its weight
       uint32_t stage = 0, phase = 0;
       bool armed[S];
       uint32_t armed_parity[S];
@@ -306,13 +306,15 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem_bytes(R);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = static_cast<unsigned>(splits);
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   LaunchScope scope(kKindRank, stream);
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, ta, p);
   if (e == cudaSuccess) e = cudaGetLastError();

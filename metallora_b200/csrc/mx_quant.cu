@@ -92,6 +92,8 @@ __global__ void __launch_bounds__(kMxThreads)
     mx_quantize_blocks_kernel(const T* __restrict__ x, uint32_t blocks, uint32_t per_row,
                               uint8_t* __restrict__ codes, const MxScales sc,
                               uint8_t* __restrict__ atoms) {
+  grid_wait();
+  launch_dependents();
   const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
   uint32_t w[kOwn][16];
 #pragma unroll
@@ -128,6 +130,8 @@ template <int kBits, typename O>
 __global__ void __launch_bounds__(kMxThreads)
     mx_dequantize_blocks_kernel(const uint8_t* __restrict__ codes, const MxScales sc,
                                 uint32_t blocks, uint32_t per_row, O* __restrict__ out) {
+  grid_wait();
+  launch_dependents();
   const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
   uint32_t c[kOwn][kBits], byte[kOwn];
 #pragma unroll
@@ -347,6 +351,21 @@ int launched(const char* what) {
   return MLORA_OK;
 }
 
+// A block kernel, as a programmatic dependent of the kernel before it.
+template <typename... P, typename... A>
+void launch_blocks(void (*kern)(P...), unsigned grid, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kMxThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);  // (launched() has its error)
+}
+
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
 template <typename T>
@@ -400,15 +419,13 @@ int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K,
     if (atoms_made != nullptr) *atoms_made = t != nullptr;
     LaunchScope scope(kKindQuant, s);
     if (dtype == MLORA_DTYPE_BF16) {
-      const auto* xt = static_cast<const __nv_bfloat16*>(x);
-      bits == 4
-          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t)
-          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t);
+      using T = __nv_bfloat16;
+      launch_blocks(bits == 4 ? mx_quantize_blocks_kernel<4, T> : mx_quantize_blocks_kernel<8, T>, grid,
+                    s, static_cast<const T*>(x), blocks, per_row, c, sc, t);
     } else {
-      const auto* xt = static_cast<const __half*>(x);
-      bits == 4
-          ? mx_quantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t)
-          : mx_quantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(xt, blocks, per_row, c, sc, t);
+      using T = __half;
+      launch_blocks(bits == 4 ? mx_quantize_blocks_kernel<4, T> : mx_quantize_blocks_kernel<8, T>, grid,
+                    s, static_cast<const T*>(x), blocks, per_row, c, sc, t);
     }
     return launched("mx quantize");
   }
@@ -437,15 +454,13 @@ int launch_mx_dequantize(int bits, const void* codes, int64_t ld, const MxScales
     const auto* c = static_cast<const uint8_t*>(codes);
     LaunchScope scope(kKindQuant, s);
     if (out_dtype == MLORA_DTYPE_BF16) {
-      auto* o = static_cast<__nv_bfloat16*>(out);
-      bits == 4
-          ? mx_dequantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o)
-          : mx_dequantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o);
+      using O = __nv_bfloat16;
+      launch_blocks(bits == 4 ? mx_dequantize_blocks_kernel<4, O> : mx_dequantize_blocks_kernel<8, O>,
+                    grid, s, c, sc, blocks, per_row, static_cast<O*>(out));
     } else {
-      auto* o = static_cast<__half*>(out);
-      bits == 4
-          ? mx_dequantize_blocks_kernel<4><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o)
-          : mx_dequantize_blocks_kernel<8><<<grid, kMxThreads, 0, s>>>(c, sc, blocks, per_row, o);
+      using O = __half;
+      launch_blocks(bits == 4 ? mx_dequantize_blocks_kernel<4, O> : mx_dequantize_blocks_kernel<8, O>,
+                    grid, s, c, sc, blocks, per_row, static_cast<O*>(out));
     }
     return launched("mx dequantize");
   }

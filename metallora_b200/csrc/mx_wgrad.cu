@@ -135,7 +135,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         load_codes(kb_begin + i, stages + i * stage_bytes(R), &full_bar[i]);
         armed[i] = true;
       }
-      asm volatile("griddepcontrol.wait;" ::: "memory");
+      grid_wait();
+      // the dx GEMM, which reads nothing that this kernel writes, may take the SMs
+      // that it frees
+      launch_dependents();
       for (int i = 0; i < ahead; ++i)
         load_u(kb_begin + i, stages + i * stage_bytes(R), &full_bar[i]);
       if (ahead == S) phase = 1;

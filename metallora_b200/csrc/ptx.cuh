@@ -59,6 +59,21 @@ __device__ __forceinline__ void record_status(uint32_t* status, uint32_t code) {
   if (status != nullptr) atomicCAS(status, 0u, code);
 }
 
+// ------------------------------------------------ programmatic dependent launch --
+// A kernel launched as a programmatic dependent may start while the one before it
+// still runs.  grid_wait() returns once that one has completed and its writes are
+// visible (at once in any other launch); launch_dependents() allows the next one
+// to start when every CTA has called it.  A kernel calls them in this order, so
+// that whatever came before the kernel before it has completed too.
+
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+__device__ __forceinline__ void launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ------------------------------------------------------------------ mbarrier --
 
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {

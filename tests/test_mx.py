@@ -1083,3 +1083,32 @@ def test_offsets_past_32_bits(cuda):
     # (adding exact zeros changes no partial sum: the bound of the n rows holds)
     _grad_check(da, db, dy[-n:], _ckpt_values(ct), saved[:, M - n:M], a, b, 32.0)
     assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", [(1, 4096, 1024), (64, 1024, 1024), (700, 1024, 512)])
+def test_calls_that_follow_their_producers(cuda, M, K, N):
+    """Every call may start while the kernel before it still runs: one that reads
+    what the call just before it wrote gives the results of waiting in between."""
+    x, w, a, b = _fwd_inputs(M, K, N, 16, BF16, cuda)
+    dy = torch.randn(M, N, generator=_gen(8)).to(BF16).to(cuda)
+
+    def chain(wait):
+        def then(v):
+            if wait:
+                torch.cuda.synchronize()
+            return v
+        ck = then(quant.checkpoint_activation(then(x * 1)))
+        back = then(ck.dequantize())
+        qw = then(quant.quantize(then(w + 0), "mxfp4"))
+        y, saved = then(kernels.qlora_linear_fwd(back, qw, a, b, 32.0, save_xa=True))
+        made = quant.empty_checkpoint(back)
+        y2, _ = then(kernels.qlora_linear_fwd(back, qw, a, b, 32.0, save_xa=True, ckpt_out=made))
+        grads = then(kernels.qlora_linear_bwd(then(y2 * dy), made, qw, a, b, 32.0, saved))
+        again = then(kernels.lora_linear_bwd(then(dy * 1), then(quant.checkpoint_activation(back)),
+                                             then(qw.dequantize(BF16)), a, b, 32.0, saved))
+        return (ck.codes, back, y, y2, made.codes, *grads, *again)
+    want = chain(True)
+    for _ in range(20):
+        _dirty(cuda)
+        assert all(torch.equal(p, q) for p, q in zip(chain(False), want))
