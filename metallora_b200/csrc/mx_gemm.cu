@@ -251,7 +251,8 @@ constexpr uint32_t kPairTmemCols = 512;  // 256 accumulator, two sets of 8 + 16 
 struct PairParams {
   int M, N, K;
   int num_kb_main, num_kb_extra, R;
-  int tiles_m, tiles_n, num_tiles, group_m;
+  int tiles_m, tiles_n, group_m;
+  int whole, num_items;  // tiles of 256 columns, then the others in halves
   int atoms_k;
   int wide;  // rows of d start on 32 bytes (else on 16)
   void* d;
@@ -259,15 +260,19 @@ struct PairParams {
   uint32_t* status;
 };
 
-// Groups of group_m tile rows, tile rows fastest inside a group (the dense
-// kernel's order: the tiles in flight cover a compact block).
-__device__ __forceinline__ void pair_tile(const PairParams& p, int tile, int& tm, int& tn) {
+// Item -> tile row, first column, width.  Groups of group_m tile rows, tile rows
+// fastest inside a group (the dense kernel's order: the tiles in flight cover a
+// compact block).
+__device__ __forceinline__ void pair_item(const PairParams& p, int item, int& tm, int& n0, int& wide) {
+  const int over = item - p.whole;
+  const int tile = over < 0 ? item : p.whole + (over >> 1);
+  wide = over < 0 ? kPairN : kPairN / 2;
   const int per_group = p.group_m * p.tiles_n;
   const int g = tile / per_group;
   const int rem = tile - g * per_group;
   const int rows = min(p.group_m, p.tiles_m - g * p.group_m);
   tm = g * p.group_m + rem % rows;
-  tn = rem / rows;
+  n0 = rem / rows * kPairN + (over >= 0 && (over & 1) != 0 ? kPairN / 2 : 0);
 }
 
 template <bool kBF16>
@@ -328,17 +333,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       for (int s = 0; s < kPairStages; ++s) armed[s] = false, armed_parity[s] = 0;
       bool ok = true;
       // (a row tile past the end lands on rows past the scale table: zeros)
-      auto load_w = [&](int kb, int tn, uint32_t s) {
+      // (a CTA holds half of an item's columns; of a narrow item's copy, 128 rows
+      // too, the second half is not used)
+      auto load_w = [&](int kb, int n0, int wide, uint32_t s) {
         uint8_t* st = smem + s * kPairStageBytes;
         const uint32_t bar = lead_full + s * 8u;
-        const int n0 = tn * kPairN + static_cast<int>(crank) * kHalf;
+        const int row = n0 + static_cast<int>(crank) * (wide / 2);
         if (kb >= p.num_kb_main) {
-          tma_load_2d_pair(st + kWOff, &tm_w2, bar, (kb - p.num_kb_main) * kBK16, n0);
+          tma_load_2d_pair(st + kWOff, &tm_w2, bar, (kb - p.num_kb_main) * kBK16, row);
         } else {
-          tma_load_2d_pair(st + kWOff, &tm_w, bar, kb * static_cast<int>(kRowBytes), n0);
-          tma_load_2d_pair(st + kWsOff, &tm_ws, bar, 0, 2 * tn * p.atoms_k + 2 * kb);
+          tma_load_2d_pair(st + kWOff, &tm_w, bar, kb * static_cast<int>(kRowBytes), row);
+          tma_load_2d_pair(st + kWsOff, &tm_ws, bar, 0, (n0 >> 7) * p.atoms_k + 2 * kb);
           tma_load_2d_pair(st + kWsOff + kSfBytes, &tm_ws, bar, 0,
-                           (2 * tn + 1) * p.atoms_k + 2 * kb);
+                           ((n0 >> 7) + 1) * p.atoms_k + 2 * kb);
         }
       };
       auto load_x = [&](int kb, int tm, uint32_t s) {
@@ -360,25 +367,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         armed_parity[s] = parity;
       };
       // W, its scales and W2 do not come from the kernel before this one: the first
-      // tile's ring of them is on its way before the wait (every pair has a tile)
-      int tm, tn;
-      pair_tile(p, pair, tm, tn);
+      // item's ring of them is on its way before the wait (every pair has an item)
+      int tm, n0, wide;
+      pair_item(p, pair, tm, n0, wide);
       const int ahead = min(kPairStages, total_kb);
-      for (int i = 0; i < ahead; ++i) arm(i, i, 0), load_w(i, tn, i);
+      for (int i = 0; i < ahead; ++i) arm(i, i, 0), load_w(i, n0, wide, i);
       grid_wait();
       for (int i = 0; i < ahead; ++i) load_x(i, tm, i);
       if (ahead == kPairStages) phase = 1;
       stage = ahead == kPairStages ? 0u : static_cast<uint32_t>(ahead);
-      for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
-        pair_tile(p, tile, tm, tn);
-        for (int kb = tile == pair ? ahead : 0; kb < total_kb; ++kb) {
+      for (int item = pair; item < p.num_items && ok; item += num_pairs) {
+        pair_item(p, item, tm, n0, wide);
+        for (int kb = item == pair ? ahead : 0; kb < total_kb; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) {
             ok = false;
             break;
           }
           arm(kb, stage, phase);
           load_x(kb, tm, stage);
-          load_w(kb, tn, stage);
+          load_w(kb, n0, wide, stage);
           if (++stage == kPairStages) stage = 0, phase ^= 1u;
         }
       }
@@ -387,12 +394,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
   } else if (warp == 1) {
     if (lead && elect_one()) {
-      constexpr uint32_t idesc16 = make_idesc_f16(2 * kHalf, kPairN, false, false, kBF16);
       const uint32_t peer_empty = mapa_shared(smem_u32(empty_bar), 1);
       const uint32_t peer_acc_full = mapa_shared(smem_u32(acc_full), 1);
       uint32_t stage = 0, phase = 0, acc_phase = 0, set = 0;
       bool ok = true;
-      for (int tile = pair; tile < p.num_tiles && ok; tile += num_pairs) {
+      for (int item = pair; item < p.num_items && ok; item += num_pairs) {
+        const uint32_t wide = item < p.whole ? kPairN : kPairN / 2;
+        const uint32_t idesc16 = make_idesc_f16(2 * kHalf, wide, false, false, kBF16);
+        const uint32_t idesc4 = make_idesc_mxf4(2 * kHalf, wide, 0);
         if (!mbar_wait(acc_empty, acc_phase ^ 1u, p.status, kDevTimeoutAccEmpty)) break;
         acc_phase ^= 1u;
         tc_fence_after();
@@ -424,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             const int nk = min(4, (p.K - kb * kBK4 + 63) / 64);
             for (int k = 0; k < nk; ++k)
               umma_mxf4_pair(tmem, desc_kmajor_sw128(sx, k), desc_kmajor_sw128(sw, k),
-                             make_idesc_mxf4(2 * kHalf, kPairN, 2u * (k & 1)), sfa + 4 * (k >> 1),
+                             idesc4 | make_idesc_mxf4(0, 0, 2u * (k & 1)), sfa + 4 * (k >> 1),
                              sfb + 8 * (k >> 1), (kb | k) != 0 ? 1u : 0u);
           }
           umma_commit_pair(smem_u32(&empty_bar[stage]));
@@ -443,12 +452,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int col0 = warp >= 6 ? 128 : 0;
     const uint32_t lead_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
     uint32_t acc_phase = 0;
-    for (int tile = pair; tile < p.num_tiles; tile += num_pairs) {
-      int tm, tn;
-      pair_tile(p, tile, tm, tn);
+    for (int item = pair; item < p.num_items; item += num_pairs) {
+      int tm, n0, wide;
+      pair_item(p, item, tm, n0, wide);
       const int m = tm * (2 * kHalf) + static_cast<int>(crank) * kHalf +
                     static_cast<int>(quarter * 32 + lane);
-      const int n0 = tn * kPairN + col0;
+      n0 += col0;
       if (!mbar_wait(acc_full, acc_phase, p.status, kDevTimeoutAccFull)) break;
       acc_phase ^= 1u;
       __syncwarp();
@@ -461,7 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(lead_acc_empty);
-      if (m >= p.M) continue;
+      if (m >= p.M || col0 >= wide) continue;
       T* out = reinterpret_cast<T*>(p.d) + static_cast<long long>(m) * p.ldd + n0;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
@@ -589,7 +598,6 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   p.num_kb_extra = static_cast<int>((a.R + kBK16 - 1) / kBK16);
   p.tiles_m = static_cast<int>((a.M + 2 * kHalf - 1) / (2 * kHalf));
   p.tiles_n = static_cast<int>((a.N + kPairN - 1) / kPairN);
-  p.num_tiles = p.tiles_m * p.tiles_n;
   p.group_m = p.tiles_m < 8 ? p.tiles_m : 8;
   p.atoms_k = static_cast<int>((a.K + 127) / 128);
   p.d = a.d;
@@ -617,7 +625,14 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
     }
     if (dev < 64) max_pairs[dev].store(pairs, std::memory_order_release);
   }
-  const int grid = 2 * (p.num_tiles < pairs ? p.num_tiles : pairs);
+  // The tiles of the last wave go in halves of 128 columns where the pairs left
+  // without one can take them (256 tokens 4096 -> 4096: 17.5 us whole, 16.6 in
+  // halves; 512 tokens 4096 -> 11008: 25.7 and 24.6).  With more of them than that,
+  // some pairs would take two halves, 1.1 of a tile's time.
+  const int tiles = p.tiles_m * p.tiles_n, last = tiles % pairs;
+  p.whole = 2 * last <= pairs ? tiles - last : tiles;
+  p.num_items = p.whole + 2 * (tiles - p.whole);
+  const int grid = 2 * (p.num_items < pairs ? p.num_items : pairs);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kPairThreads);

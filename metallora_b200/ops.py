@@ -12,12 +12,12 @@ import torch
 
 from . import kernels as _k
 from .exceptions import ConfigurationError, ShapeError
+from .quant import ActivationCheckpoint, empty_checkpoint
 
 
 def _checkpoint(x2d, checkpoint):
     """(checkpoint of ``x2d`` or None, whether the forward has to fill it):
     ``checkpoint`` is None, "mxint8", or one the caller made of the same x."""
-    from .quant import ActivationCheckpoint, empty_checkpoint
     if checkpoint is None:
         return None, False
     if x2d.dtype not in (torch.bfloat16, torch.float16):
@@ -47,7 +47,6 @@ def _keep_x(ctx, x2d, ckpt) -> tuple:
 def _kept_x(ctx, x2d, scales):
     if ctx.x_meta is None:
         return x2d
-    from .quant import ActivationCheckpoint, empty_checkpoint
     ckpt = ActivationCheckpoint(x2d, scales, *ctx.x_meta)
     if x2d.stride(0) % 16:  # a saved-tensor hook (offloading) gave it back without its row gaps
         ckpt.codes = empty_checkpoint(x2d).codes.copy_(x2d)

@@ -1112,3 +1112,17 @@ def test_calls_that_follow_their_producers(cuda, M, K, N):
     for _ in range(20):
         _dirty(cuda)
         assert all(torch.equal(p, q) for p, q in zip(chain(False), want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("M,K,N,r", [(1290, 128, 2048, 16), (2600, 96, 2104, 24), (2570, 320, 4000, 8)])
+def test_forward_waves(cuda, dt, M, K, N, r):
+    """More tiles than half a wave (whole ones), whole ones and halves in one call."""
+    x, w, a, b = _fwd_inputs(M, K, N, r, dt, cuda)
+    qw = quant.quantize(w, "mxfp4")
+    _dirty(cuda)
+    y, _ = kernels.qlora_linear_fwd(x, qw, a, b, 32.0)
+    _fwd_check(y, x, qw, a, b, 32.0)
+    assert torch.equal(y[:200], kernels.qlora_linear_fwd(x[:200], qw, a, b, 32.0)[0])
+    assert _lib.device_status() == 0
