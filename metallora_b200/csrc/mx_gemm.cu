@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(kSkinnyThreads)
 // scale copies (they run in the MMAs' queue, 15 cycles each), 0.9 until the
 // accumulator is free again, 1-2 of waiting for operands (834 MB come from L2;
 // with one MMA in four issued, the copies alone take 53 us).  9.3 tiles a pair
-// leave the tenth wave a third full, and the chip's power cap holds it at
-// 1.63 GHz.  Tried and slower: copying a block's scales ahead of the MMAs of the
+// make nine waves and one of half tiles, and the chip's power cap holds it at
+// 1.62 GHz.  Tried and slower: copying a block's scales ahead of the MMAs of the
 // block before (107 against 95 us); no effect: raster groups of 1 to 32.
 constexpr int kPairStages = 6;
 constexpr int kHalf = 128;

@@ -1126,3 +1126,48 @@ def test_forward_waves(cuda, dt, M, K, N, r):
     _fwd_check(y, x, qw, a, b, 32.0)
     assert torch.equal(y[:200], kernels.qlora_linear_fwd(x[:200], qw, a, b, 32.0)[0])
     assert _lib.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_capture_with_joined_streams(cuda):
+    """Captured calls that come first, follow a copy or a fill, or follow a join of
+    two streams (their producer is on the other one) replay as they run."""
+    x, w, a, b = _fwd_inputs(70, 256, 136, 16, BF16, cuda)
+    dy = torch.randn(70, 136, generator=_gen(8)).to(BF16).to(cuda)
+    qw = quant.quantize(w, "mxfp4")
+    xs, side = x.clone(), torch.cuda.Stream()
+    buf, scratch = torch.empty_like(x), torch.empty(1 << 20, dtype=torch.uint8, device=cuda)
+
+    def run():
+        outs = [quant.checkpoint_activation(xs).codes]
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            buf.copy_(xs * 2)
+        scratch.zero_()
+        torch.cuda.current_stream().wait_stream(side)
+        y, saved = kernels.qlora_linear_fwd(buf, qw, a, b, 32.0, save_xa=True)
+        scratch.fill_(1)
+        c = quant.checkpoint_activation(buf)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            back = c.dequantize()
+            g = dy * 3
+        scratch.zero_()
+        torch.cuda.current_stream().wait_stream(side)
+        outs += [y, back, *kernels.qlora_linear_bwd(g, c, qw, a, b, 32.0, saved)]
+        return outs
+    want = [t.clone() for t in run()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(3):
+        _dirty(cuda)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+    xs.copy_(x.flip(0))
+    want = [t.clone() for t in run()]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
