@@ -120,7 +120,8 @@ MLORA_API size_t mlora_lora_backward_workspace_bytes(int64_t M, int64_t K, int64
  *   dx = dy.w0 + s (dy.b).a                      (optional: w0/dx may be NULL)
  *   da = s (dy.b)^T . x      -> fp32 [r, K]
  *   db = s dy^T . (x.a^T)    -> fp32 [N, r]
- * clipped elementwise to [-clip_value, clip_value] when clip_value > 0.
+ * clipped elementwise to [-clip_value, clip_value] when clip_value > 0 (a NaN
+ * stays a NaN).
  * Replaces ops.lora_backward (python/metal_lora/ops.py:117-155, which clips the
  * summed gradients, default 1.0) and kernels.lora_backward_metal
  * (kernels.py:569-612); dx is the autodiff gradient of ops.py:91-94.

@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     }
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      v[i] = p.clip > 0.f ? fminf(fmaxf(in[i], -p.clip), p.clip) : in[i];
+      v[i] = p.clip > 0.f ? clip_keep_nan(in[i], p.clip) : in[i];
     const long long at = row * p.r + j;
     if (p.accumulate || j + C > p.r) {
 #pragma unroll

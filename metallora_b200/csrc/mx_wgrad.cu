@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (j + i >= p.r) continue;
-      if (p.clip > 0.f) v[i] = fminf(fmaxf(v[i], -p.clip), p.clip);
+      if (p.clip > 0.f) v[i] = clip_keep_nan(v[i], p.clip);
       const long long at = (j + i) * p.ldo + prow;
       if (p.out16) {
         T* d = reinterpret_cast<T*>(p.out) + at;

@@ -437,6 +437,11 @@ __device__ __forceinline__ void st_global_32b(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
+// v bounded to [-c, c]; a NaN stays one (fminf and fmaxf alone would make it a bound).
+__device__ __forceinline__ float clip_keep_nan(float v, float c) {
+  return v != v ? v : fminf(fmaxf(v, -c), c);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 

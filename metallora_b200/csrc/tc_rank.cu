@@ -345,8 +345,8 @@ __global__ void __launch_bounds__(kThreads, 2)
   auto emit = [&](int j, float v0, float v1) {
     if (!live) return;
     if (clip) {
-      v0 = fminf(fmaxf(v0, -q.clip), q.clip);
-      v1 = fminf(fmaxf(v1, -q.clip), q.clip);
+      v0 = clip_keep_nan(v0, q.clip);
+      v1 = clip_keep_nan(v1, q.clip);
     }
     const bool w0 = j < q.r, w1 = j + 1 < q.r;
     if (q.out16) {  // gradients in the operands' 16-bit type (sum kept in fp32)

@@ -1,0 +1,89 @@
+"""Calls over MXFP4 bases and MXINT8 checkpoints that the formats' own tests leave
+out: derivatives that the operators do not define, values that are not finite, parts
+changed in place, every base with a checkpoint, products that are exact.
+"""
+import copy
+
+import numpy as np
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from metallora_b200 import _lib, kernels, ops, quant
+from metallora_b200.exceptions import AdapterError, ConfigurationError
+from metallora_b200.layers import LoRALinear
+from metallora_b200.trainer import LoRATrainer, TrainingConfig
+
+BF16, FP16, FP32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _cpu_weight(n=24, k=64):
+    return quant.from_reference_layout("mxfp4", torch.zeros((n, k // 2), dtype=torch.uint8),
+                                       torch.full((n, k // 32), 127, dtype=torch.uint8), None, (n, k), 32)
+
+
+def _inputs(M, K, N, r, dt, cuda, seed=0):
+    g = _gen(seed + M + K + N)
+    x = torch.randn(M, K, generator=g)
+    w = torch.randn(N, K, generator=g) * 0.05
+    a = torch.randn(r, K, generator=g) / K ** 0.5
+    b = torch.randn(N, r, generator=g) * 0.1
+    dy = torch.randn(M, N, generator=g) * 0.1
+    return tuple(t.to(dt).to(cuda) for t in (x, w, a, b, dy))
+
+
+# ------------------------------------------------------- values that are not finite --
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("r", [8, 64, 128])
+def test_clip_keeps_nan(cuda, dt, r):
+    """Clipping bounds numbers: a gradient that is NaN stays NaN, with the default
+    clip, from a checkpoint and from x itself, whatever the gradients' type."""
+    M, K, N = 150, 256, 72
+    x, w, a, b, dy = _inputs(M, K, N, r, dt, cuda)
+    x[3, 70] = float("nan")   # block 2 of row 3
+    x[9, 250] = float("inf")  # block 7 of row 9
+    _, saved = kernels.lora_linear_fwd(torch.nan_to_num(x, 0.0, 1.0), w, a, b, 32.0, save_xa=True)
+    c = quant.checkpoint_activation(x)
+    dead = torch.zeros(K, dtype=torch.bool, device=cuda)
+    dead[64:96] = dead[224:256] = True
+    dirty = dy.clone()
+    dirty[5, 11] = float("nan")
+    for gdt in (None, dt):
+        _, da0, db0 = kernels.lora_linear_bwd(dy, c, None, a, b, 32.0, saved, need_dx=False,
+                                              grad_dtype=gdt)
+        _, da, db = kernels.lora_linear_bwd(dy, c, None, a, b, 32.0, saved, clip_value=0.0625,
+                                            need_dx=False, grad_dtype=gdt)
+        assert da[:, dead].isnan().all() and torch.equal(db, db0.clamp(-0.0625, 0.0625))
+        assert torch.equal(da[:, ~dead], da0[:, ~dead].clamp(-0.0625, 0.0625))
+        _, da, db = kernels.lora_linear_bwd(dirty, c, None, a, b, 32.0, saved, clip_value=0.0625,
+                                            need_dx=False, grad_dtype=gdt)
+        assert db[11].isnan().all() and not torch.cat([db[:11], db[12:]]).isnan().any()
+        assert da.isnan().all()
+    da, db = ops.lora_backward(dirty, c, a, b, 32.0, saved_xa=saved)  # clips at 1
+    assert da.isnan().all() and db[11].isnan().all()
+    # from x itself
+    da, db = ops.lora_backward(dy, x, a, b, 32.0, saved_xa=saved)
+    cols = torch.zeros(K, dtype=torch.bool, device=cuda)
+    cols[70] = True
+    assert da[:, cols].isnan().all() and not da[:, ~cols & ~dead].isnan().any()
+    da, db = ops.lora_backward(dirty, x, a, b, 32.0, saved_xa=saved)
+    assert da.isnan().all() and db[11].isnan().all()
+
+
+@pytest.mark.gpu
+def test_clip_keeps_nan_fp32(cuda):
+    x, w, a, b, dy = _inputs(40, 64, 72, 8, FP32, cuda)
+    dy[5, 11] = float("nan")
+    da, db = ops.lora_backward(dy, x, a, b, 16.0)
+    assert da.isnan().all() and db[11].isnan().all()
+
+
+def _files(tmp_path, shapes):
+    weights = {name: _cpu_weight(n, k) for name, (n, k) in shapes.items()}
+    quant.save_quantized(weights, tmp_path / "base.safetensors")
