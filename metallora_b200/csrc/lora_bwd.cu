@@ -210,7 +210,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       for (int i = 0; i < C; ++i) {
         const T h = static_cast<T>(v[i]);
         hi[i * p.ld_t] = h;
-        lo[i * p.ld_t] = static_cast<T>(v[i] - static_cast<float>(h));
+        // (an infinity has no second part: what is left of it would make a NaN)
+        const float f = static_cast<float>(h);
+        lo[i * p.ld_t] = static_cast<T>(isfinite(f) ? v[i] - f : 0.f);
       }
       return;
     }

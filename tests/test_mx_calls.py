@@ -84,6 +84,28 @@ def test_clip_keeps_nan_fp32(cuda):
     assert da.isnan().all() and db[11].isnan().all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("r", [8, 64])
+def test_infinite_intermediate(cuda, dt, r):
+    """An infinite s dy B, made by an infinite dy or by passing fp16's largest number,
+    is an infinity with its sign in dA as well."""
+    M, K, N = 70, 128, 64
+    x, w, a, b, dy = _inputs(M, K, N, r, dt, cuda)
+    x = x.abs() + 0.5
+    dy.zero_()
+    dy[4] = 100.0 if dt == FP16 else float("inf")
+    b[:, 0], b[:, 1] = 50.0, -50.0  # 4 * 64 * 100 * 50 is 20 times fp16's largest
+    b[:, 2:] = 0.25                 # 4 * 64 * 100 / 4 is a tenth of it
+    _, saved = kernels.lora_linear_fwd(x, w, a, b, 4.0 * r, save_xa=True)
+    c = quant.checkpoint_activation(x)
+    for clip, big in ((0.0, float("inf")), (1.0, 1.0)):
+        _, da, _ = kernels.lora_linear_bwd(dy, c, None, a, b, 4.0 * r, saved, clip_value=clip,
+                                           need_dx=False)
+        assert (da[0] == big).all() and (da[1] == -big).all()
+        assert torch.isfinite(da[2:]).all() if dt == FP16 else (da[2:] == big).all()
+
+
 def _files(tmp_path, shapes):
     weights = {name: _cpu_weight(n, k) for name, (n, k) in shapes.items()}
     quant.save_quantized(weights, tmp_path / "base.safetensors")
