@@ -88,14 +88,40 @@ class QuantizedWeight:
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         return dequantize(self, dtype)
 
+    def _kept_table(self) -> torch.Tensor | None:
+        """The kept scale table, if it is of these scales and zeros as they are now."""
+        kept = getattr(self, "_table_of", None)
+        if kept is None or self._prepared.device != self.codes.device:
+            return None
+        s, z = self.scales, self.zeros
+        # (what is written over in inference mode keeps no count of it)
+        if kept[0] is s and kept[1] is z and kept[2] == (-1 if s.is_inference() else s._version) and \
+                (z is None or kept[3] == (-1 if z.is_inference() else z._version)):
+            return self._prepared
+        return None
+
+    def _keep_table(self, table: torch.Tensor) -> None:
+        s, z = self.scales, self.zeros
+        self._prepared = table
+        self._table_of = (s, z, -1 if s.is_inference() else s._version,
+                          -1 if z is None or z.is_inference() else z._version)
+
+    def __getstate__(self):
+        """A copy's tensors count their writes anew: it makes its own table."""
+        return {k: v for k, v in self.__dict__.items() if k not in ("_prepared", "_table_of")}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        _with_table(self)
+
     def prepared_scales(self) -> torch.Tensor:
         """The TMA-ready scale table the GPU kernels read: [groups, rows rounded
         to 4], or for MXFP4 the product's blocks of 128 rows x 128 features
-        (built once, on first use -- for MXFP4 when the weight is made -- and
-        kept with the weight; a table built while a graph is captured belongs to
-        that graph and is not kept)."""
-        t = getattr(self, "_prepared", None)
-        if t is None or t.device != self.codes.device:
+        (built on first use -- for MXFP4 when the weight is made -- and kept with
+        the weight until its scales or zeros are written over or replaced; a table
+        built while a graph is captured belongs to that graph and is not kept)."""
+        t = self._kept_table()
+        if t is None:
             lib = _lib.load()
             N, K = self.shape
             nbytes = lib.mlora_qlora_prepared_scales_bytes(self.code, N, K, self.group)
@@ -104,7 +130,7 @@ class QuantizedWeight:
                                                 K, self.group, _ptr(t), _stream())
             _lib.check(st, "mlora_qlora_prepare_scales")
             if not torch.cuda.is_current_stream_capturing():
-                object.__setattr__(self, "_prepared", t)
+                self._keep_table(t)
         return t
 
     def check_table(self, table: torch.Tensor) -> None:
@@ -177,7 +203,7 @@ def _quantize_mxfp4(w: torch.Tensor) -> QuantizedWeight:
                                   scales.data_ptr(), table.data_ptr(), _stream())
     _lib.check(st, "mlora_quantize_mxfp4")
     qw = QuantizedWeight("mxfp4", codes, scales, None, 32, (N, K))
-    object.__setattr__(qw, "_prepared", table)
+    qw._keep_table(table)
     return qw
 
 

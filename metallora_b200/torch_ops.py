@@ -197,7 +197,7 @@ def _qweight(x, codes, scales, zeros, prepared, scheme, group, lean) -> Quantize
     if prepared is not None:
         if scheme == "mxfp4":
             qw.check_table(prepared)
-        object.__setattr__(qw, "_prepared", prepared)
+        qw._keep_table(prepared)
     return qw
 
 
@@ -285,7 +285,7 @@ def qlora_linear(x: torch.Tensor, qweight: QuantizedWeight, a: torch.Tensor, b: 
     """``y`` of ``torch.ops.metal_lora.qlora_fwd`` for a ``QuantizedWeight``:
     the traceable form of ``ops.qlora_forward``."""
     qw = qweight
-    prepared = getattr(qw, "_prepared", None)
+    prepared = getattr(qw, "_prepared", None) if torch.compiler.is_compiling() else qw._kept_table()
     if prepared is None and qw.codes.is_cuda:
         prepared = qw.prepared_scales()
     return torch.ops.metal_lora.qlora_fwd(x, qw.codes, qw.scales, qw.zeros, prepared, qw.scheme,

@@ -106,6 +106,43 @@ def test_infinite_intermediate(cuda, dt, r):
         assert torch.isfinite(da[2:]).all() if dt == FP16 else (da[2:] == big).all()
 
 
+# ------------------------------------------------------------------ the scale table --
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scheme", ["mxfp4", "nf4", "int4", "int8"])
+def test_parts_changed_in_place(cuda, scheme):
+    """A weight whose scales are written over multiplies by the new ones."""
+    dt = BF16
+    x, w, a, b, dy = _inputs(4, 256, 72, 8, dt, cuda)
+    qw = quant.quantize(w, scheme)
+    other = quant.quantize(w * 4, scheme)
+    kernels.qlora_linear_fwd(x, qw, a, b, 16.0)
+    for part in ("codes", "scales", "zeros"):
+        if getattr(qw, part) is not None:
+            getattr(qw, part).copy_(getattr(other, part))
+    for M in (1, 4):
+        want = kernels.qlora_linear_fwd(x[:M], quant.quantize(w * 4, scheme), a, b, 16.0)[0]
+        assert torch.equal(kernels.qlora_linear_fwd(x[:M], qw, a, b, 16.0)[0], want)
+    with torch.inference_mode():
+        q2 = quant.quantize(w, scheme)
+        y = kernels.qlora_linear_fwd(x, q2, a, b, 16.0)[0]
+    for _ in range(2):  # (and out of it)
+        assert torch.equal(y, kernels.qlora_linear_fwd(x, q2, a, b, 16.0)[0])
+    # a copy has scales of its own
+    twin, y = copy.deepcopy(qw), kernels.qlora_linear_fwd(x, qw, a, b, 16.0)[0]
+    assert torch.equal(kernels.qlora_linear_fwd(x, twin, a, b, 16.0)[0], y)
+    for part in ("codes", "scales", "zeros"):
+        if getattr(qw, part) is not None:
+            getattr(twin, part).copy_(getattr(q2, part))
+    assert torch.equal(kernels.qlora_linear_fwd(x, twin, a, b, 16.0)[0],
+                       kernels.qlora_linear_fwd(x, q2, a, b, 16.0)[0])
+    assert torch.equal(kernels.qlora_linear_fwd(x, qw, a, b, 16.0)[0], y)
+    # other tensors in the place of the parts
+    qw.codes, qw.scales, qw.zeros = twin.codes, twin.scales, twin.zeros
+    assert torch.equal(kernels.qlora_linear_fwd(x, qw, a, b, 16.0)[0],
+                       kernels.qlora_linear_fwd(x, q2, a, b, 16.0)[0])
+
+
 def _files(tmp_path, shapes):
     weights = {name: _cpu_weight(n, k) for name, (n, k) in shapes.items()}
     quant.save_quantized(weights, tmp_path / "base.safetensors")
