@@ -209,10 +209,11 @@ def _quantize_mxfp4(w: torch.Tensor) -> QuantizedWeight:
 
 def _with_table(qw: QuantizedWeight) -> QuantizedWeight:
     """An MXFP4 weight on the GPU gets its table at once, in the order of its codes
-    on the stream: no later call, on whatever stream, is the one that makes it."""
+    on its device's stream: no later call, on whatever stream, is the one that makes
+    it."""
     if qw.scheme == "mxfp4" and qw.codes.is_cuda:
-        _need_current(qw.codes, qw.scales)
-        qw.prepared_scales()
+        with torch.cuda.device(qw.codes.device):
+            qw.prepared_scales()
     return qw
 
 

@@ -146,3 +146,40 @@ def test_parts_changed_in_place(cuda, scheme):
 def _files(tmp_path, shapes):
     weights = {name: _cpu_weight(n, k) for name, (n, k) in shapes.items()}
     quant.save_quantized(weights, tmp_path / "base.safetensors")
+
+
+# ----------------------------------------------------------------------- settings --
+
+def test_table_of_another_device(monkeypatch):
+    """A weight that is loaded onto a GPU which is not the current one gets its table
+    there, in that device's context."""
+    events = []
+
+    class Guard:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            events.append(("in", self.device))
+
+        def __exit__(self, *exc):
+            events.append(("out", self.device))
+
+    class Weight:
+        scheme = "mxfp4"
+
+        class codes:
+            is_cuda, device = True, torch.device("cuda:1")
+
+            @staticmethod
+            def get_device():
+                return 1
+
+        scales = codes
+
+        def prepared_scales(self):
+            events.append("table")
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    quant._with_table(Weight())
+    assert events == [("in", torch.device("cuda:1")), "table", ("out", torch.device("cuda:1"))]
