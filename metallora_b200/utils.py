@@ -93,13 +93,16 @@ def load_quantized_bases(model: nn.Module, path: str | Path, name: str = "base",
     if not load_path.is_file():
         raise AdapterError(f"quantised base file not found: {load_path}")
     modules = dict(_lora_modules(model))
-    for mname, qw in load_quantized(load_path, lean=lean).items():
+    weights = load_quantized(load_path, lean=lean)
+    for mname, qw in weights.items():  # all of them before any module changes
         m = modules.get(mname)
         if m is None:
             raise AdapterError(f"no LoRA module named {mname!r} in the model")
         if tuple(qw.shape) != (m.out_features, m.in_features):
             raise AdapterError(f"{mname}: quantised base {tuple(qw.shape)} does not match "
                                f"({m.out_features}, {m.in_features})")
+    for mname, qw in weights.items():
+        m = modules[mname]
         dev = m.A.device
         m.qweight = _with_table(type(qw)(qw.scheme, qw.codes.to(dev), qw.scales.to(dev),
                                          None if qw.zeros is None else qw.zeros.to(dev), qw.group,

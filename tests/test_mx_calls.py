@@ -183,3 +183,25 @@ def test_table_of_another_device(monkeypatch):
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
     quant._with_table(Weight())
     assert events == [("in", torch.device("cuda:1")), "table", ("out", torch.device("cuda:1"))]
+
+
+def test_loading_is_all_or_nothing(tmp_path):
+    """A file that does not fit the model leaves every module as it was."""
+    from metallora_b200.utils import load_quantized_bases
+
+    def net():
+        return torch.nn.Sequential(LoRALinear(64, 24, rank=8), LoRALinear(64, 40, rank=8))
+    for second in ((48, 64), (40, 96)):
+        _files(tmp_path, {"0": (24, 64), "1": second})
+        m = net()
+        with pytest.raises(AdapterError):
+            load_quantized_bases(m, tmp_path)
+        assert all(l.qweight is None and l.W0.numel() for l in m)
+    _files(tmp_path, {"0": (24, 64), "other": (40, 64)})
+    m = net()
+    with pytest.raises(AdapterError):
+        load_quantized_bases(m, tmp_path)
+    assert all(l.qweight is None and l.W0.numel() for l in m)
+    _files(tmp_path, {"0": (24, 64), "1": (40, 64)})
+    m = load_quantized_bases(net(), tmp_path)
+    assert all(l.qweight is not None and not l.W0.numel() for l in m)
