@@ -9,6 +9,7 @@ tensor-core GEMMs, see ``kernels``).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import kernels as _k
 from .exceptions import ConfigurationError, ShapeError
@@ -164,6 +165,11 @@ class _QLoRALinearFn(torch.autograd.Function):
                 db if ctx.needs_input_grad[2] else None, None, None, None, None, None)
 
 
+def _forward_mode() -> bool:
+    """Whether a forward-mode level is open (if that cannot be told: True)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=None,  # noqa: N803
                   checkpoint=None):
     """LoRA forward over a quantised base (``quant.QuantizedWeight``):
@@ -174,7 +180,9 @@ def qlora_forward(x, qweight, A, B, alpha: float = 16.0, _compute=None, _sink=No
     shp = x.shape
     x2d = x if len(shp) == 2 else x.reshape(-1, shp[-1])
     grad = torch.is_grad_enabled() and (x.requires_grad or A.requires_grad or B.requires_grad)
-    if qweight.scheme == "mxfp4" and checkpoint is None and not grad:
+    # the short path has no place for a forward-mode tangent, which no_grad does not
+    # switch off (the function below refuses one)
+    if qweight.scheme == "mxfp4" and checkpoint is None and not grad and not _forward_mode():
         a, b = _compute if _compute is not None else _cast_ab(A, B, x.dtype)
         out = _k.qlora_linear_fwd(x2d, qweight, a, b, float(alpha))[0]
     else:

@@ -36,6 +36,29 @@ def _inputs(M, K, N, r, dt, cuda, seed=0):
     return tuple(t.to(dt).to(cuda) for t in (x, w, a, b, dy))
 
 
+# ----------------------------------------------------------------- derivatives --
+
+@pytest.mark.parametrize("which", ["x", "a", "b"])
+def test_forward_mode_is_refused(monkeypatch, which):
+    """The operator has no forward-mode rule: a dual tensor is refused, with
+    gradients switched off too, and never answered without its tangent."""
+    qw = _cpu_weight()
+    monkeypatch.setattr(kernels, "qlora_linear_fwd",
+                        lambda x, q, a, b, alpha, save_xa=False, ckpt_out=None: (
+                            x.new_zeros((x.shape[0], q.shape[0])),
+                            x.new_zeros((16, (x.shape[0] + 7) // 8 * 8)) if save_xa else None))
+    t = {"x": torch.randn(6, 64, dtype=BF16), "a": torch.randn(8, 64, dtype=BF16),
+         "b": torch.randn(24, 8, dtype=BF16)}
+    assert ops.qlora_forward(t["x"], qw, t["a"], t["b"]).shape == (6, 24)
+    with forward_ad.dual_level():
+        dual = {**t, which: forward_ad.make_dual(t[which], torch.ones_like(t[which]))}
+        with pytest.raises(NotImplementedError):
+            ops.qlora_forward(dual["x"], qw, dual["a"], dual["b"])
+        with torch.no_grad(), pytest.raises(NotImplementedError):
+            ops.qlora_forward(dual["x"], qw, dual["a"], dual["b"])
+        assert ops.qlora_forward(t["x"], qw, t["a"], t["b"]).shape == (6, 24)
+
+
 # ------------------------------------------------------- values that are not finite --
 
 @pytest.mark.gpu
