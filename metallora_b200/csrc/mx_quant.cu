@@ -79,19 +79,35 @@ __device__ __forceinline__ uint8_t* scale_of(const MxScales& sc, uint32_t block,
   return sc.data + (static_cast<int64_t>(b >> 2) * sc.rows + row) * 4 + (b & 3u);
 }
 
+// Plain loads, which stay behind grid_wait(): the block kernels start while the
+// kernel that writes their input may still run, so it is not read-only for their
+// whole life, as the read-only path (ld.global.nc, __ldg) wants.
 __device__ __forceinline__ void ld_global_32b(const void* p, uint32_t* v) {
-  asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]),
                  "=r"(v[6]), "=r"(v[7])
-               : "l"(p));
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ uint4 ld_global_16b(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_global_byte(const void* p) {
+  uint32_t v;
+  asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // x, codes: [blocks] of 32 values, without gaps between the rows.
 template <int kBits, typename T>
 __global__ void __launch_bounds__(kMxThreads)
-    mx_quantize_blocks_kernel(const T* __restrict__ x, uint32_t blocks, uint32_t per_row,
-                              uint8_t* __restrict__ codes, const MxScales sc,
-                              uint8_t* __restrict__ atoms) {
+    mx_quantize_blocks_kernel(const T* x, uint32_t blocks, uint32_t per_row, uint8_t* codes,
+                              const MxScales sc, uint8_t* atoms) {
   grid_wait();
   launch_dependents();
   const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
@@ -128,8 +144,8 @@ __global__ void __launch_bounds__(kMxThreads)
 
 template <int kBits, typename O>
 __global__ void __launch_bounds__(kMxThreads)
-    mx_dequantize_blocks_kernel(const uint8_t* __restrict__ codes, const MxScales sc,
-                                uint32_t blocks, uint32_t per_row, O* __restrict__ out) {
+    mx_dequantize_blocks_kernel(const uint8_t* codes, const MxScales sc, uint32_t blocks,
+                                uint32_t per_row, O* out) {
   grid_wait();
   launch_dependents();
   const uint32_t b0 = blockIdx.x * (kMxThreads * kOwn) + threadIdx.x;
@@ -138,9 +154,9 @@ __global__ void __launch_bounds__(kMxThreads)
   for (int i = 0; i < kOwn; ++i) {
     const uint32_t b = b0 + i * kMxThreads;
     if (b >= blocks) continue;
-    byte[i] = __ldg(scale_of(sc, b, per_row));
+    byte[i] = ld_global_byte(scale_of(sc, b, per_row));
     if constexpr (kBits == 4) {
-      const uint4 q = __ldg(reinterpret_cast<const uint4*>(codes) + b);
+      const uint4 q = ld_global_16b(codes + static_cast<int64_t>(b) * 16);
       c[i][0] = q.x, c[i][1] = q.y, c[i][2] = q.z, c[i][3] = q.w;
     } else {
       ld_global_32b(codes + static_cast<int64_t>(b) * 32, c[i]);
