@@ -64,6 +64,7 @@ struct PrepParams {
   uint8_t* q8_scales;  // words [ceil(K/128), rows8]
   long long rows8;
   int wide_rows;  // the row output starts on 32 bytes (its rows are 128 apart)
+  uint32_t no_max;  // all ones: the bits of no block's maximum
   uint32_t* status;
 };
 
@@ -179,9 +180,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       // The stage is free once its words are in registers, and they are once the
       // whole warp's maximum is known: an arrive after the loads alone overtook
       // them (a late load then read the tile copied next; seen in 1 of 8 runs of
-      // 4096 x 4096).  The maximum's bits are never all set.
+      // 4096 x 4096).  So the arrive hangs on that maximum.  It is never all ones, but
+      // no_max is a parameter: no compiler can tell, and drop the dependence.
       const uint32_t amax = block_amax<T>(w);
-      if (__reduce_max_sync(0xffffffffu, amax) != 0xFFFFFFFFu && lane_id() == 0)
+      if (__reduce_max_sync(0xffffffffu, amax) != p.no_max && lane_id() == 0)
         mbar_arrive(&empty_bar[stage]);
       if (++stage == S) stage = 0, phase ^= 1u;
 
@@ -292,6 +294,7 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   p.q8_scales = static_cast<uint8_t*>(a.q8_scales);
   p.rows8 = (a.M + 3) / 4 * 4;
   p.wide_rows = reinterpret_cast<uintptr_t>(a.out_rows) % 32 == 0;
+  p.no_max = 0xFFFFFFFFu;
   p.status = device_status_ptr();
   const int64_t tiles = (a.M + 127) / 128;
   // the plain rank projection's split, so that s x A^T has the same bits with and

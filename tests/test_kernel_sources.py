@@ -46,3 +46,12 @@ def test_programmatic_dependents_load_coherently():
         assert "__ldg(" not in body and "ld.global.nc" not in text, (file, name)
         assert "__restrict__" not in head, (file, name)
     assert seen >= 5
+
+
+def test_stage_release_depends_on_the_loads():
+    """The quantising warps hand a stage back by an arrive that hangs on what they
+    loaded.  Compared with a constant, the condition (a maximum's bits are never all
+    ones) could be folded away, and with it the order."""
+    body = next(k[3] for k in KERNELS if k[1] == "mx_prep_kernel")
+    arrive = re.search(r"if \(__reduce_max_sync\([^;]*?\) != ([\w.]+)[^;]*\)\s*mbar_arrive\(", body)
+    assert arrive and arrive.group(1).startswith("p."), arrive
