@@ -126,9 +126,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       tile < (is_db ? p.tiles_db : p.tiles_u) ? min(num_kb, kb_begin + per) : kb_begin;
   const bool has_work = kb_begin < kb_end;
 
+  // Nothing is read, and so nothing written, before the kernel before this one is
+  // through.  Each role waits for that itself, so that the limits of its bounded waits
+  // count from there: that kernel may be anyone's, and take its time.
   if (warp == 0) {
     if (elect_one()) {
-      grid_wait();  // nothing is read, and so nothing written, before
+      grid_wait();
       launch_dependents();  // the dA kernel may start its set-up and stream its codes
       uint32_t stage = 0, phase = 0;
       bool armed[S];
@@ -159,6 +162,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     }
   } else if (warp == 1) {
     if (has_work && elect_one()) {
+      grid_wait();
       constexpr uint32_t idesc_u = make_idesc_f16(128, R, false, true, kBF16);
       constexpr uint32_t idesc_db = make_idesc_f16(128, R, true, false, kBF16);
       uint32_t stage = 0, phase = 0;
@@ -189,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   const long long row = static_cast<long long>(tile) * 128 + row_local;
   bool have = false;
   if (epi && has_work) {
+    grid_wait();
     have = mbar_wait(done_bar, 0, p.status, kDevTimeoutAccFull);
     tc_fence_after();
   }

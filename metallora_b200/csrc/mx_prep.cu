@@ -106,9 +106,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   const int kb_end = min(p.num_kb, kb_begin + per);
   const bool has_work = kb_begin < kb_end;
 
+  // Nothing is read, and so nothing written, before the kernel before this one is
+  // through.  Each role waits for that itself, so that the limits of its bounded waits
+  // count from there: that kernel may be anyone's, and take its time.
   if (warp == 0) {
     if (elect_one()) {
-      grid_wait();  // nothing is read, and so nothing written, before
+      grid_wait();
       launch_dependents();  // the product may start its set-up and stream its weight
       uint32_t stage = 0, phase = 0;
       bool armed[S];
@@ -129,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     }
   } else if (warp == 1) {
     if (has_work && elect_one()) {
+      grid_wait();
       constexpr uint32_t idesc = make_idesc_f16(128, R, false, false, kBF16);
       uint32_t stage = 0, phase = 0;
       for (int kb = kb_begin; kb < kb_end; ++kb) {
@@ -145,6 +149,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       umma_commit(done_bar);
     }
   } else if (has_work) {
+    grid_wait();
     // Lanes 2i, 2i+1: the two blocks of one row's 64 features, 16 rows a warp.  A
     // tile of few tokens leaves warps without rows: they take every second, fourth
     // or eighth k-block instead (one token, K 4096: the pass 5.0 -> 3.9 us).

@@ -55,3 +55,16 @@ def test_stage_release_depends_on_the_loads():
     body = next(k[3] for k in KERNELS if k[1] == "mx_prep_kernel")
     arrive = re.search(r"if \(__reduce_max_sync\([^;]*?\) != ([\w.]+)[^;]*\)\s*mbar_arrive\(", body)
     assert arrive and arrive.group(1).startswith("p."), arrive
+
+
+def test_first_kernels_wait_in_every_role():
+    """The kernels that follow whatever ran before them wait for it in every role of
+    their warps, ahead of that role's first bounded wait: one that went on would count
+    a long predecessor against the limit."""
+    roles = {"mx_prep_kernel": ("if (warp == 0) {", "else if (warp == 1) {", "else if (has_work) {"),
+             "lora_bwd_kernel": ("if (warp == 0) {", "else if (warp == 1) {", "if (epi && has_work) {")}
+    for name, starts in roles.items():
+        body = next(k[3] for k in KERNELS if k[1] == name)
+        for start in starts:
+            role = body[body.index(start):]
+            assert "grid_wait();" in role[:role.index("mbar_wait(")], (name, start)
