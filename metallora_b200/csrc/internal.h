@@ -308,8 +308,8 @@ inline int64_t mx_atoms_bytes(int64_t rows, int64_t K) {
   return (rows + 127) / 128 * ((K + 127) / 128) * 512;
 }
 
-// s x A^T (out_rows [M, ld_rows] with columns past R zeroed, out_t [R, ld_t];
-// either may be null) and from the same read of x [M, K] its MXFP4 operand (q4
+// s x A^T (out_rows [M, ld_rows] with columns past R zeroed, and where it is not
+// null out_t [R, ld_t]) and from the same read of x [M, K] its MXFP4 operand (q4
 // codes [M, K/2] and scale atoms; K % 32 == 0) and / or its MXINT8
 // checkpoint (q8 codes ld8 bytes apart, 16-byte aligned rows; kMxGroups scales).
 struct MxPrepArgs {
@@ -317,7 +317,7 @@ struct MxPrepArgs {
   const void* a;  // [r, K]
   int64_t M, K, r, R;
   float scale;
-  void* out_rows = nullptr;
+  void* out_rows = nullptr;  // required
   int64_t ld_rows = 0;
   void* out_t = nullptr;
   int64_t ld_t = 0;

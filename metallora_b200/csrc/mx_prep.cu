@@ -344,6 +344,10 @@ int dispatch(const MxPrepArgs& a, cudaStream_t s) {
 }  // namespace
 
 int launch_mx_prep(const MxPrepArgs& a, cudaStream_t s) {
+  if (a.out_rows == nullptr) {
+    set_error("rank and quantise pass: the row output is required");
+    return MLORA_ERR_INVALID_ARG;
+  }
   return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
 }
 
