@@ -347,8 +347,10 @@ struct MxGemmArgs {
   int64_t M = 0, N = 0, K = 0, R = 0, w2_rows = 0;
   int64_t ldx2 = 0, ldw2 = 0, ldd = 0;
   Elt elt = Elt::kBF16;  // of x2, w2 and d
-  // programmatic dependent of the kernel that wrote xq, xs and x2 (nothing else
-  // it reads came from that kernel)
+  // programmatic dependent of the kernel that wrote xq, xs and x2.  wq, ws and w2 are
+  // loaded ahead of the wait for it: it may not have written them, and each of its
+  // CTAs must let dependents start only after its own wait, so that whatever did
+  // write them is through (mx_prep_kernel does)
   bool overlap_prev = false;
 };
 int launch_mx_gemm(const MxGemmArgs& a, cudaStream_t s);
@@ -367,7 +369,9 @@ struct MxWgradArgs {
   bool accumulate, out16;
   float clip;
   Elt elt;
-  bool overlap_prev = false;  // programmatic dependent of the kernel that wrote st
+  // programmatic dependent of the kernel that wrote st and st_lo; codes and scales
+  // are loaded ahead of the wait, under MxGemmArgs' rule (lora_bwd_kernel keeps it)
+  bool overlap_prev = false;
 };
 int launch_mx_wgrad(const MxWgradArgs& a, cudaStream_t s);
 

@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         }
       };
       // the weight does not come from the kernel before this one, the token
-      // operands do: a ring of weight blocks is on its way before the wait
+      // operands do: a ring of weight blocks is on its way before the wait (what
+      // wrote the weight is through: MxGemmArgs::overlap_prev)
       const int ahead = min(S, kb_end - kb_begin);
       for (int i = 0; i < ahead; ++i) {
         load_weight(kb_begin + i, smem + i * kStage, &full_bar[i]);
@@ -367,7 +368,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         armed_parity[s] = parity;
       };
       // W, its scales and W2 do not come from the kernel before this one: the first
-      // item's ring of them is on its way before the wait (every pair has an item)
+      // item's ring of them is on its way before the wait (every pair has an item;
+      // what wrote them is through: MxGemmArgs::overlap_prev)
       int tm, n0, wide;
       pair_item(p, pair, tm, n0, wide);
       const int ahead = min(kPairStages, total_kb);

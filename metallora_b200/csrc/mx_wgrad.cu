@@ -129,7 +129,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
         tma_load_2d(st + kLoOff, &tm_lo, bar, kb * kBM, 0);
       };
       // U comes from the kernel before this one, the checkpoint does not: a ring
-      // of code blocks is on its way before the wait
+      // of code blocks is on its way before the wait (what wrote it is through:
+      // MxWgradArgs::overlap_prev)
       const int ahead = min(S, kb_end - kb_begin);
       for (int i = 0; i < ahead; ++i) {
         load_codes(kb_begin + i, stages + i * stage_bytes(R), &full_bar[i]);

@@ -63,8 +63,9 @@ __device__ __forceinline__ void record_status(uint32_t* status, uint32_t code) {
 // A kernel launched as a programmatic dependent may start while the one before it
 // still runs.  grid_wait() returns once that one has completed and its writes are
 // visible (at once in any other launch); launch_dependents() allows the next one
-// to start when every CTA has called it.  A kernel calls them in this order, so
-// that whatever came before the kernel before it has completed too.
+// to start when every CTA has called it or ended.  A kernel calls them in this
+// order: whatever came before its predecessor has then completed when its successor
+// starts, which may read that ahead of its own wait, and nothing else.
 
 __device__ __forceinline__ void grid_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");

@@ -68,3 +68,11 @@ def test_first_kernels_wait_in_every_role():
         for start in starts:
             role = body[body.index(start):]
             assert "grid_wait();" in role[:role.index("mbar_wait(")], (name, start)
+
+
+def test_dependents_start_after_the_wait():
+    """A kernel lets the next one start after its own wait: the next one reads ahead of
+    its wait what is older than this kernel."""
+    for file, name, head, body in KERNELS:
+        if "grid_wait()" in body and "launch_dependents()" in body:
+            assert body.index("grid_wait()") < body.index("launch_dependents()"), (file, name)
