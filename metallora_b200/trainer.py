@@ -42,7 +42,7 @@ from .distributed import BucketedGradExchange, PeerLiveness, average_gradients
 from .exceptions import ConfigurationError
 from .layers import LoRALinear
 from .logging import logger
-from .utils import apply_lora_to_model
+from .utils import apply_lora_to_model, is_lora_target
 
 
 @dataclass
@@ -274,6 +274,28 @@ class MetalAdamW:
         self.gpu_state.copy_(sd["gpu_state"])
 
 
+def _check_activation_checkpoint(model: nn.Module, c: TrainingConfig) -> None:
+    """Refuses, before the model is changed, a setting that its layers' forward would
+    (see ``ops.lora_forward``; a quantised base takes no dropout and 16-bit inputs only)."""
+    if c.activation_checkpoint is None:
+        return
+    if c.activation_checkpoint != "mxint8":
+        raise ConfigurationError(f"unknown activation checkpoint {c.activation_checkpoint!r}")
+    layers = [(n, m) for n, m in model.named_modules() if isinstance(m, LoRALinear)]
+    dense = [(n, m.dropout if m.training else 0.0, m.W0.dtype) for n, m in layers
+             if m.qweight is None and not m.merged]
+    if not layers:  # the ones that the trainer will make
+        dense = [(n, c.dropout, m.weight.dtype) for n, m in model.named_modules()
+                 if isinstance(m, nn.Linear) and is_lora_target(n, c.target_modules)]
+    for name, dropout, dtype in dense:
+        if dropout > 0:
+            raise ConfigurationError(f"{name}: an activation checkpoint takes no LoRA dropout, "
+                                     f"which reads x itself (got {dropout})")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise ConfigurationError(f"{name}: activation checkpoints take bf16 or fp16 layers, "
+                                     f"got {dtype}")
+
+
 class LoRATrainer:
     """LoRA trainer (reference: trainer.py:173-302)."""
 
@@ -282,6 +304,7 @@ class LoRATrainer:
                  liveness_timeout: float | None = 30.0):
         self.config = config or TrainingConfig()
         c = self.config
+        _check_activation_checkpoint(model, c)
         if not any(isinstance(m, LoRALinear) for m in model.modules()):
             apply_lora_to_model(model, rank=c.rank, alpha=c.alpha,
                                 target_modules=c.target_modules, dropout=c.dropout)
@@ -289,8 +312,6 @@ class LoRATrainer:
         for p in model.parameters():
             p.requires_grad_(False)
         if c.activation_checkpoint is not None:
-            if c.activation_checkpoint != "mxint8":
-                raise ConfigurationError(f"unknown activation checkpoint {c.activation_checkpoint!r}")
             for m in model.modules():
                 if isinstance(m, LoRALinear):
                     m.activation_checkpoint = c.activation_checkpoint

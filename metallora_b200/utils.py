@@ -111,21 +111,21 @@ def load_quantized_bases(model: nn.Module, path: str | Path, name: str = "base",
     return model
 
 
+def is_lora_target(name: str, target_modules: list[str] | None) -> bool:
+    """Whether ``apply_lora_to_model`` replaces an ``nn.Linear`` of this dotted name."""
+    return any(t in name for t in target_modules or ["q_proj", "v_proj", "k_proj", "o_proj"])
+
+
 def apply_lora_to_model(model: nn.Module, rank: int = 8, alpha: float = 16.0,
                         target_modules: list[str] | None = None, dropout: float = 0.0) -> nn.Module:
     """utils.py:54-80: replaces every ``nn.Linear`` whose dotted name contains a
     target substring (default q/v/k/o_proj) with ``LoRALinear.from_linear``."""
     from .layers import LoRALinear
 
-    target_modules = target_modules or ["q_proj", "v_proj", "k_proj", "o_proj"]
-
-    def should_apply(name: str) -> bool:
-        return any(t in name for t in target_modules)
-
     def replace_linear(module: nn.Module, prefix: str = "") -> None:
         for child_name, child in list(module.named_children()):
             full_name = f"{prefix}.{child_name}" if prefix else child_name
-            if isinstance(child, nn.Linear) and should_apply(full_name):
+            if isinstance(child, nn.Linear) and is_lora_target(full_name, target_modules):
                 setattr(module, child_name,
                         LoRALinear.from_linear(child, rank=rank, alpha=alpha, dropout=dropout))
             else:

@@ -9,7 +9,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from metallora_b200 import _lib, kernels, ops, quant
+from metallora_b200 import _lib, kernels, ops, quant, trainer
 from metallora_b200.exceptions import AdapterError, ConfigurationError
 from metallora_b200.layers import LoRALinear
 from metallora_b200.trainer import LoRATrainer, TrainingConfig
@@ -228,3 +228,33 @@ def test_loading_is_all_or_nothing(tmp_path):
     _files(tmp_path, {"0": (24, 64), "1": (40, 64)})
     m = load_quantized_bases(net(), tmp_path)
     assert all(l.qweight is not None and not l.W0.numel() for l in m)
+
+
+def test_checkpoint_settings_are_checked_first(tmp_path):
+    """What the layers' forward would refuse, the trainer refuses before it touches
+    the model; what it would take is taken."""
+    def config(**kw):
+        return TrainingConfig(activation_checkpoint="mxint8", rank=8, output_dir=str(tmp_path), **kw)
+
+    def lora(dtype=BF16, **kw):
+        return torch.nn.Sequential(LoRALinear(64, 64, rank=8, dtype=dtype, **kw))
+
+    def plain(dtype):
+        return torch.nn.ModuleDict({"q_proj": torch.nn.Linear(64, 64, dtype=dtype),
+                                    "head": torch.nn.Linear(64, 64)})
+    for model, kw in ((lora(dropout=0.1), {}), (lora(FP32), {}), (plain(BF16), {"dropout": 0.1}),
+                      (plain(FP32), {})):
+        before = [(n, type(m)) for n, m in model.named_modules()]
+        grads = [p.requires_grad for p in model.parameters()]
+        with pytest.raises(ConfigurationError):
+            LoRATrainer(model, config(**kw))
+        assert [(n, type(m)) for n, m in model.named_modules()] == before
+        assert [p.requires_grad for p in model.parameters()] == grads
+        assert not any(getattr(m, "activation_checkpoint", None) for m in model.modules())
+    off = lora(dropout=0.1).eval()  # dropout that is switched off is none
+    quantised = lora(FP32, dropout=0.1)
+    quantised[0].qweight = _cpu_weight(64, 64)
+    trainer._check_activation_checkpoint(plain(BF16), config())
+    trainer._check_activation_checkpoint(off, config())
+    trainer._check_activation_checkpoint(quantised, config())
+    trainer._check_activation_checkpoint(plain(FP32), TrainingConfig(dropout=0.1))
