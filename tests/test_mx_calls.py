@@ -4,7 +4,6 @@ changed in place, every base with a checkpoint, products that are exact.
 """
 import copy
 
-import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -258,3 +257,82 @@ def test_checkpoint_settings_are_checked_first(tmp_path):
     trainer._check_activation_checkpoint(off, config())
     trainer._check_activation_checkpoint(quantised, config())
     trainer._check_activation_checkpoint(plain(FP32), TrainingConfig(dropout=0.1))
+
+
+# ---------------------------------------------------------- every base, exact products --
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("M,K,N,r", [(1, 4096, 264, 64), (16, 4096, 1024, 16), (40, 4096, 136, 8),
+                                     (100, 8160, 136, 24), (128, 4096, 264, 128), (300, 4096, 520, 16),
+                                     (700, 4096, 264, 64), (1290, 4128, 2048, 16)])
+def test_exact_products(cuda, dt, M, K, N, r):
+    """Operands that the formats hold, with sums that fp32 holds at every step: y
+    is the 64-bit result rounded once, bit for bit.  |x|, |w| <= 1.5 in halves, one
+    power of two a token and one (1, 2) a block of w: a term is a multiple of 1/4, a
+    sum at most 4.5 K < 2^18 quarters.  A has 8 entries +-1 a row, so that x A^T is a
+    multiple of 1/2 up to 12 (24 halves: 5 bits); B holds multiples of 1/4 up to 1, and
+    the rank term adds at most 12 r, in eighths."""
+    g = _gen(M + K + N + r)
+    pick = torch.tensor([-1.5, -1.0, -0.5, 0.0, 0.5, 1.0, 1.5])
+    x = pick[torch.randint(0, 7, (M, K), generator=g)]
+    x *= torch.exp2(torch.randint(-2, 3, (M, 1), generator=g).float())
+    w = pick[torch.randint(0, 7, (N, K), generator=g)]
+    w *= torch.exp2(torch.randint(0, 2, (N, K // 32), generator=g).float()).repeat_interleave(32, 1)
+    a = torch.zeros(r, K)
+    for j in range(r):
+        at = torch.randperm(K, generator=g)[:8]
+        a[j, at] = torch.randint(0, 2, (8,), generator=g).float() * 2 - 1
+    b = torch.randint(-4, 5, (N, r), generator=g) / 4
+    ref = x.double() @ w.double().t() + (x.double() @ a.double().t()) @ b.double().t()
+    x, w, a, b = (t.to(dt).to(cuda) for t in (x, w, a, b.float()))
+    qw = quant.quantize(w, "mxfp4")
+    assert torch.equal(qw.dequantize(dt), w) and torch.equal(quant.quantize(x, "mxfp4").dequantize(dt), x)
+    y = kernels.qlora_linear_fwd(x, qw, a, b, float(r))[0]
+    assert torch.equal(y.cpu(), ref.float().to(dt))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lean", [False, True])
+@pytest.mark.parametrize("scheme", ["nf4", "int4", "int8"])
+@pytest.mark.parametrize("M", [1, 16, 90, 300])
+def test_checkpoint_over_quantised_bases(cuda, scheme, lean, M):
+    """Over every base, lean weights included, a checkpoint leaves y and dx as they
+    are without it, is the one of ``checkpoint_activation``, and gives dA of its values."""
+    K, N, r = 256, 136, 16
+    x, w, a, b, dy = _inputs(M, K, N, r, BF16, cuda)
+    qw = quant.quantize(w, scheme, lean=lean)
+    made = quant.empty_checkpoint(x)
+    y0, saved0 = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True)
+    y, saved = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, save_xa=True, ckpt_out=made)
+    want = quant.checkpoint_activation(x)
+    assert torch.equal(made.codes, want.codes) and torch.equal(made.scales[:, :M], want.scales[:, :M])
+    assert torch.equal(y, y0) and torch.equal(saved[:, :M], saved0[:, :M])
+    y1, none = kernels.qlora_linear_fwd(x, qw, a, b, 32.0, ckpt_out=made)  # nothing saved
+    assert none is None and torch.equal(made.codes, want.codes) and torch.equal(y1, y0)
+    dx0, _, db0 = kernels.qlora_linear_bwd(dy, x, qw, a, b, 32.0, saved)
+    dx, da, db = kernels.qlora_linear_bwd(dy, made, qw, a, b, 32.0, saved)
+    dx2, da2, db2 = kernels.lora_linear_bwd(dy, made, None, a, b, 32.0, saved, need_dx=False)
+    assert dx2 is None and torch.equal(da, da2) and torch.equal(db, db2)
+    for x_ in (x, made):  # 16-bit gradients are the fp32 ones rounded
+        _, wa, wb = kernels.qlora_linear_bwd(dy, x_, qw, a, b, 32.0, saved)
+        _, ha, hb = kernels.qlora_linear_bwd(dy, x_, qw, a, b, 32.0, saved, grad_dtype=BF16)
+        assert torch.equal(ha, wa.to(BF16)) and torch.equal(hb, wb.to(BF16))
+    half = torch.finfo(BF16).eps / 2
+    u = 2.0 * dy.double() @ b.double()
+    acc = N * 2.0 ** -23 * 2.0 * dy.double().abs() @ b.double().abs()  # fp32 sums of U
+    # U's 16-bit rounding in dx, twice where the two differ; the fp32 sums of both
+    # products; the two results' own roundings
+    mag = dy.double().abs() @ qw.dequantize(FP32).double().abs() + u.abs() @ a.double().abs()
+    tol = 2 * ((half * u.abs() + acc) @ a.double().abs() + (N + r) * 2.0 ** -22 * mag)
+    tol = tol + half * (dx.double().abs() + dx0.double().abs()) * (1 + half)
+    assert ((dx.double() - dx0.double()).abs() <= tol).all()
+    ref = u.t() @ made.dequantize(FP32).double()
+    tol = (half ** 2 * u.abs() + acc).t() @ made.dequantize(FP32).double().abs() + \
+        2.02 * M * 2.0 ** -23 * u.abs().t() @ made.dequantize(FP32).double().abs() + 2.0 ** -22 * ref.abs()
+    assert ((da.double() - ref).abs() <= tol + 1e-40).all()
+    S = saved[:r, :M].double()
+    tol = (M + 2) * 2.0 ** -23 * dy.double().abs().t() @ S.abs().t()
+    assert ((db.double() - dy.double().t() @ S.t()).abs() <= tol + 1e-40).all()
+    assert ((db.double() - db0.double()).abs() <= 2 * tol + 1e-40).all()
+    assert _lib.device_status() == 0
