@@ -68,6 +68,11 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// A tensor of `dtype` starts on a whole element.
+bool aligned_elements(const void* p, int dtype) {
+  return reinterpret_cast<uintptr_t>(p) % (dtype == MLORA_DTYPE_F32 ? 4 : 2) == 0;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
@@ -1192,17 +1197,25 @@ int dequantize_weight(int scheme, const void* codes, const void* scales, const v
 }
 }  // namespace
 
-int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme, int64_t group,
-                   void* codes, void* scales, void* zeros, void* stream) {
-  int rc = check_quant(scheme, N, K, group);
-  if (rc) return rc;
+namespace {
+int check_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme, int64_t group,
+                   const void* codes, const void* scales, const void* zeros) {
+  if (int rc = check_quant(scheme, N, K, group)) return rc;
   if (!w || !codes || !scales || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
   if (w_dtype < MLORA_DTYPE_BF16 || w_dtype > MLORA_DTYPE_F32)
     return fail(MLORA_ERR_INVALID_ARG, "weight dtype must be BF16, F16 or F32");
   if (scheme == MLORA_QUANT_MXFP4 && (reinterpret_cast<uintptr_t>(scales) & 3u))
     return fail(MLORA_ERR_INVALID_ARG, "MXFP4 scales must be 4-byte aligned");
-  if ((rc = check_device())) return rc;
+  if (!aligned_elements(w, w_dtype))
+    return fail(MLORA_ERR_INVALID_ARG, "the weight does not start on a whole element");
+  return check_device();
+}
+}  // namespace
+
+int mlora_quantize(const void* w, int w_dtype, int64_t N, int64_t K, int scheme, int64_t group,
+                   void* codes, void* scales, void* zeros, void* stream) {
+  if (int rc = check_quantize(w, w_dtype, N, K, scheme, group, codes, scales, zeros)) return rc;
   if (scheme == MLORA_QUANT_MXFP4)
     return launch_mx_quantize(4, w, w_dtype, N, K, codes, K / 2, plain_scales(scales, N, K),
                               static_cast<cudaStream_t>(stream));
@@ -1216,14 +1229,8 @@ int mlora_quantize_mxfp4(const void* w, int w_dtype, int64_t N, int64_t K, void*
   if (!aligned16(table)) return fail(MLORA_ERR_INVALID_ARG, "the table must be 16-byte aligned");
   bool made = false;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int rc = check_quant(MLORA_QUANT_MXFP4, N, K, 32);
+  int rc = check_quantize(w, w_dtype, N, K, MLORA_QUANT_MXFP4, 32, codes, scales, nullptr);
   if (rc) return rc;
-  if (!w || !codes || !scales) return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
-  if (w_dtype < MLORA_DTYPE_BF16 || w_dtype > MLORA_DTYPE_F32)
-    return fail(MLORA_ERR_INVALID_ARG, "weight dtype must be BF16, F16 or F32");
-  if (reinterpret_cast<uintptr_t>(scales) & 3u)
-    return fail(MLORA_ERR_INVALID_ARG, "MXFP4 scales must be 4-byte aligned");
-  if ((rc = check_device())) return rc;
   if ((rc = launch_mx_quantize(4, w, w_dtype, N, K, codes, K / 2, plain_scales(scales, N, K), s,
                                table, &made)))
     return rc;
@@ -1238,6 +1245,8 @@ int mlora_dequantize(int scheme, const void* codes, const void* scales, const vo
     return fail(MLORA_ERR_INVALID_ARG, "NULL pointer");
   if (out_dtype < MLORA_DTYPE_BF16 || out_dtype > MLORA_DTYPE_F32)
     return fail(MLORA_ERR_INVALID_ARG, "out dtype must be BF16, F16 or F32");
+  if (!aligned_elements(out, out_dtype))
+    return fail(MLORA_ERR_INVALID_ARG, "out does not start on a whole element");
   if ((rc = check_device())) return rc;
   return dequantize_weight(scheme, codes, scales, zeros, N, K, group, out, out_dtype,
                            static_cast<cudaStream_t>(stream));
@@ -1260,6 +1269,8 @@ int check_act(const void* x, int dtype, const void* codes, int64_t ld, const voi
   if (ld < K) return fail(MLORA_ERR_INVALID_ARG, "code rows overlap: ld is below K");
   if (reinterpret_cast<uintptr_t>(scales) & 3u)
     return fail(MLORA_ERR_INVALID_ARG, "scales must be 4-byte aligned");
+  if (!aligned_elements(x, dtype))
+    return fail(MLORA_ERR_INVALID_ARG, "the activations do not start on a whole element");
   return check_device();
 }
 }  // namespace

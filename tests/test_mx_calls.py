@@ -3,6 +3,7 @@ out: derivatives that the operators do not define, values that are not finite, p
 changed in place, every base with a checkpoint, products that are exact.
 """
 import copy
+import ctypes
 
 import pytest
 import torch
@@ -257,6 +258,22 @@ def test_checkpoint_settings_are_checked_first(tmp_path):
     trainer._check_activation_checkpoint(off, config())
     trainer._check_activation_checkpoint(quantised, config())
     trainer._check_activation_checkpoint(plain(FP32), TrainingConfig(dropout=0.1))
+
+
+def test_c_abi_wants_whole_elements():
+    """An address inside an element would fault in the kernel: it is refused."""
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    mx, bad = _lib.QUANT_MXFP4, _lib.MLORA_ERR_INVALID_ARG
+    for dtype, off in ((0, 1), (1, 1), (2, 2)):
+        assert lib.mlora_quantize(p + off, dtype, 4, 64, mx, 32, p, p, None, None) == bad
+        assert lib.mlora_quantize(p + off, dtype, 4, 64, _lib.QUANT_NF4, 64, p, p, None, None) == bad
+        assert lib.mlora_quantize_mxfp4(p + off, dtype, 4, 64, p, p, p, None) == bad
+        assert lib.mlora_dequantize(mx, p, p, None, 4, 64, 32, p + off, dtype, None) == bad
+        assert lib.mlora_act_checkpoint(p + off, dtype, 4, 64, p, 64, p, None) == bad
+        assert lib.mlora_act_restore(p, 64, p, 4, 64, p + off, dtype, None) == bad
+        assert b"whole element" in lib.mlora_last_error_message()
 
 
 # ---------------------------------------------------------- every base, exact products --
