@@ -497,7 +497,16 @@ struct Ckpt {
   const void* scales;
 };
 
-int check_ckpt(const Ckpt& c, int64_t K, const void* saved_xa, int dtype) {
+// Token numbers are 32 bits in the kernels, up to the end of the last tile.
+int check_tokens(int64_t M) {
+  if (M > (int64_t(1) << 31) - 256)
+    return fail(MLORA_ERR_UNSUPPORTED,
+                "an MXFP4 base and a checkpoint take fewer than 2^31 - 255 tokens");
+  return MLORA_OK;
+}
+
+int check_ckpt(const Ckpt& c, int64_t M, int64_t K, const void* saved_xa, int dtype) {
+  if (int rc = check_tokens(M)) return rc;
   if (!c.codes || !c.scales) return fail(MLORA_ERR_INVALID_ARG, "NULL checkpoint pointer");
   if (!aligned16(c.codes) || !aligned16(c.scales) || c.ld < K || c.ld % 16)
     return fail(MLORA_ERR_INVALID_ARG,
@@ -950,8 +959,8 @@ int lora_forward16(const void* x, const void* w0, const void* a, const void* b, 
 
 namespace {
 // The checkpoint a forward writes.
-int check_ckpt_out(const Ckpt& c, int64_t K, int dtype) {
-  return check_ckpt(c, K, c.codes, dtype);
+int check_ckpt_out(const Ckpt& c, int64_t M, int64_t K, int dtype) {
+  return check_ckpt(c, M, K, c.codes, dtype);
 }
 
 int lora_forward_any(const void* x, const void* w0, const void* a, const void* b, void* y,
@@ -960,7 +969,7 @@ int lora_forward_any(const void* x, const void* w0, const void* a, const void* b
                      void* stream) {
   int rc = check_shapes(M, K, N, r, dtype, false);
   if (rc) return rc;
-  if (ckpt != nullptr && (rc = check_ckpt_out(*ckpt, K, dtype))) return rc;
+  if (ckpt != nullptr && (rc = check_ckpt_out(*ckpt, M, K, dtype))) return rc;
   if (!x || !w0 || !a || !b || !y) return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
   if (!aligned16(x) || !aligned16(w0) || !aligned16(a) || !aligned16(b) || !aligned16(y) ||
       (saved_xa && !aligned16(saved_xa)))
@@ -1031,7 +1040,7 @@ int lora_backward_any(const void* dy, const void* x, const Ckpt* ckpt, const voi
   if (rc) return rc;
   if (!dy || (!x && ckpt == nullptr) || !a || !b || !da || !db)
     return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
-  if (ckpt != nullptr && (rc = check_ckpt(*ckpt, K, saved_xa, dtype))) return rc;
+  if (ckpt != nullptr && (rc = check_ckpt(*ckpt, M, K, saved_xa, dtype))) return rc;
   if ((dx == nullptr) != (w0 == nullptr))
     return fail(MLORA_ERR_INVALID_ARG, "w0 and dx must be both set or both NULL");
   if (phase != kPhaseAll && (dx == nullptr || dtype == MLORA_DTYPE_F32))
@@ -1300,9 +1309,7 @@ int check_qlora(int scheme, int64_t M, int64_t K, int64_t N, int64_t r, int64_t 
     if (dtype == MLORA_DTYPE_F32)
       return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base takes BF16 or F16 activations");
     if (K % 32) return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base needs K a multiple of 32");
-    if (M > (int64_t(1) << 31) - 256)  // row numbers are 32 bits up to the last tile's end
-      return fail(MLORA_ERR_UNSUPPORTED, "an MXFP4 base takes fewer than 2^31 - 255 tokens");
-    return MLORA_OK;
+    return check_tokens(M);
   }
   if (dtype != MLORA_DTYPE_BF16)
     return fail(MLORA_ERR_UNSUPPORTED, "quantised-base paths take BF16 activations");
@@ -1486,7 +1493,7 @@ int qlora_forward_any(const void* x, int scheme, const void* codes, const void* 
                       size_t workspace_bytes, void* stream) {
   int rc = check_qlora(scheme, M, K, N, r, group, dtype);
   if (rc) return rc;
-  if (ckpt != nullptr && (rc = check_ckpt_out(*ckpt, K, dtype))) return rc;
+  if (ckpt != nullptr && (rc = check_ckpt_out(*ckpt, M, K, dtype))) return rc;
   if (!x || !codes || !scales || !a || !b || !y || (has_zeros(scheme) && !zeros))
     return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
   if ((rc = check_ptrs16({x, codes, scales, zeros, prepared, a, b, y, saved_xa, workspace})))
@@ -1635,7 +1642,7 @@ int qlora_backward_any(const void* dy, const void* x, const Ckpt* ckpt, int sche
     return fail(MLORA_ERR_INVALID_ARG, "unknown flags");
   if (!dy || (!x && ckpt == nullptr) || !a || !b || !da || !db)
     return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
-  if (ckpt != nullptr && (rc = check_ckpt(*ckpt, K, saved_xa, dtype))) return rc;
+  if (ckpt != nullptr && (rc = check_ckpt(*ckpt, M, K, saved_xa, dtype))) return rc;
   if (dx && (!codes || !scales || (has_zeros(scheme) && !zeros)))
     return fail(MLORA_ERR_INVALID_ARG, "dx needs the quantised weight");
   if ((rc = check_ptrs16({dy, x, codes, scales, zeros, prepared, a, b, saved_xa, dx, da, db,

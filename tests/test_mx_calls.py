@@ -276,6 +276,24 @@ def test_c_abi_wants_whole_elements():
         assert b"whole element" in lib.mlora_last_error_message()
 
 
+@pytest.mark.parametrize("M", [(1 << 31) - 255, (1 << 31) - 1, 1 << 31])
+def test_checkpoints_of_too_many_tokens_are_refused(M):
+    """Past 2^31 - 256 tokens a row number of the last tile would not fit 32 bits."""
+    K, N = 64, 64
+    lib = _lib.load()
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = (ctypes.addressof(buf) + 255) // 256 * 256
+    mx, no = _lib.QUANT_MXFP4, _lib.MLORA_ERR_UNSUPPORTED
+    sizes, ld = (M, K, N, 8, 1.0), K
+    assert lib.mlora_lora_forward_ckpt(p, p, p, p, p, p, p, ld, p, *sizes, 0, p, 1 << 10, None) == no
+    assert lib.mlora_lora_backward_ckpt(p, p, ld, p, None, p, p, p, None, p, p, *sizes, 0.0, 0, 0, p,
+                                        1 << 10, None) == no
+    assert lib.mlora_qlora_forward_ckpt(p, mx, p, p, None, p, 32, p, p, p, p, p, ld, p, *sizes, 0, p,
+                                        1 << 10, None) == no
+    assert lib.mlora_qlora_backward_ckpt(p, p, ld, p, mx, p, p, None, p, 32, p, p, p, p, p, p, *sizes,
+                                         0.0, 0, 0, p, 1 << 10, None) == no
+
+
 # ---------------------------------------------------------- every base, exact products --
 
 @pytest.mark.gpu
