@@ -1365,7 +1365,7 @@ size_t qbwd_lean_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int64_t group
 
 // ---- MXFP4 base: x as fp4 codes and scale atoms, s.x.A^T rows ----------------
 struct MxFwdPlan {
-  int64_t R, R64;
+  int64_t R, R64;  // R64: a row of s.x.A^T, two parts of R columns
   void* xq;
   void* xs;
   void* xa_rows;
@@ -1376,7 +1376,7 @@ struct MxFwdPlan {
 MxFwdPlan plan_mx_forward(void* ws, int64_t M, int64_t K, int64_t N, int64_t r, bool own_table) {
   MxFwdPlan p;
   p.R = rank_tile(r);
-  p.R64 = pad64(p.R);
+  p.R64 = pad64(2 * p.R);
   Carve c(ws);
   p.xq = c.take(static_cast<size_t>(M) * (K / 2));
   p.xs = c.take(static_cast<size_t>(mx_atoms_bytes(M, K)));
@@ -1411,6 +1411,7 @@ int mx_forward(const void* x, const void* codes, const void* scales, const void*
   pa.scale = alpha / static_cast<float>(r);
   pa.out_rows = p.xa_rows;
   pa.ld_rows = p.R64;
+  pa.two_parts = true;
   pa.out_t = saved_xa;
   pa.ld_t = pad8(M);
   pa.q4 = p.xq;

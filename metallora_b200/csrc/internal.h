@@ -319,6 +319,7 @@ struct MxPrepArgs {
   float scale;
   void* out_rows = nullptr;  // required
   int64_t ld_rows = 0;
+  bool two_parts = false;  // out_rows: R columns rounded, R of what that left over
   void* out_t = nullptr;
   int64_t ld_t = 0;
   void* q4 = nullptr;
@@ -335,7 +336,8 @@ int launch_mx_prep(const MxPrepArgs& a, cudaStream_t s);
 int set_max_smem(const void* kern, size_t bytes, std::atomic<bool>* done);
 
 // Y[M, N] = Q4(x) . W4^T + X2 . W2^T, both fp4 operands as codes [rows, K/2] and
-// scale atoms; x2 [M, R64] and w2 [N, r] 16-bit as in GemmArgs.
+// scale atoms; w2 [N, r] 16-bit as in GemmArgs, and X2 = the sum of x2's two parts
+// [M, R] each, side by side (MxPrepArgs::two_parts).
 struct MxGemmArgs {
   const void* xq;
   const void* xs;

@@ -27,6 +27,14 @@ constexpr int kBK16 = 64;                        // 16-bit reduction per rank k-
 constexpr uint32_t kRowBytes = 128;              // of either
 constexpr uint32_t kSfBytes = 2 * kMxAtomBytes;  // scales of 128 rows x 256 features
 
+// X2's two parts take the columns [0, R) and [R, 2R) of its rows, and both meet the
+// same W2: the W2 column of the rank block's k-block e, and the W2 step of its step k
+// (up to rank 32 both parts lie in one block, and W2 once beside them).
+__device__ __forceinline__ int rank_column(int e, int R) { return (e * kBK16) & (R - 1) & ~(kBK16 - 1); }
+__device__ __forceinline__ uint32_t rank_step(int k, int R) {
+  return static_cast<uint32_t>(R >= kBK16 ? k : k & (R / 16 - 1));
+}
+
 // ---------------------------------------------------------------------------
 // Few tokens (M <= 128): the weight rows are the MMA's M side (128 a tile) and
 // the tokens its N side, so one pass over the weight serves all tokens.
@@ -119,7 +127,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
       auto load_weight = [&](int kb, uint8_t* st, uint64_t* bar) {
         if (kb >= p.num_kb_main) {
           mbar_arrive_expect_tx(bar, (128 + NT) * kRowBytes);
-          tma_load_2d(st, &tm_w2, bar, (kb - p.num_kb_main) * kBK16, n0);
+          tma_load_2d(st, &tm_w2, bar, rank_column(kb - p.num_kb_main, p.R), n0);
         } else {
           mbar_arrive_expect_tx(bar, kStage);
           tma_load_2d(st, &tm_w, bar, kb * static_cast<int>(kRowBytes), n0);
@@ -169,11 +177,10 @@ __global__ void __launch_bounds__(kSkinnyThreads)
         const uint32_t sx = sw + kXOff;
         const uint32_t first = kb == kb_begin ? 0u : 1u;
         if (kb >= p.num_kb_main) {
-          const int rem = p.R - (kb - p.num_kb_main) * kBK16;
-          const int nk = rem >= kBK16 ? 4 : rem / 16;
+          const int nk = min(4, 2 * p.R / 16);
           for (int k = 0; k < nk; ++k)
-            umma_f16(tmem, desc_kmajor_sw128(sw, k), desc_kmajor_sw128(sx, k), idesc16,
-                     first | static_cast<uint32_t>(k != 0));
+            umma_f16(tmem, desc_kmajor_sw128(sw, rank_step(k, p.R)), desc_kmajor_sw128(sx, k),
+                     idesc16, first | static_cast<uint32_t>(k != 0));
         } else {
           const uint32_t sfa = tmem + skinny_acc_cols(NT) + static_cast<uint32_t>(kb & 1) * 16u;
           const uint32_t sfb = sfa + 8u;
@@ -341,7 +348,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t bar = lead_full + s * 8u;
         const int row = n0 + static_cast<int>(crank) * (wide / 2);
         if (kb >= p.num_kb_main) {
-          tma_load_2d_pair(st + kWOff, &tm_w2, bar, (kb - p.num_kb_main) * kBK16, row);
+          tma_load_2d_pair(st + kWOff, &tm_w2, bar, rank_column(kb - p.num_kb_main, p.R), row);
         } else {
           tma_load_2d_pair(st + kWOff, &tm_w, bar, kb * static_cast<int>(kRowBytes), row);
           tma_load_2d_pair(st + kWsOff, &tm_ws, bar, 0, (n0 >> 7) * p.atoms_k + 2 * kb);
@@ -416,11 +423,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           const uint32_t sx = smem_u32(smem + stage * kPairStageBytes);
           const uint32_t sw = sx + kWOff;
           if (kb >= p.num_kb_main) {
-            const int rem = p.R - (kb - p.num_kb_main) * kBK16;
-            const int nk = rem >= kBK16 ? 4 : rem / 16;
+            const int nk = min(4, 2 * p.R / 16);
             for (int k = 0; k < nk; ++k)
-              umma_f16_pair(tmem, desc_kmajor_sw128(sx, k), desc_kmajor_sw128(sw, k), idesc16,
-                            (kb | k) != 0 ? 1u : 0u);
+              umma_f16_pair(tmem, desc_kmajor_sw128(sx, k), desc_kmajor_sw128(sw, rank_step(k, p.R)),
+                            idesc16, (kb | k) != 0 ? 1u : 0u);
           } else {
             const uint32_t sfa = tmem + kPairN + set * 32u;
             const uint32_t sfb = sfa + 8u;
@@ -535,7 +541,7 @@ int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
   if (!map_codes(&tw, a.wq, a.N, a.K, 128) || !map_codes(&tx, a.xq, a.M, a.K, NT) ||
       !map_atoms(&tws, a.ws, a.N, a.K) || !map_atoms(&txs, a.xs, a.M, a.K))
     return MLORA_ERR_INVALID_ARG;
-  const int64_t r64 = (a.R + 63) / 64 * 64;
+  const int64_t r64 = (2 * a.R + 63) / 64 * 64;
   if (!make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, 128) ||
       !make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, NT))
     return MLORA_ERR_INVALID_ARG;
@@ -545,7 +551,7 @@ int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
   p.K = static_cast<int>(a.K);
   p.num_kb_main = static_cast<int>((a.K + kBK4 - 1) / kBK4);
   p.R = static_cast<int>(a.R);
-  p.num_kb_extra = static_cast<int>((a.R + kBK16 - 1) / kBK16);
+  p.num_kb_extra = static_cast<int>((2 * a.R + kBK16 - 1) / kBK16);
   p.atoms_k = static_cast<int>((a.K + 127) / 128);
   p.d = a.d;
   p.ldd = a.ldd;
@@ -587,7 +593,7 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   if (!map_codes(&tx, a.xq, a.M, a.K, kHalf) || !map_codes(&tw, a.wq, a.N, a.K, kHalf) ||
       !map_atoms(&txs, a.xs, a.M, a.K) || !map_atoms(&tws, a.ws, a.N, a.K))
     return MLORA_ERR_INVALID_ARG;
-  const int64_t r64 = (a.R + 63) / 64 * 64;
+  const int64_t r64 = (2 * a.R + 63) / 64 * 64;
   if (!make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK16, kHalf) ||
       !make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK16, kHalf))
     return MLORA_ERR_INVALID_ARG;
@@ -597,7 +603,7 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   p.K = static_cast<int>(a.K);
   p.num_kb_main = static_cast<int>((a.K + kBK4 - 1) / kBK4);
   p.R = static_cast<int>(a.R);
-  p.num_kb_extra = static_cast<int>((a.R + kBK16 - 1) / kBK16);
+  p.num_kb_extra = static_cast<int>((2 * a.R + kBK16 - 1) / kBK16);
   p.tiles_m = static_cast<int>((a.M + 2 * kHalf - 1) / (2 * kHalf));
   p.tiles_n = static_cast<int>((a.N + kPairN - 1) / kPairN);
   p.group_m = p.tiles_m < 8 ? p.tiles_m : 8;

@@ -53,6 +53,7 @@ struct PrepParams {
   float scale;
   void* out_rows;
   long long ld_rows;
+  int two_parts;  // the row output is followed by what its rounding left, R columns each
   void* out_t;
   long long ld_t;
   uint8_t* q4;       // codes [M, K/2], or nullptr
@@ -248,7 +249,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     float v[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = in[i] * p.scale;
-    store_columns<T>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j, v, p.wide_rows != 0);
+    T* const rows = reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + j;
+    store_columns<T>(rows, v, p.wide_rows != 0);
+    if (p.two_parts) {
+      float rest[C];
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const float f = static_cast<float>(static_cast<T>(v[i]));
+        rest[i] = isfinite(f) ? v[i] - f : 0.f;
+      }
+      store_columns<T>(rows + R, rest, p.wide_rows != 0);
+    }
     if (p.out_t != nullptr) {
       T* dst = reinterpret_cast<T*>(p.out_t) + row + j * p.ld_t;
 #pragma unroll
@@ -257,9 +268,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   };
   cluster_push_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have, recv,
                          p.splits, crank, row_local, epi, emit);
-  if (live && crank == 0) {  // zero columns past R
+  if (live && crank == 0) {  // zero columns past the last part
     T* dst = reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows;
-    for (long long j = R; j < p.ld_rows; j += 8)
+    for (long long j = p.two_parts ? 2 * R : R; j < p.ld_rows; j += 8)
       *reinterpret_cast<uint4*>(dst + j) = make_uint4(0, 0, 0, 0);
   }
   tc_fence_before();
@@ -288,6 +299,7 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   p.scale = a.scale;
   p.out_rows = a.out_rows;
   p.ld_rows = a.ld_rows;
+  p.two_parts = a.two_parts ? 1 : 0;
   p.out_t = a.out_t;
   p.ld_t = a.ld_t;
   p.q4 = static_cast<uint8_t*>(a.q4);

@@ -328,6 +328,29 @@ def test_exact_products(cuda, dt, M, K, N, r):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [BF16, FP16])
+@pytest.mark.parametrize("M", [3, 40, 300])
+@pytest.mark.parametrize("r", [8, 16, 24, 64, 128, 200])
+def test_rank_term_is_rounded_once(cuda, dt, M, r):
+    """s x A^T goes to its product with B unrounded: with x A^T of 13 significant bits
+    (multiples of 1/16 up to 384; the 16-bit types hold 8 and 11), y is still the 64-bit
+    result rounded once.  The sums stay below 2^24 steps of 1/64."""
+    K, N = 256, 136
+    g = _gen(M + r)
+    pick = torch.tensor([-1.5, -1.0, -0.5, 0.0, 0.5, 1.0, 1.5])
+    x, w = pick[torch.randint(0, 7, (M, K), generator=g)], pick[torch.randint(0, 7, (N, K), generator=g)]
+    a = torch.randint(-8, 9, (r, K), generator=g) / 8
+    b = torch.randint(-4, 5, (N, r), generator=g) / 4
+    xa = x.double() @ a.double().t()
+    assert (xa != xa.to(BF16).double()).any()
+    ref = x.double() @ w.double().t() + xa @ b.double().t()
+    x, w, a, b = (t.to(dt).to(cuda) for t in (x, w, a, b))
+    y, saved = kernels.qlora_linear_fwd(x, quant.quantize(w, "mxfp4"), a, b, float(r), save_xa=True)
+    assert torch.equal(y.cpu(), ref.float().to(dt))
+    assert torch.equal(saved[:r, :M].cpu(), xa.t().float().to(dt))  # (kept rounded)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lean", [False, True])
 @pytest.mark.parametrize("scheme", ["nf4", "int4", "int8"])
 @pytest.mark.parametrize("M", [1, 16, 90, 300])
