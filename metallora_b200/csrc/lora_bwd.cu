@@ -19,11 +19,11 @@
 // are split apart from each other, so that all CTAs have about the same number
 // of k-blocks.  Warp 0 copies, warp 1 issues the UMMAs, warps 2-5 store.
 #include <atomic>
-#include <string>
 #include <type_traits>
 
 #include "cluster_reduce.cuh"
 #include "internal.h"
+#include "launch.cuh"
 #include "ptx.cuh"
 #include "../../include/metallora_b200.h"
 
@@ -45,9 +45,6 @@ __host__ __device__ constexpr int num_stages(int R) {
 }
 constexpr size_t smem_bytes(int R) {
   return 1024 + num_stages(R) * stage_bytes(R) + push_bytes(R) + 256;
-}
-__host__ __device__ constexpr uint32_t tmem_cols(int R) {
-  return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
 }
 
 // B's tile [64 rows x R columns], R contiguous: one box of R columns in the
@@ -317,44 +314,19 @@ int launch_typed(const LoraBwdArgs& a, cudaStream_t stream) {
   auto kern = lora_bwd_kernel<R, kBF16>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas_u + ctas_db));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes(R);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
   LaunchScope scope(kKindRank, stream);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tr, tc, tb, tx, p);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e == cudaSuccess) return MLORA_OK;
-  set_error(std::string("lora backward launch: ") + cudaGetErrorString(e));
-  return MLORA_ERR_CUDA;
-}
-
-template <bool kB>
-int dispatch(const LoraBwdArgs& a, cudaStream_t s) {
-  switch (a.R) {
-    case 16: return launch_typed<16, kB>(a, s);
-    case 32: return launch_typed<32, kB>(a, s);
-    case 64: return launch_typed<64, kB>(a, s);
-    case 128: return launch_typed<128, kB>(a, s);
-    case 256: return launch_typed<256, kB>(a, s);
-    default: set_error("unsupported padded rank"); return MLORA_ERR_UNSUPPORTED;
-  }
+  return launch_status(
+      launch_kernel(kern, dim3(static_cast<unsigned>(p.ctas_u + ctas_db)), kThreads, smem_bytes(R),
+                    stream, static_cast<unsigned>(cluster), 1, true, tr, tc, tb, tx, p),
+      "lora backward launch");
 }
 
 }  // namespace
 
 int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t s) {
-  return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
+  return with_rank(a.R, [&](auto R) {
+    return a.elt == Elt::kBF16 ? launch_typed<R.value, true>(a, s) : launch_typed<R.value, false>(a, s);
+  });
 }
 
 }  // namespace mlora

@@ -16,6 +16,7 @@
 
 #include "cluster_reduce.cuh"
 #include "internal.h"
+#include "launch.cuh"
 #include "mx.cuh"
 #include "../../include/metallora_b200.h"
 
@@ -59,9 +60,7 @@ constexpr size_t skinny_smem(int NT) {
 }
 // accumulator columns, then two sets of (8 weight, 8 token) scale columns
 __host__ __device__ constexpr uint32_t skinny_acc_cols(int NT) { return NT; }
-__host__ __device__ constexpr uint32_t skinny_tmem_cols(int NT) {
-  return NT + 32 <= 64 ? 64u : (NT + 32 <= 128 ? 128u : 256u);
-}
+__host__ __device__ constexpr uint32_t skinny_tmem_cols(int NT) { return tmem_cols(NT + 32); }
 
 struct SkinnyParams {
   int M, N, K;
@@ -518,11 +517,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   }
 }
 
-int cuda_launch_error(cudaError_t e, const char* what) {
-  set_error(std::string(what) + ": " + cudaGetErrorString(e));
-  return MLORA_ERR_CUDA;
-}
-
 // Tensor maps of an fp4 operand: code rows [rows, K/2] and scale atoms.
 bool map_codes(CUtensorMap* m, const void* codes, int64_t rows, int64_t K, uint32_t box_rows) {
   return make_tmap_2d(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, codes, static_cast<uint64_t>(K / 2),
@@ -567,24 +561,12 @@ int launch_skinny(const MxGemmArgs& a, cudaStream_t stream) {
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), skinny_smem(NT), attr_set))
     return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits));
-  cfg.blockDim = dim3(kSkinnyThreads);
-  cfg.dynamicSmemBytes = skinny_smem(NT);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = static_cast<unsigned>(splits);
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.overlap_prev ? 2 : 1;
   LaunchScope scope(kKindGemm, stream);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, tx, tws, txs, tw2, tx2, p);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx skinny launch");
+  return launch_status(
+      launch_kernel(kern, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits)),
+                    kSkinnyThreads, skinny_smem(NT), stream, 1, static_cast<unsigned>(splits),
+                    a.overlap_prev, tw, tx, tws, txs, tw2, tx2, p),
+      "mx skinny launch");
 }
 
 template <bool kBF16>
@@ -621,7 +603,7 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   if (pairs == 0) {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(kPairSmem));
-    if (e != cudaSuccess) return cuda_launch_error(e, "cudaFuncSetAttribute(mx pair)");
+    if (e != cudaSuccess) return launch_status(e, "cudaFuncSetAttribute(mx pair)");
     // clusters that can be resident at once (GPCs may leave an SM unpaired)
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(num_sms() / 2 * 2));
@@ -641,20 +623,10 @@ int launch_pair(const MxGemmArgs& a, cudaStream_t stream) {
   p.whole = 2 * last <= pairs ? tiles - last : tiles;
   p.num_items = p.whole + 2 * (tiles - p.whole);
   const int grid = 2 * (p.num_items < pairs ? p.num_items : pairs);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
-  cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.overlap_prev ? 1 : 0;
   LaunchScope scope(kKindGemm, stream);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, txs, tws, tx2, tw2, p);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx pair launch");
+  return launch_status(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), kPairThreads, kPairSmem,
+                                     stream, 0, 0, a.overlap_prev, tx, tw, txs, tws, tx2, tw2, p),
+                       "mx pair launch");
 }
 
 template <bool kBF16>

@@ -17,11 +17,11 @@
 // the quantising warps bound it: about 230 instructions a thread and block, issue
 // slots 56 % used by 16 warps an SM.  At a few tokens it is latency: 4 us.
 #include <atomic>
-#include <string>
 #include <type_traits>
 
 #include "cluster_reduce.cuh"
 #include "internal.h"
+#include "launch.cuh"
 #include "mx.cuh"
 #include "../../include/metallora_b200.h"
 
@@ -42,9 +42,6 @@ __host__ __device__ constexpr int num_stages(int R) {
 }
 constexpr size_t smem_bytes(int R) {
   return 1024 + num_stages(R) * stage_bytes(R) + push_bytes(R) + 256;
-}
-__host__ __device__ constexpr uint32_t tmem_cols(int R) {
-  return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
 }
 
 struct PrepParams {
@@ -281,11 +278,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   }
 }
 
-int cuda_launch_error(cudaError_t e, const char* what) {
-  set_error(std::string(what) + ": " + cudaGetErrorString(e));
-  return MLORA_ERR_CUDA;
-}
-
 template <int R, bool kBF16>
 int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   CUtensorMap tx, ta;
@@ -321,36 +313,10 @@ int launch_typed(const MxPrepArgs& a, cudaStream_t stream) {
   auto kern = mx_prep_kernel<R, kBF16>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes(R);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 1;
-  attr[0].val.clusterDim.y = static_cast<unsigned>(splits);
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
   LaunchScope scope(kKindRank, stream);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, ta, p);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx prep launch");
-}
-
-template <bool kB>
-int dispatch(const MxPrepArgs& a, cudaStream_t s) {
-  switch (a.R) {
-    case 16: return launch_typed<16, kB>(a, s);
-    case 32: return launch_typed<32, kB>(a, s);
-    case 64: return launch_typed<64, kB>(a, s);
-    case 128: return launch_typed<128, kB>(a, s);
-    case 256: return launch_typed<256, kB>(a, s);
-    default: set_error("unsupported padded rank"); return MLORA_ERR_UNSUPPORTED;
-  }
+  return launch_status(launch_kernel(kern, dim3(static_cast<unsigned>(tiles), static_cast<unsigned>(splits)), kThreads,
+                                     smem_bytes(R), stream, 1, static_cast<unsigned>(splits), true, tx, ta, p),
+                       "mx prep launch");
 }
 
 }  // namespace
@@ -360,7 +326,9 @@ int launch_mx_prep(const MxPrepArgs& a, cudaStream_t s) {
     set_error("rank and quantise pass: the row output is required");
     return MLORA_ERR_INVALID_ARG;
   }
-  return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
+  return with_rank(a.R, [&](auto R) {
+    return a.elt == Elt::kBF16 ? launch_typed<R.value, true>(a, s) : launch_typed<R.value, false>(a, s);
+  });
 }
 
 }  // namespace mlora

@@ -11,9 +11,8 @@
 // measured copy rate; 11008 x 4096 to MXFP4 (with the product's table) and back
 // 38 us = 231 MB at 6.1 TB/s.  The eight-a-lane form, taken for whole blocks too,
 // needs 42.4 and 48.5 us: twice the instructions, half the bytes a load.
-#include <string>
-
 #include "internal.h"
+#include "launch.cuh"
 #include "mx.cuh"
 #include "../../include/metallora_b200.h"
 
@@ -358,28 +357,12 @@ int mx_grid(int64_t M, int64_t K, dim3* grid) {
   return MLORA_OK;
 }
 
-int launched(const char* what) {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    set_error(std::string(what) + ": " + cudaGetErrorString(e));
-    return MLORA_ERR_CUDA;
-  }
-  return MLORA_OK;
-}
+int launched(const char* what) { return launch_status(cudaSuccess, what); }
 
 // A block kernel, as a programmatic dependent of the kernel before it.
 template <typename... P, typename... A>
-void launch_blocks(void (*kern)(P...), unsigned grid, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(kMxThreads);
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, kern, static_cast<P>(args)...);  // (launched() has its error)
+int launch_blocks(const char* what, void (*kern)(P...), unsigned grid, cudaStream_t s, const A&... args) {
+  return launch_status(launch_kernel(kern, dim3(grid), kMxThreads, 0, s, 0, 0, true, args...), what);
 }
 
 bool aligned(const void* p, uintptr_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
@@ -434,16 +417,13 @@ int launch_mx_quantize(int bits, const void* x, int dtype, int64_t M, int64_t K,
     auto* t = K % 128 == 0 ? static_cast<uint8_t*>(atoms) : nullptr;
     if (atoms_made != nullptr) *atoms_made = t != nullptr;
     LaunchScope scope(kKindQuant, s);
-    if (dtype == MLORA_DTYPE_BF16) {
-      using T = __nv_bfloat16;
-      launch_blocks(bits == 4 ? mx_quantize_blocks_kernel<4, T> : mx_quantize_blocks_kernel<8, T>, grid,
-                    s, static_cast<const T*>(x), blocks, per_row, c, sc, t);
-    } else {
-      using T = __half;
-      launch_blocks(bits == 4 ? mx_quantize_blocks_kernel<4, T> : mx_quantize_blocks_kernel<8, T>, grid,
-                    s, static_cast<const T*>(x), blocks, per_row, c, sc, t);
-    }
-    return launched("mx quantize");
+    auto run = [&](auto type) {
+      using T = decltype(type);
+      return launch_blocks("mx quantize",
+                           bits == 4 ? mx_quantize_blocks_kernel<4, T> : mx_quantize_blocks_kernel<8, T>,
+                           grid, s, static_cast<const T*>(x), blocks, per_row, c, sc, t);
+    };
+    return dtype == MLORA_DTYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
   }
   if (atoms_made != nullptr) *atoms_made = false;
   dim3 grid;
@@ -469,16 +449,13 @@ int launch_mx_dequantize(int bits, const void* codes, int64_t ld, const MxScales
     const unsigned grid = (blocks + kMxThreads * kOwn - 1) / (kMxThreads * kOwn);
     const auto* c = static_cast<const uint8_t*>(codes);
     LaunchScope scope(kKindQuant, s);
-    if (out_dtype == MLORA_DTYPE_BF16) {
-      using O = __nv_bfloat16;
-      launch_blocks(bits == 4 ? mx_dequantize_blocks_kernel<4, O> : mx_dequantize_blocks_kernel<8, O>,
-                    grid, s, c, sc, blocks, per_row, static_cast<O*>(out));
-    } else {
-      using O = __half;
-      launch_blocks(bits == 4 ? mx_dequantize_blocks_kernel<4, O> : mx_dequantize_blocks_kernel<8, O>,
-                    grid, s, c, sc, blocks, per_row, static_cast<O*>(out));
-    }
-    return launched("mx dequantize");
+    auto run = [&](auto type) {
+      using O = decltype(type);
+      return launch_blocks("mx dequantize",
+                           bits == 4 ? mx_dequantize_blocks_kernel<4, O> : mx_dequantize_blocks_kernel<8, O>,
+                           grid, s, c, sc, blocks, per_row, static_cast<O*>(out));
+    };
+    return out_dtype == MLORA_DTYPE_BF16 ? run(__nv_bfloat16()) : run(__half());
   }
   dim3 grid;
   if (int rc = mx_grid(M, K, &grid)) return rc;

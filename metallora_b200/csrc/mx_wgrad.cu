@@ -16,11 +16,11 @@
 // order (cluster_reduce.cuh).  Warp 0 copies 64-token blocks of codes, scale words
 // and U^T (TMA ring), warps 2-9 expand the codes into the swizzled MN-major
 // operand, warp 1 issues the UMMAs, warps 2-5 store the tile.
-#include <string>
 #include <type_traits>
 
 #include "cluster_reduce.cuh"
 #include "internal.h"
+#include "launch.cuh"
 #include "mx.cuh"
 #include "../../include/metallora_b200.h"
 
@@ -51,9 +51,6 @@ __host__ __device__ constexpr int num_stages(int R) {
 }
 constexpr size_t smem_bytes(int R) {
   return 1024 + kOps * kOpBytes + num_stages(R) * stage_bytes(R) + recv_bytes(R) + 256;
-}
-__host__ __device__ constexpr uint32_t tmem_cols(int R) {
-  return R <= 32 ? 32u : (R <= 64 ? 64u : (R <= 128 ? 128u : 256u));
 }
 
 struct MxWgradParams {
@@ -259,11 +256,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
   }
 }
 
-int cuda_launch_error(cudaError_t e, const char* what) {
-  set_error(std::string(what) + ": " + cudaGetErrorString(e));
-  return MLORA_ERR_CUDA;
-}
-
 template <int R, bool kBF16>
 int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   CUtensorMap tc, ts, tu, tl;
@@ -295,42 +287,18 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   auto kern = mx_wgrad_kernel<R, kBF16>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(groups * splits));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem_bytes(R);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(splits);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = a.overlap_prev ? 2 : 1;
   LaunchScope scope(kKindWgrad, stream);
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tc, ts, tu, tl, p);
-  if (e == cudaSuccess) e = cudaGetLastError();
-  return e == cudaSuccess ? MLORA_OK : cuda_launch_error(e, "mx wgrad launch");
-}
-
-template <bool kB>
-int dispatch(const MxWgradArgs& a, cudaStream_t s) {
-  switch (a.R) {
-    case 16: return launch_typed<16, kB>(a, s);
-    case 32: return launch_typed<32, kB>(a, s);
-    case 64: return launch_typed<64, kB>(a, s);
-    case 128: return launch_typed<128, kB>(a, s);
-    case 256: return launch_typed<256, kB>(a, s);
-    default: set_error("unsupported padded rank"); return MLORA_ERR_UNSUPPORTED;
-  }
+  return launch_status(launch_kernel(kern, dim3(static_cast<unsigned>(groups * splits)), kThreads,
+                                     smem_bytes(R), stream, static_cast<unsigned>(splits), 1, a.overlap_prev, tc, ts, tu, tl, p),
+                       "mx wgrad launch");
 }
 
 }  // namespace
 
 int launch_mx_wgrad(const MxWgradArgs& a, cudaStream_t s) {
-  return a.elt == Elt::kBF16 ? dispatch<true>(a, s) : dispatch<false>(a, s);
+  return with_rank(a.R, [&](auto R) {
+    return a.elt == Elt::kBF16 ? launch_typed<R.value, true>(a, s) : launch_typed<R.value, false>(a, s);
+  });
 }
 
 }  // namespace mlora
