@@ -1661,6 +1661,8 @@ int qlora_backward_any(const void* dy, const void* x, const Ckpt* ckpt, int sche
                       ckpt);
   const size_t wbytes = staged_w_bytes(N, K);
   if (workspace != nullptr && workspace_bytes >= wbytes + bytes) {
+    // in the activations' type, the tensor cores' operand: an MXFP4 value is exact in
+    // bf16, and in fp16 but for blocks below 2^-18, whose smallest round to 2^-24 steps
     if ((rc = dequantize_weight(scheme, codes, scales, zeros, N, K, group, workspace, dtype, s)))
       return rc;
     return backward16(dy, x, workspace, nullptr, a, b, saved_xa, dx, da, db, M, K, N, r, alpha,

@@ -9,6 +9,9 @@
 // reduction tail are paid instead of two.  B is read as it lies ([N, r], the
 // MMA's MN-major operand): no transposed copy.
 //
+// U is rounded once for dx (u_rows), as without a checkpoint: dx is the same bits.
+// For dA it comes in two parts, since there its rounding would count as much as dA's.
+//
 // Measured, dy 8192 x 4096, r 16: 17 us, 11 of them streaming (67.8 MB from HBM,
 // 152 MB from L2 to the SMs: 13 TB/s, which bounds it), 3 to the first MMA, 2-3 of
 // reduction.  The two launches and the transpose it replaces took 31 us.

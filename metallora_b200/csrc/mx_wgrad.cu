@@ -288,9 +288,10 @@ int launch_typed(const MxWgradArgs& a, cudaStream_t stream) {
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), smem_bytes(R), attr_set)) return rc;
   LaunchScope scope(kKindWgrad, stream);
-  return launch_status(launch_kernel(kern, dim3(static_cast<unsigned>(groups * splits)), kThreads,
-                                     smem_bytes(R), stream, static_cast<unsigned>(splits), 1, a.overlap_prev, tc, ts, tu, tl, p),
-                       "mx wgrad launch");
+  return launch_status(
+      launch_kernel(kern, dim3(static_cast<unsigned>(groups * splits)), kThreads, smem_bytes(R),
+                    stream, static_cast<unsigned>(splits), 1, a.overlap_prev, tc, ts, tu, tl, p),
+      "mx wgrad launch");
 }
 
 }  // namespace
