@@ -221,7 +221,22 @@ __device__ __forceinline__ void cluster_push_reduce(uint32_t taddr, bool have, f
 #pragma unroll 1
   for (int pass = 0; pass < R / CP; ++pass) {
     if (pass > 0) cluster_sync();  // the slots have been summed
-    if (epi) {
+    if (epi && S == 1) {
+      // (a loop: the code that 16 columns' emit takes comes from memory once)
+#pragma unroll 1
+      for (int j = 0; j < CP; j += 16) {
+        float v[16];
+        if (have) {
+          load_acc_row<16>(taddr + pass * CP + j, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) v[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.f + v[i];
+        emit_columns(emit, pass * CP + j, v);
+      }
+    } else if (epi) {
       float acc[CP];
       if (have) {
         load_acc_row<CP>(taddr + pass * CP, acc);
@@ -229,15 +244,7 @@ __device__ __forceinline__ void cluster_push_reduce(uint32_t taddr, bool have, f
 #pragma unroll
         for (int j = 0; j < CP; ++j) acc[j] = 0.f;
       }
-      if (S == 1) {
-#pragma unroll
-        for (int j = 0; j < CP; j += 16) {
-          float v[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = 0.f + acc[j + i];
-          emit_columns(emit, pass * CP + j, v);
-        }
-      } else if (S == 2) {
+      if (S == 2) {
         push_columns<CP, 2>(acc, recv, crank, first, row_local);
       } else if (S == 4) {
         push_columns<CP, 4>(acc, recv, crank, first, row_local);

@@ -27,7 +27,7 @@
 #include "cluster_reduce.cuh"
 #include "internal.h"
 #include "launch.cuh"
-#include "ptx.cuh"
+#include "mx.cuh"
 #include "../../include/metallora_b200.h"
 
 namespace mlora {
@@ -211,13 +211,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
       // as the rounding of dA itself
       T* hi = reinterpret_cast<T*>(p.u_t) + row + j * p.ld_t;
       T* lo = reinterpret_cast<T*>(p.u_lo) + row + j * p.ld_t;
+      float rest[C];
+      second_part<T>(v, rest);
 #pragma unroll
       for (int i = 0; i < C; ++i) {
-        const T h = static_cast<T>(v[i]);
-        hi[i * p.ld_t] = h;
-        // (an infinity has no second part: what is left of it would make a NaN)
-        const float f = static_cast<float>(h);
-        lo[i * p.ld_t] = static_cast<T>(isfinite(f) ? v[i] - f : 0.f);
+        hi[i * p.ld_t] = static_cast<T>(v[i]);
+        lo[i * p.ld_t] = static_cast<T>(rest[i]);
       }
       return;
     }

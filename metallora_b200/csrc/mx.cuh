@@ -135,6 +135,24 @@ __device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
   return d;
 }
 
+// What rounding to T left of N values: the second of two 16-bit parts.  An infinite
+// first part (an overflow too) has none: inf and -inf would add up to NaN.
+template <typename T, int N>
+__device__ __forceinline__ void second_part(const float (&v)[N], float (&rest)[N]) {
+  uint64_t seen = 0;
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    const uint64_t d = f2_sub(f2_pack(v[i], v[i + 1]), widen2<T>(pack2<T>(v[i], v[i + 1])));
+    seen = f2_fma(d, 0, seen);  // stays 0 unless one is an infinity or a NaN
+    rest[i] = f2_lo(d);
+    rest[i + 1] = f2_hi(d);
+  }
+  if (f2_lo(seen) != 0.f || f2_hi(seen) != 0.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) rest[i] = isfinite(rest[i]) ? rest[i] : 0.f;
+  }
+}
+
 // The 32 e2m1 codes of a block with this scale byte.
 template <typename T>
 __device__ __forceinline__ uint4 block_fp4(const uint32_t (&w)[16], uint32_t byte) {

@@ -257,11 +257,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(R))
     store_columns<T>(rows, v, p.wide_rows != 0);
     if (p.two_parts) {
       float rest[C];
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const float f = static_cast<float>(static_cast<T>(v[i]));
-        rest[i] = isfinite(f) ? v[i] - f : 0.f;
-      }
+      second_part<T>(v, rest);
       store_columns<T>(rows + R, rest, p.wide_rows != 0);
     }
     if (p.out_t != nullptr) {
