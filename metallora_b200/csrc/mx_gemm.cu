@@ -7,9 +7,9 @@
 // dequantised.  The rank-r block is appended as 16-bit kind::f16 steps into the
 // same TMEM accumulator, as in the dense kernel, so Y is written once.  X2 comes in
 // two 16-bit parts: twice the rank steps, which up to rank 32 still fit one k-block
-// (16 tokens 4096 -> 4096, rank 16: 7.9 us with one part, 8.0 with two); from rank 64
-// every 64 columns are one more (rank 64, 4096 -> 11008: one token 11.1 and 11.3 us,
-// 4096 tokens 88.9 and 92.9).
+// (16 tokens 4096 -> 4096, rank 16: 7.9 us with one part and with two); from rank 64
+// every 64 columns are one more (rank 64: 513 tokens 6848 -> 936 23.7 and 24.0 us, 4096
+// tokens 4096 -> 11008 88.2 and 91.9).
 //
 // A shared-memory row of 128 bytes is 256 codes or 64 16-bit values, so both
 // kinds of k-block share one stage layout (128-byte swizzle, K-major) and one
@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t rank_step(int k, int R) {
 // ---------------------------------------------------------------------------
 // Few tokens (M <= 128): the weight rows are the MMA's M side (128 a tile) and
 // the tokens its N side, so one pass over the weight serves all tokens.
-// Bound by latency: one token through 4096 -> 11008 takes 11.2 us with the pass
+// Bound by latency: one token through 4096 -> 11008 takes 11.0 us with the pass
 // before it, of which the weight's 24 MB are 3.7 at the measured bandwidth; a ring
 // of weight blocks is loaded while that pass still runs.  The reduction is split
 // over the CTAs of a cluster so that about two CTAs per SM stream it, and their
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kSkinnyThreads)
 //
 // Measured, 4096 x 4096 -> 11008, R 64: alone 85 us = 4.4 PFLOP/s at the 1.62 GHz
 // that the chip's power cap leaves it (tensor pipe 68 % busy; behind the pass over x,
-// whose end it overlaps, the two take 91.5).  A tile takes 12-13 thousand cycles: 9.2
+// whose end it overlaps, the two take 91.9).  A tile takes 12-13 thousand cycles: 9.2
 // of MMA (64 fp4 of 128 cycles, 8 bf16), 1.4 of scale copies (they run in the MMAs'
 // queue, 15 cycles each), 0.9 until the
 // accumulator is free again, 1-2 of waiting for operands (907 MB come from L2; with

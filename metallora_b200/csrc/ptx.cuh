@@ -438,9 +438,17 @@ __device__ __forceinline__ void st_global_32b(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// v bounded to [-c, c]; a NaN stays one (fminf and fmaxf alone would make it a bound).
+// v bounded to [-c, c]; a NaN stays one (fminf and fmaxf would make it a bound).
 __device__ __forceinline__ float clip_keep_nan(float v, float c) {
-  return v != v ? v : fminf(fmaxf(v, -c), c);
+  float r;
+  asm("{\n\t"
+      ".reg .f32 t;\n\t"
+      "max.NaN.f32 t, %1, %2;\n\t"
+      "min.NaN.f32 %0, t, %3;\n\t"
+      "}"
+      : "=f"(r)
+      : "f"(v), "f"(-c), "f"(c));
+  return r;
 }
 
 template <typename T>
