@@ -78,7 +78,7 @@ struct SkinnyParams {
 
 // Grid (weight tiles, splits), cluster (1, splits, 1).
 template <int NT, bool kBF16>
-__global__ void __launch_bounds__(kSkinnyThreads)
+__global__ void __launch_bounds__(kSkinnyThreads, NT <= 32 ? 2 : 1)
     mx_skinny_kernel(const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_ws, const __grid_constant__ CUtensorMap tm_xs,
                      const __grid_constant__ CUtensorMap tm_w2, const __grid_constant__ CUtensorMap tm_x2,
