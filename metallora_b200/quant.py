@@ -94,7 +94,7 @@ class QuantizedWeight:
         if kept is None or self._prepared.device != self.codes.device:
             return None
         s, z = self.scales, self.zeros
-        # (what is written over in inference mode keeps no count of it)
+        # (what is written over through .data or in inference mode keeps no count of it)
         if kept[0] is s and kept[1] is z and kept[2] == (-1 if s.is_inference() else s._version) and \
                 (z is None or kept[3] == (-1 if z.is_inference() else z._version)):
             return self._prepared

@@ -4,6 +4,7 @@ changed in place, every base with a checkpoint, products that are exact.
 """
 import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -164,6 +165,21 @@ def test_parts_changed_in_place(cuda, scheme):
     qw.codes, qw.scales, qw.zeros = twin.codes, twin.scales, twin.zeros
     assert torch.equal(kernels.qlora_linear_fwd(x, qw, a, b, 16.0)[0],
                        kernels.qlora_linear_fwd(x, q2, a, b, 16.0)[0])
+
+
+def test_copies_of_a_weight():
+    """A copied or pickled weight holds its parts and no table of another's."""
+    qw = _cpu_weight()
+    qw._keep_table(torch.zeros(512, dtype=torch.uint8))
+    assert qw._kept_table() is qw._prepared
+    for twin in (copy.deepcopy(qw), copy.copy(qw), pickle.loads(pickle.dumps(qw))):
+        assert twin.shape == qw.shape and twin.scheme == "mxfp4" and twin._kept_table() is None
+        assert torch.equal(twin.codes, qw.codes) and torch.equal(twin.scales, qw.scales)
+    qw.scales.add_(1)
+    assert qw._kept_table() is None
+    qw._keep_table(torch.zeros(512, dtype=torch.uint8))
+    qw.scales = qw.scales.clone()
+    assert qw._kept_table() is None
 
 
 def _files(tmp_path, shapes):
