@@ -118,18 +118,25 @@ class QuantizedWeight:
         """The TMA-ready scale table the GPU kernels read: [groups, rows rounded
         to 4], or for MXFP4 the product's blocks of 128 rows x 128 features
         (built on first use -- for MXFP4 when the weight is made -- and kept with
-        the weight until its scales or zeros are written over or replaced; a table
-        built while a graph is captured belongs to that graph and is not kept)."""
+        the weight; a table built while a graph is captured belongs to that graph and
+        is not kept).  Once the scales or zeros are written over it is made anew, in
+        the same memory: graphs captured with it replay with the new one."""
         t = self._kept_table()
         if t is None:
             lib = _lib.load()
             N, K = self.shape
-            nbytes = lib.mlora_qlora_prepared_scales_bytes(self.code, N, K, self.group)
-            t = torch.empty(nbytes, dtype=torch.uint8, device=self.codes.device)
+            capturing = torch.cuda.is_current_stream_capturing()
+            kept = getattr(self, "_table_of", None)
+            if kept is not None and kept[0] is self.scales and kept[1] is self.zeros and \
+                    self._prepared.device == self.codes.device and not capturing:
+                t = self._prepared
+            else:
+                nbytes = lib.mlora_qlora_prepared_scales_bytes(self.code, N, K, self.group)
+                t = torch.empty(nbytes, dtype=torch.uint8, device=self.codes.device)
             st = lib.mlora_qlora_prepare_scales(self.code, _ptr(self.scales), _ptr(self.zeros), N,
                                                 K, self.group, _ptr(t), _stream())
             _lib.check(st, "mlora_qlora_prepare_scales")
-            if not torch.cuda.is_current_stream_capturing():
+            if not capturing:
                 self._keep_table(t)
         return t
 

@@ -167,6 +167,30 @@ def test_parts_changed_in_place(cuda, scheme):
                        kernels.qlora_linear_fwd(x, q2, a, b, 16.0)[0])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("scheme", ["mxfp4", "int4"])
+def test_graphs_follow_a_changed_weight(cuda, scheme):
+    """A graph captured before a weight's parts were written over replays with the new
+    weight once its table has been made anew: it never reads a table that is gone."""
+    x, w, a, b, _ = _inputs(4, 256, 72, 8, BF16, cuda)
+    qw, other = quant.quantize(w, scheme), quant.quantize(w.flip(0) * 4, scheme)
+    kernels.qlora_linear_fwd(x, qw, a, b, 16.0)
+    y = torch.empty(4, 72, dtype=BF16, device=cuda)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y.copy_(kernels.qlora_linear_fwd(x, qw, a, b, 16.0)[0])
+    for part in ("codes", "scales", "zeros"):
+        if getattr(qw, part) is not None:
+            getattr(qw, part).copy_(getattr(other, part))
+    want = kernels.qlora_linear_fwd(x, other, a, b, 16.0)[0]
+    assert torch.equal(kernels.qlora_linear_fwd(x, qw, a, b, 16.0)[0], want)
+    keep = [torch.full((n,), 255, dtype=torch.uint8, device=cuda) for n in (512, 1 << 12, 1 << 16, 1 << 20)]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want) and len(keep) == 4
+
+
 def test_copies_of_a_weight():
     """A copied or pickled weight holds its parts and no table of another's."""
     qw = _cpu_weight()
