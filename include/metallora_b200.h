@@ -494,6 +494,48 @@ MLORA_API int mlora_lora_grads_static(const void* dy, const void* x, const void*
                                       int64_t r, float alpha, float clip_value, int dtype,
                                       void* stream);
 
+/* ---- cross entropy of a linear head ------------------------------------- */
+
+/* Which gradients a call makes (flags). */
+#define MLORA_HEAD_GRAD_X 1  /* of the hidden states */
+#define MLORA_HEAD_GRAD_W 2  /* of the head's weight (trained head) */
+#define MLORA_HEAD_GRAD_AB 4 /* of the head's LoRA factors */
+
+/* Softmax cross entropy over a vocabulary of V entries, from the hidden states
+ * x [M, K], the head's weight w [V, K] and, with r > 0, its LoRA factors a [r, K]
+ * and b [V, r] (logits x.w^T + (alpha/r)(x.a^T).b^T); no [M, V] array is kept.
+ * labels: M int64; a token labelled ignore_index has no loss and no gradient, nor
+ * has one whose label is outside [0, V) (device status 0x107).  Writes the sum, or
+ * with `mean` the mean, over the other tokens to *loss, and/or each token's loss
+ * (0 for those without) to row_loss [M].  BF16 or F16; K and r multiples of 8, with
+ * r > 0 V too.
+ *   The gradients named in `grads` are made here, up to the upstream factor, and
+ * kept in `state` (256-byte aligned, mlora_linear_cross_entropy_state_bytes;
+ * overwritten) for the call below; without `grads` the state is small and only
+ * needed during the call. */
+MLORA_API size_t mlora_linear_cross_entropy_state_bytes(int64_t M, int64_t K, int64_t V, int64_t r,
+                                                        int dtype, int grads);
+MLORA_API size_t mlora_linear_cross_entropy_workspace_bytes(int64_t M, int64_t K, int64_t V,
+                                                            int64_t r, int dtype, int grads);
+MLORA_API int mlora_linear_cross_entropy(const void* x, const void* w, const void* a,
+                                         const void* b, const int64_t* labels, float* loss,
+                                         float* row_loss, void* state, size_t state_bytes,
+                                         int64_t M, int64_t K, int64_t V, int64_t r, float alpha,
+                                         int64_t ignore_index, int mean, int dtype, int grads,
+                                         void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradients of the call that filled `state` (same sizes, `mean` and grads), times
+ * the upstream gradient: *grad, or with per_row the M values grad[m] of row_loss
+ * (then only dx).  dx [M, K] and dw [V, K] are of `dtype`, da [r, K] and db [V, r]
+ * of ab_dtype; with accumulate_ab they are added to.  Each is NULL unless its
+ * flag is set.  The state is only read: a second call gives the same. */
+MLORA_API int mlora_linear_cross_entropy_backward(const void* state, size_t state_bytes,
+                                                  const float* grad, int per_row, int mean,
+                                                  const void* w, void* dx, void* da, void* db,
+                                                  int ab_dtype, int accumulate_ab, void* dw,
+                                                  int64_t M, int64_t K, int64_t V, int64_t r,
+                                                  int dtype, int grads, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,10 @@ BWD_DEFER_DX = 2
 BWD_DX_ONLY = 4
 BWD_GRADS_16BIT = 8
 
+HEAD_GRAD_X = 1
+HEAD_GRAD_W = 2
+HEAD_GRAD_AB = 4
+
 QUANT_NF4 = 1
 QUANT_INT4 = 2
 QUANT_INT8 = 3
@@ -112,6 +116,12 @@ SIGNATURES: dict[str, tuple] = {
     "mlora_lora_grads_static_scratch_bytes": (sz, []),
     "mlora_lora_grads_static": (i32, [vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, f32, f32, i32,
                                       vp]),
+    "mlora_linear_cross_entropy_state_bytes": (sz, [i64, i64, i64, i64, i32, i32]),
+    "mlora_linear_cross_entropy_workspace_bytes": (sz, [i64, i64, i64, i64, i32, i32]),
+    "mlora_linear_cross_entropy": (i32, [vp] * 8 + [sz] + [i64] * 4 + [f32, i64, i32, i32, i32, vp,
+                                                                       sz, vp]),
+    "mlora_linear_cross_entropy_backward": (i32, [vp, sz, vp, i32, i32, vp, vp, vp, vp, i32, i32,
+                                                  vp, i64, i64, i64, i64, i32, i32, vp]),
 }
 
 

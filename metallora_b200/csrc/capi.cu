@@ -819,6 +819,8 @@ int set_max_smem(const void* kern, size_t bytes, std::atomic<bool>* done) {
   return MLORA_OK;
 }
 
+int require_device() { return check_device(); }
+
 uint32_t* device_status_ptr() { return dev_info().status; }
 int num_sms() {
   const int s = dev_info().sms;

@@ -1,0 +1,410 @@
+// The three products of a vocabulary head, as one persistent tcgen05 kernel over
+// CTA pairs:
+//
+//   logits  D[m, v] = sum_k x[m, k] W[v, k]   (+ X2[m, :] . B[v, :])   both K-major
+//   dx      D[m, k] = sum_v g[m, v] W[v, k]   (+ U[m, :] . A[:, k])    W MN-major
+//   dW      D[v, k] = sum_m g[m, v] x[m, k]                            both MN-major
+//
+// A (2,1,1) cluster makes a 256 x 256 tile (tcgen05.mma.cta_group::2, M = N = 256,
+// K = 16): each CTA stages its own 128 rows of either operand in a 6-stage TMA ring
+// and holds its own 128 rows of the fp32 accumulator, two of them in TMEM, so that
+// the epilogue of one tile runs beside the main loop of the next.  The roles of the
+// warps are those of the LoRA GEMM (tc_gemm.cu).  What is new here:
+//   * the number of counted tokens is read on the device: it bounds the rows of D
+//     (logits, dx) or the reduction (dW), so that tokens that do not count cost
+//     nothing and no host waits for their number;
+//   * the reduction can be cut into `splits` ranges, each with its own fp32 copy of D
+//     (dx of few tokens has few tiles and a reduction over the whole vocabulary);
+//     whoever reads D adds the copies in order.
+// Bound: the tensor pipe; by HBM (one read of W) below some 250 tokens.
+#include <atomic>
+#include <string>
+
+#include "internal.h"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "../../include/metallora_b200.h"
+
+namespace mlora {
+namespace {
+
+constexpr int kBK = 64;
+constexpr int kHalf = 128;  // rows of either operand per CTA
+constexpr int kTile = 2 * kHalf;
+constexpr int kStages = 6;
+constexpr uint32_t kOpBytes = kHalf * kBK * 2;      // 16 KB
+constexpr uint32_t kStageBytes = 2 * kOpBytes;
+constexpr uint32_t kMNBoxBytes = 64 * kBK * 2;      // one MN-major TMA box (8 KB)
+constexpr int kEpiWarps = 4;
+constexpr int kThreads = 64 + 32 * kEpiWarps;
+constexpr uint32_t kTmemCols = 512;
+constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + 256;
+
+struct HeadGemmParams {
+  int M, N;  // of D; at most, where `rows` bounds them
+  int num_kb_main, num_kb_extra, R;
+  int tiles_n, splits, group_m;
+  const int32_t* rows;  // counted tokens (device), of which those from row0 on are meant
+  int row0;
+  int rows_on_k;  // they bound the reduction, else the rows of D
+  float* d;
+  long long ldd, split_stride;
+  int accumulate;
+  uint32_t* status;
+};
+
+struct Shape {
+  int M, num_kb, tiles_m, num_tiles, units;
+};
+
+__device__ __forceinline__ Shape device_shape(const HeadGemmParams& p) {
+  Shape s;
+  s.M = p.M;
+  s.num_kb = p.num_kb_main;
+  if (p.rows != nullptr) {
+    const int n = max(*p.rows - p.row0, 0);
+    if (p.rows_on_k)
+      s.num_kb = min(s.num_kb, (n + kBK - 1) / kBK);
+    else
+      s.M = min(s.M, n);
+  }
+  s.tiles_m = (s.M + kTile - 1) / kTile;
+  s.num_tiles = s.tiles_m * p.tiles_n;
+  s.units = s.num_tiles * p.splits;
+  return s;
+}
+
+// One unit of work: a tile of D and a range of the reduction.  Tile rows vary
+// fastest inside groups of group_m of them, so that the tiles in flight cover a
+// compact block of D and share their operands in L2.
+struct Unit {
+  int tm, tn, split, kb0, kb1, total;
+};
+
+__device__ __forceinline__ Unit unit_at(const HeadGemmParams& p, const Shape& s, int u) {
+  Unit t;
+  t.split = u / s.num_tiles;
+  const int tile = u - t.split * s.num_tiles;
+  const int per_group = p.group_m * p.tiles_n;
+  const int g = tile / per_group;
+  const int rem = tile - g * per_group;
+  const int rows = min(p.group_m, s.tiles_m - g * p.group_m);
+  t.tm = g * p.group_m + rem % rows;
+  t.tn = rem / rows;
+  t.kb0 = static_cast<int>(static_cast<long long>(s.num_kb) * t.split / p.splits);
+  t.kb1 = static_cast<int>(static_cast<long long>(s.num_kb) * (t.split + 1) / p.splits);
+  t.total = t.kb1 - t.kb0 + (t.split == 0 ? p.num_kb_extra : 0);
+  return t;
+}
+
+// This thread's row of the accumulator into D, 32 bytes at a time.
+__device__ __forceinline__ void store_row_f32(const HeadGemmParams& p, const Shape& s,
+                                              const Unit& t, int m, uint32_t taddr) {
+  float* row = p.d + t.split * p.split_stride + static_cast<long long>(m) * p.ldd +
+               static_cast<long long>(t.tn) * kTile;
+#pragma unroll 1
+  for (int c = 0; c < kTile / 32; ++c) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(taddr + c * 32, r);
+    tmem_ld_wait();
+    if (m >= s.M) continue;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      if (t.tn * kTile + c * 32 + q * 8 >= p.N) continue;
+      float* dst = row + c * 32 + q * 8;
+      uint32_t v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = t.total > 0 ? r[q * 8 + i] : 0u;
+      if (p.accumulate) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float4 o = *reinterpret_cast<const float4*>(dst + 4 * h);
+          v[4 * h] = __float_as_uint(__uint_as_float(v[4 * h]) + o.x);
+          v[4 * h + 1] = __float_as_uint(__uint_as_float(v[4 * h + 1]) + o.y);
+          v[4 * h + 2] = __float_as_uint(__uint_as_float(v[4 * h + 2]) + o.z);
+          v[4 * h + 3] = __float_as_uint(__uint_as_float(v[4 * h + 3]) + o.w);
+        }
+      }
+      st_global_32b(dst, v);
+    }
+  }
+}
+
+template <bool kXMN, bool kWMN, bool kBF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    head_gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
+                     const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_x2,
+                     const __grid_constant__ CUtensorMap tm_w2, const HeadGemmParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem<1024>(smem_raw);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
+  uint64_t* empty_bar = full_bar + kStages;
+  uint64_t* acc_full = empty_bar + kStages;  // [2]
+  uint64_t* acc_empty = acc_full + 2;        // [2]
+  uint64_t* drain_bar = acc_empty + 2;       // [1]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+
+  const uint32_t warp = warp_id();
+  const uint32_t lane = lane_id();
+  const uint32_t crank = cluster_ctarank();
+  const bool lead = crank == 0;
+  const int pair = static_cast<int>(blockIdx.x >> 1);
+  const int num_pairs = static_cast<int>(gridDim.x >> 1);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);
+    }
+    mbar_init(drain_bar, 1);
+    fence_mbarrier_init();
+    prefetch_tmap(&tm_x);
+    prefetch_tmap(&tm_w);
+    if (p.num_kb_extra > 0) {
+      prefetch_tmap(&tm_x2);
+      prefetch_tmap(&tm_w2);
+    }
+  }
+  __syncwarp();  // the allocation below is a warp-wide instruction
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, kTmemCols);
+    tmem_relinquish_pair();
+  }
+  const Shape shape = device_shape(p);
+  tc_fence_before();
+  cluster_sync();  // both CTAs' barriers initialised and TMEM allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer --
+    if (elect_one()) {
+      const uint32_t lead_full = mapa_shared(smem_u32(full_bar), 0);
+      uint32_t stage = 0, phase = 0;
+      uint32_t armed_parity[kStages];
+      bool armed[kStages];
+      for (int s = 0; s < kStages; ++s) armed[s] = false, armed_parity[s] = 0;
+      bool ok = true;
+      for (int u = pair; u < shape.units && ok; u += num_pairs) {
+        const Unit t = unit_at(p, shape, u);
+        const int m0 = t.tm * kTile + static_cast<int>(crank) * kHalf;
+        const int n0 = t.tn * kTile + static_cast<int>(crank) * kHalf;
+        const int main_kb = t.kb1 - t.kb0;
+        for (int i = 0; i < t.total; ++i) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          uint8_t* sx = smem + stage * kStageBytes;
+          uint8_t* sw = sx + kOpBytes;
+          if (lead) {
+            mbar_arrive_expect_tx(&full_bar[stage], 2 * kStageBytes);
+            armed[stage] = true;
+            armed_parity[stage] = phase;
+          }
+          const uint32_t bar = lead_full + stage * 8u;
+          const bool extra = i >= main_kb;
+          const CUtensorMap* mx = extra ? &tm_x2 : &tm_x;
+          const CUtensorMap* mw = extra ? &tm_w2 : &tm_w;
+          const int k0 = (extra ? i - main_kb : t.kb0 + i) * kBK;
+          if constexpr (kXMN) {
+            tma_load_2d_pair(sx, mx, bar, m0, k0);
+            tma_load_2d_pair(sx + kMNBoxBytes, mx, bar, m0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sx, mx, bar, k0, m0);
+          }
+          if constexpr (kWMN) {
+            tma_load_2d_pair(sw, mw, bar, n0, k0);
+            tma_load_2d_pair(sw + kMNBoxBytes, mw, bar, n0 + 64, k0);
+          } else {
+            tma_load_2d_pair(sw, mw, bar, k0, n0);
+          }
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+      }
+      // Never leave a copy in flight at exit (the even CTA's barriers count
+      // both CTAs' bytes).
+      for (int s = 0; s < kStages; ++s)
+        if (armed[s]) mbar_wait(&full_bar[s], armed_parity[s], p.status, kDevTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------- MMA (even CTA only) --
+    if (lead && elect_one()) {
+      constexpr uint32_t idesc = make_idesc_f16(kTile, kTile, kXMN, kWMN, kBF16);
+      const uint32_t peer_empty = mapa_shared(smem_u32(empty_bar), 1);
+      const uint32_t peer_acc_full = mapa_shared(smem_u32(acc_full), 1);
+      uint32_t stage = 0, phase = 0;
+      int local = 0;
+      bool ok = true;
+      for (int u = pair; u < shape.units && ok; u += num_pairs, ++local) {
+        const Unit t = unit_at(p, shape, u);
+        const int main_kb = t.kb1 - t.kb0;
+        const uint32_t buf = local & 1;
+        const uint32_t use = static_cast<uint32_t>(local >> 1) & 1u;
+        if (!mbar_wait(&acc_empty[buf], use ^ 1u, p.status, kDevTimeoutAccEmpty)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * kTile;
+        for (int i = 0; i < t.total; ++i) {
+          if (!mbar_wait(&full_bar[stage], phase, p.status, kDevTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sx = smem_u32(smem + stage * kStageBytes);
+          const uint32_t sw = sx + kOpBytes;
+          int nk = 4;
+          if (i >= main_kb) {
+            const int rem = p.R - (i - main_kb) * kBK;
+            nk = rem >= kBK ? 4 : rem / 16;
+          }
+          for (int k = 0; k < nk; ++k) {
+            const uint64_t ad = kXMN ? desc_mnmajor_sw128(sx, k, kMNBoxBytes)
+                                     : desc_kmajor_sw128(sx, k);
+            const uint64_t bd = kWMN ? desc_mnmajor_sw128(sw, k, kMNBoxBytes)
+                                     : desc_kmajor_sw128(sw, k);
+            umma_f16_pair(d_tmem, ad, bd, idesc, (i | k) != 0 ? 1u : 0u);
+          }
+          umma_commit_pair(smem_u32(&empty_bar[stage]));
+          umma_commit_pair(peer_empty + stage * 8u);
+          if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+        if (!ok) break;
+        umma_commit_pair(smem_u32(&acc_full[buf]));
+        umma_commit_pair(peer_acc_full + buf * 8u);
+      }
+      // Drain: every MMA issued above has completed before TMEM is released.
+      umma_commit_pair(smem_u32(drain_bar));
+      mbar_wait(drain_bar, 0, p.status, kDevTimeoutDrain);
+    }
+  } else {
+    // ----------------------------------------------------------- epilogue --
+    const uint32_t quarter = warp & 3u;  // TMEM lanes [32*quarter, 32*quarter+32)
+    const uint32_t lead_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
+    int local = 0;
+    for (int u = pair; u < shape.units; u += num_pairs, ++local) {
+      const Unit t = unit_at(p, shape, u);
+      const uint32_t buf = local & 1;
+      const uint32_t use = static_cast<uint32_t>(local >> 1) & 1u;
+      if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
+      tc_fence_after();
+      const int m = t.tm * kTile + static_cast<int>(crank * kHalf + quarter * 32 + lane);
+      store_row_f32(p, shape, t, m, tmem_base + ((quarter * 32u) << 16) + buf * kTile);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(lead_acc_empty + buf * 8u);
+    }
+  }
+
+  // After a failure the odd CTA may still have copies in flight that no
+  // barrier of its own tracks: give them time to land before the pair exits.
+  if (wait_failed(p.status)) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no arrival or copy from the other CTA is still pending
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, kTmemCols);
+  }
+}
+
+template <bool kXMN, bool kWMN, bool kBF16>
+int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
+  CUtensorMap tx, tw, tx2, tw2;
+  if (kXMN ? !make_tmap_2d_16b(&tx, a.x, a.M, a.K, a.ldx, 64, kBK)
+           : !make_tmap_2d_16b(&tx, a.x, a.K, a.M, a.ldx, kBK, kHalf))
+    return MLORA_ERR_INVALID_ARG;
+  if (kWMN ? !make_tmap_2d_16b(&tw, a.w, a.N, a.K, a.ldw, 64, kBK)
+           : !make_tmap_2d_16b(&tw, a.w, a.K, a.N, a.ldw, kBK, kHalf))
+    return MLORA_ERR_INVALID_ARG;
+  tx2 = tx;
+  tw2 = tw;
+  if (a.R > 0) {
+    const int64_t r64 = (a.R + 63) / 64 * 64;
+    if (!make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK, kHalf)) return MLORA_ERR_INVALID_ARG;
+    if (kWMN ? !make_tmap_2d_16b(&tw2, a.w2, a.N, a.w2_rows, a.ldw2, 64, kBK)
+             : !make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK, kHalf))
+      return MLORA_ERR_INVALID_ARG;
+  }
+  HeadGemmParams p;
+  p.M = static_cast<int>(a.M);
+  p.N = static_cast<int>(a.n_store);
+  p.num_kb_main = static_cast<int>((a.K + kBK - 1) / kBK);
+  p.R = static_cast<int>(a.R);
+  p.num_kb_extra = static_cast<int>((a.R + kBK - 1) / kBK);
+  const int tiles_m = static_cast<int>((a.M + kTile - 1) / kTile);
+  p.tiles_n = static_cast<int>((a.n_store + kTile - 1) / kTile);
+  p.splits = a.splits;
+  p.group_m = a.group_m < tiles_m ? a.group_m : tiles_m;
+  p.rows = a.rows;
+  p.row0 = static_cast<int>(a.row0);
+  p.rows_on_k = kXMN ? 1 : 0;
+  p.d = a.d;
+  p.ldd = a.ldd;
+  p.split_stride = a.split_stride;
+  p.accumulate = a.accumulate ? 1 : 0;
+  p.status = device_status_ptr();
+
+  auto kern = head_gemm_kernel<kXMN, kWMN, kBF16>;
+  static std::atomic<bool> attr_set[64];
+  if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), kSmemBytes, attr_set)) return rc;
+  const int64_t units = int64_t{tiles_m} * p.tiles_n * p.splits;
+  const int pairs = head_gemm_pairs();
+  const int grid = 2 * static_cast<int>(units < pairs ? units : pairs);
+  LaunchScope scope(kKindGemm, stream);
+  return launch_status(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), kThreads, kSmemBytes,
+                                     stream, 0, 0, false, tx, tw, tx2, tw2, p),
+                       "head gemm launch");
+}
+
+}  // namespace
+
+int head_gemm_pairs() {
+  static std::atomic<int> known[64];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int n = dev < 64 ? known[dev].load(std::memory_order_acquire) : 0;
+  if (n > 0) return n;
+  // clusters that can be resident at once (GPCs may leave an SM unpaired)
+  const int pairs = num_sms() / 2;
+  auto kern = head_gemm_kernel<false, false, true>;
+  static std::atomic<bool> attr_set[64];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kSmemBytes;
+  if (set_max_smem(reinterpret_cast<const void*>(kern), kSmemBytes, attr_set) != MLORA_OK ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = pairs;
+  }
+  if (n > pairs) n = pairs;
+  if (dev < 64) known[dev].store(n, std::memory_order_release);
+  return n;
+}
+
+int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s) {
+  const bool bf16 = a.elt == Elt::kBF16;
+  switch (a.product) {
+    case HeadProduct::kLogits:
+      return bf16 ? launch_typed<false, false, true>(a, s) : launch_typed<false, false, false>(a, s);
+    case HeadProduct::kDx:
+      return bf16 ? launch_typed<false, true, true>(a, s) : launch_typed<false, true, false>(a, s);
+    case HeadProduct::kDw:
+      return bf16 ? launch_typed<true, true, true>(a, s) : launch_typed<true, true, false>(a, s);
+  }
+  return MLORA_ERR_INVALID_ARG;
+}
+
+}  // namespace mlora

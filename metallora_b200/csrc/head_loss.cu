@@ -1,0 +1,700 @@
+// Cross entropy of a linear head over a large vocabulary, from the hidden states,
+// with its gradient, and no [tokens, vocabulary] array kept:
+//
+//   l = x . W^T (+ s (x . A^T) . B^T),   loss_m = log(sum_v exp l[m, v]) - l[m, y_m]
+//   g[m, v] = softmax(l[m])[v] - [v = y_m]
+//   dx = g . W + s (g . B) . A,  dW = g^T . x,  dB = g^T . (s x A^T),  dA = (s g B)^T . x
+//
+// Tokens labelled ignore_index have no loss and no gradient: the others are first
+// gathered into consecutive rows, and every product runs over those alone (their
+// number stays on the device).  Rows go through in pieces that bound the workspace.
+// The gradients for a unit upstream gradient are made in the forward, while a piece's
+// logits are at hand (a backward that made them would compute the logits again: half
+// as many products more behind a frozen head); the backward scales them.
+#include <algorithm>
+#include <string>
+
+#include "internal.h"
+#include "launch.cuh"
+#include "ptx.cuh"
+#include "../../include/metallora_b200.h"
+
+namespace mlora {
+namespace {
+
+constexpr int kScanThreads = 1024;
+constexpr int kScanItems = 4;
+constexpr int kRowThreads = 256;
+
+// g is kept times this in fp16, so that probabilities down to 2^-20 are normal
+// numbers there; a power of two, undone exactly by whoever scales the result.
+// |g| <= 1, and |s g B| <= 2 s max|B| stays far below fp16's largest number.
+template <typename T>
+__host__ __device__ constexpr float grad_unit() { return 1.f; }
+template <>
+__host__ __device__ constexpr float grad_unit<__half>() { return 64.f; }
+
+struct HeadCount {
+  int32_t counted;
+  float inv;  // 1 / counted, 0 for none
+};
+
+// One CTA: numbers the tokens that count in order.  slot_of[m] = the token's number
+// or -1; row_of[i], label[i] = token i's row and label (row_of = -1 past the last).
+__global__ void __launch_bounds__(kScanThreads)
+    head_scan_kernel(const int64_t* labels, int64_t M, int64_t V, int64_t ignore_index,
+                     int32_t* slot_of, int32_t* row_of, int32_t* label, float* row_loss,
+                     HeadCount* out, uint32_t* status) {
+  __shared__ int32_t warp_sum[kScanThreads / 32];
+  __shared__ int32_t total;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int32_t base = 0;
+  for (int64_t m0 = 0; m0 < M; m0 += kScanThreads * kScanItems) {
+    const int64_t first = m0 + static_cast<int64_t>(threadIdx.x) * kScanItems;
+    int32_t y[kScanItems];
+    int32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < kScanItems; ++i) {
+      y[i] = -1;
+      if (first + i < M) {
+        const int64_t v = labels[first + i];
+        if (v != ignore_index) {
+          if (v >= 0 && v < V)
+            y[i] = static_cast<int32_t>(v);
+          else
+            record_status(status, kDevBadIndex);
+        }
+      }
+      mine += y[i] >= 0;
+    }
+    int32_t run = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t t = __shfl_up_sync(0xffffffffu, run, o);
+      if (lane >= o) run += t;
+    }
+    if (lane == 31) warp_sum[warp] = run;
+    __syncthreads();
+    if (warp == 0) {
+      const int32_t v = warp_sum[lane];
+      int32_t w = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t t = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += t;
+      }
+      warp_sum[lane] = w - v;
+      if (lane == 31) total = w;
+    }
+    __syncthreads();
+    int32_t slot = base + warp_sum[warp] + run - mine;
+#pragma unroll
+    for (int i = 0; i < kScanItems; ++i) {
+      if (first + i >= M) break;
+      const bool counts = y[i] >= 0;
+      slot_of[first + i] = counts ? slot : -1;
+      if (counts) {
+        row_of[slot] = static_cast<int32_t>(first + i);
+        label[slot] = y[i];
+        ++slot;
+      } else if (row_loss != nullptr) {
+        row_loss[first + i] = 0.f;
+      }
+    }
+    base += total;
+    __syncthreads();
+  }
+  for (int64_t i = base + threadIdx.x; i < M; i += kScanThreads) row_of[i] = -1;
+  if (threadIdx.x == 0) {
+    out->counted = base;
+    out->inv = base > 0 ? 1.f / static_cast<float>(base) : 0.f;
+  }
+}
+
+// xc[i] = x[row_of[i]], zeros past the last counted token (as many as a reduction
+// over tokens reads; all of them for the LoRA products, which run over every row).
+__global__ void __launch_bounds__(128)
+    head_gather_kernel(const uint4* x, const int32_t* row_of, const HeadCount* count, int64_t K8,
+                       int zero_all, uint4* xc) {
+  const int64_t i = blockIdx.x;
+  const int32_t row = row_of[i];
+  if (row < 0 && !zero_all && i >= (count->counted + 63) / 64 * 64) return;
+  for (int64_t k = threadIdx.x; k < K8; k += 128)
+    xc[i * K8 + k] = row < 0 ? make_uint4(0, 0, 0, 0) : x[static_cast<int64_t>(row) * K8 + k];
+}
+
+__device__ __forceinline__ void join_max_sum(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2);
+  // two empty parts (or rows of -infinity): nothing to scale by
+  const float ref = top == -INFINITY ? 0.f : top;
+  s = s * __expf(m - ref) + s2 * __expf(m2 - ref);
+  m = top;
+}
+
+// One CTA per counted token of the piece: its loss, and its row of g in 16 bits.
+// What rounding g[y] left over, the largest and always present part, goes to
+// `rest`, which the gradient of x adds back times W[y].
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+    head_row_kernel(const float* logits, int64_t ld, int64_t V, int64_t row0, int64_t rows,
+                    const HeadCount* count, const int32_t* label, const int32_t* row_of,
+                    float* row_loss, float* nll, T* g, float* rest, int zero_all) {
+  __shared__ float sm[kRowThreads / 32], ss[kRowThreads / 32];
+  const int64_t i = blockIdx.x;
+  const int64_t slot = row0 + i;
+  const int32_t counted = count->counted;
+  T* grow = g + i * ld;
+  if (slot >= counted) {
+    if (g != nullptr && (zero_all || slot < (counted + 63) / 64 * 64))
+      for (int64_t v = threadIdx.x; v < ld; v += kRowThreads) grow[v] = static_cast<T>(0.f);
+    return;
+  }
+  const float* l = logits + i * ld;
+  float m = -INFINITY, s = 0.f;
+  for (int64_t v = threadIdx.x; v < V; v += kRowThreads) {
+    const float t = l[v];
+    if (t > m) {
+      s *= __expf(m - t);
+      m = t;
+    }
+    s += t == -INFINITY ? 0.f : __expf(t - m);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    join_max_sum(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m, ss[threadIdx.x >> 5] = s;
+  __syncthreads();
+  m = sm[0], s = ss[0];
+  for (int w = 1; w < kRowThreads / 32; ++w) join_max_sum(m, s, sm[w], ss[w]);
+  const int32_t y = label[slot];
+  const float log_sum = logf(s);
+  const float loss = log_sum + (m - l[y]);
+  if (threadIdx.x == 0) {
+    nll[slot] = loss;
+    if (row_loss != nullptr) row_loss[row_of[slot]] = loss;
+  }
+  if (g == nullptr) return;
+  constexpr float unit = grad_unit<T>();
+  const float inv = unit / s;
+  for (int64_t v = threadIdx.x; v < ld; v += kRowThreads) {
+    float o = v < V ? __expf(l[v] - m) * inv : 0.f;
+    if (v == y) {
+      o = unit * expm1f(-loss);  // p - 1 without cancellation
+      rest[slot] = o - static_cast<float>(static_cast<T>(o));
+    }
+    grow[v] = static_cast<T>(o);
+  }
+}
+
+// loss = sum of the counted tokens' losses, or their mean (of none: NaN, as 0 / 0 is).
+__global__ void __launch_bounds__(1024)
+    head_reduce_kernel(const float* nll, const HeadCount* count, int mean, float* loss) {
+  __shared__ double part[32];
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < count->counted; i += 1024) s += nll[i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) s += part[w];
+    *loss = static_cast<float>(mean ? s / count->counted : s);
+  }
+}
+
+// dx[row] = grad (sum over splits of part[split][slot] / unit + rest[slot] / unit W[y]);
+// zeros for tokens that do not count.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    head_dx_kernel(const float* part, int64_t split_stride, int splits, const int32_t* slot_of,
+                   const int32_t* label, const float* rest, const T* w, const HeadCount* count,
+                   const float* grad, int per_row, int mean, int64_t K, T* dx) {
+  const int64_t row = blockIdx.x;
+  const int64_t k = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * 8;
+  if (k >= K) return;
+  const int32_t slot = slot_of[row];
+  float v[8] = {};
+  if (slot >= 0) {
+    const float* src = part + static_cast<int64_t>(slot) * K + k;
+    for (int s = 0; s < splits; ++s, src += split_stride) {
+      const float4 a = *reinterpret_cast<const float4*>(src);
+      const float4 b = *reinterpret_cast<const float4*>(src + 4);
+      v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+      v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+    }
+    const float scale = grad[per_row ? row : 0] * (mean ? count->inv : 1.f) * (1.f / grad_unit<T>());
+    const float left = rest[slot];
+    const uint4 wv = *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(label[slot]) * K + k);
+    const T* we = reinterpret_cast<const T*>(&wv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = scale * fmaf(left, static_cast<float>(we[i]), v[i]);
+  }
+  uint4 o;
+  o.x = pack2<T>(v[0], v[1]);
+  o.y = pack2<T>(v[2], v[3]);
+  o.z = pack2<T>(v[4], v[5]);
+  o.w = pack2<T>(v[6], v[7]);
+  *reinterpret_cast<uint4*>(dx + row * K + k) = o;
+}
+
+template <typename O>
+__device__ __forceinline__ void store8(O* dst, const float (&v)[8]) {
+  if constexpr (sizeof(O) == 2) {
+    *reinterpret_cast<uint4*>(dst) = make_uint4(pack2<O>(v[0], v[1]), pack2<O>(v[2], v[3]),
+                                                pack2<O>(v[4], v[5]), pack2<O>(v[6], v[7]));
+  } else {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+
+// out (+)= grad / unit * src, n a multiple of 8; a gradient of a weight.  (Where no
+// token counted, src is zero and so is the result, whatever grad is.)
+template <typename O>
+__global__ void __launch_bounds__(256)
+    head_scale_kernel(const float* src, int64_t n8, const HeadCount* count, const float* grad,
+                      int mean, float inv_unit, int accumulate, O* out) {
+  const float scale = count->counted > 0 ? *grad * (mean ? count->inv : 1.f) * inv_unit : 0.f;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n8;
+       i += static_cast<int64_t>(gridDim.x) * 256) {
+    const float4 a = reinterpret_cast<const float4*>(src)[2 * i];
+    const float4 b = reinterpret_cast<const float4*>(src)[2 * i + 1];
+    float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = scale == 0.f ? 0.f : v[j] * scale;
+      if (accumulate) v[j] += static_cast<float>(out[i * 8 + j]);
+    }
+    store8(out + i * 8, v);
+  }
+}
+
+// ------------------------------------------------------------------- host --
+
+int fail(int code, const std::string& msg) {
+  set_error(msg);
+  return code;
+}
+
+bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
+
+struct Carve {
+  uint8_t* base;
+  int64_t off = 0;
+  explicit Carve(void* b) : base(static_cast<uint8_t*>(b)) {}
+  template <typename T>
+  T* take(int64_t n) {
+    off = round_up(off, 256);
+    T* p = base != nullptr ? reinterpret_cast<T*>(base + off) : nullptr;
+    off += n * static_cast<int64_t>(sizeof(T));
+    return p;
+  }
+};
+
+struct Dims {
+  int64_t M, K, V, r;
+  int grads;
+  bool lora() const { return r > 0; }
+  bool want(int g) const { return (grads & g) != 0; }
+  int64_t R() const {
+    int64_t v = 16;
+    while (v < r) v *= 2;
+    return v;
+  }
+  int64_t R64() const { return round_up(R(), 64); }
+  int64_t ld() const { return round_up(V, 8); }
+};
+
+// Ranges of the vocabulary that dx is summed over: enough for the tiles of few tokens
+// to occupy every CTA pair, against the copies that the backward then reads.  The rule
+// takes the count with the least time for whole waves of tiles (a 256 x 256 x 64 step
+// takes 0.29 us) plus writing and reading the copies.
+int dx_splits(const Dims& d) {
+  const int64_t tiles = (d.M + 255) / 256 * ((d.K + 255) / 256);
+  const int64_t kbs = (d.V + 63) / 64;
+  const int64_t pairs = num_sms() / 2;
+  int best = 1;
+  double best_us = 0;
+  for (int s = 1; s <= 32 && s <= kbs; ++s) {
+    const double waves = static_cast<double>((tiles * s + pairs - 1) / pairs);
+    const double us = waves * static_cast<double>((kbs + s - 1) / s) * 0.29 +
+                      static_cast<double>(s) * d.M * d.K * 8 / 6.0e6;
+    if (s == 1 || us < best_us) best = s, best_us = us;
+  }
+  return best;
+}
+
+// What the backward takes.
+struct State {
+  HeadCount* count;
+  int32_t *slot_of, *label;
+  float *rest, *dx, *da, *db, *dw;
+  int splits;
+  int64_t bytes;
+};
+
+State plan_state(void* base, const Dims& d) {
+  State s{};
+  Carve c(base);
+  s.splits = dx_splits(d);
+  s.count = c.take<HeadCount>(1);
+  s.slot_of = c.take<int32_t>(d.M);
+  s.label = c.take<int32_t>(d.M);
+  s.rest = c.take<float>(d.M);
+  if (d.want(MLORA_HEAD_GRAD_X)) s.dx = c.take<float>(s.splits * d.M * d.K);
+  if (d.want(MLORA_HEAD_GRAD_AB)) {
+    s.da = c.take<float>(d.r * d.K);
+    s.db = c.take<float>(d.V * d.r);
+  }
+  if (d.want(MLORA_HEAD_GRAD_W)) s.dw = c.take<float>(d.V * d.K);
+  s.bytes = round_up(c.off, 256);
+  return s;
+}
+
+struct Work {
+  int32_t* row_of;
+  float* nll;
+  void *xc, *xa_rows, *xa_t, *bt, *u_rows, *u_t, *g;
+  float* logits;
+  int64_t piece;  // rows that go through at a time
+  int64_t bytes;
+};
+
+Work plan_work(void* base, const Dims& d) {
+  Work w{};
+  Carve c(base);
+  // pieces of a gigabyte and a half (or 256 rows), equal up to the tile
+  const int64_t per_row = d.ld() * (d.grads ? 6 : 4);
+  int64_t most = std::max<int64_t>(int64_t{1536} << 20, 256 * per_row) / per_row / 256 * 256;
+  const int64_t n = (d.M + most - 1) / most;
+  w.piece = std::min(d.M, round_up((d.M + n - 1) / n, 256));
+  w.row_of = c.take<int32_t>(d.M);
+  w.nll = c.take<float>(d.M);
+  w.xc = c.take<uint16_t>(d.M * d.K);
+  if (d.lora()) {
+    w.xa_rows = c.take<uint16_t>(d.M * d.R64());
+    w.xa_t = c.take<uint16_t>(d.R() * round_up(d.M, 8));
+    if (d.grads) {
+      w.bt = c.take<uint16_t>(d.R() * d.V);
+      w.u_rows = c.take<uint16_t>(w.piece * d.R64());
+      w.u_t = c.take<uint16_t>(d.R() * round_up(w.piece, 8));
+    }
+  }
+  w.logits = c.take<float>(w.piece * d.ld());
+  if (d.grads) w.g = c.take<uint16_t>(w.piece * d.ld());
+  w.bytes = round_up(c.off, 256);
+  return w;
+}
+
+int check_dims(const Dims& d, int dtype) {
+  if (d.M <= 0 || d.K <= 0 || d.V <= 0) return fail(MLORA_ERR_INVALID_ARG, "M, K, V must be positive");
+  if (dtype != MLORA_DTYPE_BF16 && dtype != MLORA_DTYPE_F16)
+    return fail(MLORA_ERR_UNSUPPORTED, "the linear cross entropy takes BF16 or F16");
+  if (d.grads & ~(MLORA_HEAD_GRAD_X | MLORA_HEAD_GRAD_W | MLORA_HEAD_GRAD_AB))
+    return fail(MLORA_ERR_INVALID_ARG, "unknown gradient flags");
+  if (d.r < 0 || d.r > 256) return fail(MLORA_ERR_INVALID_ARG, "rank must be in [0, 256]");
+  if ((d.grads & MLORA_HEAD_GRAD_AB) && d.r == 0)
+    return fail(MLORA_ERR_INVALID_ARG, "gradients of A and B need a rank");
+  if (d.K % 8 || d.r % 8)
+    return fail(MLORA_ERR_UNSUPPORTED, "K and r must be multiples of 8 (16-byte rows)");
+  if (d.lora() && d.V % 8)
+    return fail(MLORA_ERR_UNSUPPORTED, "a LoRA head needs V % 8 == 0 (16-byte rows of B^T)");
+  if (d.M > (int64_t{1} << 31) - 256 || d.K > (1 << 24) || d.V > (1 << 24))
+    return fail(MLORA_ERR_UNSUPPORTED, "shape too large");
+  return MLORA_OK;
+}
+
+template <typename T>
+int forward(const void* x, const void* w, const void* a, const void* b, const int64_t* labels,
+            float* loss, float* row_loss, const State& st, const Work& ws, const Dims& d,
+            float alpha, int64_t ignore_index, bool mean, cudaStream_t s) {
+  const Elt elt = std::is_same<T, __half>::value ? Elt::kF16 : Elt::kBF16;
+  const int64_t M = d.M, K = d.K, V = d.V, ld = d.ld();
+  const int zero_all = d.lora() ? 1 : 0;
+  int rc;
+  {
+    LaunchScope scope(kKindElementwise, s);
+    head_scan_kernel<<<1, kScanThreads, 0, s>>>(labels, M, V, ignore_index, st.slot_of, ws.row_of,
+                                               st.label, row_loss, st.count, device_status_ptr());
+  }
+  {
+    LaunchScope scope(kKindElementwise, s);
+    head_gather_kernel<<<static_cast<unsigned>(M), 128, 0, s>>>(
+        static_cast<const uint4*>(x), ws.row_of, st.count, K / 8, zero_all,
+        static_cast<uint4*>(ws.xc));
+  }
+  if ((rc = launch_status(cudaSuccess, "linear cross entropy: gather"))) return rc;
+  RankArgs ra;
+  if (d.lora()) {
+    ra.x = ws.xc;
+    ra.l = a;
+    ra.M = M;
+    ra.K = K;
+    ra.r = d.r;
+    ra.R = d.R();
+    ra.ldx = K;
+    ra.ldl = K;
+    ra.scale = alpha / static_cast<float>(d.r);
+    ra.out_rows = ws.xa_rows;
+    ra.ld_rows = d.R64();
+    ra.out_t = ws.xa_t;
+    ra.ld_t = round_up(M, 8);
+    ra.splits = rank_splits(M, K);
+    ra.elt = elt;
+    if ((rc = launch_rank(ra, s))) return rc;
+    if (d.grads && (rc = launch_transpose_pad(b, V, d.r, d.r, ws.bt, d.R(), elt, s))) return rc;
+  }
+  for (int64_t row0 = 0; row0 < M; row0 += ws.piece) {
+    const int64_t rows = std::min(ws.piece, M - row0);
+    const T* xc = static_cast<const T*>(ws.xc) + row0 * K;
+    HeadGemmArgs l;
+    l.product = HeadProduct::kLogits;
+    l.x = xc;
+    l.w = w;
+    l.d = ws.logits;
+    l.M = rows;
+    l.N = V;
+    l.K = K;
+    l.n_store = ld;
+    l.ldx = K;
+    l.ldw = K;
+    l.ldd = ld;
+    l.rows = &st.count->counted;
+    l.row0 = row0;
+    l.elt = elt;
+    if (d.lora()) {
+      l.x2 = static_cast<const T*>(ws.xa_rows) + row0 * d.R64();
+      l.w2 = b;
+      l.R = d.R();
+      l.w2_rows = d.r;
+      l.ldx2 = d.R64();
+      l.ldw2 = d.r;
+    }
+    if ((rc = launch_head_gemm(l, s))) return rc;
+    {
+      LaunchScope scope(kKindElementwise, s);
+      head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, 0, s>>>(
+          ws.logits, ld, V, row0, rows, st.count, st.label, ws.row_of, row_loss, ws.nll,
+          static_cast<T*>(ws.g), st.rest, zero_all);
+      if ((rc = launch_status(cudaSuccess, "linear cross entropy: rows"))) return rc;
+    }
+    if (d.lora() && d.grads) {
+      RankArgs ru = ra;  // U = s g B
+      ru.x = ws.g;
+      ru.l = ws.bt;
+      ru.M = rows;
+      ru.K = V;
+      ru.r = d.R();
+      ru.ldx = ld;
+      ru.ldl = V;
+      ru.out_rows = ws.u_rows;
+      ru.out_t = ws.u_t;
+      ru.ld_t = round_up(ws.piece, 8);
+      ru.splits = rank_splits(rows, V);
+      if ((rc = launch_rank(ru, s))) return rc;
+      if (d.want(MLORA_HEAD_GRAD_AB)) {
+        WgradArgs g[2];
+        g[0].big = ws.g;
+        g[0].st = static_cast<const T*>(ws.xa_t) + row0;
+        g[0].ld_st = round_up(M, 8);
+        g[0].M = rows;
+        g[0].P = V;
+        g[0].r = d.r;
+        g[0].R = d.R();
+        g[0].ldb = ld;
+        g[0].out = st.db;
+        g[0].ldo = d.r;
+        g[0].transposed = false;
+        g[0].accumulate = row0 > 0;
+        g[0].clip = 0.f;
+        g[0].splits = wgrad_splits(rows, std::max(V, K), 2);
+        g[0].elt = elt;
+        g[1] = g[0];
+        g[1].big = xc;
+        g[1].st = ws.u_t;
+        g[1].ld_st = round_up(ws.piece, 8);
+        g[1].P = K;
+        g[1].ldb = K;
+        g[1].out = st.da;
+        g[1].ldo = K;
+        g[1].transposed = true;
+        if ((rc = launch_wgrad(g, 2, s))) return rc;
+      }
+    }
+    if (d.want(MLORA_HEAD_GRAD_X)) {
+      HeadGemmArgs q;
+      q.product = HeadProduct::kDx;
+      q.x = ws.g;
+      q.w = w;
+      q.d = st.dx + row0 * K;
+      q.M = rows;
+      q.N = K;
+      q.K = V;
+      q.n_store = K;
+      q.ldx = ld;
+      q.ldw = K;
+      q.ldd = K;
+      q.split_stride = M * K;
+      q.splits = st.splits;
+      q.rows = &st.count->counted;
+      q.row0 = row0;
+      q.elt = elt;
+      if (d.lora()) {
+        q.x2 = ws.u_rows;
+        q.w2 = a;
+        q.R = d.R();
+        q.w2_rows = d.r;
+        q.ldx2 = d.R64();
+        q.ldw2 = K;
+      }
+      if ((rc = launch_head_gemm(q, s))) return rc;
+    }
+    if (d.want(MLORA_HEAD_GRAD_W)) {
+      HeadGemmArgs q;
+      q.product = HeadProduct::kDw;
+      q.x = ws.g;
+      q.w = xc;
+      q.d = st.dw;
+      q.M = V;
+      q.N = K;
+      q.K = rows;
+      q.n_store = K;
+      q.ldx = ld;
+      q.ldw = K;
+      q.ldd = K;
+      q.rows = &st.count->counted;
+      q.row0 = row0;
+      q.group_m = 1;
+      q.accumulate = row0 > 0;
+      q.elt = elt;
+      if ((rc = launch_head_gemm(q, s))) return rc;
+    }
+  }
+  if (loss != nullptr) {
+    LaunchScope scope(kKindElementwise, s);
+    head_reduce_kernel<<<1, 1024, 0, s>>>(ws.nll, st.count, mean ? 1 : 0, loss);
+  }
+  return launch_status(cudaSuccess, "linear cross entropy: loss");
+}
+
+int launch_scale(const float* src, int64_t n, const State& st, const float* grad, bool mean,
+                 float inv_unit, bool accumulate, void* out, int dtype, cudaStream_t s) {
+  const int64_t n8 = n / 8;
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>((n8 + 255) / 256, num_sms() * 16));
+  LaunchScope scope(kKindElementwise, s);
+  const int m = mean ? 1 : 0, acc = accumulate ? 1 : 0;
+  if (dtype == MLORA_DTYPE_BF16)
+    head_scale_kernel<<<grid, 256, 0, s>>>(src, n8, st.count, grad, m, inv_unit, acc,
+                                           static_cast<__nv_bfloat16*>(out));
+  else if (dtype == MLORA_DTYPE_F16)
+    head_scale_kernel<<<grid, 256, 0, s>>>(src, n8, st.count, grad, m, inv_unit, acc,
+                                           static_cast<__half*>(out));
+  else
+    head_scale_kernel<<<grid, 256, 0, s>>>(src, n8, st.count, grad, m, inv_unit, acc,
+                                           static_cast<float*>(out));
+  return launch_status(cudaSuccess, "linear cross entropy: weight gradient");
+}
+
+template <typename T>
+int backward(const State& st, const Dims& d, const void* w, const float* grad, bool per_row,
+             bool mean, void* dx, cudaStream_t s) {
+  LaunchScope scope(kKindElementwise, s);
+  const dim3 grid(static_cast<unsigned>(d.M), static_cast<unsigned>((d.K / 8 + 255) / 256));
+  head_dx_kernel<T><<<grid, 256, 0, s>>>(st.dx, d.M * d.K, st.splits, st.slot_of, st.label, st.rest,
+                                         static_cast<const T*>(w), st.count, grad, per_row ? 1 : 0,
+                                         mean ? 1 : 0, d.K, static_cast<T*>(dx));
+  return launch_status(cudaSuccess, "linear cross entropy: dx");
+}
+
+}  // namespace
+}  // namespace mlora
+
+using namespace mlora;
+
+extern "C" {
+
+size_t mlora_linear_cross_entropy_state_bytes(int64_t M, int64_t K, int64_t V, int64_t r, int dtype,
+                                              int grads) {
+  const Dims d{M, K, V, r, grads};
+  if (check_dims(d, dtype)) return 0;
+  return static_cast<size_t>(plan_state(nullptr, d).bytes);
+}
+
+size_t mlora_linear_cross_entropy_workspace_bytes(int64_t M, int64_t K, int64_t V, int64_t r,
+                                                  int dtype, int grads) {
+  const Dims d{M, K, V, r, grads};
+  if (check_dims(d, dtype)) return 0;
+  return static_cast<size_t>(plan_work(nullptr, d).bytes);
+}
+
+int mlora_linear_cross_entropy(const void* x, const void* w, const void* a, const void* b,
+                               const int64_t* labels, float* loss, float* row_loss, void* state,
+                               size_t state_bytes, int64_t M, int64_t K, int64_t V, int64_t r,
+                               float alpha, int64_t ignore_index, int mean, int dtype, int grads,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  const Dims d{M, K, V, r, grads};
+  if (int rc = check_dims(d, dtype)) return rc;
+  if (!x || !w || !labels || !state || (!loss && !row_loss) || (r > 0 && (!a || !b)))
+    return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (!aligned(x, 16) || !aligned(w, 16) || !aligned(a, 16) || !aligned(b, 16) ||
+      !aligned(labels, 8) || !aligned(loss, 4) || !aligned(row_loss, 4))
+    return fail(MLORA_ERR_INVALID_ARG,
+                "tensor pointers must be 16-byte aligned, labels and losses whole elements");
+  const State st = plan_state(state, d);
+  if (!aligned(state, 256) || state_bytes < static_cast<size_t>(st.bytes))
+    return fail(MLORA_ERR_WORKSPACE, "the state needs " + std::to_string(st.bytes) +
+                                         " bytes on a 256-byte boundary");
+  const Work ws = plan_work(workspace, d);
+  if (!workspace || !aligned(workspace, 256) || workspace_bytes < static_cast<size_t>(ws.bytes))
+    return fail(MLORA_ERR_WORKSPACE, "the workspace needs " + std::to_string(ws.bytes) +
+                                         " bytes on a 256-byte boundary");
+  if (int rc = require_device()) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == MLORA_DTYPE_BF16
+             ? forward<__nv_bfloat16>(x, w, a, b, labels, loss, row_loss, st, ws, d, alpha,
+                                      ignore_index, mean != 0, s)
+             : forward<__half>(x, w, a, b, labels, loss, row_loss, st, ws, d, alpha, ignore_index,
+                               mean != 0, s);
+}
+
+int mlora_linear_cross_entropy_backward(const void* state, size_t state_bytes, const float* grad,
+                                        int per_row, int mean, const void* w, void* dx, void* da,
+                                        void* db, int ab_dtype, int accumulate_ab, void* dw,
+                                        int64_t M, int64_t K, int64_t V, int64_t r, int dtype,
+                                        int grads, void* stream) {
+  const Dims d{M, K, V, r, grads};
+  if (int rc = check_dims(d, dtype)) return rc;
+  if (!state || !grad || !w) return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (d.want(MLORA_HEAD_GRAD_X) != (dx != nullptr) || d.want(MLORA_HEAD_GRAD_AB) != (da != nullptr) ||
+      d.want(MLORA_HEAD_GRAD_AB) != (db != nullptr) || d.want(MLORA_HEAD_GRAD_W) != (dw != nullptr))
+    return fail(MLORA_ERR_INVALID_ARG, "the gradients asked for are those the forward made");
+  if (!aligned(w, 16) || !aligned(dx, 16) || !aligned(da, 16) || !aligned(db, 16) ||
+      !aligned(dw, 16) || !aligned(grad, 4))
+    return fail(MLORA_ERR_INVALID_ARG, "tensor pointers must be 16-byte aligned");
+  if (ab_dtype != MLORA_DTYPE_BF16 && ab_dtype != MLORA_DTYPE_F16 && ab_dtype != MLORA_DTYPE_F32)
+    return fail(MLORA_ERR_UNSUPPORTED, "gradients of A and B are BF16, F16 or F32");
+  if (per_row && (grads & ~MLORA_HEAD_GRAD_X))
+    return fail(MLORA_ERR_UNSUPPORTED, "a gradient per token reaches x alone");
+  const State st = plan_state(const_cast<void*>(state), d);
+  if (!aligned(state, 256) || state_bytes < static_cast<size_t>(st.bytes))
+    return fail(MLORA_ERR_WORKSPACE, "the state is smaller than the forward's");
+  if (int rc = require_device()) return rc;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == MLORA_DTYPE_BF16, avg = mean != 0;
+  const float inv_unit = 1.f / (bf16 ? grad_unit<__nv_bfloat16>() : grad_unit<__half>());
+  int rc = MLORA_OK;
+  if (da != nullptr) {
+    rc = launch_scale(st.da, r * K, st, grad, avg, inv_unit, accumulate_ab != 0, da, ab_dtype, s);
+    if (rc == MLORA_OK)
+      rc = launch_scale(st.db, V * r, st, grad, avg, inv_unit, accumulate_ab != 0, db, ab_dtype, s);
+  }
+  if (rc == MLORA_OK && dx != nullptr)
+    rc = bf16 ? backward<__nv_bfloat16>(st, d, w, grad, per_row != 0, avg, dx, s)
+              : backward<__half>(st, d, w, grad, per_row != 0, avg, dx, s);
+  if (rc == MLORA_OK && dw != nullptr)
+    rc = launch_scale(st.dw, V * K, st, grad, avg, inv_unit, false, dw, dtype, s);
+  return rc;
+}
+
+}  // extern "C"

@@ -63,6 +63,8 @@ class LaunchScope {
 // timeouts here).
 uint32_t* device_status_ptr();
 int num_sms();
+// MLORA_OK, or the error of a device that is not sm_100.
+int require_device();
 
 // ---------------------------------------------------------------- GEMM --------
 // D[M, N] = X[M, K] . W^T + X2[M, R] . W2^T   (fp32 accumulate, one pass over D)
@@ -226,6 +228,34 @@ struct LoraBwdArgs {
   Elt elt;
 };
 int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t stream);
+
+// ------------------------------------------------------- vocabulary head -----
+// The products of the linear cross entropy (head_gemm.cu), fp32 out.  With g the
+// gradient of the logits [tokens, V]:
+//   kLogits: D[m, v] = x . W^T + x2 . w2^T    x [M, K], w [N, K], x2 [M, R64], w2 [N, r]
+//   kDx:     D[m, k] = g . W + x2 . w2        x = g [M, K = V], w [K, N], w2 [r, N]
+//   kDw:     D[v, k] = g^T . x                x = g [K tokens, M = V], w = x [K, N]
+enum class HeadProduct { kLogits, kDx, kDw };
+struct HeadGemmArgs {
+  HeadProduct product;
+  const void* x;
+  const void* w;
+  const void* x2 = nullptr;
+  const void* w2 = nullptr;
+  float* d;                  // `splits` copies of [M, n_store], split_stride floats apart
+  int64_t M = 0, N = 0, K = 0;
+  int64_t n_store = 0;       // columns of D to store: a multiple of 8, at least N
+  int64_t R = 0, w2_rows = 0;
+  int64_t ldx = 0, ldw = 0, ldx2 = 0, ldw2 = 0, ldd = 0, split_stride = 0;
+  int splits = 1;            // at most the 64-wide blocks of the reduction
+  int group_m = 8;           // tile rows per raster group
+  const int32_t* rows = nullptr;  // counted tokens (device); those from row0 on are meant
+  int64_t row0 = 0;
+  bool accumulate = false;   // D += (splits = 1)
+  Elt elt = Elt::kBF16;
+};
+int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s);
+int head_gemm_pairs();  // CTA pairs that are resident at once
 
 // ---------------------------------------------------------------- peers ------
 // One-shot all-reduce over peer memory (see peer.cu); counter: one zeroed

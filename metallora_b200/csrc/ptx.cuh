@@ -110,6 +110,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return done != 0;
 }
 
+// A wait of this process has run out (an index outside its table, the one code that
+// is no lost arrival, stops nothing).
+__device__ __forceinline__ bool wait_failed(const uint32_t* status) {
+  if (status == nullptr) return false;
+  const uint32_t code = *reinterpret_cast<const volatile uint32_t*>(status);
+  return code != 0 && code != kDevBadIndex;
+}
+
 // Waits for the phase with the given parity to complete.  Returns false (and
 // records `code`) if it does not complete within the wait budget.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* status,
@@ -125,7 +133,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
         return false;
       }
       // a peer role may already have failed: stop waiting early
-      if (status != nullptr && *reinterpret_cast<volatile uint32_t*>(status) != 0) return false;
+      if (wait_failed(status)) return false;
     }
   }
 }

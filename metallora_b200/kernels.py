@@ -720,3 +720,111 @@ def lora_kv_cache_update(x2d: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor, 
         _ptr(v_cache), batch, int(cur_pos), max_seq, D_in, D_kv, r, float(alpha_k), code, _ptr(ws),
         ws.numel(), _stream())
     _lib.check(st, "mlora_lora_kv_cache_update")
+
+
+# --------------------------------------------------- linear cross entropy --
+
+@functools.lru_cache(maxsize=256)
+def _head_bytes(M: int, K: int, V: int, r: int, code: int, grads: int) -> tuple[int, int]:
+    """(state, workspace) bytes of a linear cross entropy (a function of the sizes alone)."""
+    lib = _lib.load()
+    args = (M, K, V, r, code, grads)
+    return (lib.mlora_linear_cross_entropy_state_bytes(*args),
+            lib.mlora_linear_cross_entropy_workspace_bytes(*args))
+
+
+def _head_dtype(x2d: torch.Tensor) -> int:
+    if x2d.dtype not in (torch.bfloat16, torch.float16):
+        raise ShapeError("the linear cross entropy takes bf16 or fp16 hidden states")
+    return _DT[x2d.dtype]
+
+
+def linear_cross_entropy_fwd(x2d: torch.Tensor, w: torch.Tensor, labels: torch.Tensor,
+                             a: torch.Tensor | None = None, b: torch.Tensor | None = None,
+                             alpha: float = 16.0, ignore_index: int = -100,
+                             reduction: str = "mean", grads: int = 0):
+    """Softmax cross entropy of the head ``x.W^T (+ (alpha/r)(x.A^T).B^T)`` for 2-D
+    x [M, K], W [V, K] and labels [M].
+
+    Returns (loss, state): loss fp32, a scalar or ("none") one per token; state
+    holds the gradients that ``grads`` (``_lib.HEAD_GRAD_*``) names for a unit
+    upstream gradient, for ``linear_cross_entropy_bwd``."""
+    _need_cuda(x2d, w, labels, a, b)
+    _need_current(x2d, w, labels, *(t for t in (a, b) if t is not None))
+    code = _head_dtype(x2d)
+    M, K = x2d.shape
+    V = w.shape[0]
+    _check_2d("weight", w, (V, K), x2d.dtype)
+    if tuple(labels.shape) != (M,):
+        raise ShapeError(f"labels shape mismatch: expected {(M,)}, got {tuple(labels.shape)}")
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise ShapeError(f"labels must be int64 or int32, got {labels.dtype}")
+    r = 0
+    if a is not None:
+        a, b, alpha, r = _pad_rank(a, b, alpha)
+        _check_2d("A", a, (r, K), x2d.dtype)
+        _check_2d("B", b, (V, r), x2d.dtype)
+        a, b = a.contiguous(), b.contiguous()
+    x2d, w, labels = x2d.contiguous(), w.contiguous(), labels.to(torch.int64).contiguous()
+    loss = torch.empty((M,) if reduction == "none" else (), dtype=torch.float32, device=x2d.device)
+    if M == 0:  # no tokens: nothing to launch (a mean over none is NaN, as 0 / 0 is)
+        return loss.fill_(float("nan") if reduction == "mean" else 0.0), loss.new_empty(0)
+    lib = _lib.load()
+    state_bytes, ws_bytes = _head_bytes(M, K, V, r, code, grads)
+    if state_bytes == 0:
+        _lib.check(_lib.MLORA_ERR_UNSUPPORTED, "mlora_linear_cross_entropy")
+    state = torch.empty(state_bytes, dtype=torch.uint8, device=x2d.device)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x2d.device)
+    rows = reduction == "none"
+    st = lib.mlora_linear_cross_entropy(
+        _ptr(x2d), _ptr(w), _ptr(a), _ptr(b), _ptr(labels), None if rows else _ptr(loss),
+        _ptr(loss) if rows else None, _ptr(state), state_bytes, M, K, V, r, float(alpha),
+        int(ignore_index), int(reduction == "mean"), code, grads, _ptr(ws), ws_bytes, _stream())
+    _lib.check(st, "mlora_linear_cross_entropy")
+    return loss, state
+
+
+def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.Tensor, M: int,
+                             r: int, reduction: str, grads: int,
+                             da_out: torch.Tensor | None = None,
+                             db_out: torch.Tensor | None = None, accumulate: bool = True,
+                             ab_dtype: torch.dtype | None = None):
+    """(dx, dA, dB, dW), those that ``grads`` names, from the state that
+    ``linear_cross_entropy_fwd`` filled with the same ``grads``, and the loss's
+    upstream gradient (fp32; one per token after "none").  r is A's rank.  With
+    ``da_out``/``db_out`` (contiguous fp32, rank a multiple of 8) dA and dB are added
+    into them, or written over them without ``accumulate``."""
+    _need_cuda(grad, state, w)
+    _need_current(grad, state, w)
+    code = _head_dtype(w)
+    V, K = w.shape
+    r8 = (r + 7) // 8 * 8
+    dx = w.new_empty((M, K)) if grads & _lib.HEAD_GRAD_X else None
+    dw = torch.empty((V, K), dtype=w.dtype, device=w.device) if grads & _lib.HEAD_GRAD_W else None
+    da = db = None
+    into = da_out is not None or db_out is not None
+    if grads & _lib.HEAD_GRAD_AB:
+        if into:
+            _check_grad_out(da_out, db_out, r8, r, K, V)
+            da, db = da_out, db_out
+        else:
+            da = w.new_empty((r8, K), dtype=ab_dtype or w.dtype)
+            db = w.new_empty((V, r8), dtype=ab_dtype or w.dtype)
+    if M == 0:  # no tokens: zero gradients (or nothing added)
+        for t in (dw, *(() if into and accumulate else (da, db))):
+            if t is not None:
+                t.zero_()
+    else:
+        w = w.contiguous()
+        rows = reduction == "none"
+        grad = grad.to(torch.float32).contiguous()
+        if rows and tuple(grad.shape) != (M,):
+            raise ShapeError(f"expected {M} upstream gradients, got {tuple(grad.shape)}")
+        st = _lib.load().mlora_linear_cross_entropy_backward(
+            _ptr(state), state.numel(), _ptr(grad), int(rows), int(reduction == "mean"), _ptr(w),
+            _ptr(dx), _ptr(da), _ptr(db), code if da is None else _dtype_code(da),
+            int(into and accumulate), _ptr(dw), M, K, V, r8, code, grads, _stream())
+        _lib.check(st, "mlora_linear_cross_entropy_backward")
+    if da is not None and r8 != r:
+        da, db = da[:r].contiguous(), db[:, :r].contiguous()
+    return dx, da, db, dw

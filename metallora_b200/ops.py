@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 from torch.autograd import forward_ad
 
+from . import _lib
 from . import kernels as _k
 from .exceptions import ConfigurationError, ShapeError
 from .quant import ActivationCheckpoint, empty_checkpoint
@@ -327,3 +328,82 @@ def multi_adapter_forward(x, W0, adapters_A, adapters_B, adapter_ids, alpha: flo
         part = _k.multi_lora_fwd(x2d, base, a_stack, b_stack, tok, r8, float(alpha) * r8 / r)
         y = part if y is None else y + part
     return y.reshape(Bsz, S, N)
+
+
+class _LinearCrossEntropyFn(torch.autograd.Function):
+    """The gradients are made in the forward, where a piece's logits are at hand, up
+    to the upstream factor, which the backward multiplies in (see
+    ``linear_cross_entropy``).  ``compute`` and ``sink`` as in _LoRALinearFn."""
+
+    @staticmethod
+    def forward(ctx, x2d, w, a, b, labels, alpha, ignore_index, reduction, compute, sink):
+        need = ctx.needs_input_grad
+        grads = (_lib.HEAD_GRAD_X if need[0] else 0) | (_lib.HEAD_GRAD_W if need[1] else 0)
+        a_c = b_c = None
+        if a is not None:
+            a_c, b_c = compute if compute is not None else _cast_ab(a, b, x2d.dtype)
+            if need[2] or need[3]:
+                grads |= _lib.HEAD_GRAD_AB
+                ctx.rank, ctx.ab_dtypes = a.shape[0], (a.dtype, b.dtype)
+        loss, state = _k.linear_cross_entropy_fwd(x2d, w, labels, a_c, b_c, alpha, ignore_index,
+                                                  reduction, grads)
+        ctx.save_for_backward(state, w)
+        ctx.plan = (x2d.shape[0], 0 if a is None else a.shape[0], reduction, grads)
+        ctx.sink = sink
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        state, w = ctx.saved_tensors
+        m, r, reduction, grads = ctx.plan
+        sink = ctx.sink if grads & _lib.HEAD_GRAD_AB else None
+        same = grads & _lib.HEAD_GRAD_AB and ctx.ab_dtypes[0] == ctx.ab_dtypes[1]
+        dx, da, db, dw = _k.linear_cross_entropy_bwd(
+            grad, state, w, m, r, reduction, grads, da_out=sink[0] if sink else None,
+            db_out=sink[1] if sink else None, accumulate=_sink_accumulates(sink),
+            ab_dtype=ctx.ab_dtypes[0] if same else torch.float32)
+        if sink is not None:
+            if len(sink) > 3 and sink[3] is not None:
+                sink[3]()
+            da = db = None
+        elif da is not None and not same:
+            da, db = da.to(ctx.ab_dtypes[0]), db.to(ctx.ab_dtypes[1])
+        need = ctx.needs_input_grad
+        return (dx, dw, da if need[2] else None, db if need[3] else None, None, None, None, None,
+                None, None)
+
+
+def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,  # noqa: N803
+                         ignore_index: int = -100, reduction: str = "mean",
+                         _compute=None, _sink=None):
+    """Softmax cross entropy of a linear head over a large vocabulary, from the hidden
+    states: ``cross_entropy(x.weight^T [+ (alpha/r)(x.A^T).B^T], labels)`` without the
+    [tokens, vocabulary] logits, in memory that does not grow with them.
+
+    x [..., K] (bf16 or fp16), weight [V, K] of the same type, labels int [...];
+    A [r, K] and B [V, r] (both or neither) are a LoRA head's factors.  Tokens
+    labelled ``ignore_index`` have no loss and cost nothing; one whose label is
+    outside [0, V) is left out too and reported in the device status (0x107).
+    ``reduction`` is "mean" (over the counted tokens; NaN for none), "sum" or
+    "none" (a loss per token, 0 where there is none); the result is fp32.
+
+    Gradients reach x, A and B, and weight where it requires one.  They are made in
+    the forward, with the logits; the backward scales them.  "none" takes
+    gradients of x alone: those of weights need to know in the forward how the
+    tokens are weighted.  K must be a multiple of 8, and V with A and B."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ConfigurationError(f"unknown reduction {reduction!r}")
+    if (A is None) != (B is None):
+        raise ConfigurationError("a LoRA head needs both A and B")
+    if x.shape[-1] != weight.shape[1]:
+        raise ShapeError(f"x last dim {x.shape[-1]} != in_features {weight.shape[1]}")
+    if labels.shape != x.shape[:-1]:
+        raise ShapeError(f"labels {tuple(labels.shape)} do not match x {tuple(x.shape)}")
+    if reduction == "none" and torch.is_grad_enabled() and \
+            any(t is not None and t.requires_grad for t in (weight, A, B)):
+        raise ConfigurationError("reduction='none' takes gradients of x alone; detach the head's "
+                                 "weights or use 'mean' or 'sum'")
+    loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, A, B, labels.reshape(-1),
+                                       float(alpha), int(ignore_index), reduction, _compute, _sink)
+    return loss.reshape(labels.shape) if reduction == "none" else loss
