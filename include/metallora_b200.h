@@ -536,6 +536,45 @@ MLORA_API int mlora_linear_cross_entropy_backward(const void* state, size_t stat
                                                   int64_t M, int64_t K, int64_t V, int64_t r,
                                                   int dtype, int grads, void* stream);
 
+/* ---- token embedding ---------------------------------------------------- */
+
+/* out[t] = scale * table[idx[t]] for T int64 indices into table [V, D] (BF16, F16 or
+ * F32, out alike); an index outside it gives a zero row and device status 0x107. */
+MLORA_API int mlora_embedding_forward(const int64_t* idx, const void* table, void* out, int64_t T,
+                                      int64_t V, int64_t D, float scale, int dtype, void* stream);
+
+/* grad[v] = scale * (sum of dy[t] over the tokens with idx[t] = v), all V rows written;
+ * summed in fp32 in token order, the same bits in every run.  Tokens of padding_idx
+ * (negative: none) and those outside the table add nothing. */
+MLORA_API size_t mlora_embedding_backward_workspace_bytes(int64_t T, int64_t D);
+MLORA_API int mlora_embedding_backward(const int64_t* idx, const void* dy, void* grad, int64_t T,
+                                       int64_t V, int64_t D, float scale, int64_t padding_idx,
+                                       int dtype, void* workspace, size_t workspace_bytes,
+                                       void* stream);
+
+/* ---- counter-based dropout ---------------------------------------------- */
+
+/* out = kept ? x * 65536 / (65536 - threshold) : 0 over n elements in a row (out may be
+ * x).  Element e is kept where half-word e % 8 (low half first) of Philox4x32-10's
+ * four words for the key `seed` and the counter (e / 8, call) is at least `threshold`
+ * (0..65536).  No mask is stored: the gradient is the same call on dy.  seed_dev, where
+ * not NULL, is a device int64 that takes the seed's place, read when the kernel runs. */
+MLORA_API int mlora_dropout(const void* x, void* out, int64_t n, int threshold, uint64_t seed,
+                            const int64_t* seed_dev, uint64_t call, int dtype, void* stream);
+
+/* y = x.W0^T + dropout((alpha/r)(x.A^T).B^T), the dropout as above over [M, N]; BF16 or
+ * F16, N a multiple of 8.  saved_xa as for mlora_lora_forward.  Its gradient: with
+ * dz = dropout(dy), mlora_lora_backward_ex of dz with MLORA_BWD_DEFER_DX, then of dy
+ * with MLORA_BWD_DX_ONLY. */
+MLORA_API size_t mlora_lora_forward_dropout_workspace_bytes(int64_t M, int64_t K, int64_t N,
+                                                            int64_t r, int dtype);
+MLORA_API int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a,
+                                         const void* b, void* y, void* saved_xa, int64_t M,
+                                         int64_t K, int64_t N, int64_t r, float alpha,
+                                         int threshold, uint64_t seed, const int64_t* seed_dev,
+                                         uint64_t call, int dtype, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

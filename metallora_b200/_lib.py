@@ -47,6 +47,7 @@ i64 = C.c_int64
 f32 = C.c_float
 i32 = C.c_int
 sz = C.c_size_t
+u64 = C.c_uint64
 
 # name -> (restype, argtypes); kept in the order of include/metallora_b200.h
 SIGNATURES: dict[str, tuple] = {
@@ -122,6 +123,13 @@ SIGNATURES: dict[str, tuple] = {
                                                                        sz, vp]),
     "mlora_linear_cross_entropy_backward": (i32, [vp, sz, vp, i32, i32, vp, vp, vp, vp, i32, i32,
                                                   vp, i64, i64, i64, i64, i32, i32, vp]),
+    "mlora_embedding_forward": (i32, [vp, vp, vp, i64, i64, i64, f32, i32, vp]),
+    "mlora_embedding_backward_workspace_bytes": (sz, [i64, i64]),
+    "mlora_embedding_backward": (i32, [vp, vp, vp, i64, i64, i64, f32, i64, i32, vp, sz, vp]),
+    "mlora_dropout": (i32, [vp, vp, i64, i32, u64, vp, u64, i32, vp]),
+    "mlora_lora_forward_dropout_workspace_bytes": (sz, [i64, i64, i64, i64, i32]),
+    "mlora_lora_forward_dropout": (i32, [vp] * 6 + [i64] * 4 + [f32, i32, u64, vp, u64, i32, vp, sz,
+                                                                vp]),
 }
 
 

@@ -11,6 +11,7 @@
 #include <vector>
 
 #include "internal.h"
+#include "philox.cuh"
 #include "../../include/metallora_b200.h"
 
 // Per-device status word written by kernels whose bounded waits ran out.
@@ -1003,6 +1004,81 @@ int mlora_lora_forward_ckpt(const void* x, const void* w0, const void* a, const 
   const Ckpt c{ckpt_codes, ckpt_ld, ckpt_scales};
   return lora_forward_any(x, w0, a, b, y, saved_xa, &c, M, K, N, r, alpha, dtype, workspace,
                           workspace_bytes, stream);
+}
+
+size_t mlora_lora_forward_dropout_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r,
+                                                  int dtype) {
+  if (check_shapes(M, K, N, r, dtype) || dtype == MLORA_DTYPE_F32) return 0;
+  return align_up(plan_forward(nullptr, M, K, r, true).bytes, 256) + static_cast<size_t>(M) * N * 2;
+}
+
+int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, const void* b, void* y,
+                               void* saved_xa, int64_t M, int64_t K, int64_t N, int64_t r,
+                               float alpha, int threshold, uint64_t seed, const int64_t* seed_dev,
+                               uint64_t call, int dtype, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  int rc = check_shapes(M, K, N, r, dtype);
+  if (rc) return rc;
+  if (dtype == MLORA_DTYPE_F32)
+    return fail(MLORA_ERR_UNSUPPORTED, "LoRA dropout takes BF16 or F16");
+  if (threshold < 0 || threshold > 65536)
+    return fail(MLORA_ERR_INVALID_ARG, "threshold must be in [0, 65536]");
+  if (!x || !w0 || !a || !b || !y || !saved_xa)
+    return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
+  if ((rc = check_ptrs16({x, w0, a, b, y, saved_xa}))) return rc;
+  if (reinterpret_cast<uintptr_t>(seed_dev) % 8)
+    return fail(MLORA_ERR_INVALID_ARG, "the seed must be a whole int64");
+  const size_t need = mlora_lora_forward_dropout_workspace_bytes(M, K, N, r, dtype);
+  if (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))
+    return fail(MLORA_ERR_WORKSPACE, "forward workspace needs " + std::to_string(need) + " bytes");
+  if ((rc = check_device())) return rc;
+  const FwdPlan p = plan_forward(workspace, M, K, r, true);
+  void* z = static_cast<uint8_t*>(workspace) + align_up(p.bytes, 256);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Elt elt = dtype == MLORA_DTYPE_BF16 ? Elt::kBF16 : Elt::kF16;
+  RankArgs ra;
+  ra.x = x;
+  ra.l = a;
+  ra.M = M;
+  ra.K = K;
+  ra.r = r;
+  ra.R = p.R;
+  ra.ldx = K;
+  ra.ldl = K;
+  ra.scale = alpha / static_cast<float>(r);
+  ra.out_rows = p.xa_rows;
+  ra.ld_rows = p.R64;
+  ra.out_t = saved_xa;
+  ra.ld_t = pad8(M);
+  ra.splits = p.splits;
+  ra.elt = elt;
+  if ((rc = launch_rank(ra, s))) return rc;
+  GemmArgs gz;  // z = (s x A^T) . B^T
+  gz.x = p.xa_rows;
+  gz.w = b;
+  gz.d = z;
+  gz.M = M;
+  gz.N = N;
+  gz.K = r;
+  gz.ldx = p.R64;
+  gz.ldw = r;
+  gz.ldd = N;
+  gz.w_mn_major = false;
+  gz.elt = elt;
+  gz.out_dtype = dtype;
+  if ((rc = launch_gemm(gz, s))) return rc;
+  const DropoutKey key{seed, seed_dev, call, static_cast<uint32_t>(threshold)};
+  if ((rc = launch_dropout(z, z, M * N, dtype, key, s))) return rc;
+  GemmArgs ga = gz;  // y = x . W0^T + drop(z)
+  ga.x = x;
+  ga.w = w0;
+  ga.d = y;
+  ga.K = K;
+  ga.ldx = K;
+  ga.ldw = K;
+  ga.c = z;
+  ga.ldc = N;
+  return launch_gemm(ga, s);
 }
 
 size_t mlora_lora_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int dtype) {

@@ -282,6 +282,12 @@ int launch_embed_da_f32(const int32_t* idx, const float* b, const float* dy, flo
                         int64_t n_tok, int64_t D, int64_t r, float scale, bool accumulate,
                         cudaStream_t s);
 
+// ------------------------------------------------------------ dropout --------
+struct DropoutKey;  // philox.cuh
+// out = dropout(x) over n elements in a row (out may be x).
+int launch_dropout(const void* x, void* out, int64_t n, int dtype, const DropoutKey& key,
+                   cudaStream_t s);
+
 // ---------------------------------------------------------- elementwise ------
 int launch_transpose_pad(const void* b, int64_t N, int64_t r, int64_t ldb, void* bt, int64_t R,
                          Elt elt, cudaStream_t stream);

@@ -18,7 +18,7 @@ import functools
 import torch
 
 from . import _lib
-from .exceptions import DeviceError, ShapeError
+from .exceptions import ConfigurationError, DeviceError, ShapeError
 
 _DT = {torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16, torch.float32: _lib.DTYPE_F32}
 
@@ -828,3 +828,176 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.T
     if da is not None and r8 != r:
         da, db = da[:r].contiguous(), db[:, :r].contiguous()
     return dx, da, db, dw
+
+
+# ------------------------------------------------------- token embedding --
+
+def _table_index(indices: torch.Tensor) -> torch.Tensor:
+    if indices.dtype not in (torch.int64, torch.int32):
+        raise ShapeError(f"indices must be int64 or int32, got {indices.dtype}")
+    return indices.reshape(-1).to(torch.int64).contiguous()
+
+
+def embedding_fwd(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[idx] for every index, [*indices.shape, D] (bf16, fp16 or fp32); an
+    index outside the table gives a zero row and device status 0x107."""
+    _need_cuda(indices, table)
+    _need_current(indices, table)
+    code = _dtype_code(table)
+    if table.dim() != 2:
+        raise ShapeError(f"the table must be [V, D], got {tuple(table.shape)}")
+    V, D = table.shape
+    idx = _table_index(indices)
+    table = table.contiguous()
+    out = torch.empty((*indices.shape, D), dtype=table.dtype, device=table.device)
+    if out.numel() == 0:
+        return out
+    st = _lib.load().mlora_embedding_forward(_ptr(idx), _ptr(table), _ptr(out), idx.numel(), V, D,
+                                             float(scale), code, _stream())
+    _lib.check(st, "mlora_embedding_forward")
+    return out
+
+
+def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, scale: float = 1.0,
+                  padding_idx: int | None = None) -> torch.Tensor:
+    """The table's gradient [num_embeddings, D] in dy's dtype: scale times the sum of
+    dy over each entry's tokens, in fp32 and in token order (the same bits in every
+    run); zero for ``padding_idx``."""
+    _need_cuda(dy, indices)
+    _need_current(dy, indices)
+    code = _dtype_code(dy)
+    idx = _table_index(indices)
+    T, D, V = idx.numel(), dy.shape[-1], int(num_embeddings)
+    dy = dy.reshape(T, D).contiguous()
+    grad = torch.empty((V, D), dtype=dy.dtype, device=dy.device)
+    if grad.numel() == 0 or T == 0:
+        return grad.zero_()
+    lib = _lib.load()
+    ws = _workspace(lib.mlora_embedding_backward_workspace_bytes(T, D), dy.device)
+    st = lib.mlora_embedding_backward(_ptr(idx), _ptr(dy), _ptr(grad), T, V, D, float(scale),
+                                      -1 if padding_idx is None else int(padding_idx), code,
+                                      _ptr(ws), ws.numel(), _stream())
+    _lib.check(st, "mlora_embedding_backward")
+    return grad
+
+
+# ---------------------------------------------------------------- dropout --
+
+def _drop_threshold(p: float) -> int:
+    """Of 65536: p to the nearest multiple of 2^-16."""
+    if not 0.0 <= p <= 1.0:
+        raise ConfigurationError(f"dropout must be in [0, 1], got {p}")
+    return round(65536 * p)
+
+
+def _drop_seed(seed) -> tuple[int, int | None]:
+    """(seed, device address or None) of an int, or of a CUDA int64 tensor of one element."""
+    if torch.is_tensor(seed):
+        _need_cuda(seed)
+        _need_current(seed)
+        if seed.dtype != torch.int64 or seed.numel() != 1:
+            raise ShapeError("a seed tensor holds one int64")
+        return 0, seed.data_ptr()
+    return int(seed) & (2 ** 64 - 1), None
+
+
+def dropout(x: torch.Tensor, p: float, seed, call: int = 0) -> torch.Tensor:
+    """x with every element dropped (0) or scaled by the counter-based mask of ``seed``
+    and ``call`` (see ``ops.dropout``); its gradient is the same call on dy."""
+    t = _drop_threshold(p)
+    _need_cuda(x)
+    _need_current(x)
+    code = _dtype_code(x)
+    s, s_dev = _drop_seed(seed)
+    x = x.contiguous()
+    out = torch.empty_like(x)
+    if x.numel():
+        st = _lib.load().mlora_dropout(_ptr(x), _ptr(out), x.numel(), t, s, s_dev,
+                                       int(call) & (2 ** 64 - 1), code, _stream())
+        _lib.check(st, "mlora_dropout")
+    return out
+
+
+def lora_linear_dropout_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor, b: torch.Tensor,
+                            alpha: float, p: float, seed, call: int = 0):
+    """(y, saved_xa) of y = x.W0^T + dropout((alpha/r).(x.A^T).B^T) for 2-D x [M, K], bf16
+    or fp16; the mask as in ``dropout``, over [M, N]."""
+    t = _drop_threshold(p)
+    _need_cuda(x2d, w0, a, b)
+    _need_current(x2d, w0, a, b)
+    dt = x2d.dtype
+    if dt not in (torch.bfloat16, torch.float16):
+        raise ShapeError("counter-based LoRA dropout takes bf16 or fp16 activations")
+    M, K = x2d.shape
+    N = w0.shape[0]
+    a, b, alpha, r = _pad_rank(a, b, alpha)
+    _check_2d("W0", w0, (N, K), dt)
+    _check_2d("A", a, (r, K), dt)
+    _check_2d("B", b, (N, r), dt)
+    s, s_dev = _drop_seed(seed)
+    x2d, w0, a, b = (v.contiguous() for v in (x2d, w0, a, b))
+    y = x2d.new_empty((M, N))
+    saved = x2d.new_empty((rank_tile(r), (M + 7) // 8 * 8))
+    if M == 0:
+        return y, saved
+    lib = _lib.load()
+    ws = _workspace(lib.mlora_lora_forward_dropout_workspace_bytes(M, K, N, r, _DT[dt]), x2d.device)
+    st = lib.mlora_lora_forward_dropout(_ptr(x2d), _ptr(w0), _ptr(a), _ptr(b), _ptr(y), _ptr(saved),
+                                        M, K, N, r, float(alpha), t, s, s_dev,
+                                        int(call) & (2 ** 64 - 1), _DT[dt], _ptr(ws), ws.numel(),
+                                        _stream())
+    _lib.check(st, "mlora_lora_forward_dropout")
+    return y, saved
+
+
+def lora_linear_dropout_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor,
+                            b: torch.Tensor, alpha: float, saved_xa: torch.Tensor, p: float, seed,
+                            call: int = 0, need_dx: bool = True,
+                            da_out: torch.Tensor | None = None, db_out: torch.Tensor | None = None,
+                            accumulate: bool = True, grad_dtype: torch.dtype | None = None,
+                            on_grads=None):
+    """(dx, dA, dB) of ``lora_linear_dropout_fwd``: the LoRA products take dropout(dy), the
+    base's takes dy.  The other arguments as for ``lora_linear_bwd``; ``on_grads`` is
+    called between dA/dB and the dx GEMM."""
+    dz = dropout(dy2d, p, seed, call)
+    dy2d = dy2d.contiguous()
+    M, K = x2d.shape
+    if not need_dx or M == 0:
+        dx, da, db = lora_linear_bwd(dz, x2d, w0 if need_dx else None, a, b, alpha, saved_xa, 0.0,
+                                     need_dx=need_dx, da_out=da_out, db_out=db_out,
+                                     accumulate=accumulate, grad_dtype=grad_dtype)
+        if on_grads is not None:
+            on_grads()
+        return dx, da, db
+    dt = x2d.dtype
+    N, r_orig = dy2d.shape[1], a.shape[0]
+    a_p, b_p, alpha_p, r = _pad_rank(a, b, alpha)
+    _check_2d("grad_output", dy2d, (M, N), dt)
+    _check_saved(saved_xa, r, M, dt)
+    x2d, w0, a_p, b_p = (v.contiguous() for v in (x2d, w0, a_p, b_p))
+    into = da_out is not None or db_out is not None
+    flags = 0
+    if into:
+        _check_grad_out(da_out, db_out, r, r_orig, K, N)
+        da, db = da_out, db_out
+        flags = _lib.BWD_ACCUMULATE if accumulate else 0
+    elif grad_dtype == dt:
+        flags = _lib.BWD_GRADS_16BIT
+        da, db = dy2d.new_empty((r, K)), dy2d.new_empty((N, r))
+    else:
+        da = dy2d.new_empty((r, K), dtype=torch.float32)
+        db = dy2d.new_empty((N, r), dtype=torch.float32)
+    dx = dy2d.new_empty((M, K))
+    lib = _lib.load()
+    ws = dy2d.new_empty(_bwd_ws_bytes(M, K, N, r, _DT[dt]), dtype=torch.uint8)
+    for phase, g in ((_lib.BWD_DEFER_DX, dz), (_lib.BWD_DX_ONLY, dy2d)):
+        st = lib.mlora_lora_backward_ex(_ptr(g), _ptr(x2d), _ptr(w0), _ptr(a_p), _ptr(b_p),
+                                        _ptr(saved_xa), _ptr(dx), _ptr(da), _ptr(db), M, K, N, r,
+                                        float(alpha_p), 0.0, _DT[dt], flags | phase, _ptr(ws),
+                                        ws.numel(), _stream())
+        _lib.check(st, "mlora_lora_backward_ex")
+        if phase == _lib.BWD_DEFER_DX and on_grads is not None:
+            on_grads()
+    if not into and r != r_orig:
+        da, db = da[:r_orig].contiguous(), db[:, :r_orig].contiguous()
+    return dx, da, db

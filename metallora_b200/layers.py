@@ -16,7 +16,7 @@ from torch import nn
 from . import kernels as _k
 from .exceptions import ConfigurationError, validate_alpha, validate_probability, validate_rank
 from .logging import logger
-from .ops import lora_forward, merge_lora_weights, qlora_forward
+from .ops import embedding, lora_forward, merge_lora_weights, qlora_forward
 
 
 class LoRALinear(nn.Module):
@@ -28,11 +28,15 @@ class LoRALinear(nn.Module):
     ``activation_checkpoint="mxint8"`` keeps the input for the backward in 8
     bits (see ``ops.lora_forward``); ``forward(x, checkpoint=c)`` uses one made
     by ``quant.checkpoint_activation`` that several layers share.
+    ``dropout_seed`` (an int, or a CUDA int64 tensor of one element) takes the dropout's
+    masks from the counter-based generator (see ``ops.dropout``); each training
+    forward uses the next ``dropout_call``, which starts at 0 and may be set.
     """
 
     def __init__(self, in_features: int, out_features: int, rank: int = 8, alpha: float = 16.0,
                  dropout: float = 0.0, use_bias: bool = False, freeze_base: bool = True,
-                 device=None, dtype=None, activation_checkpoint: str | None = None):
+                 device=None, dtype=None, activation_checkpoint: str | None = None,
+                 dropout_seed=None):
         super().__init__()
         if in_features <= 0:
             raise ConfigurationError(f"in_features must be positive, got {in_features}")
@@ -52,6 +56,8 @@ class LoRALinear(nn.Module):
         self.freeze_base = freeze_base
         self.merged = False
         self.activation_checkpoint = activation_checkpoint
+        self.dropout_seed = dropout_seed
+        self.dropout_call = 0
 
         fk = {"device": device, "dtype": dtype}
         self.W0 = nn.Parameter(torch.zeros((out_features, in_features), **fk),
@@ -80,6 +86,12 @@ class LoRALinear(nn.Module):
         """layers.py:83-106: any leading shape; the bias is added after the op."""
         if checkpoint is None and torch.is_grad_enabled():
             checkpoint = self.activation_checkpoint
+        drop = {}
+        if self.dropout_seed is not None and self.training and self.dropout > 0 and not self.merged:
+            if self.qweight is not None:
+                raise ConfigurationError("counter-based LoRA dropout needs a dense base")
+            drop = {"dropout_seed": self.dropout_seed, "dropout_call": self.dropout_call}
+            self.dropout_call += 1
         if self.qweight is not None:
             out = qlora_forward(x, self.qweight, self.A, self.B, alpha=self.alpha,
                                 _compute=self._compute_ab, _sink=self._grad_sink,
@@ -90,7 +102,7 @@ class LoRALinear(nn.Module):
         else:
             out = lora_forward(x, self.W0, self.A, self.B, alpha=self.alpha, dropout=self.dropout,
                                training=self.training, _compute=self._compute_ab,
-                               _sink=self._grad_sink, checkpoint=checkpoint)
+                               _sink=self._grad_sink, checkpoint=checkpoint, **drop)
         if self.bias is not None:
             out = out + self.bias
         return out
@@ -194,8 +206,13 @@ class _LoRAEmbeddingFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         indices, a, b = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        de = _k.embedding_bwd(dy, indices, b.shape[0]) if need[1] else None
+        if not (need[2] or need[3]):
+            return None, de, None, None, None
         da, db = _k.lora_embedding_bwd(dy, indices, a, b, ctx.alpha)
-        return None, None, da.to(a.dtype), db.to(b.dtype), None
+        return (None, de, da.to(a.dtype) if need[2] else None, db.to(b.dtype) if need[3] else None,
+                None)
 
 
 class LoRAEmbedding(nn.Module):
@@ -204,7 +221,8 @@ class LoRAEmbedding(nn.Module):
     (frozen when ``freeze_base``), A [rank, dim] ~ U(+-1/sqrt(dim)), B
     [num_embeddings, rank] = 0, E ~ N(0, 0.02^2) -- the reference's
     initialisation (:207-213).  The forward gathers on the tensor cores
-    (16-bit) or CUDA cores (fp32); gradients flow to A and B only."""
+    (16-bit) or CUDA cores (fp32); gradients flow to A and B, and to E unless the
+    base is frozen (summed by sorted tokens, see ``ops.embedding``)."""
 
     def __init__(self, num_embeddings: int, embedding_dim: int, rank: int = 8,
                  alpha: float = 16.0, freeze_base: bool = True, device=None, dtype=None):
@@ -229,11 +247,37 @@ class LoRAEmbedding(nn.Module):
         return self.alpha / self.rank
 
     def forward(self, indices: torch.Tensor) -> torch.Tensor:
-        if self.embeddings.requires_grad:
-            raise ConfigurationError("LoRAEmbedding trains A and B only (freeze_base=True)")
         return _LoRAEmbeddingFn.apply(indices, self.embeddings, self.A, self.B, float(self.alpha))
 
     @torch.no_grad()
     def merge_weights(self) -> torch.Tensor:
         """layers.py:227-230: E + (alpha/rank) B.A."""
         return _k.merge(self.embeddings, self.A, self.B, float(self.alpha))
+
+
+class TokenEmbedding(nn.Module):
+    """A trained token table: ``out = scale * weight[idx]`` (``ops.embedding``), weight
+    [num_embeddings, embedding_dim] ~ N(0, 0.02^2) as LoRAEmbedding's table.  The
+    gradient of ``padding_idx`` is zero.  A head that shares the table passes
+    ``weight`` to ``ops.linear_cross_entropy``; the two gradients add up."""
+
+    def __init__(self, num_embeddings: int, embedding_dim: int, scale: float = 1.0,
+                 padding_idx: int | None = None, device=None, dtype=None):
+        super().__init__()
+        if num_embeddings <= 0 or embedding_dim <= 0:
+            raise ConfigurationError("num_embeddings and embedding_dim must be positive")
+        if padding_idx is not None and not -num_embeddings <= padding_idx < num_embeddings:
+            raise ConfigurationError(f"padding_idx {padding_idx} is outside the table")
+        self.num_embeddings = num_embeddings
+        self.embedding_dim = embedding_dim
+        self.scale = float(scale)
+        self.padding_idx = None if padding_idx is None else padding_idx % num_embeddings
+        self.weight = nn.Parameter(torch.randn((num_embeddings, embedding_dim), device=device,
+                                               dtype=dtype) * 0.02)
+
+    def forward(self, indices: torch.Tensor) -> torch.Tensor:
+        return embedding(indices, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self) -> str:
+        return (f"{self.num_embeddings}, {self.embedding_dim}, scale={self.scale}, "
+                f"padding_idx={self.padding_idx}")

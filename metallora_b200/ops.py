@@ -127,6 +127,47 @@ class _LoRALinearFn(torch.autograd.Function):
         return dx, dw0, da, db, None, None, None, None
 
 
+def _keep_seed(ctx, seed):
+    """The seed as ``save_for_backward`` takes it: a tensor, whose being written over
+    before the backward is then noticed, or None with the number kept aside."""
+    ctx.seed = None if torch.is_tensor(seed) else seed
+    return seed if torch.is_tensor(seed) else None
+
+
+class _LoRADropoutFn(torch.autograd.Function):
+    """The LoRA linear with counter-based dropout on its LoRA term; W0 is frozen.
+    ``compute`` and ``sink`` as in _LoRALinearFn."""
+
+    @staticmethod
+    def forward(ctx, x2d, w0, a, b, alpha, p, seed, call, compute, sink):
+        a_c, b_c = compute if compute is not None else _cast_ab(a, b, x2d.dtype)
+        y, saved = _k.lora_linear_dropout_fwd(x2d, w0, a_c, b_c, alpha, p, seed, call)
+        ctx.save_for_backward(x2d, w0, a_c, b_c, saved, _keep_seed(ctx, seed))
+        ctx.plan = (alpha, p, call)
+        ctx.sink = sink
+        ctx.ab_dtypes = (a.dtype, b.dtype)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x2d, w0, a_c, b_c, saved, seed = ctx.saved_tensors
+        alpha, p, call = ctx.plan
+        sink = ctx.sink
+        same = ctx.ab_dtypes[0] == ctx.ab_dtypes[1] == x2d.dtype
+        need = ctx.needs_input_grad
+        dx, da, db = _k.lora_linear_dropout_bwd(
+            dy, x2d, w0, a_c, b_c, alpha, saved, p, ctx.seed if seed is None else seed, call,
+            need_dx=need[0], da_out=sink[0] if sink else None, db_out=sink[1] if sink else None,
+            accumulate=_sink_accumulates(sink), grad_dtype=x2d.dtype if same else None,
+            on_grads=sink[3] if sink is not None and len(sink) > 3 else None)
+        if sink is not None:
+            return dx, *(None,) * 9
+        da = da.to(ctx.ab_dtypes[0]) if need[2] else None
+        db = db.to(ctx.ab_dtypes[1]) if need[3] else None
+        return dx, None, da, db, *(None,) * 6
+
+
 class _QLoRALinearFn(torch.autograd.Function):
     """The LoRA linear over a frozen quantised base (QLoRA): no gradient for
     the base; A/B handled as in _LoRALinearFn."""
@@ -197,7 +238,8 @@ def _apply(x2d, W0, A, B, alpha, compute=None, sink=None, checkpoint=None):
 
 def lora_forward(x, W0, A, B, alpha: float = 16.0, dropout: float = 0.0,  # noqa: N803
                  training: bool = False, use_metal: bool = True, kernel_kwargs: dict | None = None,
-                 _compute=None, _sink=None, checkpoint=None):
+                 _compute=None, _sink=None, checkpoint=None, dropout_seed=None,
+                 dropout_call: int = 0):
     """LoRA forward ``h = x.W0^T + (alpha/rank).(x.A^T).B^T`` (ops.py:32-103).
 
     x is [batch, seq, in] or [seq, in] (any leading shape works); rank is read
@@ -210,6 +252,12 @@ def lora_forward(x, W0, A, B, alpha: float = 16.0, dropout: float = 0.0,  # noqa
     checkpoint's values; y does not change, and dx and dB at most in the order
     of their fp32 sums.  It needs a frozen W0 and no dropout, which read x
     itself.
+
+    ``dropout_seed`` (an int, or a CUDA int64 tensor of one element) takes the mask
+    from the counter-based generator of ``dropout`` instead of torch's: it is
+    made again in the backward and never stored, and the call runs on the fused
+    kernels.  ``dropout_call`` numbers the uses of one seed.  It needs a frozen W0,
+    bf16 or fp16, and out_features in multiples of 8.
     """
     if x.shape[-1] != W0.shape[1]:
         raise ShapeError(f"x last dim {x.shape[-1]} != in_features {W0.shape[1]}")
@@ -217,7 +265,12 @@ def lora_forward(x, W0, A, B, alpha: float = 16.0, dropout: float = 0.0,  # noqa
     x2d = x.reshape(-1, shp[-1])
     if checkpoint is not None and (W0.requires_grad or (training and dropout > 0)):
         raise ConfigurationError("an activation checkpoint needs a frozen W0 and no dropout")
-    if training and dropout > 0:
+    if training and dropout > 0 and dropout_seed is not None:
+        if W0.requires_grad:
+            raise ConfigurationError("counter-based LoRA dropout needs a frozen W0")
+        out = _LoRADropoutFn.apply(x2d, W0, A, B, float(alpha), float(dropout), dropout_seed,
+                                   int(dropout_call), _compute, _sink)
+    elif training and dropout > 0:
         # ops.py:96-98: output = w0x + scale * bax * mask / (1 - dropout)
         zero_b = torch.zeros_like(B)
         w0x = _apply(x2d, W0, A, zero_b, alpha)
@@ -407,3 +460,69 @@ def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,
     loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, A, B, labels.reshape(-1),
                                        float(alpha), int(ignore_index), reduction, _compute, _sink)
     return loss.reshape(labels.shape) if reduction == "none" else loss
+
+
+class _DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, p, seed, call):
+        ctx.save_for_backward(_keep_seed(ctx, seed))
+        ctx.plan = (p, call)
+        return _k.dropout(x, p, seed, call)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        seed, = ctx.saved_tensors
+        p, call = ctx.plan
+        return _k.dropout(dy, p, ctx.seed if seed is None else seed, call), None, None, None
+
+
+def dropout(x, p: float, seed, call: int = 0, training: bool = True):
+    """Dropout whose mask is never stored: ``kept ? x * 65536 / (65536 - t) : 0`` with
+    t = round(65536 p), a dropped element being 0 whatever it was.
+
+    The mask is a function of ``seed`` (an int, or a CUDA int64 tensor of one element,
+    which a replayed graph reads anew), ``call``, which numbers the uses of one seed,
+    and the element's place in x (row-major): half-word e % 8, the low half first, of
+    the four words that Philox4x32-10 (Salmon et al., 2011) makes of the key ``seed``
+    and the 128-bit counter (e // 8, call); kept where it is at least t.  The backward
+    makes it again.  Any shape; bf16, fp16 or fp32.  Without ``training`` x is returned
+    as it is."""
+    if not 0.0 <= p <= 1.0:
+        raise ConfigurationError(f"dropout must be in [0, 1], got {p}")
+    if not training:
+        return x
+    return _DropoutFn.apply(x, float(p), seed, int(call))
+
+
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, indices, table, scale, padding_idx):
+        ctx.save_for_backward(indices)
+        ctx.plan = (table.shape[0], scale, padding_idx)
+        return _k.embedding_fwd(indices, table, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        indices, = ctx.saved_tensors
+        rows, scale, padding_idx = ctx.plan
+        return None, _k.embedding_bwd(dy, indices, rows, scale, padding_idx), None, None
+
+
+def embedding(indices, table, scale: float = 1.0, padding_idx: int | None = None):
+    """``scale * table[indices]`` [*indices.shape, D] for int indices into table [V, D]
+    (bf16, fp16 or fp32), and the gradient of a trained table: scale times the sum of
+    dy over each entry's tokens, in fp32, in token order, the same bits in every run.
+
+    ``padding_idx`` (negative: from the end) has no gradient.  An index outside the
+    table gives a zero row and no gradient, and is reported in the device status
+    (0x107)."""
+    if table.dim() != 2:
+        raise ShapeError(f"the table must be [V, D], got {tuple(table.shape)}")
+    if padding_idx is not None:
+        rows = table.shape[0]
+        if not -rows <= padding_idx < rows:
+            raise ConfigurationError(f"padding_idx {padding_idx} is outside the table's {rows} rows")
+        padding_idx = int(padding_idx) % rows
+    return _EmbeddingFn.apply(indices, table, float(scale), padding_idx)

@@ -42,6 +42,7 @@ from .distributed import BucketedGradExchange, PeerLiveness, average_gradients
 from .exceptions import ConfigurationError
 from .layers import LoRALinear
 from .logging import logger
+from .ops import linear_cross_entropy
 from .utils import apply_lora_to_model, is_lora_target
 
 
@@ -78,6 +79,15 @@ class TrainingConfig:
 
     # "mxint8": every LoRALinear keeps its input for the backward in 8 bits
     activation_checkpoint: str | None = None
+
+    # LoRA dropout masks from the counter-based generator: made again in the backward,
+    # never stored (layer i of rank q uses the seed dropout_seed + i + q 2^32)
+    dropout_seed: int | None = None
+
+    # name of the module whose output the model returns as logits (an nn.Linear without
+    # bias, or a LoRALinear with a dense base): batches with labels take their loss
+    # from that module's input and weights, without the logits (ops.linear_cross_entropy)
+    loss_head: str | None = None
 
 
 @dataclass
@@ -296,6 +306,46 @@ def _check_activation_checkpoint(model: nn.Module, c: TrainingConfig) -> None:
                                      f"got {dtype}")
 
 
+def _check_loss_head(model: nn.Module, c: TrainingConfig) -> None:
+    """Refuses, before the model is changed, a head that the loss cannot be taken from."""
+    if c.loss_head is None:
+        return
+    head = dict(model.named_modules()).get(c.loss_head)
+    if isinstance(head, LoRALinear):
+        dense = head.qweight is None
+        weight, dropout = head.W0, head.dropout if head.training and not head.merged else 0.0
+    elif isinstance(head, nn.Linear):
+        dense, weight = True, head.weight
+        made = not any(isinstance(m, LoRALinear) for m in model.modules())
+        adapted = made and is_lora_target(c.loss_head, c.target_modules)
+        dropout = c.dropout if adapted else 0.0
+    else:
+        raise ConfigurationError(f"loss_head {c.loss_head!r} is no nn.Linear or LoRALinear of the "
+                                 "model")
+    if not dense or head.bias is not None or dropout > 0:
+        raise ConfigurationError(f"loss_head {c.loss_head!r} needs a dense weight, no bias and no "
+                                 "dropout")
+    if weight.dtype not in (torch.bfloat16, torch.float16) or weight.shape[1] % 8:
+        raise ConfigurationError(f"loss_head {c.loss_head!r} needs a bf16 or fp16 weight with "
+                                 "in_features in multiples of 8")
+
+
+def _check_dropout_seed(model: nn.Module, c: TrainingConfig) -> None:
+    """Refuses, before the model is changed, layers whose dropout has no counter-based form."""
+    if c.dropout_seed is None:
+        return
+    layers = [(n, m) for n, m in model.named_modules() if isinstance(m, LoRALinear)]
+    bases = [(n, m.W0 if m.qweight is None else None) for n, m in layers
+             if m.dropout > 0 and not m.merged]
+    if not layers and c.dropout > 0:  # the ones that the trainer will make
+        bases = [(n, m.weight) for n, m in model.named_modules()
+                 if isinstance(m, nn.Linear) and is_lora_target(n, c.target_modules)]
+    for name, w in bases:
+        if w is None or w.dtype not in (torch.bfloat16, torch.float16) or w.shape[0] % 8:
+            raise ConfigurationError(f"{name}: counter-based LoRA dropout needs a dense bf16 or "
+                                     "fp16 base with out_features in multiples of 8")
+
+
 class LoRATrainer:
     """LoRA trainer (reference: trainer.py:173-302)."""
 
@@ -305,6 +355,8 @@ class LoRATrainer:
         self.config = config or TrainingConfig()
         c = self.config
         _check_activation_checkpoint(model, c)
+        _check_loss_head(model, c)
+        _check_dropout_seed(model, c)
         if not any(isinstance(m, LoRALinear) for m in model.modules()):
             apply_lora_to_model(model, rank=c.rank, alpha=c.alpha,
                                 target_modules=c.target_modules, dropout=c.dropout)
@@ -315,6 +367,11 @@ class LoRATrainer:
             for m in model.modules():
                 if isinstance(m, LoRALinear):
                     m.activation_checkpoint = c.activation_checkpoint
+        if c.dropout_seed is not None:
+            rank = dist.get_rank(process_group) if dist.is_available() and dist.is_initialized() else 0
+            layers = [m for m in model.modules() if isinstance(m, LoRALinear)]
+            for i, m in enumerate(layers):
+                m.dropout_seed = c.dropout_seed + i + (rank << 32)
         self.params = FlatLoRAParams(model)
         self.optimizer = self._create_optimizer()
         self.state = TrainingState()
@@ -353,6 +410,8 @@ class LoRATrainer:
     def _compute_loss(self, batch: dict[str, torch.Tensor]) -> torch.Tensor:
         """trainer.py:216-226: shifted cross-entropy on ``labels``, else MSE to
         ``target_output`` (or to the output itself)."""
+        if self.config.loss_head is not None and "labels" in batch:
+            return self._head_loss(batch)
         outputs = self.model(batch["input_ids"])
         if "labels" in batch:
             logits = outputs[:, :-1, :]
@@ -361,6 +420,34 @@ class LoRATrainer:
                                                labels.reshape(-1))
         target = batch.get("target_output", outputs.detach())
         return torch.mean((outputs.float() - target.float()) ** 2)
+
+    def _head_loss(self, batch: dict[str, torch.Tensor]) -> torch.Tensor:
+        """The shifted cross-entropy of ``_compute_loss`` from the head's input: the
+        head hands its input through, and each position's label is the next one's."""
+        head = self.model.get_submodule(self.config.loss_head)
+        seen = []
+
+        def through(x, *args, **kwargs):
+            seen.append(x)
+            return x
+
+        head.forward = through
+        try:
+            hidden = self.model(batch["input_ids"])
+        finally:
+            del head.forward
+        if len(seen) != 1 or hidden is not seen[0]:
+            raise ConfigurationError(f"the model does not return the output of "
+                                     f"{self.config.loss_head!r} as it is")
+        labels = batch["labels"]
+        nxt = torch.full_like(labels, -100)
+        nxt[:, :-1] = labels[:, 1:]
+        if isinstance(head, nn.Linear):
+            return linear_cross_entropy(hidden, head.weight, nxt)
+        if head.merged:
+            return linear_cross_entropy(hidden, head.W0, nxt)
+        return linear_cross_entropy(hidden, head.W0, nxt, A=head.A, B=head.B, alpha=head.alpha,
+                                    _compute=head._compute_ab, _sink=head._grad_sink)
 
     def backward(self, batch: dict[str, torch.Tensor]) -> torch.Tensor:
         """Forward + backward of one micro-batch; LoRA gradients accumulate in
