@@ -1,9 +1,17 @@
 // The three products of a vocabulary head, as one persistent tcgen05 kernel over
 // CTA pairs:
 //
-//   logits  D[m, v] = sum_k x[m, k] W[v, k]   (+ X2[m, :] . B[v, :])   both K-major
+//   logits  l[m, v] = sum_k x[m, k] W[v, k]   (+ X2[m, :] . B[v, :])   both K-major
 //   dx      D[m, k] = sum_v g[m, v] W[v, k]   (+ U[m, :] . A[:, k])    W MN-major
 //   dW      D[v, k] = sum_m g[m, v] x[m, k]                            both MN-major
+//
+// The logits never leave the chip as such.  The epilogue takes, of each row's 256 in a
+// tile, the largest m_t and s_t = sum exp(l - m_t), and where a gradient is wanted
+// writes exp(l - m_t) as an fp16 value: 11 bits of a number in (0, 1], so that only
+// the rounding of g to its 16 bits shows, and half of what fp32 logits would move.
+// The label's own logit is left out (as -inf): it comes in 32 bits from the pass that
+// gathers x, since the tensor cores' accumulation cuts off bits at each of its K / 16
+// steps (about 2e-6 of a logit at K = 4096), which a loss shows as it is.
 //
 // A (2,1,1) cluster makes a 256 x 256 tile (tcgen05.mma.cta_group::2, M = N = 256,
 // K = 16): each CTA stages its own 128 rows of either operand in a 6-stage TMA ring
@@ -50,6 +58,11 @@ struct HeadGemmParams {
   float* d;
   long long ldd, split_stride;
   int accumulate;
+  // logits
+  const int32_t* label;  // of row m
+  __half* e;             // exp(l - m_t) * 2^15, rows ldd apart, or nullptr
+  float2* stats;         // (m_t, 2^15 s_t) of tile column t at [t * stats_ld + m]
+  long long stats_ld;
   uint32_t* status;
 };
 
@@ -128,6 +141,71 @@ __device__ __forceinline__ void store_row_f32(const HeadGemmParams& p, const Sha
       st_global_32b(dst, v);
     }
   }
+}
+
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// This thread's row of a tile of logits: largest, sum of exponentials, exponentials.
+// Two passes over the accumulator in TMEM; with K = 4096 it takes an eighth of the
+// main loop beside it.
+__device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape& s, const Unit& t,
+                                            int m, uint32_t taddr) {
+  const int n_base = t.tn * kTile;
+  const bool live = m < s.M;
+  const int y = live ? p.label[m] - n_base : -1;
+  const int width = p.N - n_base;  // columns of the vocabulary in this tile
+  float top = -INFINITY;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(taddr + c, r);
+    tmem_ld_wait();
+    if (c + 32 > width || __any_sync(0xffffffffu, static_cast<uint32_t>(y - c) < 32u)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c + i >= width || c + i == y) r[i] = __float_as_uint(-INFINITY);
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+  }
+  const float ref = top == -INFINITY ? 0.f : top;
+  float sum0 = 0.f, sum1 = 0.f;
+  __half* row = p.e + static_cast<long long>(m) * p.ldd + n_base;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(taddr + c, r);
+    tmem_ld_wait();
+    if (c + 32 > width || __any_sync(0xffffffffu, static_cast<uint32_t>(y - c) < 32u)) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (c + i >= width || c + i == y) r[i] = __float_as_uint(-INFINITY);
+    }
+    uint32_t e[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      // the difference first: exact near the top, where it counts
+      const float a = ex2(fmaf(__uint_as_float(r[2 * i]) - ref, 1.4426950408889634f, 15.f));
+      const float b = ex2(fmaf(__uint_as_float(r[2 * i + 1]) - ref, 1.4426950408889634f, 15.f));
+      sum0 += a;
+      sum1 += b;
+      e[i] = pack2<__half>(a, b);
+    }
+    if (live && p.e != nullptr) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (n_base + c + 16 * h < p.ldd) {
+          const uint32_t v[8] = {e[8 * h],     e[8 * h + 1], e[8 * h + 2], e[8 * h + 3],
+                                 e[8 * h + 4], e[8 * h + 5], e[8 * h + 6], e[8 * h + 7]};
+          st_global_32b(row + c + 16 * h, v);
+        }
+    }
+  }
+  if (live) p.stats[t.tn * p.stats_ld + m] = make_float2(top, sum0 + sum1);
 }
 
 template <bool kXMN, bool kWMN, bool kBF16>
@@ -296,7 +374,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
       tc_fence_after();
       const int m = t.tm * kTile + static_cast<int>(crank * kHalf + quarter * 32 + lane);
-      store_row_f32(p, shape, t, m, tmem_base + ((quarter * 32u) << 16) + buf * kTile);
+      const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile;
+      if constexpr (!kWMN)
+        softmax_row(p, shape, t, m, taddr);
+      else
+        store_row_f32(p, shape, t, m, taddr);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(lead_acc_empty + buf * 8u);
@@ -339,12 +421,12 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   }
   HeadGemmParams p;
   p.M = static_cast<int>(a.M);
-  p.N = static_cast<int>(a.n_store);
+  p.N = static_cast<int>(a.N);
   p.num_kb_main = static_cast<int>((a.K + kBK - 1) / kBK);
   p.R = static_cast<int>(a.R);
   p.num_kb_extra = static_cast<int>((a.R + kBK - 1) / kBK);
   const int tiles_m = static_cast<int>((a.M + kTile - 1) / kTile);
-  p.tiles_n = static_cast<int>((a.n_store + kTile - 1) / kTile);
+  p.tiles_n = static_cast<int>((a.N + kTile - 1) / kTile);
   p.splits = a.splits;
   p.group_m = a.group_m < tiles_m ? a.group_m : tiles_m;
   p.rows = a.rows;
@@ -354,6 +436,10 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   p.ldd = a.ldd;
   p.split_stride = a.split_stride;
   p.accumulate = a.accumulate ? 1 : 0;
+  p.label = a.label;
+  p.e = static_cast<__half*>(a.e);
+  p.stats = static_cast<float2*>(a.stats);
+  p.stats_ld = a.stats_ld;
   p.status = device_status_ptr();
 
   auto kern = head_gemm_kernel<kXMN, kWMN, kBF16>;

@@ -112,77 +112,133 @@ __global__ void __launch_bounds__(kScanThreads)
 }
 
 // xc[i] = x[row_of[i]], zeros past the last counted token (as many as a reduction
-// over tokens reads; all of them for the LoRA products, which run over every row).
+// over tokens reads; all of them for the LoRA products, which run over every row);
+// and target[i] = the label's logit but for a LoRA term, in 32 bits.
+template <typename T>
 __global__ void __launch_bounds__(128)
-    head_gather_kernel(const uint4* x, const int32_t* row_of, const HeadCount* count, int64_t K8,
-                       int zero_all, uint4* xc) {
+    head_gather_kernel(const uint4* x, const uint4* w, const int32_t* row_of, const int32_t* label,
+                       const HeadCount* count, int64_t K8, int zero_all, uint4* xc, float* target) {
+  __shared__ float part[4];
   const int64_t i = blockIdx.x;
   const int32_t row = row_of[i];
-  if (row < 0 && !zero_all && i >= (count->counted + 63) / 64 * 64) return;
-  for (int64_t k = threadIdx.x; k < K8; k += 128)
-    xc[i * K8 + k] = row < 0 ? make_uint4(0, 0, 0, 0) : x[static_cast<int64_t>(row) * K8 + k];
+  if (row < 0) {
+    if (zero_all || i < (count->counted + 63) / 64 * 64)
+      for (int64_t k = threadIdx.x; k < K8; k += 128) xc[i * K8 + k] = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  const uint4* xr = x + static_cast<int64_t>(row) * K8;
+  const uint4* wr = w + static_cast<int64_t>(label[i]) * K8;
+  float s = 0.f;
+#pragma unroll 4
+  for (int64_t k = threadIdx.x; k < K8; k += 128) {
+    const uint4 xv = xr[k], wv = wr[k];
+    xc[i * K8 + k] = xv;
+    const T* xe = reinterpret_cast<const T*>(&xv);
+    const T* we = reinterpret_cast<const T*>(&wv);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s = fmaf(static_cast<float>(xe[j]), static_cast<float>(we[j]), s);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) target[i] = part[0] + part[1] + (part[2] + part[3]);
 }
 
 __device__ __forceinline__ void join_max_sum(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
   // two empty parts (or rows of -infinity): nothing to scale by
   const float ref = top == -INFINITY ? 0.f : top;
-  s = s * __expf(m - ref) + s2 * __expf(m2 - ref);
+  s = s * expf(m - ref) + s2 * expf(m2 - ref);
   m = top;
 }
 
-// One CTA per counted token of the piece: its loss, and its row of g in 16 bits.
-// What rounding g[y] left over, the largest and always present part, goes to
-// `rest`, which the gradient of x adds back times W[y].
+// One CTA per counted token of the piece: its loss, and its row of g in place of the
+// exponentials, e[v] -> g[v] = 2^-15 e[v] exp(m_t - lse).  With the sum S exp(m) over
+// the other entries and u = S exp(m - l_y), the loss is log(1 + u) and
+// g[y] = -u / (1 + u), without cancellation for a token that is nearly certain.
+// What rounding g[y], the largest part, left over goes to `rest`, which the gradient
+// of x adds back times W[y].  Bound: HBM, 4 bytes a logit.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-    head_row_kernel(const float* logits, int64_t ld, int64_t V, int64_t row0, int64_t rows,
+    head_row_kernel(const float2* stats, int64_t stats_ld, int64_t V, int64_t ld, int64_t row0,
                     const HeadCount* count, const int32_t* label, const int32_t* row_of,
-                    float* row_loss, float* nll, T* g, float* rest, int zero_all) {
-  __shared__ float sm[kRowThreads / 32], ss[kRowThreads / 32];
+                    const float* target, const T* xa, const T* b, int64_t xa_ld, int r,
+                    float* row_loss, float* nll, void* eg, float* rest, int zero_all) {
+  extern __shared__ float factor[];  // of each tile of logits
+  __shared__ float sm[kRowThreads / 32], ss[kRowThreads / 32], sx[kRowThreads / 32];
   const int64_t i = blockIdx.x;
   const int64_t slot = row0 + i;
   const int32_t counted = count->counted;
-  T* grow = g + i * ld;
+  uint4* row = static_cast<uint4*>(eg) + i * (ld / 8);
   if (slot >= counted) {
-    if (g != nullptr && (zero_all || slot < (counted + 63) / 64 * 64))
-      for (int64_t v = threadIdx.x; v < ld; v += kRowThreads) grow[v] = static_cast<T>(0.f);
+    if (eg != nullptr && (zero_all || slot < (counted + 63) / 64 * 64))
+      for (int64_t v = threadIdx.x; v < ld / 8; v += kRowThreads) row[v] = make_uint4(0, 0, 0, 0);
     return;
   }
-  const float* l = logits + i * ld;
-  float m = -INFINITY, s = 0.f;
-  for (int64_t v = threadIdx.x; v < V; v += kRowThreads) {
-    const float t = l[v];
-    if (t > m) {
-      s *= __expf(m - t);
-      m = t;
-    }
-    s += t == -INFINITY ? 0.f : __expf(t - m);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    join_max_sum(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = m, ss[threadIdx.x >> 5] = s;
-  __syncthreads();
-  m = sm[0], s = ss[0];
-  for (int w = 1; w < kRowThreads / 32; ++w) join_max_sum(m, s, sm[w], ss[w]);
   const int32_t y = label[slot];
-  const float log_sum = logf(s);
-  const float loss = log_sum + (m - l[y]);
+  const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
+  float m = -INFINITY, s = 0.f, extra = 0.f;
+  for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
+    const float2 q = stats[t * stats_ld + i];
+    factor[t] = q.x;
+    join_max_sum(m, s, q.x, q.y * (1.f / 32768.f));
+  }
+  for (int j = threadIdx.x; j < r; j += kRowThreads)  // the label's LoRA term
+    extra += static_cast<float>(xa[slot * xa_ld + j]) *
+             static_cast<float>(b[static_cast<int64_t>(y) * r + j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    join_max_sum(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
+    extra += __shfl_xor_sync(0xffffffffu, extra, o);
+  }
+  if ((threadIdx.x & 31) == 0)
+    sm[threadIdx.x >> 5] = m, ss[threadIdx.x >> 5] = s, sx[threadIdx.x >> 5] = extra;
+  __syncthreads();
+  m = sm[0], s = ss[0], extra = sx[0];
+  for (int w = 1; w < kRowThreads / 32; ++w) {
+    join_max_sum(m, s, sm[w], ss[w]);
+    extra += sx[w];
+  }
+  const float ly = target[slot] + extra;
+  // log(exp(l_y) + S exp(m)) from the larger of the two
+  const float gap = m - ly;
+  const float u = s * expf(gap);
+  const float loss = gap < 0.f || s == 0.f ? log1pf(u) : gap + logf(s + expf(-gap));
   if (threadIdx.x == 0) {
     nll[slot] = loss;
     if (row_loss != nullptr) row_loss[row_of[slot]] = loss;
   }
-  if (g == nullptr) return;
+  if (eg == nullptr) return;
   constexpr float unit = grad_unit<T>();
-  const float inv = unit / s;
-  for (int64_t v = threadIdx.x; v < ld; v += kRowThreads) {
-    float o = v < V ? __expf(l[v] - m) * inv : 0.f;
-    if (v == y) {
-      o = unit * expm1f(-loss);  // p - 1 without cancellation
-      rest[slot] = o - static_cast<float>(static_cast<T>(o));
+  const float lse = loss + ly;
+  __syncthreads();
+  for (int t = threadIdx.x; t < tiles; t += kRowThreads)
+    factor[t] = factor[t] == -INFINITY ? 0.f : expf(factor[t] - lse) * (unit / 32768.f);
+  __syncthreads();
+  // -u / (1 + u), and -1 where u has no number
+  const float gy = -unit * (gap < 60.f ? u / (1.f + u) : 1.f);
+  if (threadIdx.x == 0) rest[slot] = gy - static_cast<float>(static_cast<T>(gy));
+#pragma unroll 4
+  for (int64_t q = threadIdx.x; q < ld / 8; q += kRowThreads) {
+    uint4 v = row[q];
+    const float f = factor[q * 8 / kHeadTile];
+    const __half2* e = reinterpret_cast<const __half2*>(&v);
+    float o[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 p = __half22float2(e[j]);
+      o[2 * j] = p.x * f;
+      o[2 * j + 1] = p.y * f;
     }
-    grow[v] = static_cast<T>(o);
+    if (q == y >> 3) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j == (y & 7)) o[j] = gy;
+    }
+    v = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
+                   pack2<T>(o[6], o[7]));
+    row[q] = v;
   }
 }
 
@@ -303,7 +359,8 @@ struct Dims {
     return v;
   }
   int64_t R64() const { return round_up(R(), 64); }
-  int64_t ld() const { return round_up(V, 8); }
+  int64_t ld() const { return round_up(V, 16); }  // of a row of e and g
+  int64_t tiles() const { return (V + kHeadTile - 1) / kHeadTile; }
 };
 
 // Ranges of the vocabulary that dx is summed over: enough for the tiles of few tokens
@@ -355,8 +412,9 @@ State plan_state(void* base, const Dims& d) {
 struct Work {
   int32_t* row_of;
   float* nll;
-  void *xc, *xa_rows, *xa_t, *bt, *u_rows, *u_t, *g;
-  float* logits;
+  float* target;
+  void *xc, *xa_rows, *xa_t, *bt, *u_rows, *u_t, *eg;
+  float2* stats;
   int64_t piece;  // rows that go through at a time
   int64_t bytes;
 };
@@ -364,13 +422,14 @@ struct Work {
 Work plan_work(void* base, const Dims& d) {
   Work w{};
   Carve c(base);
-  // pieces of a gigabyte and a half (or 256 rows), equal up to the tile
-  const int64_t per_row = d.ld() * (d.grads ? 6 : 4);
-  int64_t most = std::max<int64_t>(int64_t{1536} << 20, 256 * per_row) / per_row / 256 * 256;
+  // pieces of two gigabytes (or 256 rows), equal up to the tile
+  const int64_t per_row = d.tiles() * 8 + (d.grads ? d.ld() * 2 : 0);
+  const int64_t most = std::max<int64_t>(int64_t{2048} << 20, 256 * per_row) / per_row / 256 * 256;
   const int64_t n = (d.M + most - 1) / most;
   w.piece = std::min(d.M, round_up((d.M + n - 1) / n, 256));
   w.row_of = c.take<int32_t>(d.M);
   w.nll = c.take<float>(d.M);
+  w.target = c.take<float>(d.M);
   w.xc = c.take<uint16_t>(d.M * d.K);
   if (d.lora()) {
     w.xa_rows = c.take<uint16_t>(d.M * d.R64());
@@ -381,8 +440,8 @@ Work plan_work(void* base, const Dims& d) {
       w.u_t = c.take<uint16_t>(d.R() * round_up(w.piece, 8));
     }
   }
-  w.logits = c.take<float>(w.piece * d.ld());
-  if (d.grads) w.g = c.take<uint16_t>(w.piece * d.ld());
+  w.stats = c.take<float2>(d.tiles() * w.piece);
+  if (d.grads) w.eg = c.take<uint16_t>(w.piece * d.ld());
   w.bytes = round_up(c.off, 256);
   return w;
 }
@@ -400,7 +459,7 @@ int check_dims(const Dims& d, int dtype) {
     return fail(MLORA_ERR_UNSUPPORTED, "K and r must be multiples of 8 (16-byte rows)");
   if (d.lora() && d.V % 8)
     return fail(MLORA_ERR_UNSUPPORTED, "a LoRA head needs V % 8 == 0 (16-byte rows of B^T)");
-  if (d.M > (int64_t{1} << 31) - 256 || d.K > (1 << 24) || d.V > (1 << 24))
+  if (d.M > (int64_t{1} << 31) - 256 || d.K > (1 << 24) || d.V > (1 << 21))
     return fail(MLORA_ERR_UNSUPPORTED, "shape too large");
   return MLORA_OK;
 }
@@ -420,9 +479,9 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
   }
   {
     LaunchScope scope(kKindElementwise, s);
-    head_gather_kernel<<<static_cast<unsigned>(M), 128, 0, s>>>(
-        static_cast<const uint4*>(x), ws.row_of, st.count, K / 8, zero_all,
-        static_cast<uint4*>(ws.xc));
+    head_gather_kernel<T><<<static_cast<unsigned>(M), 128, 0, s>>>(
+        static_cast<const uint4*>(x), static_cast<const uint4*>(w), ws.row_of, st.label, st.count,
+        K / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target);
   }
   if ((rc = launch_status(cudaSuccess, "linear cross entropy: gather"))) return rc;
   RankArgs ra;
@@ -452,16 +511,18 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     l.product = HeadProduct::kLogits;
     l.x = xc;
     l.w = w;
-    l.d = ws.logits;
     l.M = rows;
     l.N = V;
     l.K = K;
-    l.n_store = ld;
     l.ldx = K;
     l.ldw = K;
     l.ldd = ld;
     l.rows = &st.count->counted;
     l.row0 = row0;
+    l.label = st.label + row0;
+    l.e = ws.eg;
+    l.stats = ws.stats;
+    l.stats_ld = ws.piece;
     l.elt = elt;
     if (d.lora()) {
       l.x2 = static_cast<const T*>(ws.xa_rows) + row0 * d.R64();
@@ -474,14 +535,15 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     if ((rc = launch_head_gemm(l, s))) return rc;
     {
       LaunchScope scope(kKindElementwise, s);
-      head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, 0, s>>>(
-          ws.logits, ld, V, row0, rows, st.count, st.label, ws.row_of, row_loss, ws.nll,
-          static_cast<T*>(ws.g), st.rest, zero_all);
+      head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, d.tiles() * 4, s>>>(
+          ws.stats, ws.piece, V, ld, row0, st.count, st.label, ws.row_of, ws.target,
+          static_cast<const T*>(ws.xa_rows), static_cast<const T*>(b), d.R64(),
+          static_cast<int>(d.r), row_loss, ws.nll, ws.eg, st.rest, zero_all);
       if ((rc = launch_status(cudaSuccess, "linear cross entropy: rows"))) return rc;
     }
     if (d.lora() && d.grads) {
       RankArgs ru = ra;  // U = s g B
-      ru.x = ws.g;
+      ru.x = ws.eg;
       ru.l = ws.bt;
       ru.M = rows;
       ru.K = V;
@@ -495,7 +557,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       if ((rc = launch_rank(ru, s))) return rc;
       if (d.want(MLORA_HEAD_GRAD_AB)) {
         WgradArgs g[2];
-        g[0].big = ws.g;
+        g[0].big = ws.eg;
         g[0].st = static_cast<const T*>(ws.xa_t) + row0;
         g[0].ld_st = round_up(M, 8);
         g[0].M = rows;
@@ -525,13 +587,12 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     if (d.want(MLORA_HEAD_GRAD_X)) {
       HeadGemmArgs q;
       q.product = HeadProduct::kDx;
-      q.x = ws.g;
+      q.x = ws.eg;
       q.w = w;
       q.d = st.dx + row0 * K;
       q.M = rows;
       q.N = K;
       q.K = V;
-      q.n_store = K;
       q.ldx = ld;
       q.ldw = K;
       q.ldd = K;
@@ -553,13 +614,12 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     if (d.want(MLORA_HEAD_GRAD_W)) {
       HeadGemmArgs q;
       q.product = HeadProduct::kDw;
-      q.x = ws.g;
+      q.x = ws.eg;
       q.w = xc;
       q.d = st.dw;
       q.M = V;
       q.N = K;
       q.K = rows;
-      q.n_store = K;
       q.ldx = ld;
       q.ldw = K;
       q.ldd = K;

@@ -230,11 +230,13 @@ struct LoraBwdArgs {
 int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t stream);
 
 // ------------------------------------------------------- vocabulary head -----
-// The products of the linear cross entropy (head_gemm.cu), fp32 out.  With g the
-// gradient of the logits [tokens, V]:
-//   kLogits: D[m, v] = x . W^T + x2 . w2^T    x [M, K], w [N, K], x2 [M, R64], w2 [N, r]
+// The products of the linear cross entropy (head_gemm.cu).  With g the gradient of the
+// logits [tokens, V]:
+//   kLogits: l[m, v] = x . W^T + x2 . w2^T    x [M, K], w [N, K], x2 [M, R64], w2 [N, r]
+//            out: stats and e, see there
 //   kDx:     D[m, k] = g . W + x2 . w2        x = g [M, K = V], w [K, N], w2 [r, N]
 //   kDw:     D[v, k] = g^T . x                x = g [K tokens, M = V], w = x [K, N]
+//            out: fp32 D, N a multiple of 8
 enum class HeadProduct { kLogits, kDx, kDw };
 struct HeadGemmArgs {
   HeadProduct product;
@@ -242,9 +244,8 @@ struct HeadGemmArgs {
   const void* w;
   const void* x2 = nullptr;
   const void* w2 = nullptr;
-  float* d;                  // `splits` copies of [M, n_store], split_stride floats apart
+  float* d = nullptr;        // `splits` copies of [M, N], split_stride floats apart
   int64_t M = 0, N = 0, K = 0;
-  int64_t n_store = 0;       // columns of D to store: a multiple of 8, at least N
   int64_t R = 0, w2_rows = 0;
   int64_t ldx = 0, ldw = 0, ldx2 = 0, ldw2 = 0, ldd = 0, split_stride = 0;
   int splits = 1;            // at most the 64-wide blocks of the reduction
@@ -252,8 +253,14 @@ struct HeadGemmArgs {
   const int32_t* rows = nullptr;  // counted tokens (device); those from row0 on are meant
   int64_t row0 = 0;
   bool accumulate = false;   // D += (splits = 1)
+  const int32_t* label = nullptr;  // kLogits: of row m
+  void* e = nullptr;         // kLogits: [M, ldd] fp16 exp(l - tile's largest) * 2^15 or nullptr;
+                             // ldd a multiple of 16, at least N
+  void* stats = nullptr;     // kLogits: float2 [ceil(N / 256), stats_ld]
+  int64_t stats_ld = 0;
   Elt elt = Elt::kBF16;
 };
+constexpr int kHeadTile = 256;  // columns of a tile of logits
 int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s);
 int head_gemm_pairs();  // CTA pairs that are resident at once
 
