@@ -10,8 +10,11 @@
 // writes exp(l - m_t) as an fp16 value: 11 bits of a number in (0, 1], so that only
 // the rounding of g to its 16 bits shows, and half of what fp32 logits would move.
 // The label's own logit is left out (as -inf): it comes in 32 bits from the pass that
-// gathers x, since the tensor cores' accumulation cuts off bits at each of its K / 16
-// steps (about 2e-6 of a logit at K = 4096), which a loss shows as it is.
+// gathers x, since the tensor cores' accumulation rounds toward zero at each of its
+// K / 16 steps, which a loss shows as it is.  Of the other logits that cut is given back
+// on average: it measured 1.0e-9 K of the value (0.24e-6 at K = 256, 4.0e-6 at 4096,
+// 8.4e-6 at 8192; its deviation a tenth to a half of that) for sums that drift or walk
+// to where they end, 3.5 times as much where every product has the same sign.
 //
 // A (2,1,1) cluster makes a 256 x 256 tile (tcgen05.mma.cta_group::2, M = N = 256,
 // K = 16): each CTA stages its own 128 rows of either operand in a 6-stage TMA ring
@@ -46,6 +49,7 @@ constexpr uint32_t kMNBoxBytes = 64 * kBK * 2;      // one MN-major TMA box (8 K
 constexpr int kEpiWarps = 4;
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kTmemCols = 512;
+constexpr float kCutPerK = 1.0e-9f;
 constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + 256;
 
 struct HeadGemmParams {
@@ -61,6 +65,7 @@ struct HeadGemmParams {
   // logits
   const int32_t* label;  // of row m
   __half* e;             // exp(l - m_t) * 2^15, rows ldd apart, or nullptr
+  float uncut;           // what a logit is multiplied by
   float2* stats;         // (m_t, 2^15 s_t) of tile column t at [t * stats_ld + m]
   long long stats_ld;
   uint32_t* status;
@@ -173,6 +178,7 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
     for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
   }
   const float ref = top == -INFINITY ? 0.f : top;
+  const float log2e = 1.4426950408889634f * p.uncut;
   float sum0 = 0.f, sum1 = 0.f;
   __half* row = p.e + static_cast<long long>(m) * p.ldd + n_base;
 #pragma unroll 1
@@ -189,8 +195,8 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       // the difference first: exact near the top, where it counts
-      const float a = ex2(fmaf(__uint_as_float(r[2 * i]) - ref, 1.4426950408889634f, 15.f));
-      const float b = ex2(fmaf(__uint_as_float(r[2 * i + 1]) - ref, 1.4426950408889634f, 15.f));
+      const float a = ex2(fmaf(__uint_as_float(r[2 * i]) - ref, log2e, 15.f));
+      const float b = ex2(fmaf(__uint_as_float(r[2 * i + 1]) - ref, log2e, 15.f));
       sum0 += a;
       sum1 += b;
       e[i] = pack2<__half>(a, b);
@@ -205,7 +211,7 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
         }
     }
   }
-  if (live) p.stats[t.tn * p.stats_ld + m] = make_float2(top, sum0 + sum1);
+  if (live) p.stats[t.tn * p.stats_ld + m] = make_float2(top * p.uncut, sum0 + sum1);
 }
 
 template <bool kXMN, bool kWMN, bool kBF16>
@@ -440,6 +446,7 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   p.e = static_cast<__half*>(a.e);
   p.stats = static_cast<float2*>(a.stats);
   p.stats_ld = a.stats_ld;
+  p.uncut = 1.f + kCutPerK * static_cast<float>(a.K);
   p.status = device_status_ptr();
 
   auto kern = head_gemm_kernel<kXMN, kWMN, kBF16>;
