@@ -555,17 +555,19 @@ MLORA_API int mlora_embedding_backward(const int64_t* idx, const void* dy, void*
 /* ---- counter-based dropout ---------------------------------------------- */
 
 /* out = kept ? x * 65536 / (65536 - threshold) : 0 over n elements in a row (out may be
- * x).  Element e is kept where half-word e % 8 (low half first) of Philox4x32-10's
+ * x); without `scaled` kept ? x : 0.  Element e is kept where half-word e % 8 (low half first) of Philox4x32-10's
  * four words for the key `seed` and the counter (e / 8, call) is at least `threshold`
  * (0..65536).  No mask is stored: the gradient is the same call on dy.  seed_dev, where
  * not NULL, is a device int64 that takes the seed's place, read when the kernel runs. */
-MLORA_API int mlora_dropout(const void* x, void* out, int64_t n, int threshold, uint64_t seed,
-                            const int64_t* seed_dev, uint64_t call, int dtype, void* stream);
+MLORA_API int mlora_dropout(const void* x, void* out, int64_t n, int threshold, int scaled,
+                            uint64_t seed, const int64_t* seed_dev, uint64_t call, int dtype,
+                            void* stream);
 
 /* y = x.W0^T + dropout((alpha/r)(x.A^T).B^T), the dropout as above over [M, N]; BF16 or
- * F16, N a multiple of 8.  saved_xa as for mlora_lora_forward.  Its gradient: with
- * dz = dropout(dy), mlora_lora_backward_ex of dz with MLORA_BWD_DEFER_DX, then of dy
- * with MLORA_BWD_DX_ONLY. */
+ * F16, N a multiple of 8.  saved_xa as for mlora_lora_forward with alpha times
+ * c = 65536 / (65536 - threshold).  Its gradient: with dz the dropout of dy, not scaled,
+ * mlora_lora_backward_ex of dz with alpha c and MLORA_BWD_DEFER_DX, then of dy with
+ * MLORA_BWD_DX_ONLY. */
 MLORA_API size_t mlora_lora_forward_dropout_workspace_bytes(int64_t M, int64_t K, int64_t N,
                                                             int64_t r, int dtype);
 MLORA_API int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a,

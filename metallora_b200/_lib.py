@@ -126,7 +126,7 @@ SIGNATURES: dict[str, tuple] = {
     "mlora_embedding_forward": (i32, [vp, vp, vp, i64, i64, i64, f32, i32, vp]),
     "mlora_embedding_backward_workspace_bytes": (sz, [i64, i64]),
     "mlora_embedding_backward": (i32, [vp, vp, vp, i64, i64, i64, f32, i64, i32, vp, sz, vp]),
-    "mlora_dropout": (i32, [vp, vp, i64, i32, u64, vp, u64, i32, vp]),
+    "mlora_dropout": (i32, [vp, vp, i64, i32, i32, u64, vp, u64, i32, vp]),
     "mlora_lora_forward_dropout_workspace_bytes": (sz, [i64, i64, i64, i64, i32]),
     "mlora_lora_forward_dropout": (i32, [vp] * 6 + [i64] * 4 + [f32, i32, u64, vp, u64, i32, vp, sz,
                                                                 vp]),

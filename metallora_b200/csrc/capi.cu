@@ -1045,7 +1045,9 @@ int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, con
   ra.R = p.R;
   ra.ldx = K;
   ra.ldl = K;
-  ra.scale = alpha / static_cast<float>(r);
+  // the kept elements' factor goes in here: what is left of the mask is 0 or 1, exact in
+  // any type, in the forward and on dy
+  ra.scale = alpha / static_cast<float>(r) * dropout_scale(static_cast<uint32_t>(threshold));
   ra.out_rows = p.xa_rows;
   ra.ld_rows = p.R64;
   ra.out_t = saved_xa;
@@ -1068,7 +1070,7 @@ int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, con
   gz.out_dtype = dtype;
   if ((rc = launch_gemm(gz, s))) return rc;
   const DropoutKey key{seed, seed_dev, call, static_cast<uint32_t>(threshold)};
-  if ((rc = launch_dropout(z, z, M * N, dtype, key, s))) return rc;
+  if ((rc = launch_dropout(z, z, M * N, dtype, key, false, s))) return rc;
   GemmArgs ga = gz;  // y = x . W0^T + drop(z)
   ga.x = x;
   ga.w = w0;

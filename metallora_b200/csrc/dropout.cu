@@ -44,9 +44,8 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
 // x and out may be the same; `vec`: both start on 16 bytes.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    dropout_kernel(const T* x, T* out, int64_t n, int vec, DropoutKey key) {
+    dropout_kernel(const T* x, T* out, int64_t n, int vec, float scale, DropoutKey key) {
   const uint64_t seed = dropout_seed(key);
-  const float scale = dropout_scale(key.threshold);
   const int64_t blocks = (n + 7) / 8;
   for (int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; b < blocks;
        b += static_cast<int64_t>(gridDim.x) * kThreads) {
@@ -71,7 +70,8 @@ __global__ void __launch_bounds__(kThreads)
 }  // namespace
 
 int launch_dropout(const void* x, void* out, int64_t n, int dtype, const DropoutKey& key,
-                   cudaStream_t s) {
+                   bool scaled, cudaStream_t s) {
+  const float scale = scaled ? dropout_scale(key.threshold) : 1.f;
   const int64_t blocks = (n + 7) / 8;
   const unsigned grid = static_cast<unsigned>(
       std::min<int64_t>((blocks + kThreads - 1) / kThreads, int64_t{num_sms()} * 64));
@@ -79,13 +79,13 @@ int launch_dropout(const void* x, void* out, int64_t n, int dtype, const Dropout
   LaunchScope scope(kKindElementwise, s);
   if (dtype == MLORA_DTYPE_BF16)
     dropout_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x),
-                                             static_cast<__nv_bfloat16*>(out), n, vec, key);
+                                             static_cast<__nv_bfloat16*>(out), n, vec, scale, key);
   else if (dtype == MLORA_DTYPE_F16)
     dropout_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __half*>(x),
-                                             static_cast<__half*>(out), n, vec, key);
+                                             static_cast<__half*>(out), n, vec, scale, key);
   else
     dropout_kernel<<<grid, kThreads, 0, s>>>(static_cast<const float*>(x), static_cast<float*>(out),
-                                             n, vec, key);
+                                             n, vec, scale, key);
   return launch_status(cudaSuccess, "dropout");
 }
 
@@ -93,8 +93,9 @@ int launch_dropout(const void* x, void* out, int64_t n, int dtype, const Dropout
 
 using namespace mlora;
 
-extern "C" int mlora_dropout(const void* x, void* out, int64_t n, int threshold, uint64_t seed,
-                             const int64_t* seed_dev, uint64_t call, int dtype, void* stream) {
+extern "C" int mlora_dropout(const void* x, void* out, int64_t n, int threshold, int scaled,
+                             uint64_t seed, const int64_t* seed_dev, uint64_t call, int dtype,
+                             void* stream) {
   auto fail = [](int code, const char* msg) {
     set_error(msg);
     return code;
@@ -111,5 +112,5 @@ extern "C" int mlora_dropout(const void* x, void* out, int64_t n, int threshold,
     return fail(MLORA_ERR_INVALID_ARG, "pointers must be whole elements");
   if (int rc = require_device()) return rc;
   const DropoutKey key{seed, seed_dev, call, static_cast<uint32_t>(threshold)};
-  return launch_dropout(x, out, n, dtype, key, static_cast<cudaStream_t>(stream));
+  return launch_dropout(x, out, n, dtype, key, scaled != 0, static_cast<cudaStream_t>(stream));
 }

@@ -145,6 +145,18 @@ __global__ void __launch_bounds__(128)
   if (threadIdx.x == 0) target[i] = part[0] + part[1] + (part[2] + part[3]);
 }
 
+// W2 of the logits: [B 0 | B 0], R columns each, for the two parts of s x A^T.
+__global__ void __launch_bounds__(256)
+    head_stack_kernel(const uint16_t* b, int64_t V, int r, int R, uint16_t* b2) {
+  const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e >= V * R) return;
+  const int64_t v = e / R;
+  const int j = static_cast<int>(e - v * R);
+  const uint16_t x = j < r ? b[v * r + j] : uint16_t{0};
+  b2[v * 2 * R + j] = x;
+  b2[v * 2 * R + R + j] = x;
+}
+
 __device__ __forceinline__ void join_max_sum(float& m, float& s, float m2, float s2) {
   const float top = fmaxf(m, m2);
   // two empty parts (or rows of -infinity): nothing to scale by
@@ -163,7 +175,7 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
     head_row_kernel(const float2* stats, int64_t stats_ld, int64_t V, int64_t ld, int64_t row0,
                     const HeadCount* count, const int32_t* label, const int32_t* row_of,
-                    const float* target, const T* xa, const T* b, int64_t xa_ld, int r,
+                    const float* target, const T* xa, const T* b, int64_t xa_ld, int r, int R,
                     float* row_loss, float* nll, void* eg, float* rest, int zero_all) {
   extern __shared__ float factor[];  // of each tile of logits
   __shared__ float sm[kRowThreads / 32], ss[kRowThreads / 32], sx[kRowThreads / 32];
@@ -184,9 +196,11 @@ __global__ void __launch_bounds__(kRowThreads)
     factor[t] = q.x;
     join_max_sum(m, s, q.x, q.y * (1.f / 32768.f));
   }
-  for (int j = threadIdx.x; j < r; j += kRowThreads)  // the label's LoRA term
-    extra += static_cast<float>(xa[slot * xa_ld + j]) *
+  for (int j = threadIdx.x; j < r; j += kRowThreads) {  // the label's LoRA term
+    const T* part = xa + slot * xa_ld + j;
+    extra += (static_cast<float>(part[0]) + static_cast<float>(part[R])) *
              static_cast<float>(b[static_cast<int64_t>(y) * r + j]);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     join_max_sum(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
@@ -359,6 +373,7 @@ struct Dims {
     return v;
   }
   int64_t R64() const { return round_up(R(), 64); }
+  int64_t ld_xa() const { return round_up(2 * R(), 64); }  // two parts of s x A^T
   int64_t ld() const { return round_up(V, 16); }  // of a row of e and g
   int64_t tiles() const { return (V + kHeadTile - 1) / kHeadTile; }
 };
@@ -413,7 +428,7 @@ struct Work {
   int32_t* row_of;
   float* nll;
   float* target;
-  void *xc, *xa_rows, *xa_t, *bt, *u_rows, *u_t, *eg;
+  void *xc, *xa_rows, *xa_t, *xa_lo, *b2, *bt, *u_rows, *u_t, *u_lo, *eg;
   float2* stats;
   int64_t piece;  // rows that go through at a time
   int64_t bytes;
@@ -432,12 +447,15 @@ Work plan_work(void* base, const Dims& d) {
   w.target = c.take<float>(d.M);
   w.xc = c.take<uint16_t>(d.M * d.K);
   if (d.lora()) {
-    w.xa_rows = c.take<uint16_t>(d.M * d.R64());
-    w.xa_t = c.take<uint16_t>(d.R() * round_up(d.M, 8));
+    w.xa_rows = c.take<uint16_t>(d.M * d.ld_xa());
+    w.b2 = c.take<uint16_t>(d.V * 2 * d.R());
     if (d.grads) {
+      w.xa_t = c.take<uint16_t>(d.R() * round_up(d.M, 8));
+      w.xa_lo = c.take<uint16_t>(d.R() * round_up(d.M, 8));
       w.bt = c.take<uint16_t>(d.R() * d.V);
       w.u_rows = c.take<uint16_t>(w.piece * d.R64());
       w.u_t = c.take<uint16_t>(d.R() * round_up(w.piece, 8));
+      w.u_lo = c.take<uint16_t>(d.R() * round_up(w.piece, 8));
     }
   }
   w.stats = c.take<float2>(d.tiles() * w.piece);
@@ -496,12 +514,20 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     ra.ldl = K;
     ra.scale = alpha / static_cast<float>(d.r);
     ra.out_rows = ws.xa_rows;
-    ra.ld_rows = d.R64();
+    ra.ld_rows = d.ld_xa();
+    ra.two_rows = true;
     ra.out_t = ws.xa_t;
+    ra.out_t_lo = ws.xa_lo;
     ra.ld_t = round_up(M, 8);
     ra.splits = rank_splits(M, K);
     ra.elt = elt;
     if ((rc = launch_rank(ra, s))) return rc;
+    {
+      LaunchScope scope(kKindElementwise, s);
+      head_stack_kernel<<<static_cast<unsigned>((V * d.R() + 255) / 256), 256, 0, s>>>(
+          static_cast<const uint16_t*>(b), V, static_cast<int>(d.r), static_cast<int>(d.R()),
+          static_cast<uint16_t*>(ws.b2));
+    }
     if (d.grads && (rc = launch_transpose_pad(b, V, d.r, d.r, ws.bt, d.R(), elt, s))) return rc;
   }
   for (int64_t row0 = 0; row0 < M; row0 += ws.piece) {
@@ -525,20 +551,20 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     l.stats_ld = ws.piece;
     l.elt = elt;
     if (d.lora()) {
-      l.x2 = static_cast<const T*>(ws.xa_rows) + row0 * d.R64();
-      l.w2 = b;
-      l.R = d.R();
-      l.w2_rows = d.r;
-      l.ldx2 = d.R64();
-      l.ldw2 = d.r;
+      l.x2 = static_cast<const T*>(ws.xa_rows) + row0 * d.ld_xa();
+      l.w2 = ws.b2;
+      l.R = 2 * d.R();
+      l.w2_rows = 2 * d.R();
+      l.ldx2 = d.ld_xa();
+      l.ldw2 = 2 * d.R();
     }
     if ((rc = launch_head_gemm(l, s))) return rc;
     {
       LaunchScope scope(kKindElementwise, s);
       head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, d.tiles() * 4, s>>>(
           ws.stats, ws.piece, V, ld, row0, st.count, st.label, ws.row_of, ws.target,
-          static_cast<const T*>(ws.xa_rows), static_cast<const T*>(b), d.R64(),
-          static_cast<int>(d.r), row_loss, ws.nll, ws.eg, st.rest, zero_all);
+          static_cast<const T*>(ws.xa_rows), static_cast<const T*>(b), d.ld_xa(),
+          static_cast<int>(d.r), static_cast<int>(d.R()), row_loss, ws.nll, ws.eg, st.rest, zero_all);
       if ((rc = launch_status(cudaSuccess, "linear cross entropy: rows"))) return rc;
     }
     if (d.lora() && d.grads) {
@@ -551,7 +577,10 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       ru.ldx = ld;
       ru.ldl = V;
       ru.out_rows = ws.u_rows;
+      ru.ld_rows = d.R64();
+      ru.two_rows = false;
       ru.out_t = ws.u_t;
+      ru.out_t_lo = ws.u_lo;
       ru.ld_t = round_up(ws.piece, 8);
       ru.splits = rank_splits(rows, V);
       if ((rc = launch_rank(ru, s))) return rc;
@@ -559,6 +588,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
         WgradArgs g[2];
         g[0].big = ws.eg;
         g[0].st = static_cast<const T*>(ws.xa_t) + row0;
+        g[0].st_lo = static_cast<const T*>(ws.xa_lo) + row0;
         g[0].ld_st = round_up(M, 8);
         g[0].M = rows;
         g[0].P = V;
@@ -575,6 +605,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
         g[1] = g[0];
         g[1].big = xc;
         g[1].st = ws.u_t;
+        g[1].st_lo = ws.u_lo;
         g[1].ld_st = round_up(ws.piece, 8);
         g[1].P = K;
         g[1].ldb = K;

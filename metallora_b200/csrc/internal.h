@@ -166,6 +166,10 @@ struct RankArgs {
   int64_t ld_rows;
   void* out_t;     // bf16/f16 [R, ld_t] or nullptr (ld_t >= M, multiple of 8)
   int64_t ld_t;
+  // what rounding to 16 bits left over, in 16 bits: two_rows puts it in columns
+  // [R, 2R) of out_rows, out_t_lo is shaped as out_t
+  bool two_rows = false;
+  void* out_t_lo = nullptr;
   // fp32 path: with split_out, out_rows row m = [part_0 | part_1 | part_2]
   // (R columns each) and out_t[j, s*M + m] = part_s, where part_s is the bf16
   // hi or lo part of the value as bit s of split_pattern says (0 = hi).
@@ -190,6 +194,7 @@ int launch_rank(const RankArgs& a, cudaStream_t stream);
 struct WgradArgs {
   const void* big;  // [M, P] stride ldb
   const void* st;   // [R, ld_st] (rows >= r are zero; ld_st >= M, multiple of 8)
+  const void* st_lo = nullptr;  // a second part to add to st (both problems, or neither)
   int64_t ld_st;
   int64_t M, P, r, R, ldb;
   float* out;
@@ -291,9 +296,10 @@ int launch_embed_da_f32(const int32_t* idx, const float* b, const float* dy, flo
 
 // ------------------------------------------------------------ dropout --------
 struct DropoutKey;  // philox.cuh
-// out = dropout(x) over n elements in a row (out may be x).
+// out = dropout(x) over n elements in a row (out may be x); without `scaled` the kept
+// elements are as they were.
 int launch_dropout(const void* x, void* out, int64_t n, int dtype, const DropoutKey& key,
-                   cudaStream_t s);
+                   bool scaled, cudaStream_t s);
 
 // ---------------------------------------------------------- elementwise ------
 int launch_transpose_pad(const void* b, int64_t N, int64_t r, int64_t ldb, void* bt, int64_t R,

@@ -38,7 +38,7 @@ __device__ __forceinline__ uint4 philox4x32_10(uint64_t key, uint64_t block, uin
 }
 
 // Multiplies the 8 elements of a block (elements 8 block .. 8 block + 7 of the
-// tensor in row-major order) by 0 or the scale; a dropped element is 0 whatever it
+// tensor in row-major order) by 0 or `scale`; a dropped element is 0 whatever it
 // was.  Element e takes half-word e % 8 of the block's words, the low half first.
 __device__ __forceinline__ void dropout8(float (&v)[8], const uint4& words, uint32_t threshold,
                                          float scale) {

@@ -66,13 +66,17 @@ __device__ __forceinline__ SplitWork split_work(int tile, int split, int splits,
 // Common pipeline: produces TMEM acc [128 x R] = sum over k-blocks of
 // A-tile (128 rows) x B-tile (R rows).  kAMN selects an MN-major A operand built
 // from two [64 x 64] boxes (weight gradient) instead of a K-major [128 x 64] box.
-template <int R, bool kAMN, bool kBF16>
+// kTwo: the B operand is the sum of two 16-bit parts, tm_b and tm_b_lo, whose tiles
+// share a stage; the A tile is read once for both.
+template <int R, bool kAMN, bool kBF16, bool kTwo = false>
 __device__ __forceinline__ void run_pipeline(uint8_t* smem, uint64_t* full_bar, uint64_t* empty_bar,
                                              uint64_t* done_bar, uint32_t tmem_acc,
                                              const CUtensorMap* tm_a, const CUtensorMap* tm_b,
                                              int a_row0, int kb_begin, int kb_end,
-                                             uint32_t* status) {
-  constexpr int S = num_stages(R);
+                                             uint32_t* status,
+                                             const CUtensorMap* tm_b_lo = nullptr) {
+  constexpr int RB = kTwo ? 2 * R : R;  // rows of B in a stage
+  constexpr int S = num_stages(RB);
   const uint32_t warp = warp_id();
   if (warp == 0) {
     if (elect_one()) {
@@ -82,9 +86,9 @@ __device__ __forceinline__ void run_pipeline(uint8_t* smem, uint64_t* full_bar, 
       for (int s = 0; s < S; ++s) armed[s] = false, armed_parity[s] = 0;
       for (int kb = kb_begin; kb < kb_end; ++kb) {
         if (!mbar_wait(&empty_bar[stage], phase ^ 1u, status, kDevTimeoutEmpty)) break;
-        uint8_t* sa = smem + stage * stage_bytes(R);
+        uint8_t* sa = smem + stage * stage_bytes(RB);
         uint8_t* sb = sa + kBigTileBytes;
-        mbar_arrive_expect_tx(&full_bar[stage], stage_bytes(R));
+        mbar_arrive_expect_tx(&full_bar[stage], stage_bytes(RB));
         armed[stage] = true;
         armed_parity[stage] = phase;
         const int k0 = kb * kBK;
@@ -95,6 +99,8 @@ __device__ __forceinline__ void run_pipeline(uint8_t* smem, uint64_t* full_bar, 
           tma_load_2d(sa, tm_a, &full_bar[stage], k0, a_row0);
         }
         tma_load_2d(sb, tm_b, &full_bar[stage], k0, 0);
+        if constexpr (kTwo)
+          tma_load_2d(sb + small_tile_bytes(R), tm_b_lo, &full_bar[stage], k0, 0);
         if (++stage == S) stage = 0, phase ^= 1u;
       }
       for (int s = 0; s < S; ++s)
@@ -111,7 +117,7 @@ __device__ __forceinline__ void run_pipeline(uint8_t* smem, uint64_t* full_bar, 
           break;
         }
         tc_fence_after();
-        const uint32_t sa = smem_u32(smem + stage * stage_bytes(R));
+        const uint32_t sa = smem_u32(smem + stage * stage_bytes(RB));
         const uint32_t sb = sa + kBigTileBytes;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -122,6 +128,8 @@ __device__ __forceinline__ void run_pipeline(uint8_t* smem, uint64_t* full_bar, 
             ad = desc_kmajor_sw128(sa, k);
           umma_f16(tmem_acc, ad, desc_kmajor_sw128(sb, k), idesc,
                    (kb != kb_begin || k != 0) ? 1u : 0u);
+          if constexpr (kTwo)
+            umma_f16(tmem_acc, ad, desc_kmajor_sw128(sb + small_tile_bytes(R), k), idesc, 1u);
         }
         umma_commit(&empty_bar[stage]);
         if (++stage == S) stage = 0, phase ^= 1u;
@@ -141,6 +149,8 @@ struct RankParams {
   long long ld_rows;
   void* out_t;
   long long ld_t;
+  void* out_t_lo;
+  int two_rows;
   int split_out;
   uint32_t split_pattern;
   uint32_t* status;
@@ -238,12 +248,27 @@ __global__ void __launch_bounds__(kThreads, 2)
       dst[static_cast<long long>(j) * p.ld_t] = static_cast<T>(v0);
       dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(v1);
     }
+    if (p.two_rows != 0 || p.out_t_lo != nullptr) {
+      // what rounding left over; of an infinite value nothing
+      float l0 = v0 - static_cast<float>(static_cast<T>(v0));
+      float l1 = v1 - static_cast<float>(static_cast<T>(v1));
+      if (!isfinite(l0)) l0 = 0.f;
+      if (!isfinite(l1)) l1 = 0.f;
+      if (p.two_rows != 0)
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out_rows) + row * p.ld_rows + R + j) =
+            pack2<T>(l0, l1);
+      if (p.out_t_lo != nullptr) {
+        T* dst = reinterpret_cast<T*>(p.out_t_lo) + row;
+        dst[static_cast<long long>(j) * p.ld_t] = static_cast<T>(l0);
+        dst[static_cast<long long>(j + 1) * p.ld_t] = static_cast<T>(l1);
+      }
+    }
   };
   cluster_reduce<R>(tmem + ((static_cast<uint32_t>(row_local & ~31)) << 16), have,
                     reinterpret_cast<float*>(smem), p.splits, crank, row_local, epi, emit);
   // zero padding of the row buffer past the computed columns (cluster rank 0)
   if (live && crank == 0 && p.out_rows != nullptr) {
-    const long long from = p.split_out ? 3 * R : R;
+    const long long from = p.split_out ? 3 * R : p.two_rows ? 2 * R : R;
     if (p.split_out) {
       __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.out_rows) + row * p.ld_rows;
       for (long long j = from; j < p.ld_rows; j += 8)
@@ -283,15 +308,17 @@ struct WgradParams {
 
 // 1-D grid, cluster (splits, 1, 1): CTA b of problem q works on tile
 // b / splits over token range b % splits (= its cluster rank).
-template <int R, bool kBF16>
+template <int R, bool kBF16, bool kTwo>
 __global__ void __launch_bounds__(kThreads, 2)
     wgrad_kernel(const __grid_constant__ CUtensorMap tm_big0, const __grid_constant__ CUtensorMap tm_st0,
                  const __grid_constant__ CUtensorMap tm_big1, const __grid_constant__ CUtensorMap tm_st1,
+                 const __grid_constant__ CUtensorMap tm_lo0, const __grid_constant__ CUtensorMap tm_lo1,
                  const WgradParams p) {
-  constexpr int S = num_stages(R);
+  constexpr int RB = kTwo ? 2 * R : R;
+  constexpr int S = num_stages(RB);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(R));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + S * stage_bytes(RB));
   uint64_t* empty_bar = full_bar + S;
   uint64_t* done_bar = empty_bar + S;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done_bar + 1);
@@ -321,9 +348,10 @@ __global__ void __launch_bounds__(kThreads, 2)
   const SplitWork w = split_work(tile, static_cast<int>(crank), p.splits, q.num_kb);
   const bool has_work = w.kb_begin < w.kb_end;
   if (has_work) {
-    run_pipeline<R, true, kBF16>(smem, full_bar, empty_bar, done_bar, tmem,
-                                 which ? &tm_big1 : &tm_big0, which ? &tm_st1 : &tm_st0,
-                                 tile * 128, w.kb_begin, w.kb_end, p.status);
+    run_pipeline<R, true, kBF16, kTwo>(smem, full_bar, empty_bar, done_bar, tmem,
+                                       which ? &tm_big1 : &tm_big0, which ? &tm_st1 : &tm_st0,
+                                       tile * 128, w.kb_begin, w.kb_end, p.status,
+                                       which ? &tm_lo1 : &tm_lo0);
   }
   // a programmatic dependent (the dx GEMM, which reads none of this kernel's
   // outputs) may start on the SMs this grid frees during its reduction tail
@@ -435,6 +463,8 @@ int launch_rank_typed(const RankArgs& a, cudaStream_t stream) {
   p.ld_rows = a.ld_rows;
   p.out_t = a.out_t;
   p.ld_t = a.ld_t;
+  p.out_t_lo = a.out_t_lo;
+  p.two_rows = a.two_rows && a.out_rows != nullptr ? 1 : 0;
   p.split_out = a.split_out ? 1 : 0;
   p.split_pattern = a.split_pattern;
   p.status = device_status_ptr();
@@ -454,9 +484,10 @@ int launch_rank_typed(const RankArgs& a, cudaStream_t stream) {
   return MLORA_OK;
 }
 
-template <int R, bool kBF16>
-int launch_wgrad_typed(const WgradArgs* probs, int n, cudaStream_t stream) {
-  CUtensorMap tb[2], ts[2];
+template <int R, bool kBF16, bool kTwo>
+int launch_wgrad_parts(const WgradArgs* probs, int n, cudaStream_t stream) {
+  CUtensorMap tb[2], ts[2], tl[2];
+  constexpr int RB = kTwo ? 2 * R : R;
   WgradParams p;
   p.nprobs = n;
   p.splits = probs[0].splits;
@@ -470,6 +501,9 @@ int launch_wgrad_typed(const WgradArgs* probs, int n, cudaStream_t stream) {
     const WgradArgs& a = probs[i < n ? i : 0];
     if (!make_tmap_2d_16b(&tb[i], a.big, a.P, a.M, a.ldb, 64, kBK)) return MLORA_ERR_INVALID_ARG;
     if (!make_tmap_2d_16b(&ts[i], a.st, a.M, a.R, a.ld_st, kBK, R)) return MLORA_ERR_INVALID_ARG;
+    tl[i] = ts[i];
+    if (kTwo && !make_tmap_2d_16b(&tl[i], a.st_lo, a.M, a.R, a.ld_st, kBK, R))
+      return MLORA_ERR_INVALID_ARG;
     WgradProblem& q = p.prob[i];
     q.M = a.M;
     q.P = a.P;
@@ -486,18 +520,24 @@ int launch_wgrad_typed(const WgradArgs* probs, int n, cudaStream_t stream) {
     if (i == 0) p.ctas0 = q.tiles * p.splits;
   }
   p.status = device_status_ptr();
-  auto kern = wgrad_kernel<R, kBF16>;
-  if (!set_smem_attr(kern, smem_bytes(R))) return MLORA_ERR_CUDA;
+  auto kern = wgrad_kernel<R, kBF16, kTwo>;
+  if (!set_smem_attr(kern, smem_bytes(RB))) return MLORA_ERR_CUDA;
   LaunchScope scope(kKindWgrad, stream);
-  cudaError_t e = launch_clustered(kern, dim3(static_cast<unsigned>(total)), smem_bytes(R), stream,
+  cudaError_t e = launch_clustered(kern, dim3(static_cast<unsigned>(total)), smem_bytes(RB), stream,
                                    static_cast<unsigned>(p.splits), 1u, probs[0].overlap_prev,
-                                   tb[0], ts[0], tb[1], ts[1], p);
+                                   tb[0], ts[0], tb[1], ts[1], tl[0], tl[1], p);
   if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_error(std::string("wgrad launch: ") + cudaGetErrorString(e));
     return MLORA_ERR_CUDA;
   }
   return MLORA_OK;
+}
+
+template <int R, bool kBF16>
+int launch_wgrad_typed(const WgradArgs* probs, int n, cudaStream_t stream) {
+  return probs[0].st_lo != nullptr ? launch_wgrad_parts<R, kBF16, true>(probs, n, stream)
+                                   : launch_wgrad_parts<R, kBF16, false>(probs, n, stream);
 }
 
 #define MLORA_DISPATCH_R(R_, FN, ...)                              \

@@ -901,9 +901,10 @@ def _drop_seed(seed) -> tuple[int, int | None]:
     return int(seed) & (2 ** 64 - 1), None
 
 
-def dropout(x: torch.Tensor, p: float, seed, call: int = 0) -> torch.Tensor:
+def dropout(x: torch.Tensor, p: float, seed, call: int = 0, scaled: bool = True) -> torch.Tensor:
     """x with every element dropped (0) or scaled by the counter-based mask of ``seed``
-    and ``call`` (see ``ops.dropout``); its gradient is the same call on dy."""
+    and ``call`` (see ``ops.dropout``); its gradient is the same call on dy.  Without
+    ``scaled`` the kept elements are as they were."""
     t = _drop_threshold(p)
     _need_cuda(x)
     _need_current(x)
@@ -912,7 +913,7 @@ def dropout(x: torch.Tensor, p: float, seed, call: int = 0) -> torch.Tensor:
     x = x.contiguous()
     out = torch.empty_like(x)
     if x.numel():
-        st = _lib.load().mlora_dropout(_ptr(x), _ptr(out), x.numel(), t, s, s_dev,
+        st = _lib.load().mlora_dropout(_ptr(x), _ptr(out), x.numel(), t, int(scaled), s, s_dev,
                                        int(call) & (2 ** 64 - 1), code, _stream())
         _lib.check(st, "mlora_dropout")
     return out
@@ -959,7 +960,9 @@ def lora_linear_dropout_bwd(dy2d: torch.Tensor, x2d: torch.Tensor, w0: torch.Ten
     """(dx, dA, dB) of ``lora_linear_dropout_fwd``: the LoRA products take dropout(dy), the
     base's takes dy.  The other arguments as for ``lora_linear_bwd``; ``on_grads`` is
     called between dA/dB and the dx GEMM."""
-    dz = dropout(dy2d, p, seed, call)
+    dz = dropout(dy2d, p, seed, call, scaled=False)  # exact: alpha takes the factor
+    t = _drop_threshold(p)
+    alpha = alpha * (65536 / (65536 - t) if t < 65536 else 0.0)
     dy2d = dy2d.contiguous()
     M, K = x2d.shape
     if not need_dx or M == 0:

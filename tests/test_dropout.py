@@ -67,7 +67,7 @@ def test_refusals():
     good = dict(x=4096, out=4096, n=8, t=100, seed=1, dev=None, call=0, dtype=0)
     for kw in ({"n": 0}, {"t": -1}, {"t": 65537}, {"dtype": 3}, {"x": None}, {"out": 4097}, {"dev": 4}):
         v = {**good, **kw}
-        assert lib.mlora_dropout(v["x"], v["out"], v["n"], v["t"], v["seed"], v["dev"], v["call"],
+        assert lib.mlora_dropout(v["x"], v["out"], v["n"], v["t"], 1, v["seed"], v["dev"], v["call"],
                                  v["dtype"], None) < 0, kw
     p = 1 << 20
 
