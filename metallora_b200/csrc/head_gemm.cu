@@ -5,8 +5,8 @@
 //   dx      D[m, k] = sum_v g[m, v] W[v, k]   (+ U[m, :] . A[:, k])    W MN-major
 //   dW      D[v, k] = sum_m g[m, v] x[m, k]                            both MN-major
 //
-// The logits never leave the chip as such.  The epilogue takes, of each row's 256 in a
-// tile, the largest m_t and s_t = sum exp(l - m_t), and where a gradient is wanted
+// The logits never leave the chip as such.  The epilogue takes, of each row's 128 in half
+// a tile, the largest m_t and s_t = sum exp(l - m_t), and where a gradient is wanted
 // writes exp(l - m_t) as an fp16 value: 11 bits of a number in (0, 1], so that only
 // the rounding of g to its 16 bits shows, and half of what fp32 logits would move.
 // The label's own logit is left out (as -inf): it comes in 32 bits from the pass that
@@ -46,7 +46,7 @@ constexpr int kStages = 6;
 constexpr uint32_t kOpBytes = kHalf * kBK * 2;      // 16 KB
 constexpr uint32_t kStageBytes = 2 * kOpBytes;
 constexpr uint32_t kMNBoxBytes = 64 * kBK * 2;      // one MN-major TMA box (8 KB)
-constexpr int kEpiWarps = 4;
+constexpr int kEpiWarps = 8;  // two for each quarter of the lanes: 128 columns each
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kCutPerK = 1.0e-9f;
@@ -66,7 +66,7 @@ struct HeadGemmParams {
   const int32_t* label;  // of row m
   __half* e;             // exp(l - m_t) * 2^15, rows ldd apart, or nullptr
   float uncut;           // what a logit is multiplied by
-  float2* stats;         // (m_t, 2^15 s_t) of tile column t at [t * stats_ld + m]
+  float2* stats;         // (m_t, 2^15 s_t) of the t-th 128 entries at [t * stats_ld + m]
   long long stats_ld;
   uint32_t* status;
 };
@@ -115,21 +115,21 @@ __device__ __forceinline__ Unit unit_at(const HeadGemmParams& p, const Shape& s,
   return t;
 }
 
-// This thread's row of the accumulator into D, 32 bytes at a time.
+// This thread's half row of the accumulator (128 columns from n0) into D, 32 bytes at a
+// time.
 __device__ __forceinline__ void store_row_f32(const HeadGemmParams& p, const Shape& s,
-                                              const Unit& t, int m, uint32_t taddr) {
-  float* row = p.d + t.split * p.split_stride + static_cast<long long>(m) * p.ldd +
-               static_cast<long long>(t.tn) * kTile;
+                                              const Unit& t, int m, int n0, uint32_t taddr) {
+  float* row = p.d + t.split * p.split_stride + static_cast<long long>(m) * p.ldd + n0;
 #pragma unroll 1
-  for (int c = 0; c < kTile / 32; ++c) {
+  for (int c = 0; c < kHalf; c += 32) {
     uint32_t r[32];
-    tmem_ld_32x32b_x32(taddr + c * 32, r);
+    tmem_ld_32x32b_x32(taddr + c, r);
     tmem_ld_wait();
     if (m >= s.M) continue;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      if (t.tn * kTile + c * 32 + q * 8 >= p.N) continue;
-      float* dst = row + c * 32 + q * 8;
+      if (n0 + c + q * 8 >= p.N) continue;
+      float* dst = row + c + q * 8;
       uint32_t v[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) v[i] = t.total > 0 ? r[q * 8 + i] : 0u;
@@ -154,64 +154,60 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
-// This thread's row of a tile of logits: largest, sum of exponentials, exponentials.
-// Two passes over the accumulator in TMEM; with K = 4096 it takes an eighth of the
-// main loop beside it.
-__device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape& s, const Unit& t,
-                                            int m, uint32_t taddr) {
-  const int n_base = t.tn * kTile;
+// This thread's half row of a tile of logits (128 entries from n0), all of it in
+// registers: largest, exponentials, their sum.  `release` hands the accumulator back
+// before the arithmetic, so that the main loop two tiles on does not wait for it.
+template <typename Release>
+__device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape& s, int m, int n0,
+                                            uint32_t taddr, Release&& release) {
+  if (n0 >= p.N) {  // past the vocabulary: no statistics, nothing to write
+    release();
+    return;
+  }
+  uint32_t r[4][32];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(taddr + c * 32, r[c]);
   const bool live = m < s.M;
-  const int y = live ? p.label[m] - n_base : -1;
-  const int width = p.N - n_base;  // columns of the vocabulary in this tile
-  float top = -INFINITY;
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    uint32_t r[32];
-    tmem_ld_32x32b_x32(taddr + c, r);
-    tmem_ld_wait();
-    if (c + 32 > width || __any_sync(0xffffffffu, static_cast<uint32_t>(y - c) < 32u)) {
+  const int y = live ? p.label[m] - n0 : -1;
+  const int width = p.N - n0;  // of these columns, those in the vocabulary
+  tmem_ld_wait();
+  release();
+  if (width < kHalf || __any_sync(0xffffffffu, static_cast<uint32_t>(y) < static_cast<uint32_t>(kHalf))) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (c + i >= width || c + i == y) r[i] = __float_as_uint(-INFINITY);
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+        if (c * 32 + i >= width || c * 32 + i == y) r[c][i] = __float_as_uint(-INFINITY);
   }
+  float t0 = -INFINITY, t1 = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      t0 = fmaxf(t0, __uint_as_float(r[c][i]));
+      t1 = fmaxf(t1, __uint_as_float(r[c][i + 1]));
+    }
+  const float top = fmaxf(t0, t1);
   const float ref = top == -INFINITY ? 0.f : top;
   const float log2e = 1.4426950408889634f * p.uncut;
   float sum0 = 0.f, sum1 = 0.f;
-  __half* row = p.e + static_cast<long long>(m) * p.ldd + n_base;
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    uint32_t r[32];
-    tmem_ld_32x32b_x32(taddr + c, r);
-    tmem_ld_wait();
-    if (c + 32 > width || __any_sync(0xffffffffu, static_cast<uint32_t>(y - c) < 32u)) {
+  __half* row = p.e + static_cast<long long>(m) * p.ldd + n0;
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c + i >= width || c + i == y) r[i] = __float_as_uint(-INFINITY);
-    }
-    uint32_t e[16];
+  for (int c = 0; c < 8; ++c) {
+    uint32_t v[8];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
+    for (int i = 0; i < 8; ++i) {
       // the difference first: exact near the top, where it counts
-      const float a = ex2(fmaf(__uint_as_float(r[2 * i]) - ref, log2e, 15.f));
-      const float b = ex2(fmaf(__uint_as_float(r[2 * i + 1]) - ref, log2e, 15.f));
+      const float a = ex2(fmaf(__uint_as_float(r[c / 2][16 * (c & 1) + 2 * i]) - ref, log2e, 15.f));
+      const float b =
+          ex2(fmaf(__uint_as_float(r[c / 2][16 * (c & 1) + 2 * i + 1]) - ref, log2e, 15.f));
       sum0 += a;
       sum1 += b;
-      e[i] = pack2<__half>(a, b);
+      v[i] = pack2<__half>(a, b);
     }
-    if (live && p.e != nullptr) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (n_base + c + 16 * h < p.ldd) {
-          const uint32_t v[8] = {e[8 * h],     e[8 * h + 1], e[8 * h + 2], e[8 * h + 3],
-                                 e[8 * h + 4], e[8 * h + 5], e[8 * h + 6], e[8 * h + 7]};
-          st_global_32b(row + c + 16 * h, v);
-        }
-    }
+    if (live && p.e != nullptr && n0 + c * 16 < p.ldd) st_global_32b(row + c * 16, v);
   }
-  if (live) p.stats[t.tn * p.stats_ld + m] = make_float2(top * p.uncut, sum0 + sum1);
+  if (live) p.stats[n0 / kHalf * p.stats_ld + m] = make_float2(top * p.uncut, sum0 + sum1);
 }
 
 template <bool kXMN, bool kWMN, bool kBF16>
@@ -371,6 +367,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {
     // ----------------------------------------------------------- epilogue --
     const uint32_t quarter = warp & 3u;  // TMEM lanes [32*quarter, 32*quarter+32)
+    const uint32_t half = (warp - 2u) >> 2;  // columns [128*half, 128*half+128)
     const uint32_t lead_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
     int local = 0;
     for (int u = pair; u < shape.units; u += num_pairs, ++local) {
@@ -380,14 +377,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
       tc_fence_after();
       const int m = t.tm * kTile + static_cast<int>(crank * kHalf + quarter * 32 + lane);
-      const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile;
-      if constexpr (!kWMN)
-        softmax_row(p, shape, t, m, taddr);
-      else
-        store_row_f32(p, shape, t, m, taddr);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(lead_acc_empty + buf * 8u);
+      const int n0 = t.tn * kTile + static_cast<int>(half) * kHalf;
+      const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile + half * kHalf;
+      // the arrival orders no memory: only the TMEM loads, complete by then, came before
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster_relaxed(lead_acc_empty + buf * 8u);
+      };
+      if constexpr (!kWMN) {
+        softmax_row(p, shape, m, n0, taddr, release);
+      } else {
+        store_row_f32(p, shape, t, m, n0, taddr);
+        release();
+      }
     }
   }
 

@@ -477,7 +477,7 @@ int check_dims(const Dims& d, int dtype) {
     return fail(MLORA_ERR_UNSUPPORTED, "K and r must be multiples of 8 (16-byte rows)");
   if (d.lora() && d.V % 8)
     return fail(MLORA_ERR_UNSUPPORTED, "a LoRA head needs V % 8 == 0 (16-byte rows of B^T)");
-  if (d.M > (int64_t{1} << 31) - 256 || d.K > (1 << 24) || d.V > (1 << 21))
+  if (d.M > (int64_t{1} << 31) - 256 || d.K > (1 << 24) || d.V > (1 << 20))
     return fail(MLORA_ERR_UNSUPPORTED, "shape too large");
   return MLORA_OK;
 }

@@ -261,11 +261,11 @@ struct HeadGemmArgs {
   const int32_t* label = nullptr;  // kLogits: of row m
   void* e = nullptr;         // kLogits: [M, ldd] fp16 exp(l - tile's largest) * 2^15 or nullptr;
                              // ldd a multiple of 16, at least N
-  void* stats = nullptr;     // kLogits: float2 [ceil(N / 256), stats_ld]
+  void* stats = nullptr;     // kLogits: float2 [ceil(N / 128), stats_ld]
   int64_t stats_ld = 0;
   Elt elt = Elt::kBF16;
 };
-constexpr int kHeadTile = 256;  // columns of a tile of logits
+constexpr int kHeadTile = 128;  // entries that share a largest logit
 int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s);
 int head_gemm_pairs();  // CTA pairs that are resident at once
 
