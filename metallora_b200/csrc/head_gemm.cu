@@ -6,9 +6,17 @@
 //   dW      D[v, k] = sum_m g[m, v] x[m, k]                            both MN-major
 //
 // The logits never leave the chip as such.  The epilogue takes, of each row's 128 in half
-// a tile, the largest m_t and s_t = sum exp(l - m_t), and where a gradient is wanted
-// writes exp(l - m_t) as an fp16 value: 11 bits of a number in (0, 1], so that only
-// the rounding of g to its 16 bits shows, and half of what fp32 logits would move.
+// a tile, a reference n_t and s_t = sum exp(l) 2^-n_t, and where a gradient is wanted
+// writes the exponentials exp(l) 2^-n_t in 16 bits.  Two forms:
+//   * bf16 hidden states behind a frozen head: n_t is one whole number for the whole row,
+//     the label's logit in units of log 2.  bf16 has the range for it, and a factor of
+//     a row of g can be left to the gradient of x: the exponentials are the operand of
+//     dx as they are.  A half row whose sum passes 2^90 (logits 60 above the label's)
+//     takes a reference of its own; a power of two apart, so that bringing the row to
+//     one reference rounds nothing;
+//   * else n_t is the half row's largest logit, and the exponentials are fp16 values:
+//     11 bits of a number in (0, 1], so that of g, which a pass over them makes, only
+//     the rounding to its 16 bits shows.
 // The label's own logit is left out (as -inf): it comes in 32 bits from the pass that
 // gathers x, since the tensor cores' accumulation rounds toward zero at each of its
 // K / 16 steps, which a loss shows as it is.  Of the other logits that cut is given back
@@ -50,6 +58,8 @@ constexpr int kEpiWarps = 8;  // two for each quarter of the lanes: 128 columns 
 constexpr int kThreads = 64 + 32 * kEpiWarps;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kCutPerK = 1.0e-9f;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRowLimit = 1.2379400392853803e27f;  // 2^90
 constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + 256;
 
 struct HeadGemmParams {
@@ -64,10 +74,11 @@ struct HeadGemmParams {
   int accumulate;
   // logits
   const int32_t* label;  // of row m
-  __half* e;             // exp(l - m_t) * 2^15, rows ldd apart, or nullptr
+  const float* ref;      // of row m: n_t (first form)
+  uint16_t* e;           // the exponentials (second form: times 2^15), rows ldd apart, or nullptr
   float uncut;           // what a logit is multiplied by
-  float2* stats;         // (m_t, 2^15 s_t) of the t-th 128 entries at [t * stats_ld + m]
-  long long stats_ld;
+  float2* stats;         // (n_t, s_t), second form (m_t, 2^15 s_t), of the t-th 128 entries at
+  long long stats_ld;    // [m * stats_ld + t]
   uint32_t* status;
 };
 
@@ -154,8 +165,88 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
-// This thread's half row of a tile of logits (128 entries from n0), all of it in
-// registers: largest, exponentials, their sum.  `release` hands the accumulator back
+// Logits past the vocabulary, and the label's, count as -inf (`any`: there are some
+// among the warp's).
+__device__ __forceinline__ void mask_logits(uint32_t (&r)[32], int c, int width, int y, bool any) {
+  if (!any) return;
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (c + i >= width || c + i == y) r[i] = __float_as_uint(-INFINITY);
+}
+
+// First form: this thread's half row of a tile of logits (128 entries from n0).  One
+// pass with the row's reference; the largest logit is only looked for where it fails.
+template <typename Release>
+__device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const Shape& s, int m,
+                                                int n0, uint32_t taddr, Release&& release) {
+  if (n0 >= p.N) {  // past the vocabulary: no statistics, nothing to write
+    release();
+    return;
+  }
+  const bool live = m < s.M;
+  const int y = live ? p.label[m] - n0 : -1;
+  float n = live ? p.ref[m] : 0.f;
+  const int width = p.N - n0;  // of these columns, those in the vocabulary
+  const bool any = width < kHalf || __any_sync(0xffffffffu, static_cast<uint32_t>(y) <
+                                                                static_cast<uint32_t>(kHalf));
+  const float log2e = kLog2e * p.uncut;
+  uint32_t v[kHalf / 2];
+  float sum = 0.f;
+  auto exponentials = [&] {
+    float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t r[2][32];
+      tmem_ld_32x32b_x32(taddr + h * 64, r[0]);
+      tmem_ld_32x32b_x32(taddr + h * 64 + 32, r[1]);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mask_logits(r[c], h * 64 + c * 32, width, y, any);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float a = ex2(fmaf(__uint_as_float(r[c][2 * i]), log2e, -n));
+          const float b = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), log2e, -n));
+          s0 += a;
+          s1 += b;
+          v[h * 32 + c * 16 + i] = pack2<__nv_bfloat16>(a, b);
+        }
+      }
+    }
+    sum = s0 + s1;
+  };
+  exponentials();
+  const bool over = live && !(sum <= kRowLimit);
+  if (__any_sync(0xffffffffu, over)) {
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < kHalf; c += 32) {
+      uint32_t r[32];
+      tmem_ld_32x32b_x32(taddr + c, r);
+      tmem_ld_wait();
+      mask_logits(r, c, width, y, any);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = fmaxf(top, __uint_as_float(r[i]));
+    }
+    if (over) n = fmaxf(n, ceilf(top * log2e));  // infinite: the sum becomes NaN
+    exponentials();
+  }
+  release();
+  if (!live) return;
+  if (p.e != nullptr) {
+    uint16_t* row = p.e + static_cast<long long>(m) * p.ldd + n0;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (n0 + c * 16 < p.ldd) {
+        const uint32_t q[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
+                               v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
+        st_global_32b(row + c * 16, q);
+      }
+  }
+  p.stats[static_cast<long long>(m) * p.stats_ld + n0 / kHalf] = make_float2(n, sum);
+}
+
+// Second form: all of the half row in registers: largest, exponentials, their sum.  `release` hands the accumulator back
 // before the arithmetic, so that the main loop two tiles on does not wait for it.
 template <typename Release>
 __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape& s, int m, int n0,
@@ -172,13 +263,10 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
   const int width = p.N - n0;  // of these columns, those in the vocabulary
   tmem_ld_wait();
   release();
-  if (width < kHalf || __any_sync(0xffffffffu, static_cast<uint32_t>(y) < static_cast<uint32_t>(kHalf))) {
+  const bool any = width < kHalf || __any_sync(0xffffffffu, static_cast<uint32_t>(y) <
+                                                                static_cast<uint32_t>(kHalf));
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c * 32 + i >= width || c * 32 + i == y) r[c][i] = __float_as_uint(-INFINITY);
-  }
+  for (int c = 0; c < 4; ++c) mask_logits(r[c], c * 32, width, y, any);
   float t0 = -INFINITY, t1 = -INFINITY;
 #pragma unroll
   for (int c = 0; c < 4; ++c)
@@ -189,9 +277,9 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
     }
   const float top = fmaxf(t0, t1);
   const float ref = top == -INFINITY ? 0.f : top;
-  const float log2e = 1.4426950408889634f * p.uncut;
+  const float log2e = kLog2e * p.uncut;
   float sum0 = 0.f, sum1 = 0.f;
-  __half* row = p.e + static_cast<long long>(m) * p.ldd + n0;
+  uint16_t* row = p.e + static_cast<long long>(m) * p.ldd + n0;
 #pragma unroll
   for (int c = 0; c < 8; ++c) {
     uint32_t v[8];
@@ -207,10 +295,12 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
     }
     if (live && p.e != nullptr && n0 + c * 16 < p.ldd) st_global_32b(row + c * 16, v);
   }
-  if (live) p.stats[n0 / kHalf * p.stats_ld + m] = make_float2(top * p.uncut, sum0 + sum1);
+  if (live)
+    p.stats[static_cast<long long>(m) * p.stats_ld + n0 / kHalf] =
+        make_float2(top * p.uncut, sum0 + sum1);
 }
 
-template <bool kXMN, bool kWMN, bool kBF16>
+template <bool kXMN, bool kWMN, bool kBF16, bool kRef>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_w,
@@ -386,7 +476,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_cluster_relaxed(lead_acc_empty + buf * 8u);
       };
       if constexpr (!kWMN) {
-        softmax_row(p, shape, m, n0, taddr, release);
+        if constexpr (kRef)
+          softmax_row_ref(p, shape, m, n0, taddr, release);
+        else
+          softmax_row(p, shape, m, n0, taddr, release);
       } else {
         store_row_f32(p, shape, t, m, n0, taddr);
         release();
@@ -410,7 +503,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-template <bool kXMN, bool kWMN, bool kBF16>
+template <bool kXMN, bool kWMN, bool kBF16, bool kRef>
 int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   CUtensorMap tx, tw, tx2, tw2;
   if (kXMN ? !make_tmap_2d_16b(&tx, a.x, a.M, a.K, a.ldx, 64, kBK)
@@ -446,13 +539,14 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   p.split_stride = a.split_stride;
   p.accumulate = a.accumulate ? 1 : 0;
   p.label = a.label;
-  p.e = static_cast<__half*>(a.e);
+  p.ref = a.ref;
+  p.e = static_cast<uint16_t*>(a.e);
   p.stats = static_cast<float2*>(a.stats);
   p.stats_ld = a.stats_ld;
   p.uncut = 1.f + kCutPerK * static_cast<float>(a.K);
   p.status = device_status_ptr();
 
-  auto kern = head_gemm_kernel<kXMN, kWMN, kBF16>;
+  auto kern = head_gemm_kernel<kXMN, kWMN, kBF16, kRef>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), kSmemBytes, attr_set)) return rc;
   const int64_t units = int64_t{tiles_m} * p.tiles_n * p.splits;
@@ -474,7 +568,7 @@ int head_gemm_pairs() {
   if (n > 0) return n;
   // clusters that can be resident at once (GPCs may leave an SM unpaired)
   const int pairs = num_sms() / 2;
-  auto kern = head_gemm_kernel<false, false, true>;
+  auto kern = head_gemm_kernel<false, false, true, false>;
   static std::atomic<bool> attr_set[64];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
@@ -494,11 +588,15 @@ int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s) {
   const bool bf16 = a.elt == Elt::kBF16;
   switch (a.product) {
     case HeadProduct::kLogits:
-      return bf16 ? launch_typed<false, false, true>(a, s) : launch_typed<false, false, false>(a, s);
+      if (a.ref != nullptr) return launch_typed<false, false, true, true>(a, s);
+      return bf16 ? launch_typed<false, false, true, false>(a, s)
+                  : launch_typed<false, false, false, false>(a, s);
     case HeadProduct::kDx:
-      return bf16 ? launch_typed<false, true, true>(a, s) : launch_typed<false, true, false>(a, s);
+      return bf16 ? launch_typed<false, true, true, false>(a, s)
+                  : launch_typed<false, true, false, false>(a, s);
     case HeadProduct::kDw:
-      return bf16 ? launch_typed<true, true, true>(a, s) : launch_typed<true, true, false>(a, s);
+      return bf16 ? launch_typed<true, true, true, false>(a, s)
+                  : launch_typed<true, true, false, false>(a, s);
   }
   return MLORA_ERR_INVALID_ARG;
 }

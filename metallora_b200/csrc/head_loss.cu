@@ -113,11 +113,12 @@ __global__ void __launch_bounds__(kScanThreads)
 
 // xc[i] = x[row_of[i]], zeros past the last counted token (as many as a reduction
 // over tokens reads; all of them for the LoRA products, which run over every row);
-// and target[i] = the label's logit but for a LoRA term, in 32 bits.
+// and target[i] = the label's logit but for a LoRA term, in 32 bits; ref[i] = it in whole
+// units of log 2.
 template <typename T>
 __global__ void __launch_bounds__(128)
     head_gather_kernel(const uint4* x, const uint4* w, const int32_t* row_of, const int32_t* label,
-                       const HeadCount* count, int64_t K8, int zero_all, uint4* xc, float* target) {
+                       const HeadCount* count, int64_t K8, int zero_all, uint4* xc, float* target, float* ref) {
   __shared__ float part[4];
   const int64_t i = blockIdx.x;
   const int32_t row = row_of[i];
@@ -142,7 +143,12 @@ __global__ void __launch_bounds__(128)
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
   __syncthreads();
-  if (threadIdx.x == 0) target[i] = part[0] + part[1] + (part[2] + part[3]);
+  if (threadIdx.x == 0) {
+    const float t = part[0] + part[1] + (part[2] + part[3]);
+    target[i] = t;
+    // in units of log 2, within what leaves room above and below; 0 for no number
+    if (ref != nullptr) ref[i] = fabsf(t) < INFINITY ? rintf(t * 1.4426950408889634f) : 0.f;
+  }
 }
 
 // W2 of the logits: [B 0 | B 0], R columns each, for the two parts of s x A^T.
@@ -165,18 +171,93 @@ __device__ __forceinline__ void join_max_sum(float& m, float& s, float m2, float
   m = top;
 }
 
-// One CTA per counted token of the piece: its loss, and its row of g in place of the
-// exponentials, e[v] -> g[v] = 2^-15 e[v] exp(m_t - lse).  With the sum S exp(m) over
+// The loss of a token from gap = m - l_y and s, where s exp(m) is the sum over the other
+// entries, and u = s exp(gap): log(1 + u), by way of the larger of the two terms.
+__device__ __forceinline__ float row_loss_of(float gap, float s, float u) {
+  return gap < 0.f || s == 0.f ? log1pf(u) : gap + logf(s + expf(-gap));
+}
+
+// An infinite logit has no softmax, the label's neither.
+__device__ __forceinline__ float gap_of(float gap, float ly) { return ly == INFINITY ? NAN : gap; }
+
+// After the logits with one reference a row: one CTA per counted token of the piece.
+// Its loss; the exponentials become its row of g but for a factor row_scale (left to
+// the gradient of x) by setting the label's to -S, S the sum of the others.  Only a row
+// with more than one reference is rewritten, by powers of two.
+__global__ void __launch_bounds__(kRowThreads)
+    head_ref_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0, const HeadCount* count,
+                    const int32_t* label, const int32_t* row_of, const float* target,
+                    float* row_loss, float* nll, __nv_bfloat16* eg, float* rest, float* row_scale) {
+  __shared__ float sn[kRowThreads / 32], sl[kRowThreads / 32], ss[kRowThreads / 32];
+  const int64_t i = blockIdx.x;
+  const int64_t slot = row0 + i;
+  if (slot >= count->counted) return;
+  const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
+  const float2* st = stats + i * tiles;
+  float top = -INFINITY, low = INFINITY;
+  for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
+    const float n = st[t].x;
+    top = fmaxf(top, n);
+    low = fminf(low, n);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  if ((threadIdx.x & 31) == 0) sn[threadIdx.x >> 5] = top, sl[threadIdx.x >> 5] = low;
+  __syncthreads();
+  for (int w = 0; w < kRowThreads / 32; ++w) top = fmaxf(top, sn[w]), low = fminf(low, sl[w]);
+  float s = 0.f;
+  for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
+    const float2 q = st[t];
+    s += q.x == top ? q.y : q.y * exp2f(q.x - top);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if ((threadIdx.x & 31) == 0) ss[threadIdx.x >> 5] = s;
+  __syncthreads();
+  s = ss[0];
+  for (int w = 1; w < kRowThreads / 32; ++w) s += ss[w];
+  if (eg != nullptr && low != top) {
+    __nv_bfloat16* row = eg + i * ld;
+    for (int64_t v = threadIdx.x; v < V; v += kRowThreads) {
+      const float n = st[v / kHeadTile].x;
+      if (n != top) row[v] = __float2bfloat16_rn(__bfloat162float(row[v]) * exp2f(n - top));
+    }
+    __syncthreads();
+  }
+  if (threadIdx.x != 0) return;
+  const int32_t y = label[slot];
+  // top log 2 - l_y, log 2 in two parts (the first of 12 bits: its product is exact)
+  const float ly = target[slot];
+  const float gap = gap_of(fmaf(top, 0.693115234375f, -ly) + top * 3.19461832987e-05f, ly);
+  const float u = s * expf(gap);
+  const float loss = row_loss_of(gap, s, u);
+  nll[slot] = loss;
+  if (row_loss != nullptr) row_loss[row_of[slot]] = loss;
+  if (eg == nullptr) return;
+  // 1 / (S + exp(l_y) 2^-top)
+  row_scale[slot] = u < 1.f ? expf(gap) / (1.f + u) : 1.f / (s + expf(-gap));
+  const __nv_bfloat16 gy = __float2bfloat16_rn(-s);
+  eg[i * ld + y] = gy;
+  rest[slot] = -s - __bfloat162float(gy);
+}
+
+// After the logits with a reference for each 128: one CTA per counted token of the piece.
+// Its loss, and its row of g in place of the exponentials,
+// e[v] -> g[v] = 2^-15 e[v] exp(m_t - lse).  With the sum S exp(m) over
 // the other entries and u = S exp(m - l_y), the loss is log(1 + u) and
 // g[y] = -u / (1 + u), without cancellation for a token that is nearly certain.
 // What rounding g[y], the largest part, left over goes to `rest`, which the gradient
 // of x adds back times W[y].  Bound: HBM, 4 bytes a logit.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-    head_row_kernel(const float2* stats, int64_t stats_ld, int64_t V, int64_t ld, int64_t row0,
+    head_row_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0,
                     const HeadCount* count, const int32_t* label, const int32_t* row_of,
                     const float* target, const T* xa, const T* b, int64_t xa_ld, int r, int R,
-                    float* row_loss, float* nll, void* eg, float* rest, int zero_all) {
+                    float* row_loss, float* nll, void* eg, float* rest, float* row_scale,
+                    int zero_all) {
   extern __shared__ float factor[];  // of each tile of logits
   __shared__ float sm[kRowThreads / 32], ss[kRowThreads / 32], sx[kRowThreads / 32];
   const int64_t i = blockIdx.x;
@@ -192,7 +273,7 @@ __global__ void __launch_bounds__(kRowThreads)
   const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
   float m = -INFINITY, s = 0.f, extra = 0.f;
   for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
-    const float2 q = stats[t * stats_ld + i];
+    const float2 q = stats[i * tiles + t];
     factor[t] = q.x;
     join_max_sum(m, s, q.x, q.y * (1.f / 32768.f));
   }
@@ -215,10 +296,9 @@ __global__ void __launch_bounds__(kRowThreads)
     extra += sx[w];
   }
   const float ly = target[slot] + extra;
-  // log(exp(l_y) + S exp(m)) from the larger of the two
-  const float gap = m - ly;
+  const float gap = gap_of(m - ly, ly);
   const float u = s * expf(gap);
-  const float loss = gap < 0.f || s == 0.f ? log1pf(u) : gap + logf(s + expf(-gap));
+  const float loss = row_loss_of(gap, s, u);
   if (threadIdx.x == 0) {
     nll[slot] = loss;
     if (row_loss != nullptr) row_loss[row_of[slot]] = loss;
@@ -232,7 +312,10 @@ __global__ void __launch_bounds__(kRowThreads)
   __syncthreads();
   // -u / (1 + u), and -1 where u has no number
   const float gy = -unit * (gap < 60.f ? u / (1.f + u) : 1.f);
-  if (threadIdx.x == 0) rest[slot] = gy - static_cast<float>(static_cast<T>(gy));
+  if (threadIdx.x == 0) {
+    rest[slot] = gy - static_cast<float>(static_cast<T>(gy));
+    row_scale[slot] = 1.f / unit;
+  }
 #pragma unroll 4
   for (int64_t q = threadIdx.x; q < ld / 8; q += kRowThreads) {
     uint4 v = row[q];
@@ -272,13 +355,13 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// dx[row] = grad (sum over splits of part[split][slot] / unit + rest[slot] / unit W[y]);
+// dx[row] = grad row_scale[slot] (sum over splits of part[split][slot] + rest[slot] W[y]);
 // zeros for tokens that do not count.
 template <typename T>
 __global__ void __launch_bounds__(256)
     head_dx_kernel(const float* part, int64_t split_stride, int splits, const int32_t* slot_of,
-                   const int32_t* label, const float* rest, const T* w, const HeadCount* count,
-                   const float* grad, int per_row, int mean, int64_t K, T* dx) {
+                   const int32_t* label, const float* rest, const float* row_scale, const T* w,
+                   const HeadCount* count, const float* grad, int per_row, int mean, int64_t K, T* dx) {
   const int64_t row = blockIdx.x;
   const int64_t k = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * 8;
   if (k >= K) return;
@@ -292,7 +375,7 @@ __global__ void __launch_bounds__(256)
       v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
       v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
     }
-    const float scale = grad[per_row ? row : 0] * (mean ? count->inv : 1.f) * (1.f / grad_unit<T>());
+    const float scale = grad[per_row ? row : 0] * (mean ? count->inv : 1.f) * row_scale[slot];
     const float left = rest[slot];
     const uint4 wv = *reinterpret_cast<const uint4*>(w + static_cast<int64_t>(label[slot]) * K + k);
     const T* we = reinterpret_cast<const T*>(&wv);
@@ -401,7 +484,7 @@ int dx_splits(const Dims& d) {
 struct State {
   HeadCount* count;
   int32_t *slot_of, *label;
-  float *rest, *dx, *da, *db, *dw;
+  float *rest, *row_scale, *dx, *da, *db, *dw;
   int splits;
   int64_t bytes;
 };
@@ -414,6 +497,7 @@ State plan_state(void* base, const Dims& d) {
   s.slot_of = c.take<int32_t>(d.M);
   s.label = c.take<int32_t>(d.M);
   s.rest = c.take<float>(d.M);
+  s.row_scale = c.take<float>(d.M);
   if (d.want(MLORA_HEAD_GRAD_X)) s.dx = c.take<float>(s.splits * d.M * d.K);
   if (d.want(MLORA_HEAD_GRAD_AB)) {
     s.da = c.take<float>(d.r * d.K);
@@ -427,7 +511,7 @@ State plan_state(void* base, const Dims& d) {
 struct Work {
   int32_t* row_of;
   float* nll;
-  float* target;
+  float *target, *ref;
   void *xc, *xa_rows, *xa_t, *xa_lo, *b2, *bt, *u_rows, *u_t, *u_lo, *eg;
   float2* stats;
   int64_t piece;  // rows that go through at a time
@@ -437,14 +521,15 @@ struct Work {
 Work plan_work(void* base, const Dims& d) {
   Work w{};
   Carve c(base);
-  // pieces of two gigabytes (or 256 rows), equal up to the tile
-  const int64_t per_row = d.tiles() * 8 + (d.grads ? d.ld() * 2 : 0);
+  // pieces of two gigabytes of exponentials (or 256 rows), equal up to the tile
+  const int64_t per_row = d.grads ? d.ld() * 2 : d.tiles() * 8;
   const int64_t most = std::max<int64_t>(int64_t{2048} << 20, 256 * per_row) / per_row / 256 * 256;
   const int64_t n = (d.M + most - 1) / most;
   w.piece = std::min(d.M, round_up((d.M + n - 1) / n, 256));
   w.row_of = c.take<int32_t>(d.M);
   w.nll = c.take<float>(d.M);
   w.target = c.take<float>(d.M);
+  w.ref = c.take<float>(d.M);
   w.xc = c.take<uint16_t>(d.M * d.K);
   if (d.lora()) {
     w.xa_rows = c.take<uint16_t>(d.M * d.ld_xa());
@@ -489,6 +574,8 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
   const Elt elt = std::is_same<T, __half>::value ? Elt::kF16 : Elt::kBF16;
   const int64_t M = d.M, K = d.K, V = d.V, ld = d.ld();
   const int zero_all = d.lora() ? 1 : 0;
+  // one reference a row: g's factor per row reaches x alone
+  const bool by_row = elt == Elt::kBF16 && !d.lora() && !d.want(MLORA_HEAD_GRAD_W);
   int rc;
   {
     LaunchScope scope(kKindElementwise, s);
@@ -499,7 +586,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     LaunchScope scope(kKindElementwise, s);
     head_gather_kernel<T><<<static_cast<unsigned>(M), 128, 0, s>>>(
         static_cast<const uint4*>(x), static_cast<const uint4*>(w), ws.row_of, st.label, st.count,
-        K / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target);
+        K / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target, by_row ? ws.ref : nullptr);
   }
   if ((rc = launch_status(cudaSuccess, "linear cross entropy: gather"))) return rc;
   RankArgs ra;
@@ -548,7 +635,8 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     l.label = st.label + row0;
     l.e = ws.eg;
     l.stats = ws.stats;
-    l.stats_ld = ws.piece;
+    l.stats_ld = d.tiles();
+    l.ref = by_row ? ws.ref + row0 : nullptr;
     l.elt = elt;
     if (d.lora()) {
       l.x2 = static_cast<const T*>(ws.xa_rows) + row0 * d.ld_xa();
@@ -561,10 +649,16 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     if ((rc = launch_head_gemm(l, s))) return rc;
     {
       LaunchScope scope(kKindElementwise, s);
-      head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, d.tiles() * 4, s>>>(
-          ws.stats, ws.piece, V, ld, row0, st.count, st.label, ws.row_of, ws.target,
-          static_cast<const T*>(ws.xa_rows), static_cast<const T*>(b), d.ld_xa(),
-          static_cast<int>(d.r), static_cast<int>(d.R()), row_loss, ws.nll, ws.eg, st.rest, zero_all);
+      if (by_row)
+        head_ref_kernel<<<static_cast<unsigned>(rows), kRowThreads, 0, s>>>(
+            ws.stats, V, ld, row0, st.count, st.label, ws.row_of, ws.target, row_loss, ws.nll,
+            static_cast<__nv_bfloat16*>(ws.eg), st.rest, st.row_scale);
+      else
+        head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, d.tiles() * 4, s>>>(
+            ws.stats, V, ld, row0, st.count, st.label, ws.row_of, ws.target,
+            static_cast<const T*>(ws.xa_rows), static_cast<const T*>(b), d.ld_xa(),
+            static_cast<int>(d.r), static_cast<int>(d.R()), row_loss, ws.nll, ws.eg, st.rest,
+            st.row_scale, zero_all);
       if ((rc = launch_status(cudaSuccess, "linear cross entropy: rows"))) return rc;
     }
     if (d.lora() && d.grads) {
@@ -693,7 +787,7 @@ int backward(const State& st, const Dims& d, const void* w, const float* grad, b
   LaunchScope scope(kKindElementwise, s);
   const dim3 grid(static_cast<unsigned>(d.M), static_cast<unsigned>((d.K / 8 + 255) / 256));
   head_dx_kernel<T><<<grid, 256, 0, s>>>(st.dx, d.M * d.K, st.splits, st.slot_of, st.label, st.rest,
-                                         static_cast<const T*>(w), st.count, grad, per_row ? 1 : 0,
+                                         st.row_scale, static_cast<const T*>(w), st.count, grad, per_row ? 1 : 0,
                                          mean ? 1 : 0, d.K, static_cast<T*>(dx));
   return launch_status(cudaSuccess, "linear cross entropy: dx");
 }

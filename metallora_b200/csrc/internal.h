@@ -258,10 +258,13 @@ struct HeadGemmArgs {
   const int32_t* rows = nullptr;  // counted tokens (device); those from row0 on are meant
   int64_t row0 = 0;
   bool accumulate = false;   // D += (splits = 1)
-  const int32_t* label = nullptr;  // kLogits: of row m
-  void* e = nullptr;         // kLogits: [M, ldd] fp16 exp(l - tile's largest) * 2^15 or nullptr;
-                             // ldd a multiple of 16, at least N
-  void* stats = nullptr;     // kLogits: float2 [ceil(N / 128), stats_ld]
+  // kLogits: per row m its label and, for the form with one reference a row (bf16), ref;
+  // e: [M, ldd] exponentials in 16 bits or nullptr (ldd a multiple of 16, at least N);
+  // stats: float2 [M, stats_ld], one for every 128 entries
+  const int32_t* label = nullptr;
+  const float* ref = nullptr;
+  void* e = nullptr;
+  void* stats = nullptr;
   int64_t stats_ld = 0;
   Elt elt = Elt::kBF16;
 };
