@@ -118,13 +118,13 @@ __global__ void __launch_bounds__(kScanThreads)
 template <typename T>
 __global__ void __launch_bounds__(128)
     head_gather_kernel(const uint4* x, const uint4* w, const int32_t* row_of, const int32_t* label,
-                       const HeadCount* count, int64_t K8, int zero_all, uint4* xc, float* target, float* ref) {
+                       const HeadCount* count, int64_t K8, int64_t ld8, int zero_all, uint4* xc, float* target, float* ref) {
   __shared__ float part[4];
   const int64_t i = blockIdx.x;
   const int32_t row = row_of[i];
   if (row < 0) {
     if (zero_all || i < (count->counted + 63) / 64 * 64)
-      for (int64_t k = threadIdx.x; k < K8; k += 128) xc[i * K8 + k] = make_uint4(0, 0, 0, 0);
+      for (int64_t k = threadIdx.x; k < K8; k += 128) xc[i * ld8 + k] = make_uint4(0, 0, 0, 0);
     return;
   }
   const uint4* xr = x + static_cast<int64_t>(row) * K8;
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(128)
 #pragma unroll 4
   for (int64_t k = threadIdx.x; k < K8; k += 128) {
     const uint4 xv = xr[k], wv = wr[k];
-    xc[i * K8 + k] = xv;
+    xc[i * ld8 + k] = xv;
     const T* xe = reinterpret_cast<const T*>(&xv);
     const T* we = reinterpret_cast<const T*>(&wv);
 #pragma unroll
@@ -457,7 +457,11 @@ struct Dims {
   }
   int64_t R64() const { return round_up(R(), 64); }
   int64_t ld_xa() const { return round_up(2 * R(), 64); }  // two parts of s x A^T
-  int64_t ld() const { return round_up(V, 16); }  // of a row of e and g
+  // of a row of e and g, and of the gathered x: whole 128-byte lines, since a TMA box
+  // row that crosses a line costs two requests (x of 1032 features and the weight's
+  // rows both off the lines: 870 cycles for a 256 x 256 x 64 step that takes 512)
+  int64_t ld() const { return round_up(V, 64); }
+  int64_t ldx() const { return round_up(K, 64); }
   int64_t tiles() const { return (V + kHeadTile - 1) / kHeadTile; }
 };
 
@@ -530,7 +534,7 @@ Work plan_work(void* base, const Dims& d) {
   w.nll = c.take<float>(d.M);
   w.target = c.take<float>(d.M);
   w.ref = c.take<float>(d.M);
-  w.xc = c.take<uint16_t>(d.M * d.K);
+  w.xc = c.take<uint16_t>(d.M * d.ldx());
   if (d.lora()) {
     w.xa_rows = c.take<uint16_t>(d.M * d.ld_xa());
     w.b2 = c.take<uint16_t>(d.V * 2 * d.R());
@@ -572,7 +576,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
             float* loss, float* row_loss, const State& st, const Work& ws, const Dims& d,
             float alpha, int64_t ignore_index, bool mean, cudaStream_t s) {
   const Elt elt = std::is_same<T, __half>::value ? Elt::kF16 : Elt::kBF16;
-  const int64_t M = d.M, K = d.K, V = d.V, ld = d.ld();
+  const int64_t M = d.M, K = d.K, V = d.V, ld = d.ld(), ldx = d.ldx();
   const int zero_all = d.lora() ? 1 : 0;
   // one reference a row: g's factor per row reaches x alone
   const bool by_row = elt == Elt::kBF16 && !d.lora() && !d.want(MLORA_HEAD_GRAD_W);
@@ -586,7 +590,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     LaunchScope scope(kKindElementwise, s);
     head_gather_kernel<T><<<static_cast<unsigned>(M), 128, 0, s>>>(
         static_cast<const uint4*>(x), static_cast<const uint4*>(w), ws.row_of, st.label, st.count,
-        K / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target, by_row ? ws.ref : nullptr);
+        K / 8, ldx / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target, by_row ? ws.ref : nullptr);
   }
   if ((rc = launch_status(cudaSuccess, "linear cross entropy: gather"))) return rc;
   RankArgs ra;
@@ -597,7 +601,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     ra.K = K;
     ra.r = d.r;
     ra.R = d.R();
-    ra.ldx = K;
+    ra.ldx = ldx;
     ra.ldl = K;
     ra.scale = alpha / static_cast<float>(d.r);
     ra.out_rows = ws.xa_rows;
@@ -619,7 +623,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
   }
   for (int64_t row0 = 0; row0 < M; row0 += ws.piece) {
     const int64_t rows = std::min(ws.piece, M - row0);
-    const T* xc = static_cast<const T*>(ws.xc) + row0 * K;
+    const T* xc = static_cast<const T*>(ws.xc) + row0 * ldx;
     HeadGemmArgs l;
     l.product = HeadProduct::kLogits;
     l.x = xc;
@@ -627,7 +631,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     l.M = rows;
     l.N = V;
     l.K = K;
-    l.ldx = K;
+    l.ldx = ldx;
     l.ldw = K;
     l.ldd = ld;
     l.rows = &st.count->counted;
@@ -702,7 +706,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
         g[1].st_lo = ws.u_lo;
         g[1].ld_st = round_up(ws.piece, 8);
         g[1].P = K;
-        g[1].ldb = K;
+        g[1].ldb = ldx;
         g[1].out = st.da;
         g[1].ldo = K;
         g[1].transposed = true;
@@ -746,7 +750,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       q.N = K;
       q.K = rows;
       q.ldx = ld;
-      q.ldw = K;
+      q.ldw = ldx;
       q.ldd = K;
       q.rows = &st.count->counted;
       q.row0 = row0;
