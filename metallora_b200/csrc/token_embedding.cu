@@ -4,15 +4,19 @@
 //
 // The sums run over the tokens of an entry in token order, whatever the launch, so the
 // gradient is the same bits in every run: tokens are sorted by (entry, token) first.
-// Blocks of 2048 are sorted in shared memory, then each element finds its place among
-// all of them by binary searches in the other blocks (keys are distinct: the token is
-// part of them).  Runs of equal entries in the sorted order are summed by chunks of 32
-// tokens, so that an entry that half of the batch holds (padding) is summed by many
-// CTAs; a run that crosses a chunk's border leaves fp32 partial sums, added in chunk
-// order by a second pass.  Bound: HBM (dy once, the gradient once).
+// Up to 16384 tokens each counts the ones ahead of it, a comparison a pair; of more,
+// blocks of 2048 are sorted in shared memory and each element finds its place by binary
+// searches in the other blocks (keys are distinct: the token is part of them).  Runs of equal entries
+// in the sorted order are summed by chunks of 32 tokens, so that an entry that half of
+// the batch holds is summed by many CTAs; a run that crosses a chunk's border leaves
+// fp32 partial sums, added in chunk order by a last pass.  The rows without tokens are
+// zeroed in the same launch as the sums: every row of the gradient is written once.
+// Bound: HBM (dy once, the gradient once); for few tokens the chain of launches, which
+// start as programmatic dependents of one another.
 // An index outside the table gives a zero row, no gradient, and a code in the device
 // status word; the padding entry's gradient is zero.
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "internal.h"
@@ -26,8 +30,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kSortThreads = 1024;
 constexpr int kSortBlock = 2 * kSortThreads;
+constexpr int kJoin = 64;  // threads of a CTA that joins partial sums
+constexpr int64_t kPairTokens = 16384;
+constexpr int kRankThreads = 512;
+constexpr int kRankTokens = 64;  // of a CTA that counts pairs
 constexpr int kChunk = 32;  // sorted tokens per CTA of the gradient
-constexpr uint64_t kNoEntry = ~uint64_t{0};
+constexpr uint32_t kNone = 0xFFFFFFFFu;  // entry of a token without a gradient
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -37,35 +45,86 @@ struct Vec {
   float v[kVec<T>];
 };
 
-// N elements from p (16-byte aligned where N = kVec<T>), or fewer.
+// A thread's kVec columns of a row: side by side in 16 bytes (`vec`: the rows start on
+// 16 bytes and hold a whole number of them), or else `stride` apart, so that a warp's
+// accesses are side by side.
+struct Cols {
+  bool vec;
+  int stride;
+  int64_t d, D;  // the first one, and the row's length
+  __device__ bool any() const { return d < D; }
+  __device__ bool has(int j) const { return d + static_cast<int64_t>(j) * stride < D; }
+};
+
 template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* p, bool vec, int64_t left) {
-  Vec<T> r;
-  if (vec) {
-    const uint4 q = *reinterpret_cast<const uint4*>(p);
-    const T* e = reinterpret_cast<const T*>(&q);
+__device__ __forceinline__ Cols thread_cols(int slice, int thread, int threads, bool vec, int64_t D) {
+  const int64_t base = static_cast<int64_t>(slice) * threads * kVec<T>;
+  return {vec, threads, base + (vec ? thread * kVec<T> : thread), D};
+}
+
+// As they are, 16 bytes of them (zeros past the row's end): rows in flight stay small.
+template <typename T>
+__device__ __forceinline__ uint4 load_raw(const T* row, const Cols& c) {
+  if (c.vec) return *reinterpret_cast<const uint4*>(row + c.d);
+  uint4 q;
+  T* e = reinterpret_cast<T*>(&q);
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) r.v[i] = static_cast<float>(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) r.v[i] = i < left ? static_cast<float>(p[i]) : 0.f;
-  }
-  return r;
+  for (int i = 0; i < kVec<T>; ++i)
+    e[i] = c.has(i) ? row[c.d + static_cast<int64_t>(i) * c.stride] : static_cast<T>(0.f);
+  return q;
 }
 
 template <typename T>
-__device__ __forceinline__ void store_vec(T* p, bool vec, int64_t left, const Vec<T>& r, float scale) {
-  if (vec) {
+__device__ __forceinline__ void add_raw(Vec<T>& r, const uint4& q) {
+  const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+  for (int i = 0; i < kVec<T>; ++i) r.v[i] += static_cast<float>(e[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ void store_cols(T* row, const Cols& c, const Vec<T>& r, float scale) {
+  if (c.vec) {
     uint4 q;
     T* e = reinterpret_cast<T*>(&q);
 #pragma unroll
     for (int i = 0; i < kVec<T>; ++i) e[i] = static_cast<T>(r.v[i] * scale);
-    *reinterpret_cast<uint4*>(p) = q;
+    *reinterpret_cast<uint4*>(row + c.d) = q;
   } else {
 #pragma unroll
     for (int i = 0; i < kVec<T>; ++i)
-      if (i < left) p[i] = static_cast<T>(r.v[i] * scale);
+      if (c.has(i)) row[c.d + static_cast<int64_t>(i) * c.stride] = static_cast<T>(r.v[i] * scale);
   }
+}
+
+// The same of a row of fp32 partial sums.
+template <typename T>
+__device__ __forceinline__ void store_partial(float* row, const Cols& c, const Vec<T>& r) {
+  if (c.vec) {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i += 4)
+      *reinterpret_cast<float4*>(row + c.d + i) = make_float4(r.v[i], r.v[i + 1], r.v[i + 2], r.v[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+      if (c.has(i)) row[c.d + static_cast<int64_t>(i) * c.stride] = r.v[i];
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ Vec<T> load_partial(const float* row, const Cols& c) {
+  Vec<T> r;
+  if (c.vec) {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; i += 4) {
+      const float4 q = *reinterpret_cast<const float4*>(row + c.d + i);
+      r.v[i] = q.x, r.v[i + 1] = q.y, r.v[i + 2] = q.z, r.v[i + 3] = q.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i)
+      r.v[i] = c.has(i) ? row[c.d + static_cast<int64_t>(i) * c.stride] : 0.f;
+  }
+  return r;
 }
 
 // One CTA: 256 / row_threads tokens, row_threads across a row.
@@ -82,126 +141,248 @@ __global__ void __launch_bounds__(kThreads)
   if (!ok && lane == 0) record_status(status, kDevBadIndex);
   const T* src = table + (ok ? v : 0) * D;
   T* dst = out + t * D;
-  for (int64_t d = static_cast<int64_t>(lane) * kVec<T>; d < D;
-       d += static_cast<int64_t>(row_threads) * kVec<T>) {
+  for (int slice = 0;; ++slice) {
+    const Cols c = thread_cols<T>(slice, lane, row_threads, vec != 0, D);
+    if (!c.any()) break;
     Vec<T> r = {};
-    if (ok) r = load_vec(src + d, vec != 0, D - d);
-    store_vec(dst + d, vec != 0, D - d, r, scale);
+    if (ok) add_raw(r, load_raw(src, c));
+    store_cols(dst, c, r, scale);
   }
 }
 
-// Sorts blocks of 2048 keys (entry << 32 | token), a bitonic network in shared
-// memory; tokens without a gradient sort to the end.
+__device__ __forceinline__ uint64_t make_key(uint32_t entry, int64_t token) {
+  return static_cast<uint64_t>(entry) << 32 | static_cast<uint32_t>(token);
+}
+__device__ __forceinline__ uint32_t entry_of(uint64_t key) { return static_cast<uint32_t>(key >> 32); }
+
+// The entry a token adds to.
+__device__ __forceinline__ uint32_t token_entry(int64_t v, int64_t V, int64_t padding,
+                                                uint32_t* status) {
+  const bool ok = v >= 0 && v < V;
+  if (!ok) record_status(status, kDevBadIndex);
+  return ok && v != padding ? static_cast<uint32_t>(v) : kNone;
+}
+
+// One CTA: the places of 64 tokens, eight threads a token, with every token's entry in
+// shared memory.  A token comes after those with a smaller entry, and those before it
+// with its own.
+__global__ void __launch_bounds__(kRankThreads)
+    embedding_rank_kernel(const int64_t* idx, int n_tok, int64_t V, int64_t padding,
+                          uint64_t* sorted, uint32_t* status) {
+  extern __shared__ __align__(16) uint32_t entries[];  // up to a multiple of 4, the rest above every entry
+  constexpr int kPer = kRankThreads / kRankTokens;
+  grid_wait();
+  launch_dependents();
+  const int padded = (n_tok + 3) / 4 * 4;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < padded; i += kRankThreads)
+    entries[i] = i < n_tok ? token_entry(idx[i], V, padding, status) : kNone;
+  __syncthreads();
+  const int t = static_cast<int>(blockIdx.x) * kRankTokens + static_cast<int>(threadIdx.x) / kPer;
+  const int part = static_cast<int>(threadIdx.x) % kPer;
+  uint32_t mine = 0;
+  int place = 0;
+  if (t < n_tok) {
+    mine = entries[t];
+    const int own = t & ~3;  // the four that t is among
+#pragma unroll 4
+    for (int i = part * 4; i < own; i += kPer * 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(entries + i);
+      place += (q.x <= mine) + (q.y <= mine) + (q.z <= mine) + (q.w <= mine);
+    }
+    const int after = own / 4 + 1;  // the first four past it that are this thread's
+    const int first = after + (part - after % kPer + kPer) % kPer;
+#pragma unroll 4
+    for (int i = first * 4; i < padded; i += kPer * 4) {
+      const uint4 q = *reinterpret_cast<const uint4*>(entries + i);
+      place += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
+    }
+    if (part == 0)
+      for (int i = own; i < min(own + 4, n_tok); ++i)
+        place += i < t ? entries[i] <= mine : entries[i] < mine;
+  }
+#pragma unroll
+  for (int o = kPer / 2; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+  if (part == 0 && t < n_tok) sorted[place] = make_key(mine, t);
+}
+
+// Sorts blocks of 2048 keys (entry << 32 | token), a bitonic network in shared memory
+// as wide as the block's tokens need; tokens without a gradient sort to the end.
+// Steps over less than 64 elements stay within a warp's.
 __global__ void __launch_bounds__(kSortThreads)
     embedding_sort_kernel(const int64_t* idx, int64_t n_tok, int64_t V, int64_t padding,
                           uint64_t* keys, uint32_t* status) {
   __shared__ uint64_t s[kSortBlock];
+  grid_wait();
+  launch_dependents();
   const int64_t base = static_cast<int64_t>(blockIdx.x) * kSortBlock;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = static_cast<int>(threadIdx.x) + h * kSortThreads;
+  const int n = static_cast<int>(n_tok - base < kSortBlock ? n_tok - base : kSortBlock);
+  int width = 64;
+  while (width < n) width *= 2;
+  for (int i = threadIdx.x; i < width; i += kSortThreads) {
     const int64_t t = base + i;
-    uint64_t key = kNoEntry;
-    if (t < n_tok) {
-      const int64_t v = idx[t];
-      if (v < 0 || v >= V)
-        record_status(status, kDevBadIndex);
-      else if (v != padding)
-        key = static_cast<uint64_t>(v) << 32 | static_cast<uint32_t>(t);
-      // distinct among those without an entry too, for the places they take
-      if (key == kNoEntry) key = uint64_t{0xFFFFFFFFu} << 32 | static_cast<uint32_t>(t);
-    }
+    // distinct among those without an entry too, for the places they take
+    uint64_t key = ~uint64_t{0};
+    if (i < n) key = make_key(token_entry(idx[t], V, padding, status), t);
     s[i] = key;
   }
-  for (int k = 2; k <= kSortBlock; k <<= 1) {
+  __syncthreads();
+  const int tid = static_cast<int>(threadIdx.x);
+  for (int k = 2; k <= width; k <<= 1) {
     for (int j = k >> 1; j > 0; j >>= 1) {
-      __syncthreads();
-      const int i = 2 * static_cast<int>(threadIdx.x) - (static_cast<int>(threadIdx.x) & (j - 1));
-      const uint64_t a = s[i], b = s[i + j];
-      if ((a > b) == ((i & k) == 0)) s[i] = b, s[i + j] = a;
+      if (tid < width / 2) {
+        const int i = 2 * tid - (tid & (j - 1));
+        const uint64_t a = s[i], b = s[i + j];
+        if ((a > b) == ((i & k) == 0)) s[i] = b, s[i + j] = a;
+      }
+      // the next step's pairs: of this warp's 64 elements, or of others
+      const int next = j > 1 ? j >> 1 : k;
+      if (j >= 64 || next >= 64)
+        __syncthreads();
+      else
+        __syncwarp();
     }
   }
   __syncthreads();
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int i = static_cast<int>(threadIdx.x) + h * kSortThreads;
-    if (base + i < n_tok) keys[base + i] = s[i];
-  }
+  for (int i = threadIdx.x; i < n; i += kSortThreads) keys[base + i] = s[i];
 }
 
 // Each key's place among all blocks: its place in its own plus the smaller keys of
-// the others.
+// the others, four searches at a time.
 __global__ void __launch_bounds__(kThreads)
     embedding_merge_kernel(const uint64_t* keys, int64_t n_tok, uint64_t* sorted) {
+  grid_wait();
+  launch_dependents();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= n_tok) return;
   const uint64_t key = keys[i];
-  const int64_t own = i / kSortBlock;
-  int64_t place = i - own * kSortBlock;
-  for (int64_t b0 = 0; b0 < n_tok; b0 += kSortBlock) {
-    if (b0 == own * kSortBlock) continue;
-    const int n = static_cast<int>(n_tok - b0 < kSortBlock ? n_tok - b0 : kSortBlock);
-    int lo = 0, hi = n;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (keys[b0 + mid] < key)
-        lo = mid + 1;
-      else
-        hi = mid;
+  const int64_t blocks = (n_tok + kSortBlock - 1) / kSortBlock;
+  int64_t place = 0;
+  constexpr int kAtOnce = 4;
+  for (int64_t b = 0; b < blocks; b += kAtOnce) {
+    int lo[kAtOnce], hi[kAtOnce];
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+      const int64_t left = n_tok - (b + q) * kSortBlock;
+      lo[q] = 0;
+      hi[q] = static_cast<int>(left < 0 ? 0 : left < kSortBlock ? left : kSortBlock);
     }
-    place += lo;
+    for (int step = kSortBlock; step > 0; step >>= 1) {
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+        if (lo[q] >= hi[q]) continue;
+        const int mid = (lo[q] + hi[q]) >> 1;
+        if (keys[(b + q) * kSortBlock + mid] < key)
+          lo[q] = mid + 1;
+        else
+          hi[q] = mid;
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) place += lo[q];
   }
   sorted[place] = key;
 }
 
-__device__ __forceinline__ uint32_t entry_of(uint64_t key) { return static_cast<uint32_t>(key >> 32); }
-
-// One CTA: a chunk of 32 sorted tokens, row_threads * kVec columns.  A run inside
-// the chunk is written to the gradient; one that the border cuts to the chunk's
-// partial rows: [0] continues from the chunk before, [1] goes on in the next.
+// CTAs of the first `sum_ctas`: a chunk of 32 sorted tokens, kThreads * kVec columns.  A
+// run inside the chunk is written to the gradient; one that the border cuts to the
+// chunk's partial rows: [0] continues from the chunk before, [1] goes on in the next.
+// The others: 32 entries each, those without tokens zeroed.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    embedding_grad_kernel(const uint64_t* sorted, const T* dy, int64_t n_tok, int64_t D, float scale,
-                          int vec, T* grad, float* partial) {
+__global__ void __launch_bounds__(kThreads, 4)
+    embedding_grad_kernel(const uint64_t* sorted, const T* dy, int64_t n_tok,
+                          int64_t V, int64_t D, float scale, int vec, int sum_ctas, int slices,
+                          T* grad, float* partial) {
   __shared__ uint64_t key[kChunk + 2];  // with a neighbour on either side
-  const int64_t p0 = static_cast<int64_t>(blockIdx.x) * kChunk;
+  grid_wait();
+  launch_dependents();
+  if (static_cast<int>(blockIdx.x) >= sum_ctas) {
+    const int64_t v0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - sum_ctas) * 32;
+    uint32_t* const has_tokens = reinterpret_cast<uint32_t*>(key);
+    if (threadIdx.x < 32) {  // a search for each entry
+      const uint32_t v = static_cast<uint32_t>(v0) + threadIdx.x;
+      int64_t lo = 0, hi = n_tok;
+      while (lo < hi) {
+        const int64_t mid = (lo + hi) >> 1;
+        if (entry_of(sorted[mid]) < v)
+          lo = mid + 1;
+        else
+          hi = mid;
+      }
+      const uint32_t found =
+          __ballot_sync(0xffffffffu, lo < n_tok && entry_of(sorted[lo]) == v);
+      if (threadIdx.x == 0) *has_tokens = found;
+    }
+    __syncthreads();
+    const uint32_t has = *has_tokens;
+    const int rows = static_cast<int>(V - v0 < 32 ? V - v0 : 32);
+    T* first = grad + v0 * D;
+    const int len = static_cast<int>(D), total = rows * len;  // below 2^27
+    constexpr int kStep = kThreads * kVec<T>;
+    if (vec != 0) {
+      int row = static_cast<int>(threadIdx.x) * kVec<T> / len;
+      int col = static_cast<int>(threadIdx.x) * kVec<T> % len;
+      const int step_row = kStep / len, step_col = kStep % len;
+      while (row < rows) {
+        if (((has >> row) & 1u) == 0)
+          *reinterpret_cast<uint4*>(first + row * len + col) = make_uint4(0, 0, 0, 0);
+        row += step_row;
+        col += step_col;
+        if (col >= len) col -= len, ++row;
+      }
+      return;
+    }
+    // the rows' elements in whole 16 bytes, from the boundary at or before the first
+    const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15u) / sizeof(T));
+    for (int e = static_cast<int>(threadIdx.x) * kVec<T> - lead; e < total; e += kStep) {
+      const int begin = e < 0 ? 0 : e, end = e + kVec<T> < total ? e + kVec<T> : total;
+      if (begin >= end) continue;
+      const int r0 = begin / len, r1 = (end - 1) / len;
+      // of these 16 bytes' rows (short rows: up to eight of them), whether some have tokens
+      const uint32_t span = (r1 - r0 == 31 ? ~0u : (1u << (r1 - r0 + 1)) - 1u) << r0;
+      if ((has & span) == 0 && end - e == kVec<T> && begin == e) {
+        *reinterpret_cast<uint4*>(first + e) = make_uint4(0, 0, 0, 0);
+      } else {
+        for (int i = begin; i < end; ++i)
+          if (((has >> (i / len)) & 1u) == 0) first[i] = static_cast<T>(0.f);
+      }
+    }
+    return;
+  }
+  const int64_t chunk = static_cast<int>(blockIdx.x) / slices;
+  const int64_t p0 = chunk * kChunk;
   const int n = static_cast<int>(n_tok - p0 < kChunk ? n_tok - p0 : kChunk);
   if (threadIdx.x < kChunk + 2) {
     const int64_t p = p0 + static_cast<int>(threadIdx.x) - 1;
-    key[threadIdx.x] = p >= 0 && p < n_tok ? sorted[p] : kNoEntry;
+    key[threadIdx.x] = p >= 0 && p < n_tok ? sorted[p] : ~uint64_t{0};
   }
   __syncthreads();
-  const int64_t d = (static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x) * kVec<T>;
-  if (d >= D || entry_of(key[1]) == 0xFFFFFFFFu) return;
+  const Cols c = thread_cols<T>(static_cast<int>(blockIdx.x) % slices, static_cast<int>(threadIdx.x),
+                                kThreads, vec != 0, D);
+  if (!c.any()) return;
   constexpr int kAhead = 8;
   Vec<T> acc = {};
   bool first_run = entry_of(key[0]) == entry_of(key[1]);  // begun in an earlier chunk
   for (int q0 = 0; q0 < n; q0 += kAhead) {
-    Vec<T> row[kAhead];
+    uint4 row[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (q0 + i < n && entry_of(key[q0 + i + 1]) != 0xFFFFFFFFu)
-        row[i] = load_vec(dy + static_cast<int64_t>(static_cast<uint32_t>(key[q0 + i + 1])) * D + d,
-                          vec != 0, D - d);
+      if (q0 + i < n && entry_of(key[q0 + i + 1]) != kNone)
+        row[i] = load_raw(dy + static_cast<int64_t>(static_cast<uint32_t>(key[q0 + i + 1])) * D, c);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const int q = q0 + i;
       if (q >= n) break;
       const uint32_t e = entry_of(key[q + 1]);
-      if (e == 0xFFFFFFFFu) return;
-#pragma unroll
-      for (int j = 0; j < kVec<T>; ++j) acc.v[j] += row[i].v[j];
+      if (e == kNone) return;
+      add_raw(acc, row[i]);
       const bool ends = entry_of(key[q + 2]) != e;
       if (!ends && q + 1 < n) continue;
-      if (ends && !first_run) {
-        store_vec(grad + static_cast<int64_t>(e) * D + d, vec != 0, D - d, acc, scale);
-      } else {
-        float* dst = partial + (static_cast<int64_t>(blockIdx.x) * 2 + (first_run ? 0 : 1)) * D + d;
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j)
-          if (d + j < D) dst[j] = acc.v[j];
-      }
+      if (ends && !first_run)
+        store_cols(grad + static_cast<int64_t>(e) * D, c, acc, scale);
+      else
+        store_partial(partial + (chunk * 2 + (first_run ? 0 : 1)) * D, c, acc);
       acc = {};
       first_run = false;
     }
@@ -211,37 +392,38 @@ __global__ void __launch_bounds__(kThreads)
 // One CTA for each chunk whose last run begins in it and goes on in the next: adds
 // that run's partial sums in chunk order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kJoin)
     embedding_join_kernel(const uint64_t* sorted, const float* partial, int64_t n_tok, int64_t D,
-                          float scale, T* grad) {
-  const int64_t last = (static_cast<int64_t>(blockIdx.x) + 1) * kChunk - 1;
+                          float scale, int vec, T* grad) {
+  grid_wait();
+  const int64_t first = blockIdx.x, last = (first + 1) * kChunk - 1;
   if (last + 1 >= n_tok) return;
   const uint32_t e = entry_of(sorted[last]);
-  if (e == 0xFFFFFFFFu || entry_of(sorted[last + 1]) != e) return;
-  const int64_t p0 = last - kChunk + 1;
-  if (p0 > 0 && entry_of(sorted[p0 - 1]) == e) return;  // begun before this chunk
-  // the chunk that holds the run's end
-  int64_t lo = last + 1, hi = n_tok;  // first position past the run
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) >> 1;
-    if (entry_of(sorted[mid]) == e)
-      lo = mid + 1;
-    else
-      hi = mid;
-  }
-  const int64_t end_chunk = (lo - 1) / kChunk;
-  const int64_t d = static_cast<int64_t>(blockIdx.y) * kThreads + threadIdx.x;
-  if (d >= D) return;
-  float acc = partial[(static_cast<int64_t>(blockIdx.x) * 2 + 1) * D + d];
-  constexpr int kAhead = 8;
-  for (int64_t c = static_cast<int64_t>(blockIdx.x) + 1; c <= end_chunk; c += kAhead) {
-    float v[kAhead];
+  if (e == kNone || entry_of(sorted[last + 1]) != e) return;
+  if (first > 0 && entry_of(sorted[first * kChunk - 1]) == e && entry_of(sorted[first * kChunk]) == e)
+    return;  // begun before this chunk
+  const Cols c = thread_cols<T>(static_cast<int>(blockIdx.y), static_cast<int>(threadIdx.x), kJoin,
+                                vec != 0, D);
+  if (!c.any()) return;
+  Vec<T> acc = load_partial<T>(partial + (first * 2 + 1) * D, c);
+  constexpr int kAhead = 4;
+  const int64_t chunks = (n_tok + kChunk - 1) / kChunk;
+  for (int64_t q = first + 1; q < chunks; q += kAhead) {
+    bool goes[kAhead];  // the run reaches chunk q + i
+    Vec<T> v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) v[i] = c + i <= end_chunk ? partial[(c + i) * 2 * D + d] : 0.f;
+    for (int i = 0; i < kAhead; ++i) goes[i] = q + i < chunks && entry_of(sorted[(q + i) * kChunk]) == e;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) acc += v[i];
+    for (int i = 0; i < kAhead; ++i)
+      if (goes[i]) v[i] = load_partial<T>(partial + (q + i) * 2 * D, c);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (goes[i])
+#pragma unroll
+        for (int k = 0; k < kVec<T>; ++k) acc.v[k] += v[i].v[k];
+    if (!goes[kAhead - 1]) break;
   }
-  grad[static_cast<int64_t>(e) * D + d] = static_cast<T>(acc * scale);
+  store_cols(grad + static_cast<int64_t>(e) * D, c, acc, scale);
 }
 
 // ------------------------------------------------------------------- host --
@@ -258,7 +440,7 @@ int check(int64_t T, int64_t V, int64_t D, int dtype) {
   if (T <= 0 || V <= 0 || D <= 0) return fail(MLORA_ERR_INVALID_ARG, "T, V, D must be positive");
   if (dtype != MLORA_DTYPE_BF16 && dtype != MLORA_DTYPE_F16 && dtype != MLORA_DTYPE_F32)
     return fail(MLORA_ERR_UNSUPPORTED, "dtype must be BF16, F16 or F32");
-  if (T > (int64_t{1} << 31) - 256 || V > (int64_t{1} << 31) - 256 || D > (1 << 23))
+  if (T > (int64_t{1} << 31) - 256 || V > (int64_t{1} << 31) - 256 || D > (1 << 22))
     return fail(MLORA_ERR_UNSUPPORTED, "shape too large");
   return MLORA_OK;
 }
@@ -291,46 +473,71 @@ struct Work {
 Work plan(void* base, int64_t T, int64_t D) {
   uint8_t* b = static_cast<uint8_t*>(base);
   Work w;
-  const int64_t kb = round_up(T * 8, 256);
-  w.keys = reinterpret_cast<uint64_t*>(b);
-  w.sorted = T > kSortBlock ? reinterpret_cast<uint64_t*>(b + kb) : w.keys;
-  const int64_t off = T > kSortBlock ? 2 * kb : kb;
-  w.partial = reinterpret_cast<float*>(b + off);
-  w.bytes = off + round_up(chunks(T) * 2 * D * 4, 256);
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) {
+    uint8_t* p = b != nullptr ? b + off : nullptr;
+    off += round_up(bytes, 256);
+    return p;
+  };
+  w.sorted = reinterpret_cast<uint64_t*>(take(T * 8));
+  w.keys = T > kPairTokens ? reinterpret_cast<uint64_t*>(take(T * 8)) : nullptr;
+  w.partial = reinterpret_cast<float*>(take(chunks(T) * 2 * D * 4));
+  w.bytes = off;
   return w;
 }
 
 template <typename T>
 int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int64_t V, int64_t D,
              float scale, int64_t padding, const Work& w, cudaStream_t s) {
-  cudaError_t e = cudaMemsetAsync(grad, 0, static_cast<size_t>(V * D) * sizeof(T), s);
-  if (e != cudaSuccess) return launch_status(e, "embedding gradient");
-  {
+  cudaError_t e;
+  if (n_tok <= kPairTokens) {
+    static std::atomic<bool> limit_set[64];
+    if (int rc = set_max_smem(reinterpret_cast<const void*>(embedding_rank_kernel), kPairTokens * 4,
+                              limit_set))
+      return rc;
     LaunchScope scope(kKindElementwise, s);
-    embedding_sort_kernel<<<static_cast<unsigned>((n_tok + kSortBlock - 1) / kSortBlock),
-                            kSortThreads, 0, s>>>(idx, n_tok, V, padding, w.keys,
-                                                  device_status_ptr());
-  }
-  if (n_tok > kSortBlock) {
-    LaunchScope scope(kKindElementwise, s);
-    embedding_merge_kernel<<<static_cast<unsigned>((n_tok + kThreads - 1) / kThreads), kThreads, 0,
-                             s>>>(w.keys, n_tok, w.sorted);
+    e = launch_kernel(embedding_rank_kernel,
+                      dim3(static_cast<unsigned>((n_tok + kRankTokens - 1) / kRankTokens)), kRankThreads,
+                      static_cast<size_t>(n_tok + 3) / 4 * 16, s, 0, 0, true, idx,
+                      static_cast<int>(n_tok), V, padding, w.sorted, device_status_ptr());
+  } else {
+    {
+      LaunchScope scope(kKindElementwise, s);
+      e = launch_kernel(embedding_sort_kernel,
+                        dim3(static_cast<unsigned>((n_tok + kSortBlock - 1) / kSortBlock)),
+                        kSortThreads, 0, s, 0, 0, true, idx, n_tok, V, padding, w.keys,
+                        device_status_ptr());
+    }
+    if (e == cudaSuccess) {
+      LaunchScope scope(kKindElementwise, s);
+      e = launch_kernel(embedding_merge_kernel,
+                        dim3(static_cast<unsigned>((n_tok + kThreads - 1) / kThreads)), kThreads, 0, s,
+                        0, 0, true, static_cast<const uint64_t*>(w.keys), n_tok, w.sorted);
+    }
   }
   const int vec = D % kVec<T> == 0 && aligned(dy, 16) && aligned(grad, 16);
   const int64_t cols = int64_t{kThreads} * kVec<T>;
-  const unsigned n = static_cast<unsigned>(chunks(n_tok));
-  {
+  const int slices = static_cast<int>((D + cols - 1) / cols);
+  const int64_t sum_ctas = chunks(n_tok) * slices;
+  const int64_t grid = sum_ctas + (V + 31) / 32;
+  if (grid > (int64_t{1} << 31) - 1)
+    return fail(MLORA_ERR_UNSUPPORTED, "embedding gradient: too many tokens for rows this long");
+  if (e == cudaSuccess) {
     LaunchScope scope(kKindElementwise, s);
-    embedding_grad_kernel<T><<<dim3(n, static_cast<unsigned>((D + cols - 1) / cols)), kThreads, 0, s>>>(
-        w.sorted, static_cast<const T*>(dy), n_tok, D, scale, vec, static_cast<T*>(grad), w.partial);
+    e = launch_kernel(embedding_grad_kernel<T>, dim3(static_cast<unsigned>(grid)), kThreads, 0, s, 0, 0,
+                      true, static_cast<const uint64_t*>(w.sorted), static_cast<const T*>(dy), n_tok, V,
+                      D, scale, vec, static_cast<int>(sum_ctas), slices, static_cast<T*>(grad), w.partial);
   }
-  if (n > 1) {
+  if (e == cudaSuccess && chunks(n_tok) > 1) {
     LaunchScope scope(kKindElementwise, s);
-    embedding_join_kernel<T><<<dim3(n - 1, static_cast<unsigned>((D + kThreads - 1) / kThreads)),
-                               kThreads, 0, s>>>(w.sorted, w.partial, n_tok, D, scale,
-                                                 static_cast<T*>(grad));
+    e = launch_kernel(embedding_join_kernel<T>,
+                      dim3(static_cast<unsigned>(chunks(n_tok) - 1),
+                           static_cast<unsigned>((D + kJoin * kVec<T> - 1) / (kJoin * kVec<T>))),
+                      kJoin, 0, s, 0, 0, true, static_cast<const uint64_t*>(w.sorted),
+                      static_cast<const float*>(w.partial), n_tok, D, scale, vec,
+                      static_cast<T*>(grad));
   }
-  return launch_status(cudaSuccess, "embedding gradient");
+  return launch_status(e, "embedding gradient");
 }
 
 }  // namespace
