@@ -345,11 +345,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tmem_alloc_pair(tmem_slot, kTmemCols);
     tmem_relinquish_pair();
   }
-  const Shape shape = device_shape(p);
   tc_fence_before();
   cluster_sync();  // both CTAs' barriers initialised and TMEM allocated
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  grid_wait();  // every operand but the weight is the kernels' before; in every role
+  launch_dependents();
+  const Shape shape = device_shape(p);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer --
@@ -554,7 +556,7 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   const int grid = 2 * static_cast<int>(units < pairs ? units : pairs);
   LaunchScope scope(kKindGemm, stream);
   return launch_status(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), kThreads, kSmemBytes,
-                                     stream, 0, 0, false, tx, tw, tx2, tw2, p),
+                                     stream, 0, 0, true, tx, tw, tx2, tw2, p),
                        "head gemm launch");
 }
 

@@ -37,9 +37,16 @@ __host__ __device__ constexpr float grad_unit<__half>() { return 64.f; }
 struct HeadCount {
   int32_t counted;
   float inv;  // 1 / counted, 0 for none
+  uint32_t ticket;  // CTAs that are through with their token's loss
 };
 
-// One CTA: numbers the tokens that count in order.  slot_of[m] = the token's number
+__device__ __forceinline__ void set_count(HeadCount* out, int32_t counted) {
+  out->counted = counted;
+  out->inv = counted > 0 ? 1.f / static_cast<float>(counted) : 0.f;
+  out->ticket = 0;
+}
+
+// One CTA: numbers the tokens that count in order (many tokens).  slot_of[m] = the token's number
 // or -1; row_of[i], label[i] = token i's row and label (row_of = -1 past the last).
 __global__ void __launch_bounds__(kScanThreads)
     head_scan_kernel(const int64_t* labels, int64_t M, int64_t V, int64_t ignore_index,
@@ -47,6 +54,8 @@ __global__ void __launch_bounds__(kScanThreads)
                      HeadCount* out, uint32_t* status) {
   __shared__ int32_t warp_sum[kScanThreads / 32];
   __shared__ int32_t total;
+  grid_wait();
+  launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int32_t base = 0;
   for (int64_t m0 = 0; m0 < M; m0 += kScanThreads * kScanItems) {
@@ -105,33 +114,82 @@ __global__ void __launch_bounds__(kScanThreads)
     __syncthreads();
   }
   for (int64_t i = base + threadIdx.x; i < M; i += kScanThreads) row_of[i] = -1;
-  if (threadIdx.x == 0) {
-    out->counted = base;
-    out->inv = base > 0 ? 1.f / static_cast<float>(base) : 0.f;
-  }
+  if (threadIdx.x == 0) set_count(out, base);
 }
+
+// What the scan leaves of the tokens.
+struct Numbers {
+  int32_t *slot_of, *row_of, *label;
+  HeadCount* count;
+};
 
 // xc[i] = x[row_of[i]], zeros past the last counted token (as many as a reduction
 // over tokens reads; all of them for the LoRA products, which run over every row);
 // and target[i] = the label's logit but for a LoRA term, in 32 bits; ref[i] = it in whole
-// units of log 2.
-template <typename T>
-__global__ void __launch_bounds__(128)
-    head_gather_kernel(const uint4* x, const uint4* w, const int32_t* row_of, const int32_t* label,
-                       const HeadCount* count, int64_t K8, int64_t ld8, int zero_all, uint4* xc, float* target, float* ref) {
+// units of log 2.  One CTA per row of xc, or with kNumber per token: each then counts
+// the tokens ahead of its own itself, which up to some thousands is faster than a
+// launch that numbers them.
+constexpr int kGatherThreads = 128;
+constexpr int64_t kNumberTokens = 2048;
+
+template <typename T, bool kNumber>
+__global__ void __launch_bounds__(kGatherThreads)
+    head_gather_kernel(const uint4* x, const uint4* w, const int64_t* labels, int64_t ignore_index,
+                       int64_t M, int64_t V, Numbers num, float* row_loss, int64_t K8, int64_t ld8,
+                       int zero_all, uint4* xc, float* target, float* ref, uint32_t* status) {
   __shared__ float part[4];
-  const int64_t i = blockIdx.x;
-  const int32_t row = row_of[i];
+  __shared__ int32_t parts[2][4];
+  grid_wait();
+  launch_dependents();
+  int64_t i = blockIdx.x;
+  int32_t row = -1, y = 0, counted = 0;
+  if constexpr (kNumber) {
+    const int64_t m = i;
+    int32_t ahead = 0;
+    for (int64_t q = threadIdx.x; q < M; q += kGatherThreads) {
+      const int64_t v = labels[q];
+      const bool counts = v != ignore_index && v >= 0 && v < V;
+      ahead += counts && q < m;
+      counted += counts;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+      counted += __shfl_xor_sync(0xffffffffu, counted, o);
+    }
+    if ((threadIdx.x & 31) == 0)
+      parts[0][threadIdx.x >> 5] = ahead, parts[1][threadIdx.x >> 5] = counted;
+    __syncthreads();
+    ahead = parts[0][0] + parts[0][1] + parts[0][2] + parts[0][3];
+    counted = parts[1][0] + parts[1][1] + parts[1][2] + parts[1][3];
+    const int64_t v = labels[m];
+    const bool counts = v != ignore_index && v >= 0 && v < V;
+    // the token's number, or among the rest the place behind the counted ones
+    i = counts ? ahead : counted + (m - ahead);
+    if (counts) row = static_cast<int32_t>(m), y = static_cast<int32_t>(v);
+    if (threadIdx.x == 0) {
+      if (v != ignore_index && !counts) record_status(status, kDevBadIndex);
+      num.slot_of[m] = counts ? ahead : -1;
+      num.row_of[i] = row;
+      num.label[i] = y;
+      if (!counts && row_loss != nullptr) row_loss[m] = 0.f;
+      if (m == 0) set_count(num.count, counted);
+    }
+  } else {
+    row = num.row_of[i];
+    counted = num.count->counted;
+    if (row >= 0) y = num.label[i];
+  }
   if (row < 0) {
-    if (zero_all || i < (count->counted + 63) / 64 * 64)
-      for (int64_t k = threadIdx.x; k < K8; k += 128) xc[i * ld8 + k] = make_uint4(0, 0, 0, 0);
+    if (zero_all || i < (counted + 63) / 64 * 64)
+      for (int64_t k = threadIdx.x; k < K8; k += kGatherThreads) xc[i * ld8 + k] = make_uint4(0, 0, 0, 0);
     return;
   }
   const uint4* xr = x + static_cast<int64_t>(row) * K8;
-  const uint4* wr = w + static_cast<int64_t>(label[i]) * K8;
+  const uint4* wr = w + static_cast<int64_t>(y) * K8;
   float s = 0.f;
 #pragma unroll 4
-  for (int64_t k = threadIdx.x; k < K8; k += 128) {
+  for (int64_t k = threadIdx.x; k < K8; k += kGatherThreads) {
     const uint4 xv = xr[k], wv = wr[k];
     xc[i * ld8 + k] = xv;
     const T* xe = reinterpret_cast<const T*>(&xv);
@@ -149,6 +207,39 @@ __global__ void __launch_bounds__(128)
     // in units of log 2, within what leaves room above and below; 0 for no number
     if (ref != nullptr) ref[i] = fabsf(t) < INFINITY ? rintf(t * 1.4426950408889634f) : 0.f;
   }
+}
+
+// The loss of the call, once each of the M CTAs has passed here with its token's nll (or
+// without one): the last one adds them up in order.  Sum of the counted tokens' losses,
+// or their mean (of none: NaN, as 0 / 0 is).
+struct LossOut {
+  float* loss;  // may be null
+  float* nll;
+  int64_t M;
+  int mean;
+};
+
+__device__ __forceinline__ void finish_loss(const LossOut& o, HeadCount* count) {
+  if (o.loss == nullptr) return;
+  __shared__ bool last;
+  __shared__ double part[kRowThreads / 32];
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(&count->ticket, 1u) == static_cast<uint32_t>(o.M - 1);
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const int32_t counted = count->counted;
+  double s = 0.0;
+  for (int32_t i = threadIdx.x; i < counted; i += kRowThreads) s += __ldcg(o.nll + i);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < kRowThreads / 32; ++w) s += part[w];
+  *o.loss = static_cast<float>(o.mean ? s / counted : s);
 }
 
 // W2 of the logits: [B 0 | B 0], R columns each, for the two parts of s x A^T.
@@ -185,13 +276,18 @@ __device__ __forceinline__ float gap_of(float gap, float ly) { return ly == INFI
 // the gradient of x) by setting the label's to -S, S the sum of the others.  Only a row
 // with more than one reference is rewritten, by powers of two.
 __global__ void __launch_bounds__(kRowThreads)
-    head_ref_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0, const HeadCount* count,
-                    const int32_t* label, const int32_t* row_of, const float* target,
-                    float* row_loss, float* nll, __nv_bfloat16* eg, float* rest, float* row_scale) {
+    head_ref_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0, Numbers num,
+                    const float* target, float* row_loss, LossOut out, __nv_bfloat16* eg, float* rest,
+                    float* row_scale) {
   __shared__ float sn[kRowThreads / 32], sl[kRowThreads / 32], ss[kRowThreads / 32];
+  grid_wait();
+  launch_dependents();
   const int64_t i = blockIdx.x;
   const int64_t slot = row0 + i;
-  if (slot >= count->counted) return;
+  if (slot >= num.count->counted) {
+    finish_loss(out, num.count);
+    return;
+  }
   const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
   const float2* st = stats + i * tiles;
   float top = -INFINITY, low = INFINITY;
@@ -227,21 +323,23 @@ __global__ void __launch_bounds__(kRowThreads)
     }
     __syncthreads();
   }
-  if (threadIdx.x != 0) return;
-  const int32_t y = label[slot];
-  // top log 2 - l_y, log 2 in two parts (the first of 12 bits: its product is exact)
-  const float ly = target[slot];
-  const float gap = gap_of(fmaf(top, 0.693115234375f, -ly) + top * 3.19461832987e-05f, ly);
-  const float u = s * expf(gap);
-  const float loss = row_loss_of(gap, s, u);
-  nll[slot] = loss;
-  if (row_loss != nullptr) row_loss[row_of[slot]] = loss;
-  if (eg == nullptr) return;
-  // 1 / (S + exp(l_y) 2^-top)
-  row_scale[slot] = u < 1.f ? expf(gap) / (1.f + u) : 1.f / (s + expf(-gap));
-  const __nv_bfloat16 gy = __float2bfloat16_rn(-s);
-  eg[i * ld + y] = gy;
-  rest[slot] = -s - __bfloat162float(gy);
+  if (threadIdx.x == 0) {
+    // top log 2 - l_y, log 2 in two parts (the first of 13 bits: its product is exact)
+    const float ly = target[slot];
+    const float gap = gap_of(fmaf(top, 0.693115234375f, -ly) + top * 3.19461832987e-05f, ly);
+    const float u = s * expf(gap);
+    const float loss = row_loss_of(gap, s, u);
+    out.nll[slot] = loss;
+    if (row_loss != nullptr) row_loss[num.row_of[slot]] = loss;
+    if (eg != nullptr) {
+      // 1 / (S + exp(l_y) 2^-top)
+      row_scale[slot] = u < 1.f ? expf(gap) / (1.f + u) : 1.f / (s + expf(-gap));
+      const __nv_bfloat16 gy = __float2bfloat16_rn(-s);
+      eg[i * ld + num.label[slot]] = gy;
+      rest[slot] = -s - __bfloat162float(gy);
+    }
+  }
+  finish_loss(out, num.count);
 }
 
 // After the logits with a reference for each 128: one CTA per counted token of the piece.
@@ -253,23 +351,25 @@ __global__ void __launch_bounds__(kRowThreads)
 // of x adds back times W[y].  Bound: HBM, 4 bytes a logit.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
-    head_row_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0,
-                    const HeadCount* count, const int32_t* label, const int32_t* row_of,
+    head_row_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0, Numbers num,
                     const float* target, const T* xa, const T* b, int64_t xa_ld, int r, int R,
-                    float* row_loss, float* nll, void* eg, float* rest, float* row_scale,
+                    float* row_loss, LossOut out, void* eg, float* rest, float* row_scale,
                     int zero_all) {
   extern __shared__ float factor[];  // of each tile of logits
   __shared__ float sm[kRowThreads / 32], ss[kRowThreads / 32], sx[kRowThreads / 32];
+  grid_wait();
+  launch_dependents();
   const int64_t i = blockIdx.x;
   const int64_t slot = row0 + i;
-  const int32_t counted = count->counted;
+  const int32_t counted = num.count->counted;
   uint4* row = static_cast<uint4*>(eg) + i * (ld / 8);
   if (slot >= counted) {
     if (eg != nullptr && (zero_all || slot < (counted + 63) / 64 * 64))
       for (int64_t v = threadIdx.x; v < ld / 8; v += kRowThreads) row[v] = make_uint4(0, 0, 0, 0);
+    finish_loss(out, num.count);
     return;
   }
-  const int32_t y = label[slot];
+  const int32_t y = num.label[slot];
   const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
   float m = -INFINITY, s = 0.f, extra = 0.f;
   for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
@@ -300,9 +400,10 @@ __global__ void __launch_bounds__(kRowThreads)
   const float u = s * expf(gap);
   const float loss = row_loss_of(gap, s, u);
   if (threadIdx.x == 0) {
-    nll[slot] = loss;
-    if (row_loss != nullptr) row_loss[row_of[slot]] = loss;
+    out.nll[slot] = loss;
+    if (row_loss != nullptr) row_loss[num.row_of[slot]] = loss;
   }
+  finish_loss(out, num.count);
   if (eg == nullptr) return;
   constexpr float unit = grad_unit<T>();
   const float lse = loss + ly;
@@ -336,22 +437,6 @@ __global__ void __launch_bounds__(kRowThreads)
     v = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
                    pack2<T>(o[6], o[7]));
     row[q] = v;
-  }
-}
-
-// loss = sum of the counted tokens' losses, or their mean (of none: NaN, as 0 / 0 is).
-__global__ void __launch_bounds__(1024)
-    head_reduce_kernel(const float* nll, const HeadCount* count, int mean, float* loss) {
-  __shared__ double part[32];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < count->counted; i += 1024) s += nll[i];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) s += part[w];
-    *loss = static_cast<float>(mean ? s / count->counted : s);
   }
 }
 
@@ -581,18 +666,26 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
   // one reference a row: g's factor per row reaches x alone
   const bool by_row = elt == Elt::kBF16 && !d.lora() && !d.want(MLORA_HEAD_GRAD_W);
   int rc;
-  {
+  const Numbers num{st.slot_of, ws.row_of, st.label, st.count};
+  const LossOut out{loss, ws.nll, M, mean ? 1 : 0};
+  const bool number = M <= kNumberTokens;
+  // every kernel here waits for the one before it and then lets the next one start
+  cudaError_t e = cudaSuccess;
+  if (!number) {
     LaunchScope scope(kKindElementwise, s);
-    head_scan_kernel<<<1, kScanThreads, 0, s>>>(labels, M, V, ignore_index, st.slot_of, ws.row_of,
-                                               st.label, row_loss, st.count, device_status_ptr());
+    e = launch_kernel(head_scan_kernel, dim3(1), kScanThreads, 0, s, 0, 0, true, labels, M, V,
+                      ignore_index, st.slot_of, ws.row_of, st.label, row_loss, st.count,
+                      device_status_ptr());
   }
-  {
+  if (e == cudaSuccess) {
     LaunchScope scope(kKindElementwise, s);
-    head_gather_kernel<T><<<static_cast<unsigned>(M), 128, 0, s>>>(
-        static_cast<const uint4*>(x), static_cast<const uint4*>(w), ws.row_of, st.label, st.count,
-        K / 8, ldx / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target, by_row ? ws.ref : nullptr);
+    e = launch_kernel(number ? head_gather_kernel<T, true> : head_gather_kernel<T, false>,
+                      dim3(static_cast<unsigned>(M)), kGatherThreads, 0, s, 0, 0, true,
+                      static_cast<const uint4*>(x), static_cast<const uint4*>(w), labels, ignore_index, M,
+                      V, num, row_loss, K / 8, ldx / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target,
+                      by_row ? ws.ref : nullptr, device_status_ptr());
   }
-  if ((rc = launch_status(cudaSuccess, "linear cross entropy: gather"))) return rc;
+  if ((rc = launch_status(e, "linear cross entropy: gather"))) return rc;
   RankArgs ra;
   if (d.lora()) {
     ra.x = ws.xc;
@@ -653,17 +746,19 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     if ((rc = launch_head_gemm(l, s))) return rc;
     {
       LaunchScope scope(kKindElementwise, s);
+      const dim3 grid(static_cast<unsigned>(rows));
       if (by_row)
-        head_ref_kernel<<<static_cast<unsigned>(rows), kRowThreads, 0, s>>>(
-            ws.stats, V, ld, row0, st.count, st.label, ws.row_of, ws.target, row_loss, ws.nll,
-            static_cast<__nv_bfloat16*>(ws.eg), st.rest, st.row_scale);
+        e = launch_kernel(head_ref_kernel, grid, kRowThreads, 0, s, 0, 0, true,
+                          static_cast<const float2*>(ws.stats), V, ld, row0, num,
+                          static_cast<const float*>(ws.target), row_loss, out,
+                          static_cast<__nv_bfloat16*>(ws.eg), st.rest, st.row_scale);
       else
-        head_row_kernel<T><<<static_cast<unsigned>(rows), kRowThreads, d.tiles() * 4, s>>>(
-            ws.stats, V, ld, row0, st.count, st.label, ws.row_of, ws.target,
-            static_cast<const T*>(ws.xa_rows), static_cast<const T*>(b), d.ld_xa(),
-            static_cast<int>(d.r), static_cast<int>(d.R()), row_loss, ws.nll, ws.eg, st.rest,
-            st.row_scale, zero_all);
-      if ((rc = launch_status(cudaSuccess, "linear cross entropy: rows"))) return rc;
+        e = launch_kernel(head_row_kernel<T>, grid, kRowThreads, static_cast<size_t>(d.tiles()) * 4, s, 0,
+                          0, true, static_cast<const float2*>(ws.stats), V, ld, row0, num,
+                          static_cast<const float*>(ws.target), static_cast<const T*>(ws.xa_rows),
+                          static_cast<const T*>(b), d.ld_xa(), static_cast<int>(d.r),
+                          static_cast<int>(d.R()), row_loss, out, ws.eg, st.rest, st.row_scale, zero_all);
+      if ((rc = launch_status(e, "linear cross entropy: rows"))) return rc;
     }
     if (d.lora() && d.grads) {
       RankArgs ru = ra;  // U = s g B
@@ -760,11 +855,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       if ((rc = launch_head_gemm(q, s))) return rc;
     }
   }
-  if (loss != nullptr) {
-    LaunchScope scope(kKindElementwise, s);
-    head_reduce_kernel<<<1, 1024, 0, s>>>(ws.nll, st.count, mean ? 1 : 0, loss);
-  }
-  return launch_status(cudaSuccess, "linear cross entropy: loss");
+  return MLORA_OK;
 }
 
 int launch_scale(const float* src, int64_t n, const State& st, const float* grad, bool mean,
