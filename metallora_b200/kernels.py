@@ -52,6 +52,17 @@ def _need_current(*ts: torch.Tensor) -> None:
             raise DeviceError(f"tensor on {t.device}, but cuda:{cur} is the current device")
 
 
+def _need_here(first: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """``_need_cuda`` and ``_need_current`` of all of them, short where they hold."""
+    d = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
+            d = -1
+    if d < 0 or d != _raw_device():
+        _need_cuda(first, *others)
+        _need_current(first, *(t for t in others if t is not None))
+
+
 def _dtype_code(t: torch.Tensor) -> int:
     try:
         return _DT[t.dtype]
@@ -749,37 +760,41 @@ def linear_cross_entropy_fwd(x2d: torch.Tensor, w: torch.Tensor, labels: torch.T
     Returns (loss, state): loss fp32, a scalar or ("none") one per token; state
     holds the gradients that ``grads`` (``_lib.HEAD_GRAD_*``) names for a unit
     upstream gradient, for ``linear_cross_entropy_bwd``."""
-    _need_cuda(x2d, w, labels, a, b)
-    _need_current(x2d, w, labels, *(t for t in (a, b) if t is not None))
+    _need_here(x2d, w, labels, a, b)
     code = _head_dtype(x2d)
     M, K = x2d.shape
     V = w.shape[0]
     _check_2d("weight", w, (V, K), x2d.dtype)
-    if tuple(labels.shape) != (M,):
+    if labels.shape != (M,):
         raise ShapeError(f"labels shape mismatch: expected {(M,)}, got {tuple(labels.shape)}")
-    if labels.dtype not in (torch.int64, torch.int32):
-        raise ShapeError(f"labels must be int64 or int32, got {labels.dtype}")
+    if labels.dtype != torch.int64:
+        if labels.dtype != torch.int32:
+            raise ShapeError(f"labels must be int64 or int32, got {labels.dtype}")
+        labels = labels.to(torch.int64)
     r = 0
     if a is not None:
         a, b, alpha, r = _pad_rank(a, b, alpha)
         _check_2d("A", a, (r, K), x2d.dtype)
         _check_2d("B", b, (V, r), x2d.dtype)
         a, b = a.contiguous(), b.contiguous()
-    x2d, w, labels = x2d.contiguous(), w.contiguous(), labels.to(torch.int64).contiguous()
-    loss = torch.empty((M,) if reduction == "none" else (), dtype=torch.float32, device=x2d.device)
+    x2d, w, labels = x2d.contiguous(), w.contiguous(), labels.contiguous()
+    rows = reduction == "none"
+    loss = x2d.new_empty((M,) if rows else (), dtype=torch.float32)
     if M == 0:  # no tokens: nothing to launch (a mean over none is NaN, as 0 / 0 is)
         return loss.fill_(float("nan") if reduction == "mean" else 0.0), loss.new_empty(0)
     lib = _lib.load()
     state_bytes, ws_bytes = _head_bytes(M, K, V, r, code, grads)
-    if state_bytes == 0:
-        _lib.check(_lib.MLORA_ERR_UNSUPPORTED, "mlora_linear_cross_entropy")
-    state = torch.empty(state_bytes, dtype=torch.uint8, device=x2d.device)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x2d.device)
-    rows = reduction == "none"
+    if state_bytes == 0:  # the sizes are refused: the call says why
+        _lib.check(lib.mlora_linear_cross_entropy(*(None,) * 8, 0, M, K, V, r, float(alpha), 0, 0,
+                                                  code, grads, None, 0, None),
+                   "mlora_linear_cross_entropy")
+    state = x2d.new_empty(state_bytes, dtype=torch.uint8)
+    ws = x2d.new_empty(ws_bytes, dtype=torch.uint8)
+    out = loss.data_ptr()
     st = lib.mlora_linear_cross_entropy(
-        _ptr(x2d), _ptr(w), _ptr(a), _ptr(b), _ptr(labels), None if rows else _ptr(loss),
-        _ptr(loss) if rows else None, _ptr(state), state_bytes, M, K, V, r, float(alpha),
-        int(ignore_index), int(reduction == "mean"), code, grads, _ptr(ws), ws_bytes, _stream())
+        x2d.data_ptr(), w.data_ptr(), _ptr(a), _ptr(b), labels.data_ptr(), None if rows else out,
+        out if rows else None, state.data_ptr(), state_bytes, M, K, V, r, float(alpha),
+        int(ignore_index), reduction == "mean", code, grads, ws.data_ptr(), ws_bytes, _stream())
     _lib.check(st, "mlora_linear_cross_entropy")
     return loss, state
 
@@ -794,8 +809,7 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.T
     upstream gradient (fp32; one per token after "none").  r is A's rank.  With
     ``da_out``/``db_out`` (contiguous fp32, rank a multiple of 8) dA and dB are added
     into them, or written over them without ``accumulate``."""
-    _need_cuda(grad, state, w)
-    _need_current(grad, state, w)
+    _need_here(grad, state, w)
     code = _head_dtype(w)
     V, K = w.shape
     r8 = (r + 7) // 8 * 8
@@ -817,11 +831,13 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.T
     else:
         w = w.contiguous()
         rows = reduction == "none"
-        grad = grad.to(torch.float32).contiguous()
+        if grad.dtype != torch.float32:
+            grad = grad.to(torch.float32)
+        grad = grad.contiguous()
         if rows and tuple(grad.shape) != (M,):
             raise ShapeError(f"expected {M} upstream gradients, got {tuple(grad.shape)}")
         st = _lib.load().mlora_linear_cross_entropy_backward(
-            _ptr(state), state.numel(), _ptr(grad), int(rows), int(reduction == "mean"), _ptr(w),
+            state.data_ptr(), state.numel(), grad.data_ptr(), rows, reduction == "mean", w.data_ptr(),
             _ptr(dx), _ptr(da), _ptr(db), code if da is None else _dtype_code(da),
             int(into and accumulate), _ptr(dw), M, K, V, r8, code, grads, _stream())
         _lib.check(st, "mlora_linear_cross_entropy_backward")
@@ -833,29 +849,36 @@ def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.T
 # ------------------------------------------------------- token embedding --
 
 def _table_index(indices: torch.Tensor) -> torch.Tensor:
-    if indices.dtype not in (torch.int64, torch.int32):
-        raise ShapeError(f"indices must be int64 or int32, got {indices.dtype}")
-    return indices.reshape(-1).to(torch.int64).contiguous()
+    """The indices in a row of int64."""
+    if indices.dtype != torch.int64:
+        if indices.dtype != torch.int32:
+            raise ShapeError(f"indices must be int64 or int32, got {indices.dtype}")
+        indices = indices.to(torch.int64)
+    return indices.contiguous()
 
 
 def embedding_fwd(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * table[idx] for every index, [*indices.shape, D] (bf16, fp16 or fp32); an
     index outside the table gives a zero row and device status 0x107."""
-    _need_cuda(indices, table)
-    _need_current(indices, table)
+    _need_here(table, indices)
     code = _dtype_code(table)
     if table.dim() != 2:
         raise ShapeError(f"the table must be [V, D], got {tuple(table.shape)}")
     V, D = table.shape
     idx = _table_index(indices)
     table = table.contiguous()
-    out = torch.empty((*indices.shape, D), dtype=table.dtype, device=table.device)
+    out = table.new_empty((*idx.shape, D))
     if out.numel() == 0:
         return out
-    st = _lib.load().mlora_embedding_forward(_ptr(idx), _ptr(table), _ptr(out), idx.numel(), V, D,
-                                             float(scale), code, _stream())
+    st = _lib.load().mlora_embedding_forward(idx.data_ptr(), table.data_ptr(), out.data_ptr(),
+                                             idx.numel(), V, D, float(scale), code, _stream())
     _lib.check(st, "mlora_embedding_forward")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _embedding_ws_bytes(T: int, D: int) -> int:
+    return _lib.load().mlora_embedding_backward_workspace_bytes(T, D)
 
 
 def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, scale: float = 1.0,
@@ -863,25 +886,29 @@ def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, 
     """The table's gradient [num_embeddings, D] in dy's dtype: scale times the sum of
     dy over each entry's tokens, in fp32 and in token order (the same bits in every
     run); zero for ``padding_idx``."""
-    _need_cuda(dy, indices)
-    _need_current(dy, indices)
+    _need_here(dy, indices)
     code = _dtype_code(dy)
     idx = _table_index(indices)
     T, D, V = idx.numel(), dy.shape[-1], int(num_embeddings)
-    dy = dy.reshape(T, D).contiguous()
-    grad = torch.empty((V, D), dtype=dy.dtype, device=dy.device)
+    if dy.shape != (*idx.shape, D):
+        raise ShapeError(f"grad_output {tuple(dy.shape)} does not match indices {tuple(idx.shape)}")
+    dy = dy.contiguous()
+    grad = dy.new_empty((V, D))
     if grad.numel() == 0 or T == 0:
         return grad.zero_()
-    lib = _lib.load()
-    ws = _workspace(lib.mlora_embedding_backward_workspace_bytes(T, D), dy.device)
-    st = lib.mlora_embedding_backward(_ptr(idx), _ptr(dy), _ptr(grad), T, V, D, float(scale),
-                                      -1 if padding_idx is None else int(padding_idx), code,
-                                      _ptr(ws), ws.numel(), _stream())
+    nbytes = _embedding_ws_bytes(T, D)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8)
+    st = _lib.load().mlora_embedding_backward(idx.data_ptr(), dy.data_ptr(), grad.data_ptr(), T, V, D,
+                                              float(scale), -1 if padding_idx is None else padding_idx,
+                                              code, ws.data_ptr(), nbytes, _stream())
     _lib.check(st, "mlora_embedding_backward")
     return grad
 
 
 # ---------------------------------------------------------------- dropout --
+
+_U64 = 2 ** 64 - 1
+
 
 def _drop_threshold(p: float) -> int:
     """Of 65536: p to the nearest multiple of 2^-16."""
@@ -893,12 +920,11 @@ def _drop_threshold(p: float) -> int:
 def _drop_seed(seed) -> tuple[int, int | None]:
     """(seed, device address or None) of an int, or of a CUDA int64 tensor of one element."""
     if torch.is_tensor(seed):
-        _need_cuda(seed)
-        _need_current(seed)
+        _need_here(seed)
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise ShapeError("a seed tensor holds one int64")
         return 0, seed.data_ptr()
-    return int(seed) & (2 ** 64 - 1), None
+    return int(seed) & _U64, None
 
 
 def dropout(x: torch.Tensor, p: float, seed, call: int = 0, scaled: bool = True) -> torch.Tensor:
@@ -906,15 +932,15 @@ def dropout(x: torch.Tensor, p: float, seed, call: int = 0, scaled: bool = True)
     and ``call`` (see ``ops.dropout``); its gradient is the same call on dy.  Without
     ``scaled`` the kept elements are as they were."""
     t = _drop_threshold(p)
-    _need_cuda(x)
-    _need_current(x)
+    _need_here(x)
     code = _dtype_code(x)
     s, s_dev = _drop_seed(seed)
     x = x.contiguous()
     out = torch.empty_like(x)
-    if x.numel():
-        st = _lib.load().mlora_dropout(_ptr(x), _ptr(out), x.numel(), t, int(scaled), s, s_dev,
-                                       int(call) & (2 ** 64 - 1), code, _stream())
+    n = x.numel()
+    if n:
+        st = _lib.load().mlora_dropout(x.data_ptr(), out.data_ptr(), n, t, scaled, s, s_dev,
+                                       call & _U64, code, _stream())
         _lib.check(st, "mlora_dropout")
     return out
 
@@ -924,8 +950,7 @@ def lora_linear_dropout_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor
     """(y, saved_xa) of y = x.W0^T + dropout((alpha/r).(x.A^T).B^T) for 2-D x [M, K], bf16
     or fp16; the mask as in ``dropout``, over [M, N]."""
     t = _drop_threshold(p)
-    _need_cuda(x2d, w0, a, b)
-    _need_current(x2d, w0, a, b)
+    _need_here(x2d, w0, a, b)
     dt = x2d.dtype
     if dt not in (torch.bfloat16, torch.float16):
         raise ShapeError("counter-based LoRA dropout takes bf16 or fp16 activations")
@@ -945,7 +970,7 @@ def lora_linear_dropout_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor
     ws = _workspace(lib.mlora_lora_forward_dropout_workspace_bytes(M, K, N, r, _DT[dt]), x2d.device)
     st = lib.mlora_lora_forward_dropout(_ptr(x2d), _ptr(w0), _ptr(a), _ptr(b), _ptr(y), _ptr(saved),
                                         M, K, N, r, float(alpha), t, s, s_dev,
-                                        int(call) & (2 ** 64 - 1), _DT[dt], _ptr(ws), ws.numel(),
+                                        call & _U64, _DT[dt], _ptr(ws), ws.numel(),
                                         _stream())
     _lib.check(st, "mlora_lora_forward_dropout")
     return y, saved

@@ -127,11 +127,27 @@ class _LoRALinearFn(torch.autograd.Function):
         return dx, dw0, da, db, None, None, None, None
 
 
-def _keep_seed(ctx, seed):
-    """The seed as ``save_for_backward`` takes it: a tensor, whose being written over
-    before the backward is then noticed, or None with the number kept aside."""
+def _once(backward):
+    """``once_differentiable`` where a second derivative may follow (create_graph), and
+    the backward itself, some microseconds shorter, where none can."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, grad):
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    return staticmethod(run)
+
+
+def _keep_seed(ctx, seed, *tensors):
+    """Saves the tensors, and the seed aside or, a tensor itself, with them: its being
+    written over before the backward is then noticed."""
     ctx.seed = None if torch.is_tensor(seed) else seed
-    return seed if torch.is_tensor(seed) else None
+    ctx.save_for_backward(*tensors, *(() if ctx.seed is not None else (seed,)))
+
+
+def _kept_seed(ctx):
+    """(the seed, the tensors saved with it)."""
+    saved = ctx.saved_tensors
+    return (saved[-1], saved[:-1]) if ctx.seed is None else (ctx.seed, saved)
 
 
 class _LoRADropoutFn(torch.autograd.Function):
@@ -142,22 +158,21 @@ class _LoRADropoutFn(torch.autograd.Function):
     def forward(ctx, x2d, w0, a, b, alpha, p, seed, call, compute, sink):
         a_c, b_c = compute if compute is not None else _cast_ab(a, b, x2d.dtype)
         y, saved = _k.lora_linear_dropout_fwd(x2d, w0, a_c, b_c, alpha, p, seed, call)
-        ctx.save_for_backward(x2d, w0, a_c, b_c, saved, _keep_seed(ctx, seed))
+        _keep_seed(ctx, seed, x2d, w0, a_c, b_c, saved)
         ctx.plan = (alpha, p, call)
         ctx.sink = sink
         ctx.ab_dtypes = (a.dtype, b.dtype)
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
-        x2d, w0, a_c, b_c, saved, seed = ctx.saved_tensors
+        seed, (x2d, w0, a_c, b_c, saved) = _kept_seed(ctx)
         alpha, p, call = ctx.plan
         sink = ctx.sink
         same = ctx.ab_dtypes[0] == ctx.ab_dtypes[1] == x2d.dtype
         need = ctx.needs_input_grad
         dx, da, db = _k.lora_linear_dropout_bwd(
-            dy, x2d, w0, a_c, b_c, alpha, saved, p, ctx.seed if seed is None else seed, call,
+            dy, x2d, w0, a_c, b_c, alpha, saved, p, seed, call,
             need_dx=need[0], da_out=sink[0] if sink else None, db_out=sink[1] if sink else None,
             accumulate=_sink_accumulates(sink), grad_dtype=x2d.dtype if same else None,
             on_grads=sink[3] if sink is not None and len(sink) > 3 else None)
@@ -389,7 +404,8 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
     ``linear_cross_entropy``).  ``compute`` and ``sink`` as in _LoRALinearFn."""
 
     @staticmethod
-    def forward(ctx, x2d, w, a, b, labels, alpha, ignore_index, reduction, compute, sink):
+    def forward(ctx, x2d, w, a, b, labels, plan):
+        alpha, ignore_index, reduction, compute, sink = plan
         need = ctx.needs_input_grad
         grads = (_lib.HEAD_GRAD_X if need[0] else 0) | (_lib.HEAD_GRAD_W if need[1] else 0)
         a_c = b_c = None
@@ -405,8 +421,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         ctx.sink = sink
         return loss
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, grad):
         state, w = ctx.saved_tensors
         m, r, reduction, grads = ctx.plan
@@ -423,8 +438,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         elif da is not None and not same:
             da, db = da.to(ctx.ab_dtypes[0]), db.to(ctx.ab_dtypes[1])
         need = ctx.needs_input_grad
-        return (dx, dw, da if need[2] else None, db if need[3] else None, None, None, None, None,
-                None, None)
+        return dx, dw, da if need[2] else None, db if need[3] else None, None, None
 
 
 def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,  # noqa: N803
@@ -457,24 +471,24 @@ def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,
             any(t is not None and t.requires_grad for t in (weight, A, B)):
         raise ConfigurationError("reduction='none' takes gradients of x alone; detach the head's "
                                  "weights or use 'mean' or 'sum'")
-    loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, A, B, labels.reshape(-1),
-                                       float(alpha), int(ignore_index), reduction, _compute, _sink)
-    return loss.reshape(labels.shape) if reduction == "none" else loss
+    flat = x.dim() == 2
+    loss = _LinearCrossEntropyFn.apply(x if flat else x.reshape(-1, x.shape[-1]), weight, A, B,
+                                       labels if flat else labels.reshape(-1),
+                                       (float(alpha), ignore_index, reduction, _compute, _sink))
+    return loss if flat or reduction != "none" else loss.reshape(labels.shape)
 
 
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, call):
-        ctx.save_for_backward(_keep_seed(ctx, seed))
+        _keep_seed(ctx, seed)
         ctx.plan = (p, call)
         return _k.dropout(x, p, seed, call)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
-        seed, = ctx.saved_tensors
         p, call = ctx.plan
-        return _k.dropout(dy, p, ctx.seed if seed is None else seed, call), None, None, None
+        return _k.dropout(dy, p, _kept_seed(ctx)[0], call), None, None, None
 
 
 def dropout(x, p: float, seed, call: int = 0, training: bool = True):
@@ -502,8 +516,7 @@ class _EmbeddingFn(torch.autograd.Function):
         ctx.plan = (table.shape[0], scale, padding_idx)
         return _k.embedding_fwd(indices, table, scale)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         indices, = ctx.saved_tensors
         rows, scale, padding_idx = ctx.plan
