@@ -1069,7 +1069,7 @@ int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, con
   gz.elt = elt;
   gz.out_dtype = dtype;
   if ((rc = launch_gemm(gz, s))) return rc;
-  const DropoutKey key{seed, seed_dev, call, static_cast<uint32_t>(threshold)};
+  const DropoutKey key = dropout_key(seed, seed_dev, call, threshold);
   if ((rc = launch_dropout(z, z, M * N, dtype, key, false, s))) return rc;
   GemmArgs ga = gz;  // y = x . W0^T + drop(z)
   ga.x = x;

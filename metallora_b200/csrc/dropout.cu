@@ -2,7 +2,6 @@
 // where the element's 16 bits (philox.cuh) are at least t.  The backward is the same
 // call on dy.  Eight elements share one generator call, so that its ~90 integer
 // instructions per thread hide behind the 16 (fp32: 32) bytes in and out; bound: HBM.
-#include <algorithm>
 #include <string>
 
 #include "internal.h"
@@ -14,7 +13,7 @@
 namespace mlora {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
@@ -41,28 +40,39 @@ __device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
   }
 }
 
-// x and out may be the same; `vec`: both start on 16 bytes.
-template <typename T>
+// x and out may be the same; `vec`: both start on 16 bytes.  Two blocks of eight a
+// thread, loaded ahead of the generator's calls, which run interleaved.
+template <typename T, bool kDevSeed>
 __global__ void __launch_bounds__(kThreads)
     dropout_kernel(const T* x, T* out, int64_t n, int vec, float scale, DropoutKey key) {
-  const uint64_t seed = dropout_seed(key);
-  const int64_t blocks = (n + 7) / 8;
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; b < blocks;
-       b += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t e = b * 8;
-    float v[8];
-    if (vec != 0 && e + 8 <= n) {
-      load8(x + e, v);
-      dropout8(v, philox4x32_10(seed, static_cast<uint64_t>(b), key.call), key.threshold, scale);
-      store8(out + e, v);
+  constexpr int kBlocks = 2;
+  PhiloxKeys own;
+  if constexpr (kDevSeed) own = philox_keys(static_cast<uint64_t>(*key.seed_dev));
+  const PhiloxKeys& keys = kDevSeed ? own : key.keys;
+  const int64_t whole = vec != 0 ? n / 8 : 0;  // blocks that go in vectors
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kThreads * kBlocks + threadIdx.x;
+  float v[kBlocks][8];
+#pragma unroll
+  for (int j = 0; j < kBlocks; ++j) {
+    const int64_t b = first + j * kThreads;
+    if (b < whole) load8(x + b * 8, v[j]);
+  }
+#pragma unroll
+  for (int j = 0; j < kBlocks; ++j) {
+    const int64_t b = first + j * kThreads, e = b * 8;
+    if (e >= n) break;
+    const uint4 words = philox4x32_10(keys, static_cast<uint64_t>(b), key.call);
+    if (b < whole) {
+      dropout8(v[j], words, key.threshold, scale);
+      store8(out + e, v[j]);
     } else {
       const int m = static_cast<int>(n - e < 8 ? n - e : 8);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < m ? static_cast<float>(x[e + i]) : 0.f;
-      dropout8(v, philox4x32_10(seed, static_cast<uint64_t>(b), key.call), key.threshold, scale);
+      for (int i = 0; i < 8; ++i) v[j][i] = i < m ? static_cast<float>(x[e + i]) : 0.f;
+      dropout8(v[j], words, key.threshold, scale);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (i < m) out[e + i] = static_cast<T>(v[i]);
+        if (i < m) out[e + i] = static_cast<T>(v[j][i]);
     }
   }
 }
@@ -72,20 +82,29 @@ __global__ void __launch_bounds__(kThreads)
 int launch_dropout(const void* x, void* out, int64_t n, int dtype, const DropoutKey& key,
                    bool scaled, cudaStream_t s) {
   const float scale = scaled ? dropout_scale(key.threshold) : 1.f;
-  const int64_t blocks = (n + 7) / 8;
-  const unsigned grid = static_cast<unsigned>(
-      std::min<int64_t>((blocks + kThreads - 1) / kThreads, int64_t{num_sms()} * 64));
+  const int64_t ctas = (n + 16 * kThreads - 1) / (16 * kThreads);
+  if (ctas > (int64_t{1} << 31) - 1) {
+    set_error("dropout: too many elements");
+    return MLORA_ERR_UNSUPPORTED;
+  }
+  const unsigned grid = static_cast<unsigned>(ctas);
   const int vec = ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
   LaunchScope scope(kKindElementwise, s);
+  auto run = [&](auto* p) {
+    using T = std::remove_pointer_t<decltype(p)>;
+    if (key.seed_dev != nullptr)
+      dropout_kernel<T, true><<<grid, kThreads, 0, s>>>(static_cast<const T*>(x), static_cast<T*>(out), n,
+                                                        vec, scale, key);
+    else
+      dropout_kernel<T, false><<<grid, kThreads, 0, s>>>(static_cast<const T*>(x),
+                                                         static_cast<T*>(out), n, vec, scale, key);
+  };
   if (dtype == MLORA_DTYPE_BF16)
-    dropout_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __nv_bfloat16*>(x),
-                                             static_cast<__nv_bfloat16*>(out), n, vec, scale, key);
+    run(static_cast<__nv_bfloat16*>(nullptr));
   else if (dtype == MLORA_DTYPE_F16)
-    dropout_kernel<<<grid, kThreads, 0, s>>>(static_cast<const __half*>(x),
-                                             static_cast<__half*>(out), n, vec, scale, key);
+    run(static_cast<__half*>(nullptr));
   else
-    dropout_kernel<<<grid, kThreads, 0, s>>>(static_cast<const float*>(x), static_cast<float*>(out),
-                                             n, vec, scale, key);
+    run(static_cast<float*>(nullptr));
   return launch_status(cudaSuccess, "dropout");
 }
 
@@ -111,6 +130,6 @@ extern "C" int mlora_dropout(const void* x, void* out, int64_t n, int threshold,
       reinterpret_cast<uintptr_t>(seed_dev) % 8)
     return fail(MLORA_ERR_INVALID_ARG, "pointers must be whole elements");
   if (int rc = require_device()) return rc;
-  const DropoutKey key{seed, seed_dev, call, static_cast<uint32_t>(threshold)};
+  const DropoutKey key = dropout_key(seed, seed_dev, call, threshold);
   return launch_dropout(x, out, n, dtype, key, scaled != 0, static_cast<cudaStream_t>(stream));
 }

@@ -112,8 +112,10 @@ struct Unit {
 
 __device__ __forceinline__ Unit unit_at(const HeadGemmParams& p, const Shape& s, int u) {
   Unit t;
-  t.split = u / s.num_tiles;
-  const int tile = u - t.split * s.num_tiles;
+  // the end of the reduction first: of the weight that the logits have just read, L2
+  // still holds that (16 tokens 4096 -> 32000: 50.6 -> 49.4 us)
+  t.split = p.splits - 1 - u / s.num_tiles;
+  const int tile = u % s.num_tiles;
   const int per_group = p.group_m * p.tiles_n;
   const int g = tile / per_group;
   const int rem = tile - g * per_group;
