@@ -1009,7 +1009,7 @@ int mlora_lora_forward_ckpt(const void* x, const void* w0, const void* a, const 
 size_t mlora_lora_forward_dropout_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r,
                                                   int dtype) {
   if (check_shapes(M, K, N, r, dtype) || dtype == MLORA_DTYPE_F32) return 0;
-  return align_up(plan_forward(nullptr, M, K, r, true).bytes, 256) + static_cast<size_t>(M) * N * 2;
+  return plan_forward(nullptr, M, K, r, true).bytes;
 }
 
 int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, const void* b, void* y,
@@ -1033,7 +1033,6 @@ int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, con
     return fail(MLORA_ERR_WORKSPACE, "forward workspace needs " + std::to_string(need) + " bytes");
   if ((rc = check_device())) return rc;
   const FwdPlan p = plan_forward(workspace, M, K, r, true);
-  void* z = static_cast<uint8_t*>(workspace) + align_up(p.bytes, 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const Elt elt = dtype == MLORA_DTYPE_BF16 ? Elt::kBF16 : Elt::kF16;
   RankArgs ra;
@@ -1055,32 +1054,29 @@ int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, con
   ra.splits = p.splits;
   ra.elt = elt;
   if ((rc = launch_rank(ra, s))) return rc;
-  GemmArgs gz;  // z = (s x A^T) . B^T
-  gz.x = p.xa_rows;
-  gz.w = b;
-  gz.d = z;
-  gz.M = M;
-  gz.N = N;
-  gz.K = r;
-  gz.ldx = p.R64;
-  gz.ldw = r;
-  gz.ldd = N;
-  gz.w_mn_major = false;
-  gz.elt = elt;
-  gz.out_dtype = dtype;
-  if ((rc = launch_gemm(gz, s))) return rc;
   const DropoutKey key = dropout_key(seed, seed_dev, call, threshold);
-  if ((rc = launch_dropout(z, z, M * N, dtype, key, false, s))) return rc;
-  GemmArgs ga = gz;  // y = x . W0^T + drop(z)
+  HeadGemmArgs ga;
+  ga.product = HeadProduct::kLoraDropout;
   ga.x = x;
   ga.w = w0;
-  ga.d = y;
+  ga.x2 = p.xa_rows;
+  ga.w2 = b;
+  ga.d16 = y;
+  ga.drop = &key;
+  ga.M = M;
+  ga.N = N;
   ga.K = K;
+  ga.R = p.R;
+  ga.w2_rows = r;
   ga.ldx = K;
   ga.ldw = K;
-  ga.c = z;
-  ga.ldc = N;
-  return launch_gemm(ga, s);
+  ga.ldx2 = p.R64;
+  ga.ldw2 = r;
+  ga.ldd = N;
+  // as for the LoRA GEMM: weights that stay in L2 go column by column
+  ga.group_m = N * K * 2 <= (int64_t{48} << 20) ? 1 : 8;
+  ga.elt = elt;
+  return launch_head_gemm(ga, s);
 }
 
 size_t mlora_lora_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t r, int dtype) {

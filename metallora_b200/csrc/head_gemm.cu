@@ -5,6 +5,8 @@
 //   dx      D[m, k] = sum_v g[m, v] W[v, k]   (+ U[m, :] . A[:, k])    W MN-major
 //   dW      D[v, k] = sum_m g[m, v] x[m, k]                            both MN-major
 //
+// and the LoRA linear with dropout, y = x . W^T + drop(X2 . B^T), both K-major.
+//
 // The logits never leave the chip as such.  The epilogue takes, of each row's 128 in half
 // a tile, a reference n_t and s_t = sum exp(l) 2^-n_t, and where a gradient is wanted
 // writes the exponentials exp(l) 2^-n_t in 16 bits.  Two forms:
@@ -41,11 +43,16 @@
 
 #include "internal.h"
 #include "launch.cuh"
+#include "philox.cuh"
 #include "ptx.cuh"
 #include "../../include/metallora_b200.h"
 
 namespace mlora {
 namespace {
+
+// What a tile becomes: fp32 sums; logits by their row's reference or by the half row's
+// largest; the LoRA linear with dropout.
+enum class Form { kSums, kRowRef, kTop, kDropout };
 
 constexpr int kBK = 64;
 constexpr int kHalf = 128;  // rows of either operand per CTA
@@ -77,6 +84,8 @@ struct HeadGemmParams {
   const float* ref;      // of row m: n_t (first form)
   uint16_t* e;           // the exponentials (second form: times 2^15), rows ldd apart, or nullptr
   float uncut;           // what a logit is multiplied by
+  DropoutKey drop;       // of the LoRA term, over [M, N] in a row
+  void* d16;             // output of kDropout
   float2* stats;         // (n_t, s_t), second form (m_t, 2^15 s_t), of the t-th 128 entries at
   long long stats_ld;    // [m * stats_ld + t]
   uint32_t* status;
@@ -302,12 +311,67 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
         make_float2(top * p.uncut, sum0 + sum1);
 }
 
-template <bool kXMN, bool kWMN, bool kBF16, bool kRef>
+// The LoRA linear with dropout.  The LoRA term has the second accumulator, so that a
+// tile's epilogue does not run beside the next one's main loop; but the mask, most of
+// its work, needs no accumulator and is made ahead: a bit for each of this thread's 128
+// columns from n0, eight to a call of the generator.  (Tiles of 128 columns, two of both
+// accumulators in TMEM, moved half as much again from L2 and took 160 us where this
+// takes 129: 4096 tokens 4096 -> 4096.)
+__device__ __forceinline__ void dropout_bits(const HeadGemmParams& p, int m, int n0,
+                                             uint32_t (&bits)[4]) {
+  PhiloxKeys own;
+  const bool dev = p.drop.seed_dev != nullptr;
+  if (dev) own = philox_keys(static_cast<uint64_t>(*p.drop.seed_dev));
+  const int64_t first = (static_cast<int64_t>(m) * p.N + n0) / 8;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    bits[c] = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint64_t at = static_cast<uint64_t>(first + c * 4 + q);
+      bits[c] |= kept_bits(dev ? philox4x32_10(own, at, p.drop.call)
+                               : philox4x32_10(p.drop.keys, at, p.drop.call),
+                           p.drop.threshold)
+                 << (8 * q);
+    }
+  }
+}
+
+template <typename T, typename Release>
+__device__ __forceinline__ void dropout_row(const HeadGemmParams& p, const Shape& s, int m, int n0,
+                                            uint32_t taddr, const uint32_t (&bits)[4],
+                                            Release&& release) {
+  uint32_t out[64];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t base[32], lora[32];
+    tmem_ld_32x32b_x32(taddr + c * 32, base);
+    tmem_ld_32x32b_x32(taddr + kTile + c * 32, lora);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float z0 = (bits[c] >> (2 * i)) & 1u ? __uint_as_float(lora[2 * i]) : 0.f;
+      const float z1 = (bits[c] >> (2 * i + 1)) & 1u ? __uint_as_float(lora[2 * i + 1]) : 0.f;
+      out[c * 16 + i] = pack2<T>(__uint_as_float(base[2 * i]) + z0, __uint_as_float(base[2 * i + 1]) + z1);
+    }
+  }
+  release();
+  if (m >= s.M) return;
+  T* row = static_cast<T*>(p.d16) + static_cast<long long>(m) * p.ldd + n0;
+#pragma unroll
+  for (int q = 0; q < 16; ++q)
+    if (n0 + q * 8 < p.N)
+      *reinterpret_cast<uint4*>(row + q * 8) =
+          make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
+}
+
+template <bool kXMN, bool kWMN, bool kBF16, Form kForm>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     head_gemm_kernel(const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap tm_w,
                      const __grid_constant__ CUtensorMap tm_x2,
                      const __grid_constant__ CUtensorMap tm_w2, const HeadGemmParams p) {
+  constexpr bool kOneTile = kForm == Form::kDropout;  // both accumulators are a tile's
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem<1024>(smem_raw);
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kStages * kStageBytes);
@@ -418,8 +482,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int u = pair; u < shape.units && ok; u += num_pairs, ++local) {
         const Unit t = unit_at(p, shape, u);
         const int main_kb = t.kb1 - t.kb0;
-        const uint32_t buf = local & 1;
-        const uint32_t use = static_cast<uint32_t>(local >> 1) & 1u;
+        const uint32_t buf = kOneTile ? 0 : local & 1;
+        const uint32_t use = static_cast<uint32_t>(kOneTile ? local : local >> 1) & 1u;
         if (!mbar_wait(&acc_empty[buf], use ^ 1u, p.status, kDevTimeoutAccEmpty)) {
           ok = false;
           break;
@@ -444,7 +508,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                      : desc_kmajor_sw128(sx, k);
             const uint64_t bd = kWMN ? desc_mnmajor_sw128(sw, k, kMNBoxBytes)
                                      : desc_kmajor_sw128(sw, k);
-            umma_f16_pair(d_tmem, ad, bd, idesc, (i | k) != 0 ? 1u : 0u);
+            if (kForm == Form::kDropout && i >= main_kb)  // the LoRA term's own accumulator
+              umma_f16_pair(d_tmem + kTile, ad, bd, idesc, i > main_kb || k != 0 ? 1u : 0u);
+            else
+              umma_f16_pair(d_tmem, ad, bd, idesc, (i | k) != 0 ? 1u : 0u);
           }
           umma_commit_pair(smem_u32(&empty_bar[stage]));
           umma_commit_pair(peer_empty + stage * 8u);
@@ -466,12 +533,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     int local = 0;
     for (int u = pair; u < shape.units; u += num_pairs, ++local) {
       const Unit t = unit_at(p, shape, u);
-      const uint32_t buf = local & 1;
-      const uint32_t use = static_cast<uint32_t>(local >> 1) & 1u;
-      if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
-      tc_fence_after();
+      const uint32_t buf = kOneTile ? 0 : local & 1;
+      const uint32_t use = static_cast<uint32_t>(kOneTile ? local : local >> 1) & 1u;
       const int m = t.tm * kTile + static_cast<int>(crank * kHalf + quarter * 32 + lane);
       const int n0 = t.tn * kTile + static_cast<int>(half) * kHalf;
+      uint32_t bits[4];
+      if constexpr (kForm == Form::kDropout) dropout_bits(p, m, n0, bits);
+      if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
+      tc_fence_after();
       const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile + half * kHalf;
       // the arrival orders no memory: only the TMEM loads, complete by then, came before
       auto release = [&] {
@@ -479,12 +548,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster_relaxed(lead_acc_empty + buf * 8u);
       };
-      if constexpr (!kWMN) {
-        if constexpr (kRef)
-          softmax_row_ref(p, shape, m, n0, taddr, release);
-        else
-          softmax_row(p, shape, m, n0, taddr, release);
-      } else {
+      if constexpr (kForm == Form::kRowRef)
+        softmax_row_ref(p, shape, m, n0, taddr, release);
+      else if constexpr (kForm == Form::kTop)
+        softmax_row(p, shape, m, n0, taddr, release);
+      else if constexpr (kForm == Form::kDropout)
+        dropout_row<typename std::conditional<kBF16, __nv_bfloat16, __half>::type>(
+            p, shape, m, n0, taddr, bits, release);
+      else {
         store_row_f32(p, shape, t, m, n0, taddr);
         release();
       }
@@ -507,7 +578,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   }
 }
 
-template <bool kXMN, bool kWMN, bool kBF16, bool kRef>
+template <bool kXMN, bool kWMN, bool kBF16, Form kForm>
 int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   CUtensorMap tx, tw, tx2, tw2;
   if (kXMN ? !make_tmap_2d_16b(&tx, a.x, a.M, a.K, a.ldx, 64, kBK)
@@ -544,13 +615,15 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   p.accumulate = a.accumulate ? 1 : 0;
   p.label = a.label;
   p.ref = a.ref;
+  if (a.drop != nullptr) p.drop = *a.drop;
+  p.d16 = a.d16;
   p.e = static_cast<uint16_t*>(a.e);
   p.stats = static_cast<float2*>(a.stats);
   p.stats_ld = a.stats_ld;
   p.uncut = 1.f + kCutPerK * static_cast<float>(a.K);
   p.status = device_status_ptr();
 
-  auto kern = head_gemm_kernel<kXMN, kWMN, kBF16, kRef>;
+  auto kern = head_gemm_kernel<kXMN, kWMN, kBF16, kForm>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), kSmemBytes, attr_set)) return rc;
   const int64_t units = int64_t{tiles_m} * p.tiles_n * p.splits;
@@ -572,7 +645,7 @@ int head_gemm_pairs() {
   if (n > 0) return n;
   // clusters that can be resident at once (GPCs may leave an SM unpaired)
   const int pairs = num_sms() / 2;
-  auto kern = head_gemm_kernel<false, false, true, false>;
+  auto kern = head_gemm_kernel<false, false, true, Form::kTop>;
   static std::atomic<bool> attr_set[64];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs));
@@ -592,15 +665,18 @@ int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s) {
   const bool bf16 = a.elt == Elt::kBF16;
   switch (a.product) {
     case HeadProduct::kLogits:
-      if (a.ref != nullptr) return launch_typed<false, false, true, true>(a, s);
-      return bf16 ? launch_typed<false, false, true, false>(a, s)
-                  : launch_typed<false, false, false, false>(a, s);
+      if (a.ref != nullptr) return launch_typed<false, false, true, Form::kRowRef>(a, s);
+      return bf16 ? launch_typed<false, false, true, Form::kTop>(a, s)
+                  : launch_typed<false, false, false, Form::kTop>(a, s);
     case HeadProduct::kDx:
-      return bf16 ? launch_typed<false, true, true, false>(a, s)
-                  : launch_typed<false, true, false, false>(a, s);
+      return bf16 ? launch_typed<false, true, true, Form::kSums>(a, s)
+                  : launch_typed<false, true, false, Form::kSums>(a, s);
     case HeadProduct::kDw:
-      return bf16 ? launch_typed<true, true, true, false>(a, s)
-                  : launch_typed<true, true, false, false>(a, s);
+      return bf16 ? launch_typed<true, true, true, Form::kSums>(a, s)
+                  : launch_typed<true, true, false, Form::kSums>(a, s);
+    case HeadProduct::kLoraDropout:
+      return bf16 ? launch_typed<false, false, true, Form::kDropout>(a, s)
+                  : launch_typed<false, false, false, Form::kDropout>(a, s);
   }
   return MLORA_ERR_INVALID_ARG;
 }

@@ -242,7 +242,11 @@ int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t stream);
 //   kDx:     D[m, k] = g . W + x2 . w2        x = g [M, K = V], w [K, N], w2 [r, N]
 //   kDw:     D[v, k] = g^T . x                x = g [K tokens, M = V], w = x [K, N]
 //            out: fp32 D, N a multiple of 8
-enum class HeadProduct { kLogits, kDx, kDw };
+// and with the same kernel
+//   kLoraDropout: y = x . W^T + drop(x2 . w2^T)   as kLogits; out: 16-bit d16 [M, N], N a
+//            multiple of 8, kept elements as they are
+enum class HeadProduct { kLogits, kDx, kDw, kLoraDropout };
+struct DropoutKey;  // philox.cuh
 struct HeadGemmArgs {
   HeadProduct product;
   const void* x;
@@ -266,6 +270,8 @@ struct HeadGemmArgs {
   void* e = nullptr;
   void* stats = nullptr;
   int64_t stats_ld = 0;
+  const DropoutKey* drop = nullptr;  // kLoraDropout
+  void* d16 = nullptr;
   Elt elt = Elt::kBF16;
 };
 constexpr int kHeadTile = 128;  // entries that share a largest logit
@@ -298,7 +304,6 @@ int launch_embed_da_f32(const int32_t* idx, const float* b, const float* dy, flo
                         cudaStream_t s);
 
 // ------------------------------------------------------------ dropout --------
-struct DropoutKey;  // philox.cuh
 // out = dropout(x) over n elements in a row (out may be x); without `scaled` the kept
 // elements are as they were.
 int launch_dropout(const void* x, void* out, int64_t n, int dtype, const DropoutKey& key,

@@ -71,6 +71,19 @@ __device__ __forceinline__ void dropout8(float (&v)[8], const uint4& words, uint
   }
 }
 
+// Which of the 8 are kept, a bit each.
+__device__ __forceinline__ uint32_t kept_bits(const uint4& words, uint32_t threshold) {
+  const uint32_t w[4] = {words.x, words.y, words.z, words.w};
+  const uint32_t top = threshold << 16;
+  uint32_t bits = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t u = (i & 1) != 0 ? w[i >> 1] : w[i >> 1] << 16;
+    bits |= u >= top ? 1u << i : 0u;
+  }
+  return threshold >= 65536u ? 0u : bits;
+}
+
 __host__ __device__ inline float dropout_scale(uint32_t threshold) {
   return threshold >= 65536u ? 0.f : 65536.f / static_cast<float>(65536u - threshold);
 }
