@@ -799,6 +799,24 @@ def linear_cross_entropy_fwd(x2d: torch.Tensor, w: torch.Tensor, labels: torch.T
     return loss, state
 
 
+def linear_cross_entropy_dx(grad: torch.Tensor, state: torch.Tensor, w: torch.Tensor, M: int,
+                            reduction: str) -> torch.Tensor:
+    """``linear_cross_entropy_bwd`` for the gradient of x alone, from the forward's own
+    state and (contiguous) w and an upstream gradient like its loss."""
+    V, K = w.shape
+    dx = w.new_empty((M, K))
+    if M:
+        if not grad.is_contiguous():
+            grad = grad.contiguous()
+        st = _lib.load().mlora_linear_cross_entropy_backward(
+            state.data_ptr(), state.numel(), grad.data_ptr(), reduction == "none", reduction == "mean",
+            w.data_ptr(), dx.data_ptr(), None, None, 0, 0, None, M, K, V, 0, _DT[w.dtype],
+            _lib.HEAD_GRAD_X, _stream())
+        if st:
+            _lib.check(st, "mlora_linear_cross_entropy_backward")
+    return dx
+
+
 def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.Tensor, M: int,
                              r: int, reduction: str, grads: int,
                              da_out: torch.Tensor | None = None,
@@ -857,28 +875,53 @@ def _table_index(indices: torch.Tensor) -> torch.Tensor:
     return indices.contiguous()
 
 
-def embedding_fwd(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-    """scale * table[idx] for every index, [*indices.shape, D] (bf16, fp16 or fp32); an
-    index outside the table gives a zero row and device status 0x107."""
+def embedding_run(indices: torch.Tensor, table: torch.Tensor, scale: float):
+    """``embedding_fwd``'s output, its indices as the kernels take them, and the rest of
+    ``embedding_bwd_run``'s arguments up to the scale."""
     _need_here(table, indices)
     code = _dtype_code(table)
     if table.dim() != 2:
         raise ShapeError(f"the table must be [V, D], got {tuple(table.shape)}")
     V, D = table.shape
     idx = _table_index(indices)
+    T = idx.numel()
     table = table.contiguous()
     out = table.new_empty((*idx.shape, D))
-    if out.numel() == 0:
-        return out
-    st = _lib.load().mlora_embedding_forward(idx.data_ptr(), table.data_ptr(), out.data_ptr(),
-                                             idx.numel(), V, D, float(scale), code, _stream())
-    _lib.check(st, "mlora_embedding_forward")
-    return out
+    if T and D:
+        st = _lib.load().mlora_embedding_forward(idx.data_ptr(), table.data_ptr(), out.data_ptr(), T, V,
+                                                 D, scale, code, _stream())
+        if st:
+            _lib.check(st, "mlora_embedding_forward")
+    return out, idx, (T, V, D, scale), code
+
+
+def embedding_fwd(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * table[idx] for every index, [*indices.shape, D] (bf16, fp16 or fp32); an
+    index outside the table gives a zero row and device status 0x107."""
+    return embedding_run(indices, table, float(scale))[0]
 
 
 @functools.lru_cache(maxsize=256)
 def _embedding_ws_bytes(T: int, D: int) -> int:
     return _lib.load().mlora_embedding_backward_workspace_bytes(T, D)
+
+
+def embedding_bwd_run(dy: torch.Tensor, idx: torch.Tensor, T: int, V: int, D: int, scale: float,
+                      padding_idx: int, code: int) -> torch.Tensor:
+    """The gradient of ``embedding_fwd``'s table from its own indices (a row of int64)
+    and a dy of its output's size, type and device; padding_idx < 0: none."""
+    if not dy.is_contiguous():
+        dy = dy.contiguous()
+    grad = dy.new_empty((V, D))
+    if T == 0 or D == 0:
+        return grad.zero_()
+    nbytes = _embedding_ws_bytes(T, D)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8)
+    st = _lib.load().mlora_embedding_backward(idx.data_ptr(), dy.data_ptr(), grad.data_ptr(), T, V, D,
+                                              scale, padding_idx, code, ws.data_ptr(), nbytes, _stream())
+    if st:
+        _lib.check(st, "mlora_embedding_backward")
+    return grad
 
 
 def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, scale: float = 1.0,
@@ -887,22 +930,11 @@ def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, 
     dy over each entry's tokens, in fp32 and in token order (the same bits in every
     run); zero for ``padding_idx``."""
     _need_here(dy, indices)
-    code = _dtype_code(dy)
     idx = _table_index(indices)
-    T, D, V = idx.numel(), dy.shape[-1], int(num_embeddings)
-    if dy.shape != (*idx.shape, D):
+    if dy.shape[:-1] != idx.shape:
         raise ShapeError(f"grad_output {tuple(dy.shape)} does not match indices {tuple(idx.shape)}")
-    dy = dy.contiguous()
-    grad = dy.new_empty((V, D))
-    if grad.numel() == 0 or T == 0:
-        return grad.zero_()
-    nbytes = _embedding_ws_bytes(T, D)
-    ws = dy.new_empty(nbytes, dtype=torch.uint8)
-    st = _lib.load().mlora_embedding_backward(idx.data_ptr(), dy.data_ptr(), grad.data_ptr(), T, V, D,
-                                              float(scale), -1 if padding_idx is None else padding_idx,
-                                              code, ws.data_ptr(), nbytes, _stream())
-    _lib.check(st, "mlora_embedding_backward")
-    return grad
+    return embedding_bwd_run(dy, idx, idx.numel(), int(num_embeddings), dy.shape[-1], float(scale),
+                             -1 if padding_idx is None else padding_idx, _dtype_code(dy))
 
 
 # ---------------------------------------------------------------- dropout --
@@ -927,22 +959,32 @@ def _drop_seed(seed) -> tuple[int, int | None]:
     return int(seed) & _U64, None
 
 
+def dropout_plan(x: torch.Tensor, p: float, seed, call: int = 0, scaled: bool = True) -> tuple:
+    """What ``dropout_run`` takes besides a tensor like x: all that is checked once for
+    the forward and its backward.  (A seed tensor has to outlive both.)"""
+    t = _drop_threshold(p)
+    _need_here(x)
+    s, s_dev = _drop_seed(seed)
+    return (x.numel(), t, scaled, s, s_dev, call & _U64, _dtype_code(x))
+
+
+def dropout_run(x: torch.Tensor, plan: tuple) -> torch.Tensor:
+    """The dropout of a tensor of the plan's size, type and device."""
+    if not x.is_contiguous():
+        x = x.contiguous()
+    out = torch.empty_like(x)
+    if plan[0]:
+        st = _lib.load().mlora_dropout(x.data_ptr(), out.data_ptr(), *plan, _stream())
+        if st:
+            _lib.check(st, "mlora_dropout")
+    return out
+
+
 def dropout(x: torch.Tensor, p: float, seed, call: int = 0, scaled: bool = True) -> torch.Tensor:
     """x with every element dropped (0) or scaled by the counter-based mask of ``seed``
     and ``call`` (see ``ops.dropout``); its gradient is the same call on dy.  Without
     ``scaled`` the kept elements are as they were."""
-    t = _drop_threshold(p)
-    _need_here(x)
-    code = _dtype_code(x)
-    s, s_dev = _drop_seed(seed)
-    x = x.contiguous()
-    out = torch.empty_like(x)
-    n = x.numel()
-    if n:
-        st = _lib.load().mlora_dropout(x.data_ptr(), out.data_ptr(), n, t, scaled, s, s_dev,
-                                       call & _U64, code, _stream())
-        _lib.check(st, "mlora_dropout")
-    return out
+    return dropout_run(x, dropout_plan(x, p, seed, call, scaled))
 
 
 def lora_linear_dropout_fwd(x2d: torch.Tensor, w0: torch.Tensor, a: torch.Tensor, b: torch.Tensor,

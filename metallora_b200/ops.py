@@ -127,14 +127,10 @@ class _LoRALinearFn(torch.autograd.Function):
         return dx, dw0, da, db, None, None, None, None
 
 
-def _once(backward):
-    """``once_differentiable`` where a second derivative may follow (create_graph), and
-    the backward itself, some microseconds shorter, where none can."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, grad):
-        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
-    return staticmethod(run)
+_once = torch.autograd.function.once_differentiable
+# whether a backward is to be differentiated again (create_graph); without that the
+# functions below skip what refuses it, some microseconds a call
+_grad_on = torch.is_grad_enabled
 
 
 def _keep_seed(ctx, seed, *tensors):
@@ -164,6 +160,7 @@ class _LoRADropoutFn(torch.autograd.Function):
         ctx.ab_dtypes = (a.dtype, b.dtype)
         return y
 
+    @staticmethod
     @_once
     def backward(ctx, dy):
         seed, (x2d, w0, a_c, b_c, saved) = _kept_seed(ctx)
@@ -421,8 +418,18 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         ctx.sink = sink
         return loss
 
-    @_once
+    @staticmethod
     def backward(ctx, grad):
+        state, w = ctx.saved_tensors
+        m, _, reduction, grads = ctx.plan
+        if grads == _lib.HEAD_GRAD_X and w.is_contiguous() and not _grad_on():  # a frozen head
+            return (_k.linear_cross_entropy_dx(grad, state, w, m, reduction), None, None, None, None,
+                    None)
+        return _LinearCrossEntropyFn._all(ctx, grad)
+
+    @staticmethod
+    @_once
+    def _all(ctx, grad):
         state, w = ctx.saved_tensors
         m, r, reduction, grads = ctx.plan
         sink = ctx.sink if grads & _lib.HEAD_GRAD_AB else None
@@ -481,14 +488,21 @@ def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,
 class _DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, call):
-        _keep_seed(ctx, seed)
-        ctx.plan = (p, call)
-        return _k.dropout(x, p, seed, call)
+        ctx.plan = plan = _k.dropout_plan(x, p, seed, call)
+        ctx.tensor = torch.is_tensor(seed)
+        if ctx.tensor:  # kept, and being written over before the backward noticed
+            ctx.save_for_backward(seed)
+        return _k.dropout_run(x, plan)
 
-    @_once
+    @staticmethod
     def backward(ctx, dy):
-        p, call = ctx.plan
-        return _k.dropout(dy, p, _kept_seed(ctx)[0], call), None, None, None
+        if ctx.tensor:
+            ctx.saved_tensors
+        if _grad_on():
+            return _DropoutFn._guarded(ctx, dy)
+        return _k.dropout_run(dy, ctx.plan), None, None, None
+
+    _guarded = staticmethod(_once(lambda ctx, dy: (_k.dropout_run(dy, ctx.plan), None, None, None)))
 
 
 def dropout(x, p: float, seed, call: int = 0, training: bool = True):
@@ -512,15 +526,19 @@ def dropout(x, p: float, seed, call: int = 0, training: bool = True):
 class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, indices, table, scale, padding_idx):
-        ctx.save_for_backward(indices)
-        ctx.plan = (table.shape[0], scale, padding_idx)
-        return _k.embedding_fwd(indices, table, scale)
+        out, idx, sizes, code = _k.embedding_run(indices, table, scale)
+        ctx.save_for_backward(idx)
+        ctx.plan = (*sizes, padding_idx, code)
+        return out
 
-    @_once
+    @staticmethod
     def backward(ctx, dy):
-        indices, = ctx.saved_tensors
-        rows, scale, padding_idx = ctx.plan
-        return None, _k.embedding_bwd(dy, indices, rows, scale, padding_idx), None, None
+        if _grad_on():
+            return _EmbeddingFn._guarded(ctx, dy)
+        return None, _k.embedding_bwd_run(dy, *ctx.saved_tensors, *ctx.plan), None, None
+
+    _guarded = staticmethod(_once(lambda ctx, dy: (
+        None, _k.embedding_bwd_run(dy, *ctx.saved_tensors, *ctx.plan), None, None)))
 
 
 def embedding(indices, table, scale: float = 1.0, padding_idx: int | None = None):
@@ -538,4 +556,4 @@ def embedding(indices, table, scale: float = 1.0, padding_idx: int | None = None
         if not -rows <= padding_idx < rows:
             raise ConfigurationError(f"padding_idx {padding_idx} is outside the table's {rows} rows")
         padding_idx = int(padding_idx) % rows
-    return _EmbeddingFn.apply(indices, table, float(scale), padding_idx)
+    return _EmbeddingFn.apply(indices, table, float(scale), -1 if padding_idx is None else padding_idx)
