@@ -2,7 +2,7 @@
 // CTA pairs:
 //
 //   logits  l[m, v] = sum_k x[m, k] W[v, k]   (+ X2[m, :] . B[v, :])   both K-major
-//   dx      D[m, k] = sum_v g[m, v] W[v, k]   (+ U[m, :] . A[:, k])    W MN-major
+//   dx      D[k, m] = sum_v W[v, k] g[m, v]   (+ A[:, k] . U[m, :])    W MN-major
 //   dW      D[v, k] = sum_m g[m, v] x[m, k]                            both MN-major
 //
 // and the LoRA linear with dropout, y = x . W^T + drop(X2 . B^T), both K-major.
@@ -31,8 +31,12 @@
 // and holds its own 128 rows of the fp32 accumulator, two of them in TMEM, so that
 // the epilogue of one tile runs beside the main loop of the next.  The roles of the
 // warps are those of the LoRA GEMM (tc_gemm.cu).  What is new here:
+//   * a tile may have fewer columns (a multiple of 32, which the instruction's time goes
+//     by): those of the logits so that whole waves of tiles cover the vocabulary, those of
+//     dx, whose columns are the tokens, as many as the counted ones need (412 tokens are
+//     two tiles of 224 columns, not two of 256 rows);
 //   * the number of counted tokens is read on the device: it bounds the rows of D
-//     (logits, dx) or the reduction (dW), so that tokens that do not count cost
+//     (logits), its columns (dx) or the reduction (dW), so that tokens that do not count cost
 //     nothing and no host waits for their number;
 //   * the reduction can be cut into `splits` ranges, each with its own fp32 copy of D
 //     (dx of few tokens has few tiles and a reduction over the whole vocabulary);
@@ -50,9 +54,9 @@
 namespace mlora {
 namespace {
 
-// What a tile becomes: fp32 sums; logits by their row's reference or by the half row's
+// What a tile becomes: fp32 sums, as they lie or with D's columns as rows; logits by their row's reference or by the half row's
 // largest; the LoRA linear with dropout.
-enum class Form { kSums, kRowRef, kTop, kDropout };
+enum class Form { kSums, kTransposed, kRowRef, kTop, kDropout };
 
 constexpr int kBK = 64;
 constexpr int kHalf = 128;  // rows of either operand per CTA
@@ -72,10 +76,10 @@ constexpr size_t kSmemBytes = 1024 + kStages * kStageBytes + 256;
 struct HeadGemmParams {
   int M, N;  // of D; at most, where `rows` bounds them
   int num_kb_main, num_kb_extra, R;
-  int tiles_n, splits, group_m;
+  int tile_n;  // columns of a tile (kTransposed: by the counted tokens)
+  int splits, group_m;
   const int32_t* rows;  // counted tokens (device), of which those from row0 on are meant
   int row0;
-  int rows_on_k;  // they bound the reduction, else the rows of D
   float* d;
   long long ldd, split_stride;
   int accumulate;
@@ -86,28 +90,39 @@ struct HeadGemmParams {
   float uncut;           // what a logit is multiplied by
   DropoutKey drop;       // of the LoRA term, over [M, N] in a row
   void* d16;             // output of kDropout
-  float2* stats;         // (n_t, s_t), second form (m_t, 2^15 s_t), of the t-th 128 entries at
+  float2* stats;         // (n_t, s_t), second form (m_t, 2^15 s_t), of the t-th half tile at
   long long stats_ld;    // [m * stats_ld + t]
   uint32_t* status;
 };
 
 struct Shape {
-  int M, num_kb, tiles_m, num_tiles, units;
+  int M, N, num_kb, tile_n, tiles_m, tiles_n, num_tiles, units;
 };
 
+// kRows: what the counted tokens bound.
+enum class Bound { kRows, kColumns, kReduction };
+
+template <Bound kBound>
 __device__ __forceinline__ Shape device_shape(const HeadGemmParams& p) {
   Shape s;
   s.M = p.M;
+  s.N = p.N;
   s.num_kb = p.num_kb_main;
+  s.tile_n = p.tile_n;
   if (p.rows != nullptr) {
     const int n = max(*p.rows - p.row0, 0);
-    if (p.rows_on_k)
+    if (kBound == Bound::kReduction)
       s.num_kb = min(s.num_kb, (n + kBK - 1) / kBK);
-    else
+    else if (kBound == Bound::kRows)
       s.M = min(s.M, n);
+    else
+      s.N = min(s.N, n);
   }
   s.tiles_m = (s.M + kTile - 1) / kTile;
-  s.num_tiles = s.tiles_m * p.tiles_n;
+  s.tiles_n = (s.N + s.tile_n - 1) / s.tile_n;
+  if (kBound == Bound::kColumns && s.tiles_n > 0)  // the same number, as narrow as can be
+    s.tile_n = ((s.N + s.tiles_n - 1) / s.tiles_n + 31) / 32 * 32;
+  s.num_tiles = s.tiles_m * s.tiles_n;
   s.units = s.num_tiles * p.splits;
   return s;
 }
@@ -125,7 +140,7 @@ __device__ __forceinline__ Unit unit_at(const HeadGemmParams& p, const Shape& s,
   // still holds that (16 tokens 4096 -> 32000: 50.6 -> 49.4 us)
   t.split = p.splits - 1 - u / s.num_tiles;
   const int tile = u % s.num_tiles;
-  const int per_group = p.group_m * p.tiles_n;
+  const int per_group = p.group_m * s.tiles_n;
   const int g = tile / per_group;
   const int rem = tile - g * per_group;
   const int rows = min(p.group_m, s.tiles_m - g * p.group_m);
@@ -170,22 +185,40 @@ __device__ __forceinline__ void store_row_f32(const HeadGemmParams& p, const Sha
   }
 }
 
+// This thread's row m of the accumulator as a column of the output: D's column n, a
+// token, is a row there, and a warp's 32 values of it lie side by side.
+__device__ __forceinline__ void store_column_f32(const HeadGemmParams& p, const Shape& s,
+                                                 const Unit& t, int m, int n0, uint32_t taddr) {
+  const int width = min(s.tile_n / 2, s.N - n0);
+  float* dst = p.d + t.split * p.split_stride + static_cast<long long>(n0) * p.ldd + m;
+#pragma unroll 1
+  for (int c = 0; c < width; c += 32) {
+    uint32_t r[32];
+    tmem_ld_32x32b_x32(taddr + c, r);
+    tmem_ld_wait();
+    if (m >= s.M) continue;
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (c + i < width) dst[(c + i) * p.ldd] = __uint_as_float(r[i]);
+  }
+}
+
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 
-// Logits past the vocabulary, and the label's, count as -inf (`any`: there are some
-// among the warp's).
+// Logits past the half row or the vocabulary, and the label's, count as -inf (`any`:
+// there is a label among the warp's).
 __device__ __forceinline__ void mask_logits(uint32_t (&r)[32], int c, int width, int y, bool any) {
-  if (!any) return;
+  if (!any && c + 32 <= width) return;
 #pragma unroll
   for (int i = 0; i < 32; ++i)
     if (c + i >= width || c + i == y) r[i] = __float_as_uint(-INFINITY);
 }
 
-// First form: this thread's half row of a tile of logits (128 entries from n0).  One
+// First form: this thread's half row of a tile of logits (up to 128 entries from n0).  One
 // pass with the row's reference; the largest logit is only looked for where it fails.
 template <typename Release>
 __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const Shape& s, int m,
@@ -197,9 +230,8 @@ __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const S
   const bool live = m < s.M;
   const int y = live ? p.label[m] - n0 : -1;
   float n = live ? p.ref[m] : 0.f;
-  const int width = p.N - n0;  // of these columns, those in the vocabulary
-  const bool any = width < kHalf || __any_sync(0xffffffffu, static_cast<uint32_t>(y) <
-                                                                static_cast<uint32_t>(kHalf));
+  const int half = s.tile_n / 2, width = min(half, p.N - n0);  // columns that are there
+  const bool any = __any_sync(0xffffffffu, static_cast<uint32_t>(y) < static_cast<uint32_t>(width));
   const float log2e = kLog2e * p.uncut;
   uint32_t v[kHalf / 2];
   float sum = 0.f;
@@ -248,13 +280,13 @@ __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const S
     uint16_t* row = p.e + static_cast<long long>(m) * p.ldd + n0;
 #pragma unroll
     for (int c = 0; c < 8; ++c)
-      if (n0 + c * 16 < p.ldd) {
+      if (c * 16 < half && n0 + c * 16 < p.ldd) {
         const uint32_t q[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
                                v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
         st_global_32b(row + c * 16, q);
       }
   }
-  p.stats[static_cast<long long>(m) * p.stats_ld + n0 / kHalf] = make_float2(n, sum);
+  p.stats[static_cast<long long>(m) * p.stats_ld + n0 / half] = make_float2(n, sum);
 }
 
 // Second form: all of the half row in registers: largest, exponentials, their sum.  `release` hands the accumulator back
@@ -271,11 +303,10 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
   for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(taddr + c * 32, r[c]);
   const bool live = m < s.M;
   const int y = live ? p.label[m] - n0 : -1;
-  const int width = p.N - n0;  // of these columns, those in the vocabulary
+  const int half = s.tile_n / 2, width = min(half, p.N - n0);  // columns that are there
   tmem_ld_wait();
   release();
-  const bool any = width < kHalf || __any_sync(0xffffffffu, static_cast<uint32_t>(y) <
-                                                                static_cast<uint32_t>(kHalf));
+  const bool any = __any_sync(0xffffffffu, static_cast<uint32_t>(y) < static_cast<uint32_t>(width));
 #pragma unroll
   for (int c = 0; c < 4; ++c) mask_logits(r[c], c * 32, width, y, any);
   float t0 = -INFINITY, t1 = -INFINITY;
@@ -304,10 +335,11 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
       sum1 += b;
       v[i] = pack2<__half>(a, b);
     }
-    if (live && p.e != nullptr && n0 + c * 16 < p.ldd) st_global_32b(row + c * 16, v);
+    if (live && p.e != nullptr && c * 16 < half && n0 + c * 16 < p.ldd)
+      st_global_32b(row + c * 16, v);
   }
   if (live)
-    p.stats[static_cast<long long>(m) * p.stats_ld + n0 / kHalf] =
+    p.stats[static_cast<long long>(m) * p.stats_ld + n0 / half] =
         make_float2(top * p.uncut, sum0 + sum1);
 }
 
@@ -417,7 +449,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   grid_wait();  // every operand but the weight is the kernels' before; in every role
   launch_dependents();
-  const Shape shape = device_shape(p);
+  constexpr Bound kBound = kForm == Form::kTransposed ? Bound::kColumns
+                           : kForm == Form::kSums     ? Bound::kReduction
+                                                      : Bound::kRows;
+  const Shape shape = device_shape<kBound>(p);
+  const int half_n = shape.tile_n / 2;
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer --
@@ -431,7 +467,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       for (int u = pair; u < shape.units && ok; u += num_pairs) {
         const Unit t = unit_at(p, shape, u);
         const int m0 = t.tm * kTile + static_cast<int>(crank) * kHalf;
-        const int n0 = t.tn * kTile + static_cast<int>(crank) * kHalf;
+        const int n0 = t.tn * shape.tile_n + static_cast<int>(crank) * half_n;
         const int main_kb = t.kb1 - t.kb0;
         for (int i = 0; i < t.total; ++i) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, p.status, kDevTimeoutEmpty)) {
@@ -473,7 +509,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     // ------------------------------------------------- MMA (even CTA only) --
     if (lead && elect_one()) {
-      constexpr uint32_t idesc = make_idesc_f16(kTile, kTile, kXMN, kWMN, kBF16);
+      const uint32_t idesc =
+          make_idesc_f16(kTile, static_cast<uint32_t>(shape.tile_n), kXMN, kWMN, kBF16);
       const uint32_t peer_empty = mapa_shared(smem_u32(empty_bar), 1);
       const uint32_t peer_acc_full = mapa_shared(smem_u32(acc_full), 1);
       uint32_t stage = 0, phase = 0;
@@ -528,7 +565,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else {
     // ----------------------------------------------------------- epilogue --
     const uint32_t quarter = warp & 3u;  // TMEM lanes [32*quarter, 32*quarter+32)
-    const uint32_t half = (warp - 2u) >> 2;  // columns [128*half, 128*half+128)
+    const uint32_t half = (warp - 2u) >> 2;  // of the tile's columns
     const uint32_t lead_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
     int local = 0;
     for (int u = pair; u < shape.units; u += num_pairs, ++local) {
@@ -536,12 +573,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const uint32_t buf = kOneTile ? 0 : local & 1;
       const uint32_t use = static_cast<uint32_t>(kOneTile ? local : local >> 1) & 1u;
       const int m = t.tm * kTile + static_cast<int>(crank * kHalf + quarter * 32 + lane);
-      const int n0 = t.tn * kTile + static_cast<int>(half) * kHalf;
+      const int n0 = t.tn * shape.tile_n + static_cast<int>(half) * half_n;
       uint32_t bits[4];
       if constexpr (kForm == Form::kDropout) dropout_bits(p, m, n0, bits);
       if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile + half * kHalf;
+      const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile + half * half_n;
       // the arrival orders no memory: only the TMEM loads, complete by then, came before
       auto release = [&] {
         tc_fence_before();
@@ -556,7 +593,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         dropout_row<typename std::conditional<kBF16, __nv_bfloat16, __half>::type>(
             p, shape, m, n0, taddr, bits, release);
       else {
-        store_row_f32(p, shape, t, m, n0, taddr);
+        if constexpr (kForm == Form::kTransposed)
+          store_column_f32(p, shape, t, m, n0, taddr);
+        else
+          store_row_f32(p, shape, t, m, n0, taddr);
         release();
       }
     }
@@ -591,7 +631,9 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   tw2 = tw;
   if (a.R > 0) {
     const int64_t r64 = (a.R + 63) / 64 * 64;
-    if (!make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK, kHalf)) return MLORA_ERR_INVALID_ARG;
+    if (kXMN ? !make_tmap_2d_16b(&tx2, a.x2, a.M, a.x2_rows, a.ldx2, 64, kBK)
+             : !make_tmap_2d_16b(&tx2, a.x2, r64, a.M, a.ldx2, kBK, kHalf))
+      return MLORA_ERR_INVALID_ARG;
     if (kWMN ? !make_tmap_2d_16b(&tw2, a.w2, a.N, a.w2_rows, a.ldw2, 64, kBK)
              : !make_tmap_2d_16b(&tw2, a.w2, a.w2_rows, a.N, a.ldw2, kBK, kHalf))
       return MLORA_ERR_INVALID_ARG;
@@ -603,12 +645,12 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   p.R = static_cast<int>(a.R);
   p.num_kb_extra = static_cast<int>((a.R + kBK - 1) / kBK);
   const int tiles_m = static_cast<int>((a.M + kTile - 1) / kTile);
-  p.tiles_n = static_cast<int>((a.N + kTile - 1) / kTile);
+  p.tile_n = a.tile_n;
+  const int tiles_n = static_cast<int>((a.N + a.tile_n - 1) / a.tile_n);
   p.splits = a.splits;
   p.group_m = a.group_m < tiles_m ? a.group_m : tiles_m;
   p.rows = a.rows;
   p.row0 = static_cast<int>(a.row0);
-  p.rows_on_k = kXMN ? 1 : 0;
   p.d = a.d;
   p.ldd = a.ldd;
   p.split_stride = a.split_stride;
@@ -626,7 +668,7 @@ int launch_typed(const HeadGemmArgs& a, cudaStream_t stream) {
   auto kern = head_gemm_kernel<kXMN, kWMN, kBF16, kForm>;
   static std::atomic<bool> attr_set[64];
   if (int rc = set_max_smem(reinterpret_cast<const void*>(kern), kSmemBytes, attr_set)) return rc;
-  const int64_t units = int64_t{tiles_m} * p.tiles_n * p.splits;
+  const int64_t units = int64_t{tiles_m} * tiles_n * p.splits;
   const int pairs = head_gemm_pairs();
   const int grid = 2 * static_cast<int>(units < pairs ? units : pairs);
   LaunchScope scope(kKindGemm, stream);
@@ -669,8 +711,8 @@ int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s) {
       return bf16 ? launch_typed<false, false, true, Form::kTop>(a, s)
                   : launch_typed<false, false, false, Form::kTop>(a, s);
     case HeadProduct::kDx:
-      return bf16 ? launch_typed<false, true, true, Form::kSums>(a, s)
-                  : launch_typed<false, true, false, Form::kSums>(a, s);
+      return bf16 ? launch_typed<true, false, true, Form::kTransposed>(a, s)
+                  : launch_typed<true, false, false, Form::kTransposed>(a, s);
     case HeadProduct::kDw:
       return bf16 ? launch_typed<true, true, true, Form::kSums>(a, s)
                   : launch_typed<true, true, false, Form::kSums>(a, s);

@@ -268,6 +268,13 @@ __device__ __forceinline__ float row_loss_of(float gap, float s, float u) {
   return gap < 0.f || s == 0.f ? log1pf(u) : gap + logf(s + expf(-gap));
 }
 
+// Summand j of the label's LoRA term: both parts of (s x A^T)[j] times B[y][j].
+template <typename T>
+__device__ __forceinline__ float lora_term(const T* xa, const T* b, int32_t y, int j, int r, int R) {
+  return (static_cast<float>(xa[j]) + static_cast<float>(xa[R + j])) *
+         static_cast<float>(b[static_cast<int64_t>(y) * r + j]);
+}
+
 // An infinite logit has no softmax, the label's neither.
 __device__ __forceinline__ float gap_of(float gap, float ly) { return ly == INFINITY ? NAN : gap; }
 
@@ -276,7 +283,7 @@ __device__ __forceinline__ float gap_of(float gap, float ly) { return ly == INFI
 // the gradient of x) by setting the label's to -S, S the sum of the others.  Only a row
 // with more than one reference is rewritten, by powers of two.
 __global__ void __launch_bounds__(kRowThreads)
-    head_ref_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0, Numbers num,
+    head_ref_kernel(const float2* stats, int cols, int64_t V, int64_t ld, int64_t row0, Numbers num,
                     const float* target, float* row_loss, LossOut out, __nv_bfloat16* eg, float* rest,
                     float* row_scale) {
   __shared__ float sn[kRowThreads / 32], sl[kRowThreads / 32], ss[kRowThreads / 32];
@@ -288,7 +295,7 @@ __global__ void __launch_bounds__(kRowThreads)
     finish_loss(out, num.count);
     return;
   }
-  const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
+  const int tiles = static_cast<int>((V + cols - 1) / cols);
   const float2* st = stats + i * tiles;
   float top = -INFINITY, low = INFINITY;
   for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(kRowThreads)
   if (eg != nullptr && low != top) {
     __nv_bfloat16* row = eg + i * ld;
     for (int64_t v = threadIdx.x; v < V; v += kRowThreads) {
-      const float n = st[v / kHeadTile].x;
+      const float n = st[static_cast<int>(v) / cols].x;
       if (n != top) row[v] = __float2bfloat16_rn(__bfloat162float(row[v]) * exp2f(n - top));
     }
     __syncthreads();
@@ -341,6 +348,8 @@ __global__ void __launch_bounds__(kRowThreads)
   }
   finish_loss(out, num.count);
 }
+
+constexpr int kHalfTile = 128;
 
 // After the logits with a reference for each 128: one CTA per counted token of the piece.
 // Its loss, and its row of g in place of the exponentials,
@@ -370,18 +379,14 @@ __global__ void __launch_bounds__(kRowThreads)
     return;
   }
   const int32_t y = num.label[slot];
-  const int tiles = static_cast<int>((V + kHeadTile - 1) / kHeadTile);
+  const int tiles = static_cast<int>((V + kHalfTile - 1) / kHalfTile);
   float m = -INFINITY, s = 0.f, extra = 0.f;
   for (int t = threadIdx.x; t < tiles; t += kRowThreads) {
     const float2 q = stats[i * tiles + t];
     factor[t] = q.x;
     join_max_sum(m, s, q.x, q.y * (1.f / 32768.f));
   }
-  for (int j = threadIdx.x; j < r; j += kRowThreads) {  // the label's LoRA term
-    const T* part = xa + slot * xa_ld + j;
-    extra += (static_cast<float>(part[0]) + static_cast<float>(part[R])) *
-             static_cast<float>(b[static_cast<int64_t>(y) * r + j]);
-  }
+  for (int j = threadIdx.x; j < r; j += kRowThreads) extra += lora_term(xa + slot * xa_ld, b, y, j, r, R);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     join_max_sum(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
@@ -417,26 +422,34 @@ __global__ void __launch_bounds__(kRowThreads)
     rest[slot] = gy - static_cast<float>(static_cast<T>(gy));
     row_scale[slot] = 1.f / unit;
   }
-#pragma unroll 4
-  for (int64_t q = threadIdx.x; q < ld / 8; q += kRowThreads) {
-    uint4 v = row[q];
-    const float f = factor[q * 8 / kHeadTile];
-    const __half2* e = reinterpret_cast<const __half2*>(&v);
-    float o[8];
+  const int n8 = static_cast<int>((V + 7) / 8);
+  constexpr int kAhead = 4;  // 16 bytes each in flight
+  for (int q0 = threadIdx.x; q0 < n8; q0 += kAhead * kRowThreads) {
+    uint4 v[kAhead];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 p = __half22float2(e[j]);
-      o[2 * j] = p.x * f;
-      o[2 * j + 1] = p.y * f;
-    }
-    if (q == y >> 3) {
+    for (int a = 0; a < kAhead; ++a)
+      if (q0 + a * kRowThreads < n8) v[a] = row[q0 + a * kRowThreads];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j == (y & 7)) o[j] = gy;
+    for (int a = 0; a < kAhead; ++a) {
+      const int q = q0 + a * kRowThreads;
+      if (q >= n8) break;
+      const float f = factor[q * 8 / kHalfTile];
+      const __half2* e = reinterpret_cast<const __half2*>(&v[a]);
+      float o[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 p = __half22float2(e[j]);
+        o[2 * j] = p.x * f;
+        o[2 * j + 1] = p.y * f;
+      }
+      if (q == y >> 3) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j == (y & 7)) o[j] = gy;
+      }
+      row[q] = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
+                          pack2<T>(o[6], o[7]));
     }
-    v = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
-                   pack2<T>(o[6], o[7]));
-    row[q] = v;
   }
 }
 
@@ -533,6 +546,11 @@ struct Carve {
 struct Dims {
   int64_t M, K, V, r;
   int grads;
+  bool bf16;
+  // one reference a row: g's factor per row, and what rounding its label's entry left
+  // over, go to dx (for a LoRA head, whose dA and dB would want both too, it gained 1.4 %
+  // and took their error from 0.0019 to 0.0026)
+  bool by_row() const { return bf16 && r == 0 && !want(MLORA_HEAD_GRAD_W); }
   bool lora() const { return r > 0; }
   bool want(int g) const { return (grads & g) != 0; }
   int64_t R() const {
@@ -547,8 +565,23 @@ struct Dims {
   // rows both off the lines: 870 cycles for a 256 x 256 x 64 step that takes 512)
   int64_t ld() const { return round_up(V, 64); }
   int64_t ldx() const { return round_up(K, 64); }
-  int64_t tiles() const { return (V + kHeadTile - 1) / kHeadTile; }
+  int64_t tiles(int cols) const { return (V + cols / 2 - 1) / (cols / 2); }  // half tiles
 };
+
+// Columns of a tile of logits with one reference a row (else 256, whose halves the
+// softmax pass finds by a shift): 256, or the multiple of 32 from 192 on that makes the
+// waves of tiles over the CTA pairs take at least a twelfth less together.  412 tokens
+// 4096 -> 32000: 4 waves of 256 columns take 101 us, 4 of 224 95 us; narrower tiles
+// move more per product, and 55 waves took a tenth longer for a nominal gain.
+int logit_cols(const Dims& d, int64_t rows) {
+  if (!d.by_row()) return 256;
+  const int64_t pairs = num_sms() / 2, tiles_m = (rows + 255) / 256;
+  auto time = [&](int64_t n) { return (tiles_m * ((d.V + n - 1) / n) + pairs - 1) / pairs * n; };
+  int best = 256;
+  for (int n = 224; n >= 192; n -= 32)
+    if (time(n) * 12 <= time(256) * 11 && (best == 256 || time(n) < time(best))) best = n;
+  return best;
+}
 
 // Ranges of the vocabulary that dx is summed over: enough for the tiles of few tokens
 // to occupy every CTA pair, against the copies that the backward then reads.  The rule
@@ -604,6 +637,8 @@ struct Work {
   void *xc, *xa_rows, *xa_t, *xa_lo, *b2, *bt, *u_rows, *u_t, *u_lo, *eg;
   float2* stats;
   int64_t piece;  // rows that go through at a time
+  int cols;       // of a tile of logits
+  int64_t tiles;  // half tiles: what shares a reference
   int64_t bytes;
 };
 
@@ -611,10 +646,12 @@ Work plan_work(void* base, const Dims& d) {
   Work w{};
   Carve c(base);
   // pieces of two gigabytes of exponentials (or 256 rows), equal up to the tile
-  const int64_t per_row = d.grads ? d.ld() * 2 : d.tiles() * 8;
+  const int64_t per_row = d.grads ? d.ld() * 2 : d.tiles(192) * 8;
   const int64_t most = std::max<int64_t>(int64_t{2048} << 20, 256 * per_row) / per_row / 256 * 256;
   const int64_t n = (d.M + most - 1) / most;
   w.piece = std::min(d.M, round_up((d.M + n - 1) / n, 256));
+  w.cols = logit_cols(d, w.piece);
+  w.tiles = d.tiles(w.cols);
   w.row_of = c.take<int32_t>(d.M);
   w.nll = c.take<float>(d.M);
   w.target = c.take<float>(d.M);
@@ -632,7 +669,7 @@ Work plan_work(void* base, const Dims& d) {
       w.u_lo = c.take<uint16_t>(d.R() * round_up(w.piece, 8));
     }
   }
-  w.stats = c.take<float2>(d.tiles() * w.piece);
+  w.stats = c.take<float2>(w.tiles * w.piece);
   if (d.grads) w.eg = c.take<uint16_t>(w.piece * d.ld());
   w.bytes = round_up(c.off, 256);
   return w;
@@ -663,8 +700,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
   const Elt elt = std::is_same<T, __half>::value ? Elt::kF16 : Elt::kBF16;
   const int64_t M = d.M, K = d.K, V = d.V, ld = d.ld(), ldx = d.ldx();
   const int zero_all = d.lora() ? 1 : 0;
-  // one reference a row: g's factor per row reaches x alone
-  const bool by_row = elt == Elt::kBF16 && !d.lora() && !d.want(MLORA_HEAD_GRAD_W);
+  const bool by_row = d.by_row();
   int rc;
   const Numbers num{st.slot_of, ws.row_of, st.label, st.count};
   const LossOut out{loss, ws.nll, M, mean ? 1 : 0};
@@ -732,7 +768,8 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     l.label = st.label + row0;
     l.e = ws.eg;
     l.stats = ws.stats;
-    l.stats_ld = d.tiles();
+    l.stats_ld = ws.tiles;
+    l.tile_n = ws.cols;
     l.ref = by_row ? ws.ref + row0 : nullptr;
     l.elt = elt;
     if (d.lora()) {
@@ -749,11 +786,11 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       const dim3 grid(static_cast<unsigned>(rows));
       if (by_row)
         e = launch_kernel(head_ref_kernel, grid, kRowThreads, 0, s, 0, 0, true,
-                          static_cast<const float2*>(ws.stats), V, ld, row0, num,
+                          static_cast<const float2*>(ws.stats), ws.cols / 2, V, ld, row0, num,
                           static_cast<const float*>(ws.target), row_loss, out,
                           static_cast<__nv_bfloat16*>(ws.eg), st.rest, st.row_scale);
       else
-        e = launch_kernel(head_row_kernel<T>, grid, kRowThreads, static_cast<size_t>(d.tiles()) * 4, s, 0,
+        e = launch_kernel(head_row_kernel<T>, grid, kRowThreads, static_cast<size_t>(ws.tiles) * 4, s, 0,
                           0, true, static_cast<const float2*>(ws.stats), V, ld, row0, num,
                           static_cast<const float*>(ws.target), static_cast<const T*>(ws.xa_rows),
                           static_cast<const T*>(b), d.ld_xa(), static_cast<int>(d.r),
@@ -811,14 +848,14 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     if (d.want(MLORA_HEAD_GRAD_X)) {
       HeadGemmArgs q;
       q.product = HeadProduct::kDx;
-      q.x = ws.eg;
-      q.w = w;
+      q.x = w;
+      q.w = ws.eg;
       q.d = st.dx + row0 * K;
-      q.M = rows;
-      q.N = K;
+      q.M = K;
+      q.N = rows;
       q.K = V;
-      q.ldx = ld;
-      q.ldw = K;
+      q.ldx = K;
+      q.ldw = ld;
       q.ldd = K;
       q.split_stride = M * K;
       q.splits = st.splits;
@@ -826,12 +863,13 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       q.row0 = row0;
       q.elt = elt;
       if (d.lora()) {
-        q.x2 = ws.u_rows;
-        q.w2 = a;
+        q.x2 = a;
+        q.w2 = ws.u_rows;
         q.R = d.R();
-        q.w2_rows = d.r;
-        q.ldx2 = d.R64();
-        q.ldw2 = K;
+        q.x2_rows = d.r;
+        q.w2_rows = d.R64();
+        q.ldx2 = K;
+        q.ldw2 = d.R64();
       }
       if ((rc = launch_head_gemm(q, s))) return rc;
     }
@@ -896,14 +934,14 @@ extern "C" {
 
 size_t mlora_linear_cross_entropy_state_bytes(int64_t M, int64_t K, int64_t V, int64_t r, int dtype,
                                               int grads) {
-  const Dims d{M, K, V, r, grads};
+  const Dims d{M, K, V, r, grads, dtype == MLORA_DTYPE_BF16};
   if (check_dims(d, dtype)) return 0;
   return static_cast<size_t>(plan_state(nullptr, d).bytes);
 }
 
 size_t mlora_linear_cross_entropy_workspace_bytes(int64_t M, int64_t K, int64_t V, int64_t r,
                                                   int dtype, int grads) {
-  const Dims d{M, K, V, r, grads};
+  const Dims d{M, K, V, r, grads, dtype == MLORA_DTYPE_BF16};
   if (check_dims(d, dtype)) return 0;
   return static_cast<size_t>(plan_work(nullptr, d).bytes);
 }
@@ -913,7 +951,7 @@ int mlora_linear_cross_entropy(const void* x, const void* w, const void* a, cons
                                size_t state_bytes, int64_t M, int64_t K, int64_t V, int64_t r,
                                float alpha, int64_t ignore_index, int mean, int dtype, int grads,
                                void* workspace, size_t workspace_bytes, void* stream) {
-  const Dims d{M, K, V, r, grads};
+  const Dims d{M, K, V, r, grads, dtype == MLORA_DTYPE_BF16};
   if (int rc = check_dims(d, dtype)) return rc;
   if (!x || !w || !labels || !state || (!loss && !row_loss) || (r > 0 && (!a || !b)))
     return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
@@ -943,7 +981,7 @@ int mlora_linear_cross_entropy_backward(const void* state, size_t state_bytes, c
                                         void* db, int ab_dtype, int accumulate_ab, void* dw,
                                         int64_t M, int64_t K, int64_t V, int64_t r, int dtype,
                                         int grads, void* stream) {
-  const Dims d{M, K, V, r, grads};
+  const Dims d{M, K, V, r, grads, dtype == MLORA_DTYPE_BF16};
   if (int rc = check_dims(d, dtype)) return rc;
   if (!state || !grad || !w) return fail(MLORA_ERR_INVALID_ARG, "NULL tensor pointer");
   if (d.want(MLORA_HEAD_GRAD_X) != (dx != nullptr) || d.want(MLORA_HEAD_GRAD_AB) != (da != nullptr) ||

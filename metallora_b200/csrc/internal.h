@@ -239,9 +239,10 @@ int launch_lora_bwd(const LoraBwdArgs& a, cudaStream_t stream);
 // logits [tokens, V]:
 //   kLogits: l[m, v] = x . W^T + x2 . w2^T    x [M, K], w [N, K], x2 [M, R64], w2 [N, r]
 //            out: stats and e, see there
-//   kDx:     D[m, k] = g . W + x2 . w2        x = g [M, K = V], w [K, N], w2 [r, N]
+//   kDx:     D[m, k] = g . W + w2 . x2        x = W [K = V, M], w = g [N tokens, K],
+//            x2 [x2_rows, M], w2 [N, R64]; D is [N, M] in memory
 //   kDw:     D[v, k] = g^T . x                x = g [K tokens, M = V], w = x [K, N]
-//            out: fp32 D, N a multiple of 8
+//            out: fp32 D, N a multiple of 8 (kDx: M)
 // and with the same kernel
 //   kLoraDropout: y = x . W^T + drop(x2 . w2^T)   as kLogits; out: 16-bit d16 [M, N], N a
 //            multiple of 8, kept elements as they are
@@ -253,9 +254,10 @@ struct HeadGemmArgs {
   const void* w;
   const void* x2 = nullptr;
   const void* w2 = nullptr;
-  float* d = nullptr;        // `splits` copies of [M, N], split_stride floats apart
+  float* d = nullptr;        // `splits` copies of D, split_stride floats apart
   int64_t M = 0, N = 0, K = 0;
-  int64_t R = 0, w2_rows = 0;
+  int tile_n = 256;          // columns of a tile: a multiple of 32
+  int64_t R = 0, w2_rows = 0, x2_rows = 0;
   int64_t ldx = 0, ldw = 0, ldx2 = 0, ldw2 = 0, ldd = 0, split_stride = 0;
   int splits = 1;            // at most the 64-wide blocks of the reduction
   int group_m = 8;           // tile rows per raster group
@@ -264,7 +266,7 @@ struct HeadGemmArgs {
   bool accumulate = false;   // D += (splits = 1)
   // kLogits: per row m its label and, for the form with one reference a row (bf16), ref;
   // e: [M, ldd] exponentials in 16 bits or nullptr (ldd a multiple of 16, at least N);
-  // stats: float2 [M, stats_ld], one for every 128 entries
+  // stats: float2 [M, stats_ld], one for every tile_n / 2 entries
   const int32_t* label = nullptr;
   const float* ref = nullptr;
   void* e = nullptr;
@@ -274,7 +276,6 @@ struct HeadGemmArgs {
   void* d16 = nullptr;
   Elt elt = Elt::kBF16;
 };
-constexpr int kHeadTile = 128;  // entries that share a largest logit
 int launch_head_gemm(const HeadGemmArgs& a, cudaStream_t s);
 int head_gemm_pairs();  // CTA pairs that are resident at once
 
