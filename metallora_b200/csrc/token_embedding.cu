@@ -4,7 +4,8 @@
 //
 // The sums run over the tokens of an entry in token order, whatever the launch, so the
 // gradient is the same bits in every run: tokens are sorted by (entry, token) first.
-// Up to 16384 tokens each counts the ones ahead of it, a comparison a pair; of more,
+// Up to 16384 tokens each counts the ones ahead of it, a comparison a pair (up to 512 in
+// the CTAs that add them up, for want of a launch); of more,
 // blocks of 2048 are sorted in shared memory and each element finds its place by binary
 // searches in the other blocks (keys are distinct: the token is part of them).  Runs of equal entries
 // in the sorted order are summed by chunks of 32 tokens, so that an entry that half of
@@ -34,7 +35,11 @@ constexpr int kJoin = 64;  // threads of a CTA that joins partial sums
 constexpr int64_t kPairTokens = 16384;
 constexpr int kRankThreads = 512;
 constexpr int kRankTokens = 64;  // of a CTA that counts pairs
-constexpr int kChunk = 32;  // sorted tokens per CTA of the gradient
+// Sorted tokens per CTA of the gradient: 32 (with 64, 3001 tokens of rows that fit no
+// vector took 79 us instead of 54), but 64 where one chunk then does without the joining
+// pass or it is short.
+constexpr int kChunk = 32, kOwnChunk = 64;
+constexpr int kOwnTokens = 512;  // up to which its CTAs sort them themselves
 constexpr uint32_t kNone = 0xFFFFFFFFu;  // entry of a token without a gradient
 
 template <typename T>
@@ -163,6 +168,28 @@ __device__ __forceinline__ uint32_t token_entry(int64_t v, int64_t V, int64_t pa
   return ok && v != padding ? static_cast<uint32_t>(v) : kNone;
 }
 
+// Of the tokens outside token t's own four, those that come before it: smaller entries,
+// and its own entry's tokens ahead of it; thread `part` of kPer counts its share.
+template <int kPer>
+__device__ __forceinline__ int count_ahead(const uint32_t* entries, int padded, int t, int part,
+                                           uint32_t mine) {
+  int place = 0;
+  const int own = t & ~3;
+#pragma unroll 4
+  for (int i = part * 4; i < own; i += kPer * 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(entries + i);
+    place += (q.x <= mine) + (q.y <= mine) + (q.z <= mine) + (q.w <= mine);
+  }
+  const int after = own / 4 + 1;  // the first four past it that are this thread's
+  const int first = after + (part - after % kPer + kPer) % kPer;
+#pragma unroll 4
+  for (int i = first * 4; i < padded; i += kPer * 4) {
+    const uint4 q = *reinterpret_cast<const uint4*>(entries + i);
+    place += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
+  }
+  return place;
+}
+
 // One CTA: the places of 64 tokens, eight threads a token, with every token's entry in
 // shared memory.  A token comes after those with a smaller entry, and those before it
 // with its own.
@@ -180,27 +207,11 @@ __global__ void __launch_bounds__(kRankThreads)
   __syncthreads();
   const int t = static_cast<int>(blockIdx.x) * kRankTokens + static_cast<int>(threadIdx.x) / kPer;
   const int part = static_cast<int>(threadIdx.x) % kPer;
-  uint32_t mine = 0;
-  int place = 0;
-  if (t < n_tok) {
-    mine = entries[t];
-    const int own = t & ~3;  // the four that t is among
-#pragma unroll 4
-    for (int i = part * 4; i < own; i += kPer * 4) {
-      const uint4 q = *reinterpret_cast<const uint4*>(entries + i);
-      place += (q.x <= mine) + (q.y <= mine) + (q.z <= mine) + (q.w <= mine);
-    }
-    const int after = own / 4 + 1;  // the first four past it that are this thread's
-    const int first = after + (part - after % kPer + kPer) % kPer;
-#pragma unroll 4
-    for (int i = first * 4; i < padded; i += kPer * 4) {
-      const uint4 q = *reinterpret_cast<const uint4*>(entries + i);
-      place += (q.x < mine) + (q.y < mine) + (q.z < mine) + (q.w < mine);
-    }
-    if (part == 0)
-      for (int i = own; i < min(own + 4, n_tok); ++i)
-        place += i < t ? entries[i] <= mine : entries[i] < mine;
-  }
+  const uint32_t mine = t < n_tok ? entries[t] : 0;
+  int place = t < n_tok ? count_ahead<kPer>(entries, padded, t, part, mine) : 0;
+  if (part == 0 && t < n_tok)
+    for (int i = t & ~3; i < min((t & ~3) + 4, n_tok); ++i)
+      place += i < t ? entries[i] <= mine : entries[i] < mine;
 #pragma unroll
   for (int o = kPer / 2; o > 0; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
   if (part == 0 && t < n_tok) sorted[place] = make_key(mine, t);
@@ -284,22 +295,33 @@ __global__ void __launch_bounds__(kThreads)
   sorted[place] = key;
 }
 
-// CTAs of the first `sum_ctas`: a chunk of 32 sorted tokens, kThreads * kVec columns.  A
+// CTAs of the first `sum_ctas`: a chunk of sorted tokens, kThreads * kVec columns.  A
 // run inside the chunk is written to the gradient; one that the border cuts to the
 // chunk's partial rows: [0] continues from the chunk before, [1] goes on in the next.
-// The others: 32 entries each, those without tokens zeroed.
-template <typename T>
+// The others: 32 entries each, those without tokens zeroed.  kOwn (few tokens): no launch
+// has sorted them, every CTA does for itself.
+template <typename T, bool kOwn>
 __global__ void __launch_bounds__(kThreads, 4)
-    embedding_grad_kernel(const uint64_t* sorted, const T* dy, int64_t n_tok,
-                          int64_t V, int64_t D, float scale, int vec, int sum_ctas, int slices,
-                          T* grad, float* partial) {
-  __shared__ uint64_t key[kChunk + 2];  // with a neighbour on either side
+    embedding_grad_kernel(const int64_t* idx, int64_t padding, uint64_t* sorted, const T* dy,
+                          int64_t n_tok, int64_t V, int64_t D, float scale, int vec, int sum_ctas,
+                          int slices, T* grad, float* partial, uint32_t* status) {
+  constexpr int kLen = kOwn ? kOwnChunk : kChunk;
+  __shared__ uint64_t key[kLen + 2];  // with a neighbour on either side
+  __shared__ __align__(16) uint32_t entries[kOwn ? kOwnTokens : 4];
+  __shared__ uint64_t order[kOwn ? kOwnTokens : 1];
   grid_wait();
   launch_dependents();
   if (static_cast<int>(blockIdx.x) >= sum_ctas) {
     const int64_t v0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - sum_ctas) * 32;
     uint32_t* const has_tokens = reinterpret_cast<uint32_t*>(key);
-    if (threadIdx.x < 32) {  // a search for each entry
+    if constexpr (kOwn) {
+      if (threadIdx.x == 0) *has_tokens = 0;
+      __syncthreads();
+      for (int i = threadIdx.x; i < static_cast<int>(n_tok); i += kThreads) {
+        const int64_t v = idx[i];
+        if (v >= v0 && v < v0 + 32 && v < V && v != padding) atomicOr(has_tokens, 1u << (v - v0));
+      }
+    } else if (threadIdx.x < 32) {  // a search for each entry
       const uint32_t v = static_cast<uint32_t>(v0) + threadIdx.x;
       int64_t lo = 0, hi = n_tok;
       while (lo < hi) {
@@ -350,11 +372,27 @@ __global__ void __launch_bounds__(kThreads, 4)
     return;
   }
   const int64_t chunk = static_cast<int>(blockIdx.x) / slices;
-  const int64_t p0 = chunk * kChunk;
-  const int n = static_cast<int>(n_tok - p0 < kChunk ? n_tok - p0 : kChunk);
-  if (threadIdx.x < kChunk + 2) {
+  const int64_t p0 = chunk * kLen;
+  const int n = static_cast<int>(n_tok - p0 < kLen ? n_tok - p0 : kLen);
+  if constexpr (kOwn) {
+    const int tokens = static_cast<int>(n_tok), padded = (tokens + 3) / 4 * 4;
+    for (int i = threadIdx.x; i < padded; i += kThreads)
+      entries[i] = i < tokens ? token_entry(idx[i], V, padding, status) : kNone;
+    __syncthreads();
+    for (int t = threadIdx.x; t < tokens; t += kThreads) {
+      const uint32_t mine = entries[t];
+      int place = count_ahead<1>(entries, padded, t, 0, mine);
+      for (int i = t & ~3; i < min((t & ~3) + 4, tokens); ++i)
+        place += i < t ? entries[i] <= mine : entries[i] < mine;
+      order[place] = make_key(mine, t);
+    }
+    __syncthreads();
+    if (static_cast<int>(blockIdx.x) % slices == 0)  // for the pass that joins runs
+      for (int i = threadIdx.x; i < n; i += kThreads) sorted[p0 + i] = order[p0 + i];
+  }
+  if (threadIdx.x < kLen + 2) {
     const int64_t p = p0 + static_cast<int>(threadIdx.x) - 1;
-    key[threadIdx.x] = p >= 0 && p < n_tok ? sorted[p] : ~uint64_t{0};
+    key[threadIdx.x] = p >= 0 && p < n_tok ? (kOwn ? order[kOwn ? p : 0] : sorted[p]) : ~uint64_t{0};
   }
   __syncthreads();
   const Cols c = thread_cols<T>(static_cast<int>(blockIdx.x) % slices, static_cast<int>(threadIdx.x),
@@ -393,26 +431,26 @@ __global__ void __launch_bounds__(kThreads, 4)
 // that run's partial sums in chunk order.
 template <typename T>
 __global__ void __launch_bounds__(kJoin)
-    embedding_join_kernel(const uint64_t* sorted, const float* partial, int64_t n_tok, int64_t D,
-                          float scale, int vec, T* grad) {
+    embedding_join_kernel(const uint64_t* sorted, const float* partial, int len, int64_t n_tok,
+                          int64_t D, float scale, int vec, T* grad) {
   grid_wait();
-  const int64_t first = blockIdx.x, last = (first + 1) * kChunk - 1;
+  const int64_t first = blockIdx.x, last = (first + 1) * len - 1;
   if (last + 1 >= n_tok) return;
   const uint32_t e = entry_of(sorted[last]);
   if (e == kNone || entry_of(sorted[last + 1]) != e) return;
-  if (first > 0 && entry_of(sorted[first * kChunk - 1]) == e && entry_of(sorted[first * kChunk]) == e)
+  if (first > 0 && entry_of(sorted[first * len - 1]) == e && entry_of(sorted[first * len]) == e)
     return;  // begun before this chunk
   const Cols c = thread_cols<T>(static_cast<int>(blockIdx.y), static_cast<int>(threadIdx.x), kJoin,
                                 vec != 0, D);
   if (!c.any()) return;
   Vec<T> acc = load_partial<T>(partial + (first * 2 + 1) * D, c);
   constexpr int kAhead = 4;
-  const int64_t chunks = (n_tok + kChunk - 1) / kChunk;
+  const int64_t chunks = (n_tok + len - 1) / len;
   for (int64_t q = first + 1; q < chunks; q += kAhead) {
     bool goes[kAhead];  // the run reaches chunk q + i
     Vec<T> v[kAhead];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) goes[i] = q + i < chunks && entry_of(sorted[(q + i) * kChunk]) == e;
+    for (int i = 0; i < kAhead; ++i) goes[i] = q + i < chunks && entry_of(sorted[(q + i) * len]) == e;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i)
       if (goes[i]) v[i] = load_partial<T>(partial + (q + i) * 2 * D, c);
@@ -433,7 +471,8 @@ int fail(int code, const std::string& msg) {
   return code;
 }
 
-int64_t chunks(int64_t n_tok) { return (n_tok + kChunk - 1) / kChunk; }
+int64_t chunk_len(int64_t n_tok) { return n_tok <= kOwnTokens ? kOwnChunk : kChunk; }
+int64_t chunks(int64_t n_tok) { return (n_tok + chunk_len(n_tok) - 1) / chunk_len(n_tok); }
 int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 int check(int64_t T, int64_t V, int64_t D, int dtype) {
@@ -489,8 +528,11 @@ Work plan(void* base, int64_t T, int64_t D) {
 template <typename T>
 int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int64_t V, int64_t D,
              float scale, int64_t padding, const Work& w, cudaStream_t s) {
-  cudaError_t e;
-  if (n_tok <= kPairTokens) {
+  cudaError_t e = cudaSuccess;
+  const bool own = n_tok <= kOwnTokens;
+  if (own) {
+    // sorted by the sums' own CTAs
+  } else if (n_tok <= kPairTokens) {
     static std::atomic<bool> limit_set[64];
     if (int rc = set_max_smem(reinterpret_cast<const void*>(embedding_rank_kernel), kPairTokens * 4,
                               limit_set))
@@ -524,9 +566,11 @@ int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int6
     return fail(MLORA_ERR_UNSUPPORTED, "embedding gradient: too many tokens for rows this long");
   if (e == cudaSuccess) {
     LaunchScope scope(kKindElementwise, s);
-    e = launch_kernel(embedding_grad_kernel<T>, dim3(static_cast<unsigned>(grid)), kThreads, 0, s, 0, 0,
-                      true, static_cast<const uint64_t*>(w.sorted), static_cast<const T*>(dy), n_tok, V,
-                      D, scale, vec, static_cast<int>(sum_ctas), slices, static_cast<T*>(grad), w.partial);
+    e = launch_kernel(own ? embedding_grad_kernel<T, true> : embedding_grad_kernel<T, false>,
+                      dim3(static_cast<unsigned>(grid)), kThreads, 0, s, 0, 0, true, idx, padding,
+                      w.sorted, static_cast<const T*>(dy), n_tok, V, D, scale, vec,
+                      static_cast<int>(sum_ctas), slices, static_cast<T*>(grad), w.partial,
+                      device_status_ptr());
   }
   if (e == cudaSuccess && chunks(n_tok) > 1) {
     LaunchScope scope(kKindElementwise, s);
@@ -534,8 +578,8 @@ int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int6
                       dim3(static_cast<unsigned>(chunks(n_tok) - 1),
                            static_cast<unsigned>((D + kJoin * kVec<T> - 1) / (kJoin * kVec<T>))),
                       kJoin, 0, s, 0, 0, true, static_cast<const uint64_t*>(w.sorted),
-                      static_cast<const float*>(w.partial), n_tok, D, scale, vec,
-                      static_cast<T*>(grad));
+                      static_cast<const float*>(w.partial), static_cast<int>(chunk_len(n_tok)), n_tok, D,
+                      scale, vec, static_cast<T*>(grad));
   }
   return launch_status(e, "embedding gradient");
 }

@@ -33,6 +33,10 @@ class LoRALinear(nn.Module):
     forward uses the next ``dropout_call``, which starts at 0 and may be set.
     """
 
+    # of layers pickled without them
+    dropout_seed = None
+    dropout_call = 0
+
     def __init__(self, in_features: int, out_features: int, rank: int = 8, alpha: float = 16.0,
                  dropout: float = 0.0, use_bias: bool = False, freeze_base: bool = True,
                  device=None, dtype=None, activation_checkpoint: str | None = None,

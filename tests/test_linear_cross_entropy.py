@@ -361,3 +361,37 @@ def test_threads_at_once(cuda):
     [t.start() for t in threads]
     [t.join() for t in threads]
     assert out == [True] * 20
+
+
+@pytest.mark.gpu
+def test_differentiable_once(cuda):
+    """A gradient that is to be differentiated again comes out right and refuses that."""
+    x, w, y, a, b = _case(40, 64, 304, BF16, 8, seed=14)
+    x.requires_grad_(True)
+    a.requires_grad_(True)
+    b.requires_grad_(True)
+    for kw in ({}, {"A": a, "B": b}):
+        leaves = (x, a, b) if kw else (x,)
+        want = torch.autograd.grad(ops.linear_cross_entropy(x, w, y, **kw), leaves)
+        got = torch.autograd.grad(ops.linear_cross_entropy(x, w, y, **kw), leaves, create_graph=True)
+        assert all(torch.equal(g, h) for g, h in zip(got, want))
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(got[0].float().sum(), x)
+    tab = torch.randn(20, 16, device=cuda, requires_grad=True)
+    for out, leaf in ((ops.dropout(x, 0.5, 3), x), (ops.embedding(y[:9] % 20, tab), tab)):
+        got = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)[0]
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(got.float().sum(), leaf)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_losses_without_a_gradient(cuda, dtype):
+    """Nothing asked for: the same losses, from less memory."""
+    x, w, y, a, b = _case(600, 128, 5000, dtype, 16, seed=15)
+    y[::7] = IGNORE
+    for kw in ({}, {"A": a, "B": b, "alpha": 32.0}):
+        want = ops.linear_cross_entropy(x.requires_grad_(True), w, y, reduction="none", **kw)
+        with torch.no_grad():
+            assert torch.equal(ops.linear_cross_entropy(x, w, y, reduction="none", **kw), want)
+        _check(x.detach(), w, y, kw.get("A"), kw.get("B"), kw.get("alpha", 16.0))

@@ -78,7 +78,8 @@ def _case(t, v, d, dtype, seed=0, hot=0.0):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("t,v,d", [(1, 1, 1), (1, 50, 8), (31, 3, 33), (32, 1, 64), (33, 1, 100),
-                                   (300, 40, 1001), (2048, 500, 72), (2049, 500, 8), (5000, 70000, 264),
+                                   (64, 9, 24), (65, 2, 24), (300, 40, 1001), (512, 100, 40), (513, 100, 40),
+                                   (2048, 500, 72), (2049, 500, 8), (5000, 70000, 264),
                                    (9000, 30, 520), (16384, 9000, 16), (20001, 3000, 24)])
 def test_values_and_gradients(cuda, dtype, t, v, d):
     idx, table, dy = _case(t, v, d, dtype, seed=t)
