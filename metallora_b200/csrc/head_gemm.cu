@@ -219,7 +219,8 @@ __device__ __forceinline__ void mask_logits(uint32_t (&r)[32], int c, int width,
 }
 
 // First form: this thread's half row of a tile of logits (up to 128 entries from n0).  One
-// pass with the row's reference; the largest logit is only looked for where it fails.
+// pass with the row's reference; the largest logit is only looked for where it fails, and
+// the half row written again.
 template <typename Release>
 __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const Shape& s, int m,
                                                 int n0, uint32_t taddr, Release&& release) {
@@ -233,7 +234,8 @@ __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const S
   const int half = s.tile_n / 2, width = min(half, p.N - n0);  // columns that are there
   const bool any = __any_sync(0xffffffffu, static_cast<uint32_t>(y) < static_cast<uint32_t>(width));
   const float log2e = kLog2e * p.uncut;
-  uint32_t v[kHalf / 2];
+  uint16_t* const row =
+      live && p.e != nullptr ? p.e + static_cast<long long>(m) * p.ldd + n0 : nullptr;
   float sum = 0.f;
   auto exponentials = [&] {
     float s0 = 0.f, s1 = 0.f;
@@ -247,12 +249,18 @@ __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const S
       for (int c = 0; c < 2; ++c) {
         mask_logits(r[c], h * 64 + c * 32, width, y, any);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float a = ex2(fmaf(__uint_as_float(r[c][2 * i]), log2e, -n));
-          const float b = ex2(fmaf(__uint_as_float(r[c][2 * i + 1]), log2e, -n));
-          s0 += a;
-          s1 += b;
-          v[h * 32 + c * 16 + i] = pack2<__nv_bfloat16>(a, b);
+        for (int q = 0; q < 2; ++q) {
+          uint32_t v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float a = ex2(fmaf(__uint_as_float(r[c][16 * q + 2 * i]), log2e, -n));
+            const float b = ex2(fmaf(__uint_as_float(r[c][16 * q + 2 * i + 1]), log2e, -n));
+            s0 += a;
+            s1 += b;
+            v[i] = pack2<__nv_bfloat16>(a, b);
+          }
+          const int col = h * 64 + c * 32 + q * 16;
+          if (row != nullptr && col < half && n0 + col < p.ldd) st_global_32b(row + col, v);
         }
       }
     }
@@ -275,18 +283,7 @@ __device__ __forceinline__ void softmax_row_ref(const HeadGemmParams& p, const S
     exponentials();
   }
   release();
-  if (!live) return;
-  if (p.e != nullptr) {
-    uint16_t* row = p.e + static_cast<long long>(m) * p.ldd + n0;
-#pragma unroll
-    for (int c = 0; c < 8; ++c)
-      if (c * 16 < half && n0 + c * 16 < p.ldd) {
-        const uint32_t q[8] = {v[8 * c],     v[8 * c + 1], v[8 * c + 2], v[8 * c + 3],
-                               v[8 * c + 4], v[8 * c + 5], v[8 * c + 6], v[8 * c + 7]};
-        st_global_32b(row + c * 16, q);
-      }
-  }
-  p.stats[static_cast<long long>(m) * p.stats_ld + n0 / half] = make_float2(n, sum);
+  if (live) p.stats[static_cast<long long>(m) * p.stats_ld + n0 / half] = make_float2(n, sum);
 }
 
 // Second form: all of the half row in registers: largest, exponentials, their sum.  `release` hands the accumulator back
@@ -349,11 +346,8 @@ __device__ __forceinline__ void softmax_row(const HeadGemmParams& p, const Shape
 // columns from n0, eight to a call of the generator.  (Tiles of 128 columns, two of both
 // accumulators in TMEM, moved half as much again from L2 and took 160 us where this
 // takes 129: 4096 tokens 4096 -> 4096.)
-__device__ __forceinline__ void dropout_bits(const HeadGemmParams& p, int m, int n0,
-                                             uint32_t (&bits)[4]) {
-  PhiloxKeys own;
-  const bool dev = p.drop.seed_dev != nullptr;
-  if (dev) own = philox_keys(static_cast<uint64_t>(*p.drop.seed_dev));
+__device__ __forceinline__ void dropout_bits(const HeadGemmParams& p, const PhiloxKeys& keys, int m,
+                                             int n0, uint32_t (&bits)[4]) {
   const int64_t first = (static_cast<int64_t>(m) * p.N + n0) / 8;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
@@ -361,10 +355,7 @@ __device__ __forceinline__ void dropout_bits(const HeadGemmParams& p, int m, int
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const uint64_t at = static_cast<uint64_t>(first + c * 4 + q);
-      bits[c] |= kept_bits(dev ? philox4x32_10(own, at, p.drop.call)
-                               : philox4x32_10(p.drop.keys, at, p.drop.call),
-                           p.drop.threshold)
-                 << (8 * q);
+      bits[c] |= kept_bits(philox4x32_10(keys, at, p.drop.call), p.drop.threshold) << (8 * q);
     }
   }
 }
@@ -373,28 +364,27 @@ template <typename T, typename Release>
 __device__ __forceinline__ void dropout_row(const HeadGemmParams& p, const Shape& s, int m, int n0,
                                             uint32_t taddr, const uint32_t (&bits)[4],
                                             Release&& release) {
-  uint32_t out[64];
+  T* row = static_cast<T*>(p.d16) + static_cast<long long>(m) * p.ldd + n0;
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    uint32_t base[32], lora[32];
+    uint32_t base[32], lora[32], out[16];
     tmem_ld_32x32b_x32(taddr + c * 32, base);
     tmem_ld_32x32b_x32(taddr + kTile + c * 32, lora);
     tmem_ld_wait();
+    if (c == 3) release();
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const float z0 = (bits[c] >> (2 * i)) & 1u ? __uint_as_float(lora[2 * i]) : 0.f;
       const float z1 = (bits[c] >> (2 * i + 1)) & 1u ? __uint_as_float(lora[2 * i + 1]) : 0.f;
-      out[c * 16 + i] = pack2<T>(__uint_as_float(base[2 * i]) + z0, __uint_as_float(base[2 * i + 1]) + z1);
+      out[i] = pack2<T>(__uint_as_float(base[2 * i]) + z0, __uint_as_float(base[2 * i + 1]) + z1);
     }
-  }
-  release();
-  if (m >= s.M) return;
-  T* row = static_cast<T*>(p.d16) + static_cast<long long>(m) * p.ldd + n0;
+    if (m >= s.M) continue;
 #pragma unroll
-  for (int q = 0; q < 16; ++q)
-    if (n0 + q * 8 < p.N)
-      *reinterpret_cast<uint4*>(row + q * 8) =
-          make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
+    for (int q = 0; q < 4; ++q)
+      if (n0 + c * 32 + q * 8 < p.N)
+        *reinterpret_cast<uint4*>(row + c * 32 + q * 8) =
+            make_uint4(out[4 * q], out[4 * q + 1], out[4 * q + 2], out[4 * q + 3]);
+  }
 }
 
 template <bool kXMN, bool kWMN, bool kBF16, Form kForm>
@@ -567,6 +557,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const uint32_t quarter = warp & 3u;  // TMEM lanes [32*quarter, 32*quarter+32)
     const uint32_t half = (warp - 2u) >> 2;  // of the tile's columns
     const uint32_t lead_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
+    __shared__ PhiloxKeys keys;  // of the seed in memory, where there is one
+    if constexpr (kForm == Form::kDropout) {
+      if (threadIdx.x == 64)
+        keys = p.drop.seed_dev != nullptr ? philox_keys(static_cast<uint64_t>(*p.drop.seed_dev))
+                                          : p.drop.keys;
+      named_bar_sync(1, kEpiWarps * 32);
+    }
     int local = 0;
     for (int u = pair; u < shape.units; u += num_pairs, ++local) {
       const Unit t = unit_at(p, shape, u);
@@ -575,7 +572,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int m = t.tm * kTile + static_cast<int>(crank * kHalf + quarter * 32 + lane);
       const int n0 = t.tn * shape.tile_n + static_cast<int>(half) * half_n;
       uint32_t bits[4];
-      if constexpr (kForm == Form::kDropout) dropout_bits(p, m, n0, bits);
+      if constexpr (kForm == Form::kDropout) dropout_bits(p, keys, m, n0, bits);
       if (!mbar_wait(&acc_full[buf], use, p.status, kDevTimeoutAccFull)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((quarter * 32u) << 16) + buf * kTile + half * half_n;
