@@ -508,7 +508,7 @@ MLORA_API int mlora_lora_grads_static(const void* dy, const void* x, const void*
  * has one whose label is outside [0, V) (device status 0x107).  Writes the sum, or
  * with `mean` the mean, over the other tokens to *loss, and/or each token's loss
  * (0 for those without) to row_loss [M].  BF16 or F16; K and r multiples of 8, with
- * r > 0 V too.
+ * r > 0 V too; V up to 2^20.
  *   The gradients named in `grads` are made here, up to the upstream factor, and
  * kept in `state` (256-byte aligned, mlora_linear_cross_entropy_state_bytes;
  * overwritten) for the call below; without `grads` the state is small and only
