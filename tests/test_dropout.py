@@ -287,3 +287,19 @@ def test_lora_layer_calls_and_graph(cuda):
         want = layer(x)
         wa, wb = torch.autograd.grad(want, (layer.A, layer.B), torch.ones_like(want))
         assert torch.equal(y, want) and torch.equal(ga, wa) and torch.equal(gb, wb)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda):
+    n = 2 ** 31 + 43
+    x = torch.ones(n, device=cuda, dtype=BF16)
+    got = ops.dropout(x, 0.25, 12, call=3)
+    t = round(65536 * 0.25)
+    for first in (0, 2 ** 31 - 16, n // 8 * 8 - 64):
+        want = []
+        for b in range(first // 8, min(first // 8 + 9, -(-n // 8))):
+            for w in philox((12, 0), (b & 0xFFFFFFFF, b >> 32, 3, 0)):
+                want += [w & 0xFFFF, w >> 16]
+        part = got[first:first + 72].cpu()
+        assert torch.equal(part > 0, torch.tensor([u >= t for u in want])[:part.numel()])
+

@@ -395,3 +395,32 @@ def test_losses_without_a_gradient(cuda, dtype):
         with torch.no_grad():
             assert torch.equal(ops.linear_cross_entropy(x, w, y, reduction="none", **kw), want)
         _check(x.detach(), w, y, kw.get("A"), kw.get("B"), kw.get("alpha", 16.0))
+
+
+@pytest.mark.gpu
+def test_lora_head_with_frozen_factors(cuda):
+    x, w, y, a, b = _case(300, 128, 1000, BF16, 16, seed=16)
+    y[4:90] = IGNORE
+    _check(x.requires_grad_(True), w, y, a, b, alpha=32.0)
+    _check(x, w, y, a, b, alpha=32.0, reduction="sum")
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda):
+    """More than 2^31 hidden values: rows at both ends against 64 bits."""
+    m, k, v = 530_000, 4096, 72
+    g = torch.Generator(device=cuda).manual_seed(17)
+    w = (torch.randn(v, k, generator=g, device=cuda) / 64).to(BF16)
+    x = torch.randn(m, k, generator=g, device=cuda, dtype=BF16).requires_grad_(True)
+    y = torch.randint(0, v, (m,), generator=g, device=cuda)
+    y[::3] = IGNORE
+    loss = ops.linear_cross_entropy(x, w, y, reduction="none")
+    dx = torch.autograd.grad(loss, x, torch.ones_like(loss))[0]
+    pick = torch.cat([torch.arange(100), torch.arange(m - 100, m)]).to(cuda)
+    xs, ys = x.detach()[pick].requires_grad_(True), y[pick]
+    want = ops.linear_cross_entropy(xs, w, ys, reduction="none")  # checked against 64 bits elsewhere
+    assert (loss[pick] - want).abs().max() < 1e-5
+    few = torch.autograd.grad(want, xs, torch.ones_like(want))[0].double()
+    assert ((dx[pick].double() - few).abs() <= 2.0 ** -7 * few.abs() + 1e-5).all()
+    assert torch.count_nonzero(dx[::3][-50:]) == 0
+

@@ -217,3 +217,18 @@ def test_module_and_a_head_that_shares_the_table(cuda):
     de = kernels.embedding_bwd(dh, idx, 500, 8.0, 0)
     assert torch.equal(both, de + dw)
     assert torch.count_nonzero(de[0]) == 0 and torch.count_nonzero(dw[0]) > 0
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits(cuda):
+    v, d = 530_000, 4096
+    table = torch.zeros(v, d, device=cuda, dtype=FP16)
+    idx = torch.tensor([0, v - 1, 7, v - 1, v - 2], device=cuda)
+    table[idx] = torch.randn(5, d, device=cuda).to(FP16)
+    assert torch.equal(ops.embedding(idx, table), table[idx])
+    dy = torch.randn(5, d, device=cuda).to(FP16)
+    grad = kernels.embedding_bwd(dy, idx, v)
+    assert torch.equal(grad[v - 2], dy[4]) and torch.equal(grad[7], dy[2])
+    assert torch.equal(grad[v - 1], (dy[1].float() + dy[3].float()).to(FP16))
+    assert torch.count_nonzero(grad[8:v - 2]) == 0
+
