@@ -6,6 +6,8 @@ Loading is lazy; a missing library or an unsupported device raises
 from __future__ import annotations
 
 import ctypes as C
+import importlib.machinery
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -13,6 +15,7 @@ from pathlib import Path
 from .exceptions import DeviceError, MetalLoRAError, ShapeError
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libmetallora_b200.so"
+AUTOGRAD_PATH = LIB_PATH.with_name("_autograd.so")
 
 MLORA_OK = 0
 MLORA_ERR_INVALID_ARG = -1
@@ -40,6 +43,7 @@ DTYPE_F16 = 1
 DTYPE_F32 = 2
 
 _lib = None
+_autograd = None
 _lock = threading.Lock()
 
 vp = C.c_void_p
@@ -153,6 +157,24 @@ def load(path: str | os.PathLike | None = None):
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+def autograd():
+    """Loads (once) and returns the extension with the backward nodes (csrc/autograd.cpp)."""
+    global _autograd
+    if _autograd is not None:
+        return _autograd
+    with _lock:
+        if _autograd is None:
+            if not AUTOGRAD_PATH.is_file():
+                raise DeviceError(f"{AUTOGRAD_PATH} is missing: build it with "
+                                  "`python -m metallora_b200.build`")
+            loader = importlib.machinery.ExtensionFileLoader("_autograd", str(AUTOGRAD_PATH))
+            spec = importlib.util.spec_from_file_location("_autograd", AUTOGRAD_PATH, loader=loader)
+            module = importlib.util.module_from_spec(spec)
+            loader.exec_module(module)
+            _autograd = module
+    return _autograd
 
 
 def last_error() -> str:

@@ -4,6 +4,8 @@ Each ``.cu`` file is compiled for sm_100a (``-gencode arch=compute_100a,code=sm_
 in parallel, then linked into one shared library that exports the C ABI of
 ``include/metallora_b200.h``.  Object files go to ``metallora_b200/lib/obj``;
 a source is recompiled only when it or a header is newer than its object.
+``csrc/autograd.cpp``, backward nodes for torch's engine over that ABI, becomes the
+Python extension ``metallora_b200/lib/_autograd.so``.
 
     python -m metallora_b200.build [--force] [--verbose]
 """
@@ -23,6 +25,8 @@ INCLUDE = PKG.parent / "include"
 LIB_DIR = PKG / "lib"
 OBJ_DIR = LIB_DIR / "obj"
 LIB_PATH = LIB_DIR / "libmetallora_b200.so"
+AUTOGRAD_SRC = CSRC / "autograd.cpp"
+AUTOGRAD_PATH = LIB_DIR / "_autograd.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -60,6 +64,25 @@ def _compile(src: Path, obj: Path, verbose: bool) -> None:
         print(res.stderr)
 
 
+def _build_autograd(verbose: bool) -> None:
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ext
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", str(INCLUDE),
+           *(f"-I{p}" for p in ext.include_paths("cuda")), "-I" + sysconfig.get_paths()["include"],
+           str(AUTOGRAD_SRC), "-o", str(AUTOGRAD_PATH), f"-L{LIB_DIR}", "-lmetallora_b200",
+           "-Wl,-rpath,$ORIGIN", *(f"-L{p}" for p in ext.library_paths()), "-lc10", "-lc10_cuda",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd))
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"{AUTOGRAD_SRC.name} failed:\n{res.stdout}\n{res.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
@@ -79,6 +102,8 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    if force or _stale(AUTOGRAD_SRC, AUTOGRAD_PATH, max(h.stat().st_mtime for h in INCLUDE.glob("*.h"))):
+        _build_autograd(verbose)
     return LIB_PATH
 
 

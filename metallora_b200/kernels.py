@@ -799,24 +799,6 @@ def linear_cross_entropy_fwd(x2d: torch.Tensor, w: torch.Tensor, labels: torch.T
     return loss, state
 
 
-def linear_cross_entropy_dx(grad: torch.Tensor, state: torch.Tensor, w: torch.Tensor, M: int,
-                            reduction: str) -> torch.Tensor:
-    """``linear_cross_entropy_bwd`` for the gradient of x alone, from the forward's own
-    state and (contiguous) w and an upstream gradient like its loss."""
-    V, K = w.shape
-    dx = w.new_empty((M, K))
-    if M:
-        if not grad.is_contiguous():
-            grad = grad.contiguous()
-        st = _lib.load().mlora_linear_cross_entropy_backward(
-            state.data_ptr(), state.numel(), grad.data_ptr(), reduction == "none", reduction == "mean",
-            w.data_ptr(), dx.data_ptr(), None, None, 0, 0, None, M, K, V, 0, _DT[w.dtype],
-            _lib.HEAD_GRAD_X, _stream())
-        if st:
-            _lib.check(st, "mlora_linear_cross_entropy_backward")
-    return dx
-
-
 def linear_cross_entropy_bwd(grad: torch.Tensor, state: torch.Tensor, w: torch.Tensor, M: int,
                              r: int, reduction: str, grads: int,
                              da_out: torch.Tensor | None = None,
@@ -876,8 +858,8 @@ def _table_index(indices: torch.Tensor) -> torch.Tensor:
 
 
 def embedding_run(indices: torch.Tensor, table: torch.Tensor, scale: float):
-    """``embedding_fwd``'s output, its indices as the kernels take them, and the rest of
-    ``embedding_bwd_run``'s arguments up to the scale."""
+    """``embedding_fwd``'s output, its indices as the kernels take them, (T, V, D, scale)
+    and the type's code: what its backward takes besides dy."""
     _need_here(table, indices)
     code = _dtype_code(table)
     if table.dim() != 2:
@@ -901,29 +883,6 @@ def embedding_fwd(indices: torch.Tensor, table: torch.Tensor, scale: float = 1.0
     return embedding_run(indices, table, float(scale))[0]
 
 
-@functools.lru_cache(maxsize=256)
-def _embedding_ws_bytes(T: int, D: int) -> int:
-    return _lib.load().mlora_embedding_backward_workspace_bytes(T, D)
-
-
-def embedding_bwd_run(dy: torch.Tensor, idx: torch.Tensor, T: int, V: int, D: int, scale: float,
-                      padding_idx: int, code: int) -> torch.Tensor:
-    """The gradient of ``embedding_fwd``'s table from its own indices (a row of int64)
-    and a dy of its output's size, type and device; padding_idx < 0: none."""
-    if not dy.is_contiguous():
-        dy = dy.contiguous()
-    grad = dy.new_empty((V, D))
-    if T == 0 or D == 0:
-        return grad.zero_()
-    nbytes = _embedding_ws_bytes(T, D)
-    ws = dy.new_empty(nbytes, dtype=torch.uint8)
-    st = _lib.load().mlora_embedding_backward(idx.data_ptr(), dy.data_ptr(), grad.data_ptr(), T, V, D,
-                                              scale, padding_idx, code, ws.data_ptr(), nbytes, _stream())
-    if st:
-        _lib.check(st, "mlora_embedding_backward")
-    return grad
-
-
 def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, scale: float = 1.0,
                   padding_idx: int | None = None) -> torch.Tensor:
     """The table's gradient [num_embeddings, D] in dy's dtype: scale times the sum of
@@ -933,8 +892,19 @@ def embedding_bwd(dy: torch.Tensor, indices: torch.Tensor, num_embeddings: int, 
     idx = _table_index(indices)
     if dy.shape[:-1] != idx.shape:
         raise ShapeError(f"grad_output {tuple(dy.shape)} does not match indices {tuple(idx.shape)}")
-    return embedding_bwd_run(dy, idx, idx.numel(), int(num_embeddings), dy.shape[-1], float(scale),
-                             -1 if padding_idx is None else padding_idx, _dtype_code(dy))
+    T, V, D = idx.numel(), int(num_embeddings), dy.shape[-1]
+    code = _dtype_code(dy)
+    dy = dy.contiguous()
+    grad = dy.new_empty((V, D))
+    if T == 0 or D == 0:
+        return grad.zero_()
+    nbytes = _lib.load().mlora_embedding_backward_workspace_bytes(T, D)
+    ws = dy.new_empty(nbytes, dtype=torch.uint8)
+    st = _lib.load().mlora_embedding_backward(idx.data_ptr(), dy.data_ptr(), grad.data_ptr(), T, V, D,
+                                              float(scale), -1 if padding_idx is None else padding_idx,
+                                              code, ws.data_ptr(), nbytes, _stream())
+    _lib.check(st, "mlora_embedding_backward")
+    return grad
 
 
 # ---------------------------------------------------------------- dropout --

@@ -128,9 +128,6 @@ class _LoRALinearFn(torch.autograd.Function):
 
 
 _once = torch.autograd.function.once_differentiable
-# whether a backward is to be differentiated again (create_graph); without that the
-# functions below skip what refuses it, some microseconds a call
-_grad_on = torch.is_grad_enabled
 
 
 def _keep_seed(ctx, seed, *tensors):
@@ -419,17 +416,8 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    def backward(ctx, grad):
-        state, w = ctx.saved_tensors
-        m, _, reduction, grads = ctx.plan
-        if grads == _lib.HEAD_GRAD_X and w.is_contiguous() and not _grad_on():  # a frozen head
-            return (_k.linear_cross_entropy_dx(grad, state, w, m, reduction), None, None, None, None,
-                    None)
-        return _LinearCrossEntropyFn._all(ctx, grad)
-
-    @staticmethod
     @_once
-    def _all(ctx, grad):
+    def backward(ctx, grad):
         state, w = ctx.saved_tensors
         m, r, reduction, grads = ctx.plan
         sink = ctx.sink if grads & _lib.HEAD_GRAD_AB else None
@@ -479,30 +467,29 @@ def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,
         raise ConfigurationError("reduction='none' takes gradients of x alone; detach the head's "
                                  "weights or use 'mean' or 'sum'")
     flat = x.dim() == 2
+    if A is None and not (weight.requires_grad and torch.is_grad_enabled()):  # a frozen head
+        x2d = x if flat else x.reshape(-1, x.shape[-1])
+        hang = _hang(x2d, weight)
+        loss, state = _k.linear_cross_entropy_fwd(
+            x2d, weight, labels if flat else labels.reshape(-1), None, None, 16.0, ignore_index,
+            reduction, _lib.HEAD_GRAD_X if hang else 0)
+        if hang:
+            _lib.autograd().attach_linear_cross_entropy(loss, x2d, state, weight, x2d.shape[0],
+                                                        reduction == "none", reduction == "mean",
+                                                        _k._DT[x2d.dtype])
+        return loss if flat or reduction != "none" else loss.reshape(labels.shape)
     loss = _LinearCrossEntropyFn.apply(x if flat else x.reshape(-1, x.shape[-1]), weight, A, B,
                                        labels if flat else labels.reshape(-1),
                                        (float(alpha), ignore_index, reduction, _compute, _sink))
     return loss if flat or reduction != "none" else loss.reshape(labels.shape)
 
 
-class _DropoutFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, p, seed, call):
-        ctx.plan = plan = _k.dropout_plan(x, p, seed, call)
-        ctx.tensor = torch.is_tensor(seed)
-        if ctx.tensor:  # kept, and being written over before the backward noticed
-            ctx.save_for_backward(seed)
-        return _k.dropout_run(x, plan)
-
-    @staticmethod
-    def backward(ctx, dy):
-        if ctx.tensor:
-            ctx.saved_tensors
-        if _grad_on():
-            return _DropoutFn._guarded(ctx, dy)
-        return _k.dropout_run(dy, ctx.plan), None, None, None
-
-    _guarded = staticmethod(_once(lambda ctx, dy: (_k.dropout_run(dy, ctx.plan), None, None, None)))
+def _hang(x, *rest) -> bool:
+    """Whether the output of an operator gets a backward node, for x's gradient.  (There
+    is no forward-mode derivative: a tangent of x or the rest is refused.)"""
+    if _forward_mode() and any(forward_ad.unpack_dual(t).tangent is not None for t in (x, *rest)):
+        raise NotImplementedError("this operator has no forward-mode derivative")
+    return x.requires_grad and torch.is_grad_enabled()
 
 
 def dropout(x, p: float, seed, call: int = 0, training: bool = True):
@@ -520,25 +507,13 @@ def dropout(x, p: float, seed, call: int = 0, training: bool = True):
         raise ConfigurationError(f"dropout must be in [0, 1], got {p}")
     if not training:
         return x
-    return _DropoutFn.apply(x, float(p), seed, int(call))
-
-
-class _EmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, indices, table, scale, padding_idx):
-        out, idx, sizes, code = _k.embedding_run(indices, table, scale)
-        ctx.save_for_backward(idx)
-        ctx.plan = (*sizes, padding_idx, code)
-        return out
-
-    @staticmethod
-    def backward(ctx, dy):
-        if _grad_on():
-            return _EmbeddingFn._guarded(ctx, dy)
-        return None, _k.embedding_bwd_run(dy, *ctx.saved_tensors, *ctx.plan), None, None
-
-    _guarded = staticmethod(_once(lambda ctx, dy: (
-        None, _k.embedding_bwd_run(dy, *ctx.saved_tensors, *ctx.plan), None, None)))
+    plan = _k.dropout_plan(x, p, seed, call)
+    out = _k.dropout_run(x, plan)
+    if _hang(x):
+        n, t, scaled, value, _, use, code = plan
+        _lib.autograd().attach_dropout(out, x, n, t, scaled, value, use, code,
+                                       seed if torch.is_tensor(seed) else None)
+    return out
 
 
 def embedding(indices, table, scale: float = 1.0, padding_idx: int | None = None):
@@ -556,4 +531,8 @@ def embedding(indices, table, scale: float = 1.0, padding_idx: int | None = None
         if not -rows <= padding_idx < rows:
             raise ConfigurationError(f"padding_idx {padding_idx} is outside the table's {rows} rows")
         padding_idx = int(padding_idx) % rows
-    return _EmbeddingFn.apply(indices, table, float(scale), -1 if padding_idx is None else padding_idx)
+    out, idx, sizes, code = _k.embedding_run(indices, table, float(scale))
+    if _hang(table):
+        _lib.autograd().attach_embedding(out, table, idx, *sizes,
+                                         -1 if padding_idx is None else padding_idx, code)
+    return out
