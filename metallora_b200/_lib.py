@@ -160,10 +160,12 @@ def load(path: str | os.PathLike | None = None):
 
 
 def autograd():
-    """Loads (once) and returns the extension with the backward nodes (csrc/autograd.cpp)."""
+    """Loads (once) and returns the extension with the backward nodes (csrc/autograd.cpp),
+    which call the library that ``load`` has loaded."""
     global _autograd
     if _autograd is not None:
         return _autograd
+    lib = load()
     with _lock:
         if _autograd is None:
             if not AUTOGRAD_PATH.is_file():
@@ -173,6 +175,10 @@ def autograd():
             spec = importlib.util.spec_from_file_location("_autograd", AUTOGRAD_PATH, loader=loader)
             module = importlib.util.module_from_spec(spec)
             loader.exec_module(module)
+            module.bind(*(C.cast(fn, vp).value for fn in (
+                lib.mlora_dropout, lib.mlora_embedding_backward,
+                lib.mlora_embedding_backward_workspace_bytes,
+                lib.mlora_linear_cross_entropy_backward)))
             _autograd = module
     return _autograd
 

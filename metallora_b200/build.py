@@ -73,9 +73,8 @@ def _build_autograd(verbose: bool) -> None:
     cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
            "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-I", str(INCLUDE),
            *(f"-I{p}" for p in ext.include_paths("cuda")), "-I" + sysconfig.get_paths()["include"],
-           str(AUTOGRAD_SRC), "-o", str(AUTOGRAD_PATH), f"-L{LIB_DIR}", "-lmetallora_b200",
-           "-Wl,-rpath,$ORIGIN", *(f"-L{p}" for p in ext.library_paths()), "-lc10", "-lc10_cuda",
-           "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           str(AUTOGRAD_SRC), "-o", str(AUTOGRAD_PATH), *(f"-L{p}" for p in ext.library_paths()),
+           "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     if verbose:
         print(" ".join(cmd))
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -44,6 +44,26 @@ void check(int status, const char* what) {
   }
 }
 
+// The entry points, of the library that Python has loaded: the forward's and these are
+// of one build.
+struct {
+  decltype(&mlora_dropout) dropout;
+  decltype(&mlora_embedding_backward) embedding_backward;
+  decltype(&mlora_embedding_backward_workspace_bytes) embedding_backward_workspace_bytes;
+  decltype(&mlora_linear_cross_entropy_backward) linear_cross_entropy_backward;
+} abi;
+
+void bind(uintptr_t dropout, uintptr_t embedding_backward, uintptr_t embedding_backward_workspace_bytes,
+          uintptr_t linear_cross_entropy_backward) {
+  abi.dropout = reinterpret_cast<decltype(abi.dropout)>(dropout);
+  abi.embedding_backward = reinterpret_cast<decltype(abi.embedding_backward)>(embedding_backward);
+  abi.embedding_backward_workspace_bytes =
+      reinterpret_cast<decltype(abi.embedding_backward_workspace_bytes)>(
+          embedding_backward_workspace_bytes);
+  abi.linear_cross_entropy_backward =
+      reinterpret_cast<decltype(abi.linear_cross_entropy_backward)>(linear_cross_entropy_backward);
+}
+
 void* current_stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 // depends: whether the gradient is a function of something to be differentiated.
@@ -77,7 +97,7 @@ struct MloraDropoutBackward : Node {
     const at::Tensor dy = grads[0].contiguous();
     at::Tensor dx = at::empty_like(dy);
     if (n > 0)
-      check(mlora_dropout(dy.const_data_ptr(), dx.data_ptr(), n, threshold, scaled, seed,
+      check(abi.dropout(dy.const_data_ptr(), dx.data_ptr(), n, threshold, scaled, seed,
                           held.defined() ? held.const_data_ptr<int64_t>() : nullptr, call, dtype,
                           current_stream()),
             "mlora_dropout");
@@ -104,7 +124,7 @@ struct MloraEmbeddingBackward : Node {
       grad.zero_();
     } else {
       at::Tensor ws = at::empty({workspace}, dy.options().dtype(at::kByte));
-      check(mlora_embedding_backward(index.const_data_ptr<int64_t>(), dy.const_data_ptr(),
+      check(abi.embedding_backward(index.const_data_ptr<int64_t>(), dy.const_data_ptr(),
                                      grad.data_ptr(), T, V, D, scale, padding, dtype, ws.data_ptr(),
                                      static_cast<size_t>(workspace), current_stream()),
             "mlora_embedding_backward");
@@ -130,7 +150,7 @@ struct MloraLinearCrossEntropyBackward : Node {
     const int64_t V = w.size(0), K = w.size(1);
     at::Tensor dx = at::empty({M, K}, w.options());
     if (M > 0)
-      check(mlora_linear_cross_entropy_backward(s.const_data_ptr(), static_cast<size_t>(s.numel()),
+      check(abi.linear_cross_entropy_backward(s.const_data_ptr(), static_cast<size_t>(s.numel()),
                                                 up.const_data_ptr<float>(), per_row, mean,
                                                 w.const_data_ptr(), dx.data_ptr(), nullptr, nullptr,
                                                 dtype, 0, nullptr, M, K, V, 0, dtype,
@@ -168,7 +188,7 @@ void attach_embedding(const at::Tensor& out, const at::Tensor& table, const at::
   node->padding = padding;
   node->dtype = dtype;
   node->workspace =
-      T > 0 && D > 0 ? static_cast<int64_t>(mlora_embedding_backward_workspace_bytes(T, D)) : 0;
+      T > 0 && D > 0 ? static_cast<int64_t>(abi.embedding_backward_workspace_bytes(T, D)) : 0;
   node->idx = SavedVariable(idx, false);
   attach(out, table, std::move(node));
 }
@@ -189,6 +209,7 @@ void attach_linear_cross_entropy(const at::Tensor& loss, const at::Tensor& x, co
 }  // namespace
 
 PYBIND11_MODULE(_autograd, m) {
+  m.def("bind", &bind);
   m.def("attach_dropout", &attach_dropout);
   m.def("attach_embedding", &attach_embedding);
   m.def("attach_linear_cross_entropy", &attach_linear_cross_entropy);

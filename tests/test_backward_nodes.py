@@ -1,6 +1,10 @@
 """The backward nodes that torch's engine runs without Python: dropout, token embedding,
 the loss of a frozen head."""
+import shutil
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -17,6 +21,18 @@ def test_extension_is_built():
     nodes = _lib.autograd()
     assert nodes is _lib.autograd()
     assert all(hasattr(nodes, "attach_" + n) for n in ("dropout", "embedding", "linear_cross_entropy"))
+
+
+def test_forward_and_backward_are_of_one_library(tmp_path):
+    """Loaded from another path, the kernels of both directions are that path's."""
+    other = tmp_path / "other.so"
+    shutil.copy(_lib.LIB_PATH, other)
+    out = subprocess.run(
+        [sys.executable, "-c", "import sys; from metallora_b200 import _lib; _lib.load(sys.argv[1]); "
+         "_lib.autograd(); print(open('/proc/self/maps').read())", str(other)],
+        capture_output=True, text=True, cwd=Path(__file__).resolve().parent.parent, timeout=300)
+    assert out.returncode == 0, out.stderr
+    assert str(other) in out.stdout and str(_lib.LIB_PATH) not in out.stdout
 
 
 def _calls(cuda):
