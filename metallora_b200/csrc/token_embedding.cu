@@ -35,12 +35,19 @@ constexpr int kJoin = 64;  // threads of a CTA that joins partial sums
 constexpr int64_t kPairTokens = 16384;
 constexpr int kRankThreads = 512;
 constexpr int kRankTokens = 64;  // of a CTA that counts pairs
-// Sorted tokens per CTA of the gradient: 32 (with 64, 3001 tokens of rows that fit no
-// vector took 79 us instead of 54), but 64 where one chunk then does without the joining
-// pass or it is short.
+// Sorted tokens per CTA of the gradient: 32 (gradient of 2000 tokens, 20000x101: 15 us,
+// with 64 20 us, 16 13 us; of 16000 tokens, 1000x4095: 126, 118, 137 us), but 64 where one
+// chunk then does without the joining pass or it is short.
 constexpr int kChunk = 32, kOwnChunk = 64;
 constexpr int kOwnTokens = 512;  // up to which its CTAs sort them themselves
 constexpr uint32_t kNone = 0xFFFFFFFFu;  // entry of a token without a gradient
+
+// Columns of a thread that sums rows of no whole 16 bytes, kThreads apart, 16 rows of them
+// in flight: the loads of two bytes need many CTAs and few rounds, which the zeroing
+// beside them stretches.  Gradient of 3001 tokens, 50257x1001: 31.5 us (one column 33.9,
+// four 35.8, the vector path's loop of eight columns and eight rows 47.6); of 8192,
+// 32000x4095: 103 (127, 106, 142).
+constexpr int kOddCols = 2;
 
 template <typename T>
 constexpr int kVec = 16 / static_cast<int>(sizeof(T));
@@ -295,16 +302,48 @@ __global__ void __launch_bounds__(kThreads)
   sorted[place] = key;
 }
 
+// Of the 32 entries from v0, sets the bits of those that have tokens; all of a CTA.  The
+// first of their tokens is searched with kThreads samples a round, two rounds of dependent
+// loads up to 65536 tokens (a binary search by one warp took twelve to fourteen).
+__device__ __forceinline__ void mark_entries(const uint64_t* sorted, int64_t n_tok, uint32_t v0,
+                                             uint32_t* bits) {
+  const int tid = static_cast<int>(threadIdx.x);
+  int64_t lo = 0, hi = n_tok;  // the first token of v0 or above is at lo..hi
+  while (lo < hi) {
+    const int64_t step = (hi - lo + kThreads - 1) / kThreads;
+    const int64_t p = lo + tid * step + step - 1;  // a segment's last
+    const int below = __syncthreads_count(p < hi && entry_of(sorted[p]) < v0);
+    lo += below * step;
+    hi = min(hi, lo + step - 1);
+  }
+  // (v0 + 32 is below kNone)
+  const uint32_t e = lo + tid < n_tok ? entry_of(sorted[lo + tid]) : kNone;
+  if (e < v0 + 32) atomicOr(bits, 1u << (e - v0));
+  if (__syncthreads_count(e < v0 + 32) < kThreads || tid >= 32) return;
+  // more tokens than that: a search for each entry
+  const uint32_t v = v0 + tid;
+  lo += kThreads, hi = n_tok;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (entry_of(sorted[mid]) < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  if (lo < n_tok && entry_of(sorted[lo]) == v) atomicOr(bits, 1u << tid);
+}
+
 // CTAs of the first `sum_ctas`: a chunk of sorted tokens, kThreads * kVec columns.  A
 // run inside the chunk is written to the gradient; one that the border cuts to the
 // chunk's partial rows: [0] continues from the chunk before, [1] goes on in the next.
 // The others: 32 entries each, those without tokens zeroed.  kOwn (few tokens): no launch
 // has sorted them, every CTA does for itself.
-template <typename T, bool kOwn>
+// kRows: rows of whole 16 bytes.
+template <typename T, bool kOwn, bool kRows>
 __global__ void __launch_bounds__(kThreads, 4)
     embedding_grad_kernel(const int64_t* idx, int64_t padding, uint64_t* sorted, const T* dy,
-                          int64_t n_tok, int64_t V, int64_t D, float scale, int vec, int sum_ctas,
-                          int slices, T* grad, float* partial, uint32_t* status) {
+                          int64_t n_tok, int64_t V, int64_t D, float scale, int sum_ctas, int slices,
+                          T* grad, float* partial, uint32_t* status) {
   constexpr int kLen = kOwn ? kOwnChunk : kChunk;
   __shared__ uint64_t key[kLen + 2];  // with a neighbour on either side
   __shared__ __align__(16) uint32_t entries[kOwn ? kOwnTokens : 4];
@@ -321,19 +360,9 @@ __global__ void __launch_bounds__(kThreads, 4)
         const int64_t v = idx[i];
         if (v >= v0 && v < v0 + 32 && v < V && v != padding) atomicOr(has_tokens, 1u << (v - v0));
       }
-    } else if (threadIdx.x < 32) {  // a search for each entry
-      const uint32_t v = static_cast<uint32_t>(v0) + threadIdx.x;
-      int64_t lo = 0, hi = n_tok;
-      while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (entry_of(sorted[mid]) < v)
-          lo = mid + 1;
-        else
-          hi = mid;
-      }
-      const uint32_t found =
-          __ballot_sync(0xffffffffu, lo < n_tok && entry_of(sorted[lo]) == v);
-      if (threadIdx.x == 0) *has_tokens = found;
+    } else {
+      if (threadIdx.x == 0) *has_tokens = 0;
+      mark_entries(sorted, n_tok, static_cast<uint32_t>(v0), has_tokens);
     }
     __syncthreads();
     const uint32_t has = *has_tokens;
@@ -341,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     T* first = grad + v0 * D;
     const int len = static_cast<int>(D), total = rows * len;  // below 2^27
     constexpr int kStep = kThreads * kVec<T>;
-    if (vec != 0) {
+    if constexpr (kRows) {
       int row = static_cast<int>(threadIdx.x) * kVec<T> / len;
       int col = static_cast<int>(threadIdx.x) * kVec<T> % len;
       const int step_row = kStep / len, step_col = kStep % len;
@@ -354,20 +383,29 @@ __global__ void __launch_bounds__(kThreads, 4)
       }
       return;
     }
-    // the rows' elements in whole 16 bytes, from the boundary at or before the first
+    // the rows' elements in whole 16 bytes, from the boundary at or before the first;
+    // element e is at `col` of `row` (before the first: at a negative column)
     const int lead = static_cast<int>((reinterpret_cast<uintptr_t>(first) & 15u) / sizeof(T));
-    for (int e = static_cast<int>(threadIdx.x) * kVec<T> - lead; e < total; e += kStep) {
-      const int begin = e < 0 ? 0 : e, end = e + kVec<T> < total ? e + kVec<T> : total;
-      if (begin >= end) continue;
-      const int r0 = begin / len, r1 = (end - 1) / len;
-      // of these 16 bytes' rows (short rows: up to eight of them), whether some have tokens
-      const uint32_t span = (r1 - r0 == 31 ? ~0u : (1u << (r1 - r0 + 1)) - 1u) << r0;
-      if ((has & span) == 0 && end - e == kVec<T> && begin == e) {
-        *reinterpret_cast<uint4*>(first + e) = make_uint4(0, 0, 0, 0);
+    int e = static_cast<int>(threadIdx.x) * kVec<T> - lead;
+    int row = e < 0 ? 0 : e / len, col = e - row * len;
+    const int step_row = kStep / len, step_col = kStep % len;
+    for (; e < total; e += kStep) {
+      if (len >= kVec<T> && col >= 0 && e + kVec<T> <= total) {  // of one row or two
+        const bool two = col + kVec<T> > len;
+        const bool keep0 = (has >> row) & 1u, keep1 = two ? (has >> (row + 1)) & 1u : keep0;
+        if (!keep0 && !keep1) {
+          *reinterpret_cast<uint4*>(first + e) = make_uint4(0, 0, 0, 0);
+        } else if (!keep0 || !keep1) {
+          for (int i = keep0 ? len - col : 0; i < (keep1 ? len - col : kVec<T>); ++i)
+            first[e + i] = static_cast<T>(0.f);
+        }
       } else {
-        for (int i = begin; i < end; ++i)
+        for (int i = max(e, 0); i < min(e + kVec<T>, total); ++i)
           if (((has >> (i / len)) & 1u) == 0) first[i] = static_cast<T>(0.f);
       }
+      row += step_row, col += step_col;
+      if (col >= len) col -= len, ++row;
+      if (col < 0) col += len, --row;
     }
     return;
   }
@@ -395,12 +433,55 @@ __global__ void __launch_bounds__(kThreads, 4)
     key[threadIdx.x] = p >= 0 && p < n_tok ? (kOwn ? order[kOwn ? p : 0] : sorted[p]) : ~uint64_t{0};
   }
   __syncthreads();
-  const Cols c = thread_cols<T>(static_cast<int>(blockIdx.x) % slices, static_cast<int>(threadIdx.x),
-                                kThreads, vec != 0, D);
+  const int slice = static_cast<int>(blockIdx.x) % slices;
+  bool first_run = entry_of(key[0]) == entry_of(key[1]);  // begun in an earlier chunk
+  if constexpr (!kRows) {
+    const int64_t d = static_cast<int64_t>(slice) * kThreads * kOddCols + threadIdx.x;
+    if (d >= D) return;
+    constexpr int kAhead = 16;
+    float acc[kOddCols] = {};
+    for (int q0 = 0; q0 < n; q0 += kAhead) {
+      T row[kAhead][kOddCols];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const bool in = q0 + i < n && entry_of(key[q0 + i + 1]) != kNone;
+        const int64_t token = in ? static_cast<uint32_t>(key[q0 + i + 1]) : 0;
+        const T* src = dy + token * D + d;
+#pragma unroll
+        for (int k = 0; k < kOddCols; ++k)
+          row[i][k] = in && d + k * kThreads < D ? src[k * kThreads] : static_cast<T>(0.f);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int q = q0 + i;
+        if (q >= n) break;
+        const uint32_t e = entry_of(key[q + 1]);
+        if (e == kNone) return;
+#pragma unroll
+        for (int k = 0; k < kOddCols; ++k) acc[k] += static_cast<float>(row[i][k]);
+        const bool ends = entry_of(key[q + 2]) != e;
+        if (!ends && q + 1 < n) continue;
+        const bool whole = ends && !first_run;
+        T* out = grad + static_cast<int64_t>(e) * D + d;
+        float* part = partial + (chunk * 2 + (first_run ? 0 : 1)) * D + d;
+#pragma unroll
+        for (int k = 0; k < kOddCols; ++k) {
+          if (d + k * kThreads >= D) continue;
+          if (whole)
+            out[k * kThreads] = static_cast<T>(acc[k] * scale);
+          else
+            part[k * kThreads] = acc[k];
+          acc[k] = 0.f;
+        }
+        first_run = false;
+      }
+    }
+    return;
+  }
+  const Cols c = thread_cols<T>(slice, static_cast<int>(threadIdx.x), kThreads, true, D);
   if (!c.any()) return;
   constexpr int kAhead = 8;
   Vec<T> acc = {};
-  bool first_run = entry_of(key[0]) == entry_of(key[1]);  // begun in an earlier chunk
   for (int q0 = 0; q0 < n; q0 += kAhead) {
     uint4 row[kAhead];
 #pragma unroll
@@ -558,7 +639,7 @@ int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int6
     }
   }
   const int vec = D % kVec<T> == 0 && aligned(dy, 16) && aligned(grad, 16);
-  const int64_t cols = int64_t{kThreads} * kVec<T>;
+  const int64_t cols = int64_t{kThreads} * (vec ? kVec<T> : kOddCols);
   const int slices = static_cast<int>((D + cols - 1) / cols);
   const int64_t sum_ctas = chunks(n_tok) * slices;
   const int64_t grid = sum_ctas + (V + 31) / 32;
@@ -566,9 +647,11 @@ int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int6
     return fail(MLORA_ERR_UNSUPPORTED, "embedding gradient: too many tokens for rows this long");
   if (e == cudaSuccess) {
     LaunchScope scope(kKindElementwise, s);
-    e = launch_kernel(own ? embedding_grad_kernel<T, true> : embedding_grad_kernel<T, false>,
+    auto* kernel = vec ? embedding_grad_kernel<T, false, true> : embedding_grad_kernel<T, false, false>;
+    if (own) kernel = vec ? embedding_grad_kernel<T, true, true> : embedding_grad_kernel<T, true, false>;
+    e = launch_kernel(kernel,
                       dim3(static_cast<unsigned>(grid)), kThreads, 0, s, 0, 0, true, idx, padding,
-                      w.sorted, static_cast<const T*>(dy), n_tok, V, D, scale, vec,
+                      w.sorted, static_cast<const T*>(dy), n_tok, V, D, scale,
                       static_cast<int>(sum_ctas), slices, static_cast<T*>(grad), w.partial,
                       device_status_ptr());
   }
