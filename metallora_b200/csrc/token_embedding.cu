@@ -8,7 +8,7 @@
 // the CTAs that add them up, for want of a launch); of more,
 // blocks of 2048 are sorted in shared memory and each element finds its place by binary
 // searches in the other blocks (keys are distinct: the token is part of them).  Runs of equal entries
-// in the sorted order are summed by chunks of 32 tokens, so that an entry that half of
+// in the sorted order are summed by chunks of 16 or 32 tokens, so that an entry that half of
 // the batch holds is summed by many CTAs; a run that crosses a chunk's border leaves
 // fp32 partial sums, added in chunk order by a last pass.  The rows without tokens are
 // zeroed in the same launch as the sums: every row of the gradient is written once.
@@ -36,9 +36,11 @@ constexpr int64_t kPairTokens = 16384;
 constexpr int kRankThreads = 512;
 constexpr int kRankTokens = 64;  // of a CTA that counts pairs
 // Sorted tokens per CTA of the gradient: 32 (gradient of 2000 tokens, 20000x101: 15 us,
-// with 64 20 us, 16 13 us; of 16000 tokens, 1000x4095: 126, 118, 137 us), but 64 where one
-// chunk then does without the joining pass or it is short.
-constexpr int kChunk = 32, kOwnChunk = 64;
+// with 64 20 us, 16 13 us; of 16000 tokens, 1000x4095: 126, 118, 137 us); 16 where the
+// CTAs sort for themselves (64 tokens, 1000x512: 6.8 us, with 64 and no joining pass 12.4,
+// 32 8.8, 8 5.4; 512 tokens, 32000x4096: 49, 50, 46, 52; of one entry, 1x64: 17.5, 18.6,
+// 16.5, 22).
+constexpr int kChunk = 32, kOwnChunk = 16;
 constexpr int kOwnTokens = 512;  // up to which its CTAs sort them themselves
 constexpr uint32_t kNone = 0xFFFFFFFFu;  // entry of a token without a gradient
 
@@ -333,7 +335,8 @@ __device__ __forceinline__ void mark_entries(const uint64_t* sorted, int64_t n_t
   if (lo < n_tok && entry_of(sorted[lo]) == v) atomicOr(bits, 1u << tid);
 }
 
-// CTAs of the first `sum_ctas`: a chunk of sorted tokens, kThreads * kVec columns.  A
+// CTAs of the first `sum_ctas`: a chunk of sorted tokens, kThreads * kVec columns
+// (kThreads * kOddCols without kRows).  A
 // run inside the chunk is written to the gradient; one that the border cuts to the
 // chunk's partial rows: [0] continues from the chunk before, [1] goes on in the next.
 // The others: 32 entries each, those without tokens zeroed.  kOwn (few tokens): no launch
