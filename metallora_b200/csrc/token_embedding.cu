@@ -141,6 +141,56 @@ __device__ __forceinline__ Vec<T> load_partial(const float* row, const Cols& c) 
   return r;
 }
 
+// The 16 bytes that begin `skip` bytes (even, below 16) into two blocks of 16.
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, uint32_t skip) {
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 6; ++i) w[i] = skip & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i < 5; ++i) w[i] = skip & 4 ? w[i + 1] : w[i];
+  const uint32_t bits = (skip & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                    __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+}
+
+// A row that fits no 16 bytes, of a 16-bit type: its output's whole 16 bytes from the two
+// blocks that they lie in, the ends (and what lies in a block across the table's) by the
+// element.  8192 tokens of 4095 fp16 columns take 30 us, by the element 48, 3001 of 1001
+// 5.7 and 7.3; fp32, which moves four bytes by the element, would lose on short rows (16000
+// of 101 columns 6.8 and 5.8 us) what it wins on long ones (8192 of 4095 50 and 53).
+template <typename T>
+__device__ __forceinline__ void gather_odd(const T* src, T* dst, int D, float scale, int lane,
+                                           int row_threads, uintptr_t begin, uintptr_t end) {
+  const int to_block = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(dst) & 15)) & 15);
+  const int lead = min(to_block / static_cast<int>(sizeof(T)), D);
+  const int blocks = (D - lead) / kVec<T>;
+#pragma unroll 2
+  for (int j = lane; j < blocks; j += row_threads) {
+    const int e = lead + j * kVec<T>;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src + e), block = at & ~uintptr_t{15};
+    uint4 q;
+    if (block >= begin && block + 32 <= end) {
+      const uint4* from = reinterpret_cast<const uint4*>(block);
+      q = shifted(from[0], from[1], static_cast<uint32_t>(at & 15));
+    } else {
+      T* one = reinterpret_cast<T*>(&q);
+#pragma unroll
+      for (int i = 0; i < kVec<T>; ++i) one[i] = src[e + i];
+    }
+    Vec<T> r = {};
+    add_raw(r, q);
+    T* out = reinterpret_cast<T*>(&q);
+#pragma unroll
+    for (int i = 0; i < kVec<T>; ++i) out[i] = static_cast<T>(r.v[i] * scale);
+    *reinterpret_cast<uint4*>(dst + e) = q;
+  }
+  const int tail = lead + blocks * kVec<T>;  // the ends are below 16 bytes each
+  for (int j = lane; j < lead + D - tail; j += row_threads) {
+    const int e = j < lead ? j : tail + j - lead;
+    dst[e] = static_cast<T>(static_cast<float>(src[e]) * scale);
+  }
+}
+
 // One CTA: 256 / row_threads tokens, row_threads across a row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
@@ -155,6 +205,13 @@ __global__ void __launch_bounds__(kThreads)
   if (!ok && lane == 0) record_status(status, kDevBadIndex);
   const T* src = table + (ok ? v : 0) * D;
   T* dst = out + t * D;
+  if constexpr (sizeof(T) == 2) {
+    if (vec == 0 && ok) {
+      gather_odd(src, dst, static_cast<int>(D), scale, lane, row_threads,
+                 reinterpret_cast<uintptr_t>(table), reinterpret_cast<uintptr_t>(table + V * D));
+      return;
+    }
+  }
   for (int slice = 0;; ++slice) {
     const Cols c = thread_cols<T>(slice, lane, row_threads, vec != 0, D);
     if (!c.any()) break;
