@@ -37,11 +37,15 @@ constexpr int kRankThreads = 512;
 constexpr int kRankTokens = 64;  // of a CTA that counts pairs
 // Sorted tokens per CTA of the gradient: 32 (gradient of 2000 tokens, 20000x101: 15 us,
 // with 64 20 us, 16 13 us; of 16000 tokens, 1000x4095: 126, 118, 137 us); 16 where the
-// CTAs sort for themselves (64 tokens, 1000x512: 6.8 us, with 64 and no joining pass 12.4,
-// 32 8.8, 8 5.4; 512 tokens, 32000x4096: 49, 50, 46, 52; of one entry, 1x64: 17.5, 18.6,
-// 16.5, 22).
+// CTAs sort for themselves (300 tokens, 1000x512: 11.3 us, with 64 18.0, 32 12.9, 8 10.4;
+// 512 tokens, 32000x4096: 49, 50, 46, 52; of one entry, 1x64: 17.5, 18.6, 16.5, 22).
 constexpr int kChunk = 32, kOwnChunk = 16;
 constexpr int kOwnTokens = 512;  // up to which its CTAs sort them themselves
+// Up to which the CTA of a run's first token sums the whole run, with nothing to join: a
+// launch less, of the host's time too (3 us; 64 tokens, 1000x512, take 5.8 us, with the
+// joining pass 6.9).  An entry that is all of the batch is one CTA's work then (64 tokens,
+// 1x512: 13.5 us and 6.9), so longer batches are joined.
+constexpr int kWholeTokens = 64;
 constexpr uint32_t kNone = 0xFFFFFFFFu;  // entry of a token without a gradient
 
 // Columns of a thread that sums rows of no whole 16 bytes, kThreads apart, 16 rows of them
@@ -405,14 +409,14 @@ __global__ void __launch_bounds__(kThreads, 4)
                           int64_t n_tok, int64_t V, int64_t D, float scale, int sum_ctas, int slices,
                           T* grad, float* partial, uint32_t* status) {
   constexpr int kLen = kOwn ? kOwnChunk : kChunk;
-  __shared__ uint64_t key[kLen + 2];  // with a neighbour on either side
+  // the chunk, or the whole order, with a neighbour on either side
+  __shared__ uint64_t held[(kOwn ? kOwnTokens : kLen) + 2];
   __shared__ __align__(16) uint32_t entries[kOwn ? kOwnTokens : 4];
-  __shared__ uint64_t order[kOwn ? kOwnTokens : 1];
   grid_wait();
   launch_dependents();
   if (static_cast<int>(blockIdx.x) >= sum_ctas) {
     const int64_t v0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - sum_ctas) * 32;
-    uint32_t* const has_tokens = reinterpret_cast<uint32_t*>(key);
+    uint32_t* const has_tokens = reinterpret_cast<uint32_t*>(held);
     if constexpr (kOwn) {
       if (threadIdx.x == 0) *has_tokens = 0;
       __syncthreads();
@@ -471,7 +475,9 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
   const int64_t chunk = static_cast<int>(blockIdx.x) / slices;
   const int64_t p0 = chunk * kLen;
-  const int n = static_cast<int>(n_tok - p0 < kLen ? n_tok - p0 : kLen);
+  int n = static_cast<int>(n_tok - p0 < kLen ? n_tok - p0 : kLen);
+  const bool runs = kOwn && n_tok <= kWholeTokens;  // whole ones, of those that begin here
+  const uint64_t* const key = held + (kOwn ? p0 : 0);  // of token p at [p - p0 + 1]
   if constexpr (kOwn) {
     const int tokens = static_cast<int>(n_tok), padded = (tokens + 3) / 4 * 4;
     for (int i = threadIdx.x; i < padded; i += kThreads)
@@ -482,25 +488,33 @@ __global__ void __launch_bounds__(kThreads, 4)
       int place = count_ahead<1>(entries, padded, t, 0, mine);
       for (int i = t & ~3; i < min((t & ~3) + 4, tokens); ++i)
         place += i < t ? entries[i] <= mine : entries[i] < mine;
-      order[place] = make_key(mine, t);
+      held[place + 1] = make_key(mine, t);
+    }
+    if (threadIdx.x == 0) held[0] = held[tokens + 1] = ~uint64_t{0};
+    __syncthreads();
+    if (!runs && static_cast<int>(blockIdx.x) % slices == 0)  // for the pass that joins runs
+      for (int i = threadIdx.x; i < n; i += kThreads) sorted[p0 + i] = key[i + 1];
+  } else {
+    if (threadIdx.x < kLen + 2) {
+      const int64_t p = p0 + static_cast<int>(threadIdx.x) - 1;
+      held[threadIdx.x] = p >= 0 && p < n_tok ? sorted[p] : ~uint64_t{0};
     }
     __syncthreads();
-    if (static_cast<int>(blockIdx.x) % slices == 0)  // for the pass that joins runs
-      for (int i = threadIdx.x; i < n; i += kThreads) sorted[p0 + i] = order[p0 + i];
   }
-  if (threadIdx.x < kLen + 2) {
-    const int64_t p = p0 + static_cast<int>(threadIdx.x) - 1;
-    key[threadIdx.x] = p >= 0 && p < n_tok ? (kOwn ? order[kOwn ? p : 0] : sorted[p]) : ~uint64_t{0};
+  int begin = 0;
+  if (runs) {
+    while (begin < n && entry_of(key[begin]) == entry_of(key[begin + 1])) ++begin;
+    if (begin == n) return;
+    while (p0 + n < n_tok && entry_of(key[n]) == entry_of(key[n + 1])) ++n;
   }
-  __syncthreads();
   const int slice = static_cast<int>(blockIdx.x) % slices;
-  bool first_run = entry_of(key[0]) == entry_of(key[1]);  // begun in an earlier chunk
+  bool first_run = !runs && entry_of(key[0]) == entry_of(key[1]);  // begun in an earlier chunk
   if constexpr (!kRows) {
     const int64_t d = static_cast<int64_t>(slice) * kThreads * kOddCols + threadIdx.x;
     if (d >= D) return;
     constexpr int kAhead = 16;
     float acc[kOddCols] = {};
-    for (int q0 = 0; q0 < n; q0 += kAhead) {
+    for (int q0 = begin; q0 < n; q0 += kAhead) {
       T row[kAhead][kOddCols];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
@@ -542,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (!c.any()) return;
   constexpr int kAhead = 8;
   Vec<T> acc = {};
-  for (int q0 = 0; q0 < n; q0 += kAhead) {
+  for (int q0 = begin; q0 < n; q0 += kAhead) {
     uint4 row[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -715,7 +729,7 @@ int gradient(const int64_t* idx, const void* dy, void* grad, int64_t n_tok, int6
                       static_cast<int>(sum_ctas), slices, static_cast<T*>(grad), w.partial,
                       device_status_ptr());
   }
-  if (e == cudaSuccess && chunks(n_tok) > 1) {
+  if (e == cudaSuccess && n_tok > kWholeTokens) {
     LaunchScope scope(kKindElementwise, s);
     e = launch_kernel(embedding_join_kernel<T>,
                       dim3(static_cast<unsigned>(chunks(n_tok) - 1),

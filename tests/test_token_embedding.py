@@ -232,3 +232,41 @@ def test_offsets_past_32_bits(cuda):
     assert torch.equal(grad[v - 1], (dy[1].float() + dy[3].float()).to(FP16))
     assert torch.count_nonzero(grad[8:v - 2]) == 0
 
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_rows_at_every_offset(cuda, dtype):
+    """Rows that begin and end anywhere in 16 bytes, the table's first and last among them;
+    a scale of two is exact."""
+    for d in (*range(1, 20), 31, 33, 63, 65, 130, 257, 1001, 2049, 4097):
+        for start in (0, 1, 3, 7):
+            held = torch.randn(start + 5 * d, device=cuda).to(dtype)
+            table = held[start:].view(5, d)
+            idx = torch.tensor([4, 0, 2, 4, 1, 3, 0], device=cuda)
+            assert torch.equal(kernels.embedding_fwd(idx, table, 2.0), table[idx] * 2)
+    _lib.device_status(reset=True)
+    idx = torch.tensor([4, 9, 0, -1], device=cuda)  # two of no row of this table
+    out = kernels.embedding_fwd(idx, table, 2.0)
+    torch.cuda.synchronize()
+    assert _lib.device_status(reset=True) == 0x107
+    assert torch.equal(out[::2], table[[4, 0]] * 2) and not out[1::2].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1, 15, 16, 17, 32, 33, 48, 63, 64, 65, 80, 512, 513])
+def test_runs_across_chunks(cuda, t):
+    """Runs that begin, end and go on at every border; fp32 sums of at most t terms are off
+    by (t - 1) additions, the scale and the store: under (t + 1) half steps of the
+    terms' magnitudes."""
+    g = torch.Generator(device="cuda").manual_seed(t)
+    for v, d in ((1, 36), (2, 37), (5, 600), (40, 512), (1000, 1030)):
+        dy = torch.randn(t, d, device=cuda, generator=g)
+        idx = torch.randint(0, v, (t,), device=cuda, generator=g)
+        padding = 0 if v == 5 else None
+        grad = kernels.embedding_bwd(dy, idx, v, 3.0, padding)
+        terms = dy.double() if padding is None else dy.double() * (idx != padding)[:, None]
+        want, size = (torch.zeros(v, d, device=cuda, dtype=torch.float64).index_add_(0, idx, 3 * x)
+                      for x in (terms, terms.abs()))
+        assert ((grad.double() - want).abs() <= (t + 1) * torch.finfo(torch.float32).eps / 2 * size).all()
+        assert torch.equal(grad, kernels.embedding_bwd(dy, idx, v, 3.0, padding))
