@@ -403,8 +403,9 @@ __device__ __forceinline__ void mark_entries(const uint64_t* sorted, int64_t n_t
 // The others: 32 entries each, those without tokens zeroed.  kOwn (few tokens): no launch
 // has sorted them, every CTA does for itself.
 // kRows: rows of whole 16 bytes.
+// (kOwn needs more registers, and has fewer CTAs.)
 template <typename T, bool kOwn, bool kRows>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, kOwn ? 3 : 4)
     embedding_grad_kernel(const int64_t* idx, int64_t padding, uint64_t* sorted, const T* dy,
                           int64_t n_tok, int64_t V, int64_t D, float scale, int sum_ctas, int slices,
                           T* grad, float* partial, uint32_t* status) {
