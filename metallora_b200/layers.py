@@ -19,6 +19,10 @@ from .logging import logger
 from .ops import embedding, lora_forward, merge_lora_weights, qlora_forward
 
 
+# Training forwards of a layer whose masks' numbers a recomputation can still ask for.
+_KEPT_CALLS = 1024
+
+
 class LoRALinear(nn.Module):
     """Linear layer with LoRA adaptation: ``h = x.W0^T + (alpha/rank).(x.A^T).B^T``.
 
@@ -30,12 +34,17 @@ class LoRALinear(nn.Module):
     by ``quant.checkpoint_activation`` that several layers share.
     ``dropout_seed`` (an int, or a CUDA int64 tensor of one element) takes the dropout's
     masks from the counter-based generator (see ``ops.dropout``); each training
-    forward uses the next ``dropout_call``, which starts at 0 and may be set.
+    forward uses the next ``dropout_call``, which starts at 0 and may be set.  One that
+    torch.utils.checkpoint runs again in a backward uses the first run's: such a forward
+    draws a number from torch's CPU generator, whose state the checkpoint puts back, and
+    is known by it.  Where that says nothing (``preserve_rng_state=False``, a generator
+    seeded alike before two calls) the forward in the backward is refused.
     """
 
     # of layers pickled without them
     dropout_seed = None
     dropout_call = 0
+    _calls_by_draw = None
 
     def __init__(self, in_features: int, out_features: int, rank: int = 8, alpha: float = 16.0,
                  dropout: float = 0.0, use_bias: bool = False, freeze_base: bool = True,
@@ -86,6 +95,28 @@ class LoRALinear(nn.Module):
     def scale(self) -> float:
         return self.alpha / self.rank
 
+    def _mask_call(self) -> int:
+        """The number of this training forward's mask: the next one, or in a backward the
+        one that the forward had which drew the same from the generator."""
+        draw = int(torch.randint(1 << 62, (), device="cpu"))
+        if self._calls_by_draw is None:
+            self._calls_by_draw = {}
+        known = self._calls_by_draw
+        if torch._C._current_graph_task_id() < 0:
+            call = self.dropout_call
+            self.dropout_call += 1
+            known[draw] = call if known.get(draw, call) == call else None
+            if len(known) > _KEPT_CALLS:
+                del known[next(iter(known))]
+            return call
+        call = known.get(draw)
+        if call is None:
+            raise ConfigurationError(
+                "counter-based LoRA dropout: a forward that is run again in the backward is known by "
+                "the state of torch's CPU generator, which no forward, or two with different "
+                f"masks, of the last {_KEPT_CALLS} had")
+        return call
+
     def forward(self, x: torch.Tensor, checkpoint=None) -> torch.Tensor:
         """layers.py:83-106: any leading shape; the bias is added after the op."""
         if checkpoint is None and torch.is_grad_enabled():
@@ -94,8 +125,7 @@ class LoRALinear(nn.Module):
         if self.dropout_seed is not None and self.training and self.dropout > 0 and not self.merged:
             if self.qweight is not None:
                 raise ConfigurationError("counter-based LoRA dropout needs a dense base")
-            drop = {"dropout_seed": self.dropout_seed, "dropout_call": self.dropout_call}
-            self.dropout_call += 1
+            drop = {"dropout_seed": self.dropout_seed, "dropout_call": self._mask_call()}
         if self.qweight is not None:
             out = qlora_forward(x, self.qweight, self.A, self.B, alpha=self.alpha,
                                 _compute=self._compute_ab, _sink=self._grad_sink,
