@@ -526,7 +526,8 @@ class LoRATrainer:
     def save(self, path: str | Path) -> None:
         """trainer.py:291-297: ``adapter.safetensors`` with ``{name}.lora_A`` /
         ``{name}.lora_B`` and ``config.json`` = {rank, alpha}; the optimizer
-        state goes to ``optimizer.safetensors`` so training can resume."""
+        state goes to ``optimizer.safetensors`` so training can resume, and the numbers
+        of the layers' next dropout masks, where they are counted, to ``config.json``."""
         from safetensors.torch import save_file
         p = Path(path)
         p.mkdir(parents=True, exist_ok=True)
@@ -537,12 +538,17 @@ class LoRATrainer:
         save_file(tensors, str(p / "adapter.safetensors"))
         opt = {k: v.detach().contiguous().cpu() for k, v in self.optimizer.state_dict().items()}
         save_file(opt, str(p / "optimizer.safetensors"))
+        config = {"rank": self.config.rank, "alpha": self.config.alpha,
+                  "global_step": self.state.global_step}
+        calls = {n: m.dropout_call for n, m in self.params.layers if m.dropout_seed is not None}
+        if calls:
+            config["dropout_calls"] = calls
         with open(p / "config.json", "w") as f:
-            json.dump({"rank": self.config.rank, "alpha": self.config.alpha,
-                       "global_step": self.state.global_step}, f)
+            json.dump(config, f)
 
     def load(self, path: str | Path) -> None:
-        """trainer.py:299-302 (plus the optimizer state when present)."""
+        """trainer.py:299-302 (plus the optimizer state and the numbers of the dropout
+        masks when present)."""
         from safetensors.torch import load_file
         p = Path(path)
         tensors = load_file(str(p / "adapter.safetensors"))
@@ -555,6 +561,10 @@ class LoRATrainer:
             sd = load_file(str(p / "optimizer.safetensors"))
             self.optimizer.load_state_dict({k: v.to(self.params.master.device)
                                             for k, v in sd.items()})
+        if (p / "config.json").is_file():
+            calls = json.loads((p / "config.json").read_text()).get("dropout_calls", {})
+            for name, m in self.params.layers:
+                m.dropout_call = int(calls.get(name, m.dropout_call))
         self.params.refresh_compute()
         logger.info(f"loaded adapter from {p}")
 

@@ -1,6 +1,7 @@
-"""Counter-based LoRA dropout where torch.utils.checkpoint runs the forward again: the
-masks are the first run's."""
+"""Counter-based LoRA dropout where torch.utils.checkpoint runs the forward again, and
+where a run is saved and resumed: the masks are those of the unbroken run."""
 import copy
+import json
 import pickle
 
 import pytest
@@ -10,6 +11,8 @@ from torch.utils.checkpoint import checkpoint
 from metallora_b200 import layers as layers_module
 from metallora_b200.exceptions import ConfigurationError
 from metallora_b200.layers import LoRALinear
+from metallora_b200.trainer import LoRATrainer, TrainingConfig
+from tests.test_training_ends import Model
 
 BF16 = torch.bfloat16
 
@@ -107,6 +110,37 @@ def test_what_a_layer_keeps_is_bounded_and_copied(monkeypatch):
         assert twin._mask_call() == 5 and p.dropout_call == 5
 
 
+def _trainer(path, seed=5, device="cpu", **kw):
+    torch.manual_seed(0)
+    return LoRATrainer(Model(device=device, **kw),
+                       TrainingConfig(rank=8, dropout=0.3, dropout_seed=seed, loss_head="lm_head",
+                                      learning_rate=1e-2, output_dir=str(path)))
+
+
+def test_numbers_of_masks_are_saved(tmp_path):
+    trainer = _trainer(tmp_path)
+    for i, (_, m) in enumerate(trainer.params.layers):
+        m.dropout_call = 7 + i
+    trainer.save(tmp_path / "c")
+    other = _trainer(tmp_path)
+    other.load(tmp_path / "c")
+    assert [m.dropout_call for _, m in other.params.layers] == [7, 8]
+    # what was saved without them loads as it did
+    config = json.loads((tmp_path / "c" / "config.json").read_text())
+    assert config.pop("dropout_calls") == {"q_proj": 7, "v_proj": 8}
+    (tmp_path / "c" / "config.json").write_text(json.dumps(config))
+    again = _trainer(tmp_path)
+    again.load(tmp_path / "c")
+    (tmp_path / "c" / "config.json").unlink()
+    again.load(tmp_path / "c")
+    assert [m.dropout_call for _, m in again.params.layers] == [0, 0]
+    # layers without counted masks leave the file as it was
+    plain = _trainer(tmp_path, seed=None)
+    plain.save(tmp_path / "p")
+    assert set(json.loads((tmp_path / "p" / "config.json").read_text())) == \
+        {"rank", "alpha", "global_step"}
+
+
 # ------------------------------------------------------------------ GPU --
 
 @pytest.mark.gpu
@@ -115,3 +149,23 @@ def test_recomputed_forwards_on_the_gpu(cuda, reentrant):
     pair = _pair(cuda, BF16)
     for u, v in zip(_gradients(pair, reentrant), _gradients(pair, None)):
         assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
+def test_a_resumed_run_is_the_unbroken_one(cuda, tmp_path):
+    def batch(i):
+        gen = torch.Generator(device=cuda).manual_seed(i)
+        ids = torch.randint(0, 1003, (2, 40), device=cuda, generator=gen)
+        return {"input_ids": ids, "labels": ids}
+
+    runs = []
+    for broken in (False, True):
+        trainer = _trainer(tmp_path, device=cuda)
+        for i in range(4):
+            if broken and i == 2:
+                trainer.save(tmp_path / "c")
+                trainer = _trainer(tmp_path, device=cuda)
+                trainer.load(tmp_path / "c")
+            trainer._training_step(batch(i))
+        runs.append(trainer.params.master.clone())
+    assert torch.equal(*runs)
