@@ -72,7 +72,8 @@ MLORA_API int mlora_device_supported(int device);
 /* Reads (and with reset != 0 clears) the status word of the current device.
  * *out = 0 when no kernel has recorded a fault: 0x101-0x106 a bounded wait
  * timed out (the kernel gave up instead of hanging); 0x107 a gathered row
- * index was outside its table; 0x108 a peer GPU missed a barrier.  Synchronous. */
+ * index was outside its table (which stops no kernel; another code takes its
+ * place); 0x108 a peer GPU missed a barrier.  Synchronous. */
 MLORA_API int mlora_device_status(uint32_t* out, int reset);
 
 /* ---- measurement ------------------------------------------------------- */

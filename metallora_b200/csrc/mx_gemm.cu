@@ -508,7 +508,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   // After a failure the odd CTA may still have copies in flight that no barrier
   // of its own tracks: give them time to land before the pair exits.
-  if (p.status != nullptr && *reinterpret_cast<volatile uint32_t*>(p.status) != 0) {
+  if (wait_failed(p.status)) {
     const uint64_t t0 = globaltimer_ns();
     while (globaltimer_ns() - t0 < 200000ull) {
     }

@@ -55,8 +55,12 @@ __device__ __forceinline__ uint64_t globaltimer_ns() {
   return t;
 }
 
+// The first code stands, but an index outside its table, which loses no arrival, gives
+// way to a wait that has run out.
 __device__ __forceinline__ void record_status(uint32_t* status, uint32_t code) {
-  if (status != nullptr) atomicCAS(status, 0u, code);
+  if (status == nullptr) return;
+  if (atomicCAS(status, 0u, code) == kDevBadIndex && code != kDevBadIndex)
+    atomicCAS(status, static_cast<uint32_t>(kDevBadIndex), code);
 }
 
 // ------------------------------------------------ programmatic dependent launch --
