@@ -399,8 +399,9 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2d, w, a, b, labels, plan):
-        alpha, ignore_index, reduction, compute, sink = plan
-        need = ctx.needs_input_grad
+        alpha, ignore_index, reduction, compute, sink, grad_mode = plan
+        # (what needs_input_grad says holds under no_grad too)
+        need = ctx.needs_input_grad if grad_mode else (False,) * 4
         grads = (_lib.HEAD_GRAD_X if need[0] else 0) | (_lib.HEAD_GRAD_W if need[1] else 0)
         a_c = b_c = None
         if a is not None:
@@ -480,7 +481,8 @@ def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,
         return loss if flat or reduction != "none" else loss.reshape(labels.shape)
     loss = _LinearCrossEntropyFn.apply(x if flat else x.reshape(-1, x.shape[-1]), weight, A, B,
                                        labels if flat else labels.reshape(-1),
-                                       (float(alpha), ignore_index, reduction, _compute, _sink))
+                                       (float(alpha), ignore_index, reduction, _compute, _sink,
+                                        torch.is_grad_enabled()))
     return loss if flat or reduction != "none" else loss.reshape(labels.shape)
 
 
