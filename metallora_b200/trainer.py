@@ -312,8 +312,8 @@ def _check_loss_head(model: nn.Module, c: TrainingConfig) -> None:
         return
     head = dict(model.named_modules()).get(c.loss_head)
     if isinstance(head, LoRALinear):
-        dense = head.qweight is None
-        weight, dropout = head.W0, head.dropout if head.training and not head.merged else 0.0
+        dense, adapted = head.qweight is None, not head.merged
+        weight, dropout = head.W0, head.dropout if head.training and adapted else 0.0
     elif isinstance(head, nn.Linear):
         dense, weight = True, head.weight
         made = not any(isinstance(m, LoRALinear) for m in model.modules())
@@ -328,6 +328,9 @@ def _check_loss_head(model: nn.Module, c: TrainingConfig) -> None:
     if weight.dtype not in (torch.bfloat16, torch.float16) or weight.shape[1] % 8:
         raise ConfigurationError(f"loss_head {c.loss_head!r} needs a bf16 or fp16 weight with "
                                  "in_features in multiples of 8")
+    if weight.shape[0] > 1 << 20 or (adapted and weight.shape[0] % 8):
+        raise ConfigurationError(f"loss_head {c.loss_head!r} needs at most 2^20 out_features, and "
+                                 "with LoRA factors a multiple of 8")
 
 
 def _check_dropout_seed(model: nn.Module, c: TrainingConfig) -> None:
