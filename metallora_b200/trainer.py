@@ -428,6 +428,9 @@ class LoRATrainer:
         """The shifted cross-entropy of ``_compute_loss`` from the head's input: the
         head hands its input through, and each position's label is the next one's."""
         head = self.model.get_submodule(self.config.loss_head)
+        if isinstance(head, LoRALinear) and head.training and head.dropout > 0 and not head.merged:
+            raise ConfigurationError(f"loss_head {self.config.loss_head!r} has dropout, which its "
+                                     "loss does not take: set it to 0, or to eval()")
         seen = []
 
         def through(x, *args, **kwargs):

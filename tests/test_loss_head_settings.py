@@ -34,3 +34,30 @@ def test_heads_of_sizes_that_the_loss_refuses(tmp_path):
         make(model)
     model.lm_head.merged = True
     make(model)
+
+
+def _loss_of(monkeypatch, head, tmp_path, ready=lambda model: None):
+    """The trainer's loss with the operator replaced by torch's, on the CPU."""
+    def loss(x, weight, labels, A=None, B=None, alpha=16.0, _compute=None, _sink=None):  # noqa: N803
+        return nn.functional.cross_entropy((x @ weight.T).float().flatten(0, 1), labels.flatten())
+    monkeypatch.setattr("metallora_b200.trainer.linear_cross_entropy", loss)
+    monkeypatch.setattr("metallora_b200.layers.lora_forward", lambda x, w0, *a, **kw: x @ w0.T)
+    model = nn.Sequential()
+    model.embed, model.lm_head = nn.Embedding(64, 16, dtype=BF16), head
+    ready(model)
+    trainer = LoRATrainer(model, TrainingConfig(output_dir=str(tmp_path), loss_head="lm_head",
+                                                target_modules=["lm_head"]))
+    ids = torch.arange(8).reshape(2, 4)
+    return trainer, lambda: trainer._compute_loss({"input_ids": ids, "labels": ids})
+
+
+def test_a_head_with_dropout_is_refused_when_it_trains(monkeypatch, tmp_path):
+    """Put to train() after the trainer was made; in eval() its dropout takes no part."""
+    head = LoRALinear(16, 64, rank=8, dropout=0.5, dtype=BF16)
+    _, loss = _loss_of(monkeypatch, head, tmp_path, ready=lambda model: model.eval())
+    assert torch.isfinite(loss())
+    head.train()
+    with pytest.raises(ConfigurationError, match="dropout"):
+        loss()
+    head.merged = True
+    assert torch.isfinite(loss())
