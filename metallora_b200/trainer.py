@@ -431,6 +431,7 @@ class LoRATrainer:
         if isinstance(head, LoRALinear) and head.training and head.dropout > 0 and not head.merged:
             raise ConfigurationError(f"loss_head {self.config.loss_head!r} has dropout, which its "
                                      "loss does not take: set it to 0, or to eval()")
+        own = vars(head).get("forward")
         seen = []
 
         def through(x, *args, **kwargs):
@@ -441,7 +442,10 @@ class LoRATrainer:
         try:
             hidden = self.model(batch["input_ids"])
         finally:
-            del head.forward
+            if own is None:
+                del head.forward
+            else:
+                head.forward = own
         if len(seen) != 1 or hidden is not seen[0]:
             raise ConfigurationError(f"the model does not return the output of "
                                      f"{self.config.loss_head!r} as it is")

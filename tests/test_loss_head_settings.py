@@ -61,3 +61,13 @@ def test_a_head_with_dropout_is_refused_when_it_trains(monkeypatch, tmp_path):
         loss()
     head.merged = True
     assert torch.isfinite(loss())
+
+
+def test_a_heads_own_forward_is_given_back(monkeypatch, tmp_path):
+    head = LoRALinear(16, 64, rank=8, dtype=BF16)
+    _, loss = _loss_of(monkeypatch, head, tmp_path)
+    loss()
+    assert "forward" not in vars(head)
+    head.forward = wrapped = lambda x: LoRALinear.forward(head, x)
+    loss()
+    assert vars(head)["forward"] is wrapped
