@@ -356,8 +356,9 @@ constexpr int kHalfTile = 128;
 // e[v] -> g[v] = 2^-15 e[v] exp(m_t - lse).  With the sum S exp(m) over
 // the other entries and u = S exp(m - l_y), the loss is log(1 + u) and
 // g[y] = -u / (1 + u), without cancellation for a token that is nearly certain.
-// What rounding g[y], the largest part, left over goes to `rest`, which the gradient
-// of x adds back times W[y].  Bound: HBM, 4 bytes a logit.
+// What rounding g[y], the largest part, left over goes to `rest` (0 for tokens that do not
+// count), which every gradient adds back: dx times W[y], U times B[y], rows y of dW and dB
+// times x and s x A^T.  Bound: HBM, 4 bytes a logit.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads)
     head_row_kernel(const float2* stats, int64_t V, int64_t ld, int64_t row0, Numbers num,
@@ -375,6 +376,7 @@ __global__ void __launch_bounds__(kRowThreads)
   if (slot >= counted) {
     if (eg != nullptr && (zero_all || slot < (counted + 63) / 64 * 64))
       for (int64_t v = threadIdx.x; v < ld / 8; v += kRowThreads) row[v] = make_uint4(0, 0, 0, 0);
+    if (eg != nullptr && threadIdx.x == 0) rest[slot] = 0.f;
     finish_loss(out, num.count);
     return;
   }
@@ -450,6 +452,70 @@ __global__ void __launch_bounds__(kRowThreads)
       row[q] = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]),
                           pack2<T>(o[6], o[7]));
     }
+  }
+}
+
+// out[y] += the sum of rest[i] src[i] over the counted tokens i of label y, in token order:
+// what rounding their g[y] left over, of which row y of dW and dB would show all where
+// y has few tokens (with one, up to the half step that rounding the row adds again).
+// src rows have `cols` columns and, with `second`, their second part that far behind.
+// A CTA per token and 2048 columns; the label's first token does the work of all.
+// Searching for it and for the others reads 4 bytes for each pair of a token and
+// a label's first one, where the products moved 6 for each pair of a token and an entry.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads)
+    head_rest_kernel(Numbers num, const float* rest, const T* src, int64_t ld, int second, int64_t cols,
+                     float* out) {
+  __shared__ uint32_t same[kRowThreads / 32];
+  grid_wait();
+  launch_dependents();
+  const int64_t counted = num.count->counted;
+  const int64_t slot = blockIdx.x;
+  if (slot >= counted) return;
+  const int32_t y = num.label[slot];
+  constexpr int kAhead = 4;
+  for (int64_t j0 = 0; j0 < slot; j0 += kAhead * kRowThreads) {
+    bool found = false;
+#pragma unroll
+    for (int a = 0; a < kAhead; ++a) {
+      const int64_t j = j0 + a * kRowThreads + threadIdx.x;
+      if (j < slot) found |= num.label[j] == y;
+    }
+    if (__syncthreads_or(found)) return;
+  }
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * kRowThreads + threadIdx.x) * 8;
+  float acc[8] = {};
+  for (int64_t j0 = slot; j0 < counted; j0 += kRowThreads) {
+    const int64_t j = j0 + threadIdx.x;
+    const uint32_t votes = __ballot_sync(0xffffffffu, j < counted && num.label[j] == y);
+    if ((threadIdx.x & 31) == 0) same[threadIdx.x >> 5] = votes;
+    __syncthreads();
+    if (c < cols) {
+      for (int w = 0; w < kRowThreads / 32; ++w) {
+        for (uint32_t bits = same[w]; bits != 0; bits &= bits - 1) {
+          const int64_t i = j0 + w * 32 + (__ffs(static_cast<int>(bits)) - 1);
+          const float left = rest[i];
+          const uint4 q = *reinterpret_cast<const uint4*>(src + i * ld + c);
+          const T* e = reinterpret_cast<const T*>(&q);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = fmaf(left, static_cast<float>(e[k]), acc[k]);
+          if (second == 0) continue;
+          const uint4 q2 = *reinterpret_cast<const uint4*>(src + i * ld + second + c);
+          const T* e2 = reinterpret_cast<const T*>(&q2);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) acc[k] = fmaf(left, static_cast<float>(e2[k]), acc[k]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (c >= cols) return;
+  float4* row = reinterpret_cast<float4*>(out + static_cast<int64_t>(y) * cols + c);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float4 v = row[h];
+    v.x += acc[4 * h], v.y += acc[4 * h + 1], v.z += acc[4 * h + 2], v.w += acc[4 * h + 3];
+    row[h] = v;
   }
 }
 
@@ -812,6 +878,10 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       ru.out_t = ws.u_t;
       ru.out_t_lo = ws.u_lo;
       ru.ld_t = round_up(ws.piece, 8);
+      ru.add_weight = st.rest + row0;
+      ru.add_row = st.label + row0;
+      ru.add = b;
+      ru.add_cols = d.r;
       ru.splits = rank_splits(rows, V);
       if ((rc = launch_rank(ru, s))) return rc;
       if (d.want(MLORA_HEAD_GRAD_AB)) {
@@ -893,6 +963,19 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       if ((rc = launch_head_gemm(q, s))) return rc;
     }
   }
+  auto add_rest = [&](const void* src, int64_t ld_src, int second, int64_t cols, float* out_rows) {
+    LaunchScope scope(kKindElementwise, s);
+    const int64_t width = kRowThreads * 8;
+    const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((cols + width - 1) / width));
+    return launch_status(launch_kernel(head_rest_kernel<T>, grid, kRowThreads, 0, s, 0, 0, true, num,
+                                       static_cast<const float*>(st.rest), static_cast<const T*>(src),
+                                       ld_src, second, cols, out_rows),
+                         "linear cross entropy: rest of the label's entry");
+  };
+  if (d.want(MLORA_HEAD_GRAD_W) && (rc = add_rest(ws.xc, ldx, 0, K, st.dw))) return rc;
+  if (d.want(MLORA_HEAD_GRAD_AB) &&
+      (rc = add_rest(ws.xa_rows, d.ld_xa(), static_cast<int>(d.R()), d.r, st.db)))
+    return rc;
   return MLORA_OK;
 }
 

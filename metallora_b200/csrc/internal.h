@@ -184,6 +184,12 @@ struct RankArgs {
   // of out_rows, g = row_group[m] (nullptr: all columns)
   const int32_t* row_group = nullptr;
   int64_t group_cols = 0;
+  // row m's sums take add_weight[m] times row add_row[m] of add [., add_cols] (16 bit, an
+  // even number of columns) before they are scaled; add_row is not read where that is 0
+  const float* add_weight = nullptr;
+  const int32_t* add_row = nullptr;
+  const void* add = nullptr;
+  int64_t add_cols = 0;
 };
 int rank_splits(int64_t M, int64_t K);
 int launch_rank(const RankArgs& a, cudaStream_t stream);

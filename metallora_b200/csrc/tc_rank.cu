@@ -156,11 +156,16 @@ struct RankParams {
   uint32_t* status;
   const int32_t* row_group;  // optional: keep only columns [g*group_cols, (g+1)*group_cols)
   int group_cols;
+  // kAdd: row m's sums take add_weight[m] (where that is not 0) times row add_row[m] of add
+  const float* add_weight;
+  const int32_t* add_row;
+  const void* add;
+  int add_cols;
 };
 
 // Grid (tiles, splits), cluster (1, splits, 1): the splits of one 128-row tile
 // are one cluster.
-template <int R, bool kBF16>
+template <int R, bool kBF16, bool kAdd>
 __global__ void __launch_bounds__(kThreads, 2)
     rank_proj_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ CUtensorMap tm_l,
                      const RankParams p) {
@@ -212,8 +217,21 @@ __global__ void __launch_bounds__(kThreads, 2)
   int group = -1;
   if (epi && p.row_group != nullptr && row < p.M) group = p.row_group[row];
   const bool live = epi && row < p.M;
+  float weight = 0.f;
+  const T* added = nullptr;
+  if constexpr (kAdd) {
+    if (live) weight = p.add_weight[row];
+    if (weight != 0.f)
+      added = static_cast<const T*>(p.add) + static_cast<int64_t>(p.add_row[row]) * p.add_cols;
+  }
   auto emit = [&](int j, float v0, float v1) {
     if (!live) return;
+    if constexpr (kAdd) {
+      if (weight != 0.f && j < p.add_cols) {  // (an even number of columns)
+        v0 = fmaf(weight, static_cast<float>(added[j]), v0);
+        v1 = fmaf(weight, static_cast<float>(added[j + 1]), v1);
+      }
+    }
     v0 *= p.scale;
     v1 *= p.scale;
     if (p.split_out) {
@@ -470,7 +488,11 @@ int launch_rank_typed(const RankArgs& a, cudaStream_t stream) {
   p.status = device_status_ptr();
   p.row_group = a.row_group;
   p.group_cols = a.group_cols > 0 ? static_cast<int>(a.group_cols) : R;
-  auto kern = rank_proj_kernel<R, kBF16>;
+  p.add_weight = a.add_weight;
+  p.add_row = a.add_row;
+  p.add = a.add;
+  p.add_cols = static_cast<int>(a.add_cols);
+  auto kern = a.add_weight != nullptr ? rank_proj_kernel<R, kBF16, true> : rank_proj_kernel<R, kBF16, false>;
   if (!set_smem_attr(kern, smem_bytes(R))) return MLORA_ERR_CUDA;
   dim3 grid(static_cast<unsigned>((a.M + 127) / 128), static_cast<unsigned>(a.splits));
   LaunchScope scope(kKindRank, stream);

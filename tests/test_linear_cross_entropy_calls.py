@@ -60,3 +60,77 @@ def test_a_lora_head_under_no_grad_takes_less_memory(cuda):
     with torch.no_grad():
         least, got = peak()
     assert torch.equal(got, want) and most > 2048 * 16384 * 2 > 8 * least
+
+
+def _few(cuda, dtype, m, seed, v=2000, k=64, r=8):
+    """A few tokens, one of them not counted, two of one label, and what 64 bits make of them."""
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+
+    def randn(*s, scale):
+        return (torch.randn(*s, device=cuda, generator=gen) * scale).to(dtype)
+    x, w = randn(m, k, scale=1.0), randn(v, k, scale=0.2)
+    a, b = randn(r, k, scale=0.1), randn(v, r, scale=0.3)
+    y = torch.randint(0, v, (m,), device=cuda, generator=gen)
+    if m > 2:
+        y[2], y[1] = y[0], IGNORE
+    return x, w, a, b, y
+
+
+def _gradient(x, w, a, b, y, s):
+    """Logits' gradient of the summed loss, its part at the labels, and s x A^T, in 64 bits."""
+    xa = s * x.double() @ a.double().T
+    rows = (y != IGNORE).nonzero()[:, 0]
+    g = torch.softmax(x.double() @ w.double().T + xa @ b.double().T, 1)
+    at = torch.zeros_like(g)
+    g[rows, y[rows]] -= 1
+    at[rows, y[rows]] = g[rows, y[rows]]
+    g[y == IGNORE] = 0
+    return g, at, xa
+
+
+# relative error of softmax's values: ex2.approx, logits of up to 15 cut by 2^-19 at each of
+# the sum's few steps, exp and log of them
+SOFT = 2.0 ** -14
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m", [1, 2, 5])
+def test_gradients_of_weights_from_few_tokens(cuda, dtype, m):
+    """The label's entry of the logits' gradient, nearly all of a row of dW and dB where its
+    label has one token, is not seen rounded: those rows are off by their own rounding."""
+    half = torch.finfo(dtype).eps / 2
+    # entries but the label's are rounded twice: the exponentials are fp16 values (off by
+    # 2^-11 at most), and g, that times the row's factor, is one of the type's
+    twice = half + 2.0 ** -11 + SOFT
+    tiny = torch.finfo(dtype).smallest_normal * half if dtype == FP16 else 0.0
+    for seed in range(8):
+        x, w, a, b, y = _few(cuda, dtype, m, seed)
+        no = torch.zeros_like(a), torch.zeros_like(b)
+        g, at, _ = _gradient(x, w, *no, y, 0.0)
+        w1 = w.clone().requires_grad_(True)
+        dw = torch.autograd.grad(ops.linear_cross_entropy(x, w1, y, reduction="sum"), w1)[0].double()
+        want = g.T @ x.double()
+        # (fp16: 64 g is kept, its subnormals are off by 2^-31 of g)
+        rest = (g - at).abs().T @ x.double().abs()
+        bound = (half + SOFT) * want.abs() + twice * rest * (1 + half) + 2 * tiny + SOFT * (
+            at.abs().T @ x.double().abs())
+        assert bool(((dw - want).abs() <= bound).all()), (seed, m)
+        # a LoRA head: the others' roundings are many and of random sign, six deviations
+        s = 2.0
+        g, at, xa = _gradient(x, w, a, b, y, s)
+        leaves = [t.clone().requires_grad_(True) for t in (a, b)]
+        loss = ops.linear_cross_entropy(x, w, y, A=leaves[0], B=leaves[1], alpha=s * 8, reduction="sum")
+        da, db = (t.double() for t in torch.autograd.grad(loss, leaves))
+        want = g.T @ xa
+        rest = (g - at).abs().T @ xa.abs()
+        part = 2.0 ** -14  # s x A^T in two parts of 8 bits or more
+        bound = (half + SOFT + part) * want.abs() + twice * rest * (1 + half) + 2 * tiny + \
+            (SOFT + part) * (at.abs().T @ xa.abs())
+        assert bool(((db - want).abs() <= bound).all()), (seed, m)
+        u = s * g @ b.double()
+        want = u.T @ x.double()
+        off = 6 * twice / 3 ** 0.5 * s * ((g - at).square() @ b.double().square()).sqrt()
+        size = s * g.abs() @ b.double().abs()
+        bound = half * want.abs() + (1 + half) * ((off + (SOFT + part) * size).T @ x.double().abs()) + tiny
+        assert bool(((da - want).abs() <= bound).all()), (seed, m)
