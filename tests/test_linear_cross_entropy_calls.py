@@ -134,3 +134,117 @@ def test_gradients_of_weights_from_few_tokens(cuda, dtype, m):
         size = s * g.abs() @ b.double().abs()
         bound = half * want.abs() + (1 + half) * ((off + (SOFT + part) * size).T @ x.double().abs()) + tiny
         assert bool(((da - want).abs() <= bound).all()), (seed, m)
+
+
+def _workspace(m, k, v, r, dtype, grads):
+    code = _lib.DTYPE_BF16 if dtype == BF16 else _lib.DTYPE_F16
+    return _lib.load().mlora_linear_cross_entropy_workspace_bytes(m, k, v, r, code, grads)
+
+
+def _check_in_blocks(x, w, y, a=None, b=None, s=2.0, rows=256):
+    """Summed loss and gradients against 64 bits, 256 tokens at a time; the bounds are
+    those of each rounding, elementwise."""
+    dtype, (m, k), v = x.dtype, x.shape, w.shape[0]
+    h = torch.finfo(dtype).eps / 2
+    tiny, sub = (2.0 ** -31, 2.0 ** -25) if dtype == FP16 else (0.0, 0.0)
+    eps = 2.0 ** -20
+    leaves = [t for t in (x, w, a, b) if t is not None and t.requires_grad]
+    r = 0 if a is None else a.shape[0]
+    loss = ops.linear_cross_entropy(x, w, y, A=a, B=b, alpha=s * max(r, 1), reduction="sum")
+    got = dict(zip([id(t) for t in leaves], torch.autograd.grad(loss, leaves)))
+    xs, wd = x.detach().double(), w.detach().double()
+    dw, bw = torch.zeros_like(wd), torch.zeros_like(wd)
+    if r:
+        ad, bd = a.detach().double(), b.detach().double()
+        da, ba, db, bb = (torch.zeros_like(t) for t in (ad, ad, bd, bd))
+    total = most = 0.0
+    # logits: a random walk of K fp32 roundings, four deviations
+    dl = 2.0 ** -24 * 4 * k ** 0.5 * float(xs.norm(dim=1).max() * wd.norm(dim=1).max()) + 2e-6
+    if r:  # s x A^T in two parts of 16 bits
+        xa_all = s * xs @ ad.T
+        dl += 2.0 ** -14 * float((xa_all.abs().max(1).values).max() * bd.abs().sum(1).max())
+    rel = h + 2.0 ** -11 + 2 * dl
+    for part in torch.arange(m, device=x.device).split(rows):
+        xd, yd = xs[part], y[part]
+        counted = yd != IGNORE
+        at = yd.clamp_min(0)[:, None]
+        logits = xd @ wd.T
+        if r:
+            logits += xa_all[part] @ bd.T
+        nll = (torch.logsumexp(logits, 1) - logits.gather(1, at)[:, 0]) * counted
+        total, most = total + float(nll.sum()), max(most, float(nll.max()))
+        g = torch.softmax(logits, 1, out=logits)
+        off = (g * rel + tiny) * counted[:, None]
+        g.scatter_add_(1, at, torch.full_like(at, -1, dtype=g.dtype)).mul_(counted[:, None])
+        eg = off + h * g.abs()
+        dx, bx = g @ wd, off @ wd.abs() + eps * (g.abs() @ wd.abs())
+        if r:
+            u = s * g @ bd
+            eu = s * (eg @ bd.abs()) + h * u.abs() + eps * s * (g.abs() @ bd.abs())
+            dx, bx = dx + u @ ad, bx + eu @ ad.abs() + eps * (u.abs() @ ad.abs())
+            xa = xa_all[part]
+            da += u.T @ xd
+            ba += (eu + eps * u.abs()).T @ xd.abs()
+            db += g.T @ xa
+            bb += (eg + (h + eps) * g.abs()).T @ xa.abs()
+        if x.requires_grad:
+            e = (got[id(x)][part].double() - dx).abs() - (bx + h * dx.abs() * 1.01 + sub)
+            assert e.max() <= 0, f"dx of tokens {int(part[0])}.. beyond its bound by {e.max()}"
+            assert torch.count_nonzero(got[id(x)][part][~counted]) == 0
+        if w.requires_grad:
+            dw += g.T @ xd
+            bw += (eg + eps * g.abs()).T @ xd.abs()
+    assert abs(float(loss.detach()) - total) <= (2 * dl + 2.0 ** -22 * most) * m
+    for t, want, bound in ((w, dw, bw),) + (((a, da, ba), (b, db, bb)) if r else ()):
+        if t.requires_grad:
+            e = (got[id(t)].double() - want).abs() - (bound + h * want.abs() * 1.01 + sub)
+            assert e.max() <= 0, f"beyond its bound by {e.max()}"
+    assert _lib.device_status(reset=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("counted", [2050, 1200, 700])
+@pytest.mark.parametrize("head,dtype", [("frozen", BF16), ("frozen", FP16), ("trained", BF16),
+                                        ("lora", BF16), ("lora", FP16)])
+def test_more_tokens_than_a_piece(cuda, head, dtype, counted):
+    """Vocabularies of which 768 tokens are a piece: three of them, the last or the last two
+    without counted tokens, the last counted one inside a piece."""
+    m, k = 2100, 16
+    v = (1 << 20) - (8 if head == "lora" else 5)
+    gen = torch.Generator(device=cuda).manual_seed(counted)
+
+    def randn(*shape, scale=1.0):
+        return (torch.randn(*shape, device=cuda, generator=gen) * scale).to(dtype)
+    x, w = randn(m, k).requires_grad_(True), randn(v, k, scale=0.4).requires_grad_(head == "trained")
+    y = torch.randint(0, v, (m,), device=cuda, generator=gen)
+    y[1::3] = y[::3][: y[1::3].numel()]  # labels that recur, within a piece and across
+    y[1500:1600] = y[:100]
+    y[torch.randperm(m, device=cuda, generator=gen)[: m - counted]] = IGNORE
+    a = b = None
+    if head == "lora":
+        a = randn(8, k, scale=0.3).requires_grad_(True)
+        b = randn(v, 8, scale=0.1).requires_grad_(True)
+    grads = 1 + 2 * (head == "trained") + 4 * (head == "lora")
+    # all exponentials at once would take more than the whole workspace, twice over
+    assert 2 * _workspace(m, k, v, 8 if a is not None else 0, dtype, grads) < 2 * m * v * 2
+    _check_in_blocks(x, w, y, a, b)
+
+
+@pytest.mark.gpu
+def test_losses_of_more_tokens_than_a_piece(cuda):
+    """Without a gradient a token costs a piece 8 bytes for each 96 entries or more; the
+    losses are those of calls with fewer tokens, but for the order of sums over tiles."""
+    m, k, v = 50_000, 16, (1 << 20) - 5
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    x = torch.randn(m, k, device=cuda, generator=gen).to(BF16)
+    w = (torch.randn(v, k, device=cuda, generator=gen) * 0.4).to(BF16)
+    y = torch.randint(0, v, (m,), device=cuda, generator=gen)
+    y[::5] = IGNORE
+    assert _workspace(m, k, v, 0, BF16, 0) < m * v // 128 * 8
+    got = ops.linear_cross_entropy(x, w, y, reduction="none")
+    for lo in range(0, m, 6250):
+        part = slice(lo, lo + 6250)
+        want = ops.linear_cross_entropy(x[part], w, y[part], reduction="none")
+        # sums of 8192 tiles in another order and by another reference
+        assert bool(((got[part] - want).abs() <= 2.0 ** -18 * want.abs()).all())
+        assert torch.equal(got[part] == 0, y[part] == IGNORE)
