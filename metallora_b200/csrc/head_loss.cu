@@ -126,19 +126,23 @@ struct Numbers {
 // xc[i] = x[row_of[i]], zeros past the last counted token (as many as a reduction
 // over tokens reads; all of them for the LoRA products, which run over every row);
 // and target[i] = the label's logit but for a LoRA term, in 32 bits; ref[i] = it in whole
-// units of log 2.  One CTA per row of xc, or with kNumber per token: each then counts
+// units of log 2; and uncut[i] = what gives the row's logits back what the tensor cores'
+// accumulation cuts off on average (head_gemm.cu).  One CTA per row of xc, or with kNumber per token: each then counts
 // the tokens ahead of its own itself, which up to some thousands is faster than a
 // launch that numbers them.
 constexpr int kGatherThreads = 128;
 constexpr int64_t kNumberTokens = 2048;
+constexpr float kCutPerGroup = 8.0e-9f;  // of 8 features
+constexpr int kCutGroups = 1024;         // as many as were measured
 
 template <typename T, bool kNumber>
 __global__ void __launch_bounds__(kGatherThreads)
     head_gather_kernel(const uint4* x, const uint4* w, const int64_t* labels, int64_t ignore_index,
                        int64_t M, int64_t V, Numbers num, float* row_loss, int64_t K8, int64_t ld8,
-                       int zero_all, uint4* xc, float* target, float* ref, uint32_t* status) {
+                       int zero_all, uint4* xc, float* target, float* ref, float* uncut,
+                       uint32_t* status) {
   __shared__ float part[4];
-  __shared__ int32_t parts[2][4];
+  __shared__ int32_t parts[2][4], groups[4];
   grid_wait();
   launch_dependents();
   int64_t i = blockIdx.x;
@@ -188,20 +192,27 @@ __global__ void __launch_bounds__(kGatherThreads)
   const uint4* xr = x + static_cast<int64_t>(row) * K8;
   const uint4* wr = w + static_cast<int64_t>(y) * K8;
   float s = 0.f;
+  int32_t nonzero = 0;  // groups of 8 features, of either sign of zero
 #pragma unroll 4
   for (int64_t k = threadIdx.x; k < K8; k += kGatherThreads) {
     const uint4 xv = xr[k], wv = wr[k];
     xc[i * ld8 + k] = xv;
+    nonzero += ((xv.x | xv.y | xv.z | xv.w) & 0x7fff7fffu) != 0;
     const T* xe = reinterpret_cast<const T*>(&xv);
     const T* we = reinterpret_cast<const T*>(&wv);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s = fmaf(static_cast<float>(xe[j]), static_cast<float>(we[j]), s);
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    nonzero += __shfl_xor_sync(0xffffffffu, nonzero, o);
+  }
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s, groups[threadIdx.x >> 5] = nonzero;
   __syncthreads();
   if (threadIdx.x == 0) {
+    const int32_t all = groups[0] + groups[1] + groups[2] + groups[3];
+    uncut[i] = 1.f + kCutPerGroup * static_cast<float>(min(all, kCutGroups));
     const float t = part[0] + part[1] + (part[2] + part[3]);
     target[i] = t;
     // in units of log 2, within what leaves room above and below; 0 for no number
@@ -699,7 +710,7 @@ State plan_state(void* base, const Dims& d) {
 struct Work {
   int32_t* row_of;
   float* nll;
-  float *target, *ref;
+  float *target, *ref, *uncut;
   void *xc, *xa_rows, *xa_t, *xa_lo, *b2, *bt, *u_rows, *u_t, *u_lo, *eg;
   float2* stats;
   int64_t piece;  // rows that go through at a time
@@ -722,6 +733,7 @@ Work plan_work(void* base, const Dims& d) {
   w.nll = c.take<float>(d.M);
   w.target = c.take<float>(d.M);
   w.ref = c.take<float>(d.M);
+  w.uncut = c.take<float>(d.M);
   w.xc = c.take<uint16_t>(d.M * d.ldx());
   if (d.lora()) {
     w.xa_rows = c.take<uint16_t>(d.M * d.ld_xa());
@@ -785,7 +797,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
                       dim3(static_cast<unsigned>(M)), kGatherThreads, 0, s, 0, 0, true,
                       static_cast<const uint4*>(x), static_cast<const uint4*>(w), labels, ignore_index, M,
                       V, num, row_loss, K / 8, ldx / 8, zero_all, static_cast<uint4*>(ws.xc), ws.target,
-                      by_row ? ws.ref : nullptr, device_status_ptr());
+                      by_row ? ws.ref : nullptr, ws.uncut, device_status_ptr());
   }
   if ((rc = launch_status(e, "linear cross entropy: gather"))) return rc;
   RankArgs ra;
@@ -836,6 +848,7 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
     l.stats = ws.stats;
     l.stats_ld = ws.tiles;
     l.tile_n = ws.cols;
+    l.uncut = ws.uncut + row0;
     l.ref = by_row ? ws.ref + row0 : nullptr;
     l.elt = elt;
     if (d.lora()) {

@@ -270,10 +270,12 @@ struct HeadGemmArgs {
   const int32_t* rows = nullptr;  // counted tokens (device); those from row0 on are meant
   int64_t row0 = 0;
   bool accumulate = false;   // D += (splits = 1)
-  // kLogits: per row m its label and, for the form with one reference a row (bf16), ref;
+  // kLogits: per row m its label, what its logits are multiplied by, and for the form with
+  // one reference a row (bf16) ref;
   // e: [M, ldd] exponentials in 16 bits or nullptr (ldd a multiple of 16, at least N);
   // stats: float2 [M, stats_ld], one for every tile_n / 2 entries
   const int32_t* label = nullptr;
+  const float* uncut = nullptr;
   const float* ref = nullptr;
   void* e = nullptr;
   void* stats = nullptr;

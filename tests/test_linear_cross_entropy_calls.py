@@ -248,3 +248,74 @@ def test_losses_of_more_tokens_than_a_piece(cuda):
         # sums of 8192 tiles in another order and by another reference
         assert bool(((got[part] - want).abs() <= 2.0 ** -18 * want.abs()).all())
         assert torch.equal(got[part] == 0, y[part] == IGNORE)
+
+
+def _loss_error(x, w, y):
+    """|error| of the mean loss; the mean softmax-weighted |logit| of the other entries, what
+    a relative error of the logits is seen times; the fp32 steps' share: ex2.approx and
+    l log2(e) - n, rounded at 2^-24 of |l| log2(e) + 1 twice, and the result."""
+    got = ops.linear_cross_entropy(x, w, y).double()
+    logits = x.double() @ w.double().T
+    want = torch.nn.functional.cross_entropy(logits, y)
+    sens = torch.softmax(logits, 1).scatter_(1, y[:, None], 0.0).mul_(logits.abs()).sum(1).mean()
+    fp32 = 2.0 ** -22 * (float(logits.abs().max()) + 4) + 2.0 ** -23 * float(want)
+    return abs(float(got - want)), float(sens), fp32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("k", [256, 1024, 4096, 8192])
+def test_loss_of_dense_hidden_states(cuda, dtype, k):
+    """What the tensor cores cut off the logits, 1e-9 K of them, is given back to within
+    half: without that the loss would be off by all of it."""
+    gen = torch.Generator(device=cuda).manual_seed(k)
+    x, w = (torch.randn(*s, device=cuda, generator=gen) for s in ((512, k), (3000, k)))
+    y = torch.randint(0, 3000, (512,), device=cuda, generator=gen)
+    off, sens, fp32 = _loss_error(x.to(dtype), (w * 6 / k ** 0.5).to(dtype), y)
+    assert off <= 0.5e-9 * k * sens + 2.0 ** -24 * 20
+    assert k < 4096 or 0.5e-9 * k * sens > 2.0 ** -24 * 20  # the bound is the cut's
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("k", [256, 4096, 65536])
+def test_loss_of_sparse_hidden_states(cuda, dtype, k):
+    """One feature a token: the logits are single products, of which nothing is cut."""
+    gen = torch.Generator(device=cuda).manual_seed(k)
+    x = torch.zeros(200, k, device=cuda, dtype=dtype)
+    at = torch.randint(0, k, (200,), device=cuda, generator=gen)
+    x[torch.arange(200, device=cuda), at] = 1.5
+    x[::2] *= -1  # the zeros beside them negative
+    w = (torch.randn(1000, k, device=cuda, generator=gen) * 6).to(dtype)
+    y = torch.randint(0, 1000, (200,), device=cuda, generator=gen)
+    off, _, fp32 = _loss_error(x, w, y)
+    assert off <= fp32
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_loss_of_more_features_than_were_measured(cuda, dtype):
+    """Exact sums of 2^17 features of one size: what is given back stops at 8192 features'."""
+    k = 1 << 17
+    gen = torch.Generator(device=cuda).manual_seed(0)
+    x, w = (torch.randint(0, 2, s, device=cuda, generator=gen).mul_(2).sub_(1).to(dtype)
+            for s in ((200, k), (1000, k)))
+    y = torch.randint(0, 1000, (200,), device=cuda, generator=gen)
+    off, sens, fp32 = _loss_error(x, w * 2.0 ** -5, y)
+    assert off <= 1.0e-9 * 8192 * sens + fp32 < 1.0e-9 * k * sens / 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("k", [1024, 4096])
+def test_loss_of_products_of_one_sign(cuda, dtype, k):
+    """Sums that only grow lose most.  Each of K additions cuts at most 2^-23 of what is
+    summed by then, on average half of the sum: K 2^-24 of it.  (Measured 3.5e-9 K in
+    bf16 and 6.3e-9 K in fp16, of which 1e-9 K are given back.)"""
+    gen = torch.Generator(device=cuda).manual_seed(k)
+    x = torch.rand(300, k, device=cuda, generator=gen).to(dtype)
+    w = (torch.rand(1000, k, device=cuda, generator=gen) * torch.rand(1000, 1, device=cuda, generator=gen)
+         * 100 / k).to(dtype)
+    y = torch.randint(0, 1000, (300,), device=cuda, generator=gen)
+    off, sens, fp32 = _loss_error(x, w, y)
+    assert off <= k * 2.0 ** -24 * sens + fp32
