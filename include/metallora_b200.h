@@ -504,7 +504,9 @@ MLORA_API int mlora_lora_grads_static(const void* dy, const void* x, const void*
 
 /* Softmax cross entropy over a vocabulary of V entries, from the hidden states
  * x [M, K], the head's weight w [V, K] and, with r > 0, its LoRA factors a [r, K]
- * and b [V, r] (logits x.w^T + (alpha/r)(x.a^T).b^T); no [M, V] array is kept.
+ * and b [V, r] (logits x.w^T + (alpha/r)(x.a^T).b^T).  What is held of [M, V]
+ * is, for gradients alone, 16 bits of each entry of up to 2 GiB of rows (256 rows or
+ * more) at a time, in the workspace.
  * labels: M int64; a token labelled ignore_index has no loss and no gradient, nor
  * has one whose label is outside [0, V) (device status 0x107).  Writes the sum, or
  * with `mean` the mean, over the other tokens to *loss, and/or each token's loss

@@ -1045,7 +1045,10 @@ int mlora_lora_forward_dropout(const void* x, const void* w0, const void* a, con
   ra.ldx = K;
   ra.ldl = K;
   // the kept elements' factor goes in here: what is left of the mask is 0 or 1, exact in
-  // any type, in the forward and on dy
+  // any type, in the forward and on dy.  s x A^T and, in the backward, s dz B are rounded to
+  // 16 bits once before their products, as in the LoRA linear without dropout: y and dx
+  // are off by 0.0017 to 0.0020 of themselves in bf16, dA and dB by 0.0024, a rounded
+  // result by 0.0017
   ra.scale = alpha / static_cast<float>(r) * dropout_scale(static_cast<uint32_t>(threshold));
   ra.out_rows = p.xa_rows;
   ra.ld_rows = p.R64;

@@ -7,7 +7,7 @@
 //
 // and the LoRA linear with dropout, y = x . W^T + drop(X2 . B^T), both K-major.
 //
-// The logits never leave the chip as such.  The epilogue takes, of each row's 128 in half
+// The logits never go to memory as such.  The epilogue takes, of each row's 128 in half
 // a tile, a reference n_t and s_t = sum exp(l) 2^-n_t, and where a gradient is wanted
 // writes the exponentials exp(l) 2^-n_t in 16 bits.  Two forms:
 //   * bf16 hidden states behind a frozen head: n_t is one whole number for the whole row,

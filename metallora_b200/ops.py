@@ -442,7 +442,9 @@ def linear_cross_entropy(x, weight, labels, A=None, B=None, alpha: float = 16.0,
                          _compute=None, _sink=None):
     """Softmax cross entropy of a linear head over a large vocabulary, from the hidden
     states: ``cross_entropy(x.weight^T [+ (alpha/r)(x.A^T).B^T], labels)`` without the
-    [tokens, vocabulary] logits, in memory that does not grow with them.
+    [tokens, vocabulary] logits.  During the forward, and for gradients alone, 16 bits
+    of each are held for as many tokens as fill 2 GiB (256 at least); a loss without
+    gradients holds 8 bytes for each 96 to 128 of them.
 
     x [..., K] (bf16 or fp16), weight [V, K] of the same type, labels int [...];
     A [r, K] and B [V, r] (both or neither) are a LoRA head's factors.  Tokens
