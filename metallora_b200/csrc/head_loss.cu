@@ -467,70 +467,133 @@ __global__ void __launch_bounds__(kRowThreads)
   }
 }
 
-// out[y] += the sum of rest[i] src[i] over the counted tokens i of label y, in token order:
-// what rounding their g[y] left over, of which row y of dW and dB would show all where
-// y has few tokens (with one, up to the half step that rounding the row adds again).
-// src rows have `cols` columns and, with `second`, their second part that far behind.
-// A CTA per token and 2048 columns; the label's first token does the work of all.
-// Searching for it and for the others reads 4 bytes for each pair of a token and
-// a label's first one, where the products moved 6 for each pair of a token and an entry.
-// Bound: HBM, a row of dW read and written for each label, of 4096 tokens and 2048 features
-// some 20 of 2930 us (dW from two tokens is off by 0.0017 of itself, without it 0.0031).
-template <typename T>
+// What rounding g[y] left over, for the rows of dW and dB, by ranges of kRestTokens counted
+// tokens, which bounds the search for tokens of one label and the work of a CTA.
+//
+// First each token's place in its range by (label, token), by counting: order[place] = the
+// token, run[token] = (its label's first place, how many tokens that has, how many of them
+// are ahead, the label).  A warp a token, all labels in shared memory.
+constexpr int kRestTokens = 4096;
+constexpr int kRunThreads = 32;
+
 __global__ void __launch_bounds__(kRowThreads)
-    head_rest_kernel(Numbers num, const float* rest, const T* src, int64_t ld, int second, int64_t cols,
-                     float* out) {
-  __shared__ uint32_t same[kRowThreads / 32];
+    head_runs_kernel(Numbers num, int32_t* order, int4* run) {
+  __shared__ __align__(16) int32_t label[kRestTokens];
   grid_wait();
   launch_dependents();
+  constexpr int kTokens = kRowThreads / kRunThreads;  // of a CTA, all of one range
+  static_assert(kRestTokens % kTokens == 0, "ranges of whole CTAs");
+  const int64_t cta_first = static_cast<int64_t>(blockIdx.x) * kTokens;
+  const int64_t first = cta_first / kRestTokens * kRestTokens;
   const int64_t counted = num.count->counted;
-  const int64_t slot = blockIdx.x;
-  if (slot >= counted) return;
-  const int32_t y = num.label[slot];
-  constexpr int kAhead = 4;
-  for (int64_t j0 = 0; j0 < slot; j0 += kAhead * kRowThreads) {
-    bool found = false;
-#pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      const int64_t j = j0 + a * kRowThreads + threadIdx.x;
-      if (j < slot) found |= num.label[j] == y;
-    }
-    if (__syncthreads_or(found)) return;
+  if (cta_first >= counted) return;
+  const int tokens = static_cast<int>(min(counted - first, static_cast<int64_t>(kRestTokens)));
+  const int own = static_cast<int>(cta_first - first) + static_cast<int>(threadIdx.x) / kRunThreads;
+  const int padded = (tokens + 3) / 4 * 4;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < padded; i += kRowThreads)
+    label[i] = i < tokens ? num.label[first + i] : INT32_MAX;  // (behind every label)
+  __syncthreads();
+  const int32_t y = own < tokens ? label[own] : 0;
+  int less = 0, ahead = 0, same = 0;
+#pragma unroll 4
+  for (int i = static_cast<int>(threadIdx.x) % kRunThreads * 4; i < padded; i += kRunThreads * 4) {
+    const int4 q = *reinterpret_cast<const int4*>(label + i);
+    less += (q.x < y) + (q.y < y) + (q.z < y) + (q.w < y);
+    const int equal = (q.x == y) + (q.y == y) + (q.z == y) + (q.w == y);
+    same += equal;
+    if (i + 3 < own)
+      ahead += equal;
+    else if (i < own)
+      ahead += (q.x == y) + (i + 1 < own && q.y == y) + (i + 2 < own && q.z == y);
   }
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * kRowThreads + threadIdx.x) * 8;
+#pragma unroll
+  for (int o = kRunThreads / 2; o > 0; o >>= 1) {
+    less += __shfl_xor_sync(0xffffffffu, less, o);
+    ahead += __shfl_xor_sync(0xffffffffu, ahead, o);
+    same += __shfl_xor_sync(0xffffffffu, same, o);
+  }
+  if (threadIdx.x % kRunThreads != 0 || own >= tokens) return;
+  order[first + less + ahead] = own;
+  run[first + own] = make_int4(less, same, ahead, y);
+}
+
+// Then, a launch for each range in order, out[y] += the sum of rest[i] src[i] over the tokens
+// i of label y: row y of dW and dB
+// would show all of it where y has few tokens (with one, up to the half step that rounding
+// the row adds again).  src rows have `cols` columns and, with `second`, their second part
+// that far behind.  A CTA per token and 2048 columns: of a label's CTAs the first one sums
+// its tokens, or, where they are many, the first 16 do, 128 columns each and their tokens in
+// 16 groups of threads; in a fixed order either way.
+// Bound: HBM, a row of dW read and written for each label: 60 us of 8192 tokens and 4096
+// features, where the call takes 3.6 ms (a label that all of them have: 305 us); their
+// places take 14 us.  What it is for: dW from two tokens is off by 0.0017 of itself,
+// without it by 0.0031.
+constexpr int kRestCols = 8 * kRowThreads;
+constexpr int kRestMany = 16;  // and the groups
+
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads, 4)
+    head_rest_kernel(const HeadCount* count, int64_t first, const int32_t* order, const int4* run,
+                     const float* rest, const T* src, int64_t ld, int second, int64_t cols, float* out) {
+  __shared__ float4 sums[2 * kRowThreads];
+  grid_wait();
+  launch_dependents();
+  const int own = static_cast<int>(blockIdx.x);  // of the tokens from `first` on
+  if (first + own >= count->counted) return;
+  const int4 r = run[first + own];
+  const int n = r.y;
+  const int tid = static_cast<int>(threadIdx.x);
+  const int groups = n < kRestMany ? 1 : kRestMany;
+  const int lanes = kRowThreads / groups, group = tid / lanes;
+  const int64_t first_col = static_cast<int64_t>(blockIdx.y) * kRestCols;
+  const int64_t width = min(cols - first_col, static_cast<int64_t>(kRestCols));
+  if (r.z >= groups || r.z * lanes * 8 >= width) return;
+  const int c = r.z * lanes * 8 + (tid - group * lanes) * 8;  // of `width` columns
+  float4* const row =
+      reinterpret_cast<float4*>(out + static_cast<int64_t>(r.w) * cols + first_col + c);
+  const bool writes = group == 0 && c < width;
+  float4 was[2];
+  if (writes) was[0] = row[0], was[1] = row[1];
   float acc[8] = {};
-  for (int64_t j0 = slot; j0 < counted; j0 += kRowThreads) {
-    const int64_t j = j0 + threadIdx.x;
-    const uint32_t votes = __ballot_sync(0xffffffffu, j < counted && num.label[j] == y);
-    if ((threadIdx.x & 31) == 0) same[threadIdx.x >> 5] = votes;
-    __syncthreads();
-    if (c < cols) {
-      for (int w = 0; w < kRowThreads / 32; ++w) {
-        for (uint32_t bits = same[w]; bits != 0; bits &= bits - 1) {
-          const int64_t i = j0 + w * 32 + (__ffs(static_cast<int>(bits)) - 1);
-          const float left = rest[i];
-          const uint4 q = *reinterpret_cast<const uint4*>(src + i * ld + c);
-          const T* e = reinterpret_cast<const T*>(&q);
+  for (int part = 0; c < width && part <= second; part += second > 0 ? second : 1) {
+    const T* const from = src + first * ld + part + first_col + c;
+    constexpr int kAhead = 4;
+    for (int i0 = group; i0 < n; i0 += groups * kAhead) {
+      uint4 q[kAhead];
+      float left[kAhead];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] = fmaf(left, static_cast<float>(e[k]), acc[k]);
-          if (second == 0) continue;
-          const uint4 q2 = *reinterpret_cast<const uint4*>(src + i * ld + second + c);
-          const T* e2 = reinterpret_cast<const T*>(&q2);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) acc[k] = fmaf(left, static_cast<float>(e2[k]), acc[k]);
+      for (int a = 0; a < kAhead; ++a) {
+        const int i = i0 + a * groups;
+        left[a] = 0.f;
+        if (i < n) {
+          const int64_t token = n == 1 ? own : order[first + r.x + i];
+          q[a] = *reinterpret_cast<const uint4*>(from + token * ld);
+          left[a] = rest[first + token];
         }
       }
-    }
-    __syncthreads();
-  }
-  if (c >= cols) return;
-  float4* row = reinterpret_cast<float4*>(out + static_cast<int64_t>(y) * cols + c);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float4 v = row[h];
-    v.x += acc[4 * h], v.y += acc[4 * h + 1], v.z += acc[4 * h + 2], v.w += acc[4 * h + 3];
-    row[h] = v;
+      for (int a = 0; a < kAhead; ++a) {
+        if (i0 + a * groups >= n) break;
+        const T* e = reinterpret_cast<const T*>(&q[a]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) acc[k] = fmaf(left[a], static_cast<float>(e[k]), acc[k]);
+      }
+    }
   }
+  if (groups > 1) {
+    sums[2 * tid] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    sums[2 * tid + 1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+    __syncthreads();
+    for (int g = 1; writes && g < groups; ++g) {
+      const float4 a = sums[2 * (tid + g * lanes)], b = sums[2 * (tid + g * lanes) + 1];
+      acc[0] += a.x, acc[1] += a.y, acc[2] += a.z, acc[3] += a.w;
+      acc[4] += b.x, acc[5] += b.y, acc[6] += b.z, acc[7] += b.w;
+    }
+  }
+  if (!writes) return;
+  row[0] = make_float4(was[0].x + acc[0], was[0].y + acc[1], was[0].z + acc[2], was[0].w + acc[3]);
+  row[1] = make_float4(was[1].x + acc[4], was[1].y + acc[5], was[1].z + acc[6], was[1].w + acc[7]);
 }
 
 // dx[row] = grad row_scale[slot] (sum over splits of part[split][slot] + rest[slot] W[y]);
@@ -711,7 +774,8 @@ State plan_state(void* base, const Dims& d) {
 }
 
 struct Work {
-  int32_t* row_of;
+  int32_t *row_of, *order;
+  int4* run;
   float* nll;
   float *target, *ref, *uncut;
   void *xc, *xa_rows, *xa_t, *xa_lo, *b2, *bt, *u_rows, *u_t, *u_lo, *eg;
@@ -733,6 +797,10 @@ Work plan_work(void* base, const Dims& d) {
   w.cols = logit_cols(d, w.piece);
   w.tiles = d.tiles(w.cols);
   w.row_of = c.take<int32_t>(d.M);
+  if (d.grads & (MLORA_HEAD_GRAD_W | MLORA_HEAD_GRAD_AB)) {
+    w.order = c.take<int32_t>(d.M);
+    w.run = c.take<int4>(d.M);
+  }
   w.nll = c.take<float>(d.M);
   w.target = c.take<float>(d.M);
   w.ref = c.take<float>(d.M);
@@ -982,19 +1050,30 @@ int forward(const void* x, const void* w, const void* a, const void* b, const in
       if ((rc = launch_head_gemm(q, s))) return rc;
     }
   }
-  auto add_rest = [&](const void* src, int64_t ld_src, int second, int64_t cols, float* out_rows) {
+  auto add_rest = [&](int64_t first, const void* src, int64_t ld_src, int second, int64_t cols,
+                      float* out_rows) {
     LaunchScope scope(kKindElementwise, s);
-    const int64_t width = kRowThreads * 8;
-    const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((cols + width - 1) / width));
-    return launch_status(launch_kernel(head_rest_kernel<T>, grid, kRowThreads, 0, s, 0, 0, true, num,
-                                       static_cast<const float*>(st.rest), static_cast<const T*>(src),
-                                       ld_src, second, cols, out_rows),
-                         "linear cross entropy: rest of the label's entry");
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(M - first, kRestTokens)),
+                    static_cast<unsigned>((cols + kRestCols - 1) / kRestCols));
+    return launch_kernel(head_rest_kernel<T>, grid, kRowThreads, 0, s, 0, 0, true,
+                         static_cast<const HeadCount*>(st.count), first,
+                         static_cast<const int32_t*>(ws.order), static_cast<const int4*>(ws.run),
+                         static_cast<const float*>(st.rest), static_cast<const T*>(src), ld_src, second,
+                         cols, out_rows);
   };
-  if (d.want(MLORA_HEAD_GRAD_W) && (rc = add_rest(ws.xc, ldx, 0, K, st.dw))) return rc;
-  if (d.want(MLORA_HEAD_GRAD_AB) &&
-      (rc = add_rest(ws.xa_rows, d.ld_xa(), static_cast<int>(d.R()), d.r, st.db)))
-    return rc;
+  const bool dw = d.want(MLORA_HEAD_GRAD_W), db = d.want(MLORA_HEAD_GRAD_AB);
+  if (dw || db) {
+    LaunchScope scope(kKindElementwise, s);
+    const int64_t per = kRowThreads / kRunThreads;
+    e = launch_kernel(head_runs_kernel, dim3(static_cast<unsigned>((M + per - 1) / per)), kRowThreads, 0,
+                      s, 0, 0, true, num, ws.order, ws.run);
+  }
+  for (int64_t first = 0; (dw || db) && first < M; first += kRestTokens) {
+    if (e == cudaSuccess && dw) e = add_rest(first, ws.xc, ldx, 0, K, st.dw);
+    if (e == cudaSuccess && db)
+      e = add_rest(first, ws.xa_rows, d.ld_xa(), static_cast<int>(d.R()), d.r, st.db);
+    if ((rc = launch_status(e, "linear cross entropy: rest of the labels' entries"))) return rc;
+  }
   return MLORA_OK;
 }
 

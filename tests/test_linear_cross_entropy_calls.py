@@ -136,6 +136,37 @@ def test_gradients_of_weights_from_few_tokens(cuda, dtype, m):
         assert bool(((da - want).abs() <= bound).all()), (seed, m)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("m,k", [(40, 64), (60, 2056), (4096, 136), (4097, 520), (9000, 2184)])
+def test_gradients_of_weights_from_tokens_that_recur(cuda, dtype, m, k):
+    """Three tokens over and over, so that their roundings add up, around the 16 that a
+    label's tokens are many from, the ranges of 4096 tokens and 2048 columns: the rows of
+    their labels are off by their own rounding still, and by m additions, each of which
+    cuts at most 2^-23 of what is summed by then, on average half of the sum."""
+    half = torch.finfo(dtype).eps / 2
+    soft = SOFT + m * 2.0 ** -24
+    twice = half + 2.0 ** -11 + soft
+    x, w, _, _, y = _few(cuda, dtype, 3, 7, v=300, k=k)
+    x, w = x / 4, w * (8 / k ** 0.5)
+    y = torch.stack([y[0], (y[0] + 1) % 300, (y[0] + 2) % 300])
+    gen = torch.Generator(device=cuda).manual_seed(m)
+    which = torch.randint(0, 3, (m,), device=cuda, generator=gen)
+    x, y = x[which], y[which]
+    y[::50] = IGNORE
+    w1 = w.clone().requires_grad_(True)
+    dw = [torch.autograd.grad(ops.linear_cross_entropy(x, w1, y, reduction="sum"), w1)[0]
+          for _ in range(2)]
+    assert torch.equal(*dw)
+    no = torch.zeros(8, k, device=cuda, dtype=dtype), torch.zeros(300, 8, device=cuda, dtype=dtype)
+    g, at, _ = _gradient(x, w, *no, y, 0.0)
+    want = g.T @ x.double()
+    tiny = m * 2.0 ** -31 * float(x.abs().max()) + 2.0 ** -25 if dtype == FP16 else 0.0
+    bound = half * want.abs() + (1 + half) * (
+        twice * (g - at).abs().T @ x.double().abs() + soft * (at.abs().T @ x.double().abs())) + tiny
+    assert bool(((dw[0].double() - want).abs() <= bound).all())
+
+
 def _workspace(m, k, v, r, dtype, grads):
     code = _lib.DTYPE_BF16 if dtype == BF16 else _lib.DTYPE_F16
     return _lib.load().mlora_linear_cross_entropy_workspace_bytes(m, k, v, r, code, grads)
