@@ -105,7 +105,7 @@ class LoRALinear(nn.Module):
         if torch._C._current_graph_task_id() < 0:
             call = self.dropout_call
             self.dropout_call += 1
-            known[draw] = call if known.get(draw, call) == call else None
+            known[draw] = call if known.pop(draw, call) == call else None  # the youngest now
             if len(known) > _KEPT_CALLS:
                 del known[next(iter(known))]
             return call

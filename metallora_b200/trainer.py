@@ -550,7 +550,7 @@ class LoRATrainer:
         save_file(opt, str(p / "optimizer.safetensors"))
         config = {"rank": self.config.rank, "alpha": self.config.alpha,
                   "global_step": self.state.global_step}
-        calls = {n: m.dropout_call for n, m in self.params.layers if m.dropout_seed is not None}
+        calls = {n: int(m.dropout_call) for n, m in self.params.layers if m.dropout_seed is not None}
         if calls:
             config["dropout_calls"] = calls
         with open(p / "config.json", "w") as f:

@@ -99,6 +99,15 @@ def test_what_a_layer_keeps_is_bounded_and_copied(monkeypatch):
     outs[1].sum().backward()
     with pytest.raises(ConfigurationError):
         outs[0].sum().backward()
+    # one with the draw and the number of another takes its place among the youngest
+    p.dropout_call, outs = 0, []
+    for seed in (1, 2, 3, 4, 1, 5):
+        torch.manual_seed(seed)
+        p.dropout_call = seed - 1
+        outs.append(checkpoint(lambda h: torch.tanh(p(h)), x, use_reentrant=False))
+    outs[4].sum().backward()
+    with pytest.raises(ConfigurationError):
+        outs[1].sum().backward()
     p.eval()
     with torch.no_grad():
         monkeypatch.setattr(layers_module, "lora_forward", lambda x, *a, **k: x)
