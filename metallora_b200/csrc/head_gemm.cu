@@ -25,10 +25,11 @@
 // on average: it measured 1.0e-9 K of the value (0.24e-6 at K = 256, 4.0e-6 at 4096,
 // 8.4e-6 at 8192; its deviation a tenth to a half of that) for sums that drift or walk
 // to where they end, 3.5 (bf16) to 6.3 (fp16) times as much where every product has the
-// same sign, nothing where the sums are exact.  A step that adds zeros cuts nothing, so a row's features
-// count by the groups of 8 that are not all zero, and beyond the 8192 that were measured
-// no more is given back: where nothing was cut a logit is off by 1.0e-9 K of itself, 8.2e-6
-// at most, and where most was by 5.3e-9 K.  (Loss of 512 tokens at 4096 features against 64 bits 0.7e-7, without 12e-7.)
+// same sign, nothing where the sums are exact.  A step that adds zeros cuts nothing, so a
+// row's features count by the groups of 8 that are not all zero, and beyond the 8192 that
+// were measured no more is given back: where nothing was cut a logit is off by 1.0e-9 K of
+// itself, 8.2e-6 at most, and where most was by 5.3e-9 K.  (Loss of 512 tokens at 4096
+// features against 64 bits 0.7e-7, without 12e-7.)
 //
 // A (2,1,1) cluster makes a 256 x 256 tile (tcgen05.mma.cta_group::2, M = N = 256,
 // K = 16): each CTA stages its own 128 rows of either operand in a 6-stage TMA ring

@@ -128,9 +128,9 @@ struct Numbers {
 // over tokens reads; all of them for the LoRA products, which run over every row);
 // and target[i] = the label's logit but for a LoRA term, in 32 bits; ref[i] = it in whole
 // units of log 2; and uncut[i] = what gives the row's logits back what the tensor cores'
-// accumulation cuts off on average (head_gemm.cu).  One CTA per row of xc, or with kNumber per token: each then counts
-// the tokens ahead of its own itself, which up to some thousands is faster than a
-// launch that numbers them.
+// accumulation cuts off on average (head_gemm.cu).  One CTA per row of xc, or with kNumber
+// per token: each then counts the tokens ahead of its own itself, which up to some
+// thousands is faster than a launch that numbers them.
 constexpr int kGatherThreads = 128;
 constexpr int64_t kNumberTokens = 2048;
 constexpr float kCutPerGroup = 8.0e-9f;  // of 8 features
@@ -518,13 +518,12 @@ __global__ void __launch_bounds__(kRowThreads)
   run[first + own] = make_int4(less, same, ahead, y);
 }
 
-// Then, a launch for each range in order, out[y] += the sum of rest[i] src[i] over the tokens
-// i of label y: row y of dW and dB
-// would show all of it where y has few tokens (with one, up to the half step that rounding
-// the row adds again).  src rows have `cols` columns and, with `second`, their second part
-// that far behind.  A CTA per token and 2048 columns: of a label's CTAs the first one sums
-// its tokens, or, where they are many, the first 16 do, 128 columns each and their tokens in
-// 16 groups of threads; in a fixed order either way.
+// Then, a launch for each range in order, out[y] += the sum of rest[i] src[i] over the
+// tokens i of label y: row y of dW and dB would show all of it where y has few tokens (with
+// one, up to the half step that rounding the row adds again).  src rows have `cols` columns
+// and, with `second`, their second part that far behind.  A CTA per token and 2048 columns:
+// of a label's CTAs the first one sums its tokens, or, where they are many, the first 16
+// do, 128 columns each and their tokens in 16 groups of threads; in a fixed order either way.
 // Bound: HBM, a row of dW read and written for each label: 60 us of 8192 tokens and 4096
 // features, where the call takes 3.6 ms (a label that all of them have: 305 us); their
 // places take 14 us.  What it is for: dW from two tokens is off by 0.0017 of itself,
